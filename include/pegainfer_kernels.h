@@ -718,6 +718,53 @@ int pk_gla_seq(const void* qkv, int ld, int q_off, int k_off, int v_off, const f
 /* z [tokens, channels] <- logistic(z + bias)^(1 / tau) in place */
 int pk_logistic_decay(float* z, const float* bias, float tau, int tokens, int channels, pk_stream st);
 
+/* =============== a K/V cache of 8 bits: append, attention, eviction ===============
+ * 16 consecutive slots of one kv head are a record: e4m3 codes and two exponents (K's and V's); a value is code * 2^exponent, the exponent the least e with
+ * (largest magnitude of the record) <= 448 * 2^e, -110 <= e <= 120; values are rounded to nearest even.
+ *   record: K [2 groups of 8 slots][dim/16][8 slots][16 entries] | V [vdim][16 slots] | int8 exponent of K, int8 exponent of V, 14 zero bytes
+ *   page:   [kv_heads][page_size/16] records, pk_kv8_page_bytes() bytes; page_stride (bytes, a multiple of 16) may be larger.  cache: 16-byte aligned.
+ * The slot s of request r is in page pages[page_off[r] + s / page_size].  A slot is an index into the request's cache: the token's position, or less where
+ * tokens were evicted.  page_size is a multiple of 16, dim and vdim multiples of 32 up to 256.  A token with an entry of k or v that is not finite makes the
+ * rows that see it NaN (in the heads that read that kv head), and no others.  f32 selects the element type of activations, as above; the cache has one form.
+ * -1: invalid argument.  Nothing is allocated, everything may be captured into a graph. */
+/* Bytes of a page; -1: sizes that the cache does not have */
+long pk_kv8_page_bytes(int page_size, int kv_heads, int dim, int vdim);
+/* qkv [tokens, ld] = [q (heads*dim) | k (kv_heads*dim) | v (kv_heads*vdim)] (+ bias of the same layout, may be NULL): q and k rotate over their first `dims`
+ * entries by positions[t] * freq[i] as in pk_gqa_rope_append (angles are reduced in 64 bits); q goes to q_out [tokens, heads*dim], k and v into the cache at
+ * slots[t] (slots NULL: at positions[t]).  heads may be 0 (rows of k and v alone, q_out NULL).  A request's tokens are consecutive rows with consecutive slots,
+ * in one run per call.  A token at a record's first slot begins the record anew (slots behind the call's last are zero); else the record goes on from the slots
+ * before, whose codes are rounded again where its exponent grows.  Rows with a negative slot are not cached (their q is rotated all the same). */
+int pk_kv8_append(const void* qkv, int ld, const void* bias, const int* positions, const int* slots, const int* req, const int* page_off, const int* pages,
+                  void* q_out, void* cache, long page_stride, int page_size, int heads, int kv_heads, int dim, int vdim, int dims, int interleaved,
+                  const float* freq, float mag, int tokens, int f32, pk_stream st);
+/* Options of pk_kv8_attention; a zero / NULL field switches its option off, except max_kv_len, which every call needs. */
+typedef struct pk_kv8_options {
+  int window;      /* the query at slot p sees slots p - window + 1 .. p */
+  float softcap;   /* scaled score <- softcap * tanh(score / softcap) */
+  int max_kv_len;  /* no query's slot is max_kv_len or more */
+  int max_q_len;   /* no request has more tokens in the call (0: unknown): a hint for the choice of a kernel */
+  long out_ld;     /* elements from one row of out to the next (0: heads * vdim) */
+  float* lse;      /* [tokens, heads]: log(sum over the visible slots of exp(score), plus exp(sink)); -inf where there is neither */
+  float* mass;     /* [requests, kv_heads, mass_ld]: mass[req[t]][g][j] += the weights of slot j in the rows of the call, over the heads of group g */
+  long mass_ld;    /* slots from mass_ld on are not counted */
+} pk_kv8_options;
+/* Bytes of workspace that the call needs (0: none, -1: invalid argument).  Workspaces of calls that may run at the same time, those of captured graphs among
+ * them, are separate; 16-byte aligned; any contents. */
+long pk_kv8_attention_workspace_bytes(int tokens, int heads, int kv_heads, int dim, int vdim, const pk_kv8_options* options, int f32);
+/* out[t,h] = sum_j w_j v_j, w = softmax over the visible slots j <= slots[t] of q[t,h] . k_j * scale (options applied; exp(sink[h]) added to the denominator when
+ * sink != NULL).  A request's tokens are consecutive rows with ascending slots, in one run per call.  A row with a negative slot sees nothing: zeros. */
+int pk_kv8_attention(const void* q, const void* cache, const void* sink, const int* slots, const int* req, const int* page_off, const int* pages, void* out,
+                     long page_stride, int page_size, int tokens, int heads, int kv_heads, int dim, int vdim, float scale, const pk_kv8_options* options,
+                     void* workspace, long workspace_bytes, int f32, pk_stream st);
+/* Of request r's lens[r] slots (< 0 counts as 0, at most max_kv_len) every kv head keeps min(lens[r], budget): the first keep_first, the last keep_recent, of the others those with the
+ * largest mass (equal: the lower slot; NaN least).  They move, in order, to the pages of new_pages / new_page_off (other pages of the same pool, room for
+ * min(lens[r], budget) slots each), into records with exponents of their own; the old pages are left as they were.  kept [requests, kv_heads, budget]: the
+ * old slot of each new one, -1 behind the last; new_mass [requests, kv_heads, new_mass_ld]: the masses of the kept, zero behind; new_lens[r]: slots kept.
+ * keep_first + keep_recent <= budget; mass_ld >= max_kv_len, new_mass_ld >= budget.  New tokens go on at slot new_lens[r] with their true positions. */
+int pk_kv8_evict(void* cache, long page_stride, int page_size, const int* page_off, const int* pages, const int* lens, const float* mass, long mass_ld,
+                 const int* new_page_off, const int* new_pages, int* new_lens, float* new_mass, long new_mass_ld, int* kept, int requests, int kv_heads,
+                 int dim, int vdim, int budget, int keep_first, int keep_recent, int max_kv_len, pk_stream st);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,301 @@
+// Append to the 8-bit paged cache (kv8.cuh): rotation of q and k, quantisation of k and v, record by record.
+//
+// The tokens of a request are consecutive rows with consecutive slots.  The first of them that falls into a record is the record's leader; its warp writes the
+// record whole.  Where the leader's slot is the record's first, the record begins anew (what the page held before is forgotten, slots behind the last token are
+// zero); else the record goes on: its exponent is the larger of the old one and what the new tokens need, and the old codes are rounded again where it grew.
+//
+// q' = rot(q), k' = rot(k): pairs (i, i + dims/2) or (2i, 2i + 1) of the first `dims` entries turn by positions * freq[i].  The angle is reduced to turns in 64
+// bits (a float product is off by 0.004 at position 100000), the sine and cosine and the rotation are fp32.
+//
+// A CTA looks at 16 tokens: a table of their sines and cosines in shared memory, then a warp to every (record, kv head), then all threads over q.  The grid's
+// y axis shares a window's work out, so that few tokens still fill the GPU.
+#include <algorithm>
+
+#include "kv8.cuh"
+
+namespace pk {
+namespace kv8 {
+
+constexpr int kAppendWarps = 4;
+constexpr int kWindow = 16;
+
+// 8 consecutive entries as floats
+template <typename E>
+__device__ __forceinline__ void load8(const E* p, bool vec, float (&v)[8]) {
+  if constexpr (sizeof(E) == 2) {
+    if (vec) {
+      const uint4 u = *reinterpret_cast<const uint4*>(p);
+      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[2 * i] = bf16_lo(w[i]);
+        v[2 * i + 1] = bf16_hi(w[i]);
+      }
+      return;
+    }
+  } else {
+    if (vec) {
+      const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+      return;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = to_f(p[i]);
+}
+template <typename E>
+__device__ __forceinline__ void store8(E* p, bool vec, const float (&v)[8]) {
+  if constexpr (sizeof(E) == 2) {
+    if (vec) {
+      *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+      return;
+    }
+  } else {
+    if (vec) {
+      *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+      *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
+      return;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) p[i] = from_f<E>(v[i]);
+}
+
+struct AppendArgs {
+  const int *positions, *slots, *req;
+  Pool pool;
+  const float* freq;
+  float mag;
+  int ld, H, T, dims, interleaved, vec;
+};
+
+// rows [at, at + count) of a projection's part into shared memory (fp32), with the bias; returns the rows with an entry that is not finite
+template <typename E>
+__device__ __forceinline__ uint32_t load_rows(float* rows, const E* src, const E* bias, int ld, int at, int count, int width, bool vec, int lane) {
+  const int per = width / 8, many = 32 / per, sub = lane / per, piece = lane % per;
+  uint32_t bad = 0;
+  for (int r0 = 0; r0 < count; r0 += many) {
+    const int r = r0 + sub;
+    bool odd = false;
+    if (sub < many && r < count) {
+      float v[8];
+      load8(src + (size_t)r * ld + piece * 8, vec, v);
+      if (bias) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] += to_f(bias[piece * 8 + i]);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) odd |= (__float_as_uint(v[i]) & 0x7f800000u) == 0x7f800000u;
+      float4* d = reinterpret_cast<float4*>(rows + (at + r) * row_ld(width) + piece * 8);
+      d[0] = make_float4(v[0], v[1], v[2], v[3]);
+      d[1] = make_float4(v[4], v[5], v[6], v[7]);
+    }
+    const uint32_t who = __ballot_sync(0xffffffffu, odd);
+    for (int i = 0; i < many; ++i)
+      if (who >> (i * per) & ((1u << (per - 1) << 1) - 1u)) bad |= 1u << (at + r0 + i);
+  }
+  __syncwarp();
+  return bad;
+}
+
+template <typename E>
+__global__ void __launch_bounds__(kAppendWarps * 32) kv8_append_kernel(const E* __restrict__ qkv, const E* __restrict__ bias, E* __restrict__ q_out, AppendArgs a) {
+  extern __shared__ __align__(16) float ap_sm[];
+  __shared__ uint32_t s_lead;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, half = a.dims >> 1;
+  const int w0 = blockIdx.x * kWindow, n_tok = min(kWindow, a.T - w0);
+  const int D = a.pool.dim, V = a.pool.vdim, G = a.pool.G, H = a.H;
+  float2* table = reinterpret_cast<float2*>(ap_sm);                                            // [token][pair] cosine, sine
+  float* rows = ap_sm + kWindow * half * 2 + warp * kBlock * row_ld(max(D, V));
+  pdl_wait();
+  pdl_launch_dependents();
+  if (warp == 0) {  // which tokens of the window lead a record
+    bool lead = false;
+    const int t = w0 + lane;
+    if (lane < n_tok) {
+      const int slot = a.slots[t];
+      lead = slot >= 0 && (slot % kBlock == 0 || t == 0 || a.req[t - 1] != a.req[t] || a.slots[t - 1] != slot - 1);
+    }
+    const uint32_t all = __ballot_sync(0xffffffffu, lead);
+    if (lane == 0) s_lead = all;
+  }
+  for (int i = threadIdx.x; i < n_tok * half; i += blockDim.x) {
+    const int tok = i / half, f = i - tok * half;
+    const double turns = (double)a.positions[w0 + tok] * (double)a.freq[f] * 0.15915494309189533577;
+    float s, c;
+    sincospif((float)(2.0 * (turns - rint(turns))), &s, &c);
+    table[i] = make_float2(c * a.mag, s * a.mag);
+  }
+  __syncthreads();
+
+  // ---- records
+  const uint32_t leads = s_lead;
+  const int items = __popc(leads) * G;
+  for (int it = blockIdx.y * kAppendWarps + warp; it < items; it += gridDim.y * kAppendWarps) {
+    const int g = it % G, tok = __fns(leads, 0, it / G + 1), t = w0 + tok;
+    const int slot = a.slots[t], req = a.req[t], first = slot % kBlock;
+    const bool mine = lane + first < kBlock && t + lane < a.T && a.req[min(t + lane, a.T - 1)] == req && a.slots[min(t + lane, a.T - 1)] == slot + lane;
+    const int count = __ffs(~__ballot_sync(0xffffffffu, mine)) - 1;  // tokens of this record in the call (lane 16 and up never count)
+    uint8_t* rec = a.pool.record(req, slot, g);
+    const uint32_t fresh = ((1u << count) - 1u) << first, none = ~(fresh | ((1u << first) - 1u)) & 0xffffu;
+    const uint32_t tail = first ? *reinterpret_cast<const uint32_t*>(rec + kBlock * (D + V)) : 0u;
+    const E* src = qkv + (size_t)t * a.ld;
+
+    // values
+    uint8_t* vdst = rec + kBlock * D;
+    if (first) {
+      const float f = pow2(tail_ev(tail));
+      for (int d = lane; d < V; d += 32) {
+        float v[16];
+        values16(*reinterpret_cast<const uint4*>(vdst + d * 16), v);
+        for (int r = 0; r < first; ++r) rows[r * row_ld(V) + d] = v[r] * f;
+      }
+    }
+    const uint32_t bad_v = load_rows(rows, src + H * D + G * D + g * V, bias ? bias + H * D + G * D + g * V : nullptr, a.ld, first, count, V, a.vec, lane);
+    int ev = exponent_for(rows_amax(rows, V, fresh & ~bad_v, lane));
+    if (first) ev = max(ev, tail_ev(tail));
+    emit_v(vdst, rows, V, ev, bad_v | none, lane);
+    __syncwarp();
+
+    // keys
+    uint32_t bad_old = 0;
+    if (first) {
+      const float f = pow2(tail_ek(tail));
+      for (int u = lane; u < D; u += 32) {
+        const int r = (u >= D / 2 ? 8 : 0) + (u & 7), c = (u % (D / 2)) >> 3;
+        if (r < first) {
+          const uint4 code = *reinterpret_cast<const uint4*>(rec + u * 16);
+          if ((code.x & 0x7fu) == 0x7fu) bad_old |= 1u << r;
+          float v[16];
+          values16(code, v);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) rows[r * row_ld(D) + c * 16 + i] = v[i] * f;
+        }
+      }
+      bad_old = __reduce_or_sync(0xffffffffu, bad_old);
+    }
+    const uint32_t bad_k = load_rows(rows, src + H * D + g * D, bias ? bias + H * D + g * D : nullptr, a.ld, first, count, D, a.vec, lane) | bad_v;
+    for (int i = lane; i < count * half; i += 32) {
+      const int r = i / half, f = i - r * half;
+      float* row = rows + (first + r) * row_ld(D);
+      // the table has the window's 16 tokens; a record that reaches into the next one has its own angles
+      float2 cs;
+      if (tok + r < n_tok) {
+        cs = table[(tok + r) * half + f];
+      } else {
+        const double turns = (double)a.positions[t + r] * (double)a.freq[f] * 0.15915494309189533577;
+        float s, c;
+        sincospif((float)(2.0 * (turns - rint(turns))), &s, &c);
+        cs = make_float2(c * a.mag, s * a.mag);
+      }
+      const int i1 = a.interleaved ? 2 * f : f, i2 = a.interleaved ? 2 * f + 1 : f + half;
+      const float x = row[i1], y = row[i2];
+      row[i1] = x * cs.x - y * cs.y;
+      row[i2] = x * cs.y + y * cs.x;
+    }
+    for (int r = 0; r < kBlock; ++r)
+      if (none >> r & 1)
+        for (int d = lane; d < D; d += 32) rows[r * row_ld(D) + d] = 0.f;
+    __syncwarp();
+    int ek = exponent_for(rows_amax(rows, D, fresh & ~bad_k, lane));
+    if (first) ek = max(ek, tail_ek(tail));
+    emit_k(rec, rows, D, ek, bad_k | bad_old, lane);
+    if (lane == 0) emit_tail(rec + kBlock * (D + V), ek, ev);
+    __syncwarp();
+  }
+
+  // ---- queries: a thread takes eight pairs (or eight entries that only pass)
+  const bool by8 = a.interleaved ? a.dims % 8 == 0 : half % 8 == 0;
+  if (by8) {
+    const int turn = a.interleaved ? a.dims / 8 : half / 8, pass = (D - a.dims) / 8, units = turn + pass;
+    for (int i = blockIdx.y * blockDim.x + threadIdx.x; i < n_tok * H * units; i += gridDim.y * blockDim.x) {
+      const int u = i % units, h = i / units % H, tok = i / units / H;
+      const size_t from = (size_t)(w0 + tok) * a.ld + h * D, to = ((size_t)(w0 + tok) * H + h) * D;
+      const E* b = bias ? bias + h * D : nullptr;
+      auto get = [&](int d, float (&v)[8]) {
+        load8(qkv + from + d, a.vec, v);
+        if (b) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) v[k] += to_f(b[d + k]);
+        }
+      };
+      float x[8], y[8];
+      if (u >= turn) {
+        get(a.dims + (u - turn) * 8, x);
+        store8(q_out + to + a.dims + (u - turn) * 8, a.vec, x);
+      } else if (a.interleaved) {
+        get(u * 8, x);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float2 cs = table[tok * half + u * 4 + k];
+          y[2 * k] = x[2 * k] * cs.x - x[2 * k + 1] * cs.y;
+          y[2 * k + 1] = x[2 * k] * cs.y + x[2 * k + 1] * cs.x;
+        }
+        store8(q_out + to + u * 8, a.vec, y);
+      } else {
+        get(u * 8, x);
+        get(half + u * 8, y);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const float2 cs = table[tok * half + u * 8 + k];
+          const float p = x[k], q = y[k];
+          x[k] = p * cs.x - q * cs.y;
+          y[k] = p * cs.y + q * cs.x;
+        }
+        store8(q_out + to + u * 8, a.vec, x);
+        store8(q_out + to + half + u * 8, a.vec, y);
+      }
+    }
+  } else {
+    for (int i = blockIdx.y * blockDim.x + threadIdx.x; i < n_tok * H * D; i += gridDim.y * blockDim.x) {
+      const int d = i % D, h = i / D % H, tok = i / D / H;
+      const size_t from = (size_t)(w0 + tok) * a.ld + h * D;
+      auto get = [&](int k) { return to_f(qkv[from + k]) + (bias ? to_f(bias[h * D + k]) : 0.f); };
+      float v = get(d);
+      if (d < a.dims) {
+        const int f = a.interleaved ? d >> 1 : d < half ? d : d - half;
+        const bool one = a.interleaved ? (d & 1) == 0 : d < half;
+        const float o = get(a.interleaved ? d ^ 1 : one ? d + half : d - half);
+        const float2 cs = table[tok * half + f];
+        v = one ? v * cs.x - o * cs.y : o * cs.y + v * cs.x;
+      }
+      q_out[((size_t)(w0 + tok) * H + h) * D + d] = from_f<E>(v);
+    }
+  }
+}
+
+}  // namespace kv8
+}  // namespace pk
+
+using namespace pk;
+
+extern "C" long pk_kv8_page_bytes(int page_size, int kv_heads, int dim, int vdim) {
+  if (!kv8::sizes_ok(page_size, kv_heads, dim, vdim)) return -1;
+  return (long)kv_heads * (page_size / kv8::kBlock) * kv8::record_bytes(dim, vdim);
+}
+
+extern "C" int pk_kv8_append(const void* qkv, int ld, const void* bias, const int* positions, const int* slots, const int* req, const int* page_off,
+                             const int* pages, void* q_out, void* cache, long page_stride, int page_size, int heads, int kv_heads, int dim, int vdim,
+                             int dims, int interleaved, const float* freq, float mag, int tokens, int f32, pk_stream st) {
+  if (!qkv || !positions || !req || !page_off || !pages || !cache || tokens <= 0 || heads < 0 || (heads > 0 && !q_out) || !kv8::sizes_ok(page_size, kv_heads, dim, vdim) ||
+      !kv8::pool_ok(cache, page_stride, page_size, kv_heads, dim, vdim) || dims < 0 || dims > dim || (dims & 1) || (dims > 0 && !freq) ||
+      ld < heads * dim + kv_heads * (dim + vdim))
+    return -1;
+  const int es = f32 ? 4 : 2;
+  const bool vec = ((reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(q_out)) & 15) == 0 && (long)ld * es % 16 == 0;
+  const kv8::AppendArgs a{positions, slots ? slots : positions, req, kv8::make_pool(cache, page_stride, page_off, pages, page_size, kv_heads, dim, vdim),
+                          freq,      mag,                       ld,  heads, tokens, dims, interleaved, vec};
+  const int windows = (tokens + kv8::kWindow - 1) / kv8::kWindow;
+  const int items = (std::min(tokens, kv8::kWindow) * kv_heads + kv8::kAppendWarps - 1) / kv8::kAppendWarps;
+  const int parts = std::max(1, std::min(items, (4 * sm_count() + windows - 1) / windows));
+  const size_t smem = ((size_t)kv8::kWindow * dims + (size_t)kv8::kAppendWarps * kv8::kBlock * kv8::row_ld(std::max(dim, vdim))) * sizeof(float);
+  const dim3 grid(windows, parts), block(kv8::kAppendWarps * 32);
+  if (f32) {
+    static std::atomic<uint64_t> set{0};
+    if (const cudaError_t e = allow_smem(set, (const void*)kv8::kv8_append_kernel<float>, 96 * 1024); e != cudaSuccess) return (int)e;
+    return (int)launch(kv8::kv8_append_kernel<float>, grid, block, smem, st, true, (const float*)qkv, (const float*)bias, (float*)q_out, a);
+  }
+  static std::atomic<uint64_t> set{0};
+  if (const cudaError_t e = allow_smem(set, (const void*)kv8::kv8_append_kernel<bf16>, 96 * 1024); e != cudaSuccess) return (int)e;
+  return (int)launch(kv8::kv8_append_kernel<bf16>, grid, block, smem, st, true, (const bf16*)qkv, (const bf16*)bias, (bf16*)q_out, a);
+}

@@ -1,0 +1,50 @@
+// Attention over the 8-bit paged cache: what its kernels share.
+#pragma once
+
+#include "kv8.cuh"
+
+namespace pk {
+namespace kv8 {
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+struct AttnArgs {
+  Pool pool;
+  const int *slots, *req;
+  int T, H;
+  float scale, cap;
+  int window, max_kv_len;
+  long out_ld;        // elements from one row of the output to the next
+  float* lse;         // [T, H] or null
+  float* mass;        // [requests, G, mass_ld] or null
+  long mass_ld;
+  float* part_o;      // [shares, T, H, vdim]  states of the shares of a row's keys
+  float2* part_ml;    // [shares, T, H]        largest score (log2), sum
+};
+
+// q . k -> score in units of log2; c = scale * log2(e)
+__device__ __forceinline__ float shaped(float dot, float c, float cap) {
+  return cap > 0.f ? cap * kLog2e * tanhf(dot * c / (cap * kLog2e)) : dot * c;
+}
+
+// Largest score M (log2), sum of 2^(s - M): what the row's accumulated values are multiplied with, and its lse.  A row that saw nothing gives zeros.
+struct RowEnd {
+  float factor, lse;
+};
+__device__ __forceinline__ RowEnd row_end(float M, float den, float sink, bool has_sink) {
+  RowEnd r;
+  float top = M, f = 1.f;
+  if (has_sink) {
+    const float sk = sink * kLog2e;
+    top = fmaxf(M, sk);
+    f = M == -INFINITY ? 0.f : exp2f(M - top);
+    den = den * f + exp2f(sk - top);
+  }
+  const bool none = top == -INFINITY;  // neither key nor sink
+  r.factor = M == -INFINITY ? 0.f : f / den;
+  r.lse = none ? -INFINITY : (top + log2f(den)) * kLn2;
+  return r;
+}
+
+}  // namespace kv8
+}  // namespace pk

@@ -129,6 +129,12 @@ class QkPrep(C.Structure):
                 ("values_are_keys", i32), ("q_only", i32)]
 
 
+class Kv8Options(C.Structure):
+    """pk_kv8_options: options of pk_kv8_attention (a zero / NULL field switches its option off; max_kv_len is always given)."""
+    _fields_ = [("window", i32), ("softcap", f32), ("max_kv_len", i32), ("max_q_len", i32), ("out_ld", i64l), ("lse", vp), ("mass", vp),
+                ("mass_ld", i64l)]
+
+
 RES32_SIGNATURES = {
     "pk_res32_embed": (i32, [vp, vp, vp, vp, i32, i32, i32, vp]),
     "pk_res32_offset_norm_add": (i32, [vp, i32, vp, vp, vp, i32, i32, f32, i32, vp]),
@@ -204,6 +210,12 @@ RES32_SIGNATURES = {
     "pk_gemm_strided_gated": (i32, [vp] * 4 + [i32] * 3 + [i64l] * 3 + [i32] + [i64l] * 5 + [i32, vp]),
     "pk_gla_seq": (i32, [vp, i32, i32, i32, i32, vp, i32, i32, vp, f32, vp, i64l, vp, vp, vp, vp] + [i32] * 5 + [vp]),
     "pk_logistic_decay": (i32, [vp, vp, f32, i32, i32, vp]),
+    # 8-bit K/V cache
+    "pk_kv8_page_bytes": (i64l, [i32] * 4),
+    "pk_kv8_append": (i32, [vp, i32] + [vp] * 8 + [i64l] + [i32] * 7 + [vp, f32, i32, i32, vp]),
+    "pk_kv8_attention_workspace_bytes": (i64l, [i32] * 5 + [C.POINTER(Kv8Options), i32]),
+    "pk_kv8_attention": (i32, [vp] * 8 + [i64l] + [i32] * 6 + [f32, C.POINTER(Kv8Options), vp, i64l, i32, vp]),
+    "pk_kv8_evict": (i32, [vp, i64l, i32, vp, vp, vp, vp, i64l, vp, vp, vp, vp, i64l, vp] + [i32] * 8 + [vp]),
 }
 
 
