@@ -78,6 +78,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) kv8_row_kernel(const E* __rest
         }
     }
   }
+  if (l != l) m = INFINITY;  // a NaN among the scores: no other warp or share may hide it
   if (lane == 0) {
     s_m[warp] = m;
     s_l[warp] = l;
@@ -201,23 +202,30 @@ __global__ void __launch_bounds__(128) kv8_mass_row_kernel(const E* __restrict__
 
 // what a call runs: the shares of its keys and its workspace
 struct Plan {
+  bool few;  // kv8_few.cu
+  FewNeed need;
   int shares;
   size_t o_bytes, ml_bytes, lse_bytes;
-  long bytes() const { return (long)(o_bytes + ml_bytes + lse_bytes); }
+  long bytes() const { return (long)((few ? need.bytes() : o_bytes + ml_bytes) + lse_bytes); }
 };
 static size_t up16(size_t n) { return (n + 15) / 16 * 16; }
 static Plan plan(int T, int H, int G, int dim, int vdim, const pk_kv8_options& o, int f32) {
+  Plan p{};
+  if (o.mass && !o.lse) p.lse_bytes = up16((size_t)T * H * sizeof(float));
+  if (!f32 && few_takes(T, H, G, dim, vdim, o.max_kv_len, o.max_q_len)) {
+    p.few = true;
+    p.need = few_need(T, H, G, dim, o.max_kv_len, o.mass != nullptr);
+    return p;
+  }
   int span = o.max_kv_len;
   if (o.window > 0) span = std::min(span, o.window + kBlock);
   const int records = (span + kBlock - 1) / kBlock;
   // a share has at least two rounds of its warps
-  const int shares = std::max(1, std::min((records + 2 * kRowWarps - 1) / (2 * kRowWarps), (4 * sm_count() + T * H - 1) / (T * H)));
-  Plan p{shares, 0, 0, 0};
-  if (shares > 1) {
-    p.o_bytes = up16((size_t)shares * T * H * vdim * sizeof(float));
-    p.ml_bytes = up16((size_t)shares * T * H * sizeof(float2));
+  p.shares = std::max(1, std::min((records + 2 * kRowWarps - 1) / (2 * kRowWarps), (4 * sm_count() + T * H - 1) / (T * H)));
+  if (p.shares > 1) {
+    p.o_bytes = up16((size_t)p.shares * T * H * vdim * sizeof(float));
+    p.ml_bytes = up16((size_t)p.shares * T * H * sizeof(float2));
   }
-  if (o.mass && !o.lse) p.lse_bytes = up16((size_t)T * H * sizeof(float));
   return p;
 }
 
@@ -268,11 +276,13 @@ extern "C" int pk_kv8_attention(const void* q, const void* cache, const void* si
   a.window = options->window;
   a.max_kv_len = options->max_kv_len;
   a.out_ld = options->out_ld ? options->out_ld : (long)heads * vdim;
-  a.part_o = reinterpret_cast<float*>(ws);
-  a.part_ml = reinterpret_cast<float2*>(ws + p.o_bytes);
-  a.lse = options->lse ? options->lse : options->mass ? reinterpret_cast<float*>(ws + p.o_bytes + p.ml_bytes) : nullptr;
+  a.lse = options->lse ? options->lse : options->mass ? reinterpret_cast<float*>(ws) : nullptr;
+  ws += p.lse_bytes;
   a.mass = options->mass;
   a.mass_ld = options->mass_ld;
+  if (p.few) return kv8::few_attention((const bf16*)q, (const bf16*)sink, (bf16*)out, a, p.need, ws, st);
+  a.part_o = reinterpret_cast<float*>(ws);
+  a.part_ml = reinterpret_cast<float2*>(ws + p.o_bytes);
   if (f32) return kv8::attention((const float*)q, (const float*)sink, (float*)out, a, p, st);
   return kv8::attention((const bf16*)q, (const bf16*)sink, (bf16*)out, a, p, st);
 }

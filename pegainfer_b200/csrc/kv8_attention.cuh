@@ -1,6 +1,8 @@
 // Attention over the 8-bit paged cache: what its kernels share.
 #pragma once
 
+#include <climits>
+
 #include "kv8.cuh"
 
 namespace pk {
@@ -45,6 +47,18 @@ __device__ __forceinline__ RowEnd row_end(float M, float den, float sink, bool h
   r.lse = none ? -INFINITY : (top + log2f(den)) * kLn2;
   return r;
 }
+
+// records of a warp's run (kv8_few.cu), an even number: `total` records over `warps` warps
+__host__ __device__ inline int few_run(int total, int warps) { return max(2, ((total + warps - 1) / warps + 1) / 2 * 2); }
+// kv8_few.cu: whether it takes a call, what it needs (bytes), the call itself (with the weights' sums)
+struct FewNeed {
+  size_t o, ml, plan, scores;
+  long scores_ld;
+  size_t bytes() const { return o + ml + plan + scores; }
+};
+bool few_takes(int T, int H, int G, int dim, int vdim, int max_kv_len, int max_q_len);
+FewNeed few_need(int T, int H, int G, int dim, int max_kv_len, bool mass);
+int few_attention(const bf16* q, const bf16* sink, bf16* out, const AttnArgs& a, const FewNeed& need, uint8_t* ws, cudaStream_t st);
 
 }  // namespace kv8
 }  // namespace pk

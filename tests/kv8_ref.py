@@ -61,21 +61,23 @@ class Cache:
         n = self.page // BLOCK
         return self.data[page, :self.G * n * self.rec].view(self.G, n, self.rec)[:, sub]
 
+    def values(self, rec):
+        """records [n, G, bytes] -> K [16 n, G, D] and V [16 n, G, V] in 64 bits"""
+        n, num = rec.shape[0], NUMBERS.to(rec.device)
+        e = rec[..., BLOCK * (self.D + self.V):BLOCK * (self.D + self.V) + 2].contiguous().view(I8).double()
+        kc = rec[..., :BLOCK * self.D].reshape(n, self.G, 2, self.D // 16, 8, 16).transpose(3, 4).reshape(n, self.G, BLOCK, self.D)
+        vc = rec[..., BLOCK * self.D:BLOCK * (self.D + self.V)].reshape(n, self.G, self.V, BLOCK).transpose(2, 3)
+        k, v = num[kc.long()] * torch.exp2(e[..., 0])[..., None, None], num[vc.long()] * torch.exp2(e[..., 1])[..., None, None]
+        return k.transpose(1, 2).reshape(n * BLOCK, self.G, self.D), v.transpose(1, 2).reshape(n * BLOCK, self.G, self.V)
+
     def read(self, r, n, off=None, order=None):
         """K [n, G, D] and V [n, G, V] of a request's first n slots, in 64 bits"""
-        k, v = [], []
-        num = NUMBERS.to(self.data.device)
-        for b in range(-(-n // BLOCK)):
-            rec = self.record(r, b, off, order)
-            e = rec[:, BLOCK * (self.D + self.V):BLOCK * (self.D + self.V) + 2].contiguous().view(I8).double()
-            kc = rec[:, :BLOCK * self.D].reshape(self.G, 2, self.D // 16, 8, 16).permute(0, 1, 3, 2, 4).reshape(self.G, BLOCK, self.D)
-            vc = rec[:, BLOCK * self.D:BLOCK * (self.D + self.V)].reshape(self.G, self.V, BLOCK).transpose(1, 2)
-            k.append((num[kc.long()] * torch.exp2(e[:, 0])[:, None, None]).transpose(0, 1))
-            v.append((num[vc.long()] * torch.exp2(e[:, 1])[:, None, None]).transpose(0, 1))
-        if not k:
-            z = torch.zeros(0, self.G, 1, dtype=F64, device=self.data.device)
-            return z.expand(0, self.G, self.D), z.expand(0, self.G, self.V)
-        return torch.cat(k)[:n], torch.cat(v)[:n]
+        off, order = off or self.off, order or self.order
+        per, b = self.page // BLOCK, torch.arange(-(-n // BLOCK))
+        page = torch.tensor(order, dtype=torch.long)[off[r] + b // per].to(self.data.device)
+        rec = self.data[:, :self.G * per * self.rec].view(-1, self.G, per, self.rec)[page, :, (b % per).to(page.device)]
+        k, v = self.values(rec)
+        return k[:n], v[:n]
 
     def write_record(self, r, b, k, v, bad, ek, ev, off=None, order=None):
         """k [16, G, D], v [16, G, V] values; bad [16, G]: tokens whose key is NaN; ek, ev [G]"""
@@ -115,10 +117,10 @@ def append(cache, r, first, k, v):
     for b in range(first // BLOCK, (first + n - 1) // BLOCK + 1):
         lo, hi = max(first, b * BLOCK), min(first + n, b * BLOCK + BLOCK)
         goes_on = lo > b * BLOCK
-        ok, ov = cache.read(r, b * BLOCK + BLOCK)
-        K, V = torch.zeros_like(ok[:BLOCK]), torch.zeros_like(ov[:BLOCK])
+        ok, ov = cache.values(cache.record(r, b)[None])
+        K, V = torch.zeros_like(ok), torch.zeros_like(ov)
         old = lo - b * BLOCK
-        K[:old], V[:old] = ok[b * BLOCK:lo], ov[b * BLOCK:lo]
+        K[:old], V[:old] = ok[:old], ov[:old]
         K[old:old + hi - lo], V[old:old + hi - lo] = k[lo - first:hi - first], v[lo - first:hi - first]
         bad_v = ~torch.isfinite(V).all(-1)
         bad = ~torch.isfinite(K).all(-1) | bad_v
@@ -129,6 +131,27 @@ def append(cache, r, first, k, v):
         if goes_on:
             ek, ev = [max(e, t[0]) for e, t in zip(ek, tails)], [max(e, t[1]) for e, t in zip(ev, tails)]
         cache.write_record(r, b, K, V, bad, ek, ev)
+
+
+def fill(cache, r, k, v):
+    """append of finite tokens to an empty request, all records at once"""
+    n, nb, per, G = k.shape[0], -(-k.shape[0] // BLOCK), cache.page // BLOCK, cache.G
+    out = []
+    for x in (k, v):
+        y = torch.zeros(nb * BLOCK, G, x.shape[2], dtype=F64)
+        y[:n] = x
+        y = y.view(nb, BLOCK, G, -1).transpose(1, 2)
+        m, e = torch.frexp(y.abs().amax((2, 3)))
+        e = torch.where(m == 0, LOW, torch.where(m <= 0.875, e - 9, e - 8).clamp(LOW, HIGH))
+        out.append((encode(y * torch.exp2(-e.double())[..., None, None], 0), e))
+    (kc, ek), (vc, ev) = out
+    rec = torch.zeros(nb, G, cache.rec, dtype=U8)
+    rec[..., :BLOCK * cache.D] = kc.reshape(nb, G, 2, 8, cache.D // 16, 16).transpose(3, 4).reshape(nb, G, -1)
+    rec[..., BLOCK * cache.D:BLOCK * (cache.D + cache.V)] = vc.transpose(2, 3).reshape(nb, G, -1)
+    rec[..., -16], rec[..., -15] = ek.to(I8).view(U8), ev.to(I8).view(U8)
+    b = torch.arange(nb)
+    page = torch.tensor(cache.order, dtype=torch.long)[cache.off[r] + b // per]
+    cache.data[:, :G * per * cache.rec].view(-1, G, per, cache.rec)[page, :, b % per] = rec
 
 
 def attention(q, k, v, slots, scale, window=0, softcap=0.0, sink=None):

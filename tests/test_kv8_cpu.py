@@ -111,3 +111,14 @@ def test_plain_record_goes_on():
     assert torch.allclose(weights[0], torch.softmax(s, -1)) and torch.allclose(lse[0], torch.logsumexp(s, -1))
     assert torch.allclose(out[0], torch.einsum("hj,jhd->hd", torch.softmax(s, -1), gv.repeat_interleave(2, 1)))
     assert math.isinf(K.attention(w, gk, gv, torch.tensor([-1]), 0.2)[1][0, 0])
+
+
+def test_plain_fill_is_the_plain_append():
+    g = torch.Generator().manual_seed(2)
+    for n, page in ((1, 16), (16, 32), (53, 48)):
+        k, v = torch.randn(n, 3, 32, generator=g).double(), torch.randn(n, 3, 64, generator=g).double()
+        v[n // 2] = 0
+        a, b = K.Cache([n], 3, 32, 64, page, seed=n), K.Cache([n], 3, 32, 64, page, seed=n)
+        K.append(a, 0, 0, k, v)
+        K.fill(b, 0, k, v)
+        assert torch.equal(a.data, b.data)

@@ -72,7 +72,7 @@ def filled(lens, G, D, V, page, seed=0, room=None, **kw):
         if n:
             k = torch.randn(n, G, D, generator=g) * torch.exp(0.5 * torch.randn(1, G, D, generator=g))
             v = torch.randn(n, G, V, generator=g) * torch.exp(0.5 * torch.randn(n, 1, 1, generator=g))
-            K.append(c, r, 0, k.to(BF16).double(), v.to(BF16).double())
+            K.fill(c, r, k.to(BF16).double(), v.to(BF16).double())
     c.data, c.page_off, c.pages = c.data.to(DEV), c.page_off.to(DEV), c.pages.to(DEV)
     return c
 
@@ -372,6 +372,76 @@ def test_captured_and_on_another_stream(lib, T, max_q):
         for x in o:
             assert ((x.double() - want).abs() <= out_bound(want, size, False)).all()
         assert torch.equal(o[0], o[1])
+
+
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("T", [1, 6, 100])
+def test_a_row_that_sees_nothing_but_what_is_not_finite(lib, f32, T):
+    """no share, warp or piece of the keys may hide a NaN behind its largest score"""
+    G, D, n = 2, 64, 2000
+    c = filled([n], G, D, D, 16)
+    for blk in range(n // 16):  # every key of head 1
+        rec = c.record(0, blk)
+        rec[1, :16 * D] = 0x7f
+    q = torch.randn(T, 4, D, device=DEV).to(F32 if f32 else BF16)
+    for window in (0, 1, 40):
+        out, lse = call_attention(lib, c, q, i32(range(n - T, n)), i32([0] * T), 0.125, longest=n, max_q=T, window=window)
+        assert torch.isnan(out[:, 2:]).all() and torch.isnan(lse[:, 2:]).all() and torch.isfinite(out[:, :2]).all() and torch.isfinite(lse[:, :2]).all()
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("T", [3, 100])
+def test_a_query_that_is_not_finite(lib, bad, f32, T):
+    """stays in its row and head"""
+    G, D, n = 2, 64, 300
+    c = filled([n], G, D, D, 16)
+    q = torch.randn(T, 4, D, device=DEV).to(F32 if f32 else BF16)
+    q[1, 1, 5] = bad
+    out, lse = call_attention(lib, c, q, i32(range(n - T, n)), i32([0] * T), 0.125, longest=n, max_q=T)
+    hit = torch.zeros(T, 4, dtype=torch.bool, device=DEV)
+    hit[1, 1] = True
+    assert torch.equal(torch.isnan(out).any(-1), hit) and torch.isfinite(out[~hit]).all() and torch.isnan(out[1, 1]).all()
+
+
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("T", [2, 90])
+def test_rows_that_start_anywhere(lib, f32, T):
+    """queries and results on addresses that only their type aligns"""
+    G, H, D, n = 2, 6, 64, 333
+    E = F32 if f32 else BF16
+    c = filled([n], G, D, D, 16)
+    room = torch.randn(T * H * D + 3, device=DEV).to(E)
+    q = room[3:].view(T, H, D)
+    o = torch.zeros(T * (H * D + 1) + 1, dtype=E, device=DEV)
+    slots, req = i32(range(n - T, n)), i32([0] * T)
+    call_attention(lib, c, q, slots, req, 0.125, longest=n, max_q=T, out_ld=H * D + 1, out=o[1:])
+    want, _, _, size = K.attention(q, *c.read(0, n), slots, 0.125)
+    got = o[1:].view(T, H * D + 1)
+    assert ((got[:, :H * D].reshape(T, H, D).double() - want).abs() <= out_bound(want, size, f32)).all() and (got[:, H * D] == 0).all()
+
+
+@pytest.mark.parametrize("steps", [[(1, 40 + 13 * i) for i in range(600)], [(1, 7)] * 513 + [(1, 3000)], [(1 + i % 7, 20 * (i % 9)) for i in range(200)]], ids=["600", "513", "200x4"])
+def test_many_requests(lib, steps):
+    """more tokens than a launch of the few-row kernel looks at"""
+    check_attention(lib, steps, 4, 1, 64, mass=True)
+
+
+@pytest.mark.parametrize("big", [1e30, 1e-30])
+def test_values_of_very_different_sizes(lib, big):
+    """records whose exponents lie far apart, the large ones first, last and in between: the small ones' part of the result is lost only where it is small"""
+    G, D, n = 1, 64, 200
+    c = K.Cache([n], G, D, D, 16)
+    g = torch.Generator().manual_seed(2)
+    v = torch.randn(n, G, D, generator=g).double()
+    v[64:96] *= big
+    K.append(c, 0, 0, torch.randn(n, G, D, generator=g).double(), v)
+    c.data, c.page_off, c.pages = c.data.to(DEV), c.page_off.to(DEV), c.pages.to(DEV)
+    q = torch.randn(1, 8, D, generator=g).to(BF16).to(DEV)
+    for last in (63, 95, 199):
+        out, _ = call_attention(lib, c, q, i32([last]), i32([0]), 0.125, longest=n, max_q=1)
+        want, _, _, size = K.attention(q, *c.read(0, n), i32([last]), 0.125)
+        assert ((out.double() - want).abs() <= out_bound(want, size, False)).all()
 
 
 # ------------------------------------------------------------------ eviction
