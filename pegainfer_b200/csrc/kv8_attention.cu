@@ -280,7 +280,7 @@ extern "C" int pk_kv8_attention(const void* q, const void* cache, const void* si
   ws += p.lse_bytes;
   a.mass = options->mass;
   a.mass_ld = options->mass_ld;
-  if (p.few) return kv8::few_attention((const bf16*)q, (const bf16*)sink, (bf16*)out, a, p.need, ws, st);
+  if (p.few) return kv8::few_attention((const bf16*)q, (const bf16*)sink, (bf16*)out, a, options->max_q_len, p.need, ws, st);
   a.part_o = reinterpret_cast<float*>(ws);
   a.part_ml = reinterpret_cast<float2*>(ws + p.o_bytes);
   if (f32) return kv8::attention((const float*)q, (const float*)sink, (float*)out, a, p, st);

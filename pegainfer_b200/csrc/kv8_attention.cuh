@@ -58,7 +58,7 @@ struct FewNeed {
 };
 bool few_takes(int T, int H, int G, int dim, int vdim, int max_kv_len, int max_q_len);
 FewNeed few_need(int T, int H, int G, int dim, int max_kv_len, bool mass);
-int few_attention(const bf16* q, const bf16* sink, bf16* out, const AttnArgs& a, const FewNeed& need, uint8_t* ws, cudaStream_t st);
+int few_attention(const bf16* q, const bf16* sink, bf16* out, const AttnArgs& a, int max_q_len, const FewNeed& need, uint8_t* ws, cudaStream_t st);
 
 }  // namespace kv8
 }  // namespace pk
