@@ -6,13 +6,12 @@
 //     score, sum, accumulated values) go through the workspace to kv8_few_merge_kernel.
 //   * A warp's records come by bulk copies (K, V and exponents of 16 tokens: 4112 bytes at 128 entries) through a ring of its own, two records to a stage; no
 //     warp waits for another.
-//   * mma.sync m16n8k16 in f16: K's and V's codes become f16 in registers (exactly; two codes an instruction), q becomes f16 with a power of two for each row that
-//     puts its largest entry at 2^14 .. 2^15 (bf16 entries down to 2^-21 of it stay exact), and P, which is held 2^15 times too large, keeps 11 bits down to 2^-29.
-//     (The e4m3 form of mma.sync, with q and P as two codes each, is two of these products and the conversion of both operands every time: 828 instead of 400
-//     instructions for 32 tokens.)
+//   * mma.sync m16n8k16 in f16, turned round: S^T = K q^T and O^T = V^T P^T, so that 16 tokens (16 entries of V) fill a product's long side and up to eight rows its
+//     short one; a tile of up to 16 rows (WIDE) takes two.  K's and V's codes become f16 in registers (exactly; two codes an instruction), q becomes f16 with a power of
+//     two for each row that puts its largest entry at 2^14 .. 2^15 (bf16 entries down to 2^-21 of it stay exact), and P, which is held 2^15 times too large,
+//     keeps 11 bits down to 2^-29.  movmatrix turns P.  (The e4m3 form of mma.sync is two of these products and a conversion of both operands each time.)
 //   * Scores: the exponents of K and of the row's q multiply them.  P takes V's exponent e in as 2^(e - E), E the largest so far, so that records of different
 //     exponents add up.
-//   * A tile of up to eight rows leaves the lower half of the product empty, and its exponentials out (HALF).
 // A group of more than 16 heads is several tiles, which read the records again (from L2).
 #include <algorithm>
 
@@ -27,14 +26,17 @@ constexpr int kTopQ = 14, kTopP = 15;  // exponents of the largest entry of a ro
 template <int D>
 constexpr int few_warps() { return D <= 128 ? 8 : 4; }
 template <int D>
-constexpr int few_stages() { return D == 128 || D == 256 ? 3 : 4; }
+constexpr int few_stages() { return D <= 64 ? 4 : D <= 96 ? 3 : 2; }
 
 struct FewArgs {
   AttnArgs a;
-  int t_first, U, per;      // first token of the launch; tiles of a token (kv heads x eights of rows), tokens of a tile
-  int q_by4;                // q's rows start on 8-byte boundaries
+  int t_first, U, per;      // first token of the launch; tiles of a token (kv heads x sixteens of rows), tokens of a tile
+  int abreast;              // warps that go through the same records of different tiles of a token
+  int q_by4, out_by4;       // rows start on 8-byte boundaries
+  uint32_t inv_r;           // row / R = row * inv_r >> 16 for the rows of a tile
   int* plan;                // [T + 1] records before a token's tiles, [T] the tile's first token, the length of a run: for the merge
-  float* scores;            // [T, H, scores_ld] scores (log2), for the weights' sums; or null
+  float* scores;            // scores (log2) for the weights' sums, or null: [tiles of a token][t_all][min(R, 16)][scores_ld], a tile's at its first token as [slot][row]
+  int t_all;                // tokens of the call
   long scores_ld;
   unsigned int* err;
 };
@@ -58,6 +60,12 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
+// an 8 x 8 matrix of f16 turned round
+__device__ __forceinline__ uint32_t turned(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // two entries that need not lie on a 4-byte boundary
@@ -65,16 +73,16 @@ __device__ __forceinline__ uint32_t two(const bf16* p) {
   return (uint32_t)__bfloat16_as_ushort(p[0]) | (uint32_t)__bfloat16_as_ushort(p[1]) << 16;
 }
 
-template <int D, bool SCORES, bool HALF>
+template <int D, bool SCORES, bool WIDE>
 __global__ void __launch_bounds__(few_warps<D>() * 32, 1) kv8_few_kernel(const bf16* __restrict__ q, const bf16* __restrict__ sink, bf16* __restrict__ out, const FewArgs f) {
-  constexpr int WARPS = few_warps<D>(), ST = few_stages<D>(), REC = kBlock * 2 * D + 16, THREADS = WARPS * 32, ROWS = HALF ? 1 : 2;
+  constexpr int WARPS = few_warps<D>(), ST = few_stages<D>(), REC = kBlock * 2 * D + 16, THREADS = WARPS * 32, NT = WIDE ? 2 : 1;
   extern __shared__ __align__(128) uint8_t fw_sm[];
   __shared__ int s_pre[kFewTokens + 1], s_b0[kFewTokens], s_off[kFewTokens], s_req[kFewTokens], s_slot[kFewTokens], s_scan[WARPS], s_scan2[WARPS];
   __shared__ uint64_t s_full[WARPS][ST];
   __shared__ int s_dead;
   const AttnArgs& a = f.a;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gq = lane >> 2, tq = lane & 3;
-  const int R = a.H / a.pool.G, O = (R + 15) / 16, U = f.U, per = f.per;
+  const int R = a.H / a.pool.G, O = (R + 15) / 16, AB = f.abreast, U = f.U / AB, per = f.per;  // U: of the tiles that a warp sees
   volatile int* dead = &s_dead;
   if (tid == 0) s_dead = 0;
   if (lane == 0)
@@ -85,14 +93,19 @@ __global__ void __launch_bounds__(few_warps<D>() * 32, 1) kv8_few_kernel(const b
 
   // ---- the tiles of the step: their first records and how many, summed up.  Threads have consecutive tokens.
   {
-    constexpr int N = kFewTokens / THREADS;
+    constexpr int N = (kFewTokens + THREADS - 1) / THREADS;
     const int T = a.T;
     int req[N], start[N], n[N], mine = 0, from = -1;
-    for (int t = tid; t < T; t += THREADS) {
+    int off[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int t = tid + i * THREADS;
+      off[i] = 0;
+      if (t >= T) continue;
       const int r = a.req[t], p = a.slots[t];
       s_req[t] = r;
       s_slot[t] = p;
-      s_off[t] = p >= 0 ? a.pool.page_off[r] : 0;
+      if (p >= 0) off[i] = a.pool.page_off[r];  // under way until the tiles are known
     }
     __syncthreads();
 #pragma unroll
@@ -131,7 +144,6 @@ __global__ void __launch_bounds__(few_warps<D>() * 32, 1) kv8_few_kernel(const b
       if (top < 0) continue;
       const int b0 = a.window > 0 ? max(0, low - a.window + 1) / kBlock : 0;
       s_b0[t] = b0;
-      if (s_slot[t] < 0) s_off[t] = a.pool.page_off[req[i]];
       n[i] = top / kBlock - b0 + 1;
       mine += n[i];
     }
@@ -142,6 +154,9 @@ __global__ void __launch_bounds__(few_warps<D>() * 32, 1) kv8_few_kernel(const b
       if (lane >= d) sum += o;
     }
     if (lane == 31) s_scan2[warp] = sum;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (tid + i * THREADS < T) s_off[tid + i * THREADS] = off[i];
     __syncthreads();
     sum -= mine;
     for (int w = 0; w < warp; ++w) sum += s_scan2[w];
@@ -155,18 +170,21 @@ __global__ void __launch_bounds__(few_warps<D>() * 32, 1) kv8_few_kernel(const b
     __syncthreads();
   }
   const int total = s_pre[a.T] * U;
-  const int run = few_run(total, (int)gridDim.x * WARPS);
+  const int run = few_run(total, (int)gridDim.x * WARPS / AB);
   if (blockIdx.x == 0) {
     for (int t = tid; t <= a.T; t += THREADS) f.plan[t] = s_pre[t];
     if (tid == 0) f.plan[2 * a.T + 1] = run;
   }
-  const int x0 = min((blockIdx.x * WARPS + warp) * (long)run, (long)total), x1 = min(x0 + run, total);
+  const int who = (blockIdx.x * WARPS + warp) / AB, mine = warp % AB;
+  const int x0 = min(who * (long)run, (long)total), x1 = min(x0 + run, total);
 
   // ---- the run's records: stages of two, never of two tiles
+  constexpr int TURN_LD = D + 4;
   uint8_t* ring = fw_sm + (size_t)warp * ST * 2 * REC;
-  const int rpp = a.pool.page_size / kBlock;
+  float* turn = reinterpret_cast<float*>(fw_sm + (size_t)WARPS * ST * 2 * REC) + warp * 8 * TURN_LD;
+  const int rpp = a.pool.page_size / kBlock, rpp_shift = (rpp & (rpp - 1)) == 0 ? 31 - __clz(rpp) : -1;
   struct Cursor {
-    int t, u, rec, n;  // token of the tile, which of its tiles, record inside, records of the tile
+    int t, u, rec, n;  // token of the tile, which of its tiles (u * AB + mine), record inside, records of the tile
   };
   auto locate = [&](int x) {
     int lo = 0, hi = a.T;  // s_pre[lo] <= x / U < s_pre[hi]
@@ -190,119 +208,174 @@ __global__ void __launch_bounds__(few_warps<D>() * 32, 1) kv8_few_kernel(const b
     while (c.t < a.T && s_pre[c.t + 1] == s_pre[c.t]);
     c.n = c.t < a.T ? s_pre[c.t + 1] - s_pre[c.t] : 0;
   };
-  // the copies' own walk along the run; lanes 0 and 1 know where the next stage's records are
+  // the copies' own walk along the run: px is where the next stage begins, p_take its records
   Cursor pc{0, 0, 0, 0};
-  int px = x0, p_take = 0;
+  int px = x0, p_take = 0, p_b0 = 0, p_off = 0, p_g = 0;
   const uint8_t* p_src = nullptr;
-  auto look_up = [&] {  // of the stage at px
-    p_take = min(2, min(pc.n - pc.rec, x1 - px));
-    if (lane < p_take) {
-      const int b = s_b0[pc.t] + pc.rec + lane, g = pc.u / O;
-      p_src = a.pool.data + (size_t)a.pool.pages[s_off[pc.t] + b / rpp] * a.pool.page_stride + (size_t)(g * rpp + b % rpp) * REC;
-    }
+  auto enter = [&] {
+    p_b0 = s_b0[pc.t];
+    int t = pc.t;
+    while (s_slot[t] < 0) ++t;  // (a tile with records has a token with a slot)
+    p_off = s_off[t];
+    p_g = (pc.u * AB + mine) / O;
   };
-  auto advance = [&] {
+  auto source = [&](int b0, int off, int g, int rec) {
+    const int b = b0 + rec, page = rpp_shift >= 0 ? b >> rpp_shift : b / rpp;
+    return a.pool.data + (size_t)a.pool.pages[off + page] * a.pool.page_stride + (size_t)(g * rpp + b - page * rpp) * REC;
+  };
+  auto step = [&] {  // on to the next stage
     px += p_take;
     pc.rec += p_take;
     if (px >= x1) {
       p_take = 0;
       return;
     }
-    if (pc.rec == pc.n) next_tile(pc);
-    look_up();
+    if (pc.rec == pc.n) {
+      next_tile(pc);
+      enter();
+    }
+    p_take = min(2, min(pc.n - pc.rec, x1 - px));
   };
-  auto issue = [&](int s) {
-    if (p_take <= 0) return;
-    if (lane == 0) mbar_expect_tx(&s_full[warp][s], p_take * REC);
-    __syncwarp();
-    if (lane < p_take)
-      asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(ring + (s * 2 + lane) * REC)), "l"(p_src),
-                   "r"(REC), "r"(smem_u32(&s_full[warp][s]))
-                   : "memory");
+  auto copy = [&](int s, int r, const uint8_t* src) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(ring + (s * 2 + r) * REC)), "l"(src), "r"(REC),
+                 "r"(smem_u32(&s_full[warp][s]))
+                 : "memory");
+  };
+  // the rows of q that this lane turns into f16: of tile (t, unit)
+  auto tokens_of = [&](int t) {
+    int n = 1;
+    while (n < per && t + n < a.T && s_req[t + n] == s_req[t]) ++n;
+    return n;
+  };
+  uint2 raw[NT][D / 16];
+  auto load_q = [&](const Cursor& cur) {
+    const int unit = cur.u * AB + mine, g = unit / O, n_tok = tokens_of(cur.t);
+#pragma unroll
+    for (int w = 0; w < NT; ++w) {
+      const int row = unit % O * 16 + 8 * w + gq, k = (int)((uint32_t)row * f.inv_r >> 16);
+      const bool on = row < R * per && k < n_tok;
+      const bf16* src = q + ((size_t)(cur.t + (on ? k : 0)) * a.H + g * R + (on ? row - k * R : 0)) * D + 4 * tq;
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) {
+        raw[w][i] = make_uint2(0, 0);
+        if (on) {
+          if (f.q_by4) raw[w][i] = *reinterpret_cast<const uint2*>(src + i * 16);
+          else raw[w][i] = make_uint2(two(src + i * 16), two(src + i * 16 + 2));
+        }
+      }
+    }
   };
   int issued = 0;
+  Cursor first{0, 0, 0, 0};
   if (x0 < x1) {
-    pc = locate(x0);
-    look_up();
-    for (int s = 0; s < ST; ++s) {
-      if (p_take > 0) ++issued;
-      issue(s);
-      advance();
+    first = locate(x0);
+    load_q(first);  // ahead of the copies in the memory's queues
+  }
+  if (x0 < x1) {  // the first stages: their pages are looked up by a lane each
+    pc = first;
+    enter();
+    p_take = min(2, min(pc.n - pc.rec, x1 - px));
+    int b0 = 0, off = 0, g = 0, rec = -1;
+    for (int s = 0; s < ST && p_take > 0; ++s) {
+      if (lane >> 1 == s && (lane & 1) < p_take) {
+        b0 = p_b0;
+        off = p_off;
+        g = p_g;
+        rec = pc.rec + (lane & 1);
+      }
+      if (lane == 0) mbar_expect_tx(&s_full[warp][s], p_take * REC);
+      ++issued;
+      step();
     }
+    __syncwarp();
+    if (rec >= 0) copy(lane >> 1, lane & 1, source(b0, off, g, rec));
+    if (lane < p_take) p_src = source(p_b0, p_off, p_g, pc.rec + lane);  // of the next one: lanes 0 and 1
   }
 
-  // shared-memory offsets of this lane's rows for ldmatrix: K (matrix: 8 tokens x 16 entries; of the two products of a record the first has, for the thread that
-  // holds them, the lower or the upper two of its four tokens, so that a matrix' rows lie in eight different groups of banks), V (8 entries x 16 tokens)
-  const int mi = lane >> 3, mr = lane & 7, mt = 4 * (mr >> 1) + (((mi >> 1) ^ (mr >> 2)) << 1) + (mr & 1);
-  const uint32_t k_at = (uint32_t)((mt >> 3) * (8 * D) + (mi & 1) * 128 + (mt & 7) * 16);
-  const uint32_t v_at = (uint32_t)(kBlock * D + (mi >> 1) * 128 + mr * 16);
-  const float c = a.scale * kLog2e;
+  // shared-memory offsets of this lane's rows for ldmatrix.  K: 8 tokens x 16 entries; the first and the second eight of a product's 16 tokens are, behind the turn, the
+  // lower or the upper two of a thread's four tokens, chosen so that the eight rows lie in different groups of banks.  V: 8 entries x 16 tokens.
+  const int mi = lane >> 3, mr = lane & 7;
+  auto token_of = [](int which, int i) { return 4 * (i >> 1) + (((i >> 2) ^ which) << 1) + (i & 1); };
+  const int mt = token_of(mi & 1, mr);
+  const uint32_t k_at = (uint32_t)((mt >> 3) * (8 * D) + (mi >> 1) * 128 + (mt & 7) * 16);
+  const uint32_t v_at = (uint32_t)(kBlock * D + (mi & 1) * 128 + mr * 16);
+  const int tok[2] = {token_of(0, gq), token_of(1, gq)};  // this thread's tokens of a record
+  const float c = a.scale * kLog2e, cap2 = a.cap * kLog2e, cap_c = a.cap > 0.f ? 2.f * a.scale / a.cap * kLog2e : 0.f;
 
   uint32_t parity = 0;
   int slot = 0;
   bool alive = true;
-  Cursor cc{0, 0, 0, 0};
-  if (x0 < x1) cc = locate(x0);
+  Cursor cc = first;
   for (int x = x0; x < x1;) {
-    // ---- a piece: the run's records of one tile
+    // ---- a piece: the run's records of one tile.  Row r of the tile: token t + r / R, head r % R of the group (from the tile's 16 on).
     const int count = min(cc.n - cc.rec, x1 - x);
-    const int t = cc.t, g = cc.u / O;
-    // rows gq and gq + 8 of the tile: token t + row / R, head row % R of the group (from the tile's 16 on).  Rows that the tile does not have see all and go
-    // nowhere: the masks are left out where every row sees a stage whole.
-    int tr[ROWS], h[ROWS], p[ROWS], lo[ROWS];
-    bool on[ROWS];
-    float row_c[ROWS];  // what a product of q's f16 and K's codes is multiplied with, but for K's exponent
-    uint32_t qa[D / 16][2 * ROWS];
+    const int t = cc.t, unit = cc.u * AB + mine, g = unit / O, row0 = unit % O * 16;
+    const int n_tok = tokens_of(t);
+    auto token = [&](int row) {  // -1: no such row
+      const int k = (int)((uint32_t)row * f.inv_r >> 16);
+      return row < R * per && k < n_tok ? t + k : -1;
+    };
+    auto head = [&](int row) { return row - (int)((uint32_t)row * f.inv_r >> 16) * R; };
+    uint32_t qb[D / 16][2 * NT];
+    float row_c[2 * NT];  // what a product of q's f16 and K's codes is multiplied with, but for K's exponent; rows 8 w + 2 tq + e at 2 w + e
+    int p[2 * NT], lo[2 * NT];
 #pragma unroll
-    for (int i = 0; i < ROWS; ++i) {
-      const int row = (cc.u % O) * 16 + gq + 8 * i, ti = t + row / R;
-      on[i] = row < R * per && ti < a.T && s_req[min(ti, a.T - 1)] == s_req[t];
-      tr[i] = on[i] ? ti : t;
-      h[i] = g * R + (on[i] ? row % R : 0);
-      p[i] = on[i] ? s_slot[tr[i]] : INT_MAX;
-      lo[i] = on[i] && a.window > 0 ? p[i] - a.window + 1 : 0;
-      const bf16* src = q + ((size_t)tr[i] * a.H + h[i]) * D + 4 * tq;
-      uint2 raw[D / 16];
+    for (int w = 0; w < NT; ++w) {
       float amax = 0.f;
 #pragma unroll
-      for (int k = 0; k < D / 16; ++k) {
-        raw[k] = make_uint2(0, 0);
-        if (on[i]) {
-          if (f.q_by4) raw[k] = *reinterpret_cast<const uint2*>(src + k * 16);
-          else raw[k] = make_uint2(two(src + k * 16), two(src + k * 16 + 2));
-        }
-        amax = fmaxf(fmaxf(amax, fmaxf(fabsf(bf16_lo(raw[k].x)), fabsf(bf16_hi(raw[k].x)))), fmaxf(fabsf(bf16_lo(raw[k].y)), fabsf(bf16_hi(raw[k].y))));
-      }
+      for (int k = 0; k < D / 16; ++k)
+        amax = fmaxf(fmaxf(amax, fmaxf(fabsf(bf16_lo(raw[w][k].x)), fabsf(bf16_hi(raw[w][k].x)))), fmaxf(fabsf(bf16_lo(raw[w][k].y)), fabsf(bf16_hi(raw[w][k].y))));
       amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
       amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
       const int e = min(max((int)(__float_as_uint(amax) >> 23) - 127 - kTopQ, kLowExp), kHighExp);
-      const float down = pow2(-e), qf = amax == INFINITY ? NAN : pow2(e);  // (an infinite entry: the row is NaN)
-      row_c[i] = a.cap > 0.f ? qf : qf * c;
+      const float down = pow2(-e), qf = amax == INFINITY ? NAN : a.cap > 0.f ? pow2(e) : pow2(e) * c;  // (an infinite entry: the row is NaN)
 #pragma unroll
       for (int k = 0; k < D / 16; ++k) {
-        qa[k][i] = pack_f16(bf16_lo(raw[k].x) * down, bf16_hi(raw[k].x) * down);
-        qa[k][ROWS + i] = pack_f16(bf16_lo(raw[k].y) * down, bf16_hi(raw[k].y) * down);
+        qb[k][2 * w] = pack_f16(bf16_lo(raw[w][k].x) * down, bf16_hi(raw[w][k].x) * down);
+        qb[k][2 * w + 1] = pack_f16(bf16_lo(raw[w][k].y) * down, bf16_hi(raw[w][k].y) * down);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        row_c[2 * w + i] = __shfl_sync(0xffffffffu, qf, (2 * tq + i) * 4);
+        const int to = token(row0 + 8 * w + 2 * tq + i);
+        // rows that the tile does not have see all and go nowhere: the masks are left out where every row sees a stage whole
+        p[2 * w + i] = to >= 0 ? s_slot[to] : INT_MAX;
+        lo[2 * w + i] = to >= 0 && a.window > 0 ? s_slot[to] - a.window + 1 : 0;
       }
     }
-    float o[D / 8][4];
+    int all_lo = 0, all_p = INT_MAX;
 #pragma unroll
-    for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-    float m[ROWS], l[ROWS];
+    for (int i = 0; i < 2 * NT; ++i) {
+      all_lo = max(all_lo, lo[i]);
+      all_p = min(all_p, p[i]);
+    }
+    all_lo = __reduce_max_sync(0xffffffffu, all_lo);
+    all_p = __reduce_min_sync(0xffffffffu, all_p);
+    float o[D / 16][NT][4];
 #pragma unroll
-    for (int i = 0; i < ROWS; ++i) {
+    for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+      for (int w = 0; w < NT; ++w) o[d][w][0] = o[d][w][1] = o[d][w][2] = o[d][w][3] = 0.f;
+    float m[2 * NT], l[2 * NT];
+#pragma unroll
+    for (int i = 0; i < 2 * NT; ++i) {
       m[i] = -INFINITY;
       l[i] = 0.f;
     }
-    const int all_lo = __reduce_max_sync(0xffffffffu, ROWS == 2 ? max(lo[0], lo[ROWS - 1]) : lo[0]);
-    const int all_p = __reduce_min_sync(0xffffffffu, ROWS == 2 ? min(p[0], p[ROWS - 1]) : p[0]);
-    int E = kLowExp - 1;
-    for (int i = 0; i < count;) {
+    int tile_rows = 0;  // of the tile
+    float* kept = nullptr;
+    if constexpr (SCORES) {
+      while (tile_rows < 16 && token(row0 + tile_rows) >= 0) tile_rows += R <= 16 ? R : 1;
+      kept = f.scores + ((size_t)unit * f.t_all + f.t_first + t) * min(R, 16) * f.scores_ld;
+    }
+    int E = kLowExp - 1, j0 = (s_b0[t] + cc.rec) * kBlock;
+    for (int i = 0; i < count; j0 += 2 * kBlock) {
       const int take = min(2, count - i);
       if (alive) alive = mbar_wait_bounded(&s_full[warp][slot], parity, dead);
       __syncwarp();
       const uint8_t* stage = ring + slot * 2 * REC;
       const uint32_t at = smem_u32(stage), second = take == 2 ? REC : 0;  // (a missing second record: the first again, with P = 0)
-      float s[4][4] = {};
+      float s[2][NT][4] = {};
 #pragma unroll
       for (int kk = 0; kk < D / 32; ++kk) {
 #pragma unroll
@@ -310,147 +383,181 @@ __global__ void __launch_bounds__(few_warps<D>() * 32, 1) kv8_few_kernel(const b
           uint32_t b[4];
           ldsm_x4_at(b, at + (r ? second : 0) + k_at + kk * 256);
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {  // product x / 2 of the record, piece of 16 entries 2 kk + x % 2
-            uint32_t b0, b1;
-            widen(b[x], b0, b1);
-            const uint32_t(&qk)[2 * ROWS] = qa[2 * kk + (x & 1)];
-            mma_f16(s[2 * r + (x >> 1)], qk[0], ROWS == 2 ? qk[1] : 0u, qk[ROWS], ROWS == 2 ? qk[2 * ROWS - 1] : 0u, b0, b1);
+          for (int y = 0; y < 2; ++y) {  // 16 entries each
+            uint32_t a0, a1, a2, a3;
+            widen(b[2 * y], a0, a2);
+            widen(b[2 * y + 1], a1, a3);
+#pragma unroll
+            for (int w = 0; w < NT; ++w) mma_f16(s[r][w], a0, a1, a2, a3, qb[2 * kk + y][2 * w], qb[2 * kk + y][2 * w + 1]);
           }
         }
       }
       const uint32_t tail_a = *reinterpret_cast<const uint32_t*>(stage + kBlock * 2 * D), tail_b = *reinterpret_cast<const uint32_t*>(stage + second + kBlock * 2 * D);
-      const int j0 = (s_b0[t] + cc.rec + i) * kBlock;
       const bool inside = j0 >= all_lo && j0 + 31 <= all_p && take == 2;
       const int ea = tail_ev(tail_a), eb = tail_ev(tail_b), e_new = max(E, max(ea, eb));
-      const float fe = pow2(max(E - e_new, -126));
+      const float fe = pow2(max(E - e_new, -126)), fka = pow2(tail_ek(tail_a)), fkb = pow2(tail_ek(tail_b));
       E = e_new;
-      float fo[ROWS], ref[ROWS];
+      float fo[2 * NT], ref[2 * NT];
+      bool same = true;
 #pragma unroll
-      for (int w = 0; w < ROWS; ++w) {
-        float mx = m[w];
+      for (int i2 = 0; i2 < 2 * NT; ++i2) {
+        const int w = i2 >> 1, e = i2 & 1;
+        float mx = m[i2];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const float fk = pow2(tail_ek(r ? tail_b : tail_a)) * row_c[w];
+          const float fk = (r ? fkb : fka) * row_c[i2];
 #pragma unroll
-          for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              float v = s[2 * r + n][2 * w + e] * fk;
-              if (a.cap > 0.f) v = shaped(v, c, a.cap);
-              if (!inside) {
-                const int j = j0 + 16 * r + 4 * tq + ((n ^ (tq >> 1)) << 1) + e;
-                v = j >= lo[w] && j <= p[w] && r < take ? v : -INFINITY;
-              }
-              s[2 * r + n][2 * w + e] = v;
-              mx = fmaxf(mx, v);
+          for (int y = 0; y < 2; ++y) {
+            float v = s[r][w][2 * y + e] * fk;
+            if (a.cap > 0.f) v = fmaf(-2.f * cap2, __fdividef(1.f, ex2(fminf(v * cap_c, 80.f)) + 1.f), cap2);  // cap tanh(x) = cap - 2 cap / (e^(2 x) + 1)
+            if (!inside) {
+              const int j = j0 + 16 * r + tok[y];
+              v = j >= lo[i2] && j <= p[i2] && r < take ? v : -INFINITY;
             }
+            s[r][w][2 * y + e] = v;
+            mx = fmaxf(mx, v);
+          }
         }
-        if constexpr (SCORES) {
-          if (on[w]) {
-            float* to = f.scores + ((size_t)(f.t_first + tr[w]) * a.H + h[w]) * f.scores_ld + j0 + 4 * tq;
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+        ref[i2] = mx == -INFINITY ? 0.f : mx;
+        const float fl = ex2(m[i2] - ref[i2]);
+        fo[i2] = fl * fe;
+        same = same && fo[i2] == 1.f;
+        m[i2] = mx;
+        l[i2] *= fl;
+      }
+      if constexpr (SCORES) {  // [slot][row of the tile]
 #pragma unroll
-            for (int r = 0; r < 2; ++r)
-              if (r < take && j0 + 16 * r + kBlock <= f.scores_ld) {
-                const float w0 = s[2 * r][2 * w], w1 = s[2 * r][2 * w + 1], w2 = s[2 * r + 1][2 * w], w3 = s[2 * r + 1][2 * w + 1];
-                *reinterpret_cast<float4*>(to + 16 * r) = tq < 2 ? make_float4(w0, w1, w2, w3) : make_float4(w2, w3, w0, w1);
+        for (int w = 0; w < NT; ++w)
+#pragma unroll
+          for (int r = 0; r < 2; ++r)
+            if (r < take && j0 + 16 * r + kBlock <= f.scores_ld)
+#pragma unroll
+              for (int y = 0; y < 2; ++y) {
+                float* dst = kept + (size_t)(j0 + 16 * r + tok[y]) * tile_rows + 8 * w + 2 * tq;
+                const int left = tile_rows - 8 * w - 2 * tq;
+                if (left >= 2 && tile_rows % 2 == 0) {
+                  *reinterpret_cast<float2*>(dst) = make_float2(s[r][w][2 * y], s[r][w][2 * y + 1]);
+                } else {
+                  if (left >= 1) dst[0] = s[r][w][2 * y];
+                  if (left >= 2) dst[1] = s[r][w][2 * y + 1];
+                }
               }
-          }
-        }
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        ref[w] = mx == -INFINITY ? 0.f : mx;
-        const float fl = ex2(m[w] - ref[w]);
-        fo[w] = fl * fe;
-        m[w] = mx;
-        l[w] *= fl;
       }
-      if (__any_sync(0xffffffffu, fo[0] != 1.f || fo[ROWS - 1] != 1.f)) {
+      if (__any_sync(0xffffffffu, !same)) {
 #pragma unroll
-        for (int d = 0; d < D / 8; ++d)
+        for (int d = 0; d < D / 16; ++d)
 #pragma unroll
-          for (int w = 0; w < ROWS; ++w) {
-            o[d][2 * w] *= fo[w];
-            o[d][2 * w + 1] *= fo[w];
-          }
+          for (int w = 0; w < NT; ++w)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) o[d][w][k] *= fo[2 * w + (k & 1)];
       }
-      uint32_t pa[2][2 * ROWS];  // of a record: the lower and the upper two of the thread's four tokens, for its rows
+      uint32_t pb[2][2 * NT];  // of a record: tokens 4 tq, 4 tq + 1 and 4 tq + 2, 4 tq + 3 of row gq
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         const float fv = pow2(max((r ? eb : ea) - E, -100) + kTopP);
 #pragma unroll
-        for (int w = 0; w < ROWS; ++w) {
+        for (int w = 0; w < NT; ++w) {
           uint32_t y[2];
 #pragma unroll
           for (int n = 0; n < 2; ++n) {
-            const float p0 = ex2(s[2 * r + n][2 * w] - ref[w]), p1 = ex2(s[2 * r + n][2 * w + 1] - ref[w]);
-            l[w] += p0 + p1;
-            y[n] = pack_f16(p0 * fv, p1 * fv);
+            const float p0 = ex2(s[r][w][2 * n] - ref[2 * w]), p1 = ex2(s[r][w][2 * n + 1] - ref[2 * w + 1]);
+            l[2 * w] += p0;
+            l[2 * w + 1] += p1;
+            y[n] = turned(pack_f16(p0 * fv, p1 * fv));
           }
-          pa[r][w] = tq < 2 ? y[0] : y[1];
-          pa[r][ROWS + w] = tq < 2 ? y[1] : y[0];
+          pb[r][2 * w] = tq < 2 ? y[0] : y[1];
+          pb[r][2 * w + 1] = tq < 2 ? y[1] : y[0];
         }
       }
 #pragma unroll
       for (int d = 0; d < D / 16; ++d) {
         uint32_t b[4];
-        ldsm_x4_at(b, at + (mi & 1 ? second : 0) + v_at + d * 256);
+        ldsm_x4_at(b, at + (mi & 2 ? second : 0) + v_at + d * 256);
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {  // record x % 2, entries 8 (2 d + x / 2) ..
-          uint32_t b0, b1;
-          widen(b[x], b0, b1);
-          const uint32_t(&pr)[2 * ROWS] = pa[x & 1];
-          mma_f16(o[2 * d + (x >> 1)], pr[0], ROWS == 2 ? pr[1] : 0u, pr[ROWS], ROWS == 2 ? pr[2 * ROWS - 1] : 0u, b0, b1);
+        for (int r = 0; r < 2; ++r) {
+          uint32_t a0, a1, a2, a3;
+          widen(b[2 * r], a0, a2);
+          widen(b[2 * r + 1], a1, a3);
+#pragma unroll
+          for (int w = 0; w < NT; ++w) mma_f16(o[d][w], a0, a1, a2, a3, pb[r][2 * w], pb[r][2 * w + 1]);
         }
       }
       i += take;
       __syncwarp();
-      if (alive) {
-        if (p_take > 0) {
-          ++issued;
-          fence_async_smem();
-        }
-        issue(slot);
-        advance();
+      if (alive && p_take > 0) {  // this stage is free again
+        ++issued;
+        fence_async_smem();
+        if (lane == 0) mbar_expect_tx(&s_full[warp][slot], p_take * REC);
+        __syncwarp();
+        if (lane < p_take) copy(slot, lane, p_src);
+        step();
+        if (lane < p_take) p_src = source(p_b0, p_off, p_g, pc.rec + lane);
       }
       if (++slot == ST) {
         slot = 0;
         parity ^= 1u;
       }
     }
+    // ---- the piece's state: the accumulated values are turned back in shared memory, so that rows leave in 16-byte pieces
     const float up = pow2(max(E, kLowExp) - kTopP);
+    const bool whole = count == cc.n;
+    const size_t part = (((size_t)who + (size_t)t * U + cc.u) * AB + mine) * (8 * NT);
 #pragma unroll
-    for (int w = 0; w < ROWS; ++w) {
-      l[w] += __shfl_xor_sync(0xffffffffu, l[w], 1);
-      l[w] += __shfl_xor_sync(0xffffffffu, l[w], 2);
-      if (l[w] != l[w]) m[w] = INFINITY;  // a NaN among the scores: no other piece may hide it
-      if (count == cc.n) {
-        const RowEnd end = row_end(m[w], l[w], sink ? bf2f(sink[h[w]]) : 0.f, sink != nullptr);
-        if (on[w]) {
-          const float fac = end.factor * up;
-          bf16* dst = out + (size_t)tr[w] * a.out_ld + h[w] * D + 2 * tq;
-          const bool pair = (reinterpret_cast<uintptr_t>(out) & 3) == 0 && (a.out_ld & 1) == 0;
+    for (int w = 0; w < NT; ++w) {
 #pragma unroll
-          for (int d = 0; d < D / 8; ++d) {
-            if (pair) {
-              *reinterpret_cast<uint32_t*>(dst + d * 8) = pack_bf16(o[d][2 * w] * fac, o[d][2 * w + 1] * fac);
-            } else {
-              dst[d * 8] = f2bf(o[d][2 * w] * fac);
-              dst[d * 8 + 1] = f2bf(o[d][2 * w + 1] * fac);
-            }
-          }
-          if (tq == 0 && a.lse) a.lse[(size_t)tr[w] * a.H + h[w]] = end.lse;
+      for (int e = 0; e < 2; ++e) {
+        const int r = 8 * w + 2 * tq + e, to = token(row0 + r), h = g * R + (to >= 0 ? head(row0 + r) : 0);
+        float sum = l[2 * w + e];
+        sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+        const float top = sum != sum ? INFINITY : m[2 * w + e];  // a NaN among the scores: no other piece may hide it
+        float fac = up;
+        if (whole) {
+          const RowEnd end = row_end(top, sum, sink ? bf2f(sink[h]) : 0.f, sink != nullptr);
+          fac *= end.factor;
+          if (gq == 0 && to >= 0 && a.lse) a.lse[(size_t)to * a.H + h] = end.lse;
+        } else if (gq == 0 && to >= 0) {
+          a.part_ml[part + r] = make_float2(top, sum);
         }
-      } else if (on[w]) {
-        const size_t at = ((size_t)(blockIdx.x * WARPS + warp) + (size_t)t * U + cc.u) * (8 * ROWS) + gq + 8 * w;
-        float* dst = a.part_o + at * D + 2 * tq;
 #pragma unroll
-        for (int d = 0; d < D / 8; ++d) *reinterpret_cast<float2*>(dst + d * 8) = make_float2(o[d][2 * w] * up, o[d][2 * w + 1] * up);
-        if (tq == 0) a.part_ml[at] = make_float2(m[w], l[w]);
+        for (int d = 0; d < D / 16; ++d) {
+          turn[(2 * tq + e) * TURN_LD + d * 16 + gq] = o[d][w][e] * fac;
+          turn[(2 * tq + e) * TURN_LD + d * 16 + 8 + gq] = o[d][w][2 + e] * fac;
+        }
       }
+      __syncwarp();
+      for (int r = 0; r < 8; ++r) {
+        const int to = token(row0 + 8 * w + r);
+        if (to < 0) continue;
+        for (int d = lane * 4; d < D; d += 128) {
+          const float4 v = *reinterpret_cast<const float4*>(turn + r * TURN_LD + d);
+          if (whole) {
+            bf16* dst = out + (size_t)to * a.out_ld + (g * R + head(row0 + 8 * w + r)) * D + d;
+            if (f.out_by4) {
+              *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
+            } else {
+              dst[0] = f2bf(v.x);
+              dst[1] = f2bf(v.y);
+              dst[2] = f2bf(v.z);
+              dst[3] = f2bf(v.w);
+            }
+          } else {
+            *reinterpret_cast<float4*>(a.part_o + (part + 8 * w + r) * D + d) = v;
+          }
+        }
+      }
+      __syncwarp();
     }
     x += count;
     cc.rec += count;
-    if (cc.rec == cc.n && x < x1) next_tile(cc);
+    if (x < x1) {
+      next_tile(cc);
+      load_q(cc);
+    }
   }
   if (!alive) {  // copies under way land in shared memory: their barriers were armed in order
     for (int j = max(0, issued - ST); j < issued; ++j) mbar_drain(&s_full[warp][j % ST], (uint32_t)(j / ST & 1));
@@ -469,24 +576,25 @@ __global__ void __launch_bounds__(256) kv8_few_merge_kernel(const bf16* __restri
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = warp % share, rh = blockIdx.x * (8 / share) + warp / share, rows = a.T * a.H;
   const int t = min(rh, rows - 1) / a.H, h = min(rh, rows - 1) - t * a.H, R = a.H / a.pool.G, O = (R + 15) / 16;
   const int first = f.plan[a.T + 1 + t], run = f.plan[2 * a.T + 1], before = f.plan[first], n = f.plan[first + 1] - before;
-  const int row = (t - first) * R + h % R, u = h / R * O + row / 16;
-  const int x0 = before * f.U + u * n, w0 = x0 / run, pieces = n > 0 ? (x0 + n - 1) / run - w0 + 1 : 0;
-  const size_t at = ((size_t)w0 + (size_t)first * f.U + u) * tile_rows + row % 16;  // of the first piece; the others a tile further each
+  const int row = (t - first) * R + h % R, u = h / R * O + row / 16, AB = f.abreast, U = f.U / AB;
+  const int x0 = before * U + u / AB * n, w0 = x0 / run, pieces = n > 0 ? (x0 + n - 1) / run - w0 + 1 : 0;
+  const size_t at = (((size_t)w0 + (size_t)first * U + u / AB) * AB + u % AB) * tile_rows + row % 16;  // of the first piece; the others so much further each:
+  const size_t apart = (size_t)AB * tile_rows;
   float M = -INFINITY, den = 0.f;
   constexpr int PAIRS = D / 2, NP = (PAIRS + 31) / 32, AT_ONCE = 8 / NP;
   float2 acc[NP];
 #pragma unroll
   for (int i = 0; i < NP; ++i) acc[i] = make_float2(0.f, 0.f);
   if (pieces > 1) {
-    for (int s = lane; s < pieces; s += 32) M = fmaxf(M, a.part_ml[at + (size_t)s * tile_rows].x);
+    for (int s = lane; s < pieces; s += 32) M = fmaxf(M, a.part_ml[at + s * apart].x);
     M = warp_max(M);
     for (int s0 = part; s0 < pieces; s0 += AT_ONCE * share) {
       float2 v[AT_ONCE][NP], ml[AT_ONCE];
 #pragma unroll
       for (int k = 0; k < AT_ONCE; ++k) {
         const int s = s0 + k * share;
-        ml[k] = s < pieces ? a.part_ml[at + (size_t)s * tile_rows] : make_float2(-INFINITY, 0.f);
-        const float2* src = reinterpret_cast<const float2*>(a.part_o + (at + (size_t)s * tile_rows) * D) + lane;
+        ml[k] = s < pieces ? a.part_ml[at + s * apart] : make_float2(-INFINITY, 0.f);
+        const float2* src = reinterpret_cast<const float2*>(a.part_o + (at + s * apart) * D) + lane;
 #pragma unroll
         for (int i = 0; i < NP; ++i) v[k][i] = s < pieces && lane + 32 * i < PAIRS ? src[32 * i] : make_float2(0.f, 0.f);
       }
@@ -533,19 +641,29 @@ __global__ void __launch_bounds__(256) kv8_few_merge_kernel(const bf16* __restri
 }
 
 // weights of the keys out of the kept scores and the finished lse, summed over a run's tokens and the group's heads in their order: a thread to (slot, kv head, run)
-__global__ void __launch_bounds__(256) kv8_few_mass_kernel(const float* __restrict__ scores, long scores_ld, AttnArgs a) {
+__global__ void __launch_bounds__(256) kv8_few_mass_kernel(FewArgs f) {
   pdl_wait();
   pdl_launch_dependents();
-  const int t0 = blockIdx.z, g = blockIdx.y, R = a.H / a.pool.G, req = a.req[t0], j = blockIdx.x * 256 + threadIdx.x;
+  const AttnArgs& a = f.a;
+  const int t0 = blockIdx.z, g = blockIdx.y, R = a.H / a.pool.G, O = (R + 15) / 16, req = a.req[t0], j = blockIdx.x * 256 + threadIdx.x;
   if (t0 > 0 && a.req[t0 - 1] == req) return;  // a run's first token
   float sum = 0.f;
   bool any = false;
-  for (int t = t0; t < a.T && a.req[t] == req; ++t) {
-    const int p = a.slots[t];
-    if (j > p || (a.window > 0 && j <= p - a.window) || j >= scores_ld) continue;
-    any = true;
-    const size_t row = (size_t)t * a.H + g * R;
-    for (int r = 0; r < R; ++r) sum += ex2(scores[(row + r) * scores_ld + j] - a.lse[row + r] * kLog2e);
+  for (int t = t0; t < a.T && a.req[t] == req;) {  // tiles: at most `per` tokens, none over the end of a launch of the first kernel
+    const int most = min(f.per, min(a.T, (t / kFewTokens + 1) * kFewTokens) - t);
+    int n = 1;
+    while (n < most && a.req[t + n] == req) ++n;
+    for (int o = 0; o < O; ++o) {
+      const int rows = R <= 16 ? n * R : min(16, R - 16 * o);
+      const float* s = f.scores + (((size_t)(g * O + o) * f.t_all + t) * min(R, 16)) * f.scores_ld + (size_t)j * rows;
+      for (int r = 0; r < rows; ++r) {
+        const int to = t + (R <= 16 ? r / R : 0), p = a.slots[to];
+        if (j > p || (a.window > 0 && j <= p - a.window) || j >= f.scores_ld) continue;
+        any = true;
+        sum += ex2(s[r] - a.lse[(size_t)to * a.H + g * R + (R <= 16 ? r % R : 16 * o + r)] * kLog2e);
+      }
+    }
+    t += n;
   }
   if (any && j < a.mass_ld) a.mass[((size_t)req * a.pool.G + g) * a.mass_ld + j] += sum;
 }
@@ -561,20 +679,20 @@ static cudaError_t follow(void (*kernel)(KArgs...), dim3 grid, dim3 block, cudaS
   return e;
 }
 
-template <int D, bool SCORES, bool HALF>
+template <int D, bool SCORES, bool WIDE>
 static int launch_few(const bf16* q, const bf16* sink, bf16* out, const FewArgs& f, int ctas, cudaStream_t st) {
-  constexpr size_t smem = (size_t)few_warps<D>() * few_stages<D>() * 2 * (kBlock * 2 * D + 16);
+  constexpr size_t smem = (size_t)few_warps<D>() * (few_stages<D>() * 2 * (kBlock * 2 * D + 16) + 8 * (D + 4) * sizeof(float));
   static std::atomic<uint64_t> set{0};
-  if (const cudaError_t e = allow_smem(set, (const void*)kv8_few_kernel<D, SCORES, HALF>, smem); e != cudaSuccess) return (int)e;
-  if (const cudaError_t e = launch(kv8_few_kernel<D, SCORES, HALF>, dim3(ctas), dim3(few_warps<D>() * 32), smem, st, true, q, sink, out, f); e != cudaSuccess) return (int)e;
+  if (const cudaError_t e = allow_smem(set, (const void*)kv8_few_kernel<D, SCORES, WIDE>, smem); e != cudaSuccess) return (int)e;
+  if (const cudaError_t e = launch(kv8_few_kernel<D, SCORES, WIDE>, dim3(ctas), dim3(few_warps<D>() * 32), smem, st, true, q, sink, out, f); e != cudaSuccess) return (int)e;
   // few rows have many pieces each
   const int rows = f.a.T * f.a.H, share = rows <= 4 * sm_count() ? 8 : rows <= 16 * sm_count() ? 2 : 1;
-  return (int)follow(kv8_few_merge_kernel<D>, dim3((rows * share + 7) / 8), dim3(256), st, sink, out, share, HALF ? 8 : 16, f);
+  return (int)follow(kv8_few_merge_kernel<D>, dim3((rows * share + 7) / 8), dim3(256), st, sink, out, share, WIDE ? 16 : 8, f);
 }
 template <int D>
-static int launch_few(const bf16* q, const bf16* sink, bf16* out, const FewArgs& f, int ctas, bool half, cudaStream_t st) {
-  if (f.scores) return half ? launch_few<D, true, true>(q, sink, out, f, ctas, st) : launch_few<D, true, false>(q, sink, out, f, ctas, st);
-  return half ? launch_few<D, false, true>(q, sink, out, f, ctas, st) : launch_few<D, false, false>(q, sink, out, f, ctas, st);
+static int launch_few(const bf16* q, const bf16* sink, bf16* out, const FewArgs& f, int ctas, bool wide, cudaStream_t st) {
+  if (f.scores) return wide ? launch_few<D, true, true>(q, sink, out, f, ctas, st) : launch_few<D, true, false>(q, sink, out, f, ctas, st);
+  return wide ? launch_few<D, false, true>(q, sink, out, f, ctas, st) : launch_few<D, false, false>(q, sink, out, f, ctas, st);
 }
 
 bool few_takes(int T, int H, int G, int dim, int vdim, int max_kv_len, int max_q_len) {
@@ -593,7 +711,7 @@ FewNeed few_need(int T, int H, int G, int dim, int max_kv_len, bool mass) {
   n.plan = ((size_t)2 * few_tokens(T) + 2) * sizeof(int);
   n.plan = (n.plan + 15) / 16 * 16;
   n.scores_ld = (max_kv_len + kBlock - 1) / kBlock * kBlock;
-  n.scores = mass ? (size_t)T * H * n.scores_ld * sizeof(float) : 0;
+  n.scores = mass ? (size_t)U * T * std::min(H / G, 16) * n.scores_ld * sizeof(float) : 0;
   return n;
 }
 
@@ -601,12 +719,16 @@ int few_attention(const bf16* q, const bf16* sink, bf16* out, const AttnArgs& al
   const int D = all.pool.dim, R = all.H / all.pool.G;
   FewArgs f{};
   f.U = all.pool.G * ((R + 15) / 16);
-  const bool half = max_q_len > 0 && R * max_q_len <= 8;  // the rows of a tile fit into half a product
-  f.per = half ? max_q_len : std::max(1, 16 / R);
+  const bool wide = max_q_len <= 0 || R * max_q_len > 8;  // the rows of a tile do not fit into one product
+  f.abreast = f.U % few_warps_of(D) == 0 ? few_warps_of(D) : few_warps_of(D) % f.U == 0 ? f.U : 1;
+  f.per = wide ? std::max(1, 16 / R) : max_q_len;
   f.plan = reinterpret_cast<int*>(ws);
   f.scores = all.mass ? reinterpret_cast<float*>(ws + need.plan) : nullptr;
   f.scores_ld = need.scores_ld;
+  f.t_all = all.T;
+  f.inv_r = (65536u + R - 1) / R;
   f.q_by4 = (reinterpret_cast<uintptr_t>(q) & 7) == 0;
+  f.out_by4 = (reinterpret_cast<uintptr_t>(out) & 7) == 0 && all.out_ld % 4 == 0;
   f.err = wait_err_word();
   uint8_t* rest = ws + need.plan + need.scores;
   for (int t = 0; t < all.T; t += kFewTokens) {
@@ -623,17 +745,18 @@ int few_attention(const bf16* q, const bf16* sink, bf16* out, const AttnArgs& al
     const int ctas = (int)std::max(1L, std::min((long)sm_count(), (most + 2 * few_warps_of(D) - 1) / (2 * few_warps_of(D))));
     const bf16* qt = q + (size_t)t * a.H * D;
     bf16* ot = out + (size_t)t * a.out_ld;
-    const int rc = D == 32    ? launch_few<32>(qt, sink, ot, f, ctas, half, st)
-                   : D == 64  ? launch_few<64>(qt, sink, ot, f, ctas, half, st)
-                   : D == 96  ? launch_few<96>(qt, sink, ot, f, ctas, half, st)
-                   : D == 128 ? launch_few<128>(qt, sink, ot, f, ctas, half, st)
-                   : D == 192 ? launch_few<192>(qt, sink, ot, f, ctas, half, st)
-                              : launch_few<256>(qt, sink, ot, f, ctas, half, st);
+    const int rc = D == 32    ? launch_few<32>(qt, sink, ot, f, ctas, wide, st)
+                   : D == 64  ? launch_few<64>(qt, sink, ot, f, ctas, wide, st)
+                   : D == 96  ? launch_few<96>(qt, sink, ot, f, ctas, wide, st)
+                   : D == 128 ? launch_few<128>(qt, sink, ot, f, ctas, wide, st)
+                   : D == 192 ? launch_few<192>(qt, sink, ot, f, ctas, wide, st)
+                              : launch_few<256>(qt, sink, ot, f, ctas, wide, st);
     if (rc != 0) return rc;
   }
   if (!all.mass) return 0;
   const int keys = (int)std::min((long)all.max_kv_len, all.mass_ld);
-  return (int)follow(kv8_few_mass_kernel, dim3((keys + 255) / 256, all.pool.G, all.T), dim3(256), st, (const float*)f.scores, f.scores_ld, all);
+  f.a = all;
+  return (int)follow(kv8_few_mass_kernel, dim3((keys + 255) / 256, all.pool.G, all.T), dim3(256), st, f);
 }
 
 }  // namespace kv8
