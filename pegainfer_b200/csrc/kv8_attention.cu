@@ -202,7 +202,7 @@ __global__ void __launch_bounds__(128) kv8_mass_row_kernel(const E* __restrict__
 
 // what a call runs: the shares of its keys and its workspace
 struct Plan {
-  bool few;  // kv8_few.cu
+  bool few, prompt;  // kv8_few.cu, kv8_prompt.cu
   FewNeed need;
   int shares;
   size_t o_bytes, ml_bytes, lse_bytes;
@@ -215,6 +215,10 @@ static Plan plan(int T, int H, int G, int dim, int vdim, const pk_kv8_options& o
   if (!f32 && few_takes(T, H, G, dim, vdim, o.max_kv_len, o.max_q_len)) {
     p.few = true;
     p.need = few_need(T, H, G, dim, o.max_kv_len, o.mass != nullptr);
+    return p;
+  }
+  if (!f32 && prompt_takes(T, H, G, dim, vdim)) {
+    p.prompt = true;
     return p;
   }
   int span = o.max_kv_len;
@@ -230,15 +234,17 @@ static Plan plan(int T, int H, int G, int dim, int vdim, const pk_kv8_options& o
 }
 
 template <typename E>
+static int mass_rows(const E* q, const AttnArgs& a, cudaStream_t st) {
+  return (int)launch(kv8_mass_row_kernel<E>, dim3((a.max_kv_len + 63) / 64, a.pool.G), dim3(128), 0, st, true, q, a);
+}
+template <typename E>
 static int attention(const E* q, const E* sink, E* out, const AttnArgs& a, const Plan& p, cudaStream_t st) {
   const size_t smem = (size_t)(a.pool.dim + kRowWarps * a.pool.vdim) * sizeof(float);
   if (const cudaError_t e = launch(kv8_row_kernel<E>, dim3(a.T, a.H, p.shares), dim3(kRowWarps * 32), smem, st, true, q, sink, out, a); e != cudaSuccess) return (int)e;
   if (p.shares > 1)
     if (const cudaError_t e = launch(kv8_merge_kernel<E>, dim3((unsigned)(((size_t)a.T * a.H + 3) / 4)), dim3(128), 0, st, true, sink, out, p.shares, a); e != cudaSuccess)
       return (int)e;
-  if (a.mass)
-    return (int)launch(kv8_mass_row_kernel<E>, dim3((a.max_kv_len + 63) / 64, a.pool.G), dim3(128), 0, st, true, q, a);
-  return 0;
+  return a.mass ? mass_rows(q, a, st) : 0;
 }
 
 static bool options_ok(const pk_kv8_options* o, int tokens, int heads, int kv_heads, int vdim) {
@@ -281,6 +287,10 @@ extern "C" int pk_kv8_attention(const void* q, const void* cache, const void* si
   a.mass = options->mass;
   a.mass_ld = options->mass_ld;
   if (p.few) return kv8::few_attention((const bf16*)q, (const bf16*)sink, (bf16*)out, a, options->max_q_len, p.need, ws, st);
+  if (p.prompt) {
+    const int rc = kv8::prompt_attention((const bf16*)q, (const bf16*)sink, (bf16*)out, a, st);
+    return rc != 0 || !a.mass ? rc : kv8::mass_rows((const bf16*)q, a, st);
+  }
   a.part_o = reinterpret_cast<float*>(ws);
   a.part_ml = reinterpret_cast<float2*>(ws + p.o_bytes);
   if (f32) return kv8::attention((const float*)q, (const float*)sink, (float*)out, a, p, st);

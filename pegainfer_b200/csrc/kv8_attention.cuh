@@ -60,5 +60,9 @@ bool few_takes(int T, int H, int G, int dim, int vdim, int max_kv_len, int max_q
 FewNeed few_need(int T, int H, int G, int dim, int max_kv_len, bool mass);
 int few_attention(const bf16* q, const bf16* sink, bf16* out, const AttnArgs& a, int max_q_len, const FewNeed& need, uint8_t* ws, cudaStream_t st);
 
+// kv8_prompt.cu: whether it takes a call, and the call (no workspace)
+bool prompt_takes(int T, int H, int G, int dim, int vdim);
+int prompt_attention(const bf16* q, const bf16* sink, bf16* out, const AttnArgs& a, cudaStream_t st);
+
 }  // namespace kv8
 }  // namespace pk

@@ -698,7 +698,8 @@ static int launch_few(const bf16* q, const bf16* sink, bf16* out, const FewArgs&
 bool few_takes(int T, int H, int G, int dim, int vdim, int max_kv_len, int max_q_len) {
   if (T > 65535 || dim != vdim || !(dim == 32 || dim == 64 || dim == 96 || dim == 128 || dim == 192 || dim == 256)) return false;
   if ((long)std::min(T, kFewTokens) * G * ((H / G + 15) / 16) * (max_kv_len / kBlock + 2) >= 1L << 31) return false;
-  return max_q_len > 0 ? max_q_len <= 16 || T < 64 : T < 64;
+  // (where the kernel for prompts does not take the heads' size, any call: its rows in tiles of 16)
+  return T < 64 || (max_q_len > 0 && max_q_len <= 16) || !prompt_takes(T, H, G, dim, vdim);
 }
 static int few_tokens(int T) { return std::min(T, kFewTokens); }
 static int few_warps_of(int dim) { return dim <= 128 ? 8 : 4; }

@@ -1,0 +1,608 @@
+// Attention over the 8-bit paged cache for prompts and prompt portions, on tcgen05 (kv8.cuh, kv8_attention.cuh).
+//
+// A CTA has two tiles of 128 rows of one kv head: the group's R query heads of 128 / R consecutive tokens each, so that a key is fetched once for the whole group and
+// few scores lie behind the diagonal.  It goes through the keys in blocks of 128, run by run where its tokens belong to several requests (the other rows are masked).
+//   * K's and V's codes are operands as they lie in the cache: a record's K is two groups of 8 tokens and its V one column of 16 tokens of the canonical layout without
+//     swizzle (8 x 16-byte matrices), so plain bulk copies fill the operands and nothing is converted.
+//   * kind::f8f6f4 wants both operands in 8 bits at most.  q and P have more, so each goes in as two numbers, the nearest e4m3 and the rest as e5m2, whose exponents
+//     reach 2^10 further down (4 + 1 + 3 significant bits; bf16 has 8): S = q_hi K^T + q_lo K^T and O += P_hi V + P_lo V, as many cycles as one product in
+//     16 bits.  A row of q is scaled by a power of two to the upper end of the codes' range: a bf16 entry is exact down to 2^-17 of the row's largest.  P is held 2^8
+//     times too large: a weight is off by at most 2^-8 of it down to 2^-14 of the largest, and by 2^-25 of the largest below 2^-22.  (With the rest in e4m3 too, scores of
+//     a peaked row were off by 1.4e-4 and weights by 2^-18 of the largest.)
+//   * K's exponents multiply the scores 16 columns at a time, V's go into P's exponent: 2^(s - m + e - E + 8), E the largest so far; the denominator takes them out.
+//   * The softmax is a thread per row, 128 a tile, with the tiles in turn; O stays in tensor memory and is rescaled by a third group of warps where a maximum moved.
+// Warps: 0-3 softmax tile 0 | 4-7 softmax tile 1 | 8-11 rescaling, results | 12, 13 MMA issuers | 14 copies.
+// Tensor memory: S0 | S1 (128 columns each, P over the first 64: 32 of hi, 32 of lo) | O0 | O1.
+#include <algorithm>
+
+#include "kv8_attention.cuh"
+#include "tcgen05.cuh"
+
+namespace pk {
+namespace kv8 {
+
+constexpr int kPrRows = 128, kPrKeys = 128, kPrRecords = kPrKeys / kBlock;
+constexpr int kPrStages = 3;
+constexpr int kPrCorr = 8, kPrMma = 12, kPrLoad = 14, kPrThreads = 15 * 32;
+constexpr int kPrEarly = 3;        // k-steps of 32 keys of P V that begin before the last one's P is there
+constexpr int kPrTop = 8;          // exponent of P = 1
+constexpr uint32_t kRestA = 1u << 7;  // instruction descriptor: A is e5m2
+constexpr int kPrMaxSeg = 256;     // runs that a CTA's tokens can belong to
+
+struct PromptArgs {
+  AttnArgs a;
+  int per;           // tokens of a tile
+  int q_by8, out_by8;
+  unsigned int* err;
+};
+
+__device__ __forceinline__ float pr_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void pr_fma2(float& x0, float& x1, float s, float c) {
+  unsigned long long v, sv, cv;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x0), "f"(x1));
+  asm("mov.b64 %0, {%1, %1};" : "=l"(sv) : "f"(s));
+  asm("mov.b64 %0, {%1, %1};" : "=l"(cv) : "f"(c));
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(v), "l"(sv), "l"(cv));
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(x0), "=f"(x1) : "l"(v));
+}
+// operand without swizzle, inner dimension contiguous: 8 x 16-byte matrices of 128 bytes; lead: to the next one along the inner dimension, stride: to the next
+// eight rows
+__device__ __forceinline__ uint64_t plain_desc(uint32_t smem_addr, uint32_t lead, uint32_t stride) {
+  return (uint64_t)((smem_addr >> 4) & 0x3fff) | (uint64_t)((lead >> 4) & 0x3fff) << 16 | (uint64_t)((stride >> 4) & 0x3fff) << 32 | (uint64_t)1 << 46;
+}
+__device__ __forceinline__ void umma_f8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// A from tensor memory: lane = row, four consecutive inner elements a column
+__device__ __forceinline__ void umma_f8_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void pr_put8(uint32_t taddr, const uint32_t* v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]),
+               "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+__device__ __forceinline__ void pr_copy(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+}
+// two values of P -> two e4m3 codes and two e5m2 codes of the rest
+__device__ __forceinline__ void split2(float p0, float p1, uint32_t& hi, uint32_t& lo) {
+  asm("{\n\t.reg .b32 h, b, r;\n\t.reg .b16 c, d;\n\t"
+      "cvt.rn.f16x2.f32 h, %3, %2;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f16x2 c, h;\n\t"
+      "cvt.rn.f16x2.e4m3x2 b, c;\n\t"
+      "sub.rn.f16x2 r, h, b;\n\t"
+      "cvt.rn.satfinite.e5m2x2.f16x2 d, r;\n\t"
+      "cvt.u32.u16 %0, c;\n\tcvt.u32.u16 %1, d;\n\t}"
+      : "=r"(hi), "=r"(lo)
+      : "f"(p0), "f"(p1));
+}
+
+__device__ __forceinline__ uint32_t rest4(float a, float b, float c, float d) {
+  uint16_t x, y;
+  asm("cvt.rn.satfinite.e5m2x2.f32 %0, %1, %2;" : "=h"(x) : "f"(b), "f"(a));
+  asm("cvt.rn.satfinite.e5m2x2.f32 %0, %1, %2;" : "=h"(y) : "f"(d), "f"(c));
+  return (uint32_t)x | (uint32_t)y << 16;
+}
+
+template <int D>
+__global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* __restrict__ q, const bf16* __restrict__ sink, bf16* __restrict__ out, const PromptArgs f) {
+  constexpr int QB = kPrRows * D, KB = kPrKeys * D, REC_K = kBlock * D;  // bytes of a part of q's tile, of a stage's K (or V), of a record's K
+  extern __shared__ uint8_t pr_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pr_raw) + 127) & ~(uintptr_t)127);
+  uint8_t* Qs = smem;                                    // [tile][hi, lo]
+  uint8_t* Ks = Qs + 4 * QB;                             // [stage]
+  uint8_t* Vs = Ks + kPrStages * KB;                     // [stage]
+  uint8_t* Ts = Vs + kPrStages * KB;                     // [stage][record] tails
+  float* alpha_s = reinterpret_cast<float*>(Ts + kPrStages * kPrRecords * 16);  // [tile][row]
+  float* end_s = alpha_s + 2 * kPrRows;                  // [tile][row]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(end_s + 2 * kPrRows);
+  uint64_t *k_full = bars, *k_empty = bars + 4, *v_full = bars + 8, *v_empty = bars + 12;  // [stage]
+  uint64_t* s_full = bars + 16;    // [tile] S complete                                      MMA -> softmax
+  uint64_t* po_ready = bars + 18;  // [tile] P up to kPrEarly stored, O rescaled (4 + 4 warps)  softmax, rescaling -> MMA
+  uint64_t* p_rest = bars + 20;    // [tile] the rest of P stored (4 warps)                    softmax -> MMA
+  uint64_t* a_ready = bars + 22;   // [tile] factors of O published (4 warps)                  softmax -> rescaling
+  uint64_t* pv_done = bars + 24;   // [tile] P V complete                                     MMA -> rescaling
+  uint64_t* d_ready = bars + 26;   // [tile] last factors published (4 warps)                  softmax -> results
+  uint64_t* done = bars + 28;      // behind a run-out: the MMAs under way
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 29);
+  volatile int* dead = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  __shared__ int s_req[2 * kPrRows], s_slot[2 * kPrRows], s_seg[2 * kPrRows];
+  __shared__ int seg_off[kPrMaxSeg], seg_lo[2][kPrMaxSeg], seg_hi[2][kPrMaxSeg];  // page table of a run; blocks of keys that its rows of a tile see
+  __shared__ int s_count[kPrThreads / 32], s_segs;
+
+  const AttnArgs& a = f.a;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int g = blockIdx.x, R = a.H / a.pool.G, per = f.per;
+  const int t0 = ((int)gridDim.y - 1 - (int)blockIdx.y) * 2 * per, n_tok = min(2 * per, a.T - t0);  // late tokens, which see most, first
+
+  if (tid == 0) {
+    for (int s = 0; s < kPrStages; ++s) {
+      mbar_init(k_full + s, 1);
+      mbar_init(k_empty + s, 2);
+      mbar_init(v_full + s, 1);
+      mbar_init(v_empty + s, 2);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(s_full + i, 1);
+      mbar_init(po_ready + i, 8);
+      mbar_init(p_rest + i, 4);
+      mbar_init(a_ready + i, 4);
+      mbar_init(pv_done + i, 1);
+      mbar_init(d_ready + i, 4);
+    }
+    mbar_init(done, 2);
+    *dead = 0;
+    mbar_fence_init();
+  }
+  if (warp == kPrMma) tmem_alloc(tmem_slot, 512);
+  pdl_wait();
+  pdl_launch_dependents();
+
+  // ---- the runs that the tokens belong to
+  for (int i = tid; i < kPrMaxSeg; i += kPrThreads)
+    for (int k = 0; k < 2; ++k) {
+      seg_lo[k][i] = INT_MAX;
+      seg_hi[k][i] = -1;
+    }
+  bool begins = false;
+  int my_req = 0, my_slot = -1;
+  if (tid < n_tok) {
+    my_req = a.req[t0 + tid];
+    my_slot = a.slots[t0 + tid];
+    begins = tid == 0 || a.req[t0 + tid - 1] != my_req;
+    s_req[tid] = my_req;
+    s_slot[tid] = my_slot;
+  }
+  const uint32_t starts = __ballot_sync(0xffffffffu, begins);
+  if (lane == 0) s_count[warp] = __popc(starts);
+  __syncthreads();
+  {
+    int before = 0;
+    for (int w = 0; w < warp; ++w) before += s_count[w];
+    const int seg = before + __popc(starts & (0xffffffffu >> (31 - lane))) - 1;
+    if (tid < n_tok) {
+      s_seg[tid] = seg;
+      if (my_slot >= 0) {
+        const int tile = tid >= per, lo = a.window > 0 ? max(0, my_slot - a.window + 1) : 0;
+        atomicMin(&seg_lo[tile][seg], lo / kPrKeys);
+        atomicMax(&seg_hi[tile][seg], my_slot / kPrKeys);
+        seg_off[seg] = a.pool.page_off[my_req];  // (the same from every token of the run)
+      }
+    }
+    if (tid == 0) {
+      int all = 0;
+      for (int w = 0; w < kPrThreads / 32; ++w) all += s_count[w];
+      s_segs = all;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  const int segs = s_segs;
+  WaitTries tries;
+  auto first_block = [&](int seg) { return min(seg_lo[0][seg], seg_lo[1][seg]); };
+  auto last_block = [&](int seg) { return max(seg_hi[0][seg], seg_hi[1][seg]); };
+  auto needs = [&](int tile, int seg, int j) { return j >= seg_lo[tile][seg] && j <= seg_hi[tile][seg]; };
+
+  if (warp == kPrLoad) {
+    // =========================== copies ===========================
+    int n = 0;
+    bool go = true;  // false behind a run-out: a barrier must not be armed twice in one phase
+    for (int seg = 0; seg < segs && go; ++seg) {
+      const int j1 = last_block(seg);
+      if (j1 < 0) continue;
+      // the run's last slot that anybody here has: records behind it may not exist
+      int top = -1;
+      for (int i = lane; i < n_tok; i += 32)
+        if (s_seg[i] == seg) top = max(top, s_slot[i]);
+      top = __reduce_max_sync(0xffffffffu, top) / kBlock;
+      const int off = seg_off[seg], rpp = a.pool.page_size / kBlock;
+      auto source = [&](int j) {  // lane i: the block's i-th record, the last one again behind the end
+        const int b = min(j * kPrRecords + min(lane, kPrRecords - 1), top);
+        return a.pool.data + (size_t)a.pool.pages[off + b / rpp] * a.pool.page_stride + (size_t)(g * rpp + b % rpp) * (2 * REC_K + 16);
+      };
+      const uint8_t* src = source(first_block(seg));
+      for (int j = first_block(seg); j <= j1 && go; ++j, ++n) {
+        const int s = n % kPrStages;
+        const uint32_t ph = (uint32_t)((n / kPrStages) & 1) ^ 1u;
+        const uint8_t* now = src;
+        if (j < j1) src = source(j + 1);
+        go = mbar_wait_bounded(k_empty + s, ph, dead, tries);
+        if (!go) break;
+        if (lane == 0) mbar_expect_tx(k_full + s, KB);
+        __syncwarp();
+        if (lane < kPrRecords) pr_copy(smem_u32(Ks + s * KB) + lane * REC_K, now, REC_K, k_full + s);
+        go = mbar_wait_bounded(v_empty + s, ph, dead, tries);
+        if (!go) break;
+        if (lane == 0) mbar_expect_tx(v_full + s, KB + kPrRecords * 16);
+        __syncwarp();
+        if (lane < kPrRecords) {
+          pr_copy(smem_u32(Vs + s * KB) + lane * REC_K, now + REC_K, REC_K, v_full + s);
+          pr_copy(smem_u32(Ts + (s * kPrRecords + lane) * 16), now + 2 * REC_K, 16, v_full + s);
+        }
+      }
+    }
+    if (!go) wait_for_copies();
+  } else if (warp >= kPrMma) {
+    // =========================== MMA issuers, one per tile ===========================
+    const int i = warp - kPrMma;
+    asm volatile("bar.sync 1, %0;" ::"n"(10 * 32) : "memory");  // q is there
+    constexpr uint32_t idesc_s = (1u << 4) | ((uint32_t)(kPrKeys >> 3) << 17) | ((uint32_t)(kPrRows >> 4) << 24);  // e4m3 x e4m3 -> fp32, both inner-contiguous
+    constexpr uint32_t idesc_pv = (1u << 4) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(kPrRows >> 4) << 24);
+    const uint64_t q_hi = plain_desc(smem_u32(Qs + i * 2 * QB), 128, 8 * D), q_lo = plain_desc(smem_u32(Qs + (i * 2 + 1) * QB), 128, 8 * D);
+    const uint32_t t_s = tmem_base + (uint32_t)(i * kPrKeys), t_o = tmem_base + (uint32_t)(2 * kPrKeys + i * 128);
+    int n = 0, mine = 0;  // blocks so far, of them this tile's
+    // S of the next block of this tile is issued behind P V of the last one: `pending` is that block
+    int p_stage = -1;
+    auto finish = [&] {  // P V of the pending block
+      const int s = p_stage;
+      mbar_wait_bounded(po_ready + i, (uint32_t)((mine - 1) & 1), dead, tries);
+      tc_fence_after();
+      const uint64_t v_desc = plain_desc(smem_u32(Vs + s * KB), REC_K, 128);
+      if (tc_elect_one()) {
+#pragma unroll
+        for (int k = 0; k < kPrEarly; ++k) {
+          umma_f8_ts(t_o, t_s + (uint32_t)(k * 8), v_desc + (uint64_t)(k * (2 * REC_K >> 4)), idesc_pv, (mine > 1 || k > 0) ? 1u : 0u);
+          umma_f8_ts(t_o, t_s + (uint32_t)(32 + k * 8), v_desc + (uint64_t)(k * (2 * REC_K >> 4)), idesc_pv | kRestA, 1u);
+        }
+      }
+      __syncwarp();
+      mbar_wait_bounded(p_rest + i, (uint32_t)((mine - 1) & 1), dead, tries);
+      tc_fence_after();
+      if (tc_elect_one()) {
+#pragma unroll
+        for (int k = kPrEarly; k < kPrKeys / 32; ++k) {
+          umma_f8_ts(t_o, t_s + (uint32_t)(k * 8), v_desc + (uint64_t)(k * (2 * REC_K >> 4)), idesc_pv, 1u);
+          umma_f8_ts(t_o, t_s + (uint32_t)(32 + k * 8), v_desc + (uint64_t)(k * (2 * REC_K >> 4)), idesc_pv | kRestA, 1u);
+        }
+        umma_commit(pv_done + i);
+        umma_commit(v_empty + s);
+      }
+      __syncwarp();
+      p_stage = -1;
+    };
+    for (int seg = 0; seg < segs; ++seg) {
+      const int j1 = last_block(seg);
+      for (int j = j1 < 0 ? 0 : first_block(seg); j <= j1; ++j, ++n) {
+        const int s = n % kPrStages;
+        const uint32_t ph = (uint32_t)((n / kPrStages) & 1);
+        if (!needs(i, seg, j)) {  // not this tile's: its arrivals, each in its phase
+          if (p_stage >= 0) finish();  // (the copies of later blocks wait for it)
+          mbar_wait_bounded(k_full + s, ph, dead, tries);
+          if (lane == 0) mbar_arrive(k_empty + s);
+          mbar_wait_bounded(v_full + s, ph, dead, tries);
+          if (lane == 0) mbar_arrive(v_empty + s);
+          __syncwarp();
+          continue;
+        }
+        mbar_wait_bounded(k_full + s, ph, dead, tries);
+        if (p_stage >= 0) finish();
+        else if (i == 1 && mine == 0 && n == 0 && needs(0, seg, j)) mbar_wait_bounded(po_ready + 0, 0, dead, tries);  // half a block behind the other tile
+        tc_fence_after();
+        const uint64_t k_desc = plain_desc(smem_u32(Ks + s * KB), 128, 8 * D);
+        if (tc_elect_one()) {
+#pragma unroll
+          for (int k = 0; k < D / 32; ++k) {
+            umma_f8(t_s, q_hi + (uint64_t)(k * 16), k_desc + (uint64_t)(k * 16), idesc_s, k > 0 ? 1u : 0u);
+            umma_f8(t_s, q_lo + (uint64_t)(k * 16), k_desc + (uint64_t)(k * 16), idesc_s | kRestA, 1u);
+          }
+          umma_commit(s_full + i);
+          umma_commit(k_empty + s);
+        }
+        __syncwarp();
+        ++mine;
+        mbar_wait_bounded(v_full + s, ph, dead, tries);
+        p_stage = s;
+      }
+    }
+    if (p_stage >= 0) finish();
+  } else if (warp >= kPrCorr) {
+    // =========================== rescaling of O, results ===========================
+    const int q4 = warp & 3, r = q4 * 32 + lane;
+    const uint32_t lane_base = tmem_base + ((uint32_t)(q4 * 32) << 16);
+    int mine[2] = {0, 0};
+    for (int seg = 0; seg < segs; ++seg) {
+      const int j1 = last_block(seg);
+      for (int j = j1 < 0 ? 0 : first_block(seg); j <= j1; ++j)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if (!needs(i, seg, j)) continue;
+          if (mine[i] > 0) {
+            mbar_wait_bounded(a_ready + i, (uint32_t)((mine[i] - 1) & 1), dead, tries);
+            const float alpha = alpha_s[i * kPrRows + r];
+            const bool need = !__all_sync(0xffffffffu, alpha == 1.0f);
+            mbar_wait_bounded(pv_done + i, (uint32_t)((mine[i] - 1) & 1), dead, tries);
+            tc_fence_after();
+            if (need) {
+              const uint32_t t_o = lane_base + (uint32_t)(2 * kPrKeys + i * 128);
+#pragma unroll
+              for (int c = 0; c < D; c += 32) {
+                uint32_t t[32];
+                tmem_ld32(t_o + c, t);
+#pragma unroll
+                for (int x = 0; x < 32; ++x) t[x] = __float_as_uint(__uint_as_float(t[x]) * alpha);
+                tmem_put32(t_o + c, t);
+              }
+              tmem_put_wait();
+            }
+            tc_fence_before();
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(po_ready + i);
+          ++mine[i];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      mbar_wait_bounded(d_ready + i, 0, dead, tries);
+      if (mine[i] > 0) mbar_wait_bounded(pv_done + i, (uint32_t)((mine[i] - 1) & 1), dead, tries);
+      tc_fence_after();
+      const int k = r / R, ti = i * per + k;
+      const bool on = k < per && ti < n_tok;
+      const float factor = end_s[i * kPrRows + r];
+      bf16* dst = out + (size_t)(t0 + (on ? ti : 0)) * a.out_ld + (g * R + (on ? r - k * R : 0)) * D;
+      const uint32_t t_o = lane_base + (uint32_t)(2 * kPrKeys + i * 128);
+#pragma unroll
+      for (int c = 0; c < D; c += 32) {
+        uint32_t t[32];
+        if (mine[i] > 0) {
+          tmem_ld32(t_o + c, t);
+        } else {
+#pragma unroll
+          for (int x = 0; x < 32; ++x) t[x] = 0u;
+        }
+        if (!on) continue;
+#pragma unroll
+        for (int x = 0; x < 32; ++x) t[x] = __float_as_uint(__uint_as_float(t[x]) * factor);
+        if (f.out_by8) {
+#pragma unroll
+          for (int x = 0; x < 32; x += 8)
+            *reinterpret_cast<uint4*>(dst + c + x) = make_uint4(pack_bf16(__uint_as_float(t[x]), __uint_as_float(t[x + 1])), pack_bf16(__uint_as_float(t[x + 2]), __uint_as_float(t[x + 3])),
+                                                                pack_bf16(__uint_as_float(t[x + 4]), __uint_as_float(t[x + 5])), pack_bf16(__uint_as_float(t[x + 6]), __uint_as_float(t[x + 7])));
+        } else {
+#pragma unroll
+          for (int x = 0; x < 32; ++x) dst[c + x] = f2bf(__uint_as_float(t[x]));
+        }
+      }
+    }
+  } else {
+    // =========================== softmax: a thread per row ===========================
+    const int i = warp >> 2, q4 = warp & 3, r = q4 * 32 + lane, k = r / R, ti = i * per + k;
+    const bool on = k < per && ti < n_tok;
+    const int h = g * R + (on ? r - k * R : 0);
+    const int p = on ? s_slot[ti] : -1, lo = on && a.window > 0 ? p - a.window + 1 : 0, my_seg = on ? s_seg[ti] : -1;
+    // q: scaled to the codes' upper end, split, into the operands
+    float row_c;
+    {
+      const bf16* src = q + ((size_t)(t0 + (on ? ti : 0)) * a.H + h) * D;
+      float amax = 0.f;
+      uint4 raw[D / 8];
+#pragma unroll
+      for (int c = 0; c < D / 8; ++c) {
+        raw[c] = make_uint4(0, 0, 0, 0);
+        if (on) {
+          if (f.q_by8) {
+            raw[c] = *reinterpret_cast<const uint4*>(src + c * 8);
+          } else {
+            uint32_t w[4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) w[x] = (uint32_t)__bfloat16_as_ushort(src[c * 8 + 2 * x]) | (uint32_t)__bfloat16_as_ushort(src[c * 8 + 2 * x + 1]) << 16;
+            raw[c] = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+        const uint32_t w[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
+#pragma unroll
+        for (int x = 0; x < 4; ++x) amax = fmaxf(amax, fmaxf(fabsf(bf16_lo(w[x])), fabsf(bf16_hi(w[x]))));
+      }
+      const int e = exponent_for(amax);
+      const float down = pow2(-e), qf = amax == INFINITY ? NAN : pow2(e);  // (an infinite entry: the row is NaN)
+      row_c = a.cap > 0.f ? qf : qf * a.scale * kLog2e;
+#pragma unroll
+      for (int c = 0; c < D / 16; ++c) {
+        uint32_t hi[4], rest[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const uint4 u = raw[2 * c + (x >> 1)];
+          const uint32_t w0 = x & 1 ? u.z : u.x, w1 = x & 1 ? u.w : u.y;
+          const float v0 = bf16_lo(w0) * down, v1 = bf16_hi(w0) * down, v2 = bf16_lo(w1) * down, v3 = bf16_hi(w1) * down;
+          hi[x] = codes4(v0, v1, v2, v3);
+          float y[4];
+          values4(hi[x], y);
+          rest[x] = rest4(v0 - y[0], v1 - y[1], v2 - y[2], v3 - y[3]);
+        }
+        uint8_t* dst = Qs + i * 2 * QB + (r >> 3) * (8 * D) + c * 128 + (r & 7) * 16;
+        *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        *reinterpret_cast<uint4*>(dst + QB) = make_uint4(rest[0], rest[1], rest[2], rest[3]);
+      }
+    }
+    fence_proxy_async_smem();
+    asm volatile("bar.sync 1, %0;" ::"n"(10 * 32) : "memory");
+
+    const uint32_t t_s = tmem_base + ((uint32_t)(q4 * 32) << 16) + (uint32_t)(i * kPrKeys);
+    const float cap2 = a.cap * kLog2e, cap_c = a.cap > 0.f ? 2.f * a.scale / a.cap * kLog2e : 0.f;
+    float m = -INFINITY, l = 0.f;
+    int E = kLowExp - 1, n = 0, mine = 0;
+    for (int seg = 0; seg < segs; ++seg) {
+      const int j1 = last_block(seg);
+      for (int j = j1 < 0 ? 0 : first_block(seg); j <= j1; ++j, ++n) {
+        if (!needs(i, seg, j)) continue;
+        const int s = n % kPrStages;
+        // S first: it says that the stage's phases before this block's are over (a tile that skipped blocks would take an older one for it)
+        mbar_wait_bounded(s_full + i, (uint32_t)(mine & 1), dead, tries);
+        mbar_wait_bounded(v_full + s, (uint32_t)((n / kPrStages) & 1), dead, tries);
+        tc_fence_after();
+        int ev[kPrRecords], e_new = E;
+        float fk[kPrRecords];
+#pragma unroll
+        for (int b = 0; b < kPrRecords; ++b) {
+          const uint32_t tail = *reinterpret_cast<const uint32_t*>(Ts + (s * kPrRecords + b) * 16);
+          ev[b] = tail_ev(tail);
+          const float x = pow2(tail_ek(tail)) * row_c;
+          fk[b] = x < 1e-37f ? 1e-37f : x;  // never zero: -inf times it stays -inf (and a NaN stays one)
+          e_new = max(e_new, ev[b]);
+        }
+        const int c0 = my_seg == seg ? max(lo - j * kPrKeys, 0) : kPrKeys, c1 = my_seg == seg ? min(p - j * kPrKeys, kPrKeys - 1) : -1;  // the columns that the row sees
+        const bool masked = !__all_sync(0xffffffffu, c0 <= 0 && c1 >= kPrKeys - 1);
+        // scores of 64 columns: what the row does not see becomes -inf, caps are applied (the columns' factors are one then)
+        auto shape = [&](uint32_t* v, int at) {
+          if (a.cap > 0.f) {
+#pragma unroll
+            for (int x = 0; x < 64; ++x)
+              v[x] = __float_as_uint(fmaf(-2.f * cap2, __fdividef(1.f, pr_ex2(fminf(__uint_as_float(v[x]) * fk[(at + x) / kBlock] * cap_c, 80.f)) + 1.f), cap2));
+          }
+          if (masked) {
+#pragma unroll
+            for (int x = 0; x < 64; ++x)
+              if (at + x < c0 || at + x > c1) v[x] = 0xff800000u;
+          }
+        };
+        auto factor = [&](int b) { return a.cap > 0.f ? 1.f : fk[b]; };
+        uint32_t v[64];
+        float mx = m;
+        auto largest = [&](int at) {
+#pragma unroll
+          for (int b = 0; b < 4; ++b) {
+            float y[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+            for (int x = 0; x < 16; x += 2) {
+              y[0] = fmaxf(y[0], __uint_as_float(v[b * 16 + x]));
+              y[1] = fmaxf(y[1], __uint_as_float(v[b * 16 + x + 1]));
+            }
+            mx = fmaxf(mx, fmaxf(y[0], y[1]) * factor(at / kBlock + b));
+          }
+        };
+        // row maximum: columns 64..127 first (read again later), then 0..63 (kept)
+        tmem_ld32_nowait(t_s + 64, v);
+        tmem_ld32_nowait(t_s + 96, v + 32);
+        tmem_ld_wait64(v);
+        shape(v, 64);
+        largest(64);
+        tmem_ld32_nowait(t_s, v);
+        tmem_ld32_nowait(t_s + 32, v + 32);
+        tmem_ld_wait64(v);
+        shape(v, 0);
+        largest(0);
+        const float ref = mx == -INFINITY ? 0.f : mx, fl = pr_ex2(m - ref);
+        if (mine > 0) {
+          alpha_s[i * kPrRows + r] = fl * pow2(max(E - e_new, -126));
+          __syncwarp();
+          if (lane == 0) mbar_arrive(a_ready + i);
+        }
+        m = mx;
+        E = e_new;
+        l *= fl;
+        // P of 16 columns -> four columns of each part
+        auto part = [&](const uint32_t* s16, int b, uint32_t* hi, uint32_t* lo4) {
+          const int shift = max(ev[b] - E, -60) + kPrTop;
+          const float fb = factor(b), add = (float)shift - ref;
+          float d0 = 0.f, d1 = 0.f;
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            uint32_t h2[2], l2[2];
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              float s0 = __uint_as_float(s16[4 * x + 2 * y]), s1 = __uint_as_float(s16[4 * x + 2 * y + 1]);
+              pr_fma2(s0, s1, fb, add);
+              s0 = pr_ex2(s0);
+              s1 = pr_ex2(s1);
+              d0 += s0;
+              d1 += s1;
+              split2(s0, s1, h2[y], l2[y]);
+            }
+            hi[x] = h2[0] | h2[1] << 16;
+            lo4[x] = l2[0] | l2[1] << 16;
+          }
+          l = fmaf(d0 + d1, pow2(-shift), l);
+        };
+        uint32_t hi[16], rest[16];
+#pragma unroll
+        for (int b = 0; b < 4; ++b) part(v + b * 16, b, hi + b * 4, rest + b * 4);
+        tmem_ld32_nowait(t_s + 64, v);
+        tmem_ld32_nowait(t_s + 96, v + 32);
+        tmem_ld_wait64(v);  // (ahead of the stores: the columns from 64 on are S's alone)
+        tmem_put16(t_s, hi);
+        tmem_put16(t_s + 32, rest);
+        shape(v, 64);
+#pragma unroll
+        for (int b = 0; b < 2; ++b) part(v + b * 16, 4 + b, hi + b * 4, rest + b * 4);
+        pr_put8(t_s + 16, hi);
+        pr_put8(t_s + 48, rest);
+        tmem_put_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(po_ready + i);
+#pragma unroll
+        for (int b = 2; b < 4; ++b) part(v + b * 16, 4 + b, hi + (b - 2) * 4, rest + (b - 2) * 4);
+        pr_put8(t_s + 24, hi);
+        pr_put8(t_s + 56, rest);
+        tmem_put_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_rest + i);
+        ++mine;
+      }
+    }
+    const float top = l != l ? INFINITY : m;  // a NaN among the scores
+    const RowEnd end = row_end(top, l, sink ? bf2f(sink[h]) : 0.f, sink != nullptr);
+    end_s[i * kPrRows + r] = l != l ? NAN : end.factor * pow2(max(E, kLowExp) - kPrTop);
+    if (on && a.lse) a.lse[(size_t)(t0 + ti) * a.H + h] = end.lse;
+    __syncwarp();
+    if (lane == 0) mbar_arrive(d_ready + i);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (*dead) {  // (for all alike, behind the barrier)
+    __syncwarp();
+    if (warp == kPrMma || warp == kPrMma + 1) {
+      if (tc_elect_one()) umma_commit(done);
+      mbar_drain(done, 0);
+    }
+    __syncthreads();
+  }
+  if (warp == kPrMma) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, 512);
+  }
+  if (tid == 0) count_run_out(dead, f.err);
+}
+
+template <int D>
+static int launch_prompt(const bf16* q, const bf16* sink, bf16* out, const PromptArgs& f, cudaStream_t st) {
+  constexpr size_t smem = 128 + (size_t)4 * kPrRows * D + (size_t)2 * kPrStages * kPrKeys * D + kPrStages * kPrRecords * 16 + 4 * kPrRows * sizeof(float) + 32 * 8;
+  static std::atomic<uint64_t> set{0};
+  if (const cudaError_t e = allow_smem(set, (const void*)kv8_prompt_kernel<D>, smem); e != cudaSuccess) return (int)e;
+  return (int)launch(kv8_prompt_kernel<D>, dim3(f.a.pool.G, (f.a.T + 2 * f.per - 1) / (2 * f.per)), dim3(kPrThreads), smem, st, true, q, sink, out, f);
+}
+
+bool prompt_takes(int T, int H, int G, int dim, int vdim) {
+  const int R = H / G, tokens = R <= kPrRows ? 2 * (kPrRows / R) : 0;  // of a CTA
+  return dim == vdim && (dim == 64 || dim == 96 || dim == 128) && tokens > 0 && (T + tokens - 1) / tokens <= 65535;
+}
+int prompt_attention(const bf16* q, const bf16* sink, bf16* out, const AttnArgs& a, cudaStream_t st) {
+  PromptArgs f{};
+  f.a = a;
+  f.per = kPrRows / (a.H / a.pool.G);
+  f.q_by8 = (reinterpret_cast<uintptr_t>(q) & 15) == 0;
+  f.out_by8 = (reinterpret_cast<uintptr_t>(out) & 15) == 0 && a.out_ld % 8 == 0;
+  f.err = wait_err_word();
+  return a.pool.dim == 64 ? launch_prompt<64>(q, sink, out, f, st) : a.pool.dim == 96 ? launch_prompt<96>(q, sink, out, f, st) : launch_prompt<128>(q, sink, out, f, st);
+}
+
+}  // namespace kv8
+}  // namespace pk
