@@ -289,7 +289,8 @@ extern "C" int pk_kv8_attention(const void* q, const void* cache, const void* si
   if (p.few) return kv8::few_attention((const bf16*)q, (const bf16*)sink, (bf16*)out, a, options->max_q_len, p.need, ws, st);
   if (p.prompt) {
     const int rc = kv8::prompt_attention((const bf16*)q, (const bf16*)sink, (bf16*)out, a, st);
-    return rc != 0 || !a.mass ? rc : kv8::mass_rows((const bf16*)q, a, st);
+    if (rc != 0 || !a.mass) return rc;
+    return kv8::mass_takes((const bf16*)q, dim, vdim) ? kv8::mass_rows_mma((const bf16*)q, a, options->max_q_len, st) : kv8::mass_rows((const bf16*)q, a, st);
   }
   a.part_o = reinterpret_cast<float*>(ws);
   a.part_ml = reinterpret_cast<float2*>(ws + p.o_bytes);

@@ -63,6 +63,9 @@ int few_attention(const bf16* q, const bf16* sink, bf16* out, const AttnArgs& a,
 // kv8_prompt.cu: whether it takes a call, and the call (no workspace)
 bool prompt_takes(int T, int H, int G, int dim, int vdim);
 int prompt_attention(const bf16* q, const bf16* sink, bf16* out, const AttnArgs& a, cudaStream_t st);
+// kv8_mass.cu: the weights' sums of such a call
+bool mass_takes(const bf16* q, int dim, int vdim);
+int mass_rows_mma(const bf16* q, const AttnArgs& a, int max_q_len, cudaStream_t st);
 
 }  // namespace kv8
 }  // namespace pk

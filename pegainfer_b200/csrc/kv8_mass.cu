@@ -1,0 +1,190 @@
+// Weights of a prompt's keys, added up over its queries (kv8_attention.cuh), on the tensor cores: mass[j] += sum over the run's rows of 2^(s_j - lse).
+//
+// The scores are computed again from q and the finished lse: the products q K^T are half of the attention's work, and every key has one owner, who adds its weights in
+// the rows' order.  A warp keeps 32 keys (16 from 192 entries on) as bf16 operands in registers, where e4m3 codes are exact; the run's rows pass by in tiles of 64
+// through shared memory, as they are (mma.sync m16n8k16 in bf16, S^T = K q^T, fp32 sums).  A thread has the scores of two rows of four keys: the exponential and the sum
+// over rows need no exchange.  The grid's z axis takes the runs by turns.
+#include <algorithm>
+
+#include "kv8_attention.cuh"
+#include "mma.cuh"
+
+namespace pk {
+namespace kv8 {
+
+constexpr int kMassWarps = 4, kMassRows = 64;
+constexpr int mass_records(int D) { return D <= 128 ? 2 : 1; }  // of a warp
+
+__device__ __forceinline__ float ms_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// two codes -> two bf16
+__device__ __forceinline__ uint32_t bf16_of(uint32_t two) {
+  const float2 v = values2(two);
+  return pack_bf16(v.x, v.y);
+}
+
+template <int D>
+__global__ void __launch_bounds__(kMassWarps * 32) kv8_mass_kernel(const bf16* __restrict__ q, AttnArgs a) {
+  constexpr int RECS = mass_records(D), LD = D + 8, REC = kBlock * 2 * D + 16;
+  extern __shared__ __align__(16) bf16 ms_q[];  // [2][rows][LD]
+  __shared__ float s_lse[2][kMassRows];         // log2; +inf: no such row
+  __shared__ int s_p[2][kMassRows];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gq = lane >> 2, tq = lane & 3, g = blockIdx.y, R = a.H / a.pool.G, V = a.pool.vdim;
+  const int b0 = (blockIdx.x * kMassWarps + warp) * RECS;  // the warp's first record
+  const int key0 = blockIdx.x * kMassWarps * RECS * kBlock, key1 = key0 + kMassWarps * RECS * kBlock - 1;
+  const float c = a.scale * kLog2e, cap2 = a.cap * kLog2e, cap_c = a.cap > 0.f ? 2.f * a.scale / a.cap * kLog2e : 0.f;
+  pdl_wait();
+  pdl_launch_dependents();
+  int nth = 0;
+  for (int t0 = 0, t1 = 0; t0 < a.T; t0 = t1, ++nth) {
+    // the run's end, its largest and smallest slot
+    const int req = a.req[t0];
+    int last = -1, lowest = INT_MAX;
+    t1 = t0;
+    for (bool more = true; more;) {
+      const bool in = t1 + lane < a.T && a.req[min(t1 + lane, a.T - 1)] == req;
+      const uint32_t same = __ballot_sync(0xffffffffu, in);
+      const int n = same == 0xffffffffu ? 32 : __ffs(~same) - 1, slot = lane < n ? a.slots[t1 + lane] : -1;
+      last = max(last, __reduce_max_sync(0xffffffffu, slot));
+      lowest = min(lowest, __reduce_min_sync(0xffffffffu, slot < 0 ? INT_MAX : slot));
+      t1 += n;
+      more = n == 32;
+    }
+    if (nth % (int)gridDim.z != (int)blockIdx.z || key0 > last || (a.window > 0 && key1 <= lowest - a.window)) continue;  // (for all threads alike)
+
+    // the warp's keys: a product's 16 tokens are a record's, its inner index the entries in order
+    uint32_t ka[RECS][D / 16][4];
+    float fk[RECS];
+#pragma unroll
+    for (int r = 0; r < RECS; ++r) {
+      fk[r] = 0.f;
+      const bool there = (b0 + r) * kBlock <= last;
+      const uint8_t* rec = there ? a.pool.record(req, (b0 + r) * kBlock, g) : nullptr;
+      if (there) fk[r] = pow2(tail_ek(*reinterpret_cast<const uint32_t*>(rec + kBlock * (D + V)))) * (a.cap > 0.f ? 1.f : c);
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+        for (int x = 0; x < 4; ++x)  // tokens gq (+ 8), entries 2 tq (+ 8)
+          ka[r][k][x] = there ? bf16_of(*reinterpret_cast<const uint16_t*>(rec + (x & 1) * (8 * D) + k * 128 + gq * 16 + 2 * tq + (x >> 1) * 8)) : 0u;
+    }
+    float sum[RECS][2];
+#pragma unroll
+    for (int r = 0; r < RECS; ++r) sum[r][0] = sum[r][1] = 0.f;
+
+    const int rows = (t1 - t0) * R, tiles = (rows + kMassRows - 1) / kMassRows;
+    auto load = [&](int tile, int s) {
+      bf16* dst = ms_q + (size_t)s * kMassRows * LD;
+      for (int i = threadIdx.x; i < kMassRows * (D / 8); i += kMassWarps * 32) {
+        const int row = i / (D / 8), piece = i % (D / 8), at = min(tile * kMassRows + row, rows - 1), t = t0 + at / R;
+        cp_async16(dst + row * LD + piece * 8, q + ((size_t)t * a.H + g * R + at % R) * D + piece * 8);
+      }
+      if (threadIdx.x < kMassRows) {
+        const int at = tile * kMassRows + threadIdx.x, t = t0 + min(at, rows - 1) / R, p = at < rows ? a.slots[t] : -1;
+        s_p[s][threadIdx.x] = p;
+        s_lse[s][threadIdx.x] = p >= 0 ? a.lse[(size_t)t * a.H + g * R + at % R] * kLog2e : INFINITY;
+      }
+      cp_async_commit();
+    };
+    // tiles whose rows see none of the CTA's keys pass (every thread looks at the same slots)
+    auto seen = [&](int tile) {
+      const int ta = t0 + tile * kMassRows / R, tb = t0 + min((tile + 1) * kMassRows, rows) / R - ((min((tile + 1) * kMassRows, rows) % R) == 0 ? 1 : 0);
+      int top = -1, low = INT_MAX;
+      for (int t = ta + lane; t <= tb; t += 32) {
+        const int p = a.slots[t];
+        top = max(top, p);
+        if (p >= 0) low = min(low, p);
+      }
+      top = __reduce_max_sync(0xffffffffu, top);
+      low = __reduce_min_sync(0xffffffffu, low);
+      return top >= key0 && (a.window <= 0 || low - a.window < key1);
+    };
+    auto next = [&](int tile) {
+      while (tile < tiles && !seen(tile)) ++tile;
+      return tile;
+    };
+    int tile = next(0), s = 0;
+    if (tile < tiles) load(tile, 0);
+    while (tile < tiles) {
+      const int after = next(tile + 1);
+      if (after < tiles) load(after, s ^ 1);
+      else cp_async_commit();
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
+      __syncthreads();
+      const bf16* qt = ms_q + (size_t)s * kMassRows * LD;
+#pragma unroll 1
+      for (int n = 0; n < kMassRows / 8; ++n) {
+        float acc[RECS][4] = {};
+#pragma unroll
+        for (int k = 0; k < D / 32; ++k) {
+          uint32_t b[4];
+          ldsm_x4(b, qt + (n * 8 + (lane & 7)) * LD + k * 32 + (lane >> 3) * 8);
+#pragma unroll
+          for (int r = 0; r < RECS; ++r) {
+            mma_bf16_16816(acc[r], ka[r][2 * k], b[0], b[1]);
+            mma_bf16_16816(acc[r], ka[r][2 * k + 1], b[2], b[3]);
+          }
+        }
+        const int row = n * 8 + 2 * tq;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float lse = s_lse[s][row + e];
+          const int p = s_p[s][row + e], lo = a.window > 0 ? p - a.window + 1 : 0;
+#pragma unroll
+          for (int r = 0; r < RECS; ++r)
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              float v = acc[r][2 * y + e] * fk[r];
+              if (a.cap > 0.f) v = fmaf(-2.f * cap2, __fdividef(1.f, ms_ex2(fminf(v * cap_c, 80.f)) + 1.f), cap2);
+              const int j = (b0 + r) * kBlock + 8 * y + gq;
+              const float w = ms_ex2(v - lse);
+              sum[r][y] += j <= p && j >= lo ? w : 0.f;
+            }
+        }
+      }
+      __syncthreads();
+      tile = after;
+      s ^= 1;
+    }
+#pragma unroll
+    for (int r = 0; r < RECS; ++r)
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        float v = sum[r][y];
+        v += __shfl_xor_sync(0xffffffffu, v, 1);
+        v += __shfl_xor_sync(0xffffffffu, v, 2);
+        const int j = (b0 + r) * kBlock + 8 * y + gq;
+        if (tq == 0 && j <= last && j < a.mass_ld) a.mass[((size_t)req * a.pool.G + g) * a.mass_ld + j] += v;
+      }
+    __syncthreads();  // the next run's rows may come
+  }
+}
+
+template <int D>
+static int launch_mass(const bf16* q, const AttnArgs& a, int runs, cudaStream_t st) {
+  constexpr size_t smem = (size_t)2 * kMassRows * (D + 8) * sizeof(bf16);
+  static std::atomic<uint64_t> set{0};
+  if (const cudaError_t e = allow_smem(set, (const void*)kv8_mass_kernel<D>, smem); e != cudaSuccess) return (int)e;
+  const int keys = kMassWarps * mass_records(D) * kBlock;
+  const long span = std::min((long)a.max_kv_len, a.mass_ld);
+  return (int)launch(kv8_mass_kernel<D>, dim3((unsigned)((span + keys - 1) / keys), a.pool.G, std::max(1, std::min(runs, 16))), dim3(kMassWarps * 32), smem, st, true, q, a);
+}
+bool mass_takes(const bf16* q, int dim, int vdim) {
+  return dim == vdim && (dim == 32 || dim == 64 || dim == 96 || dim == 128 || dim == 192 || dim == 256) && (reinterpret_cast<uintptr_t>(q) & 15) == 0;
+}
+int mass_rows_mma(const bf16* q, const AttnArgs& a, int max_q_len, cudaStream_t st) {
+  const int runs = max_q_len > 0 ? (a.T + max_q_len - 1) / max_q_len : 4;  // at least; unknown: some
+  switch (a.pool.dim) {
+    case 32: return launch_mass<32>(q, a, runs, st);
+    case 64: return launch_mass<64>(q, a, runs, st);
+    case 96: return launch_mass<96>(q, a, runs, st);
+    case 128: return launch_mass<128>(q, a, runs, st);
+    case 192: return launch_mass<192>(q, a, runs, st);
+    default: return launch_mass<256>(q, a, runs, st);
+  }
+}
+
+}  // namespace kv8
+}  // namespace pk
