@@ -2,17 +2,17 @@
 //
 // A CTA has two tiles of 128 rows of one kv head: the group's R query heads of 128 / R consecutive tokens each, so that a key is fetched once for the whole group and
 // few scores lie behind the diagonal.  It goes through the keys in blocks of 128, run by run where its tokens belong to several requests (the other rows are masked).
-//   * K's and V's codes are operands as they lie in the cache: a record's K is two groups of 8 tokens and its V one column of 16 tokens of the canonical layout without
-//     swizzle (8 x 16-byte matrices), so plain bulk copies fill the operands and nothing is converted.
-//   * kind::f8f6f4 wants both operands in 8 bits at most.  q and P have more, so each goes in as two numbers, the nearest e4m3 and the rest as e5m2, whose exponents
-//     reach 2^10 further down (4 + 1 + 3 significant bits; bf16 has 8): S = q_hi K^T + q_lo K^T and O += P_hi V + P_lo V, as many cycles as one product in
-//     16 bits.  A row of q is scaled by a power of two to the upper end of the codes' range: a bf16 entry is exact down to 2^-17 of the row's largest.  P is held 2^8
-//     times too large: a weight is off by at most 2^-8 of it down to 2^-14 of the largest, and by 2^-25 of the largest below 2^-22.  (With the rest in e4m3 too, scores of
-//     a peaked row were off by 1.4e-4 and weights by 2^-18 of the largest.)
-//   * K's exponents multiply the scores 16 columns at a time, V's go into P's exponent: 2^(s - m + e - E + 8), E the largest so far; the denominator takes them out.
+//   * S = q K^T: K's codes are an operand as they lie in the cache (a record's K is two groups of 8 tokens of the canonical layout without swizzle, 8 x 16-byte matrices),
+//     so plain bulk copies fill it.  kind::f8f6f4 wants 8 bits of q too, which has more: it goes in as two numbers, the nearest e4m3 and the rest as e5m2, whose exponents
+//     reach 2^10 further down (4 + 1 + 3 significant bits; bf16 has 8), as many cycles as one product in 16 bits.  A row of q is scaled by a power of two to the upper
+//     end of the codes' range: a bf16 entry is exact down to 2^-17 of the row's largest.
+//   * O += P V in f16: the warps that rescale O turn a block's V into f16 (exactly) before, once for both tiles' 256 rows, which is an eighth of the instructions that
+//     P in two 8-bit parts takes (B200, prompt of 4096, 32 heads in 8 groups: 240 us so).  P is held 2^15 times too large: 11 bits down to 2^-29 of the largest weight.
+//   * K's exponents multiply the scores 16 columns at a time, V's go into P's exponent: 2^(s - m + e - E + 15), E the largest so far; the denominator takes them out.
 //   * The softmax is a thread per row, 128 a tile, with the tiles in turn; O stays in tensor memory and is rescaled by a third group of warps where a maximum moved.
-// Warps: 0-3 softmax tile 0 | 4-7 softmax tile 1 | 8-11 rescaling, results | 12, 13 MMA issuers | 14 copies.
-// Tensor memory: S0 | S1 (128 columns each, P over the first 64: 32 of hi, 32 of lo) | O0 | O1.
+// Warps: 0-3 softmax tile 0 | 4-7 softmax tile 1 | 8-11 V, rescaling, results | 12, 13 MMA issuers | 14 copies | 15 nothing.  Of the block's registers a softmax thread
+// has 192 (a row's 128 scores stay in them), the others 80 and 48.
+// Tensor memory: S0 | S1 (128 columns each, P over the first 64) | O0 | O1.
 #include <algorithm>
 
 #include "kv8_attention.cuh"
@@ -22,10 +22,12 @@ namespace pk {
 namespace kv8 {
 
 constexpr int kPrRows = 128, kPrKeys = 128, kPrRecords = kPrKeys / kBlock;
-constexpr int kPrStages = 3;
-constexpr int kPrCorr = 8, kPrMma = 12, kPrLoad = 14, kPrThreads = 15 * 32;
-constexpr int kPrEarly = 3;        // k-steps of 32 keys of P V that begin before the last one's P is there
-constexpr int kPrTop = 8;          // exponent of P = 1
+constexpr int kPrStages = 3, kPrStagesV = 2;  // of K; of V as it comes and as f16
+constexpr int kPrCorr = 8, kPrMma = 12, kPrLoad = 14, kPrThreads = 16 * 32;
+constexpr int kPrRegsSoft = 192, kPrRegsCorr = 80, kPrRegsMma = 48;
+static_assert(256 * kPrRegsSoft + 128 * kPrRegsCorr + 128 * kPrRegsMma <= kPrThreads * (65536 / kPrThreads), "more registers than the block was launched with");
+constexpr int kPrEarly = 6;        // k-steps of 16 keys of P V (of eight) that begin before the rest of P is there
+constexpr int kPrTop = 15;         // exponent of P = 1
 constexpr uint32_t kRestA = 1u << 7;  // instruction descriptor: A is e5m2
 constexpr int kPrMaxSeg = 256;     // runs that a CTA's tokens can belong to
 
@@ -62,36 +64,35 @@ __device__ __forceinline__ void umma_f8(uint32_t d_tmem, uint64_t adesc, uint64_
       "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-// A from tensor memory: lane = row, four consecutive inner elements a column
-__device__ __forceinline__ void umma_f8_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+// f16, A from tensor memory: lane = row, two consecutive inner elements a column
+__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
       "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
       : "memory");
-}
-__device__ __forceinline__ void pr_put8(uint32_t taddr, const uint32_t* v) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]),
-               "r"(v[6]), "r"(v[7])
-               : "memory");
 }
 __device__ __forceinline__ void pr_copy(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
 }
-// two values of P -> two e4m3 codes and two e5m2 codes of the rest
-__device__ __forceinline__ void split2(float p0, float p1, uint32_t& hi, uint32_t& lo) {
-  asm("{\n\t.reg .b32 h, b, r;\n\t.reg .b16 c, d;\n\t"
-      "cvt.rn.f16x2.f32 h, %3, %2;\n\t"
-      "cvt.rn.satfinite.e4m3x2.f16x2 c, h;\n\t"
-      "cvt.rn.f16x2.e4m3x2 b, c;\n\t"
-      "sub.rn.f16x2 r, h, b;\n\t"
-      "cvt.rn.satfinite.e5m2x2.f16x2 d, r;\n\t"
-      "cvt.u32.u16 %0, c;\n\tcvt.u32.u16 %1, d;\n\t}"
-      : "=r"(hi), "=r"(lo)
-      : "f"(p0), "f"(p1));
+__device__ __forceinline__ uint32_t pr_pack(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
 }
-
+// four codes -> two pairs of f16
+__device__ __forceinline__ void pr_widen(uint32_t four, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=&r"(lo), "=&r"(hi) : "r"(four));
+}
+// {a0, a1} += {x0, x1}
+__device__ __forceinline__ void pr_add2(float& a0, float& a1, float x0, float x1) {
+  unsigned long long v, w;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a0), "f"(a1));
+  asm("mov.b64 %0, {%1, %2};" : "=l"(w) : "f"(x0), "f"(x1));
+  asm("add.rn.f32x2 %0, %0, %1;" : "+l"(v) : "l"(w));
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a0), "=f"(a1) : "l"(v));
+}
 __device__ __forceinline__ uint32_t rest4(float a, float b, float c, float d) {
   uint16_t x, y;
   asm("cvt.rn.satfinite.e5m2x2.f32 %0, %1, %2;" : "=h"(x) : "f"(b), "f"(a));
@@ -106,12 +107,14 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* _
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pr_raw) + 127) & ~(uintptr_t)127);
   uint8_t* Qs = smem;                                    // [tile][hi, lo]
   uint8_t* Ks = Qs + 4 * QB;                             // [stage]
-  uint8_t* Vs = Ks + kPrStages * KB;                     // [stage]
-  uint8_t* Ts = Vs + kPrStages * KB;                     // [stage][record] tails
-  float* alpha_s = reinterpret_cast<float*>(Ts + kPrStages * kPrRecords * 16);  // [tile][row]
+  uint8_t* Vs = Ks + kPrStages * KB;                     // [stage] V as it comes
+  uint8_t* Hs = Vs + kPrStagesV * KB;                    // [stage] V as f16: [8 keys][entry][8 keys' f16]
+  uint8_t* Ts = Hs + kPrStagesV * 2 * KB;                // [stage][record] tails as they come
+  uint32_t* Es = reinterpret_cast<uint32_t*>(Ts + kPrStagesV * kPrRecords * 16);  // [stage][record] tails of the f16's
+  float* alpha_s = reinterpret_cast<float*>(Es + kPrStagesV * kPrRecords);  // [tile][row]
   float* end_s = alpha_s + 2 * kPrRows;                  // [tile][row]
   uint64_t* bars = reinterpret_cast<uint64_t*>(end_s + 2 * kPrRows);
-  uint64_t *k_full = bars, *k_empty = bars + 4, *v_full = bars + 8, *v_empty = bars + 12;  // [stage]
+  uint64_t *k_full = bars, *k_empty = bars + 4, *v_full = bars + 8, *v_empty = bars + 10, *h_full = bars + 12, *h_empty = bars + 14;  // [stage]
   uint64_t* s_full = bars + 16;    // [tile] S complete                                      MMA -> softmax
   uint64_t* po_ready = bars + 18;  // [tile] P up to kPrEarly stored, O rescaled (4 + 4 warps)  softmax, rescaling -> MMA
   uint64_t* p_rest = bars + 20;    // [tile] the rest of P stored (4 warps)                    softmax -> MMA
@@ -133,9 +136,13 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* _
   if (tid == 0) {
     for (int s = 0; s < kPrStages; ++s) {
       mbar_init(k_full + s, 1);
-      mbar_init(k_empty + s, 2);
+      mbar_init(k_empty + s, 2);  // both tiles
+    }
+    for (int s = 0; s < kPrStagesV; ++s) {
       mbar_init(v_full + s, 1);
-      mbar_init(v_empty + s, 2);
+      mbar_init(v_empty + s, 4);  // the warps that turn it into f16
+      mbar_init(h_full + s, 4);
+      mbar_init(h_empty + s, 2);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(s_full + i, 1);
@@ -200,6 +207,8 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* _
   auto last_block = [&](int seg) { return max(seg_hi[0][seg], seg_hi[1][seg]); };
   auto needs = [&](int tile, int seg, int j) { return j >= seg_lo[tile][seg] && j <= seg_hi[tile][seg]; };
 
+  if (warp >= kPrMma) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPrRegsMma));
   if (warp == kPrLoad) {
     // =========================== copies ===========================
     int n = 0;
@@ -228,18 +237,19 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* _
         if (lane == 0) mbar_expect_tx(k_full + s, KB);
         __syncwarp();
         if (lane < kPrRecords) pr_copy(smem_u32(Ks + s * KB) + lane * REC_K, now, REC_K, k_full + s);
-        go = mbar_wait_bounded(v_empty + s, ph, dead, tries);
+        const int sv = n % kPrStagesV;
+        go = mbar_wait_bounded(v_empty + sv, (uint32_t)((n / kPrStagesV) & 1) ^ 1u, dead, tries);
         if (!go) break;
-        if (lane == 0) mbar_expect_tx(v_full + s, KB + kPrRecords * 16);
+        if (lane == 0) mbar_expect_tx(v_full + sv, KB + kPrRecords * 16);
         __syncwarp();
         if (lane < kPrRecords) {
-          pr_copy(smem_u32(Vs + s * KB) + lane * REC_K, now + REC_K, REC_K, v_full + s);
-          pr_copy(smem_u32(Ts + (s * kPrRecords + lane) * 16), now + 2 * REC_K, 16, v_full + s);
+          pr_copy(smem_u32(Vs + sv * KB) + lane * REC_K, now + REC_K, REC_K, v_full + sv);
+          pr_copy(smem_u32(Ts + (sv * kPrRecords + lane) * 16), now + 2 * REC_K, 16, v_full + sv);
         }
       }
     }
     if (!go) wait_for_copies();
-  } else if (warp >= kPrMma) {
+  } else if (warp < kPrLoad) {
     // =========================== MMA issuers, one per tile ===========================
     const int i = warp - kPrMma;
     asm volatile("bar.sync 1, %0;" ::"n"(10 * 32) : "memory");  // q is there
@@ -254,25 +264,20 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* _
       const int s = p_stage;
       mbar_wait_bounded(po_ready + i, (uint32_t)((mine - 1) & 1), dead, tries);
       tc_fence_after();
-      const uint64_t v_desc = plain_desc(smem_u32(Vs + s * KB), REC_K, 128);
+      const uint64_t v_desc = plain_desc(smem_u32(Hs + s * 2 * KB), REC_K, 128);  // 8 keys x 8 entries
       if (tc_elect_one()) {
 #pragma unroll
-        for (int k = 0; k < kPrEarly; ++k) {
-          umma_f8_ts(t_o, t_s + (uint32_t)(k * 8), v_desc + (uint64_t)(k * (2 * REC_K >> 4)), idesc_pv, (mine > 1 || k > 0) ? 1u : 0u);
-          umma_f8_ts(t_o, t_s + (uint32_t)(32 + k * 8), v_desc + (uint64_t)(k * (2 * REC_K >> 4)), idesc_pv | kRestA, 1u);
-        }
+        for (int k = 0; k < kPrEarly; ++k)
+          umma_f16_ts(t_o, t_s + (uint32_t)(k * 8), v_desc + (uint64_t)(k * (2 * REC_K >> 4)), idesc_pv, (mine > 1 || k > 0) ? 1u : 0u);
       }
       __syncwarp();
       mbar_wait_bounded(p_rest + i, (uint32_t)((mine - 1) & 1), dead, tries);
       tc_fence_after();
       if (tc_elect_one()) {
 #pragma unroll
-        for (int k = kPrEarly; k < kPrKeys / 32; ++k) {
-          umma_f8_ts(t_o, t_s + (uint32_t)(k * 8), v_desc + (uint64_t)(k * (2 * REC_K >> 4)), idesc_pv, 1u);
-          umma_f8_ts(t_o, t_s + (uint32_t)(32 + k * 8), v_desc + (uint64_t)(k * (2 * REC_K >> 4)), idesc_pv | kRestA, 1u);
-        }
+        for (int k = kPrEarly; k < kPrKeys / 16; ++k) umma_f16_ts(t_o, t_s + (uint32_t)(k * 8), v_desc + (uint64_t)(k * (2 * REC_K >> 4)), idesc_pv, 1u);
         umma_commit(pv_done + i);
-        umma_commit(v_empty + s);
+        umma_commit(h_empty + s);
       }
       __syncwarp();
       p_stage = -1;
@@ -280,14 +285,14 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* _
     for (int seg = 0; seg < segs; ++seg) {
       const int j1 = last_block(seg);
       for (int j = j1 < 0 ? 0 : first_block(seg); j <= j1; ++j, ++n) {
-        const int s = n % kPrStages;
-        const uint32_t ph = (uint32_t)((n / kPrStages) & 1);
+        const int s = n % kPrStages, sv = n % kPrStagesV;
+        const uint32_t ph = (uint32_t)((n / kPrStages) & 1), phv = (uint32_t)((n / kPrStagesV) & 1);
         if (!needs(i, seg, j)) {  // not this tile's: its arrivals, each in its phase
           if (p_stage >= 0) finish();  // (the copies of later blocks wait for it)
           mbar_wait_bounded(k_full + s, ph, dead, tries);
           if (lane == 0) mbar_arrive(k_empty + s);
-          mbar_wait_bounded(v_full + s, ph, dead, tries);
-          if (lane == 0) mbar_arrive(v_empty + s);
+          mbar_wait_bounded(h_full + sv, phv, dead, tries);
+          if (lane == 0) mbar_arrive(h_empty + sv);
           __syncwarp();
           continue;
         }
@@ -307,19 +312,48 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* _
         }
         __syncwarp();
         ++mine;
-        mbar_wait_bounded(v_full + s, ph, dead, tries);
-        p_stage = s;
+        mbar_wait_bounded(h_full + sv, phv, dead, tries);
+        p_stage = sv;
       }
     }
     if (p_stage >= 0) finish();
+  }
   } else if (warp >= kPrCorr) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPrRegsCorr));
     // =========================== rescaling of O, results ===========================
     const int q4 = warp & 3, r = q4 * 32 + lane;
     const uint32_t lane_base = tmem_base + ((uint32_t)(q4 * 32) << 16);
-    int mine[2] = {0, 0};
+    int mine[2] = {0, 0}, n = 0;
     for (int seg = 0; seg < segs; ++seg) {
       const int j1 = last_block(seg);
-      for (int j = j1 < 0 ? 0 : first_block(seg); j <= j1; ++j)
+      for (int j = j1 < 0 ? 0 : first_block(seg); j <= j1; ++j, ++n) {
+        {  // the block's V: a thread takes an entry's 16 keys of a record at a time
+          const int sv = n % kPrStagesV;
+          const uint32_t phv = (uint32_t)((n / kPrStagesV) & 1);
+          mbar_wait_bounded(v_full + sv, phv, dead, tries);
+          mbar_wait_bounded(h_empty + sv, phv ^ 1u, dead, tries);
+          const uint8_t* from = Vs + sv * KB;
+          uint8_t* to = Hs + sv * 2 * KB;
+#pragma unroll 4
+          for (int u = r; u < kPrRecords * D; u += 128) {
+            const int b = u / D, d = u - b * D;
+            const uint4 x = *reinterpret_cast<const uint4*>(from + u * 16);
+            uint32_t h[8];
+            pr_widen(x.x, h[0], h[1]);
+            pr_widen(x.y, h[2], h[3]);
+            pr_widen(x.z, h[4], h[5]);
+            pr_widen(x.w, h[6], h[7]);
+            *reinterpret_cast<uint4*>(to + (2 * b) * REC_K + d * 16) = make_uint4(h[0], h[1], h[2], h[3]);
+            *reinterpret_cast<uint4*>(to + (2 * b + 1) * REC_K + d * 16) = make_uint4(h[4], h[5], h[6], h[7]);
+          }
+          if (r < kPrRecords) Es[sv * kPrRecords + r] = *reinterpret_cast<const uint32_t*>(Ts + (sv * kPrRecords + r) * 16);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(h_full + sv);
+            mbar_arrive(v_empty + sv);
+          }
+        }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           if (!needs(i, seg, j)) continue;
@@ -347,6 +381,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* _
           if (lane == 0) mbar_arrive(po_ready + i);
           ++mine[i];
         }
+      }
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -382,6 +417,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* _
       }
     }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPrRegsSoft));
     // =========================== softmax: a thread per row ===========================
     const int i = warp >> 2, q4 = warp & 3, r = q4 * 32 + lane, k = r / R, ti = i * per + k;
     const bool on = k < per && ti < n_tok;
@@ -442,16 +478,16 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* _
       const int j1 = last_block(seg);
       for (int j = j1 < 0 ? 0 : first_block(seg); j <= j1; ++j, ++n) {
         if (!needs(i, seg, j)) continue;
-        const int s = n % kPrStages;
+        const int s = n % kPrStagesV;
         // S first: it says that the stage's phases before this block's are over (a tile that skipped blocks would take an older one for it)
         mbar_wait_bounded(s_full + i, (uint32_t)(mine & 1), dead, tries);
-        mbar_wait_bounded(v_full + s, (uint32_t)((n / kPrStages) & 1), dead, tries);
+        mbar_wait_bounded(h_full + s, (uint32_t)((n / kPrStagesV) & 1), dead, tries);
         tc_fence_after();
         int ev[kPrRecords], e_new = E;
         float fk[kPrRecords];
 #pragma unroll
         for (int b = 0; b < kPrRecords; ++b) {
-          const uint32_t tail = *reinterpret_cast<const uint32_t*>(Ts + (s * kPrRecords + b) * 16);
+          const uint32_t tail = Es[s * kPrRecords + b];
           ev[b] = tail_ev(tail);
           const float x = pow2(tail_ek(tail)) * row_c;
           fk[b] = x < 1e-37f ? 1e-37f : x;  // never zero: -inf times it stays -inf (and a NaN stays one)
@@ -459,45 +495,35 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* _
         }
         const int c0 = my_seg == seg ? max(lo - j * kPrKeys, 0) : kPrKeys, c1 = my_seg == seg ? min(p - j * kPrKeys, kPrKeys - 1) : -1;  // the columns that the row sees
         const bool masked = !__all_sync(0xffffffffu, c0 <= 0 && c1 >= kPrKeys - 1);
-        // scores of 64 columns: what the row does not see becomes -inf, caps are applied (the columns' factors are one then)
-        auto shape = [&](uint32_t* v, int at) {
-          if (a.cap > 0.f) {
-#pragma unroll
-            for (int x = 0; x < 64; ++x)
-              v[x] = __float_as_uint(fmaf(-2.f * cap2, __fdividef(1.f, pr_ex2(fminf(__uint_as_float(v[x]) * fk[(at + x) / kBlock] * cap_c, 80.f)) + 1.f), cap2));
-          }
-          if (masked) {
-#pragma unroll
-            for (int x = 0; x < 64; ++x)
-              if (at + x < c0 || at + x > c1) v[x] = 0xff800000u;
-          }
-        };
         auto factor = [&](int b) { return a.cap > 0.f ? 1.f : fk[b]; };
-        uint32_t v[64];
-        float mx = m;
-        auto largest = [&](int at) {
-#pragma unroll
-          for (int b = 0; b < 4; ++b) {
-            float y[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-            for (int x = 0; x < 16; x += 2) {
-              y[0] = fmaxf(y[0], __uint_as_float(v[b * 16 + x]));
-              y[1] = fmaxf(y[1], __uint_as_float(v[b * 16 + x + 1]));
-            }
-            mx = fmaxf(mx, fmaxf(y[0], y[1]) * factor(at / kBlock + b));
-          }
-        };
-        // row maximum: columns 64..127 first (read again later), then 0..63 (kept)
-        tmem_ld32_nowait(t_s + 64, v);
-        tmem_ld32_nowait(t_s + 96, v + 32);
-        tmem_ld_wait64(v);
-        shape(v, 64);
-        largest(64);
+        uint32_t v[kPrKeys];
         tmem_ld32_nowait(t_s, v);
         tmem_ld32_nowait(t_s + 32, v + 32);
+        tmem_ld32_nowait(t_s + 64, v + 64);
+        tmem_ld32_nowait(t_s + 96, v + 96);
         tmem_ld_wait64(v);
-        shape(v, 0);
-        largest(0);
+        tmem_ld_wait64(v + 64);
+        if (a.cap > 0.f) {  // (the columns' factors are in the scores then)
+#pragma unroll
+          for (int x = 0; x < kPrKeys; ++x)
+            v[x] = __float_as_uint(fmaf(-2.f * cap2, __fdividef(1.f, pr_ex2(fminf(__uint_as_float(v[x]) * fk[x / kBlock] * cap_c, 80.f)) + 1.f), cap2));
+        }
+        if (masked) {
+#pragma unroll
+          for (int x = 0; x < kPrKeys; ++x)
+            if (x < c0 || x > c1) v[x] = 0xff800000u;
+        }
+        float mx = m;
+#pragma unroll
+        for (int b = 0; b < kPrRecords; ++b) {
+          float y = fmaxf(__uint_as_float(v[b * 16]), __uint_as_float(v[b * 16 + 1])), z = fmaxf(__uint_as_float(v[b * 16 + 2]), __uint_as_float(v[b * 16 + 3]));
+#pragma unroll
+          for (int x = 4; x < 16; x += 4) {
+            y = fmaxf(fmaxf(y, __uint_as_float(v[b * 16 + x])), __uint_as_float(v[b * 16 + x + 1]));
+            z = fmaxf(fmaxf(z, __uint_as_float(v[b * 16 + x + 2])), __uint_as_float(v[b * 16 + x + 3]));
+          }
+          mx = fmaxf(mx, fmaxf(y, z) * factor(b));
+        }
         const float ref = mx == -INFINITY ? 0.f : mx, fl = pr_ex2(m - ref);
         if (mine > 0) {
           alpha_s[i * kPrRows + r] = fl * pow2(max(E - e_new, -126));
@@ -507,50 +533,36 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* _
         m = mx;
         E = e_new;
         l *= fl;
-        // P of 16 columns -> four columns of each part
-        auto part = [&](const uint32_t* s16, int b, uint32_t* hi, uint32_t* lo4) {
+        // P of 16 columns -> eight columns, into the scores' registers
+        auto part = [&](int b, uint32_t* to) {
           const int shift = max(ev[b] - E, -60) + kPrTop;
           const float fb = factor(b), add = (float)shift - ref;
           float d0 = 0.f, d1 = 0.f;
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            uint32_t h2[2], l2[2];
-#pragma unroll
-            for (int y = 0; y < 2; ++y) {
-              float s0 = __uint_as_float(s16[4 * x + 2 * y]), s1 = __uint_as_float(s16[4 * x + 2 * y + 1]);
-              pr_fma2(s0, s1, fb, add);
-              s0 = pr_ex2(s0);
-              s1 = pr_ex2(s1);
-              d0 += s0;
-              d1 += s1;
-              split2(s0, s1, h2[y], l2[y]);
-            }
-            hi[x] = h2[0] | h2[1] << 16;
-            lo4[x] = l2[0] | l2[1] << 16;
+          for (int x = 0; x < 8; ++x) {
+            float s0 = __uint_as_float(v[b * 16 + 2 * x]), s1 = __uint_as_float(v[b * 16 + 2 * x + 1]);
+            pr_fma2(s0, s1, fb, add);
+            s0 = pr_ex2(s0);
+            s1 = pr_ex2(s1);
+            pr_add2(d0, d1, s0, s1);
+            to[x] = pr_pack(s0, s1);
           }
           l = fmaf(d0 + d1, pow2(-shift), l);
         };
-        uint32_t hi[16], rest[16];
+        uint32_t w[32];
 #pragma unroll
-        for (int b = 0; b < 4; ++b) part(v + b * 16, b, hi + b * 4, rest + b * 4);
-        tmem_ld32_nowait(t_s + 64, v);
-        tmem_ld32_nowait(t_s + 96, v + 32);
-        tmem_ld_wait64(v);  // (ahead of the stores: the columns from 64 on are S's alone)
-        tmem_put16(t_s, hi);
-        tmem_put16(t_s + 32, rest);
-        shape(v, 64);
+        for (int b = 0; b < 4; ++b) part(b, w + b * 8);
+        tmem_put32(t_s, w);
 #pragma unroll
-        for (int b = 0; b < 2; ++b) part(v + b * 16, 4 + b, hi + b * 4, rest + b * 4);
-        pr_put8(t_s + 16, hi);
-        pr_put8(t_s + 48, rest);
+        for (int b = 0; b < 2; ++b) part(4 + b, w + b * 8);
+        tmem_put16(t_s + 32, w);
         tmem_put_wait();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(po_ready + i);
 #pragma unroll
-        for (int b = 2; b < 4; ++b) part(v + b * 16, 4 + b, hi + (b - 2) * 4, rest + (b - 2) * 4);
-        pr_put8(t_s + 24, hi);
-        pr_put8(t_s + 56, rest);
+        for (int b = 0; b < 2; ++b) part(6 + b, w + b * 8);
+        tmem_put16(t_s + 48, w);
         tmem_put_wait();
         tc_fence_before();
         __syncwarp();
@@ -584,7 +596,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* _
 
 template <int D>
 static int launch_prompt(const bf16* q, const bf16* sink, bf16* out, const PromptArgs& f, cudaStream_t st) {
-  constexpr size_t smem = 128 + (size_t)4 * kPrRows * D + (size_t)2 * kPrStages * kPrKeys * D + kPrStages * kPrRecords * 16 + 4 * kPrRows * sizeof(float) + 32 * 8;
+  constexpr size_t smem = 128 + (size_t)4 * kPrRows * D + (size_t)(kPrStages + 3 * kPrStagesV) * kPrKeys * D + kPrStagesV * kPrRecords * 20 + 4 * kPrRows * sizeof(float) + 32 * 8;
   static std::atomic<uint64_t> set{0};
   if (const cudaError_t e = allow_smem(set, (const void*)kv8_prompt_kernel<D>, smem); e != cudaSuccess) return (int)e;
   return (int)launch(kv8_prompt_kernel<D>, dim3(f.a.pool.G, (f.a.T + 2 * f.per - 1) / (2 * f.per)), dim3(kPrThreads), smem, st, true, q, sink, out, f);
