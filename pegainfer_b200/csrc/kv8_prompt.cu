@@ -1,18 +1,21 @@
 // Attention over the 8-bit paged cache for prompts and prompt portions, on tcgen05 (kv8.cuh, kv8_attention.cuh).
 //
 // A CTA has two tiles of 128 rows of one kv head: the group's R query heads of 128 / R consecutive tokens each, so that a key is fetched once for the whole group and
-// few scores lie behind the diagonal.  It goes through the keys in blocks of 128, run by run where its tokens belong to several requests (the other rows are masked).
+// few scores lie behind the diagonal.  It goes through the keys in blocks of 64, run by run where its tokens belong to several requests (the other rows are masked).
 //   * S = q K^T: K's codes are an operand as they lie in the cache (a record's K is two groups of 8 tokens of the canonical layout without swizzle, 8 x 16-byte matrices),
 //     so plain bulk copies fill it.  kind::f8f6f4 wants 8 bits of q too, which has more: it goes in as two numbers, the nearest e4m3 and the rest as e5m2, whose exponents
 //     reach 2^10 further down (4 + 1 + 3 significant bits; bf16 has 8), as many cycles as one product in 16 bits.  A row of q is scaled by a power of two to the upper
 //     end of the codes' range: a bf16 entry is exact down to 2^-17 of the row's largest.
 //   * O += P V in f16: the warps that rescale O turn a block's V into f16 (exactly) before, once for both tiles' 256 rows, which is an eighth of the instructions that
-//     P in two 8-bit parts takes (B200, prompt of 4096, 32 heads in 8 groups: 240 us so).  P is held 2^15 times too large: 11 bits down to 2^-29 of the largest weight.
-//   * K's exponents multiply the scores 16 columns at a time, V's go into P's exponent: 2^(s - m + e - E + 15), E the largest so far; the denominator takes them out.
-//   * The softmax is a thread per row, 128 a tile, with the tiles in turn; O stays in tensor memory and is rescaled by a third group of warps where a maximum moved.
-// Warps: 0-3 softmax tile 0 | 4-7 softmax tile 1 | 8-11 V, rescaling, results | 12, 13 MMA issuers | 14 copies | 15 nothing.  Of the block's registers a softmax thread
-// has 192 (a row's 128 scores stay in them), the others 80 and 48.
-// Tensor memory: S0 | S1 (128 columns each, P over the first 64) | O0 | O1.
+//     P in two 8-bit parts takes (B200, prompt of 4096, 32 heads in 8 groups: 240 us so).
+//   * K's exponents multiply the scores 16 columns at a time, V's go into P's exponent: 2^(s - m + e - E + 7), E the largest so far; the denominator takes them out.
+//   * Blocks of 64 keys with two S per tile: S of the block after next is issued behind P V of this one, so the softmax finds its scores waiting.  (Blocks of 128 with one S: a
+//     tile waited 1600 of 5200 clocks for it.)
+//   * m is a maximum of before that the row's own may have passed by up to 2^8: O, which stays in tensor memory, is rescaled only where one did by more.  P, held 2^7 times
+//     too large, stays within f16's range then, with 11 bits down to 2^-21 of the largest weight.
+// Warps: 0-3 softmax tile 0, a thread per row | 4-7 softmax tile 1 | 8-11 V, rescaling, results | 12, 13 MMA issuers | 14 copies | 15 nothing.  Of the block's registers a
+// softmax thread has 192, the others 80 and 48.
+// Tensor memory: tile 0's two S (64 columns each, P over the first 32) | tile 1's | O0 | O1.
 #include <algorithm>
 
 #include "kv8_attention.cuh"
@@ -21,13 +24,12 @@
 namespace pk {
 namespace kv8 {
 
-constexpr int kPrRows = 128, kPrKeys = 128, kPrRecords = kPrKeys / kBlock;
-constexpr int kPrStages = 3, kPrStagesV = 2;  // of K; of V as it comes and as f16
+constexpr int kPrRows = 128, kPrKeys = 64, kPrRecords = kPrKeys / kBlock;
+constexpr int kPrStages = 4, kPrStagesV = 3;  // of K; of V as it comes and as f16
 constexpr int kPrCorr = 8, kPrMma = 12, kPrLoad = 14, kPrThreads = 16 * 32;
 constexpr int kPrRegsSoft = 192, kPrRegsCorr = 80, kPrRegsMma = 48;
 static_assert(256 * kPrRegsSoft + 128 * kPrRegsCorr + 128 * kPrRegsMma <= kPrThreads * (65536 / kPrThreads), "more registers than the block was launched with");
-constexpr int kPrEarly = 6;        // k-steps of 16 keys of P V (of eight) that begin before the rest of P is there
-constexpr int kPrTop = 15;         // exponent of P = 1
+constexpr int kPrTop = 7, kPrSlack = 8;  // exponents of P = 1 and of what a row's maximum may grow by before O is rescaled: 2^15 in f16
 constexpr uint32_t kRestA = 1u << 7;  // instruction descriptor: A is e5m2
 constexpr int kPrMaxSeg = 256;     // runs that a CTA's tokens can belong to
 
@@ -111,18 +113,17 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* _
   uint8_t* Hs = Vs + kPrStagesV * KB;                    // [stage] V as f16: [8 keys][entry][8 keys' f16]
   uint8_t* Ts = Hs + kPrStagesV * 2 * KB;                // [stage][record] tails as they come
   uint32_t* Es = reinterpret_cast<uint32_t*>(Ts + kPrStagesV * kPrRecords * 16);  // [stage][record] tails of the f16's
-  float* alpha_s = reinterpret_cast<float*>(Es + kPrStagesV * kPrRecords);  // [tile][row]
-  float* end_s = alpha_s + 2 * kPrRows;                  // [tile][row]
+  float* alpha_s = reinterpret_cast<float*>(Es + kPrStagesV * kPrRecords);  // [tile][buffer][row]
+  float* end_s = alpha_s + 4 * kPrRows;                  // [tile][row]
   uint64_t* bars = reinterpret_cast<uint64_t*>(end_s + 2 * kPrRows);
-  uint64_t *k_full = bars, *k_empty = bars + 4, *v_full = bars + 8, *v_empty = bars + 10, *h_full = bars + 12, *h_empty = bars + 14;  // [stage]
-  uint64_t* s_full = bars + 16;    // [tile] S complete                                      MMA -> softmax
-  uint64_t* po_ready = bars + 18;  // [tile] P up to kPrEarly stored, O rescaled (4 + 4 warps)  softmax, rescaling -> MMA
-  uint64_t* p_rest = bars + 20;    // [tile] the rest of P stored (4 warps)                    softmax -> MMA
-  uint64_t* a_ready = bars + 22;   // [tile] factors of O published (4 warps)                  softmax -> rescaling
-  uint64_t* pv_done = bars + 24;   // [tile] P V complete                                     MMA -> rescaling
-  uint64_t* d_ready = bars + 26;   // [tile] last factors published (4 warps)                  softmax -> results
-  uint64_t* done = bars + 28;      // behind a run-out: the MMAs under way
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 29);
+  uint64_t *k_full = bars, *k_empty = bars + 4, *v_full = bars + 8, *v_empty = bars + 11, *h_full = bars + 14, *h_empty = bars + 17;  // [stage]
+  uint64_t* s_full = bars + 20;    // [tile][buffer] S complete                       MMA -> softmax
+  uint64_t* po_ready = bars + 24;  // [tile][buffer] P stored, O rescaled (4 + 4 warps)  softmax, rescaling -> MMA
+  uint64_t* a_ready = bars + 28;   // [tile][buffer] factors of O published (4 warps)    softmax -> rescaling
+  uint64_t* pv_done = bars + 32;   // [tile][buffer] P V complete                      MMA -> rescaling
+  uint64_t* d_ready = bars + 36;   // [tile] last factors published (4 warps)           softmax -> results
+  uint64_t* done = bars + 38;      // behind a run-out: the MMAs under way
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 39);
   volatile int* dead = reinterpret_cast<volatile int*>(tmem_slot + 1);
   __shared__ int s_req[2 * kPrRows], s_slot[2 * kPrRows], s_seg[2 * kPrRows];
   __shared__ int seg_off[kPrMaxSeg], seg_lo[2][kPrMaxSeg], seg_hi[2][kPrMaxSeg];  // page table of a run; blocks of keys that its rows of a tile see
@@ -144,12 +145,13 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* _
       mbar_init(h_full + s, 4);
       mbar_init(h_empty + s, 2);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < 4; ++i) {
       mbar_init(s_full + i, 1);
       mbar_init(po_ready + i, 8);
-      mbar_init(p_rest + i, 4);
       mbar_init(a_ready + i, 4);
       mbar_init(pv_done + i, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
       mbar_init(d_ready + i, 4);
     }
     mbar_init(done, 2);
@@ -206,6 +208,28 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* _
   auto first_block = [&](int seg) { return min(seg_lo[0][seg], seg_lo[1][seg]); };
   auto last_block = [&](int seg) { return max(seg_hi[0][seg], seg_hi[1][seg]); };
   auto needs = [&](int tile, int seg, int j) { return j >= seg_lo[tile][seg] && j <= seg_hi[tile][seg]; };
+  // the blocks of all runs in order, the same for every role
+  struct Step {
+    int seg, j, n;  // n: blocks before it
+  };
+  auto settle = [&](Step& x) {  // on to a run that has a block
+    while (x.seg < segs && last_block(x.seg) < 0) ++x.seg;
+    if (x.seg < segs) x.j = first_block(x.seg);
+  };
+  auto begin = [&] {
+    Step x{0, 0, 0};
+    settle(x);
+    return x;
+  };
+  auto next = [&](Step& x) {
+    ++x.n;
+    if (x.j < last_block(x.seg)) {
+      ++x.j;
+    } else {
+      ++x.seg;
+      settle(x);
+    }
+  };
 
   if (warp >= kPrMma) {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPrRegsMma));
@@ -256,143 +280,143 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* _
     constexpr uint32_t idesc_s = (1u << 4) | ((uint32_t)(kPrKeys >> 3) << 17) | ((uint32_t)(kPrRows >> 4) << 24);  // e4m3 x e4m3 -> fp32, both inner-contiguous
     constexpr uint32_t idesc_pv = (1u << 4) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(kPrRows >> 4) << 24);
     const uint64_t q_hi = plain_desc(smem_u32(Qs + i * 2 * QB), 128, 8 * D), q_lo = plain_desc(smem_u32(Qs + (i * 2 + 1) * QB), 128, 8 * D);
-    const uint32_t t_s = tmem_base + (uint32_t)(i * kPrKeys), t_o = tmem_base + (uint32_t)(2 * kPrKeys + i * 128);
-    int n = 0, mine = 0;  // blocks so far, of them this tile's
-    // S of the next block of this tile is issued behind P V of the last one: `pending` is that block
-    int p_stage = -1;
-    auto finish = [&] {  // P V of the pending block
-      const int s = p_stage;
-      mbar_wait_bounded(po_ready + i, (uint32_t)((mine - 1) & 1), dead, tries);
+    const uint32_t t_s = tmem_base + (uint32_t)(i * 2 * kPrKeys), t_o = tmem_base + (uint32_t)(4 * kPrKeys + i * 128);
+    int issued = 0, finished = 0, waiting[2] = {0, 0};  // this tile's blocks: S issued, P V issued; the stages of V of those between
+    auto finish = [&] {
+      const int sv = waiting[finished & 1] % kPrStagesV;
+      mbar_wait_bounded(h_full + sv, (uint32_t)((waiting[finished & 1] / kPrStagesV) & 1), dead, tries);
+      mbar_wait_bounded(po_ready + i * 2 + (finished & 1), (uint32_t)((finished >> 1) & 1), dead, tries);
       tc_fence_after();
-      const uint64_t v_desc = plain_desc(smem_u32(Hs + s * 2 * KB), REC_K, 128);  // 8 keys x 8 entries
+      const uint64_t v_desc = plain_desc(smem_u32(Hs + sv * 2 * KB), REC_K, 128);  // 8 keys x 8 entries
+      const uint32_t t_p = t_s + (uint32_t)((finished & 1) * kPrKeys);
       if (tc_elect_one()) {
 #pragma unroll
-        for (int k = 0; k < kPrEarly; ++k)
-          umma_f16_ts(t_o, t_s + (uint32_t)(k * 8), v_desc + (uint64_t)(k * (2 * REC_K >> 4)), idesc_pv, (mine > 1 || k > 0) ? 1u : 0u);
+        for (int k = 0; k < kPrKeys / 16; ++k)
+          umma_f16_ts(t_o, t_p + (uint32_t)(k * 8), v_desc + (uint64_t)(k * (2 * REC_K >> 4)), idesc_pv, (finished > 0 || k > 0) ? 1u : 0u);
+        umma_commit(pv_done + i * 2 + (finished & 1));
+        umma_commit(h_empty + sv);
       }
       __syncwarp();
-      mbar_wait_bounded(p_rest + i, (uint32_t)((mine - 1) & 1), dead, tries);
-      tc_fence_after();
-      if (tc_elect_one()) {
-#pragma unroll
-        for (int k = kPrEarly; k < kPrKeys / 16; ++k) umma_f16_ts(t_o, t_s + (uint32_t)(k * 8), v_desc + (uint64_t)(k * (2 * REC_K >> 4)), idesc_pv, 1u);
-        umma_commit(pv_done + i);
-        umma_commit(h_empty + s);
-      }
-      __syncwarp();
-      p_stage = -1;
+      ++finished;
     };
-    for (int seg = 0; seg < segs; ++seg) {
-      const int j1 = last_block(seg);
-      for (int j = j1 < 0 ? 0 : first_block(seg); j <= j1; ++j, ++n) {
-        const int s = n % kPrStages, sv = n % kPrStagesV;
-        const uint32_t ph = (uint32_t)((n / kPrStages) & 1), phv = (uint32_t)((n / kPrStagesV) & 1);
-        if (!needs(i, seg, j)) {  // not this tile's: its arrivals, each in its phase
-          if (p_stage >= 0) finish();  // (the copies of later blocks wait for it)
-          mbar_wait_bounded(k_full + s, ph, dead, tries);
-          if (lane == 0) mbar_arrive(k_empty + s);
-          mbar_wait_bounded(h_full + sv, phv, dead, tries);
-          if (lane == 0) mbar_arrive(h_empty + sv);
-          __syncwarp();
-          continue;
-        }
+    for (Step x = begin(); x.seg < segs; next(x)) {
+      const int s = x.n % kPrStages, sv = x.n % kPrStagesV;
+      const uint32_t ph = (uint32_t)((x.n / kPrStages) & 1);
+      if (!needs(i, x.seg, x.j)) {  // not this tile's: its arrivals, each in its phase
+        while (finished < issued) finish();  // (the copies of later blocks wait for them)
         mbar_wait_bounded(k_full + s, ph, dead, tries);
-        if (p_stage >= 0) finish();
-        else if (i == 1 && mine == 0 && n == 0 && needs(0, seg, j)) mbar_wait_bounded(po_ready + 0, 0, dead, tries);  // half a block behind the other tile
-        tc_fence_after();
-        const uint64_t k_desc = plain_desc(smem_u32(Ks + s * KB), 128, 8 * D);
-        if (tc_elect_one()) {
-#pragma unroll
-          for (int k = 0; k < D / 32; ++k) {
-            umma_f8(t_s, q_hi + (uint64_t)(k * 16), k_desc + (uint64_t)(k * 16), idesc_s, k > 0 ? 1u : 0u);
-            umma_f8(t_s, q_lo + (uint64_t)(k * 16), k_desc + (uint64_t)(k * 16), idesc_s | kRestA, 1u);
-          }
-          umma_commit(s_full + i);
-          umma_commit(k_empty + s);
-        }
+        if (lane == 0) mbar_arrive(k_empty + s);
+        mbar_wait_bounded(h_full + sv, (uint32_t)((x.n / kPrStagesV) & 1), dead, tries);
+        if (lane == 0) mbar_arrive(h_empty + sv);
         __syncwarp();
-        ++mine;
-        mbar_wait_bounded(h_full + sv, phv, dead, tries);
-        p_stage = sv;
+        continue;
       }
+      if (issued - finished == 2) finish();  // its S and P lie where the next S goes
+      mbar_wait_bounded(k_full + s, ph, dead, tries);
+      tc_fence_after();
+      const uint64_t k_desc = plain_desc(smem_u32(Ks + s * KB), 128, 8 * D);
+      const uint32_t t_d = t_s + (uint32_t)((issued & 1) * kPrKeys);
+      if (tc_elect_one()) {
+#pragma unroll
+        for (int k = 0; k < D / 32; ++k) {
+          umma_f8(t_d, q_hi + (uint64_t)(k * 16), k_desc + (uint64_t)(k * 16), idesc_s, k > 0 ? 1u : 0u);
+          umma_f8(t_d, q_lo + (uint64_t)(k * 16), k_desc + (uint64_t)(k * 16), idesc_s | kRestA, 1u);
+        }
+        umma_commit(s_full + i * 2 + (issued & 1));
+        umma_commit(k_empty + s);
+      }
+      __syncwarp();
+      waiting[issued & 1] = x.n;
+      ++issued;
     }
-    if (p_stage >= 0) finish();
+    while (finished < issued) finish();
   }
   } else if (warp >= kPrCorr) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPrRegsCorr));
     // =========================== rescaling of O, results ===========================
     const int q4 = warp & 3, r = q4 * 32 + lane;
     const uint32_t lane_base = tmem_base + ((uint32_t)(q4 * 32) << 16);
-    int mine[2] = {0, 0}, n = 0;
-    for (int seg = 0; seg < segs; ++seg) {
-      const int j1 = last_block(seg);
-      for (int j = j1 < 0 ? 0 : first_block(seg); j <= j1; ++j, ++n) {
-        {  // the block's V: a thread takes an entry's 16 keys of a record at a time
-          const int sv = n % kPrStagesV;
-          const uint32_t phv = (uint32_t)((n / kPrStagesV) & 1);
-          mbar_wait_bounded(v_full + sv, phv, dead, tries);
-          mbar_wait_bounded(h_empty + sv, phv ^ 1u, dead, tries);
-          const uint8_t* from = Vs + sv * KB;
-          uint8_t* to = Hs + sv * 2 * KB;
+    int mine[2] = {0, 0};
+    auto widen_v = [&](int n) {  // the V of block n: a thread takes an entry's 16 keys of a record at a time
+      const int sv = n % kPrStagesV;
+      const uint32_t phv = (uint32_t)((n / kPrStagesV) & 1);
+      mbar_wait_bounded(v_full + sv, phv, dead, tries);
+      mbar_wait_bounded(h_empty + sv, phv ^ 1u, dead, tries);
+      const uint8_t* from = Vs + sv * KB;
+      uint8_t* to = Hs + sv * 2 * KB;
 #pragma unroll 4
-          for (int u = r; u < kPrRecords * D; u += 128) {
-            const int b = u / D, d = u - b * D;
-            const uint4 x = *reinterpret_cast<const uint4*>(from + u * 16);
-            uint32_t h[8];
-            pr_widen(x.x, h[0], h[1]);
-            pr_widen(x.y, h[2], h[3]);
-            pr_widen(x.z, h[4], h[5]);
-            pr_widen(x.w, h[6], h[7]);
-            *reinterpret_cast<uint4*>(to + (2 * b) * REC_K + d * 16) = make_uint4(h[0], h[1], h[2], h[3]);
-            *reinterpret_cast<uint4*>(to + (2 * b + 1) * REC_K + d * 16) = make_uint4(h[4], h[5], h[6], h[7]);
-          }
-          if (r < kPrRecords) Es[sv * kPrRecords + r] = *reinterpret_cast<const uint32_t*>(Ts + (sv * kPrRecords + r) * 16);
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            mbar_arrive(h_full + sv);
-            mbar_arrive(v_empty + sv);
-          }
-        }
+      for (int u = r; u < kPrRecords * D; u += 128) {
+        const int b = u / D, d = u - b * D;
+        const uint4 x = *reinterpret_cast<const uint4*>(from + u * 16);
+        uint32_t h[8];
+        pr_widen(x.x, h[0], h[1]);
+        pr_widen(x.y, h[2], h[3]);
+        pr_widen(x.z, h[4], h[5]);
+        pr_widen(x.w, h[6], h[7]);
+        *reinterpret_cast<uint4*>(to + (2 * b) * REC_K + d * 16) = make_uint4(h[0], h[1], h[2], h[3]);
+        *reinterpret_cast<uint4*>(to + (2 * b + 1) * REC_K + d * 16) = make_uint4(h[4], h[5], h[6], h[7]);
+      }
+      if (r < kPrRecords) Es[sv * kPrRecords + r] = *reinterpret_cast<const uint32_t*>(Ts + (sv * kPrRecords + r) * 16);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(h_full + sv);
+        mbar_arrive(v_empty + sv);
+      }
+    };
+    // O holds all blocks before this one.  (Only waited for where somebody needs it: of a buffer's phases at most the last is not over by then, since S of the block
+    // before this one came behind the P V before it.)
+    auto all_added = [&](int i) {
+      if (mine[i] > 0) mbar_wait_bounded(pv_done + i * 2 + ((mine[i] - 1) & 1), (uint32_t)(((mine[i] - 1) >> 1) & 1), dead, tries);
+    };
+    Step ahead = begin();
+    if (ahead.seg < segs) {
+      widen_v(0);
+      next(ahead);
+    }
+    for (Step x = begin(); x.seg < segs; next(x)) {
+      if (ahead.seg < segs) {  // a block ahead of the softmax
+        widen_v(ahead.n);
+        next(ahead);
+      }
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          if (!needs(i, seg, j)) continue;
-          if (mine[i] > 0) {
-            mbar_wait_bounded(a_ready + i, (uint32_t)((mine[i] - 1) & 1), dead, tries);
-            const float alpha = alpha_s[i * kPrRows + r];
-            const bool need = !__all_sync(0xffffffffu, alpha == 1.0f);
-            mbar_wait_bounded(pv_done + i, (uint32_t)((mine[i] - 1) & 1), dead, tries);
+      for (int i = 0; i < 2; ++i) {
+        if (!needs(i, x.seg, x.j)) continue;
+        const int at = i * 2 + (mine[i] & 1);
+        mbar_wait_bounded(a_ready + at, (uint32_t)((mine[i] >> 1) & 1), dead, tries);
+        const float alpha = alpha_s[at * kPrRows + r];
+        if (mine[i] > 0) {
+          if (!__all_sync(0xffffffffu, alpha == 1.0f)) {
+            all_added(i);
             tc_fence_after();
-            if (need) {
-              const uint32_t t_o = lane_base + (uint32_t)(2 * kPrKeys + i * 128);
+            const uint32_t t_o = lane_base + (uint32_t)(4 * kPrKeys + i * 128);
 #pragma unroll
-              for (int c = 0; c < D; c += 32) {
-                uint32_t t[32];
-                tmem_ld32(t_o + c, t);
+            for (int c = 0; c < D; c += 32) {
+              uint32_t t[32];
+              tmem_ld32(t_o + c, t);
 #pragma unroll
-                for (int x = 0; x < 32; ++x) t[x] = __float_as_uint(__uint_as_float(t[x]) * alpha);
-                tmem_put32(t_o + c, t);
-              }
-              tmem_put_wait();
+              for (int k = 0; k < 32; ++k) t[k] = __float_as_uint(__uint_as_float(t[k]) * alpha);
+              tmem_put32(t_o + c, t);
             }
+            tmem_put_wait();
             tc_fence_before();
           }
-          __syncwarp();
-          if (lane == 0) mbar_arrive(po_ready + i);
-          ++mine[i];
         }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(po_ready + at);
+        ++mine[i];
       }
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       mbar_wait_bounded(d_ready + i, 0, dead, tries);
-      if (mine[i] > 0) mbar_wait_bounded(pv_done + i, (uint32_t)((mine[i] - 1) & 1), dead, tries);
+      all_added(i);
       tc_fence_after();
       const int k = r / R, ti = i * per + k;
       const bool on = k < per && ti < n_tok;
       const float factor = end_s[i * kPrRows + r];
       bf16* dst = out + (size_t)(t0 + (on ? ti : 0)) * a.out_ld + (g * R + (on ? r - k * R : 0)) * D;
-      const uint32_t t_o = lane_base + (uint32_t)(2 * kPrKeys + i * 128);
+      const uint32_t t_o = lane_base + (uint32_t)(4 * kPrKeys + i * 128);
 #pragma unroll
       for (int c = 0; c < D; c += 32) {
         uint32_t t[32];
@@ -470,105 +494,89 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* _
     fence_proxy_async_smem();
     asm volatile("bar.sync 1, %0;" ::"n"(10 * 32) : "memory");
 
-    const uint32_t t_s = tmem_base + ((uint32_t)(q4 * 32) << 16) + (uint32_t)(i * kPrKeys);
+    const uint32_t t_tile = tmem_base + ((uint32_t)(q4 * 32) << 16) + (uint32_t)(i * 2 * kPrKeys);
     const float cap2 = a.cap * kLog2e, cap_c = a.cap > 0.f ? 2.f * a.scale / a.cap * kLog2e : 0.f;
     float m = -INFINITY, l = 0.f;
-    int E = kLowExp - 1, n = 0, mine = 0;
-    for (int seg = 0; seg < segs; ++seg) {
-      const int j1 = last_block(seg);
-      for (int j = j1 < 0 ? 0 : first_block(seg); j <= j1; ++j, ++n) {
-        if (!needs(i, seg, j)) continue;
-        const int s = n % kPrStagesV;
-        // S first: it says that the stage's phases before this block's are over (a tile that skipped blocks would take an older one for it)
-        mbar_wait_bounded(s_full + i, (uint32_t)(mine & 1), dead, tries);
-        mbar_wait_bounded(h_full + s, (uint32_t)((n / kPrStagesV) & 1), dead, tries);
-        tc_fence_after();
-        int ev[kPrRecords], e_new = E;
-        float fk[kPrRecords];
+    int E = kLowExp - 1, mine = 0;
+    for (Step x = begin(); x.seg < segs; next(x)) {
+      if (!needs(i, x.seg, x.j)) continue;
+      const int sv = x.n % kPrStagesV;
+      const uint32_t t_s = t_tile + (uint32_t)((mine & 1) * kPrKeys);
+      // S first: it says that the stage's phases before this block's are over (a tile that skipped blocks would take an older one for it)
+      mbar_wait_bounded(s_full + i * 2 + (mine & 1), (uint32_t)((mine >> 1) & 1), dead, tries);
+      tc_fence_after();
+      uint32_t v[kPrKeys];
+      tmem_ld32_nowait(t_s, v);
+      tmem_ld32_nowait(t_s + 32, v + 32);
+      mbar_wait_bounded(h_full + sv, (uint32_t)((x.n / kPrStagesV) & 1), dead, tries);
+      int ev[kPrRecords], e_new = E;
+      float fk[kPrRecords];
 #pragma unroll
-        for (int b = 0; b < kPrRecords; ++b) {
-          const uint32_t tail = Es[s * kPrRecords + b];
-          ev[b] = tail_ev(tail);
-          const float x = pow2(tail_ek(tail)) * row_c;
-          fk[b] = x < 1e-37f ? 1e-37f : x;  // never zero: -inf times it stays -inf (and a NaN stays one)
-          e_new = max(e_new, ev[b]);
-        }
-        const int c0 = my_seg == seg ? max(lo - j * kPrKeys, 0) : kPrKeys, c1 = my_seg == seg ? min(p - j * kPrKeys, kPrKeys - 1) : -1;  // the columns that the row sees
-        const bool masked = !__all_sync(0xffffffffu, c0 <= 0 && c1 >= kPrKeys - 1);
-        auto factor = [&](int b) { return a.cap > 0.f ? 1.f : fk[b]; };
-        uint32_t v[kPrKeys];
-        tmem_ld32_nowait(t_s, v);
-        tmem_ld32_nowait(t_s + 32, v + 32);
-        tmem_ld32_nowait(t_s + 64, v + 64);
-        tmem_ld32_nowait(t_s + 96, v + 96);
-        tmem_ld_wait64(v);
-        tmem_ld_wait64(v + 64);
-        if (a.cap > 0.f) {  // (the columns' factors are in the scores then)
-#pragma unroll
-          for (int x = 0; x < kPrKeys; ++x)
-            v[x] = __float_as_uint(fmaf(-2.f * cap2, __fdividef(1.f, pr_ex2(fminf(__uint_as_float(v[x]) * fk[x / kBlock] * cap_c, 80.f)) + 1.f), cap2));
-        }
-        if (masked) {
-#pragma unroll
-          for (int x = 0; x < kPrKeys; ++x)
-            if (x < c0 || x > c1) v[x] = 0xff800000u;
-        }
-        float mx = m;
-#pragma unroll
-        for (int b = 0; b < kPrRecords; ++b) {
-          float y = fmaxf(__uint_as_float(v[b * 16]), __uint_as_float(v[b * 16 + 1])), z = fmaxf(__uint_as_float(v[b * 16 + 2]), __uint_as_float(v[b * 16 + 3]));
-#pragma unroll
-          for (int x = 4; x < 16; x += 4) {
-            y = fmaxf(fmaxf(y, __uint_as_float(v[b * 16 + x])), __uint_as_float(v[b * 16 + x + 1]));
-            z = fmaxf(fmaxf(z, __uint_as_float(v[b * 16 + x + 2])), __uint_as_float(v[b * 16 + x + 3]));
-          }
-          mx = fmaxf(mx, fmaxf(y, z) * factor(b));
-        }
-        const float ref = mx == -INFINITY ? 0.f : mx, fl = pr_ex2(m - ref);
-        if (mine > 0) {
-          alpha_s[i * kPrRows + r] = fl * pow2(max(E - e_new, -126));
-          __syncwarp();
-          if (lane == 0) mbar_arrive(a_ready + i);
-        }
-        m = mx;
-        E = e_new;
-        l *= fl;
-        // P of 16 columns -> eight columns, into the scores' registers
-        auto part = [&](int b, uint32_t* to) {
-          const int shift = max(ev[b] - E, -60) + kPrTop;
-          const float fb = factor(b), add = (float)shift - ref;
-          float d0 = 0.f, d1 = 0.f;
-#pragma unroll
-          for (int x = 0; x < 8; ++x) {
-            float s0 = __uint_as_float(v[b * 16 + 2 * x]), s1 = __uint_as_float(v[b * 16 + 2 * x + 1]);
-            pr_fma2(s0, s1, fb, add);
-            s0 = pr_ex2(s0);
-            s1 = pr_ex2(s1);
-            pr_add2(d0, d1, s0, s1);
-            to[x] = pr_pack(s0, s1);
-          }
-          l = fmaf(d0 + d1, pow2(-shift), l);
-        };
-        uint32_t w[32];
-#pragma unroll
-        for (int b = 0; b < 4; ++b) part(b, w + b * 8);
-        tmem_put32(t_s, w);
-#pragma unroll
-        for (int b = 0; b < 2; ++b) part(4 + b, w + b * 8);
-        tmem_put16(t_s + 32, w);
-        tmem_put_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(po_ready + i);
-#pragma unroll
-        for (int b = 0; b < 2; ++b) part(6 + b, w + b * 8);
-        tmem_put16(t_s + 48, w);
-        tmem_put_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(p_rest + i);
-        ++mine;
+      for (int b = 0; b < kPrRecords; ++b) {
+        const uint32_t tail = Es[sv * kPrRecords + b];
+        ev[b] = tail_ev(tail);
+        const float y = pow2(tail_ek(tail)) * row_c;
+        fk[b] = y < 1e-37f ? 1e-37f : y;  // never zero: -inf times it stays -inf (and a NaN stays one)
+        e_new = max(e_new, ev[b]);
       }
+      const int c0 = my_seg == x.seg ? max(lo - x.j * kPrKeys, 0) : kPrKeys, c1 = my_seg == x.seg ? min(p - x.j * kPrKeys, kPrKeys - 1) : -1;  // the columns that the row sees
+      const bool masked = !__all_sync(0xffffffffu, c0 <= 0 && c1 >= kPrKeys - 1);
+      auto factor = [&](int b) { return a.cap > 0.f ? 1.f : fk[b]; };
+      tmem_ld_wait64(v);
+      if (a.cap > 0.f) {  // (the columns' factors are in the scores then)
+#pragma unroll
+        for (int k = 0; k < kPrKeys; ++k)
+          v[k] = __float_as_uint(fmaf(-2.f * cap2, __fdividef(1.f, pr_ex2(fminf(__uint_as_float(v[k]) * fk[k / kBlock] * cap_c, 80.f)) + 1.f), cap2));
+      }
+      if (masked) {
+#pragma unroll
+        for (int k = 0; k < kPrKeys; ++k)
+          if (k < c0 || k > c1) v[k] = 0xff800000u;
+      }
+      float mx = m;
+#pragma unroll
+      for (int b = 0; b < kPrRecords; ++b) {
+        float y = fmaxf(__uint_as_float(v[b * 16]), __uint_as_float(v[b * 16 + 1])), z = fmaxf(__uint_as_float(v[b * 16 + 2]), __uint_as_float(v[b * 16 + 3]));
+#pragma unroll
+        for (int k = 4; k < 16; k += 4) {
+          y = fmaxf(fmaxf(y, __uint_as_float(v[b * 16 + k])), __uint_as_float(v[b * 16 + k + 1]));
+          z = fmaxf(fmaxf(z, __uint_as_float(v[b * 16 + k + 2])), __uint_as_float(v[b * 16 + k + 3]));
+        }
+        mx = fmaxf(mx, fmaxf(y, z) * factor(b));
+      }
+      const float m_new = mx > m + (float)kPrSlack ? mx : m;  // (m = -inf: mx)
+      const float ref = m_new == -INFINITY ? 0.f : m_new, fl = pr_ex2(m - ref);
+      // (a row that saw nothing so far has nothing in O; nothing is rescaled at the first block)
+      alpha_s[(i * 2 + (mine & 1)) * kPrRows + r] = (m == -INFINITY ? 1.f : fl) * pow2(max(E - e_new, -126));
+      __syncwarp();
+      if (lane == 0) mbar_arrive(a_ready + i * 2 + (mine & 1));
+      m = m_new;
+      E = e_new;
+      l *= fl;
+      // P of 16 columns -> eight columns
+      uint32_t w[kPrKeys / 2];
+#pragma unroll
+      for (int b = 0; b < kPrRecords; ++b) {
+        const int shift = max(ev[b] - E, -60) + kPrTop;
+        const float fb = factor(b), add = (float)shift - ref;
+        float d0 = 0.f, d1 = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          float s0 = __uint_as_float(v[b * 16 + 2 * k]), s1 = __uint_as_float(v[b * 16 + 2 * k + 1]);
+          pr_fma2(s0, s1, fb, add);
+          s0 = pr_ex2(s0);
+          s1 = pr_ex2(s1);
+          pr_add2(d0, d1, s0, s1);
+          w[b * 8 + k] = pr_pack(s0, s1);
+        }
+        l = fmaf(d0 + d1, pow2(-shift), l);
+      }
+      tmem_put32(t_s, w);
+      tmem_put_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(po_ready + i * 2 + (mine & 1));
+      ++mine;
     }
     const float top = l != l ? INFINITY : m;  // a NaN among the scores
     const RowEnd end = row_end(top, l, sink ? bf2f(sink[h]) : 0.f, sink != nullptr);
@@ -596,7 +604,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* _
 
 template <int D>
 static int launch_prompt(const bf16* q, const bf16* sink, bf16* out, const PromptArgs& f, cudaStream_t st) {
-  constexpr size_t smem = 128 + (size_t)4 * kPrRows * D + (size_t)(kPrStages + 3 * kPrStagesV) * kPrKeys * D + kPrStagesV * kPrRecords * 20 + 4 * kPrRows * sizeof(float) + 32 * 8;
+  constexpr size_t smem = 128 + (size_t)4 * kPrRows * D + (size_t)(kPrStages + 3 * kPrStagesV) * kPrKeys * D + kPrStagesV * kPrRecords * 20 + 6 * kPrRows * sizeof(float) + 40 * 8;
   static std::atomic<uint64_t> set{0};
   if (const cudaError_t e = allow_smem(set, (const void*)kv8_prompt_kernel<D>, smem); e != cudaSuccess) return (int)e;
   return (int)launch(kv8_prompt_kernel<D>, dim3(f.a.pool.G, (f.a.T + 2 * f.per - 1) / (2 * f.per)), dim3(kPrThreads), smem, st, true, q, sink, out, f);
