@@ -219,13 +219,14 @@ static Plan plan(int T, int H, int G, int dim, int vdim, const pk_kv8_options& o
   }
   if (!f32 && prompt_takes(T, H, G, dim, vdim)) {
     p.prompt = true;
-    return p;
+    p.shares = prompt_shares(T, H, G, o.max_kv_len, o.window);
+  } else {
+    int span = o.max_kv_len;
+    if (o.window > 0) span = std::min(span, o.window + kBlock);
+    const int records = (span + kBlock - 1) / kBlock;
+    // a share has at least two rounds of its warps
+    p.shares = (int)std::max(1L, std::min((long)(records + 2 * kRowWarps - 1) / (2 * kRowWarps), (4L * sm_count() + (long)T * H - 1) / ((long)T * H)));
   }
-  int span = o.max_kv_len;
-  if (o.window > 0) span = std::min(span, o.window + kBlock);
-  const int records = (span + kBlock - 1) / kBlock;
-  // a share has at least two rounds of its warps
-  p.shares = std::max(1, std::min((records + 2 * kRowWarps - 1) / (2 * kRowWarps), (4 * sm_count() + T * H - 1) / (T * H)));
   if (p.shares > 1) {
     p.o_bytes = up16((size_t)p.shares * T * H * vdim * sizeof(float));
     p.ml_bytes = up16((size_t)p.shares * T * H * sizeof(float2));
@@ -238,12 +239,15 @@ static int mass_rows(const E* q, const AttnArgs& a, cudaStream_t st) {
   return (int)launch(kv8_mass_row_kernel<E>, dim3((a.max_kv_len + 63) / 64, a.pool.G), dim3(128), 0, st, true, q, a);
 }
 template <typename E>
+static int merge(const E* sink, E* out, int shares, const AttnArgs& a, cudaStream_t st) {
+  return (int)launch(kv8_merge_kernel<E>, dim3((unsigned)(((size_t)a.T * a.H + 3) / 4)), dim3(128), 0, st, true, sink, out, shares, a);
+}
+template <typename E>
 static int attention(const E* q, const E* sink, E* out, const AttnArgs& a, const Plan& p, cudaStream_t st) {
   const size_t smem = (size_t)(a.pool.dim + kRowWarps * a.pool.vdim) * sizeof(float);
   if (const cudaError_t e = launch(kv8_row_kernel<E>, dim3(a.T, a.H, p.shares), dim3(kRowWarps * 32), smem, st, true, q, sink, out, a); e != cudaSuccess) return (int)e;
   if (p.shares > 1)
-    if (const cudaError_t e = launch(kv8_merge_kernel<E>, dim3((unsigned)(((size_t)a.T * a.H + 3) / 4)), dim3(128), 0, st, true, sink, out, p.shares, a); e != cudaSuccess)
-      return (int)e;
+    if (const int rc = merge(sink, out, p.shares, a, st); rc != 0) return rc;
   return a.mass ? mass_rows(q, a, st) : 0;
 }
 
@@ -287,13 +291,14 @@ extern "C" int pk_kv8_attention(const void* q, const void* cache, const void* si
   a.mass = options->mass;
   a.mass_ld = options->mass_ld;
   if (p.few) return kv8::few_attention((const bf16*)q, (const bf16*)sink, (bf16*)out, a, options->max_q_len, p.need, ws, st);
+  a.part_o = reinterpret_cast<float*>(ws);
+  a.part_ml = reinterpret_cast<float2*>(ws + p.o_bytes);
   if (p.prompt) {
-    const int rc = kv8::prompt_attention((const bf16*)q, (const bf16*)sink, (bf16*)out, a, st);
+    int rc = kv8::prompt_attention((const bf16*)q, (const bf16*)sink, (bf16*)out, a, p.shares, st);
+    if (rc == 0 && p.shares > 1) rc = kv8::merge((const bf16*)sink, (bf16*)out, p.shares, a, st);
     if (rc != 0 || !a.mass) return rc;
     return kv8::mass_takes((const bf16*)q, dim, vdim) ? kv8::mass_rows_mma((const bf16*)q, a, options->max_q_len, st) : kv8::mass_rows((const bf16*)q, a, st);
   }
-  a.part_o = reinterpret_cast<float*>(ws);
-  a.part_ml = reinterpret_cast<float2*>(ws + p.o_bytes);
   if (f32) return kv8::attention((const float*)q, (const float*)sink, (float*)out, a, p, st);
   return kv8::attention((const bf16*)q, (const bf16*)sink, (bf16*)out, a, p, st);
 }

@@ -60,9 +60,10 @@ bool few_takes(int T, int H, int G, int dim, int vdim, int max_kv_len, int max_q
 FewNeed few_need(int T, int H, int G, int dim, int max_kv_len, bool mass);
 int few_attention(const bf16* q, const bf16* sink, bf16* out, const AttnArgs& a, int max_q_len, const FewNeed& need, uint8_t* ws, cudaStream_t st);
 
-// kv8_prompt.cu: whether it takes a call, and the call (no workspace)
+// kv8_prompt.cu: whether it takes a call, the shares that it cuts the keys into (more than one: states to part_o, part_ml, for kv8_merge_kernel), and the call
 bool prompt_takes(int T, int H, int G, int dim, int vdim);
-int prompt_attention(const bf16* q, const bf16* sink, bf16* out, const AttnArgs& a, cudaStream_t st);
+int prompt_shares(int T, int H, int G, int max_kv_len, int window);
+int prompt_attention(const bf16* q, const bf16* sink, bf16* out, const AttnArgs& a, int shares, cudaStream_t st);
 // kv8_mass.cu: the weights' sums of such a call
 bool mass_takes(const bf16* q, int dim, int vdim);
 int mass_rows_mma(const bf16* q, const AttnArgs& a, int max_q_len, cudaStream_t st);

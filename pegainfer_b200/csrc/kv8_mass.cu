@@ -13,7 +13,6 @@ namespace pk {
 namespace kv8 {
 
 constexpr int kMassWarps = 4, kMassRows = 64;
-constexpr int mass_records(int D) { return D <= 128 ? 2 : 1; }  // of a warp
 
 __device__ __forceinline__ float ms_ex2(float x) {
   float y;
@@ -26,12 +25,13 @@ __device__ __forceinline__ uint32_t bf16_of(uint32_t two) {
   return pack_bf16(v.x, v.y);
 }
 
-template <int D>
+template <int D, int RECS>
 __global__ void __launch_bounds__(kMassWarps * 32) kv8_mass_kernel(const bf16* __restrict__ q, AttnArgs a) {
-  constexpr int RECS = mass_records(D), LD = D + 8, REC = kBlock * 2 * D + 16;
+  constexpr int LD = D + 8;
   extern __shared__ __align__(16) bf16 ms_q[];  // [2][rows][LD]
-  __shared__ float s_lse[2][kMassRows];         // log2; +inf: no such row
-  __shared__ int s_p[2][kMassRows];
+  __shared__ __align__(8) float s_lse[2][kMassRows];  // log2; +inf: no such row
+  __shared__ __align__(8) int s_p[2][kMassRows];
+  __shared__ int s_half[2][2];  // whether 32 rows see every key of the CTA
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gq = lane >> 2, tq = lane & 3, g = blockIdx.y, R = a.H / a.pool.G, V = a.pool.vdim;
   const int b0 = (blockIdx.x * kMassWarps + warp) * RECS;  // the warp's first record
   const int key0 = blockIdx.x * kMassWarps * RECS * kBlock, key1 = key0 + kMassWarps * RECS * kBlock - 1;
@@ -85,6 +85,12 @@ __global__ void __launch_bounds__(kMassWarps * 32) kv8_mass_kernel(const bf16* _
         const int at = tile * kMassRows + threadIdx.x, t = t0 + min(at, rows - 1) / R, p = at < rows ? a.slots[t] : -1;
         s_p[s][threadIdx.x] = p;
         s_lse[s][threadIdx.x] = p >= 0 ? a.lse[(size_t)t * a.H + g * R + at % R] * kLog2e : INFINITY;
+        const bool all = p >= key1 && (a.window <= 0 || key0 > p - a.window);
+        if (threadIdx.x < 32) {  // (two halves of the rows)
+          s_half[s][0] = __all_sync(0xffffffffu, all);
+        } else {
+          s_half[s][1] = __all_sync(0xffffffffu, all);
+        }
       }
       cp_async_commit();
     };
@@ -114,34 +120,46 @@ __global__ void __launch_bounds__(kMassWarps * 32) kv8_mass_kernel(const bf16* _
       asm volatile("cp.async.wait_group 1;" ::: "memory");
       __syncthreads();
       const bf16* qt = ms_q + (size_t)s * kMassRows * LD;
+      const bool whole = s_half[s][0] && s_half[s][1];
 #pragma unroll 1
-      for (int n = 0; n < kMassRows / 8; ++n) {
-        float acc[RECS][4] = {};
+      for (int n = 0; n < kMassRows / 8; n += 2) {  // two chains of products
+        float acc[2][RECS][4] = {};
 #pragma unroll
-        for (int k = 0; k < D / 32; ++k) {
-          uint32_t b[4];
-          ldsm_x4(b, qt + (n * 8 + (lane & 7)) * LD + k * 32 + (lane >> 3) * 8);
+        for (int k = 0; k < D / 32; ++k)
 #pragma unroll
-          for (int r = 0; r < RECS; ++r) {
-            mma_bf16_16816(acc[r], ka[r][2 * k], b[0], b[1]);
-            mma_bf16_16816(acc[r], ka[r][2 * k + 1], b[2], b[3]);
-          }
-        }
-        const int row = n * 8 + 2 * tq;
+          for (int x = 0; x < 2; ++x) {
+            uint32_t b[4];
+            ldsm_x4(b, qt + ((n + x) * 8 + (lane & 7)) * LD + k * 32 + (lane >> 3) * 8);
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float lse = s_lse[s][row + e];
-          const int p = s_p[s][row + e], lo = a.window > 0 ? p - a.window + 1 : 0;
-#pragma unroll
-          for (int r = 0; r < RECS; ++r)
-#pragma unroll
-            for (int y = 0; y < 2; ++y) {
-              float v = acc[r][2 * y + e] * fk[r];
-              if (a.cap > 0.f) v = fmaf(-2.f * cap2, __fdividef(1.f, ms_ex2(fminf(v * cap_c, 80.f)) + 1.f), cap2);
-              const int j = (b0 + r) * kBlock + 8 * y + gq;
-              const float w = ms_ex2(v - lse);
-              sum[r][y] += j <= p && j >= lo ? w : 0.f;
+            for (int r = 0; r < RECS; ++r) {
+              mma_bf16_16816(acc[x][r], ka[r][2 * k], b[0], b[1]);
+              mma_bf16_16816(acc[x][r], ka[r][2 * k + 1], b[2], b[3]);
             }
+          }
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const int row = (n + x) * 8 + 2 * tq;
+          const float2 lse = *reinterpret_cast<const float2*>(&s_lse[s][row]);
+          const int2 p = *reinterpret_cast<const int2*>(&s_p[s][row]);
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int r = 0; r < RECS; ++r)
+#pragma unroll
+              for (int y = 0; y < 2; ++y) {
+                float w;
+                if (a.cap > 0.f) {
+                  const float v = fmaf(-2.f * cap2, __fdividef(1.f, ms_ex2(fminf(acc[x][r][2 * y + e] * fk[r] * cap_c, 80.f)) + 1.f), cap2);
+                  w = ms_ex2(v - (e ? lse.y : lse.x));
+                } else {
+                  w = ms_ex2(fmaf(acc[x][r][2 * y + e], fk[r], e ? -lse.y : -lse.x));
+                }
+                if (!whole) {
+                  const int j = (b0 + r) * kBlock + 8 * y + gq, pe = e ? p.y : p.x;
+                  w = j <= pe && (a.window <= 0 || j > pe - a.window) ? w : 0.f;
+                }
+                sum[r][y] += w;
+              }
         }
       }
       __syncthreads();
@@ -162,14 +180,22 @@ __global__ void __launch_bounds__(kMassWarps * 32) kv8_mass_kernel(const bf16* _
   }
 }
 
-template <int D>
+template <int D, int RECS>
 static int launch_mass(const bf16* q, const AttnArgs& a, int runs, cudaStream_t st) {
   constexpr size_t smem = (size_t)2 * kMassRows * (D + 8) * sizeof(bf16);
   static std::atomic<uint64_t> set{0};
-  if (const cudaError_t e = allow_smem(set, (const void*)kv8_mass_kernel<D>, smem); e != cudaSuccess) return (int)e;
-  const int keys = kMassWarps * mass_records(D) * kBlock;
+  if (const cudaError_t e = allow_smem(set, (const void*)kv8_mass_kernel<D, RECS>, smem); e != cudaSuccess) return (int)e;
+  const int keys = kMassWarps * RECS * kBlock;
   const long span = std::min((long)a.max_kv_len, a.mass_ld);
-  return (int)launch(kv8_mass_kernel<D>, dim3((unsigned)((span + keys - 1) / keys), a.pool.G, std::max(1, std::min(runs, 16))), dim3(kMassWarps * 32), smem, st, true, q, a);
+  return (int)launch(kv8_mass_kernel<D, RECS>, dim3((unsigned)((span + keys - 1) / keys), a.pool.G, runs), dim3(kMassWarps * 32), smem, st, true, q, a);
+}
+template <int D>
+static int launch_mass(const bf16* q, const AttnArgs& a, int runs, cudaStream_t st) {
+  runs = std::max(1, std::min(runs, 16));
+  // half as many keys to a warp where the others would leave the SMs with fewer than four CTAs
+  if constexpr (D <= 128)
+    if (std::min((long)a.max_kv_len, a.mass_ld) / (kMassWarps * 2 * kBlock) * a.pool.G * runs >= 4L * sm_count()) return launch_mass<D, 2>(q, a, runs, st);
+  return launch_mass<D, 1>(q, a, runs, st);
 }
 bool mass_takes(const bf16* q, int dim, int vdim) {
   return dim == vdim && (dim == 32 || dim == 64 || dim == 96 || dim == 128 || dim == 192 || dim == 256) && (reinterpret_cast<uintptr_t>(q) & 15) == 0;

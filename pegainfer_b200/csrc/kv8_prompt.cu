@@ -216,13 +216,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* _
     while (x.seg < segs && last_block(x.seg) < 0) ++x.seg;
     if (x.seg < segs) x.j = first_block(x.seg);
   };
-  auto begin = [&] {
-    Step x{0, 0, 0};
-    settle(x);
-    return x;
-  };
-  auto next = [&](Step& x) {
-    ++x.n;
+  auto pass = [&](Step& x) {
     if (x.j < last_block(x.seg)) {
       ++x.j;
     } else {
@@ -230,46 +224,72 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* _
       settle(x);
     }
   };
+  // this CTA's share of them (the grid's z axis), counted from its own first
+  int share = 0;
+  Step origin{0, 0, 0};
+  {
+    int all = 0;
+    for (int k = 0; k < segs; ++k)
+      if (last_block(k) >= 0) all += last_block(k) - first_block(k) + 1;
+    const int each = (all + (int)gridDim.z - 1) / (int)gridDim.z, skip = min(each * (int)blockIdx.z, all);
+    share = min(each, all - skip);
+    settle(origin);
+    for (int k = 0; k < skip;) {  // run by run
+      const int here = last_block(origin.seg) - origin.j + 1, go = min(here, skip - k);
+      k += go;
+      if (go < here) {
+        origin.j += go;
+      } else {
+        ++origin.seg;
+        settle(origin);
+      }
+    }
+    if (share == 0) origin.seg = segs;
+  }
+  auto begin = [&] { return origin; };
+  auto next = [&](Step& x) {
+    if (++x.n == share) x.seg = segs;
+    else pass(x);
+  };
 
   if (warp >= kPrMma) {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPrRegsMma));
   if (warp == kPrLoad) {
     // =========================== copies ===========================
-    int n = 0;
     bool go = true;  // false behind a run-out: a barrier must not be armed twice in one phase
-    for (int seg = 0; seg < segs && go; ++seg) {
-      const int j1 = last_block(seg);
-      if (j1 < 0) continue;
-      // the run's last slot that anybody here has: records behind it may not exist
-      int top = -1;
-      for (int i = lane; i < n_tok; i += 32)
-        if (s_seg[i] == seg) top = max(top, s_slot[i]);
-      top = __reduce_max_sync(0xffffffffu, top) / kBlock;
-      const int off = seg_off[seg], rpp = a.pool.page_size / kBlock;
-      auto source = [&](int j) {  // lane i: the block's i-th record, the last one again behind the end
-        const int b = min(j * kPrRecords + min(lane, kPrRecords - 1), top);
-        return a.pool.data + (size_t)a.pool.pages[off + b / rpp] * a.pool.page_stride + (size_t)(g * rpp + b % rpp) * (2 * REC_K + 16);
-      };
-      const uint8_t* src = source(first_block(seg));
-      for (int j = first_block(seg); j <= j1 && go; ++j, ++n) {
-        const int s = n % kPrStages;
-        const uint32_t ph = (uint32_t)((n / kPrStages) & 1) ^ 1u;
-        const uint8_t* now = src;
-        if (j < j1) src = source(j + 1);
-        go = mbar_wait_bounded(k_empty + s, ph, dead, tries);
-        if (!go) break;
-        if (lane == 0) mbar_expect_tx(k_full + s, KB);
-        __syncwarp();
-        if (lane < kPrRecords) pr_copy(smem_u32(Ks + s * KB) + lane * REC_K, now, REC_K, k_full + s);
-        const int sv = n % kPrStagesV;
-        go = mbar_wait_bounded(v_empty + sv, (uint32_t)((n / kPrStagesV) & 1) ^ 1u, dead, tries);
-        if (!go) break;
-        if (lane == 0) mbar_expect_tx(v_full + sv, KB + kPrRecords * 16);
-        __syncwarp();
-        if (lane < kPrRecords) {
-          pr_copy(smem_u32(Vs + sv * KB) + lane * REC_K, now + REC_K, REC_K, v_full + sv);
-          pr_copy(smem_u32(Ts + (sv * kPrRecords + lane) * 16), now + 2 * REC_K, 16, v_full + sv);
-        }
+    const int rpp = a.pool.page_size / kBlock;
+    int seg = -1, top = 0, off = 0;
+    auto source = [&](const Step& x) {  // lane i: the block's i-th record, the run's last one again behind the end
+      if (x.seg != seg) {
+        seg = x.seg;
+        top = -1;  // the last slot that anybody here has: records behind it may not exist
+        for (int i = lane; i < n_tok; i += 32)
+          if (s_seg[i] == seg) top = max(top, s_slot[i]);
+        top = __reduce_max_sync(0xffffffffu, top) / kBlock;
+        off = seg_off[seg];
+      }
+      const int b = min(x.j * kPrRecords + min(lane, kPrRecords - 1), top);
+      return a.pool.data + (size_t)a.pool.pages[off + b / rpp] * a.pool.page_stride + (size_t)(g * rpp + b % rpp) * (2 * REC_K + 16);
+    };
+    Step x = begin();
+    const uint8_t* src = x.seg < segs ? source(x) : nullptr;
+    while (x.seg < segs && go) {
+      const int n = x.n, s = n % kPrStages, sv = n % kPrStagesV;
+      const uint8_t* now = src;
+      next(x);
+      if (x.seg < segs) src = source(x);  // its page is looked up under this block's waits
+      go = mbar_wait_bounded(k_empty + s, (uint32_t)((n / kPrStages) & 1) ^ 1u, dead, tries);
+      if (!go) break;
+      if (lane == 0) mbar_expect_tx(k_full + s, KB);
+      __syncwarp();
+      if (lane < kPrRecords) pr_copy(smem_u32(Ks + s * KB) + lane * REC_K, now, REC_K, k_full + s);
+      go = mbar_wait_bounded(v_empty + sv, (uint32_t)((n / kPrStagesV) & 1) ^ 1u, dead, tries);
+      if (!go) break;
+      if (lane == 0) mbar_expect_tx(v_full + sv, KB + kPrRecords * 16);
+      __syncwarp();
+      if (lane < kPrRecords) {
+        pr_copy(smem_u32(Vs + sv * KB) + lane * REC_K, now + REC_K, REC_K, v_full + sv);
+        pr_copy(smem_u32(Ts + (sv * kPrRecords + lane) * 16), now + 2 * REC_K, 16, v_full + sv);
       }
     }
     if (!go) wait_for_copies();
@@ -429,7 +449,12 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* _
         if (!on) continue;
 #pragma unroll
         for (int x = 0; x < 32; ++x) t[x] = __float_as_uint(__uint_as_float(t[x]) * factor);
-        if (f.out_by8) {
+        if (gridDim.z > 1) {
+          float* part = a.part_o + (((size_t)blockIdx.z * a.T + t0 + ti) * a.H + g * R + r - k * R) * D + c;
+#pragma unroll
+          for (int x = 0; x < 32; x += 4)
+            *reinterpret_cast<uint4*>(part + x) = make_uint4(t[x], t[x + 1], t[x + 2], t[x + 3]);
+        } else if (f.out_by8) {
 #pragma unroll
           for (int x = 0; x < 32; x += 8)
             *reinterpret_cast<uint4*>(dst + c + x) = make_uint4(pack_bf16(__uint_as_float(t[x]), __uint_as_float(t[x + 1])), pack_bf16(__uint_as_float(t[x + 2]), __uint_as_float(t[x + 3])),
@@ -579,9 +604,15 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* _
       ++mine;
     }
     const float top = l != l ? INFINITY : m;  // a NaN among the scores
-    const RowEnd end = row_end(top, l, sink ? bf2f(sink[h]) : 0.f, sink != nullptr);
-    end_s[i * kPrRows + r] = l != l ? NAN : end.factor * pow2(max(E, kLowExp) - kPrTop);
-    if (on && a.lse) a.lse[(size_t)(t0 + ti) * a.H + h] = end.lse;
+    const float up = pow2(max(E, kLowExp) - kPrTop);
+    if (gridDim.z > 1) {  // a share's state: kv8_merge_kernel
+      end_s[i * kPrRows + r] = up;
+      if (on) a.part_ml[((size_t)blockIdx.z * a.T + t0 + ti) * a.H + h] = make_float2(top, l);
+    } else {
+      const RowEnd end = row_end(top, l, sink ? bf2f(sink[h]) : 0.f, sink != nullptr);
+      end_s[i * kPrRows + r] = l != l ? NAN : end.factor * up;
+      if (on && a.lse) a.lse[(size_t)(t0 + ti) * a.H + h] = end.lse;
+    }
     __syncwarp();
     if (lane == 0) mbar_arrive(d_ready + i);
   }
@@ -603,25 +634,34 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* _
 }
 
 template <int D>
-static int launch_prompt(const bf16* q, const bf16* sink, bf16* out, const PromptArgs& f, cudaStream_t st) {
+static int launch_prompt(const bf16* q, const bf16* sink, bf16* out, const PromptArgs& f, int shares, cudaStream_t st) {
   constexpr size_t smem = 128 + (size_t)4 * kPrRows * D + (size_t)(kPrStages + 3 * kPrStagesV) * kPrKeys * D + kPrStagesV * kPrRecords * 20 + 6 * kPrRows * sizeof(float) + 40 * 8;
   static std::atomic<uint64_t> set{0};
   if (const cudaError_t e = allow_smem(set, (const void*)kv8_prompt_kernel<D>, smem); e != cudaSuccess) return (int)e;
-  return (int)launch(kv8_prompt_kernel<D>, dim3(f.a.pool.G, (f.a.T + 2 * f.per - 1) / (2 * f.per)), dim3(kPrThreads), smem, st, true, q, sink, out, f);
+  return (int)launch(kv8_prompt_kernel<D>, dim3(f.a.pool.G, (f.a.T + 2 * f.per - 1) / (2 * f.per), shares), dim3(kPrThreads), smem, st, true, q, sink, out, f);
 }
 
 bool prompt_takes(int T, int H, int G, int dim, int vdim) {
   const int R = H / G, tokens = R <= kPrRows ? 2 * (kPrRows / R) : 0;  // of a CTA
   return dim == vdim && (dim == 64 || dim == 96 || dim == 128) && tokens > 0 && (T + tokens - 1) / tokens <= 65535;
 }
-int prompt_attention(const bf16* q, const bf16* sink, bf16* out, const AttnArgs& a, cudaStream_t st) {
+// Shares of the keys where the tiles leave SMs idle: as many CTAs as SMs, and 16 blocks of keys to a share at least (of the longest context, which is all that is known).
+// A share's start and end take 6 us, a block 1.5; the merge 5.
+int prompt_shares(int T, int H, int G, int max_kv_len, int window) {
+  const int per = kPrRows / (H / G), ctas = (T + 2 * per - 1) / (2 * per) * G;
+  const int span = window > 0 ? std::min(max_kv_len, window + 2 * per) : max_kv_len;
+  return std::max(1, std::min(sm_count() / std::max(ctas, 1), span / (16 * kPrKeys)));
+}
+int prompt_attention(const bf16* q, const bf16* sink, bf16* out, const AttnArgs& a, int shares, cudaStream_t st) {
   PromptArgs f{};
   f.a = a;
   f.per = kPrRows / (a.H / a.pool.G);
   f.q_by8 = (reinterpret_cast<uintptr_t>(q) & 15) == 0;
   f.out_by8 = (reinterpret_cast<uintptr_t>(out) & 15) == 0 && a.out_ld % 8 == 0;
   f.err = wait_err_word();
-  return a.pool.dim == 64 ? launch_prompt<64>(q, sink, out, f, st) : a.pool.dim == 96 ? launch_prompt<96>(q, sink, out, f, st) : launch_prompt<128>(q, sink, out, f, st);
+  return a.pool.dim == 64   ? launch_prompt<64>(q, sink, out, f, shares, st)
+         : a.pool.dim == 96 ? launch_prompt<96>(q, sink, out, f, shares, st)
+                            : launch_prompt<128>(q, sink, out, f, shares, st);
 }
 
 }  // namespace kv8

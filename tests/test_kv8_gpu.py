@@ -427,6 +427,14 @@ def test_many_requests(lib, steps):
     check_attention(lib, steps, 4, 1, 64, mass=True)
 
 
+@pytest.mark.parametrize("H,G,D", [(8, 2, 64), (16, 4, 128), (6, 2, 96), (24, 1, 128)])
+@pytest.mark.parametrize("steps", [[(70, 5000)], [(64, 2047), (1, 3000), (90, 4100)], [(333, 2500), (100, 0)], [(5, 3000)] * 20], ids=["one", "mixed", "two", "twenty"])
+@pytest.mark.parametrize("opts", [dict(), dict(window=1500, softcap=20.0, sink=True), dict(sink=True, longest=9000)], ids=["plain", "window", "sink"])
+def test_portions_behind_long_contexts(lib, H, G, D, steps, opts):
+    """the keys of a few tiles are dealt out to several CTAs"""
+    check_attention(lib, steps, H, G, D, mass=True, max_q=0, **opts)
+
+
 @pytest.mark.parametrize("big", [1e30, 1e-30])
 def test_values_of_very_different_sizes(lib, big):
     """records whose exponents lie far apart, the large ones first, last and in between: the small ones' part of the result is lost only where it is small"""
