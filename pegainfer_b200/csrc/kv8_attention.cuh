@@ -29,6 +29,9 @@ __device__ __forceinline__ float shaped(float dot, float c, float cap) {
   return cap > 0.f ? cap * kLog2e * tanhf(dot * c / (cap * kLog2e)) : dot * c;
 }
 
+// at most 80, and NaN where x is
+__device__ __forceinline__ float at_most80(float x) { return x > 80.f ? 80.f : x; }
+
 // Largest score M (log2), sum of 2^(s - M): what the row's accumulated values are multiplied with, and its lse.  A row that saw nothing gives zeros.
 struct RowEnd {
   float factor, lse;

@@ -409,7 +409,7 @@ __global__ void __launch_bounds__(few_warps<D>() * 32, 1) kv8_few_kernel(const b
 #pragma unroll
           for (int y = 0; y < 2; ++y) {
             float v = s[r][w][2 * y + e] * fk;
-            if (a.cap > 0.f) v = fmaf(-2.f * cap2, __fdividef(1.f, ex2(fminf(v * cap_c, 80.f)) + 1.f), cap2);  // cap tanh(x) = cap - 2 cap / (e^(2 x) + 1)
+            if (a.cap > 0.f) v = fmaf(-2.f * cap2, __fdividef(1.f, ex2(at_most80(v * cap_c)) + 1.f), cap2);  // cap tanh(x) = cap - 2 cap / (e^(2 x) + 1)
             if (!inside) {
               const int j = j0 + 16 * r + tok[y];
               v = j >= lo[i2] && j <= p[i2] && r < take ? v : -INFINITY;

@@ -149,7 +149,7 @@ __global__ void __launch_bounds__(kMassWarps * 32) kv8_mass_kernel(const bf16* _
               for (int y = 0; y < 2; ++y) {
                 float w;
                 if (a.cap > 0.f) {
-                  const float v = fmaf(-2.f * cap2, __fdividef(1.f, ms_ex2(fminf(acc[x][r][2 * y + e] * fk[r] * cap_c, 80.f)) + 1.f), cap2);
+                  const float v = fmaf(-2.f * cap2, __fdividef(1.f, ms_ex2(at_most80(acc[x][r][2 * y + e] * fk[r] * cap_c)) + 1.f), cap2);
                   w = ms_ex2(v - (e ? lse.y : lse.x));
                 } else {
                   w = ms_ex2(fmaf(acc[x][r][2 * y + e], fk[r], e ? -lse.y : -lse.x));

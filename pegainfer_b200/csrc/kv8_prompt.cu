@@ -78,6 +78,12 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, ui
 __device__ __forceinline__ void pr_copy(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
 }
+// the larger, NaN where one is
+__device__ __forceinline__ float pr_max(float x, float y) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
+  return r;
+}
 __device__ __forceinline__ uint32_t pr_pack(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
@@ -94,6 +100,33 @@ __device__ __forceinline__ void pr_add2(float& a0, float& a1, float x0, float x1
   asm("mov.b64 %0, {%1, %2};" : "=l"(w) : "f"(x0), "f"(x1));
   asm("add.rn.f32x2 %0, %0, %1;" : "+l"(v) : "l"(w));
   asm("mov.b64 {%0, %1}, %2;" : "=f"(a0), "=f"(a1) : "l"(v));
+}
+// {y0, y1} = {y0 x0 + c, y1 x1 + c}
+__device__ __forceinline__ void pr_mad2(float& y0, float& y1, float x0, float x1, float c) {
+  unsigned long long y, x, k;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "f"(y0), "f"(y1));
+  asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(x0), "f"(x1));
+  asm("mov.b64 %0, {%1, %1};" : "=l"(k) : "f"(c));
+  asm("fma.rn.f32x2 %0, %0, %1, %2;" : "+l"(y) : "l"(x), "l"(k));
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(y0), "=f"(y1) : "l"(y));
+}
+// {2^x0, 2^x1} without the special-function unit: 2^(x - n) by a polynomial of degree 4 for n the nearest whole number (fitted over [-1/2, 1/2] by reweighted least squares
+// to a relative error of 2.6e-6), n into the exponent.  x >= -125 (what lies below is 2^-125), no NaN.
+__device__ __forceinline__ void pr_poly2(float& x0, float& x1) {
+  x0 = fmaxf(x0, -125.f);
+  x1 = fmaxf(x1, -125.f);
+  float t0 = x0, t1 = x1;
+  pr_add2(t0, t1, 12582912.f, 12582912.f);  // 1.5 * 2^23: the whole number in the low bits
+  float n0 = t0, n1 = t1;
+  pr_add2(n0, n1, -12582912.f, -12582912.f);
+  pr_add2(x0, x1, -n0, -n1);
+  float y0 = 0.009570102f, y1 = 0.009570102f;
+  pr_mad2(y0, y1, x0, x1, 0.05591786f);
+  pr_mad2(y0, y1, x0, x1, 0.24024744f);
+  pr_mad2(y0, y1, x0, x1, 0.6931218f);
+  pr_mad2(y0, y1, x0, x1, 0.99999928f);
+  x0 = __uint_as_float(__float_as_uint(y0) + (__float_as_uint(t0) << 23));
+  x1 = __uint_as_float(__float_as_uint(y1) + (__float_as_uint(t1) << 23));
 }
 __device__ __forceinline__ uint32_t rest4(float a, float b, float c, float d) {
   uint16_t x, y;
@@ -112,7 +145,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* _
   uint8_t* Vs = Ks + kPrStages * KB;                     // [stage] V as it comes
   uint8_t* Hs = Vs + kPrStagesV * KB;                    // [stage] V as f16: [8 keys][entry][8 keys' f16]
   uint8_t* Ts = Hs + kPrStagesV * 2 * KB;                // [stage][record] tails as they come
-  uint32_t* Es = reinterpret_cast<uint32_t*>(Ts + kPrStagesV * kPrRecords * 16);  // [stage][record] tails of the f16's
+  int2* Es = reinterpret_cast<int2*>(Ts + kPrStagesV * kPrRecords * 16);  // [stage][record] of the f16's: 2^(K's exponent), V's exponent
   float* alpha_s = reinterpret_cast<float*>(Es + kPrStagesV * kPrRecords);  // [tile][buffer][row]
   float* end_s = alpha_s + 4 * kPrRows;                  // [tile][row]
   uint64_t* bars = reinterpret_cast<uint64_t*>(end_s + 2 * kPrRows);
@@ -376,7 +409,10 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* _
         *reinterpret_cast<uint4*>(to + (2 * b) * REC_K + d * 16) = make_uint4(h[0], h[1], h[2], h[3]);
         *reinterpret_cast<uint4*>(to + (2 * b + 1) * REC_K + d * 16) = make_uint4(h[4], h[5], h[6], h[7]);
       }
-      if (r < kPrRecords) Es[sv * kPrRecords + r] = *reinterpret_cast<const uint32_t*>(Ts + (sv * kPrRecords + r) * 16);
+      if (r < kPrRecords) {
+        const uint32_t tail = *reinterpret_cast<const uint32_t*>(Ts + (sv * kPrRecords + r) * 16);
+        Es[sv * kPrRecords + r] = make_int2(__float_as_int(pow2(tail_ek(tail))), tail_ev(tail));
+      }
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
@@ -523,24 +559,26 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* _
     const float cap2 = a.cap * kLog2e, cap_c = a.cap > 0.f ? 2.f * a.scale / a.cap * kLog2e : 0.f;
     float m = -INFINITY, l = 0.f;
     int E = kLowExp - 1, mine = 0;
-    for (Step x = begin(); x.seg < segs; next(x)) {
-      if (!needs(i, x.seg, x.j)) continue;
+    bool s_there = false, h_there = false;  // looked up under the block before
+    Step x = begin();
+    while (x.seg < segs && !needs(i, x.seg, x.j)) next(x);
+    while (x.seg < segs) {
       const int sv = x.n % kPrStagesV;
       const uint32_t t_s = t_tile + (uint32_t)((mine & 1) * kPrKeys);
       // S first: it says that the stage's phases before this block's are over (a tile that skipped blocks would take an older one for it)
-      mbar_wait_bounded(s_full + i * 2 + (mine & 1), (uint32_t)((mine >> 1) & 1), dead, tries);
+      if (!s_there) mbar_wait_bounded(s_full + i * 2 + (mine & 1), (uint32_t)((mine >> 1) & 1), dead, tries);
       tc_fence_after();
       uint32_t v[kPrKeys];
       tmem_ld32_nowait(t_s, v);
       tmem_ld32_nowait(t_s + 32, v + 32);
-      mbar_wait_bounded(h_full + sv, (uint32_t)((x.n / kPrStagesV) & 1), dead, tries);
+      if (!h_there) mbar_wait_bounded(h_full + sv, (uint32_t)((x.n / kPrStagesV) & 1), dead, tries);
       int ev[kPrRecords], e_new = E;
       float fk[kPrRecords];
 #pragma unroll
       for (int b = 0; b < kPrRecords; ++b) {
-        const uint32_t tail = Es[sv * kPrRecords + b];
-        ev[b] = tail_ev(tail);
-        const float y = pow2(tail_ek(tail)) * row_c;
+        const int2 e = Es[sv * kPrRecords + b];
+        ev[b] = e.y;
+        const float y = __int_as_float(e.x) * row_c;
         fk[b] = y < 1e-37f ? 1e-37f : y;  // never zero: -inf times it stays -inf (and a NaN stays one)
         e_new = max(e_new, ev[b]);
       }
@@ -551,7 +589,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* _
       if (a.cap > 0.f) {  // (the columns' factors are in the scores then)
 #pragma unroll
         for (int k = 0; k < kPrKeys; ++k)
-          v[k] = __float_as_uint(fmaf(-2.f * cap2, __fdividef(1.f, pr_ex2(fminf(__uint_as_float(v[k]) * fk[k / kBlock] * cap_c, 80.f)) + 1.f), cap2));
+          v[k] = __float_as_uint(fmaf(-2.f * cap2, __fdividef(1.f, pr_ex2(at_most80(__uint_as_float(v[k]) * fk[k / kBlock] * cap_c)) + 1.f), cap2));
       }
       if (masked) {
 #pragma unroll
@@ -561,13 +599,17 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* _
       float mx = m;
 #pragma unroll
       for (int b = 0; b < kPrRecords; ++b) {
-        float y = fmaxf(__uint_as_float(v[b * 16]), __uint_as_float(v[b * 16 + 1])), z = fmaxf(__uint_as_float(v[b * 16 + 2]), __uint_as_float(v[b * 16 + 3]));
+        float y = pr_max(__uint_as_float(v[b * 16]), __uint_as_float(v[b * 16 + 1])), z = pr_max(__uint_as_float(v[b * 16 + 2]), __uint_as_float(v[b * 16 + 3]));
 #pragma unroll
         for (int k = 4; k < 16; k += 4) {
-          y = fmaxf(fmaxf(y, __uint_as_float(v[b * 16 + k])), __uint_as_float(v[b * 16 + k + 1]));
-          z = fmaxf(fmaxf(z, __uint_as_float(v[b * 16 + k + 2])), __uint_as_float(v[b * 16 + k + 3]));
+          y = pr_max(pr_max(y, __uint_as_float(v[b * 16 + k])), __uint_as_float(v[b * 16 + k + 1]));
+          z = pr_max(pr_max(z, __uint_as_float(v[b * 16 + k + 2])), __uint_as_float(v[b * 16 + k + 3]));
         }
-        mx = fmaxf(mx, fmaxf(y, z) * factor(b));
+        mx = pr_max(mx, pr_max(y, z) * factor(b));
+      }
+      if (mx != mx) {  // a NaN among what the row sees: its sum says so at the end, whatever P holds
+        l = NAN;
+        mx = m;
       }
       const float m_new = mx > m + (float)kPrSlack ? mx : m;  // (m = -inf: mx)
       const float ref = m_new == -INFINITY ? 0.f : m_new, fl = pr_ex2(m - ref);
@@ -578,7 +620,15 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* _
       m = m_new;
       E = e_new;
       l *= fl;
-      // P of 16 columns -> eight columns
+      // this tile's next block: asked for now, answered under the exponentials
+      Step after = x;
+      do next(after);
+      while (after.seg < segs && !needs(i, after.seg, after.j));
+      if (after.seg < segs) {
+        s_there = mbar_test_wait(s_full + i * 2 + ((mine + 1) & 1), (uint32_t)(((mine + 1) >> 1) & 1));
+        h_there = after.n == x.n + 1 && mbar_test_wait(h_full + after.n % kPrStagesV, (uint32_t)((after.n / kPrStagesV) & 1));
+      }
+      // P of 16 columns -> eight columns; one pair of four without the special-function unit, which two tiles' exponentials alone keep busy for 1024 clocks a block
       uint32_t w[kPrKeys / 2];
 #pragma unroll
       for (int b = 0; b < kPrRecords; ++b) {
@@ -589,8 +639,12 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* _
         for (int k = 0; k < 8; ++k) {
           float s0 = __uint_as_float(v[b * 16 + 2 * k]), s1 = __uint_as_float(v[b * 16 + 2 * k + 1]);
           pr_fma2(s0, s1, fb, add);
-          s0 = pr_ex2(s0);
-          s1 = pr_ex2(s1);
+          if (k % 4 == 3) {
+            pr_poly2(s0, s1);
+          } else {
+            s0 = pr_ex2(s0);
+            s1 = pr_ex2(s1);
+          }
           pr_add2(d0, d1, s0, s1);
           w[b * 8 + k] = pr_pack(s0, s1);
         }
@@ -602,6 +656,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* _
       __syncwarp();
       if (lane == 0) mbar_arrive(po_ready + i * 2 + (mine & 1));
       ++mine;
+      x = after;
     }
     const float top = l != l ? INFINITY : m;  // a NaN among the scores
     const float up = pow2(max(E, kLowExp) - kPrTop);
@@ -635,7 +690,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* _
 
 template <int D>
 static int launch_prompt(const bf16* q, const bf16* sink, bf16* out, const PromptArgs& f, int shares, cudaStream_t st) {
-  constexpr size_t smem = 128 + (size_t)4 * kPrRows * D + (size_t)(kPrStages + 3 * kPrStagesV) * kPrKeys * D + kPrStagesV * kPrRecords * 20 + 6 * kPrRows * sizeof(float) + 40 * 8;
+  constexpr size_t smem = 128 + (size_t)4 * kPrRows * D + (size_t)(kPrStages + 3 * kPrStagesV) * kPrKeys * D + kPrStagesV * kPrRecords * 24 + 6 * kPrRows * sizeof(float) + 40 * 8;
   static std::atomic<uint64_t> set{0};
   if (const cudaError_t e = allow_smem(set, (const void*)kv8_prompt_kernel<D>, smem); e != cudaSuccess) return (int)e;
   return (int)launch(kv8_prompt_kernel<D>, dim3(f.a.pool.G, (f.a.T + 2 * f.per - 1) / (2 * f.per), shares), dim3(kPrThreads), smem, st, true, q, sink, out, f);

@@ -384,8 +384,8 @@ def test_a_row_that_sees_nothing_but_what_is_not_finite(lib, f32, T):
         rec = c.record(0, blk)
         rec[1, :16 * D] = 0x7f
     q = torch.randn(T, 4, D, device=DEV).to(F32 if f32 else BF16)
-    for window in (0, 1, 40):
-        out, lse = call_attention(lib, c, q, i32(range(n - T, n)), i32([0] * T), 0.125, longest=n, max_q=T, window=window)
+    for window, cap in ((0, 0.0), (1, 0.0), (40, 0.0), (0, 20.0), (1, 20.0)):
+        out, lse = call_attention(lib, c, q, i32(range(n - T, n)), i32([0] * T), 0.125, longest=n, max_q=T, window=window, softcap=cap)
         assert torch.isnan(out[:, 2:]).all() and torch.isnan(lse[:, 2:]).all() and torch.isfinite(out[:, :2]).all() and torch.isfinite(lse[:, :2]).all()
 
 
@@ -398,10 +398,29 @@ def test_a_query_that_is_not_finite(lib, bad, f32, T):
     c = filled([n], G, D, D, 16)
     q = torch.randn(T, 4, D, device=DEV).to(F32 if f32 else BF16)
     q[1, 1, 5] = bad
-    out, lse = call_attention(lib, c, q, i32(range(n - T, n)), i32([0] * T), 0.125, longest=n, max_q=T)
     hit = torch.zeros(T, 4, dtype=torch.bool, device=DEV)
     hit[1, 1] = True
-    assert torch.equal(torch.isnan(out).any(-1), hit) and torch.isfinite(out[~hit]).all() and torch.isnan(out[1, 1]).all()
+    for cap in (0.0, 20.0):
+        if cap and math.isinf(bad):
+            continue  # (a capped infinite score is the cap)
+        out, lse = call_attention(lib, c, q, i32(range(n - T, n)), i32([0] * T), 0.125, longest=n, max_q=T, softcap=cap)
+        assert torch.equal(torch.isnan(out).any(-1), hit) and torch.isfinite(out[~hit]).all() and torch.isnan(out[1, 1]).all()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_one_key_that_is_not_finite(lib, D):
+    """whichever column of a block it is in: the rows that see it are NaN, and no others"""
+    G, n = 1, 150
+    q = torch.randn(n, 2, D, device=DEV).to(BF16)
+    for bad in list(range(60, 80)) + [0, 127, 149]:
+        c = filled([n], G, D, D, 16)
+        rec = c.record(0, bad // 16)
+        at = bad % 16
+        for ch in range(D // 16):
+            rec[0, at // 8 * 8 * D + ch * 128 + at % 8 * 16:][:16] = 0x7f
+        out, lse = call_attention(lib, c, q, i32(range(n)), i32([0] * n), 0.125, longest=n, max_q=n)
+        hit = (torch.arange(n, device=DEV) >= bad)[:, None].expand(n, 2)
+        assert torch.equal(torch.isnan(out).all(-1), hit) and torch.equal(torch.isnan(out).any(-1), hit) and torch.equal(torch.isnan(lse), hit)
 
 
 @pytest.mark.parametrize("f32", [False, True])
