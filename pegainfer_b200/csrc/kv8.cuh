@@ -50,6 +50,17 @@ inline Pool make_pool(const void* cache, long page_stride, const int* page_off, 
   return Pool{static_cast<uint8_t*>(const_cast<void*>(cache)), page_stride, page_off, pages, page_size, G, dim, vdim};
 }
 
+// behind a kernel of the same call: its launch may always overlap that one's end
+template <typename... KArgs, typename... Args>
+static cudaError_t follow(void (*kernel)(KArgs...), dim3 grid, dim3 block, cudaStream_t st, Args... args) {
+  ThreadState& ts = tls();
+  const bool pdl = ts.pdl;
+  ts.pdl = true;
+  const cudaError_t e = launch(kernel, grid, block, 0, st, true, args...);
+  ts.pdl = pdl;
+  return e;
+}
+
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // -126 <= e <= 127
 
 // the least e with amax <= 448 * 2^e (448 = 1.75 * 2^8)

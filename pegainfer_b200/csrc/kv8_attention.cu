@@ -136,13 +136,18 @@ __global__ void __launch_bounds__(128) kv8_merge_kernel(const E* __restrict__ si
   float o[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) o[i] = 0.f;
-  for (int s = 0; s < shares; ++s) {
-    const float m = a.part_ml[s * rows + row].x;
-    if (m == -INFINITY) continue;
-    const float f = exp2f(m - M);
+  for (int s0 = 0; s0 < shares; s0 += 32) {
+    const float m = s0 + lane < shares ? a.part_ml[(s0 + lane) * rows + row].x : -INFINITY, w = m == -INFINITY ? 0.f : exp2f(m - M);
+#pragma unroll 4
+    for (int s = s0; s < min(shares, s0 + 32); ++s) {
+      const float f = __shfl_sync(0xffffffffu, w, s - s0);
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (lane + 32 * i < V) o[i] = fmaf(a.part_o[(s * rows + row) * V + lane + 32 * i], f, o[i]);
+      for (int i = 0; i < 8; ++i)
+        if (lane + 32 * i < V) {
+          const float x = a.part_o[(s * rows + row) * V + lane + 32 * i];
+          o[i] = f != 0.f ? fmaf(x, f, o[i]) : o[i];
+        }
+    }
   }
 #pragma unroll
   for (int i = 0; i < 8; ++i)
@@ -236,11 +241,11 @@ static Plan plan(int T, int H, int G, int dim, int vdim, const pk_kv8_options& o
 
 template <typename E>
 static int mass_rows(const E* q, const AttnArgs& a, cudaStream_t st) {
-  return (int)launch(kv8_mass_row_kernel<E>, dim3((a.max_kv_len + 63) / 64, a.pool.G), dim3(128), 0, st, true, q, a);
+  return (int)follow(kv8_mass_row_kernel<E>, dim3((a.max_kv_len + 63) / 64, a.pool.G), dim3(128), st, q, a);
 }
 template <typename E>
 static int merge(const E* sink, E* out, int shares, const AttnArgs& a, cudaStream_t st) {
-  return (int)launch(kv8_merge_kernel<E>, dim3((unsigned)(((size_t)a.T * a.H + 3) / 4)), dim3(128), 0, st, true, sink, out, shares, a);
+  return (int)follow(kv8_merge_kernel<E>, dim3((unsigned)(((size_t)a.T * a.H + 3) / 4)), dim3(128), st, sink, out, shares, a);
 }
 template <typename E>
 static int attention(const E* q, const E* sink, E* out, const AttnArgs& a, const Plan& p, cudaStream_t st) {
@@ -297,7 +302,7 @@ extern "C" int pk_kv8_attention(const void* q, const void* cache, const void* si
     int rc = kv8::prompt_attention((const bf16*)q, (const bf16*)sink, (bf16*)out, a, p.shares, st);
     if (rc == 0 && p.shares > 1) rc = kv8::merge((const bf16*)sink, (bf16*)out, p.shares, a, st);
     if (rc != 0 || !a.mass) return rc;
-    return kv8::mass_takes((const bf16*)q, dim, vdim) ? kv8::mass_rows_mma((const bf16*)q, a, options->max_q_len, st) : kv8::mass_rows((const bf16*)q, a, st);
+    return kv8::mass_takes((const bf16*)q, tokens, dim, vdim) ? kv8::mass_rows_mma((const bf16*)q, a, options->max_q_len, st) : kv8::mass_rows((const bf16*)q, a, st);
   }
   if (f32) return kv8::attention((const float*)q, (const float*)sink, (float*)out, a, p, st);
   return kv8::attention((const bf16*)q, (const bf16*)sink, (bf16*)out, a, p, st);

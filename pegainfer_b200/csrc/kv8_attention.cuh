@@ -68,7 +68,7 @@ bool prompt_takes(int T, int H, int G, int dim, int vdim);
 int prompt_shares(int T, int H, int G, int max_kv_len, int window);
 int prompt_attention(const bf16* q, const bf16* sink, bf16* out, const AttnArgs& a, int shares, cudaStream_t st);
 // kv8_mass.cu: the weights' sums of such a call
-bool mass_takes(const bf16* q, int dim, int vdim);
+bool mass_takes(const bf16* q, int T, int dim, int vdim);
 int mass_rows_mma(const bf16* q, const AttnArgs& a, int max_q_len, cudaStream_t st);
 
 }  // namespace kv8

@@ -668,17 +668,6 @@ __global__ void __launch_bounds__(256) kv8_few_mass_kernel(FewArgs f) {
   if (any && j < a.mass_ld) a.mass[((size_t)req * a.pool.G + g) * a.mass_ld + j] += sum;
 }
 
-// behind a kernel of the same call: its launch may always overlap that one's end
-template <typename... KArgs, typename... Args>
-static cudaError_t follow(void (*kernel)(KArgs...), dim3 grid, dim3 block, cudaStream_t st, Args... args) {
-  ThreadState& ts = tls();
-  const bool pdl = ts.pdl;
-  ts.pdl = true;
-  const cudaError_t e = launch(kernel, grid, block, 0, st, true, args...);
-  ts.pdl = pdl;
-  return e;
-}
-
 template <int D, bool SCORES, bool WIDE>
 static int launch_few(const bf16* q, const bf16* sink, bf16* out, const FewArgs& f, int ctas, cudaStream_t st) {
   constexpr size_t smem = (size_t)few_warps<D>() * (few_stages<D>() * 2 * (kBlock * 2 * D + 16) + 8 * (D + 4) * sizeof(float));

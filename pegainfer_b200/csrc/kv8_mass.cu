@@ -12,7 +12,7 @@
 namespace pk {
 namespace kv8 {
 
-constexpr int kMassWarps = 4, kMassRows = 64;
+constexpr int kMassWarps = 4, kMassRows = 64, kMassTokens = 65536;  // of a call, at most
 
 __device__ __forceinline__ float ms_ex2(float x) {
   float y;
@@ -31,6 +31,8 @@ __global__ void __launch_bounds__(kMassWarps * 32) kv8_mass_kernel(const bf16* _
   extern __shared__ __align__(16) bf16 ms_q[];  // [2][rows][LD]
   __shared__ __align__(8) float s_lse[2][kMassRows];  // log2; +inf: no such row
   __shared__ __align__(8) int s_p[2][kMassRows];
+  __shared__ uint32_t ms_starts[kMassTokens / 32];
+  __shared__ int4 s_run[kMassWarps];
   __shared__ int s_half[2][2];  // whether 32 rows see every key of the CTA
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gq = lane >> 2, tq = lane & 3, g = blockIdx.y, R = a.H / a.pool.G, V = a.pool.vdim;
   const int b0 = (blockIdx.x * kMassWarps + warp) * RECS;  // the warp's first record
@@ -38,22 +40,48 @@ __global__ void __launch_bounds__(kMassWarps * 32) kv8_mass_kernel(const bf16* _
   const float c = a.scale * kLog2e, cap2 = a.cap * kLog2e, cap_c = a.cap > 0.f ? 2.f * a.scale / a.cap * kLog2e : 0.f;
   pdl_wait();
   pdl_launch_dependents();
+  // where runs begin
+  const int words = (a.T + 31) / 32;
+#pragma unroll 4
+  for (int i = warp; i < words; i += kMassWarps) {
+    const int t = i * 32 + lane;
+    const bool begins = t < a.T && (t == 0 || a.req[t] != a.req[t - 1]);
+    const uint32_t all = __ballot_sync(0xffffffffu, begins);
+    if (lane == 0) ms_starts[i] = all;
+  }
+  __syncthreads();
+  auto next_start = [&](int t) {  // the first run behind token t
+    int i = (t + 1) >> 5;
+    if (i >= words) return a.T;
+    uint32_t m = ms_starts[i] & (0xffffffffu << ((t + 1) & 31));
+    while (m == 0 && ++i < words) m = ms_starts[i];
+    return m ? i * 32 + __ffs(m) - 1 : a.T;
+  };
   int nth = 0;
   for (int t0 = 0, t1 = 0; t0 < a.T; t0 = t1, ++nth) {
-    // the run's end, its largest and smallest slot
+    t1 = next_start(t0);
+    if (nth % (int)gridDim.z != (int)blockIdx.z) continue;
     const int req = a.req[t0];
-    int last = -1, lowest = INT_MAX;
-    t1 = t0;
-    for (bool more = true; more;) {
-      const bool in = t1 + lane < a.T && a.req[min(t1 + lane, a.T - 1)] == req;
-      const uint32_t same = __ballot_sync(0xffffffffu, in);
-      const int n = same == 0xffffffffu ? 32 : __ffs(~same) - 1, slot = lane < n ? a.slots[t1 + lane] : -1;
-      last = max(last, __reduce_max_sync(0xffffffffu, slot));
-      lowest = min(lowest, __reduce_min_sync(0xffffffffu, slot < 0 ? INT_MAX : slot));
-      t1 += n;
-      more = n == 32;
+    // the run's largest and smallest slot, and where they are: slots ascend by one at least
+    int last = -1, lowest = INT_MAX, at_last = -1, at_lowest = INT_MAX;
+    for (int t = t0 + (int)threadIdx.x; t < t1; t += kMassWarps * 32) {
+      const int p = a.slots[t];
+      if (p >= 0 && p >= last) last = p, at_last = t;
+      if (p >= 0 && p < lowest) lowest = p, at_lowest = t;
     }
-    if (nth % (int)gridDim.z != (int)blockIdx.z || key0 > last || (a.window > 0 && key1 <= lowest - a.window)) continue;  // (for all threads alike)
+    {
+      const int wl = __reduce_max_sync(0xffffffffu, last), ws = __reduce_min_sync(0xffffffffu, lowest);
+      const int al = __reduce_max_sync(0xffffffffu, last == wl ? at_last : -1), as = __reduce_min_sync(0xffffffffu, lowest == ws ? at_lowest : INT_MAX);
+      __syncthreads();  // (the words of a run before)
+      if (lane == 0) s_run[warp] = make_int4(wl, al, ws, as);
+      __syncthreads();
+      const int4 x = s_run[lane % kMassWarps];
+      last = __reduce_max_sync(0xffffffffu, x.x);
+      at_last = __reduce_max_sync(0xffffffffu, x.x == last ? x.y : -1);
+      lowest = __reduce_min_sync(0xffffffffu, x.z);
+      at_lowest = __reduce_min_sync(0xffffffffu, x.z == lowest ? x.w : INT_MAX);
+    }
+    if (key0 > last || (a.window > 0 && key1 <= lowest - a.window)) continue;  // (for all threads alike)
 
     // the warp's keys: a product's 16 tokens are a record's, its inner index the entries in order
     uint32_t ka[RECS][D / 16][4];
@@ -94,28 +122,13 @@ __global__ void __launch_bounds__(kMassWarps * 32) kv8_mass_kernel(const bf16* _
       }
       cp_async_commit();
     };
-    // tiles whose rows see none of the CTA's keys pass (every thread looks at the same slots)
-    auto seen = [&](int tile) {
-      const int ta = t0 + tile * kMassRows / R, tb = t0 + min((tile + 1) * kMassRows, rows) / R - ((min((tile + 1) * kMassRows, rows) % R) == 0 ? 1 : 0);
-      int top = -1, low = INT_MAX;
-      for (int t = ta + lane; t <= tb; t += 32) {
-        const int p = a.slots[t];
-        top = max(top, p);
-        if (p >= 0) low = min(low, p);
-      }
-      top = __reduce_max_sync(0xffffffffu, top);
-      low = __reduce_min_sync(0xffffffffu, low);
-      return top >= key0 && (a.window <= 0 || low - a.window < key1);
-    };
-    auto next = [&](int tile) {
-      while (tile < tiles && !seen(tile)) ++tile;
-      return tile;
-    };
-    int tile = next(0), s = 0;
-    if (tile < tiles) load(tile, 0);
-    while (tile < tiles) {
-      const int after = next(tile + 1);
-      if (after < tiles) load(after, s ^ 1);
+    // rows that see none of the CTA's keys: before token `from`, and from token `to` on where there is a window
+    const int from = max(t0, at_last - (last - key0)), to = a.window > 0 ? (int)min((long)t1, (long)at_lowest + (key1 + (long)a.window - lowest)) : t1;
+    const int tile0 = (int)((long)(from - t0) * R / kMassRows), tile1 = min(tiles, (int)(((long)(to - t0) * R + kMassRows - 1) / kMassRows));
+    int s = 0;
+    if (tile0 < tile1) load(tile0, 0);
+    for (int tile = tile0; tile < tile1; ++tile) {
+      if (tile + 1 < tile1) load(tile + 1, s ^ 1);
       else cp_async_commit();
       asm volatile("cp.async.wait_group 1;" ::: "memory");
       __syncthreads();
@@ -163,7 +176,6 @@ __global__ void __launch_bounds__(kMassWarps * 32) kv8_mass_kernel(const bf16* _
         }
       }
       __syncthreads();
-      tile = after;
       s ^= 1;
     }
 #pragma unroll
@@ -185,9 +197,14 @@ static int launch_mass(const bf16* q, const AttnArgs& a, int runs, cudaStream_t 
   constexpr size_t smem = (size_t)2 * kMassRows * (D + 8) * sizeof(bf16);
   static std::atomic<uint64_t> set{0};
   if (const cudaError_t e = allow_smem(set, (const void*)kv8_mass_kernel<D, RECS>, smem); e != cudaSuccess) return (int)e;
-  const int keys = kMassWarps * RECS * kBlock;
+  constexpr int keys = kMassWarps * RECS * kBlock;
   const long span = std::min((long)a.max_kv_len, a.mass_ld);
-  return (int)launch(kv8_mass_kernel<D, RECS>, dim3((unsigned)((span + keys - 1) / keys), a.pool.G, runs), dim3(kMassWarps * 32), smem, st, true, q, a);
+  ThreadState& ts = tls();
+  const bool pdl = ts.pdl;
+  ts.pdl = true;  // behind a kernel of the same call
+  const cudaError_t e = launch(kv8_mass_kernel<D, RECS>, dim3((unsigned)((span + keys - 1) / keys), a.pool.G, runs), dim3(kMassWarps * 32), smem, st, true, q, a);
+  ts.pdl = pdl;
+  return (int)e;
 }
 template <int D>
 static int launch_mass(const bf16* q, const AttnArgs& a, int runs, cudaStream_t st) {
@@ -197,8 +214,8 @@ static int launch_mass(const bf16* q, const AttnArgs& a, int runs, cudaStream_t 
     if (std::min((long)a.max_kv_len, a.mass_ld) / (kMassWarps * 2 * kBlock) * a.pool.G * runs >= 4L * sm_count()) return launch_mass<D, 2>(q, a, runs, st);
   return launch_mass<D, 1>(q, a, runs, st);
 }
-bool mass_takes(const bf16* q, int dim, int vdim) {
-  return dim == vdim && (dim == 32 || dim == 64 || dim == 96 || dim == 128 || dim == 192 || dim == 256) && (reinterpret_cast<uintptr_t>(q) & 15) == 0;
+bool mass_takes(const bf16* q, int T, int dim, int vdim) {
+  return T <= kMassTokens && dim == vdim && (dim == 32 || dim == 64 || dim == 96 || dim == 128 || dim == 192 || dim == 256) && (reinterpret_cast<uintptr_t>(q) & 15) == 0;
 }
 int mass_rows_mma(const bf16* q, const AttnArgs& a, int max_q_len, cudaStream_t st) {
   const int runs = max_q_len > 0 ? (a.T + max_q_len - 1) / max_q_len : 4;  // at least; unknown: some

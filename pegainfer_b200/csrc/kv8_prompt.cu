@@ -700,12 +700,12 @@ bool prompt_takes(int T, int H, int G, int dim, int vdim) {
   const int R = H / G, tokens = R <= kPrRows ? 2 * (kPrRows / R) : 0;  // of a CTA
   return dim == vdim && (dim == 64 || dim == 96 || dim == 128) && tokens > 0 && (T + tokens - 1) / tokens <= 65535;
 }
-// Shares of the keys where the tiles leave SMs idle: as many CTAs as SMs, and 16 blocks of keys to a share at least (of the longest context, which is all that is known).
-// A share's start and end take 6 us, a block 1.5; the merge 5.
+// Shares of the keys where the tiles leave SMs idle: twice as many CTAs as SMs (a tile between two runs has both their keys to go through), and 12 blocks of keys to a
+// share at least (of the longest context, which is all that is known).  A share's start and end take 6 us, a block 1.5; the merge 5.
 int prompt_shares(int T, int H, int G, int max_kv_len, int window) {
   const int per = kPrRows / (H / G), ctas = (T + 2 * per - 1) / (2 * per) * G;
   const int span = window > 0 ? std::min(max_kv_len, window + 2 * per) : max_kv_len;
-  return std::max(1, std::min(sm_count() / std::max(ctas, 1), span / (16 * kPrKeys)));
+  return std::max(1, std::min(2 * sm_count() / std::max(ctas, 1), span / (12 * kPrKeys)));
 }
 int prompt_attention(const bf16* q, const bf16* sink, bf16* out, const AttnArgs& a, int shares, cudaStream_t st) {
   PromptArgs f{};

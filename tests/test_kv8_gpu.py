@@ -557,6 +557,46 @@ def test_evict_keeps_what_is_not_finite(lib):
     check_evict(lib, [50], 30, 8, 5, 2, 64, 64, poison=True)
 
 
+@pytest.mark.parametrize("n,budget,first,recent", [(33000, 1000, 3, 40), (40001, 40000, 1, 1), (32768, 77, 0, 0)])
+def test_evict_from_long_contexts(lib, n, budget, first, recent):
+    """around the longest that the keys' registers hold, and behind it"""
+    check_evict(lib, [n], budget, first, recent, 1, 32, 32)
+
+
+def test_evict_of_records_with_far_exponents(lib):
+    """tokens whose codes are all zero beside a large neighbour, moved to records of small ones and the other way round"""
+    G, D, n = 1, 32, 64
+    c = K.Cache([n], G, D, D, 16, spare=4)
+    g = torch.Generator().manual_seed(8)
+    k, v = torch.randn(n, G, D, generator=g).double(), torch.randn(n, G, D, generator=g).double()
+    for b, (x, y) in enumerate(((1e30, 1e-30), (1e-30, 1e-35), (1.0, 1e30), (1e-12, 3e38))):
+        k[b * 16:b * 16 + 5] *= x
+        k[b * 16 + 5:b * 16 + 16] *= y if y < 1e31 else 1e-20
+        v[b * 16:b * 16 + 9] *= y if y < 1e31 else 1e37
+        v[b * 16 + 9:b * 16 + 16] *= x
+    v[40:] = 0
+    K.fill(c, 0, k, v)
+    old_k, old_v = c.read(0, n)
+    c.data = c.data.to(DEV)
+    for keep in (range(5, 21), range(0, 64, 4), list(range(10, 16)) + list(range(40, 64)), range(16)):
+        keep = list(keep)
+        m = torch.zeros(1, G, n, device=DEV)
+        m[0, 0, keep] = 1.0
+        B = len(keep)
+        kept, new_lens, new_m = torch.zeros(1, G, B, dtype=I32, device=DEV), torch.zeros(1, dtype=I32, device=DEV), torch.zeros(1, G, B, device=DEV)
+        ln, off, pages, no, npg = i32([n]), c.page_off.to(DEV), c.pages.to(DEV), i32([0]), i32(c.spare)
+        assert lib.pk_kv8_evict(c.data.data_ptr(), c.stride, 16, off.data_ptr(), pages.data_ptr(), ln.data_ptr(), m.data_ptr(), n, no.data_ptr(), npg.data_ptr(),
+                                new_lens.data_ptr(), new_m.data_ptr(), B, kept.data_ptr(), 1, G, D, D, B, 0, 0, n, stream()) == 0
+        assert kept[0, 0].tolist() == keep
+        want = K.Cache([n], G, D, D, 16, spare=4, fill=0)
+        pad = -(-B // 16) * 16 - B
+        kk, vv = (torch.cat([x[keep], torch.zeros(pad, G, D, dtype=F64)]) for x in (old_k, old_v))
+        for blk in range(-(-B // 16)):
+            s = slice(blk * 16, blk * 16 + 16)
+            want.write_record(0, blk, kk[s], vv[s], torch.zeros(16, G, dtype=torch.bool), [K.exponent(kk[s].abs().max().item())], [K.exponent(vv[s].abs().max().item())], [0], c.spare)
+            assert torch.equal(c.record(0, blk, [0], c.spare).cpu(), want.record(0, blk, [0], c.spare))
+
+
 def test_evict_longer_than_told(lib):
     """no slot from max_kv_len on is looked at"""
     G, D = 2, 32
