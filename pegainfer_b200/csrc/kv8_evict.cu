@@ -99,9 +99,11 @@ __global__ void __launch_bounds__(kPickThreads) kv8_pick_kernel(EvictArgs a) {
   const int each = (w.n + kPickThreads - 1) / kPickThreads, j0 = warp * 32 * each + lane;  // this thread's i-th token is j0 + 32 i, i < each
   uint32_t key[EACH];
 #pragma unroll
+  for (int i = 0; i < EACH; ++i) key[i] = i < each && j0 + 32 * i < w.n ? __float_as_uint(__ldg(w.mass + j0 + 32 * i)) : 0u;  // (all under way at once)
+#pragma unroll
   for (int i = 0; i < EACH; ++i) {
     const int j = j0 + 32 * i;
-    key[i] = i < each && j < w.n ? mass_key(w.mass[j], j < a.first || j >= w.n - a.recent) : 0u;
+    key[i] = i < each && j < w.n ? mass_key(__uint_as_float(key[i]), j < a.first || j >= w.n - a.recent) : 0u;
   }
   // those above `least` are kept, and of those equal to it the first `left`
   uint32_t least = 0, left = w.keep;

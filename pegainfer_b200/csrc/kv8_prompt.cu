@@ -78,12 +78,6 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, ui
 __device__ __forceinline__ void pr_copy(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
 }
-// the larger, NaN where one is
-__device__ __forceinline__ float pr_max(float x, float y) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
-  return r;
-}
 __device__ __forceinline__ uint32_t pr_pack(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
@@ -101,38 +95,21 @@ __device__ __forceinline__ void pr_add2(float& a0, float& a1, float x0, float x1
   asm("add.rn.f32x2 %0, %0, %1;" : "+l"(v) : "l"(w));
   asm("mov.b64 {%0, %1}, %2;" : "=f"(a0), "=f"(a1) : "l"(v));
 }
-// {y0, y1} = {y0 x0 + c, y1 x1 + c}
-__device__ __forceinline__ void pr_mad2(float& y0, float& y1, float x0, float x1, float c) {
-  unsigned long long y, x, k;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "f"(y0), "f"(y1));
-  asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(x0), "f"(x1));
-  asm("mov.b64 %0, {%1, %1};" : "=l"(k) : "f"(c));
-  asm("fma.rn.f32x2 %0, %0, %1, %2;" : "+l"(y) : "l"(x), "l"(k));
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(y0), "=f"(y1) : "l"(y));
-}
-// {2^x0, 2^x1} without the special-function unit: 2^(x - n) by a polynomial of degree 4 for n the nearest whole number (fitted over [-1/2, 1/2] by reweighted least squares
-// to a relative error of 2.6e-6), n into the exponent.  x >= -125 (what lies below is 2^-125), no NaN.
-__device__ __forceinline__ void pr_poly2(float& x0, float& x1) {
-  x0 = fmaxf(x0, -125.f);
-  x1 = fmaxf(x1, -125.f);
-  float t0 = x0, t1 = x1;
-  pr_add2(t0, t1, 12582912.f, 12582912.f);  // 1.5 * 2^23: the whole number in the low bits
-  float n0 = t0, n1 = t1;
-  pr_add2(n0, n1, -12582912.f, -12582912.f);
-  pr_add2(x0, x1, -n0, -n1);
-  float y0 = 0.009570102f, y1 = 0.009570102f;
-  pr_mad2(y0, y1, x0, x1, 0.05591786f);
-  pr_mad2(y0, y1, x0, x1, 0.24024744f);
-  pr_mad2(y0, y1, x0, x1, 0.6931218f);
-  pr_mad2(y0, y1, x0, x1, 0.99999928f);
-  x0 = __uint_as_float(__float_as_uint(y0) + (__float_as_uint(t0) << 23));
-  x1 = __uint_as_float(__float_as_uint(y1) + (__float_as_uint(t1) << 23));
-}
-__device__ __forceinline__ uint32_t rest4(float a, float b, float c, float d) {
-  uint16_t x, y;
-  asm("cvt.rn.satfinite.e5m2x2.f32 %0, %1, %2;" : "=h"(x) : "f"(b), "f"(a));
-  asm("cvt.rn.satfinite.e5m2x2.f32 %0, %1, %2;" : "=h"(y) : "f"(d), "f"(c));
-  return (uint32_t)x | (uint32_t)y << 16;
+// four bf16 times a power of two (448 at most) -> the nearest e4m3 and the rests as e5m2.  f16 holds them exactly but below 2^-14, and there to 2^-25.
+__device__ __forceinline__ void q_parts(uint32_t w0, uint32_t w1, float down, uint32_t& near, uint32_t& rest) {
+  const uint32_t h0 = pr_pack(bf16_lo(w0) * down, bf16_hi(w0) * down), h1 = pr_pack(bf16_lo(w1) * down, bf16_hi(w1) * down);
+  uint16_t c[2], d[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    asm("{\n\t.reg .b32 b;\n\t"
+        "cvt.rn.satfinite.e4m3x2.f16x2 %0, %2;\n\t"
+        "cvt.rn.f16x2.e4m3x2 b, %0;\n\t"
+        "sub.rn.f16x2 b, %2, b;\n\t"
+        "cvt.rn.satfinite.e5m2x2.f16x2 %1, b;\n\t}"
+        : "=&h"(c[i]), "=&h"(d[i])
+        : "r"(i ? h1 : h0));
+  near = (uint32_t)c[0] | (uint32_t)c[1] << 16;
+  rest = (uint32_t)d[0] | (uint32_t)d[1] << 16;
 }
 
 template <int D>
@@ -145,7 +122,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* _
   uint8_t* Vs = Ks + kPrStages * KB;                     // [stage] V as it comes
   uint8_t* Hs = Vs + kPrStagesV * KB;                    // [stage] V as f16: [8 keys][entry][8 keys' f16]
   uint8_t* Ts = Hs + kPrStagesV * 2 * KB;                // [stage][record] tails as they come
-  int2* Es = reinterpret_cast<int2*>(Ts + kPrStagesV * kPrRecords * 16);  // [stage][record] of the f16's: 2^(K's exponent), V's exponent
+  uint32_t* Es = reinterpret_cast<uint32_t*>(Ts + kPrStagesV * kPrRecords * 16);  // [stage][record] tails of the f16's
   float* alpha_s = reinterpret_cast<float*>(Es + kPrStagesV * kPrRecords);  // [tile][buffer][row]
   float* end_s = alpha_s + 4 * kPrRows;                  // [tile][row]
   uint64_t* bars = reinterpret_cast<uint64_t*>(end_s + 2 * kPrRows);
@@ -194,6 +171,27 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* _
   if (warp == kPrMma) tmem_alloc(tmem_slot, 512);
   pdl_wait();
   pdl_launch_dependents();
+
+  // a softmax thread's row of q: under way while the runs are looked up
+  uint4 raw[D / 8];
+  if (warp < kPrCorr) {
+    const int r = tid & 127, k = r / R, ti = (warp >> 2) * per + k;
+    const bool on = k < per && ti < n_tok;
+    const bf16* src = q + ((size_t)(t0 + (on ? ti : 0)) * a.H + g * R + (on ? r - k * R : 0)) * D;
+#pragma unroll
+    for (int c = 0; c < D / 8; ++c) {
+      raw[c] = make_uint4(0, 0, 0, 0);
+      if (!on) continue;
+      if (f.q_by8) {
+        raw[c] = *reinterpret_cast<const uint4*>(src + c * 8);
+      } else {
+        uint32_t w[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) w[x] = (uint32_t)__bfloat16_as_ushort(src[c * 8 + 2 * x]) | (uint32_t)__bfloat16_as_ushort(src[c * 8 + 2 * x + 1]) << 16;
+        raw[c] = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+  }
 
   // ---- the runs that the tokens belong to
   for (int i = tid; i < kPrMaxSeg; i += kPrThreads)
@@ -258,9 +256,11 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* _
     }
   };
   // this CTA's share of them (the grid's z axis), counted from its own first
-  int share = 0;
+  int share = INT_MAX;
   Step origin{0, 0, 0};
-  {
+  if (gridDim.z == 1) {
+    settle(origin);
+  } else {
     int all = 0;
     for (int k = 0; k < segs; ++k)
       if (last_block(k) >= 0) all += last_block(k) - first_block(k) + 1;
@@ -409,10 +409,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* _
         *reinterpret_cast<uint4*>(to + (2 * b) * REC_K + d * 16) = make_uint4(h[0], h[1], h[2], h[3]);
         *reinterpret_cast<uint4*>(to + (2 * b + 1) * REC_K + d * 16) = make_uint4(h[4], h[5], h[6], h[7]);
       }
-      if (r < kPrRecords) {
-        const uint32_t tail = *reinterpret_cast<const uint32_t*>(Ts + (sv * kPrRecords + r) * 16);
-        Es[sv * kPrRecords + r] = make_int2(__float_as_int(pow2(tail_ek(tail))), tail_ev(tail));
-      }
+      if (r < kPrRecords) Es[sv * kPrRecords + r] = *reinterpret_cast<const uint32_t*>(Ts + (sv * kPrRecords + r) * 16);
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
@@ -511,22 +508,9 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* _
     // q: scaled to the codes' upper end, split, into the operands
     float row_c;
     {
-      const bf16* src = q + ((size_t)(t0 + (on ? ti : 0)) * a.H + h) * D;
       float amax = 0.f;
-      uint4 raw[D / 8];
 #pragma unroll
       for (int c = 0; c < D / 8; ++c) {
-        raw[c] = make_uint4(0, 0, 0, 0);
-        if (on) {
-          if (f.q_by8) {
-            raw[c] = *reinterpret_cast<const uint4*>(src + c * 8);
-          } else {
-            uint32_t w[4];
-#pragma unroll
-            for (int x = 0; x < 4; ++x) w[x] = (uint32_t)__bfloat16_as_ushort(src[c * 8 + 2 * x]) | (uint32_t)__bfloat16_as_ushort(src[c * 8 + 2 * x + 1]) << 16;
-            raw[c] = make_uint4(w[0], w[1], w[2], w[3]);
-          }
-        }
         const uint32_t w[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
 #pragma unroll
         for (int x = 0; x < 4; ++x) amax = fmaxf(amax, fmaxf(fabsf(bf16_lo(w[x])), fabsf(bf16_hi(w[x]))));
@@ -540,12 +524,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* _
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
           const uint4 u = raw[2 * c + (x >> 1)];
-          const uint32_t w0 = x & 1 ? u.z : u.x, w1 = x & 1 ? u.w : u.y;
-          const float v0 = bf16_lo(w0) * down, v1 = bf16_hi(w0) * down, v2 = bf16_lo(w1) * down, v3 = bf16_hi(w1) * down;
-          hi[x] = codes4(v0, v1, v2, v3);
-          float y[4];
-          values4(hi[x], y);
-          rest[x] = rest4(v0 - y[0], v1 - y[1], v2 - y[2], v3 - y[3]);
+          q_parts(x & 1 ? u.z : u.x, x & 1 ? u.w : u.y, down, hi[x], rest[x]);
         }
         uint8_t* dst = Qs + i * 2 * QB + (r >> 3) * (8 * D) + c * 128 + (r & 7) * 16;
         *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
@@ -559,26 +538,24 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* _
     const float cap2 = a.cap * kLog2e, cap_c = a.cap > 0.f ? 2.f * a.scale / a.cap * kLog2e : 0.f;
     float m = -INFINITY, l = 0.f;
     int E = kLowExp - 1, mine = 0;
-    bool s_there = false, h_there = false;  // looked up under the block before
-    Step x = begin();
-    while (x.seg < segs && !needs(i, x.seg, x.j)) next(x);
-    while (x.seg < segs) {
+    for (Step x = begin(); x.seg < segs; next(x)) {
+      if (!needs(i, x.seg, x.j)) continue;
       const int sv = x.n % kPrStagesV;
       const uint32_t t_s = t_tile + (uint32_t)((mine & 1) * kPrKeys);
       // S first: it says that the stage's phases before this block's are over (a tile that skipped blocks would take an older one for it)
-      if (!s_there) mbar_wait_bounded(s_full + i * 2 + (mine & 1), (uint32_t)((mine >> 1) & 1), dead, tries);
+      mbar_wait_bounded(s_full + i * 2 + (mine & 1), (uint32_t)((mine >> 1) & 1), dead, tries);
       tc_fence_after();
       uint32_t v[kPrKeys];
       tmem_ld32_nowait(t_s, v);
       tmem_ld32_nowait(t_s + 32, v + 32);
-      if (!h_there) mbar_wait_bounded(h_full + sv, (uint32_t)((x.n / kPrStagesV) & 1), dead, tries);
+      mbar_wait_bounded(h_full + sv, (uint32_t)((x.n / kPrStagesV) & 1), dead, tries);
       int ev[kPrRecords], e_new = E;
       float fk[kPrRecords];
 #pragma unroll
       for (int b = 0; b < kPrRecords; ++b) {
-        const int2 e = Es[sv * kPrRecords + b];
-        ev[b] = e.y;
-        const float y = __int_as_float(e.x) * row_c;
+        const uint32_t tail = Es[sv * kPrRecords + b];
+        ev[b] = tail_ev(tail);
+        const float y = pow2(tail_ek(tail)) * row_c;
         fk[b] = y < 1e-37f ? 1e-37f : y;  // never zero: -inf times it stays -inf (and a NaN stays one)
         e_new = max(e_new, ev[b]);
       }
@@ -599,17 +576,13 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* _
       float mx = m;
 #pragma unroll
       for (int b = 0; b < kPrRecords; ++b) {
-        float y = pr_max(__uint_as_float(v[b * 16]), __uint_as_float(v[b * 16 + 1])), z = pr_max(__uint_as_float(v[b * 16 + 2]), __uint_as_float(v[b * 16 + 3]));
+        float y = fmaxf(__uint_as_float(v[b * 16]), __uint_as_float(v[b * 16 + 1])), z = fmaxf(__uint_as_float(v[b * 16 + 2]), __uint_as_float(v[b * 16 + 3]));
 #pragma unroll
         for (int k = 4; k < 16; k += 4) {
-          y = pr_max(pr_max(y, __uint_as_float(v[b * 16 + k])), __uint_as_float(v[b * 16 + k + 1]));
-          z = pr_max(pr_max(z, __uint_as_float(v[b * 16 + k + 2])), __uint_as_float(v[b * 16 + k + 3]));
+          y = fmaxf(fmaxf(y, __uint_as_float(v[b * 16 + k])), __uint_as_float(v[b * 16 + k + 1]));
+          z = fmaxf(fmaxf(z, __uint_as_float(v[b * 16 + k + 2])), __uint_as_float(v[b * 16 + k + 3]));
         }
-        mx = pr_max(mx, pr_max(y, z) * factor(b));
-      }
-      if (mx != mx) {  // a NaN among what the row sees: its sum says so at the end, whatever P holds
-        l = NAN;
-        mx = m;
+        mx = fmaxf(mx, fmaxf(y, z) * factor(b));
       }
       const float m_new = mx > m + (float)kPrSlack ? mx : m;  // (m = -inf: mx)
       const float ref = m_new == -INFINITY ? 0.f : m_new, fl = pr_ex2(m - ref);
@@ -620,15 +593,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* _
       m = m_new;
       E = e_new;
       l *= fl;
-      // this tile's next block: asked for now, answered under the exponentials
-      Step after = x;
-      do next(after);
-      while (after.seg < segs && !needs(i, after.seg, after.j));
-      if (after.seg < segs) {
-        s_there = mbar_test_wait(s_full + i * 2 + ((mine + 1) & 1), (uint32_t)(((mine + 1) >> 1) & 1));
-        h_there = after.n == x.n + 1 && mbar_test_wait(h_full + after.n % kPrStagesV, (uint32_t)((after.n / kPrStagesV) & 1));
-      }
-      // P of 16 columns -> eight columns; one pair of four without the special-function unit, which two tiles' exponentials alone keep busy for 1024 clocks a block
+      // P of 16 columns -> eight columns
       uint32_t w[kPrKeys / 2];
 #pragma unroll
       for (int b = 0; b < kPrRecords; ++b) {
@@ -639,12 +604,8 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* _
         for (int k = 0; k < 8; ++k) {
           float s0 = __uint_as_float(v[b * 16 + 2 * k]), s1 = __uint_as_float(v[b * 16 + 2 * k + 1]);
           pr_fma2(s0, s1, fb, add);
-          if (k % 4 == 3) {
-            pr_poly2(s0, s1);
-          } else {
-            s0 = pr_ex2(s0);
-            s1 = pr_ex2(s1);
-          }
+          s0 = pr_ex2(s0);
+          s1 = pr_ex2(s1);
           pr_add2(d0, d1, s0, s1);
           w[b * 8 + k] = pr_pack(s0, s1);
         }
@@ -656,7 +617,6 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* _
       __syncwarp();
       if (lane == 0) mbar_arrive(po_ready + i * 2 + (mine & 1));
       ++mine;
-      x = after;
     }
     const float top = l != l ? INFINITY : m;  // a NaN among the scores
     const float up = pow2(max(E, kLowExp) - kPrTop);
@@ -690,7 +650,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* _
 
 template <int D>
 static int launch_prompt(const bf16* q, const bf16* sink, bf16* out, const PromptArgs& f, int shares, cudaStream_t st) {
-  constexpr size_t smem = 128 + (size_t)4 * kPrRows * D + (size_t)(kPrStages + 3 * kPrStagesV) * kPrKeys * D + kPrStagesV * kPrRecords * 24 + 6 * kPrRows * sizeof(float) + 40 * 8;
+  constexpr size_t smem = 128 + (size_t)4 * kPrRows * D + (size_t)(kPrStages + 3 * kPrStagesV) * kPrKeys * D + kPrStagesV * kPrRecords * 20 + 6 * kPrRows * sizeof(float) + 40 * 8;
   static std::atomic<uint64_t> set{0};
   if (const cudaError_t e = allow_smem(set, (const void*)kv8_prompt_kernel<D>, smem); e != cudaSuccess) return (int)e;
   return (int)launch(kv8_prompt_kernel<D>, dim3(f.a.pool.G, (f.a.T + 2 * f.per - 1) / (2 * f.per), shares), dim3(kPrThreads), smem, st, true, q, sink, out, f);
@@ -700,12 +660,12 @@ bool prompt_takes(int T, int H, int G, int dim, int vdim) {
   const int R = H / G, tokens = R <= kPrRows ? 2 * (kPrRows / R) : 0;  // of a CTA
   return dim == vdim && (dim == 64 || dim == 96 || dim == 128) && tokens > 0 && (T + tokens - 1) / tokens <= 65535;
 }
-// Shares of the keys where the tiles leave SMs idle: twice as many CTAs as SMs (a tile between two runs has both their keys to go through), and 12 blocks of keys to a
-// share at least (of the longest context, which is all that is known).  A share's start and end take 6 us, a block 1.5; the merge 5.
+// Shares of the keys where the tiles leave SMs idle: as many CTAs as SMs, and 16 blocks of keys to a share at least (of the longest context, which is all that is known).
+// A share's start and end take 6 us, a block 1.5; the merge 5.
 int prompt_shares(int T, int H, int G, int max_kv_len, int window) {
   const int per = kPrRows / (H / G), ctas = (T + 2 * per - 1) / (2 * per) * G;
   const int span = window > 0 ? std::min(max_kv_len, window + 2 * per) : max_kv_len;
-  return std::max(1, std::min(2 * sm_count() / std::max(ctas, 1), span / (12 * kPrKeys)));
+  return std::max(1, std::min(sm_count() / std::max(ctas, 1), span / (16 * kPrKeys)));
 }
 int prompt_attention(const bf16* q, const bf16* sink, bf16* out, const AttnArgs& a, int shares, cudaStream_t st) {
   PromptArgs f{};
