@@ -264,6 +264,334 @@ __global__ void __launch_bounds__(kAppendWarps * 32) kv8_append_kernel(const E* 
   }
 }
 
+
+// ---- bf16 rows on 16-byte boundaries, rotated dimensions a multiple of 32: everything in registers.
+//
+// The first CTAs take records, a warp to each (record, kv head); the rest take q.
+//   K    a lane has units of 16 entries of a token two by two, those that turn into one another: (u, u + dims/2) or 16 consecutive pairs
+//   V    a lane has two entries of all 16 tokens: the code's 16 tokens of an entry need no transposition
+// All loads are under way before the first angle is there.  Where a record goes on under its old exponent of K, K's old codes are not touched.
+constexpr int kTurnRows = 32;  // a window's tokens, and those of its last record
+
+__device__ __forceinline__ float2 turn_of(int position, float freq, float mag) {
+  const double turns = (double)position * (double)freq * 0.15915494309189533577;
+  float s, c;
+  sincospif((float)(2.0 * (turns - rint(turns))), &s, &c);
+  return make_float2(c * mag, s * mag);
+}
+// eight pairs: (x[j], y[j]), or side by side in x and then y
+__device__ __forceinline__ void turn_pairs(float* x, float* y, const float2 (&cs)[8], int side_by_side) {
+  if (side_by_side) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      float* z = j < 4 ? x + 2 * j : y + 2 * j - 8;
+      const float p = z[0], r = z[1];
+      z[0] = p * cs[j].x - r * cs[j].y;
+      z[1] = p * cs[j].y + r * cs[j].x;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float p = x[j], r = y[j];
+      x[j] = p * cs[j].x - r * cs[j].y;
+      y[j] = p * cs[j].y + r * cs[j].x;
+    }
+  }
+}
+__device__ __forceinline__ void widen8(const uint4& u, float* v) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = bf16_lo(w[i]);
+    v[2 * i + 1] = bf16_hi(w[i]);
+  }
+}
+__device__ __forceinline__ uint4 narrow8(const float* v) { return make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7])); }
+__device__ __forceinline__ bool odd_one(float v) { return (__float_as_uint(v) & 0x7f800000u) == 0x7f800000u; }
+// 16 codes under an exponent `down` = 2^(old - new) -> under the new one
+__device__ __forceinline__ uint4 again16(const uint4& old, float down) {
+  float v[16];
+  values16(old, v);
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = codes4(v[4 * i] * down, v[4 * i + 1] * down, v[4 * i + 2] * down, v[4 * i + 3] * down);
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+struct WideArgs {
+  AppendArgs a;
+  int rec_ctas, rec_parts;  // CTAs of records: windows * rec_parts
+  int by;                   // heads that a thread of q turns by the same angles
+};
+
+// N: 64ths of the larger width
+template <int N>
+__global__ void __launch_bounds__(kAppendWarps * 32, N <= 2 ? 4 : 2) kv8_append_wide_kernel(const bf16* __restrict__ qkv, const bf16* __restrict__ bias, bf16* __restrict__ q_out, const WideArgs f) {
+  extern __shared__ __align__(16) float2 ap_turns[];  // [token][pair], rows 16 bytes apart from a multiple of the banks
+  const AppendArgs& a = f.a;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, half = a.dims >> 1;
+  const int D = a.pool.dim, V = a.pool.vdim, G = a.pool.G, H = a.H;
+  pdl_wait();
+  pdl_launch_dependents();
+
+  if ((int)blockIdx.x >= f.rec_ctas) {
+    // ---- queries: 16 entries (eight pairs, or eight and eight of those that only pass) of `by` heads
+    const int units = D / 16, groups = (H + f.by - 1) / f.by;
+    const long i = (long)((int)blockIdx.x - f.rec_ctas) * blockDim.x + threadIdx.x;
+    if (i >= (long)a.T * units * groups) return;
+    const int u = (int)(i % units), t = (int)(i / units % a.T), h0 = (int)(i / units / a.T) * f.by, h1 = min(h0 + f.by, H);
+    const bool turns = u < half / 8;
+    const int d0 = turns ? (a.interleaved ? u * 16 : u * 8) : a.dims + (u - half / 8) * 16, d1 = turns && !a.interleaved ? d0 + half : d0 + 8;
+    const bf16* src = qkv + (size_t)t * a.ld;
+    bf16* dst = q_out + (size_t)t * H * D;
+    float2 cs[8];
+    for (int h = h0; h < h1; h += 4) {
+      uint4 raw[4][2];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (h + k < h1) {
+          raw[k][0] = *reinterpret_cast<const uint4*>(src + (h + k) * D + d0);
+          raw[k][1] = *reinterpret_cast<const uint4*>(src + (h + k) * D + d1);
+        }
+      if (h == h0 && turns) {
+        const int at = a.positions[t];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) cs[k] = turn_of(at, a.freq[u * 8 + k], a.mag);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (h + k < h1) {
+          float x[8], y[8];
+          widen8(raw[k][0], x);
+          widen8(raw[k][1], y);
+          if (bias) {
+            const bf16* b = bias + (h + k) * D;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              x[j] += to_f(b[d0 + j]);
+              y[j] += to_f(b[d1 + j]);
+            }
+          }
+          if (turns) turn_pairs(x, y, cs, a.interleaved);
+          *reinterpret_cast<uint4*>(dst + (h + k) * D + d0) = narrow8(x);
+          *reinterpret_cast<uint4*>(dst + (h + k) * D + d1) = narrow8(y);
+        }
+    }
+    return;
+  }
+
+  // ---- records
+  const int w0 = (int)blockIdx.x / f.rec_parts * kWindow, part = (int)blockIdx.x % f.rec_parts, n_tok = min(kWindow, a.T - w0);
+  // lane i: token i of the window, and of the next one (a record may reach into it)
+  const int t_l = min(w0 + lane, a.T - 1);
+  const int slot_l = a.slots[t_l], req_l = a.req[t_l];
+  int slot_b = __shfl_up_sync(0xffffffffu, slot_l, 1), req_b = __shfl_up_sync(0xffffffffu, req_l, 1);
+  if (lane == 0 && w0 > 0) {
+    slot_b = a.slots[w0 - 1];
+    req_b = a.req[w0 - 1];
+  }
+  const bool follows = w0 + lane > 0 && slot_b == slot_l - 1 && req_b == req_l && w0 + lane < a.T;
+  const uint32_t on = __ballot_sync(0xffffffffu, follows && slot_l >= 0 && slot_l % kBlock != 0);  // goes on with the record of the token before
+  const uint32_t leads = __ballot_sync(0xffffffffu, lane < n_tok && slot_l >= 0) & ~on;
+  const int items = __popc(leads) * G, ld_t = half + 2;
+  const int pos_rows = min(kTurnRows, a.T - w0);
+  if (part * kAppendWarps >= items) return;
+  bool table = false;
+  for (int at = part * kAppendWarps; at < items; at += f.rec_parts * kAppendWarps) {
+    const int it = at + warp;
+    const bool busy = it < items;
+    const int g = it % G, tok = busy ? (int)__fns(leads, 0, it / G + 1) : 0;
+    const int slot = __shfl_sync(0xffffffffu, slot_l, tok), req = __shfl_sync(0xffffffffu, req_l, tok), first = slot & (kBlock - 1);
+    const int count = busy ? __ffs(~(on >> (tok + 1))) : 0;  // the leader and those that go on behind it
+    const uint32_t fresh = ((1u << count) - 1u) << first;
+    const bf16* src = qkv + (size_t)(w0 + tok - first) * a.ld + H * D;  // row of the record's slot 0
+    // everything that is read from the rows
+    uint4 kr[N][4];
+    uint32_t vr[N][16];
+    const int pos = lane & 15;
+    const bool mine = fresh >> pos & 1;
+    int c0[N], c1[N];
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int p = (lane >> 4) + 2 * n;
+      c0[n] = p < half / 16 ? (a.interleaved ? 2 * p : p) : 2 * p;
+      c1[n] = p < half / 16 && !a.interleaved ? p + half / 16 : c0[n] + 1;
+      if (mine && p < D / 32) {
+        const bf16* row = src + (size_t)pos * a.ld + g * D;
+        kr[n][0] = *reinterpret_cast<const uint4*>(row + c0[n] * 16);
+        kr[n][1] = *reinterpret_cast<const uint4*>(row + c0[n] * 16 + 8);
+        kr[n][2] = *reinterpret_cast<const uint4*>(row + c1[n] * 16);
+        kr[n][3] = *reinterpret_cast<const uint4*>(row + c1[n] * 16 + 8);
+      } else {
+        kr[n][0] = kr[n][1] = kr[n][2] = kr[n][3] = make_uint4(0, 0, 0, 0);
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int d = 2 * lane + 64 * n;
+        vr[n][r] = fresh >> r & 1 && d < V ? *reinterpret_cast<const uint32_t*>(src + (size_t)r * a.ld + G * D + g * V + d) : 0u;
+      }
+    uint8_t* rec = nullptr;
+    uint32_t tail = 0;
+    uint4 v_old[N][2];
+    if (busy) rec = a.pool.record(req, slot, g);
+    if (busy && first) {
+      tail = *reinterpret_cast<const uint32_t*>(rec + kBlock * (D + V));
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+        if (2 * lane + 64 * n < V) {
+          v_old[n][0] = *reinterpret_cast<const uint4*>(rec + kBlock * (D + 2 * lane + 64 * n));
+          v_old[n][1] = *reinterpret_cast<const uint4*>(rec + kBlock * (D + 2 * lane + 64 * n + 1));
+        }
+    }
+    if (!table) {  // under the loads
+      for (int i = threadIdx.x; i < pos_rows * half; i += blockDim.x) {
+        const int r = i / half, k = i - r * half;
+        if (r < kWindow || on >> kWindow & 1) ap_turns[r * ld_t + k] = turn_of(a.positions[w0 + r], a.freq[k], a.mag);
+      }
+      table = true;
+      __syncthreads();
+    }
+    if (!busy) continue;
+
+    // values
+    float b0[N], b1[N];
+    uint32_t bad = 0;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int d = 2 * lane + 64 * n;
+      b0[n] = bias && d < V ? to_f(bias[(H + G) * D + g * V + d]) : 0.f;
+      b1[n] = bias && d < V ? to_f(bias[(H + G) * D + g * V + d + 1]) : 0.f;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) bad |= (odd_one(bf16_lo(vr[n][r]) + b0[n]) || odd_one(bf16_hi(vr[n][r]) + b1[n]) ? 1u : 0u) << r;
+    }
+    const uint32_t bad_v = __reduce_or_sync(0xffffffffu, bad) & fresh, good_v = fresh & ~bad_v;
+    float amax = 0.f;
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (good_v >> r & 1) amax = fmaxf(amax, fmaxf(fabsf(bf16_lo(vr[n][r]) + b0[n]), fabsf(bf16_hi(vr[n][r]) + b1[n])));
+    const int had_v = tail_ev(tail), had_k = tail_ek(tail);
+    int ev = exponent_for(warp_max(amax));
+    if (first) ev = max(ev, had_v);
+    {
+      const float down = pow2(-ev), move = pow2(max(had_v - ev, -126));
+      const bool grown = first && ev != had_v;
+      uint8_t* dst = rec + kBlock * D;
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        const int d = 2 * lane + 64 * n;
+        if (d >= V) continue;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          uint32_t w[4];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            float y[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const uint32_t two = vr[n][4 * x + j];
+              y[j] = good_v >> (4 * x + j) & 1 ? (k ? bf16_hi(two) + b1[n] : bf16_lo(two) + b0[n]) * down : 0.f;
+            }
+            w[x] = codes4(y[0], y[1], y[2], y[3]);
+          }
+          if (first) {
+            const uint4 old = grown ? again16(v_old[n][k], move) : v_old[n][k];
+            const uint32_t o[4] = {old.x, old.y, old.z, old.w};
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {  // (the new codes are zero where old tokens lie)
+              const int keep = min(max(first - 4 * x, 0), 4);
+              w[x] |= keep == 4 ? o[x] : o[x] & ((1u << (8 * keep)) - 1u);
+            }
+          }
+          *reinterpret_cast<uint4*>(dst + (d + k) * kBlock) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      }
+    }
+
+    // keys
+    bad = 0;
+    amax = 0.f;
+    float x[N][16], y[N][16];
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int p = (lane >> 4) + 2 * n;
+      widen8(kr[n][0], x[n]);
+      widen8(kr[n][1], x[n] + 8);
+      widen8(kr[n][2], y[n]);
+      widen8(kr[n][3], y[n] + 8);
+      if (!mine || p >= D / 32) continue;
+      bool odd = false;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        if (bias) {
+          x[n][j] += to_f(bias[(H + g) * D + c0[n] * 16 + j]);
+          y[n][j] += to_f(bias[(H + g) * D + c1[n] * 16 + j]);
+        }
+        odd |= odd_one(x[n][j]) || odd_one(y[n][j]);
+      }
+      if (odd) bad = 1u << pos;
+      if (p < half / 16) {
+        const float2* row = ap_turns + (tok + pos - first) * ld_t + p * 16;
+#pragma unroll
+        for (int j = 0; j < 16; j += 8) {
+          float2 cs[8];
+#pragma unroll
+          for (int k = 0; k < 8; k += 2) {
+            const float4 two = *reinterpret_cast<const float4*>(row + j + k);
+            cs[k] = make_float2(two.x, two.y);
+            cs[k + 1] = make_float2(two.z, two.w);
+          }
+          // 16 entries in a row are eight pairs where they lie side by side
+          if (a.interleaved) turn_pairs(j ? y[n] : x[n], j ? y[n] + 8 : x[n] + 8, cs, 1);
+          else turn_pairs(x[n] + j, y[n] + j, cs, 0);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 16; ++j) amax = fmaxf(amax, fmaxf(fabsf(x[n][j]), fabsf(y[n][j])));
+    }
+    const uint32_t bad_k = __reduce_or_sync(0xffffffffu, bad) | bad_v;
+    int ek = exponent_for(warp_max(bad_k >> pos & 1 ? 0.f : amax));
+    if (first) ek = max(ek, had_k);
+    {
+      const float down = pow2(-ek), move = pow2(max(had_k - ek, -126));
+      const bool grown = first && ek != had_k;
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        if ((lane >> 4) + 2 * n >= D / 32) continue;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          uint4* at16 = reinterpret_cast<uint4*>(rec + (pos >= 8 ? 8 * D : 0) + (k ? c1[n] : c0[n]) * 128 + (pos & 7) * 16);
+          const float* z = k ? y[n] : x[n];
+          uint32_t w[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) w[j] = bad_k >> pos & 1 ? 0x7f7f7f7fu : codes4(z[4 * j] * down, z[4 * j + 1] * down, z[4 * j + 2] * down, z[4 * j + 3] * down);
+          if (pos >= first) *at16 = make_uint4(w[0], w[1], w[2], w[3]);  // (zeros behind the last token)
+          else if (grown) *at16 = again16(*at16, move);
+        }
+      }
+    }
+    if (lane == 0) emit_tail(rec + kBlock * (D + V), ek, ev);
+  }
+}
+
+template <int N>
+static int append_wide(const bf16* qkv, const bf16* bias, bf16* q_out, const AppendArgs& a, cudaStream_t st) {
+  const int windows = (a.T + kWindow - 1) / kWindow;
+  // a warp for every record, or as many CTAs as the GPU holds at once; whole records (consecutive slots) come to one a head
+  const int most = (std::min(a.T, kWindow) * a.pool.G + kAppendWarps - 1) / kAppendWarps, whole = (a.pool.G + kAppendWarps - 1) / kAppendWarps;
+  WideArgs f{a, 0, std::min(most, std::max(whole, 4 * sm_count() / windows)), 8};
+  f.rec_ctas = windows * f.rec_parts;
+  const long threads = kAppendWarps * 32, units = (long)a.T * (a.pool.dim / 16);
+  while (f.by > 1 && units * ((a.H + f.by - 1) / f.by) < threads * 4 * sm_count()) f.by /= 2;
+  const long ctas = a.H ? (units * ((a.H + f.by - 1) / f.by) + threads - 1) / threads : 0;
+  const size_t smem = (size_t)kTurnRows * (a.dims / 2 + 2) * sizeof(float2);
+  return (int)launch(kv8_append_wide_kernel<N>, dim3((unsigned)(f.rec_ctas + ctas)), dim3((unsigned)threads), smem, st, true, qkv, bias, q_out, f);
+}
+
 }  // namespace kv8
 }  // namespace pk
 
@@ -285,6 +613,13 @@ extern "C" int pk_kv8_append(const void* qkv, int ld, const void* bias, const in
   const bool vec = ((reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(q_out)) & 15) == 0 && (long)ld * es % 16 == 0;
   const kv8::AppendArgs a{positions, slots ? slots : positions, req, kv8::make_pool(cache, page_stride, page_off, pages, page_size, kv_heads, dim, vdim),
                           freq,      mag,                       ld,  heads, tokens, dims, interleaved, vec};
+  if (!f32 && vec && dims % 32 == 0) {
+    const int wide = std::max(dim, vdim);
+    const bf16 *x = (const bf16*)qkv, *b = (const bf16*)bias;
+    if (wide <= 64) return kv8::append_wide<1>(x, b, (bf16*)q_out, a, st);
+    if (wide <= 128) return kv8::append_wide<2>(x, b, (bf16*)q_out, a, st);
+    return kv8::append_wide<4>(x, b, (bf16*)q_out, a, st);
+  }
   const int windows = (tokens + kv8::kWindow - 1) / kv8::kWindow;
   const int items = (std::min(tokens, kv8::kWindow) * kv_heads + kv8::kAppendWarps - 1) / kv8::kAppendWarps;
   const int parts = std::max(1, std::min(items, (4 * sm_count() + windows - 1) / windows));
