@@ -273,11 +273,12 @@ __global__ void __launch_bounds__(kAppendWarps * 32) kv8_append_kernel(const E* 
 // All loads are under way before the first angle is there.  Where a record goes on under its old exponent of K, K's old codes are not touched.
 constexpr int kTurnRows = 32;  // a window's tokens, and those of its last record
 
+// The angle, within half a turn, goes to the special-function unit: 2^-21 off, where the results are rounded to 2^-9 at best.  (With the library's sine and cosine two of
+// five instructions of the kernel were angles: 27.5 us for 4096 tokens, XX us so.)
 __device__ __forceinline__ float2 turn_of(int position, float freq, float mag) {
   const double turns = (double)position * (double)freq * 0.15915494309189533577;
-  float s, c;
-  sincospif((float)(2.0 * (turns - rint(turns))), &s, &c);
-  return make_float2(c * mag, s * mag);
+  const float angle = (float)(turns - rint(turns)) * 6.2831853071795865f;
+  return make_float2(__cosf(angle) * mag, __sinf(angle) * mag);
 }
 // eight pairs: (x[j], y[j]), or side by side in x and then y
 __device__ __forceinline__ void turn_pairs(float* x, float* y, const float2 (&cs)[8], int side_by_side) {
@@ -316,6 +317,128 @@ __device__ __forceinline__ uint4 again16(const uint4& old, float down) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) w[i] = codes4(v[4 * i] * down, v[4 * i + 1] * down, v[4 * i + 2] * down, v[4 * i + 3] * down);
   return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// a token alone in its record, by one warp
+template <int N>
+__device__ __forceinline__ void append_one(const bf16* row, const bf16* bias, const AppendArgs& a, int t, int g, int lane) {
+  const int D = a.pool.dim, V = a.pool.vdim, G = a.pool.G, H = a.H, half = a.dims >> 1;
+  const int slot = a.slots[t], pos = slot & (kBlock - 1);
+  const bf16* k_src = row + (H + g) * D;
+  const bf16* v_src = row + (H + G) * D + g * V;
+  const bf16* k_bias = bias ? bias + (H + g) * D : nullptr;
+  const bf16* v_bias = bias ? bias + (H + G) * D + g * V : nullptr;
+  // pairs of K, those that only pass two by two behind the others; entries of V
+  float x[N], y[N], v[2 * N];
+  int ix[N], iy[N];
+  const int at = a.positions[t];
+  float2 cs[N];
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    const int p = lane + 32 * n;
+    const bool turns = p < half;
+    ix[n] = a.interleaved || !turns ? 2 * p : p;
+    iy[n] = a.interleaved || !turns ? 2 * p + 1 : p + half;
+    x[n] = y[n] = v[2 * n] = v[2 * n + 1] = 0.f;
+    cs[n] = make_float2(1.f, 0.f);
+    if (2 * p < D) {
+      x[n] = to_f(k_src[ix[n]]);
+      y[n] = to_f(k_src[iy[n]]);
+      if (turns) cs[n].x = a.freq[p];
+    }
+    if (2 * p < V) {
+      const uint32_t two = *reinterpret_cast<const uint32_t*>(v_src + 2 * p);
+      v[2 * n] = bf16_lo(two);
+      v[2 * n + 1] = bf16_hi(two);
+    }
+  }
+  uint8_t* rec = a.pool.record(a.req[t], slot, g);
+  uint8_t* vdst = rec + kBlock * D;
+  uint4 old[2 * N];
+  uint32_t tail = 0;
+#pragma unroll
+  for (int n = 0; n < 2 * N; ++n) old[n] = make_uint4(0, 0, 0, 0);
+  if (pos) {
+    tail = *reinterpret_cast<const uint32_t*>(rec + kBlock * (D + V));
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+      if (2 * (lane + 32 * n) < V) {
+        old[2 * n] = *reinterpret_cast<const uint4*>(vdst + (lane + 32 * n) * 2 * kBlock);
+        old[2 * n + 1] = *reinterpret_cast<const uint4*>(vdst + (lane + 32 * n) * 2 * kBlock + kBlock);
+      }
+  }
+  bool bad_k = false, bad_v = false;
+  float most_k = 0.f, most_v = 0.f;
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    const int p = lane + 32 * n;
+    if (2 * p < D) {
+      if (k_bias) {
+        x[n] += to_f(k_bias[ix[n]]);
+        y[n] += to_f(k_bias[iy[n]]);
+      }
+      bad_k |= odd_one(x[n]) || odd_one(y[n]);
+      if (p < half) {
+        cs[n] = turn_of(at, cs[n].x, a.mag);
+        const float x0 = x[n], y0 = y[n];
+        x[n] = x0 * cs[n].x - y0 * cs[n].y;
+        y[n] = x0 * cs[n].y + y0 * cs[n].x;
+      }
+      most_k = fmaxf(most_k, fmaxf(fabsf(x[n]), fabsf(y[n])));
+    }
+    if (2 * p < V) {
+      if (v_bias) {
+        v[2 * n] += to_f(v_bias[2 * p]);
+        v[2 * n + 1] += to_f(v_bias[2 * p + 1]);
+      }
+      bad_v |= odd_one(v[2 * n]) || odd_one(v[2 * n + 1]);
+      most_v = fmaxf(most_v, fmaxf(fabsf(v[2 * n]), fabsf(v[2 * n + 1])));
+    }
+  }
+  bad_v = __any_sync(0xffffffffu, bad_v);
+  bad_k = __any_sync(0xffffffffu, bad_k) || bad_v;
+  int ek = exponent_for(bad_k ? 0.f : warp_max(most_k)), ev = exponent_for(bad_v ? 0.f : warp_max(most_v));
+  const int had_k = tail_ek(tail), had_v = tail_ev(tail);
+  if (pos) {
+    ek = max(ek, had_k);
+    ev = max(ev, had_v);
+  }
+  // V: the token's byte, zeros behind it
+  const float down_k = pow2(-ek), down_v = pow2(-ev), move = pow2(max(had_v - ev, -126));
+#pragma unroll
+  for (int n = 0; n < 2 * N; ++n) {
+    const int d = 2 * (lane + 32 * (n >> 1)) + (n & 1);
+    if (d >= V) continue;
+    uint4 o = old[n];
+    if (pos && ev != had_v) o = again16(o, move);
+    const uint32_t code = bad_v ? 0u : codes2(v[n] * down_v, 0.f) & 0xffu;
+    uint32_t w[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int keep = min(max(pos - 4 * i, 0), 4);
+      w[i] = keep == 4 ? w[i] : (w[i] & ((1u << (8 * keep)) - 1u)) | (pos >> 2 == i ? code << (8 * keep) : 0u);
+    }
+    *reinterpret_cast<uint4*>(vdst + d * kBlock) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  // K: the token's bytes; rows behind it zero, rows before it again where the exponent grew
+  const float again = pow2(max(had_k - ek, -126));
+  const bool grown = pos && ek != had_k;
+#pragma unroll 1
+  for (int u = lane; u < D; u += 32) {
+    const int r = (u >= D / 2 ? 8 : 0) + (u & 7);
+    uint4* unit = reinterpret_cast<uint4*>(rec + u * 16);
+    if (r > pos) *unit = make_uint4(0, 0, 0, 0);
+    else if (grown && r < pos) *unit = again16(*unit, again);
+  }
+  uint8_t* k_row = rec + (pos >= 8 ? 8 * D : 0) + (pos & 7) * 16;
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+    if (2 * (lane + 32 * n) < D) {
+      const uint32_t two = bad_k ? 0x7f7fu : codes2(x[n] * down_k, y[n] * down_k);
+      k_row[(ix[n] >> 4) * 128 + (ix[n] & 15)] = (uint8_t)two;
+      k_row[(iy[n] >> 4) * 128 + (iy[n] & 15)] = (uint8_t)(two >> 8);
+    }
+  if (lane == 0) emit_tail(rec + kBlock * (D + V), ek, ev);
 }
 
 struct WideArgs {
@@ -396,6 +519,14 @@ __global__ void __launch_bounds__(kAppendWarps * 32, N <= 2 ? 4 : 2) kv8_append_
   const int items = __popc(leads) * G, ld_t = half + 2;
   const int pos_rows = min(kTurnRows, a.T - w0);
   if (part * kAppendWarps >= items) return;
+  if (!on) {
+    // no two tokens of the window share a record: a token at a time, in few instructions (a call of a few tokens spends its time on fetching them)
+    for (int it = part * kAppendWarps + warp; it < items; it += f.rec_parts * kAppendWarps) {
+      const int tok = (int)__fns(leads, 0, it / G + 1);
+      append_one<N>(qkv + (size_t)(w0 + tok) * a.ld, bias, a, w0 + tok, it % G, lane);
+    }
+    return;
+  }
   bool table = false;
   for (int at = part * kAppendWarps; at < items; at += f.rec_parts * kAppendWarps) {
     const int it = at + warp;
