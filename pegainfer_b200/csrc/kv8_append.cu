@@ -274,9 +274,9 @@ __global__ void __launch_bounds__(kAppendWarps * 32) kv8_append_kernel(const E* 
 constexpr int kTurnRows = 32;  // a window's tokens, and those of its last record
 
 // The angle, within half a turn, goes to the special-function unit: 2^-21 off, where the results are rounded to 2^-9 at best.  (With the library's sine and cosine two of
-// five instructions of the kernel were angles: 27.5 us for 4096 tokens, XX us so.)
-__device__ __forceinline__ float2 turn_of(int position, float freq, float mag) {
-  const double turns = (double)position * (double)freq * 0.15915494309189533577;
+// five instructions of the kernel were angles: 27.5 us for 4096 tokens, 26.5 us so.)
+__device__ __forceinline__ float2 turn_of(int position, double freq, float mag) {  // freq in turns
+  const double turns = (double)position * freq;
   const float angle = (float)(turns - rint(turns)) * 6.2831853071795865f;
   return make_float2(__cosf(angle) * mag, __sinf(angle) * mag);
 }
@@ -299,6 +299,15 @@ __device__ __forceinline__ void turn_pairs(float* x, float* y, const float2 (&cs
     }
   }
 }
+constexpr double kTurns = 0.15915494309189533577;  // 1 / 2 pi
+// the set bit that has n set bits below it
+__device__ __forceinline__ int nth_bit(uint32_t bits, int n) {
+  for (int i = 0; i < n; ++i) bits &= bits - 1u;
+  return __ffs(bits) - 1;
+}
+// the larger magnitude of bf16 pairs, as bits
+__device__ __forceinline__ uint32_t larger2(uint32_t most, uint32_t two) { return __vmaxu2(most, two & 0x7fff7fffu); }
+__device__ __forceinline__ uint32_t larger_of(uint32_t most) { return max(most >> 16, most & 0xffffu); }
 __device__ __forceinline__ void widen8(const uint4& u, float* v) {
   const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
@@ -379,7 +388,7 @@ __device__ __forceinline__ void append_one(const bf16* row, const bf16* bias, co
       }
       bad_k |= odd_one(x[n]) || odd_one(y[n]);
       if (p < half) {
-        cs[n] = turn_of(at, cs[n].x, a.mag);
+        cs[n] = turn_of(at, (double)cs[n].x * kTurns, a.mag);
         const float x0 = x[n], y0 = y[n];
         x[n] = x0 * cs[n].x - y0 * cs[n].y;
         y[n] = x0 * cs[n].y + y0 * cs[n].x;
@@ -448,7 +457,7 @@ struct WideArgs {
 };
 
 // N: 64ths of the larger width
-template <int N>
+template <int N, bool BIAS>
 __global__ void __launch_bounds__(kAppendWarps * 32, N <= 2 ? 4 : 2) kv8_append_wide_kernel(const bf16* __restrict__ qkv, const bf16* __restrict__ bias, bf16* __restrict__ q_out, const WideArgs f) {
   extern __shared__ __align__(16) float2 ap_turns[];  // [token][pair], rows 16 bytes apart from a multiple of the banks
   const AppendArgs& a = f.a;
@@ -479,7 +488,7 @@ __global__ void __launch_bounds__(kAppendWarps * 32, N <= 2 ? 4 : 2) kv8_append_
       if (h == h0 && turns) {
         const int at = a.positions[t];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) cs[k] = turn_of(at, a.freq[u * 8 + k], a.mag);
+        for (int k = 0; k < 8; ++k) cs[k] = turn_of(at, (double)a.freq[u * 8 + k] * kTurns, a.mag);
       }
 #pragma unroll
       for (int k = 0; k < 4; ++k)
@@ -487,7 +496,7 @@ __global__ void __launch_bounds__(kAppendWarps * 32, N <= 2 ? 4 : 2) kv8_append_
           float x[8], y[8];
           widen8(raw[k][0], x);
           widen8(raw[k][1], y);
-          if (bias) {
+          if constexpr (BIAS) {
             const bf16* b = bias + (h + k) * D;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
@@ -522,8 +531,8 @@ __global__ void __launch_bounds__(kAppendWarps * 32, N <= 2 ? 4 : 2) kv8_append_
   if (!on) {
     // no two tokens of the window share a record: a token at a time, in few instructions (a call of a few tokens spends its time on fetching them)
     for (int it = part * kAppendWarps + warp; it < items; it += f.rec_parts * kAppendWarps) {
-      const int tok = (int)__fns(leads, 0, it / G + 1);
-      append_one<N>(qkv + (size_t)(w0 + tok) * a.ld, bias, a, w0 + tok, it % G, lane);
+      const int tok = nth_bit(leads, it / G);
+      append_one<N>(qkv + (size_t)(w0 + tok) * a.ld, BIAS ? bias : nullptr, a, w0 + tok, it % G, lane);
     }
     return;
   }
@@ -531,7 +540,7 @@ __global__ void __launch_bounds__(kAppendWarps * 32, N <= 2 ? 4 : 2) kv8_append_
   for (int at = part * kAppendWarps; at < items; at += f.rec_parts * kAppendWarps) {
     const int it = at + warp;
     const bool busy = it < items;
-    const int g = it % G, tok = busy ? (int)__fns(leads, 0, it / G + 1) : 0;
+    const int g = it % G, tok = busy ? nth_bit(leads, it / G) : 0;
     const int slot = __shfl_sync(0xffffffffu, slot_l, tok), req = __shfl_sync(0xffffffffu, req_l, tok), first = slot & (kBlock - 1);
     const int count = busy ? __ffs(~(on >> (tok + 1))) : 0;  // the leader and those that go on behind it
     const uint32_t fresh = ((1u << count) - 1u) << first;
@@ -578,9 +587,10 @@ __global__ void __launch_bounds__(kAppendWarps * 32, N <= 2 ? 4 : 2) kv8_append_
         }
     }
     if (!table) {  // under the loads
-      for (int i = threadIdx.x; i < pos_rows * half; i += blockDim.x) {
-        const int r = i / half, k = i - r * half;
-        if (r < kWindow || on >> kWindow & 1) ap_turns[r * ld_t + k] = turn_of(a.positions[w0 + r], a.freq[k], a.mag);
+      const int rows = on >> kWindow & 1 ? pos_rows : n_tok;
+      for (int k = lane; k < half; k += 32) {
+        const double freq = (double)a.freq[k] * kTurns;
+        for (int r = warp; r < rows; r += kAppendWarps) ap_turns[r * ld_t + k] = turn_of(a.positions[w0 + r], freq, a.mag);
       }
       table = true;
       __syncthreads();
@@ -588,23 +598,54 @@ __global__ void __launch_bounds__(kAppendWarps * 32, N <= 2 ? 4 : 2) kv8_append_
     if (!busy) continue;
 
     // values
-    float b0[N], b1[N];
+    float b0[N] = {}, b1[N] = {};
     uint32_t bad = 0;
-#pragma unroll
-    for (int n = 0; n < N; ++n) {
-      const int d = 2 * lane + 64 * n;
-      b0[n] = bias && d < V ? to_f(bias[(H + G) * D + g * V + d]) : 0.f;
-      b1[n] = bias && d < V ? to_f(bias[(H + G) * D + g * V + d + 1]) : 0.f;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) bad |= (odd_one(bf16_lo(vr[n][r]) + b0[n]) || odd_one(bf16_hi(vr[n][r]) + b1[n]) ? 1u : 0u) << r;
-    }
-    const uint32_t bad_v = __reduce_or_sync(0xffffffffu, bad) & fresh, good_v = fresh & ~bad_v;
     float amax = 0.f;
+    auto value = [&](int n, int r, int k) { return k ? bf16_hi(vr[n][r]) + (BIAS ? b1[n] : 0.f) : bf16_lo(vr[n][r]) + (BIAS ? b0[n] : 0.f); };
+    uint32_t bad_v, good_v;
+    if constexpr (BIAS) {
 #pragma unroll
-    for (int n = 0; n < N; ++n)
+      for (int n = 0; n < N; ++n) {
+        const int d = 2 * lane + 64 * n;
+        b0[n] = d < V ? to_f(bias[(H + G) * D + g * V + d]) : 0.f;
+        b1[n] = d < V ? to_f(bias[(H + G) * D + g * V + d + 1]) : 0.f;
 #pragma unroll
-      for (int r = 0; r < 16; ++r)
-        if (good_v >> r & 1) amax = fmaxf(amax, fmaxf(fabsf(bf16_lo(vr[n][r]) + b0[n]), fabsf(bf16_hi(vr[n][r]) + b1[n])));
+        for (int r = 0; r < 16; ++r) bad |= (odd_one(value(n, r, 0)) || odd_one(value(n, r, 1)) ? 1u : 0u) << r;
+      }
+      bad_v = __reduce_or_sync(0xffffffffu, bad) & fresh, good_v = fresh & ~bad_v;
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (good_v >> r & 1) amax = fmaxf(amax, fmaxf(fabsf(value(n, r, 0)), fabsf(value(n, r, 1))));
+    } else {
+      uint32_t most = 0, all = 0, row[16];  // (all of them at most: mostly there is nothing that is not finite)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        row[r] = 0;
+#pragma unroll
+        for (int n = 0; n < N; ++n) row[r] = larger2(row[r], vr[n][r]);
+        all = __vmaxu2(all, row[r]);
+      }
+      if (__any_sync(0xffffffffu, larger_of(all) >= 0x7f80u)) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) bad |= (larger_of(row[r]) >= 0x7f80u ? 1u : 0u) << r;
+        bad = __reduce_or_sync(0xffffffffu, bad);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          if (bad >> r & 1) {
+#pragma unroll
+            for (int n = 0; n < N; ++n) vr[n][r] = 0;
+          } else {
+            most = __vmaxu2(most, row[r]);
+          }
+        }
+      } else {
+        most = all;
+      }
+      bad_v = bad & fresh, good_v = 0xffffu;  // (rows without a token, and bad ones, are zeros now)
+      amax = __uint_as_float(larger_of(most) << 16);
+    }
     const int had_v = tail_ev(tail), had_k = tail_ek(tail);
     int ev = exponent_for(warp_max(amax));
     if (first) ev = max(ev, had_v);
@@ -623,10 +664,7 @@ __global__ void __launch_bounds__(kAppendWarps * 32, N <= 2 ? 4 : 2) kv8_append_
           for (int x = 0; x < 4; ++x) {
             float y[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const uint32_t two = vr[n][4 * x + j];
-              y[j] = good_v >> (4 * x + j) & 1 ? (k ? bf16_hi(two) + b1[n] : bf16_lo(two) + b0[n]) * down : 0.f;
-            }
+            for (int j = 0; j < 4; ++j) y[j] = !BIAS || good_v >> (4 * x + j) & 1 ? value(n, 4 * x + j, k) * down : 0.f;
             w[x] = codes4(y[0], y[1], y[2], y[3]);
           }
           if (first) {
@@ -656,13 +694,18 @@ __global__ void __launch_bounds__(kAppendWarps * 32, N <= 2 ? 4 : 2) kv8_append_
       widen8(kr[n][3], y[n] + 8);
       if (!mine || p >= D / 32) continue;
       bool odd = false;
+      if constexpr (BIAS) {
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        if (bias) {
+        for (int j = 0; j < 16; ++j) {
           x[n][j] += to_f(bias[(H + g) * D + c0[n] * 16 + j]);
           y[n][j] += to_f(bias[(H + g) * D + c1[n] * 16 + j]);
+          odd |= odd_one(x[n][j]) || odd_one(y[n][j]);
         }
-        odd |= odd_one(x[n][j]) || odd_one(y[n][j]);
+      } else {
+        uint32_t most = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) most = larger2(larger2(larger2(larger2(most, kr[n][j].x), kr[n][j].y), kr[n][j].z), kr[n][j].w);
+        odd = larger_of(most) >= 0x7f80u;
       }
       if (odd) bad = 1u << pos;
       if (p < half / 16) {
@@ -720,7 +763,7 @@ static int append_wide(const bf16* qkv, const bf16* bias, bf16* q_out, const App
   while (f.by > 1 && units * ((a.H + f.by - 1) / f.by) < threads * 4 * sm_count()) f.by /= 2;
   const long ctas = a.H ? (units * ((a.H + f.by - 1) / f.by) + threads - 1) / threads : 0;
   const size_t smem = (size_t)kTurnRows * (a.dims / 2 + 2) * sizeof(float2);
-  return (int)launch(kv8_append_wide_kernel<N>, dim3((unsigned)(f.rec_ctas + ctas)), dim3((unsigned)threads), smem, st, true, qkv, bias, q_out, f);
+  return (int)launch(bias ? kv8_append_wide_kernel<N, true> : kv8_append_wide_kernel<N, false>, dim3((unsigned)(f.rec_ctas + ctas)), dim3((unsigned)threads), smem, st, true, qkv, bias, q_out, f);
 }
 
 }  // namespace kv8
