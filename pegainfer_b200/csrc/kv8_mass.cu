@@ -8,6 +8,7 @@
 
 #include "kv8_attention.cuh"
 #include "mma.cuh"
+#include "tcgen05.cuh"
 
 namespace pk {
 namespace kv8 {
@@ -25,6 +26,58 @@ __device__ __forceinline__ uint32_t bf16_of(uint32_t two) {
   return pack_bf16(v.x, v.y);
 }
 
+// ---- the runs, for all threads of a CTA alike
+struct Runs {
+  const uint32_t* starts;  // a bit per token that begins one
+  int words, T;
+  __device__ __forceinline__ int after(int t) const {  // the first run behind token t
+    int i = (t + 1) >> 5;
+    if (i >= words) return T;
+    uint32_t m = starts[i] & (0xffffffffu << ((t + 1) & 31));
+    while (m == 0 && ++i < words) m = starts[i];
+    return m ? i * 32 + __ffs(m) - 1 : T;
+  }
+};
+template <int WARPS>
+__device__ __forceinline__ Runs find_runs(uint32_t* starts, const AttnArgs& a) {
+  const int lane = threadIdx.x & 31, words = (a.T + 31) / 32;
+#pragma unroll 4
+  for (int i = threadIdx.x >> 5; i < words; i += WARPS) {
+    const int t = i * 32 + lane;
+    const bool begins = t < a.T && (t == 0 || a.req[t] != a.req[t - 1]);
+    const uint32_t all = __ballot_sync(0xffffffffu, begins);
+    if (lane == 0) starts[i] = all;
+  }
+  __syncthreads();
+  return Runs{starts, words, a.T};
+}
+// a run's largest and smallest slot, and where they are: slots ascend by one at least
+struct Ends {
+  int last, at_last, lowest, at_lowest;
+};
+template <int WARPS>
+__device__ __forceinline__ Ends run_ends(int4* s_run, const AttnArgs& a, int t0, int t1) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int last = -1, lowest = INT_MAX, at_last = -1, at_lowest = INT_MAX;
+  for (int t = t0 + (int)threadIdx.x; t < t1; t += WARPS * 32) {
+    const int p = a.slots[t];
+    if (p >= 0 && p >= last) last = p, at_last = t;
+    if (p >= 0 && p < lowest) lowest = p, at_lowest = t;
+  }
+  const int wl = __reduce_max_sync(0xffffffffu, last), ws = __reduce_min_sync(0xffffffffu, lowest);
+  const int al = __reduce_max_sync(0xffffffffu, last == wl ? at_last : -1), as = __reduce_min_sync(0xffffffffu, lowest == ws ? at_lowest : INT_MAX);
+  __syncthreads();  // (the words of a run before)
+  if (lane == 0) s_run[warp] = make_int4(wl, al, ws, as);
+  __syncthreads();
+  const int4 x = s_run[lane % WARPS];
+  Ends e;
+  e.last = __reduce_max_sync(0xffffffffu, x.x);
+  e.at_last = __reduce_max_sync(0xffffffffu, x.x == e.last ? x.y : -1);
+  e.lowest = __reduce_min_sync(0xffffffffu, x.z);
+  e.at_lowest = __reduce_min_sync(0xffffffffu, x.z == e.lowest ? x.w : INT_MAX);
+  return e;
+}
+
 template <int D, int RECS>
 __global__ void __launch_bounds__(kMassWarps * 32) kv8_mass_kernel(const bf16* __restrict__ q, AttnArgs a) {
   constexpr int LD = D + 8;
@@ -40,47 +93,13 @@ __global__ void __launch_bounds__(kMassWarps * 32) kv8_mass_kernel(const bf16* _
   const float c = a.scale * kLog2e, cap2 = a.cap * kLog2e, cap_c = a.cap > 0.f ? 2.f * a.scale / a.cap * kLog2e : 0.f;
   pdl_wait();
   pdl_launch_dependents();
-  // where runs begin
-  const int words = (a.T + 31) / 32;
-#pragma unroll 4
-  for (int i = warp; i < words; i += kMassWarps) {
-    const int t = i * 32 + lane;
-    const bool begins = t < a.T && (t == 0 || a.req[t] != a.req[t - 1]);
-    const uint32_t all = __ballot_sync(0xffffffffu, begins);
-    if (lane == 0) ms_starts[i] = all;
-  }
-  __syncthreads();
-  auto next_start = [&](int t) {  // the first run behind token t
-    int i = (t + 1) >> 5;
-    if (i >= words) return a.T;
-    uint32_t m = ms_starts[i] & (0xffffffffu << ((t + 1) & 31));
-    while (m == 0 && ++i < words) m = ms_starts[i];
-    return m ? i * 32 + __ffs(m) - 1 : a.T;
-  };
+  const Runs runs = find_runs<kMassWarps>(ms_starts, a);
   int nth = 0;
   for (int t0 = 0, t1 = 0; t0 < a.T; t0 = t1, ++nth) {
-    t1 = next_start(t0);
+    t1 = runs.after(t0);
     if (nth % (int)gridDim.z != (int)blockIdx.z) continue;
     const int req = a.req[t0];
-    // the run's largest and smallest slot, and where they are: slots ascend by one at least
-    int last = -1, lowest = INT_MAX, at_last = -1, at_lowest = INT_MAX;
-    for (int t = t0 + (int)threadIdx.x; t < t1; t += kMassWarps * 32) {
-      const int p = a.slots[t];
-      if (p >= 0 && p >= last) last = p, at_last = t;
-      if (p >= 0 && p < lowest) lowest = p, at_lowest = t;
-    }
-    {
-      const int wl = __reduce_max_sync(0xffffffffu, last), ws = __reduce_min_sync(0xffffffffu, lowest);
-      const int al = __reduce_max_sync(0xffffffffu, last == wl ? at_last : -1), as = __reduce_min_sync(0xffffffffu, lowest == ws ? at_lowest : INT_MAX);
-      __syncthreads();  // (the words of a run before)
-      if (lane == 0) s_run[warp] = make_int4(wl, al, ws, as);
-      __syncthreads();
-      const int4 x = s_run[lane % kMassWarps];
-      last = __reduce_max_sync(0xffffffffu, x.x);
-      at_last = __reduce_max_sync(0xffffffffu, x.x == last ? x.y : -1);
-      lowest = __reduce_min_sync(0xffffffffu, x.z);
-      at_lowest = __reduce_min_sync(0xffffffffu, x.z == lowest ? x.w : INT_MAX);
-    }
+    const auto [last, at_last, lowest, at_lowest] = run_ends<kMassWarps>(s_run, a, t0, t1);
     if (key0 > last || (a.window > 0 && key1 <= lowest - a.window)) continue;  // (for all threads alike)
 
     // the warp's keys: a product's 16 tokens are a record's, its inner index the entries in order
@@ -192,6 +211,189 @@ __global__ void __launch_bounds__(kMassWarps * 32) kv8_mass_kernel(const bf16* _
   }
 }
 
+// ---- the same on tcgen05: S^T of 128 keys x 128 rows in tensor memory, K as bf16 and the rows of q as they are in shared memory (128-byte swizzle).  A thread has a key and
+// half of the rows: the exponent is one number, the sums need no exchange until the end.  The product of the next tile runs under the exponentials of this one, which bound
+// it (one per score, 16 a clock and SM); two CTAs to an SM cover one another's waits.
+constexpr int kWideKeys = 128, kWideRows = 128, kWideWarps = 8;
+
+template <int D>
+__global__ void __launch_bounds__(kWideWarps * 32, 2) kv8_mass_wide_kernel(const bf16* __restrict__ q, AttnArgs a, unsigned int* err) {
+  constexpr int HALF = 128 * 128, TILE = HALF * (D / 64);  // bytes of 64 entries of 128 rows, of an operand
+  extern __shared__ uint8_t mw_raw[];
+  uint8_t* ks = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(mw_raw) + 1023) & ~(uintptr_t)1023);
+  uint8_t* qs = ks + TILE;  // [2]
+  __shared__ __align__(16) float s_neg[4][kWideRows];  // -lse in log2; -inf: no such row.  (Four: a tile's are read while the next but one's come.)
+  __shared__ __align__(16) int s_p[4][kWideRows];
+  __shared__ int s_all[4][kWideRows / 32];  // whether 32 rows see every key of the CTA
+  __shared__ uint32_t ms_starts[kMassTokens / 32];
+  __shared__ int4 s_run[kWideWarps];
+  __shared__ uint64_t s_full[2], drained;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int s_dead;
+  volatile int* dead = &s_dead;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = blockIdx.y, R = a.H / a.pool.G, V = a.pool.vdim;
+  const int key0 = blockIdx.x * kWideKeys, key1 = key0 + kWideKeys - 1;
+  const int key = key0 + (warp & 3) * 32 + lane, col0 = (warp >> 2) * 64;
+  const float cap2 = a.cap * kLog2e, cap_c = a.cap > 0.f ? 2.f * a.scale / a.cap * kLog2e : 0.f;
+  if (tid == 0) {
+    mbar_init(s_full, 1);
+    mbar_init(s_full + 1, 1);
+    mbar_init(&drained, 1);
+    s_dead = 0;
+    mbar_fence_init();
+  }
+  if (warp == 0) tmem_alloc(&tmem_slot, 2 * kWideRows);
+  pdl_wait();
+  pdl_launch_dependents();
+  tc_fence_before();
+  const Runs runs = find_runs<kWideWarps>(ms_starts, a);  // (a barrier)
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  WaitTries tries;
+  int nth = 0, n = 0;  // n: tiles so far
+  for (int t0 = 0, t1 = 0; t0 < a.T; t0 = t1, ++nth) {
+    t1 = runs.after(t0);
+    if (nth % (int)gridDim.z != (int)blockIdx.z) continue;
+    const int req = a.req[t0];
+    const auto [last, at_last, lowest, at_lowest] = run_ends<kWideWarps>(s_run, a, t0, t1);
+    if (key0 > last || (a.window > 0 && key1 <= lowest - a.window)) continue;  // (for all threads alike)
+    // rows that see none of the CTA's keys: before token `from`, and from token `to` on where there is a window
+    const int rows = (t1 - t0) * R, tiles = (rows + kWideRows - 1) / kWideRows;
+    const int from = max(t0, at_last - (last - key0)), to = a.window > 0 ? (int)min((long)t1, (long)at_lowest + (key1 + (long)a.window - lowest)) : t1;
+    const int tile0 = (int)((long)(from - t0) * R / kWideRows), count = min(tiles, (int)(((long)(to - t0) * R + kWideRows - 1) / kWideRows)) - tile0;
+    auto load = [&](int i) {  // the run's i-th tile
+      uint8_t* dst = qs + (size_t)((n + i) & 1) * TILE;
+      const int at0 = (tile0 + i) * kWideRows;
+#pragma unroll 4
+      for (int x = tid; x < kWideRows * (D / 8); x += kWideWarps * 32) {
+        const int row = x / (D / 8), piece = x % (D / 8), at = min(at0 + row, rows - 1), t = t0 + at / R;
+        cp_async16(dst + (piece >> 3) * HALF + row * 128 + (((piece & 7) ^ (row & 7)) << 4), q + ((size_t)t * a.H + g * R + at % R) * D + piece * 8);
+      }
+      cp_async_commit();
+      if (tid < kWideRows) {
+        const int at = at0 + tid, t = t0 + min(at, rows - 1) / R, p = at < rows ? a.slots[t] : -1, s = (n + i) & 3;
+        s_p[s][tid] = p;
+        s_neg[s][tid] = p >= 0 ? a.lse[(size_t)t * a.H + g * R + at % R] * -kLog2e : -INFINITY;
+        const bool all = __all_sync(0xffffffffu, p >= key1 && (a.window <= 0 || key0 > p - a.window));
+        if (lane == 0) s_all[s][warp] = all;
+      }
+    };
+    if (count > 0) load(0);
+    // the keys
+#pragma unroll 4
+    for (int x = tid; x < kWideKeys * (D / 16); x += kWideWarps * 32) {
+      const int r = x / D, u = x % D, row = r * kBlock + (u >= D / 2 ? 8 : 0) + (u & 7), c = (u % (D / 2)) >> 3;
+      uint32_t w[8] = {};
+      if (key0 + r * kBlock <= last) {
+        const uint4 codes = *reinterpret_cast<const uint4*>(a.pool.record(req, key0 + r * kBlock, g) + u * 16);
+        const uint32_t four[4] = {codes.x, codes.y, codes.z, codes.w};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = bf16_of(four[i / 2] >> (i % 2 * 16) & 0xffffu);
+      }
+      uint8_t* dst = ks + (c >> 2) * HALF + row * 128;
+      *reinterpret_cast<uint4*>(dst + (((c & 3) * 2 ^ (row & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+      *reinterpret_cast<uint4*>(dst + (((c & 3) * 2 + 1 ^ (row & 7)) << 4)) = make_uint4(w[4], w[5], w[6], w[7]);
+    }
+    float fk = 0.f;
+    if (key / kBlock <= last / kBlock)
+      fk = pow2(tail_ek(*reinterpret_cast<const uint32_t*>(a.pool.record(req, key, g) + kBlock * (D + V)))) * (a.cap > 0.f ? cap_c : a.scale * kLog2e);
+
+    float sum0 = 0.f, sum1 = 0.f;
+    for (int i = 0; i <= count; ++i) {
+      if (i < count) {
+        cp_async_wait_all();
+        fence_proxy_async_smem();
+        tc_fence_before();
+        __syncthreads();
+        if (warp == 0 && tc_elect_one()) {
+          tc_fence_after();
+          constexpr uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(kWideRows >> 3) << 17) | ((uint32_t)(kWideKeys >> 4) << 24);  // bf16 x bf16 -> fp32
+          const uint64_t kd = make_sw128_desc(smem_u32(ks)), qd = make_sw128_desc(smem_u32(qs + (size_t)((n + i) & 1) * TILE));
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k)
+            umma_bf16(tmem + (uint32_t)(((n + i) & 1) * kWideRows), kd + (uint64_t)((k >> 2) * (HALF >> 4) + (k & 3) * 2), qd + (uint64_t)((k >> 2) * (HALF >> 4) + (k & 3) * 2), idesc, k > 0 ? 1u : 0u);
+          umma_commit(s_full + ((n + i) & 1));
+        }
+        __syncwarp();
+      }
+      const int m = n + i - 1, s = m & 3;  // the tile before
+      if (i > 0) {
+        mbar_wait_bounded(s_full + (m & 1), (uint32_t)((m >> 1) & 1), dead, tries);
+        tc_fence_after();
+      }
+      if (i + 1 < count) load(i + 1);  // its place was the tile before's
+      if (i == 0) continue;
+      uint32_t v[64];
+      tmem_ld64(tmem + (uint32_t)((m & 1) * kWideRows + col0) + ((uint32_t)((warp & 3) * 32) << 16), v);
+      const bool whole = s_all[s][col0 / 32] && s_all[s][col0 / 32 + 1];
+      if (a.cap > 0.f) {
+#pragma unroll
+        for (int j = 0; j < 64; ++j)
+          v[j] = __float_as_uint(fmaf(-2.f * cap2, __fdividef(1.f, ms_ex2(at_most80(__uint_as_float(v[j]) * fk)) + 1.f), cap2));
+      }
+      const float f = a.cap > 0.f ? 1.f : fk;
+      if (whole) {
+#pragma unroll
+        for (int j = 0; j < 64; j += 4) {
+          const float4 neg = *reinterpret_cast<const float4*>(&s_neg[s][col0 + j]);
+          sum0 += ms_ex2(fmaf(__uint_as_float(v[j]), f, neg.x));
+          sum1 += ms_ex2(fmaf(__uint_as_float(v[j + 1]), f, neg.y));
+          sum0 += ms_ex2(fmaf(__uint_as_float(v[j + 2]), f, neg.z));
+          sum1 += ms_ex2(fmaf(__uint_as_float(v[j + 3]), f, neg.w));
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 64; ++j) {
+          const int p = s_p[s][col0 + j];
+          const float w = ms_ex2(fmaf(__uint_as_float(v[j]), f, s_neg[s][col0 + j]));
+          (j & 1 ? sum1 : sum0) += key <= p && (a.window <= 0 || key > p - a.window) ? w : 0.f;
+        }
+      }
+    }
+    n += max(count, 0);
+    // both halves of the rows
+    sum0 += sum1;
+    __syncthreads();
+    float* other = reinterpret_cast<float*>(ks);  // (the products are done)
+    if (warp >= 4) other[tid - 128] = sum0;
+    __syncthreads();
+    if (warp < 4 && key <= last && key < a.mass_ld) a.mass[((size_t)req * a.pool.G + g) * a.mass_ld + key] += *dead ? NAN : sum0 + other[tid];
+    tc_fence_before();
+    __syncthreads();  // the next run's keys may come
+    tc_fence_after();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (*dead) {  // (for all alike, behind the barrier)
+    if (warp == 0) {
+      if (tc_elect_one()) umma_commit(&drained);
+      __syncwarp();
+      mbar_drain(&drained, 0);
+    }
+    __syncthreads();
+  }
+  if (warp == 0) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 2 * kWideRows);
+  }
+  if (tid == 0) count_run_out(dead, err);
+}
+
+template <int D>
+static int launch_mass_wide(const bf16* q, const AttnArgs& a, int runs, cudaStream_t st) {
+  constexpr size_t smem = 1024 + (size_t)3 * 256 * D;
+  static std::atomic<uint64_t> set{0};
+  if (const cudaError_t e = allow_smem(set, (const void*)kv8_mass_wide_kernel<D>, smem); e != cudaSuccess) return (int)e;
+  const long span = std::min((long)a.max_kv_len, a.mass_ld);
+  ThreadState& ts = tls();
+  const bool pdl = ts.pdl;
+  ts.pdl = true;  // behind a kernel of the same call
+  const cudaError_t e = launch(kv8_mass_wide_kernel<D>, dim3((unsigned)((span + kWideKeys - 1) / kWideKeys), a.pool.G, std::max(1, std::min(runs, 16))), dim3(kWideWarps * 32), smem, st, true, q, a,
+                               wait_err_word());
+  ts.pdl = pdl;
+  return (int)e;
+}
+
 template <int D, int RECS>
 static int launch_mass(const bf16* q, const AttnArgs& a, int runs, cudaStream_t st) {
   constexpr size_t smem = (size_t)2 * kMassRows * (D + 8) * sizeof(bf16);
@@ -221,9 +423,9 @@ int mass_rows_mma(const bf16* q, const AttnArgs& a, int max_q_len, cudaStream_t 
   const int runs = max_q_len > 0 ? (a.T + max_q_len - 1) / max_q_len : 4;  // at least; unknown: some
   switch (a.pool.dim) {
     case 32: return launch_mass<32>(q, a, runs, st);
-    case 64: return launch_mass<64>(q, a, runs, st);
+    case 64: return launch_mass_wide<64>(q, a, runs, st);
     case 96: return launch_mass<96>(q, a, runs, st);
-    case 128: return launch_mass<128>(q, a, runs, st);
+    case 128: return launch_mass_wide<128>(q, a, runs, st);
     case 192: return launch_mass<192>(q, a, runs, st);
     default: return launch_mass<256>(q, a, runs, st);
   }
