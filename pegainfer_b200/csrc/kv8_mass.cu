@@ -214,6 +214,23 @@ __global__ void __launch_bounds__(kMassWarps * 32) kv8_mass_kernel(const bf16* _
 // ---- the same on tcgen05: S^T of 128 keys x 128 rows in tensor memory, K as bf16 and the rows of q as they are in shared memory (128-byte swizzle).  A thread has a key and
 // half of the rows: the exponent is one number, the sums need no exchange until the end.  The product of the next tile runs under the exponentials of this one, which bound
 // it (one per score, 16 a clock and SM); two CTAs to an SM cover one another's waits.
+// {s0, s1} += 2^(x f + n), two at a time
+__device__ __forceinline__ void add_weights(float& s0, float& s1, uint32_t x0, uint32_t x1, float f, float n0, float n1) {
+  unsigned long long x, y, z;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "r"(x0), "r"(x1));
+  asm("mov.b64 %0, {%1, %1};" : "=l"(y) : "f"(f));
+  asm("mov.b64 %0, {%1, %2};" : "=l"(z) : "f"(n0), "f"(n1));
+  asm("fma.rn.f32x2 %0, %0, %1, %2;" : "+l"(x) : "l"(y), "l"(z));
+  float w0, w1;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(w0), "=f"(w1) : "l"(x));
+  w0 = ms_ex2(w0);
+  w1 = ms_ex2(w1);
+  asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(w0), "f"(w1));
+  asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "f"(s0), "f"(s1));
+  asm("add.rn.f32x2 %0, %0, %1;" : "+l"(y) : "l"(x));
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(s0), "=f"(s1) : "l"(y));
+}
+
 constexpr int kWideKeys = 128, kWideRows = 128, kWideWarps = 8;
 
 template <int D>
@@ -250,6 +267,7 @@ __global__ void __launch_bounds__(kWideWarps * 32, 2) kv8_mass_wide_kernel(const
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
   WaitTries tries;
+  const unsigned long long r_inv = (1ull << 32) / (unsigned)R + 1;  // at / R is exact for at < 2^32 / R
   int nth = 0, n = 0;  // n: tiles so far
   for (int t0 = 0, t1 = 0; t0 < a.T; t0 = t1, ++nth) {
     t1 = runs.after(t0);
@@ -261,20 +279,32 @@ __global__ void __launch_bounds__(kWideWarps * 32, 2) kv8_mass_wide_kernel(const
     const int rows = (t1 - t0) * R, tiles = (rows + kWideRows - 1) / kWideRows;
     const int from = max(t0, at_last - (last - key0)), to = a.window > 0 ? (int)min((long)t1, (long)at_lowest + (key1 + (long)a.window - lowest)) : t1;
     const int tile0 = (int)((long)(from - t0) * R / kWideRows), count = min(tiles, (int)(((long)(to - t0) * R + kWideRows - 1) / kWideRows)) - tile0;
+    const bf16* q_run = q + ((size_t)t0 * a.H + g * R) * D;
+    auto by_r = [&](int at) { return (int)((unsigned long long)(uint32_t)at * r_inv >> 32); };
+    int next_p = -1;
+    float next_lse = INFINITY;
     auto load = [&](int i) {  // the run's i-th tile
       uint8_t* dst = qs + (size_t)((n + i) & 1) * TILE;
       const int at0 = (tile0 + i) * kWideRows;
 #pragma unroll 4
       for (int x = tid; x < kWideRows * (D / 8); x += kWideWarps * 32) {
-        const int row = x / (D / 8), piece = x % (D / 8), at = min(at0 + row, rows - 1), t = t0 + at / R;
-        cp_async16(dst + (piece >> 3) * HALF + row * 128 + (((piece & 7) ^ (row & 7)) << 4), q + ((size_t)t * a.H + g * R + at % R) * D + piece * 8);
+        const int row = x / (D / 8), piece = x % (D / 8), at = min(at0 + row, rows - 1);
+        cp_async16(dst + (piece >> 3) * HALF + row * 128 + (((piece & 7) ^ (row & 7)) << 4), q_run + ((size_t)by_r(at) * (a.H - R) + at) * D + piece * 8);
       }
       cp_async_commit();
+      next_p = -1, next_lse = INFINITY;
+      if (tid < kWideRows && at0 + tid < rows) {
+        const int at = at0 + tid, t = by_r(at);
+        next_p = a.slots[t0 + t];
+        next_lse = a.lse[(size_t)(t0 + t) * a.H + g * R + at - t * R];
+      }
+    };
+    auto put = [&](int i) {  // and what came with it, a tile's exponentials later
       if (tid < kWideRows) {
-        const int at = at0 + tid, t = t0 + min(at, rows - 1) / R, p = at < rows ? a.slots[t] : -1, s = (n + i) & 3;
-        s_p[s][tid] = p;
-        s_neg[s][tid] = p >= 0 ? a.lse[(size_t)t * a.H + g * R + at % R] * -kLog2e : -INFINITY;
-        const bool all = __all_sync(0xffffffffu, p >= key1 && (a.window <= 0 || key0 > p - a.window));
+        const int s = (n + i) & 3;
+        s_p[s][tid] = next_p;
+        s_neg[s][tid] = next_p >= 0 ? next_lse * -kLog2e : -INFINITY;
+        const bool all = __all_sync(0xffffffffu, next_p >= key1 && (a.window <= 0 || key0 > next_p - a.window));
         if (lane == 0) s_all[s][warp] = all;
       }
     };
@@ -301,6 +331,7 @@ __global__ void __launch_bounds__(kWideWarps * 32, 2) kv8_mass_wide_kernel(const
     float sum0 = 0.f, sum1 = 0.f;
     for (int i = 0; i <= count; ++i) {
       if (i < count) {
+        put(i);
         cp_async_wait_all();
         fence_proxy_async_smem();
         tc_fence_before();
@@ -336,10 +367,8 @@ __global__ void __launch_bounds__(kWideWarps * 32, 2) kv8_mass_wide_kernel(const
 #pragma unroll
         for (int j = 0; j < 64; j += 4) {
           const float4 neg = *reinterpret_cast<const float4*>(&s_neg[s][col0 + j]);
-          sum0 += ms_ex2(fmaf(__uint_as_float(v[j]), f, neg.x));
-          sum1 += ms_ex2(fmaf(__uint_as_float(v[j + 1]), f, neg.y));
-          sum0 += ms_ex2(fmaf(__uint_as_float(v[j + 2]), f, neg.z));
-          sum1 += ms_ex2(fmaf(__uint_as_float(v[j + 3]), f, neg.w));
+          add_weights(sum0, sum1, v[j], v[j + 1], f, neg.x, neg.y);
+          add_weights(sum0, sum1, v[j + 2], v[j + 3], f, neg.z, neg.w);
         }
       } else {
 #pragma unroll
@@ -421,11 +450,16 @@ bool mass_takes(const bf16* q, int T, int dim, int vdim) {
 }
 int mass_rows_mma(const bf16* q, const AttnArgs& a, int max_q_len, cudaStream_t st) {
   const int runs = max_q_len > 0 ? (a.T + max_q_len - 1) / max_q_len : 4;  // at least; unknown: some
+  const long R = a.H / a.pool.G;
+  if (a.T * R * R < 1L << 32) {  // (rows are divided by R through a product)
+    if (a.pool.dim == 64) return launch_mass_wide<64>(q, a, runs, st);
+    if (a.pool.dim == 128) return launch_mass_wide<128>(q, a, runs, st);
+  }
   switch (a.pool.dim) {
     case 32: return launch_mass<32>(q, a, runs, st);
-    case 64: return launch_mass_wide<64>(q, a, runs, st);
+    case 64: return launch_mass<64>(q, a, runs, st);
     case 96: return launch_mass<96>(q, a, runs, st);
-    case 128: return launch_mass_wide<128>(q, a, runs, st);
+    case 128: return launch_mass<128>(q, a, runs, st);
     case 192: return launch_mass<192>(q, a, runs, st);
     default: return launch_mass<256>(q, a, runs, st);
   }
