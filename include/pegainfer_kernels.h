@@ -730,7 +730,7 @@ int pk_logistic_decay(float* z, const float* bias, float tau, int tokens, int ch
 /* Bytes of a page; -1: sizes that the cache does not have */
 long pk_kv8_page_bytes(int page_size, int kv_heads, int dim, int vdim);
 /* qkv [tokens, ld] = [q (heads*dim) | k (kv_heads*dim) | v (kv_heads*vdim)] (+ bias of the same layout, may be NULL): q and k rotate over their first `dims`
- * entries by positions[t] * freq[i] as in pk_gqa_rope_append (angles are reduced in 64 bits); q goes to q_out [tokens, heads*dim], k and v into the cache at
+ * entries by positions[t] * freq[i] as in pk_gqa_rope_append (angles are reduced in 64 bits; sine and cosine are off by 2^-20 at most where the rows are bf16); q goes to q_out [tokens, heads*dim], k and v into the cache at
  * slots[t] (slots NULL: at positions[t]).  heads may be 0 (rows of k and v alone, q_out NULL).  A request's tokens are consecutive rows with consecutive slots,
  * in one run per call.  A token at a record's first slot begins the record anew (slots behind the call's last are zero); else the record goes on from the slots
  * before, whose codes are rounded again where its exponent grows.  Rows with a negative slot are not cached (their q is rotated all the same). */
@@ -741,7 +741,7 @@ int pk_kv8_append(const void* qkv, int ld, const void* bias, const int* position
 typedef struct pk_kv8_options {
   int window;      /* the query at slot p sees slots p - window + 1 .. p */
   float softcap;   /* scaled score <- softcap * tanh(score / softcap) */
-  int max_kv_len;  /* no query's slot is max_kv_len or more */
+  int max_kv_len;  /* no query's slot is max_kv_len or more; 2^30 at most */
   int max_q_len;   /* no request has more tokens in the call (0: unknown): a hint for the choice of a kernel */
   long out_ld;     /* elements from one row of out to the next (0: heads * vdim) */
   float* lse;      /* [tokens, heads]: log(sum over the visible slots of exp(score), plus exp(sink)); -inf where there is neither */
@@ -760,7 +760,7 @@ int pk_kv8_attention(const void* q, const void* cache, const void* sink, const i
  * largest mass (equal: the lower slot; NaN least).  They move, in order, to the pages of new_pages / new_page_off (other pages of the same pool, room for
  * min(lens[r], budget) slots each), into records with exponents of their own; the old pages are left as they were.  kept [requests, kv_heads, budget]: the
  * old slot of each new one, -1 behind the last; new_mass [requests, kv_heads, new_mass_ld]: the masses of the kept, zero behind; new_lens[r]: slots kept.
- * keep_first + keep_recent <= budget; mass_ld >= max_kv_len, new_mass_ld >= budget.  New tokens go on at slot new_lens[r] with their true positions. */
+ * new_lens, new_mass and new_pages are other arrays than the old ones.  keep_first + keep_recent <= budget; max_kv_len <= 2^30; mass_ld >= max_kv_len, new_mass_ld >= budget.  New tokens go on at slot new_lens[r] with their true positions. */
 int pk_kv8_evict(void* cache, long page_stride, int page_size, const int* page_off, const int* pages, const int* lens, const float* mass, long mass_ld,
                  const int* new_page_off, const int* new_pages, int* new_lens, float* new_mass, long new_mass_ld, int* kept, int requests, int kv_heads,
                  int dim, int vdim, int budget, int keep_first, int keep_recent, int max_kv_len, pk_stream st);

@@ -22,6 +22,7 @@ namespace pk {
 namespace kv8 {
 
 constexpr int kBlock = 16;           // tokens of a record
+constexpr int kMaxSlots = 1 << 30;   // of a request
 constexpr int kLowExp = -110, kHighExp = 120;
 
 __host__ __device__ inline int record_bytes(int dim, int vdim) { return kBlock * (dim + vdim) + 16; }

@@ -213,6 +213,8 @@ struct Plan {
   size_t o_bytes, ml_bytes, lse_bytes;
   long bytes() const { return (long)((few ? need.bytes() : o_bytes + ml_bytes) + lse_bytes); }
 };
+// slots are below max_kv_len: a window of that or more hides nothing
+static int window_of(const pk_kv8_options& o) { return o.window < o.max_kv_len ? o.window : 0; }
 static size_t up16(size_t n) { return (n + 15) / 16 * 16; }
 static Plan plan(int T, int H, int G, int dim, int vdim, const pk_kv8_options& o, int f32) {
   Plan p{};
@@ -224,10 +226,10 @@ static Plan plan(int T, int H, int G, int dim, int vdim, const pk_kv8_options& o
   }
   if (!f32 && prompt_takes(T, H, G, dim, vdim)) {
     p.prompt = true;
-    p.shares = prompt_shares(T, H, G, o.max_kv_len, o.window);
+    p.shares = prompt_shares(T, H, G, o.max_kv_len, window_of(o));
   } else {
     int span = o.max_kv_len;
-    if (o.window > 0) span = std::min(span, o.window + kBlock);
+    if (window_of(o) > 0) span = std::min(span, window_of(o) + kBlock);
     const int records = (span + kBlock - 1) / kBlock;
     // a share has at least two rounds of its warps
     p.shares = (int)std::max(1L, std::min((long)(records + 2 * kRowWarps - 1) / (2 * kRowWarps), (4L * sm_count() + (long)T * H - 1) / ((long)T * H)));
@@ -257,7 +259,7 @@ static int attention(const E* q, const E* sink, E* out, const AttnArgs& a, const
 }
 
 static bool options_ok(const pk_kv8_options* o, int tokens, int heads, int kv_heads, int vdim) {
-  return o && tokens > 0 && heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && heads <= 65535 && o->window >= 0 && o->softcap >= 0.f && o->max_kv_len > 0 &&
+  return o && tokens > 0 && heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && heads <= 65535 && o->window >= 0 && o->softcap >= 0.f && o->max_kv_len > 0 && o->max_kv_len <= kMaxSlots &&
          o->max_q_len >= 0 && (o->out_ld == 0 || o->out_ld >= (long)heads * vdim) && (!o->mass || o->mass_ld > 0);
 }
 
@@ -288,7 +290,7 @@ extern "C" int pk_kv8_attention(const void* q, const void* cache, const void* si
   a.H = heads;
   a.scale = scale;
   a.cap = options->softcap;
-  a.window = options->window;
+  a.window = kv8::window_of(*options);
   a.max_kv_len = options->max_kv_len;
   a.out_ld = options->out_ld ? options->out_ld : (long)heads * vdim;
   a.lse = options->lse ? options->lse : options->mass ? reinterpret_cast<float*>(ws) : nullptr;

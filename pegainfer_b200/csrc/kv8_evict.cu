@@ -8,6 +8,7 @@
 //   kv8_move_kernel   a warp to a new record.  Bound by the bytes it has to look at: a token's V lies in every 16-byte row of its record, so nearly the whole old cache is
 //                     read where a quarter of it is kept.  A source record's V is loaded once for all its kept tokens (rows of 16 tokens a lane), codes whose exponent
 //                     stays are moved as they are.
+// B200, 16 requests of 16384, 8 kv heads of 128 in both, to 4096: 24 us and 109; the sources' V rows and the kept K rows are 0.5 GB, 4.6 TB/s.
 #include <algorithm>
 
 #include "kv8.cuh"
@@ -324,8 +325,8 @@ extern "C" int pk_kv8_evict(void* cache, long page_stride, int page_size, const 
                             const int* new_page_off, const int* new_pages, int* new_lens, float* new_mass, long new_mass_ld, int* kept, int requests, int kv_heads,
                             int dim, int vdim, int budget, int keep_first, int keep_recent, int max_kv_len, pk_stream st) {
   if (!cache || !page_off || !pages || !lens || !mass || !new_page_off || !new_pages || !new_lens || !new_mass || !kept || requests <= 0 || requests > 65535 ||
-      budget <= 0 || keep_first < 0 || keep_recent < 0 || (long)keep_first + keep_recent > budget || max_kv_len <= 0 || mass_ld < max_kv_len ||
-      new_mass_ld < budget || new_mass == mass || new_pages == pages || !kv8::sizes_ok(page_size, kv_heads, dim, vdim) || kv_heads > 65535 ||
+      budget <= 0 || keep_first < 0 || keep_recent < 0 || (long)keep_first + keep_recent > budget || max_kv_len <= 0 || max_kv_len > kv8::kMaxSlots || mass_ld < max_kv_len ||
+      new_mass_ld < budget || new_mass == mass || new_pages == pages || new_lens == lens || !kv8::sizes_ok(page_size, kv_heads, dim, vdim) || kv_heads > 65535 ||
       !kv8::pool_ok(cache, page_stride, page_size, kv_heads, dim, vdim))
     return -1;
   const kv8::EvictArgs a{kv8::make_pool(cache, page_stride, page_off, pages, page_size, kv_heads, dim, vdim),

@@ -53,7 +53,8 @@ def attend(lib, **change):
 
 @pytest.mark.parametrize("change", [
     dict(q=None), dict(cache=None), dict(slots=None), dict(req=None), dict(page_off=None), dict(pages=None), dict(out=None), dict(tokens=0), dict(heads=0), dict(heads=3),
-    dict(kv_heads=0), dict(dim=16), dict(vdim=320), dict(page_size=40), dict(options=None), dict(options=dict(max_kv_len=0)), dict(options=dict(window=-1)),
+    dict(kv_heads=0), dict(dim=16), dict(vdim=320), dict(page_size=40), dict(options=None), dict(options=dict(max_kv_len=0)), dict(options=dict(max_kv_len=2 ** 30 + 1)),
+    dict(options=dict(window=-1)),
     dict(options=dict(softcap=-1.0)), dict(options=dict(max_q_len=-1)), dict(options=dict(out_ld=255)), dict(options=dict(mass=P)), dict(cache=P + 4),
     dict(page_stride=16 * 128 + 16), dict(options=dict(mass=P, mass_ld=100), workspace=None), dict(options=dict(mass=P, mass_ld=100), workspace_bytes=8),
     dict(options=dict(mass=P, mass_ld=100), workspace=P + 4), dict(options=dict(max_kv_len=100000), workspace=None)])
@@ -68,14 +69,15 @@ def test_workspace_bytes(lib):
     assert lib.pk_kv8_attention_workspace_bytes(1, 4, 2, 64, 64, None, 0) == -1
 
 
-EVICT = dict(cache=P, page_stride=2 * (16 * 128 + 16), page_size=16, page_off=P, pages=P, lens=P, mass=P, mass_ld=100, new_page_off=P, new_pages=P + 512, new_lens=P,
+EVICT = dict(cache=P, page_stride=2 * (16 * 128 + 16), page_size=16, page_off=P, pages=P, lens=P, mass=P, mass_ld=100, new_page_off=P, new_pages=P + 512, new_lens=P + 768,
              new_mass=P + 256, new_mass_ld=50, kept=P, requests=1, kv_heads=2, dim=64, vdim=64, budget=50, keep_first=4, keep_recent=10, max_kv_len=100, st=None)
 
 
 @pytest.mark.parametrize("change", [
     *(dict([(k, None)]) for k in ("cache", "page_off", "pages", "lens", "mass", "new_page_off", "new_pages", "new_lens", "new_mass", "kept")),
     dict(requests=0), dict(requests=70000), dict(kv_heads=0), dict(dim=8), dict(vdim=33), dict(budget=0), dict(keep_first=-1), dict(keep_recent=-1), dict(keep_first=41),
-    dict(keep_first=2 ** 31 - 1, keep_recent=2 ** 31 - 1), dict(max_kv_len=0), dict(max_kv_len=101), dict(new_mass_ld=49), dict(new_mass=P), dict(new_pages=P),
+    dict(keep_first=2 ** 31 - 1, keep_recent=2 ** 31 - 1), dict(max_kv_len=0), dict(max_kv_len=101), dict(new_mass_ld=49), dict(new_mass=P), dict(new_pages=P), dict(new_lens=P),
+    dict(max_kv_len=2 ** 30 + 1, mass_ld=2 ** 31),
     dict(page_size=20), dict(cache=P + 1), dict(page_stride=16)])
 def test_evict_refuses(lib, change):
     assert lib.pk_kv8_evict(*{**EVICT, **change}.values()) == -1

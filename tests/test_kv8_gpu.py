@@ -281,6 +281,14 @@ def test_options(lib, steps, opts):
     check_attention(lib, steps, 6, 2, 64, mass=True, seed=1, **o)
 
 
+@pytest.mark.parametrize("steps", [[(1, 400), (3, 31)], [(100, 33), (40, 300)]], ids=["few", "prompts"])
+def test_window_that_hides_nothing(lib, steps):
+    """as long as the longest context, one token less than it, the largest number"""
+    for window in (433, 432, 2 ** 31 - 1):
+        check_attention(lib, steps, 8, 2, 64, mass=True, longest=433, window=window)
+        check_attention(lib, steps, 4, 2, 32, f32=True, mass=True, longest=433, window=window, seed=1)
+
+
 @pytest.mark.parametrize("V", [32, 64, 192])
 def test_values_of_another_width(lib, V):
     check_attention(lib, [(1, 333), (20, 40)], 8, 2, 128, V, mass=True)
