@@ -742,7 +742,8 @@ typedef struct pk_kv8_options {
   int window;      /* the query at slot p sees slots p - window + 1 .. p */
   float softcap;   /* scaled score <- softcap * tanh(score / softcap) */
   int max_kv_len;  /* no query's slot is max_kv_len or more; 2^30 at most */
-  int max_q_len;   /* no request has more tokens in the call (0: unknown): a hint for the choice of a kernel */
+  int max_q_len;   /* no request has more tokens in the call (1: decoded tokens): a hint for the choice of a kernel; with 0 (unknown) calls of up to 512
+                      tokens are taken for decoded ones, larger ones for prompts */
   long out_ld;     /* elements from one row of out to the next (0: heads * vdim) */
   float* lse;      /* [tokens, heads]: log(sum over the visible slots of exp(score), plus exp(sink)); -inf where there is neither */
   float* mass;     /* [requests, kv_heads, mass_ld]: mass[req[t]][g][j] += the weights of slot j in the rows of the call, over the heads of group g */

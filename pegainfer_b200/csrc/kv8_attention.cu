@@ -207,7 +207,7 @@ __global__ void __launch_bounds__(128) kv8_mass_row_kernel(const E* __restrict__
 
 // what a call runs: the shares of its keys and its workspace
 struct Plan {
-  bool few, prompt;  // kv8_few.cu, kv8_prompt.cu
+  bool few, prompt, tile;  // kv8_few.cu, kv8_prompt.cu, kv8_tile.cu
   FewNeed need;
   int shares;
   size_t o_bytes, ml_bytes, lse_bytes;
@@ -227,6 +227,9 @@ static Plan plan(int T, int H, int G, int dim, int vdim, const pk_kv8_options& o
   if (!f32 && prompt_takes(T, H, G, dim, vdim)) {
     p.prompt = true;
     p.shares = prompt_shares(T, H, G, o.max_kv_len, window_of(o));
+  } else if (tile_takes(T, H, G, o.max_q_len)) {
+    p.tile = true;
+    p.shares = tile_shares(T, H, G, o.max_kv_len, window_of(o));
   } else {
     int span = o.max_kv_len;
     if (window_of(o) > 0) span = std::min(span, window_of(o) + kBlock);
@@ -242,7 +245,9 @@ static Plan plan(int T, int H, int G, int dim, int vdim, const pk_kv8_options& o
 }
 
 template <typename E>
-static int mass_rows(const E* q, const AttnArgs& a, cudaStream_t st) {
+static int mass_rows(const E* q, const AttnArgs& a, int max_q_len, cudaStream_t st) {
+  if constexpr (sizeof(E) == 2)
+    if (mass_takes(q, a.T, a.pool.dim)) return mass_rows_mma(q, a, max_q_len, st);
   return (int)follow(kv8_mass_row_kernel<E>, dim3((a.max_kv_len + 63) / 64, a.pool.G), dim3(128), st, q, a);
 }
 template <typename E>
@@ -250,12 +255,18 @@ static int merge(const E* sink, E* out, int shares, const AttnArgs& a, cudaStrea
   return (int)follow(kv8_merge_kernel<E>, dim3((unsigned)(((size_t)a.T * a.H + 3) / 4)), dim3(128), st, sink, out, shares, a);
 }
 template <typename E>
-static int attention(const E* q, const E* sink, E* out, const AttnArgs& a, const Plan& p, cudaStream_t st) {
+static int attention(const E* q, const E* sink, E* out, const AttnArgs& a, const Plan& p, int max_q_len, cudaStream_t st) {
+  if (p.tile) {
+    if (const int rc = tile_attention(q, sink, out, a, p.shares, st); rc != 0) return rc;
+    if (p.shares > 1)
+      if (const int rc = merge(sink, out, p.shares, a, st); rc != 0) return rc;
+    return a.mass ? mass_rows(q, a, max_q_len, st) : 0;
+  }
   const size_t smem = (size_t)(a.pool.dim + kRowWarps * a.pool.vdim) * sizeof(float);
   if (const cudaError_t e = launch(kv8_row_kernel<E>, dim3(a.T, a.H, p.shares), dim3(kRowWarps * 32), smem, st, true, q, sink, out, a); e != cudaSuccess) return (int)e;
   if (p.shares > 1)
     if (const int rc = merge(sink, out, p.shares, a, st); rc != 0) return rc;
-  return a.mass ? mass_rows(q, a, st) : 0;
+  return a.mass ? mass_rows(q, a, max_q_len, st) : 0;
 }
 
 static bool options_ok(const pk_kv8_options* o, int tokens, int heads, int kv_heads, int vdim) {
@@ -304,8 +315,8 @@ extern "C" int pk_kv8_attention(const void* q, const void* cache, const void* si
     int rc = kv8::prompt_attention((const bf16*)q, (const bf16*)sink, (bf16*)out, a, p.shares, st);
     if (rc == 0 && p.shares > 1) rc = kv8::merge((const bf16*)sink, (bf16*)out, p.shares, a, st);
     if (rc != 0 || !a.mass) return rc;
-    return kv8::mass_takes((const bf16*)q, tokens, dim, vdim) ? kv8::mass_rows_mma((const bf16*)q, a, options->max_q_len, st) : kv8::mass_rows((const bf16*)q, a, st);
+    return kv8::mass_rows((const bf16*)q, a, options->max_q_len, st);
   }
-  if (f32) return kv8::attention((const float*)q, (const float*)sink, (float*)out, a, p, st);
-  return kv8::attention((const bf16*)q, (const bf16*)sink, (bf16*)out, a, p, st);
+  if (f32) return kv8::attention((const float*)q, (const float*)sink, (float*)out, a, p, options->max_q_len, st);
+  return kv8::attention((const bf16*)q, (const bf16*)sink, (bf16*)out, a, p, options->max_q_len, st);
 }

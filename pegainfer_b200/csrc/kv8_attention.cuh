@@ -51,6 +51,27 @@ __device__ __forceinline__ RowEnd row_end(float M, float den, float sink, bool h
   return r;
 }
 
+// ---- products in f16 (mma.sync): codes widened, exactly
+constexpr int kTopQ = 14, kTopP = 15;  // exponents of the largest entry of a row of q, and of P = 1, in f16
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// four codes -> two pairs of f16
+__device__ __forceinline__ void widen(uint32_t four, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(lo), "=r"(hi) : "r"(four));
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
 // records of a warp's run (kv8_few.cu), an even number: `total` records over `warps` warps
 __host__ __device__ inline int few_run(int total, int warps) { return max(2, ((total + warps - 1) / warps + 1) / 2 * 2); }
 // kv8_few.cu: whether it takes a call, what it needs (bytes), the call itself (with the weights' sums)
@@ -67,8 +88,13 @@ int few_attention(const bf16* q, const bf16* sink, bf16* out, const AttnArgs& a,
 bool prompt_takes(int T, int H, int G, int dim, int vdim);
 int prompt_shares(int T, int H, int G, int max_kv_len, int window);
 int prompt_attention(const bf16* q, const bf16* sink, bf16* out, const AttnArgs& a, int shares, cudaStream_t st);
-// kv8_mass.cu: the weights' sums of such a call
-bool mass_takes(const bf16* q, int T, int dim, int vdim);
+// kv8_tile.cu: the same for any sizes and types
+bool tile_takes(int T, int H, int G, int max_q_len);
+int tile_shares(int T, int H, int G, int max_kv_len, int window);
+template <typename E>
+int tile_attention(const E* q, const E* sink, E* out, const AttnArgs& a, int shares, cudaStream_t st);
+// kv8_mass.cu: the weights' sums of such calls
+bool mass_takes(const bf16* q, int T, int dim);
 int mass_rows_mma(const bf16* q, const AttnArgs& a, int max_q_len, cudaStream_t st);
 
 }  // namespace kv8

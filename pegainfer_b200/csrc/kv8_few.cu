@@ -25,7 +25,6 @@ namespace pk {
 namespace kv8 {
 
 constexpr int kFewTokens = 512;  // of a launch: their tiles are looked up in shared memory
-constexpr int kTopQ = 14, kTopP = 15;  // exponents of the largest entry of a row of q, and of P = 1, in f16
 template <int D>
 constexpr int few_warps() { return D <= 128 ? 8 : 4; }
 template <int D>
@@ -44,25 +43,6 @@ struct FewArgs {
   unsigned int* err;
 };
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-// four codes -> two pairs of f16
-__device__ __forceinline__ void widen(uint32_t four, uint32_t& lo, uint32_t& hi) {
-  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(lo), "=r"(hi) : "r"(four));
-}
-__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
 // an 8 x 8 matrix of f16 turned round
 __device__ __forceinline__ uint32_t turned(uint32_t v) {
   uint32_t r;
@@ -688,11 +668,15 @@ static int launch_few(const bf16* q, const bf16* sink, bf16* out, const FewArgs&
   return wide ? launch_few<D, false, true>(q, sink, out, f, ctas, st) : launch_few<D, false, false>(q, sink, out, f, ctas, st);
 }
 
+// Against the kernel for prompts (B200, us here : there, 32 heads of 128 in 8 groups): a portion behind 2000 of 48 tokens 38 : 56, 96 48 : 54, 256 85 : 60, behind 8000 of
+// 32 54 : 52, 64 81 : 63, 256 234 : 89; 16 portions of 16 behind 2000 83 : 176, 8 of 32 83 : 95, 4 of 64 83 : 60; decoded tokens of 64 requests 69 : 2637 (there a tile's
+// tokens belong to 64 requests, one after the other).  So up to 32 tokens of a request come here; with no word about them calls of up to 512 tokens, where a wrong guess
+// costs a factor of 3 here and 40 there.
 bool few_takes(int T, int H, int G, int dim, int vdim, int max_kv_len, int max_q_len) {
   if (T > 65535 || dim != vdim || !(dim == 32 || dim == 64 || dim == 96 || dim == 128 || dim == 192 || dim == 256)) return false;
   if ((long)std::min(T, kFewTokens) * G * ((H / G + 15) / 16) * (max_kv_len / kBlock + 2) >= 1L << 31) return false;
   // (where the kernel for prompts does not take the heads' size, any call: its rows in tiles of 16)
-  return T < 64 || (max_q_len > 0 && max_q_len <= 16) || !prompt_takes(T, H, G, dim, vdim);
+  return T < 64 || (max_q_len > 0 ? max_q_len <= 32 : T <= kFewTokens) || !prompt_takes(T, H, G, dim, vdim);
 }
 static int few_tokens(int T) { return std::min(T, kFewTokens); }
 static int few_warps_of(int dim) { return dim <= 128 ? 8 : 4; }

@@ -448,8 +448,8 @@ static int launch_mass(const bf16* q, const AttnArgs& a, int runs, cudaStream_t 
     if (std::min((long)a.max_kv_len, a.mass_ld) / (kMassWarps * 2 * kBlock) * a.pool.G * runs >= 4L * sm_count()) return launch_mass<D, 2>(q, a, runs, st);
   return launch_mass<D, 1>(q, a, runs, st);
 }
-bool mass_takes(const bf16* q, int T, int dim, int vdim) {
-  return T <= kMassTokens && dim == vdim && (dim == 32 || dim == 64 || dim == 96 || dim == 128 || dim == 192 || dim == 256) && (reinterpret_cast<uintptr_t>(q) & 15) == 0;
+bool mass_takes(const bf16* q, int T, int dim) {
+  return T <= kMassTokens && (dim == 32 || dim == 64 || dim == 96 || dim == 128 || dim == 192 || dim == 256) && (reinterpret_cast<uintptr_t>(q) & 15) == 0;
 }
 int mass_rows_mma(const bf16* q, const AttnArgs& a, int max_q_len, cudaStream_t st) {
   const int runs = max_q_len > 0 ? (a.T + max_q_len - 1) / max_q_len : 4;  // at least; unknown: some

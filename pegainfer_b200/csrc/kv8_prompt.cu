@@ -664,7 +664,7 @@ bool prompt_takes(int T, int H, int G, int dim, int vdim) {
   return dim == vdim && (dim == 64 || dim == 96 || dim == 128) && tokens > 0 && (T + tokens - 1) / tokens <= 65535;
 }
 // Shares of the keys where the tiles leave SMs idle: as many CTAs as SMs, and 16 blocks of keys to a share at least (of the longest context, which is all that is known).
-// A share's start and end take 6 us, a block 1.5; the merge 13 for 10656 rows.  (666 tokens of two portions behind 5003, 16 heads: 104 + 13 us in three shares, 230 whole.)
+// A share's start and end take 6 us, a block 1.5; the merge 13 for 10656 rows.  (666 tokens of two portions behind 5003, 16 heads: 104 + 13 us in three shares, 248 whole.)
 int prompt_shares(int T, int H, int G, int max_kv_len, int window) {
   const int per = kPrRows / (H / G), ctas = (T + 2 * per - 1) / (2 * per) * G;
   const int span = window > 0 ? std::min(max_kv_len, window + 2 * per) : max_kv_len;

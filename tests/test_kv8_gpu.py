@@ -289,6 +289,15 @@ def test_window_that_hides_nothing(lib, steps):
         check_attention(lib, steps, 4, 2, 32, f32=True, mass=True, longest=433, window=window, seed=1)
 
 
+@pytest.mark.parametrize("H,G,D,V", [(4, 2, 128, 64), (3, 3, 32, 256), (14, 2, 64, 96), (70, 1, 64, 32), (130, 2, 32, 32), (6, 2, 256, 160), (5, 1, 96, 96)])
+@pytest.mark.parametrize("steps", [[(64, 0)], [(33, 700), (8, 1), (40, 64)], [(9, 5000)], [(100, 13), (1, 0), (1, 90), (63, 65)]], ids=["prompt", "portions", "long", "mixed"])
+@pytest.mark.parametrize("f32", [False, True])
+def test_tiles(lib, H, G, D, V, steps, f32):
+    """fp32 rows, and sizes of keys and values that differ: tiles of rows that cross requests, groups larger than a tile, keys in shares"""
+    check_attention(lib, steps, H, G, D, V, f32=f32)
+    check_attention(lib, steps, H, G, D, V, page=48, f32=f32, mass=True, sink=True, window=77, softcap=15.0, seed=1, max_q=0, out_ld=H * V + 3)
+
+
 @pytest.mark.parametrize("V", [32, 64, 192])
 def test_values_of_another_width(lib, V):
     check_attention(lib, [(1, 333), (20, 40)], 8, 2, 128, V, mass=True)
