@@ -155,56 +155,6 @@ __global__ void __launch_bounds__(128) kv8_merge_kernel(const E* __restrict__ si
   if (lane == 0 && a.lse) a.lse[row] = end.lse;
 }
 
-// Weights of the keys, added up over the call's queries: a warp to (record, kv head), which goes through the requests' runs of tokens.  The scores are
-// computed again from q and the finished lse, so every key has one owner and the sum one order.
-template <typename E>
-__global__ void __launch_bounds__(128) kv8_mass_row_kernel(const E* __restrict__ q, AttnArgs a) {
-  pdl_wait();
-  pdl_launch_dependents();
-  const int lane = threadIdx.x & 31, b = blockIdx.x * 4 + (threadIdx.x >> 5), g = blockIdx.y, R = a.H / a.pool.G;
-  const int D = a.pool.dim, V = a.pool.vdim, tok = lane & 15, part = lane >> 4, chunks = D / 32, j = b * kBlock + tok;
-  const float c = a.scale * kLog2e;
-  for (int t0 = 0; t0 < a.T;) {
-    const int req = a.req[t0];
-    int t1 = t0, last = -1, lowest = INT_MAX;  // the run's end, its largest and smallest slot
-    for (bool more = true; more;) {
-      const bool in = t1 + lane < a.T && a.req[min(t1 + lane, a.T - 1)] == req;
-      const uint32_t same = __ballot_sync(0xffffffffu, in);
-      const int n = same == 0xffffffffu ? 32 : __ffs(~same) - 1, slot = lane < n ? a.slots[t1 + lane] : -1;
-      last = max(last, __reduce_max_sync(0xffffffffu, slot));
-      lowest = min(lowest, __reduce_min_sync(0xffffffffu, slot < 0 ? INT_MAX : slot));
-      t1 += n;
-      more = n == 32;
-    }
-    if (b * kBlock <= last && (a.window <= 0 || b * kBlock + kBlock - 1 > lowest - a.window)) {
-      const uint8_t* rec = a.pool.record(req, b * kBlock, g);
-      const float ek = pow2(tail_ek(*reinterpret_cast<const uint32_t*>(rec + kBlock * (D + V))));
-      const uint8_t* k = rec + (tok >> 3) * (8 * D) + part * chunks * 128 + (tok & 7) * 16;
-      float sum = 0.f;
-      for (int t = t0; t < t1; ++t) {
-        const int p = a.slots[t];
-        if (p < b * kBlock) continue;
-        const bool seen = j <= p && (a.window <= 0 || j > p - a.window);
-        for (int r = 0; r < R; ++r) {
-          const size_t row = (size_t)t * a.H + g * R + r;
-          const E* x = q + row * D + part * chunks * 16;
-          float s = 0.f;
-          for (int i = 0; i < chunks; ++i) {
-            float v[16];
-            values16(*reinterpret_cast<const uint4*>(k + i * 128), v);
-#pragma unroll
-            for (int d = 0; d < 16; ++d) s = fmaf(v[d], to_f(x[i * 16 + d]), s);
-          }
-          s += __shfl_xor_sync(0xffffffffu, s, 16);
-          if (seen) sum += exp2f(shaped(s * ek, c, a.cap) - a.lse[row] * kLog2e);
-        }
-      }
-      if (part == 0 && j <= last && j < a.mass_ld) a.mass[((size_t)req * a.pool.G + g) * a.mass_ld + j] += sum;
-    }
-    t0 = t1;
-  }
-}
-
 // what a call runs: the shares of its keys and its workspace
 struct Plan {
   bool few, prompt, tile;  // kv8_few.cu, kv8_prompt.cu, kv8_tile.cu
@@ -244,12 +194,6 @@ static Plan plan(int T, int H, int G, int dim, int vdim, const pk_kv8_options& o
   return p;
 }
 
-template <typename E>
-static int mass_rows(const E* q, const AttnArgs& a, int max_q_len, cudaStream_t st) {
-  if constexpr (sizeof(E) == 2)
-    if (mass_takes(q, a.T, a.pool.dim)) return mass_rows_mma(q, a, max_q_len, st);
-  return (int)follow(kv8_mass_row_kernel<E>, dim3((a.max_kv_len + 63) / 64, a.pool.G), dim3(128), st, q, a);
-}
 template <typename E>
 static int merge(const E* sink, E* out, int shares, const AttnArgs& a, cudaStream_t st) {
   return (int)follow(kv8_merge_kernel<E>, dim3((unsigned)(((size_t)a.T * a.H + 3) / 4)), dim3(128), st, sink, out, shares, a);

@@ -94,8 +94,8 @@ int tile_shares(int T, int H, int G, int max_kv_len, int window);
 template <typename E>
 int tile_attention(const E* q, const E* sink, E* out, const AttnArgs& a, int shares, cudaStream_t st);
 // kv8_mass.cu: the weights' sums of such calls
-bool mass_takes(const bf16* q, int T, int dim);
-int mass_rows_mma(const bf16* q, const AttnArgs& a, int max_q_len, cudaStream_t st);
+template <typename E>
+int mass_rows(const E* q, const AttnArgs& a, int max_q_len, cudaStream_t st);
 
 }  // namespace kv8
 }  // namespace pk

@@ -671,12 +671,13 @@ static int launch_few(const bf16* q, const bf16* sink, bf16* out, const FewArgs&
 // Against the kernel for prompts (B200, us here : there, 32 heads of 128 in 8 groups): a portion behind 2000 of 48 tokens 38 : 56, 96 48 : 54, 256 85 : 60, behind 8000 of
 // 32 54 : 52, 64 81 : 63, 256 234 : 89; 16 portions of 16 behind 2000 83 : 176, 8 of 32 83 : 95, 4 of 64 83 : 60; decoded tokens of 64 requests 69 : 2637 (there a tile's
 // tokens belong to 64 requests, one after the other).  So up to 32 tokens of a request come here; with no word about them calls of up to 512 tokens, where a wrong guess
-// costs a factor of 3 here and 40 there.
+// costs a factor of 3 here and 40 there.  Against tiles (kv8_tile.cu), where the kernel for prompts does not take the heads' size: 64 behind 2000, 16 heads of 32 in 4
+// groups, 29 : 53, 16 of 256 in one 70 : 113, 32 of 192 in 8 82 : 102; 256 70 : 59, 135 : 129, 277 : 186; six prompts of 608 596 : 98, 2270 : 311, 2360 : 571.
 bool few_takes(int T, int H, int G, int dim, int vdim, int max_kv_len, int max_q_len) {
   if (T > 65535 || dim != vdim || !(dim == 32 || dim == 64 || dim == 96 || dim == 128 || dim == 192 || dim == 256)) return false;
   if ((long)std::min(T, kFewTokens) * G * ((H / G + 15) / 16) * (max_kv_len / kBlock + 2) >= 1L << 31) return false;
-  // (where the kernel for prompts does not take the heads' size, any call: its rows in tiles of 16)
-  return T < 64 || (max_q_len > 0 ? max_q_len <= 32 : T <= kFewTokens) || !prompt_takes(T, H, G, dim, vdim);
+  const bool prompt = prompt_takes(T, H, G, dim, vdim);
+  return T < 64 || (max_q_len > 0 ? max_q_len <= (prompt ? 32 : 64) : T <= kFewTokens) || !(prompt || tile_takes(T, H, G, max_q_len));
 }
 static int few_tokens(int T) { return std::min(T, kFewTokens); }
 static int few_warps_of(int dim) { return dim <= 128 ? 8 : 4; }

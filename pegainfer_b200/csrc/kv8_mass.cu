@@ -16,7 +16,7 @@
 namespace pk {
 namespace kv8 {
 
-constexpr int kMassWarps = 4, kMassRows = 64, kMassTokens = 65536;  // of a call, at most
+constexpr int kMassWarps = 4, kMassRows = 64, kMassTokens = 65536;  // of a launch, at most
 
 __device__ __forceinline__ float ms_ex2(float x) {
   float y;
@@ -448,11 +448,74 @@ static int launch_mass(const bf16* q, const AttnArgs& a, int runs, cudaStream_t 
     if (std::min((long)a.max_kv_len, a.mass_ld) / (kMassWarps * 2 * kBlock) * a.pool.G * runs >= 4L * sm_count()) return launch_mass<D, 2>(q, a, runs, st);
   return launch_mass<D, 1>(q, a, runs, st);
 }
-bool mass_takes(const bf16* q, int T, int dim) {
-  return T <= kMassTokens && (dim == 32 || dim == 64 || dim == 96 || dim == 128 || dim == 192 || dim == 256) && (reinterpret_cast<uintptr_t>(q) & 15) == 0;
+// ---- any sizes and types, in fp32: a CTA to a record, its warps to four rows of the run at a time; their sums come together in the warps' order.  Two lanes have a
+// token's key, half of the entries each.  (fp32, 36 tokens of 16 heads of 128 in 4 groups: the whole call 37 us; with a warp to a record 164.)
+constexpr int kPlainWarps = 8, kPlainRows = 4;
+
+template <typename E>
+__global__ void __launch_bounds__(kPlainWarps * 32) kv8_mass_plain_kernel(const E* __restrict__ q, AttnArgs a) {
+  __shared__ uint32_t ms_starts[kMassTokens / 32];
+  __shared__ int4 s_run[kPlainWarps];
+  __shared__ float s_sum[kPlainWarps][kBlock];
+  pdl_wait();
+  pdl_launch_dependents();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, b = blockIdx.x, g = blockIdx.y, R = a.H / a.pool.G;
+  const int D = a.pool.dim, V = a.pool.vdim, tok = lane & 15, part = lane >> 4, chunks = D / 32, key0 = b * kBlock, key1 = key0 + kBlock - 1, j = key0 + tok;
+  const float c = a.scale * kLog2e;
+  const Runs runs = find_runs<kPlainWarps>(ms_starts, a);
+  int nth = 0;
+  for (int t0 = 0, t1 = 0; t0 < a.T; t0 = t1, ++nth) {
+    t1 = runs.after(t0);
+    if (nth % (int)gridDim.z != (int)blockIdx.z) continue;
+    const int req = a.req[t0];
+    const auto [last, at_last, lowest, at_lowest] = run_ends<kPlainWarps>(s_run, a, t0, t1);
+    if (key0 > last || (a.window > 0 && key1 <= lowest - a.window)) continue;  // (for all threads alike)
+    const int from = max(t0, at_last - (last - key0)), to = a.window > 0 ? (int)min((long)t1, (long)at_lowest + (key1 + (long)a.window - lowest)) : t1;
+    const uint8_t* rec = a.pool.record(req, key0, g);
+    const float ek = pow2(tail_ek(*reinterpret_cast<const uint32_t*>(rec + kBlock * (D + V))));
+    const uint8_t* k = rec + (tok >> 3) * (8 * D) + part * chunks * 128 + (tok & 7) * 16;
+    float sum = 0.f;
+    const long rows = (long)(to - from) * R;
+    for (long i0 = warp * kPlainRows; i0 < rows; i0 += kPlainWarps * kPlainRows) {
+      const E* x[kPlainRows];
+      size_t row[kPlainRows];
+      int p[kPlainRows];
+#pragma unroll
+      for (int i = 0; i < kPlainRows; ++i) {
+        const long at = min(i0 + i, rows - 1);
+        const int t = from + (int)(at / R);
+        row[i] = (size_t)t * a.H + g * R + (int)(at % R);
+        x[i] = q + row[i] * D + part * chunks * 16;
+        p[i] = i0 + i < rows ? a.slots[t] : -1;
+      }
+      float s[kPlainRows] = {};
+      for (int n = 0; n < chunks; ++n) {
+        float v[16];
+        values16(*reinterpret_cast<const uint4*>(k + n * 128), v);
+#pragma unroll
+        for (int i = 0; i < kPlainRows; ++i)
+#pragma unroll
+          for (int d = 0; d < 16; ++d) s[i] = fmaf(v[d], to_f(x[i][n * 16 + d]), s[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < kPlainRows; ++i) {
+        s[i] += __shfl_xor_sync(0xffffffffu, s[i], 16);
+        if (j <= p[i] && (a.window <= 0 || j > p[i] - a.window)) sum += exp2f(shaped(s[i] * ek, c, a.cap) - a.lse[row[i]] * kLog2e);
+      }
+    }
+    if (part == 0) s_sum[warp][tok] = sum;
+    __syncthreads();
+    if (warp == 0 && part == 0 && j <= last && j < a.mass_ld) {
+      float all = 0.f;
+#pragma unroll
+      for (int w = 0; w < kPlainWarps; ++w) all += s_sum[w][tok];
+      a.mass[((size_t)req * a.pool.G + g) * a.mass_ld + j] += all;
+    }
+    __syncthreads();  // the next run's sums may come
+  }
 }
-int mass_rows_mma(const bf16* q, const AttnArgs& a, int max_q_len, cudaStream_t st) {
-  const int runs = max_q_len > 0 ? (a.T + max_q_len - 1) / max_q_len : 4;  // at least; unknown: some
+
+static int mass_mma(const bf16* q, const AttnArgs& a, int runs, cudaStream_t st) {
   const long R = a.H / a.pool.G;
   if (a.T * R * R < 1L << 32) {  // (rows are divided by R through a product)
     if (a.pool.dim == 64) return launch_mass_wide<64>(q, a, runs, st);
@@ -467,6 +530,30 @@ int mass_rows_mma(const bf16* q, const AttnArgs& a, int max_q_len, cudaStream_t 
     default: return launch_mass<256>(q, a, runs, st);
   }
 }
+template <typename E>
+int mass_rows(const E* q, const AttnArgs& a, int max_q_len, cudaStream_t st) {
+  const int T = a.T, D = a.pool.dim;
+  for (int t0 = 0; t0 < T; t0 += kMassTokens) {  // (a run that a launch's end cuts is added up in both)
+    AttnArgs x = a;
+    x.T = std::min(kMassTokens, T - t0);
+    x.slots += t0;
+    x.req += t0;
+    x.lse += (size_t)t0 * a.H;
+    const E* rows = q + (size_t)t0 * a.H * D;
+    const int runs = max_q_len > 0 ? (x.T + max_q_len - 1) / max_q_len : 4;  // at least; unknown: some
+    if constexpr (sizeof(E) == 2)
+      if ((D == 32 || D == 64 || D == 96 || D == 128 || D == 192 || D == 256) && (reinterpret_cast<uintptr_t>(q) & 15) == 0) {
+        if (const int rc = mass_mma(rows, x, runs, st); rc != 0) return rc;
+        continue;
+      }
+    const long span = std::min((long)a.max_kv_len, a.mass_ld);
+    const dim3 grid((unsigned)((span + kBlock - 1) / kBlock), a.pool.G, std::max(1, std::min(runs, 64)));
+    if (const cudaError_t e = follow(kv8_mass_plain_kernel<E>, grid, dim3(kPlainWarps * 32), st, rows, x); e != cudaSuccess) return (int)e;
+  }
+  return 0;
+}
+template int mass_rows<float>(const float*, const AttnArgs&, int, cudaStream_t);
+template int mass_rows<bf16>(const bf16*, const AttnArgs&, int, cudaStream_t);
 
 }  // namespace kv8
 }  // namespace pk
