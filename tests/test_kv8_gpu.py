@@ -209,13 +209,13 @@ def test_append_leaves_rows_without_a_slot(lib):
 
 # ------------------------------------------------------------------ attention
 def out_bound(want, size, f32, split=True):
-    """bf16: one rounding of the result (2^-8), one of each weight where it goes into the product (hi + lo e4m3 parts: 2^-9, taken as 2^-8), fp32 sums and
-    exponentials (1e-5 of the weights); fp32: exponentials, sums and scores of about 20 in fp32"""
+    """bf16: one rounding of the result (2^-8), one of each weight where it goes into the product (f16: 2^-11, taken as 2^-8), fp32 sums and
+    exponentials (1e-5 of the weights); fp32: exponentials, sums and scores of about 20 in fp32 (weights and q as two f16: 2^-22)"""
     return (2.0 ** -8 + 2e-5) * size + 2.0 ** -8 * want.abs() + 1e-6 if not f32 else 2e-5 * size + 1e-7
 
 
 def lse_bound(q, k, scale, f32):
-    """scores: D products in fp32 and q as two e4m3 parts (2^-18 of its largest entry); the logarithm: a few units of fp32"""
+    """scores: D products in fp32 and q as two 8-bit numbers (2^-18 of its largest entry) or one or two f16 (less); the logarithm: a few units of fp32"""
     kk = torch.nan_to_num(k).abs().sum(-1).max() if k.numel() else torch.tensor(0.0)
     qm = q.abs().double().max()
     return float(scale * qm * kk * ((0 if f32 else 2.0 ** -18) + 64 * 2.0 ** -24)) + 2e-6
@@ -279,6 +279,12 @@ def test_options(lib, steps, opts):
     o = dict(opts)
     o.update(out_ld=0)
     check_attention(lib, steps, 6, 2, 64, mass=True, seed=1, **o)
+
+
+@pytest.mark.parametrize("f32", [False, True])
+def test_weights_of_more_tokens_than_a_launch_looks_at(lib, f32):
+    """65536; the portion of one request lies on both sides"""
+    check_attention(lib, [(61, 0)] * 1076, 2, 1, 64, f32=f32, mass=True)
 
 
 @pytest.mark.parametrize("steps", [[(1, 400), (3, 31)], [(100, 33), (40, 300)]], ids=["few", "prompts"])
