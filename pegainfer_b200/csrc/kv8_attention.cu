@@ -144,8 +144,7 @@ __global__ void __launch_bounds__(128) kv8_merge_kernel(const E* __restrict__ si
 #pragma unroll
       for (int i = 0; i < 8; ++i)
         if (lane + 32 * i < V) {
-          const float x = a.part_o[(s * rows + row) * V + lane + 32 * i];
-          o[i] = f != 0.f ? fmaf(x, f, o[i]) : o[i];
+          if (f != 0.f) o[i] = fmaf(a.part_o[(s * rows + row) * V + lane + 32 * i], f, o[i]);  // (for the warp alike; a share without keys stores none)
         }
     }
   }

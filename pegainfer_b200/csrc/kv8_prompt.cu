@@ -13,7 +13,7 @@
 //     tile waited 1600 of 5200 clocks for it.)
 //   * m is a maximum of before that the row's own may have passed by up to 2^8: O, which stays in tensor memory, is rescaled only where one did by more.  P, held 2^7 times
 //     too large, stays within f16's range then, with 11 bits down to 2^-21 of the largest weight.
-// B200, prompt of 4096 tokens, 32 heads of 128 in 8 groups: 194 us, 0.71 PFLOP/s.  Bound by a softmax thread's latency: 1200 of 2500 clocks of a block of 64 keys are its
+// B200, prompt of 4096 tokens, 32 heads of 128 in 8 groups: 193 us, 0.71 PFLOP/s.  Bound by a softmax thread's latency: 1200 of 2500 clocks of a block of 64 keys are its
 // exponentials and P, 500 waits; a CTA's start takes 12000.  Tried and slower: operands in the 128-byte swizzle (206), a degree-4 polynomial for a quarter of the
 // exponentials (210), blocks of 128 keys (231).
 // Warps: 0-3 softmax tile 0, a thread per row | 4-7 softmax tile 1 | 8-11 V, rescaling, results | 12, 13 MMA issuers | 14 copies | 15 nothing.  Of the block's registers a
@@ -39,6 +39,7 @@ constexpr int kPrMaxSeg = 256;     // runs that a CTA's tokens can belong to
 struct PromptArgs {
   AttnArgs a;
   int per;           // tokens of a tile
+  int each;          // blocks of a share, at least
   int q_by8, out_by8;
   unsigned int* err;
 };
@@ -115,7 +116,8 @@ __device__ __forceinline__ void q_parts(uint32_t w0, uint32_t w1, float down, ui
   rest = (uint32_t)d[0] | (uint32_t)d[1] << 16;
 }
 
-template <int D>
+// CUT: the keys of a tile are cut into shares
+template <int D, bool CUT>
 __global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* __restrict__ q, const bf16* __restrict__ sink, bf16* __restrict__ out, const PromptArgs f) {
   constexpr int QB = kPrRows * D, KB = kPrKeys * D, REC_K = kBlock * D;  // bytes of a part of q's tile, of a stage's K (or V), of a record's K
   extern __shared__ uint8_t pr_raw[];
@@ -144,8 +146,8 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* _
 
   const AttnArgs& a = f.a;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int g = blockIdx.x, R = a.H / a.pool.G, per = f.per;
-  const int t0 = ((int)gridDim.y - 1 - (int)blockIdx.y) * 2 * per, n_tok = min(2 * per, a.T - t0);  // late tokens, which see most, first
+  const int g = blockIdx.y, R = a.H / a.pool.G, per = f.per;
+  const int t0 = ((int)gridDim.z - 1 - (int)blockIdx.z) * 2 * per, n_tok = min(2 * per, a.T - t0);  // late tokens, which see most, first
 
   if (tid == 0) {
     for (int s = 0; s < kPrStages; ++s) {
@@ -258,17 +260,23 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* _
       settle(x);
     }
   };
-  // this CTA's share of them (the grid's z axis), counted from its own first
+  // this CTA's share of them (the grid's x axis, so that a tile's CTAs without one leave early), counted from its own first
   int share = INT_MAX;
   Step origin{0, 0, 0};
-  if (gridDim.z == 1) {
+  if constexpr (!CUT) {
     settle(origin);
   } else {
     int all = 0;
     for (int k = 0; k < segs; ++k)
       if (last_block(k) >= 0) all += last_block(k) - first_block(k) + 1;
-    const int each = (all + (int)gridDim.z - 1) / (int)gridDim.z, skip = min(each * (int)blockIdx.z, all);
+    const int each = max(f.each, (all + (int)gridDim.x - 1) / (int)gridDim.x), skip = (int)min((long)each * blockIdx.x, (long)all);
     share = min(each, all - skip);
+    if (share == 0) {  // (for all threads alike)
+      const int r = tid & 127, k = r / R, ti = (tid >> 7) * per + k;
+      if (tid < 2 * kPrRows && k < per && ti < n_tok) a.part_ml[((size_t)blockIdx.x * a.T + t0 + ti) * a.H + g * R + r - k * R] = make_float2(-INFINITY, 0.f);
+      if (warp == kPrMma) tmem_dealloc(tmem_base, 512);
+      return;
+    }
     settle(origin);
     for (int k = 0; k < skip;) {  // run by run
       const int here = last_block(origin.seg) - origin.j + 1, go = min(here, skip - k);
@@ -280,11 +288,11 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* _
         settle(origin);
       }
     }
-    if (share == 0) origin.seg = segs;
   }
   auto begin = [&] { return origin; };
   auto next = [&](Step& x) {
-    if (++x.n == share) x.seg = segs;
+    ++x.n;
+    if (CUT && x.n == share) x.seg = segs;
     else pass(x);
   };
 
@@ -485,8 +493,8 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* _
         if (!on) continue;
 #pragma unroll
         for (int x = 0; x < 32; ++x) t[x] = __float_as_uint(__uint_as_float(t[x]) * factor);
-        if (gridDim.z > 1) {
-          float* part = a.part_o + (((size_t)blockIdx.z * a.T + t0 + ti) * a.H + g * R + r - k * R) * D + c;
+        if constexpr (CUT) {
+          float* part = a.part_o + (((size_t)blockIdx.x * a.T + t0 + ti) * a.H + g * R + r - k * R) * D + c;
 #pragma unroll
           for (int x = 0; x < 32; x += 4)
             *reinterpret_cast<uint4*>(part + x) = make_uint4(t[x], t[x + 1], t[x + 2], t[x + 3]);
@@ -623,9 +631,9 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* _
     }
     const float top = l != l ? INFINITY : m;  // a NaN among the scores
     const float up = pow2(max(E, kLowExp) - kPrTop);
-    if (gridDim.z > 1) {  // a share's state: kv8_merge_kernel
+    if constexpr (CUT) {  // a share's state: kv8_merge_kernel
       end_s[i * kPrRows + r] = up;
-      if (on) a.part_ml[((size_t)blockIdx.z * a.T + t0 + ti) * a.H + h] = make_float2(top, l);
+      if (on) a.part_ml[((size_t)blockIdx.x * a.T + t0 + ti) * a.H + h] = make_float2(top, l);
     } else {
       const RowEnd end = row_end(top, l, sink ? bf2f(sink[h]) : 0.f, sink != nullptr);
       end_s[i * kPrRows + r] = l != l ? NAN : end.factor * up;
@@ -651,12 +659,16 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* _
   if (tid == 0) count_run_out(dead, f.err);
 }
 
-template <int D>
+template <int D, bool CUT>
 static int launch_prompt(const bf16* q, const bf16* sink, bf16* out, const PromptArgs& f, int shares, cudaStream_t st) {
   constexpr size_t smem = 128 + (size_t)4 * kPrRows * D + (size_t)(kPrStages + 3 * kPrStagesV) * kPrKeys * D + kPrStagesV * kPrRecords * 20 + 6 * kPrRows * sizeof(float) + 40 * 8;
   static std::atomic<uint64_t> set{0};
-  if (const cudaError_t e = allow_smem(set, (const void*)kv8_prompt_kernel<D>, smem); e != cudaSuccess) return (int)e;
-  return (int)launch(kv8_prompt_kernel<D>, dim3(f.a.pool.G, (f.a.T + 2 * f.per - 1) / (2 * f.per), shares), dim3(kPrThreads), smem, st, true, q, sink, out, f);
+  if (const cudaError_t e = allow_smem(set, (const void*)kv8_prompt_kernel<D, CUT>, smem); e != cudaSuccess) return (int)e;
+  return (int)launch(kv8_prompt_kernel<D, CUT>, dim3(shares, f.a.pool.G, (f.a.T + 2 * f.per - 1) / (2 * f.per)), dim3(kPrThreads), smem, st, true, q, sink, out, f);
+}
+template <int D>
+static int launch_prompt(const bf16* q, const bf16* sink, bf16* out, const PromptArgs& f, int shares, cudaStream_t st) {
+  return shares > 1 ? launch_prompt<D, true>(q, sink, out, f, shares, st) : launch_prompt<D, false>(q, sink, out, f, shares, st);
 }
 
 bool prompt_takes(int T, int H, int G, int dim, int vdim) {
@@ -664,16 +676,25 @@ bool prompt_takes(int T, int H, int G, int dim, int vdim) {
   return dim == vdim && (dim == 64 || dim == 96 || dim == 128) && tokens > 0 && (T + tokens - 1) / tokens <= 65535;
 }
 // Shares of the keys where the tiles leave SMs idle: as many CTAs as SMs, and 16 blocks of keys to a share at least (of the longest context, which is all that is known).
-// A share's start and end take 6 us, a block 1.5; the merge 13 for 10656 rows.  (666 tokens of two portions behind 5003, 16 heads: 104 + 13 us in three shares, 248 whole.)
-int prompt_shares(int T, int H, int G, int max_kv_len, int window) {
+// A share's start and end take 6 us, a block 1.5; the merge 13 for 10656 rows.  (666 tokens of two portions behind 5003, 16 heads: 80 + 14 us in shares of 28 blocks, 248 whole.)
+static int prompt_span(int H, int G, int max_kv_len, int window) { return window > 0 ? std::min(max_kv_len, window + 2 * (kPrRows / (H / G))) : max_kv_len; }
+static int prompt_pieces(int T, int H, int G, int max_kv_len, int window) {
   const int per = kPrRows / (H / G), ctas = (T + 2 * per - 1) / (2 * per) * G;
-  const int span = window > 0 ? std::min(max_kv_len, window + 2 * per) : max_kv_len;
-  return std::max(1, std::min(sm_count() / std::max(ctas, 1), span / (16 * kPrKeys)));
+  return std::max(1, std::min(sm_count() / std::max(ctas, 1), prompt_span(H, G, max_kv_len, window) / (16 * kPrKeys)));
+}
+// Twice as many CTAs to a tile as one context makes shares: a tile whose tokens belong to two requests has two contexts to read, and its shares are as long as the others'
+// (their other CTAs leave at once).  (The same portions: 80 us, 104 with three CTAs to a
+// tile.)  A tile's CTAs follow one another in the grid: those that leave make room for the next tile's (94 us with a tile's shares a grid of tiles apart).
+int prompt_shares(int T, int H, int G, int max_kv_len, int window) {
+  const int pieces = prompt_pieces(T, H, G, max_kv_len, window);
+  return pieces > 1 ? 2 * pieces : 1;
 }
 int prompt_attention(const bf16* q, const bf16* sink, bf16* out, const AttnArgs& a, int shares, cudaStream_t st) {
   PromptArgs f{};
   f.a = a;
   f.per = kPrRows / (a.H / a.pool.G);
+  const int pieces = prompt_pieces(a.T, a.H, a.pool.G, a.max_kv_len, a.window), blocks = prompt_span(a.H, a.pool.G, a.max_kv_len, a.window) / kPrKeys + 2;
+  f.each = (blocks + pieces - 1) / pieces;
   f.q_by8 = (reinterpret_cast<uintptr_t>(q) & 15) == 0;
   f.out_by8 = (reinterpret_cast<uintptr_t>(out) & 15) == 0 && a.out_ld % 8 == 0;
   f.err = wait_err_word();
