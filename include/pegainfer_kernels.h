@@ -730,7 +730,7 @@ int pk_logistic_decay(float* z, const float* bias, float tau, int tokens, int ch
 /* Bytes of a page; -1: sizes that the cache does not have */
 long pk_kv8_page_bytes(int page_size, int kv_heads, int dim, int vdim);
 /* qkv [tokens, ld] = [q (heads*dim) | k (kv_heads*dim) | v (kv_heads*vdim)] (+ bias of the same layout, may be NULL): q and k rotate over their first `dims`
- * entries by positions[t] * freq[i] as in pk_gqa_rope_append (angles are reduced in 64 bits; sine and cosine are off by 2^-20 at most where the rows are bf16); q goes to q_out [tokens, heads*dim], k and v into the cache at
+ * entries by positions[t] * freq[i] as in pk_gqa_rope_append (angles are reduced in 64 bits; those of bf16 q have sine and cosine to 2^-20); q goes to q_out [tokens, heads*dim], k and v into the cache at
  * slots[t] (slots NULL: at positions[t]).  heads may be 0 (rows of k and v alone, q_out NULL).  A request's tokens are consecutive rows with consecutive slots,
  * in one run per call.  A token at a record's first slot begins the record anew (slots behind the call's last are zero); else the record goes on from the slots
  * before, whose codes are rounded again where its exponent grows.  Rows with a negative slot are not cached (their q is rotated all the same). */

@@ -278,12 +278,20 @@ __global__ void __launch_bounds__(kAppendWarps * 32) kv8_append_kernel(const E* 
 // All loads are under way before the first angle is there.  Where a record goes on under its old exponent of K, K's old codes are not touched.
 constexpr int kTurnRows = 32;  // a window's tokens, and those of its last record
 
-// The angle, within half a turn, goes to the special-function unit: 2^-21 off, where the results are rounded to 2^-9 at best.  (With the library's sine and cosine two of
-// five instructions of the kernel were angles: 27.5 us for 4096 tokens, 26.5 us so.)
+// FAST, for q: the angle, within half a turn, goes to the special-function unit, 2^-21 off, where the results are rounded to 2^-9.  (With the library's sine and cosine two
+// of five instructions of the kernel were q's angles.)  Not for k: an error next to 448 * 2^e changes a record's exponent.
+template <bool FAST>
 __device__ __forceinline__ float2 turn_of(int position, double freq, float mag) {  // freq in turns
   const double turns = (double)position * freq;
-  const float angle = (float)(turns - rint(turns)) * 6.2831853071795865f;
-  return make_float2(__cosf(angle) * mag, __sinf(angle) * mag);
+  const float part = (float)(turns - rint(turns));
+  float s, c;
+  if (FAST) {
+    s = __sinf(part * 6.2831853071795865f);
+    c = __cosf(part * 6.2831853071795865f);
+  } else {
+    sincospif(2.f * part, &s, &c);
+  }
+  return make_float2(c * mag, s * mag);
 }
 // eight pairs: (x[j], y[j]), or side by side in x and then y
 __device__ __forceinline__ void turn_pairs(float* x, float* y, const float2 (&cs)[8], int side_by_side) {
@@ -393,7 +401,7 @@ __device__ __forceinline__ void append_one(const bf16* row, const bf16* bias, co
       }
       bad_k |= odd_one(x[n]) || odd_one(y[n]);
       if (p < half) {
-        cs[n] = turn_of(at, (double)cs[n].x * kTurns, a.mag);
+        cs[n] = turn_of<false>(at, (double)cs[n].x * kTurns, a.mag);
         const float x0 = x[n], y0 = y[n];
         x[n] = x0 * cs[n].x - y0 * cs[n].y;
         y[n] = x0 * cs[n].y + y0 * cs[n].x;
@@ -493,7 +501,7 @@ __global__ void __launch_bounds__(kAppendWarps * 32, N <= 2 ? 4 : 2) kv8_append_
       if (h == h0 && turns) {
         const int at = a.positions[t];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) cs[k] = turn_of(at, (double)a.freq[u * 8 + k] * kTurns, a.mag);
+        for (int k = 0; k < 8; ++k) cs[k] = turn_of<true>(at, (double)a.freq[u * 8 + k] * kTurns, a.mag);
       }
 #pragma unroll
       for (int k = 0; k < 4; ++k)
@@ -595,7 +603,7 @@ __global__ void __launch_bounds__(kAppendWarps * 32, N <= 2 ? 4 : 2) kv8_append_
       const int rows = on >> kWindow & 1 ? pos_rows : n_tok;
       for (int k = lane; k < half; k += 32) {
         const double freq = (double)a.freq[k] * kTurns;
-        for (int r = warp; r < rows; r += kAppendWarps) ap_turns[r * ld_t + k] = turn_of(a.positions[w0 + r], freq, a.mag);
+        for (int r = warp; r < rows; r += kAppendWarps) ap_turns[r * ld_t + k] = turn_of<false>(a.positions[w0 + r], freq, a.mag);
       }
       table = true;
       __syncthreads();

@@ -24,6 +24,7 @@
 namespace pk {
 namespace kv8 {
 
+constexpr size_t kMostScores = (size_t)1 << 30;  // bytes that are kept for the weights' sums; with more the scores are computed again (kv8_mass.cu)
 constexpr int kFewTokens = 512;  // of a launch: their tiles are looked up in shared memory
 template <int D>
 constexpr int few_warps() { return D <= 128 ? 8 : 4; }
@@ -691,6 +692,7 @@ FewNeed few_need(int T, int H, int G, int dim, int max_kv_len, bool mass) {
   n.plan = (n.plan + 15) / 16 * 16;
   n.scores_ld = (max_kv_len + kBlock - 1) / kBlock * kBlock;
   n.scores = mass ? (size_t)U * T * std::min(H / G, 16) * n.scores_ld * sizeof(float) : 0;
+  if (n.scores > kMostScores) n.scores = 0;
   return n;
 }
 
@@ -702,7 +704,7 @@ int few_attention(const bf16* q, const bf16* sink, bf16* out, const AttnArgs& al
   f.abreast = f.U % few_warps_of(D) == 0 ? few_warps_of(D) : few_warps_of(D) % f.U == 0 ? f.U : 1;
   f.per = wide ? std::max(1, 16 / R) : max_q_len;
   f.plan = reinterpret_cast<int*>(ws);
-  f.scores = all.mass ? reinterpret_cast<float*>(ws + need.plan) : nullptr;
+  f.scores = need.scores > 0 ? reinterpret_cast<float*>(ws + need.plan) : nullptr;
   f.scores_ld = need.scores_ld;
   f.t_all = all.T;
   f.inv_r = (65536u + R - 1) / R;
@@ -733,6 +735,7 @@ int few_attention(const bf16* q, const bf16* sink, bf16* out, const AttnArgs& al
     if (rc != 0) return rc;
   }
   if (!all.mass) return 0;
+  if (!f.scores) return mass_rows(q, all, max_q_len, st);
   const int keys = (int)std::min((long)all.max_kv_len, all.mass_ld);
   f.a = all;
   return (int)follow(kv8_few_mass_kernel, dim3((keys + 255) / 256, all.pool.G, all.T), dim3(256), st, f);

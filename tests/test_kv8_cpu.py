@@ -66,6 +66,7 @@ def test_workspace_bytes(lib):
     ask = lambda T, H=4, G=2, D=64, V=64, f32=0, **o: lib.pk_kv8_attention_workspace_bytes(T, H, G, D, V, C.byref(ffi.Kv8Options(**{**dict(max_kv_len=100), **o})), f32)  # noqa: E731
     assert ask(0) == -1 and ask(1, H=3) == -1 and ask(1, D=40) == -1 and ask(1, max_kv_len=0) == -1
     assert ask(1) >= 0 and ask(7, mass=P, mass_ld=5) >= 7 * 4 * 4 and ask(1, max_kv_len=1 << 20) > 0
+    assert ask(256, 32, 8, max_kv_len=1 << 20, max_q_len=1, mass=P, mass_ld=1 << 20) < 1 << 28  # (the scores of all rows would be 34 GB)
     assert lib.pk_kv8_attention_workspace_bytes(1, 4, 2, 64, 64, None, 0) == -1
 
 

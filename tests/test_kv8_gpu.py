@@ -281,6 +281,12 @@ def test_options(lib, steps, opts):
     check_attention(lib, steps, 6, 2, 64, mass=True, seed=1, **o)
 
 
+@pytest.mark.parametrize("D", [64, 96])
+def test_weights_where_the_scores_are_not_kept(lib, D):
+    """2 GB of them by what max_kv_len allows"""
+    check_attention(lib, [(1, 400), (32, 31), (20, 129)], 32, 8, D, mass=True, longest=300000, window=100)
+
+
 @pytest.mark.parametrize("f32", [False, True])
 def test_weights_of_more_tokens_than_a_launch_looks_at(lib, f32):
     """65536; the portion of one request lies on both sides"""
