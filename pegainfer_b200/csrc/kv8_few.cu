@@ -36,7 +36,7 @@ struct FewArgs {
   int t_first, U, per;      // first token of the launch; tiles of a token (kv heads x sixteens of rows), tokens of a tile
   int abreast;              // warps that go through the same records of different tiles of a token
   int q_by4, out_by4;       // rows start on 8-byte boundaries
-  uint32_t inv_r;           // row / R = row * inv_r >> 16 for the rows of a tile
+  uint32_t inv_r;           // row / R = row * inv_r >> 16 for the rows of a tile of several tokens (at most 16 rows); 0 where a tile has one token's
   int* plan;                // [T + 1] records before a token's tiles, [T] the tile's first token, the length of a run: for the merge
   float* scores;            // scores (log2) for the weights' sums, or null: [tiles of a token][t_all][min(R, 16)][scores_ld], a tile's at its first token as [slot][row]
   int t_all;                // tokens of the call
@@ -707,7 +707,7 @@ int few_attention(const bf16* q, const bf16* sink, bf16* out, const AttnArgs& al
   f.scores = need.scores > 0 ? reinterpret_cast<float*>(ws + need.plan) : nullptr;
   f.scores_ld = need.scores_ld;
   f.t_all = all.T;
-  f.inv_r = (65536u + R - 1) / R;
+  f.inv_r = f.per > 1 ? (65536u + R - 1) / R : 0u;
   f.q_by4 = (reinterpret_cast<uintptr_t>(q) & 7) == 0;
   f.out_by4 = (reinterpret_cast<uintptr_t>(out) & 7) == 0 && all.out_ld % 4 == 0;
   f.err = wait_err_word();
