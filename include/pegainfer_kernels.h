@@ -732,7 +732,7 @@ long pk_kv8_page_bytes(int page_size, int kv_heads, int dim, int vdim);
 /* qkv [tokens, ld] = [q (heads*dim) | k (kv_heads*dim) | v (kv_heads*vdim)] (+ bias of the same layout, may be NULL): q and k rotate over their first `dims`
  * entries by positions[t] * freq[i] as in pk_gqa_rope_append (angles are reduced in 64 bits; those of bf16 q have sine and cosine to 2^-20); q goes to q_out [tokens, heads*dim], k and v into the cache at
  * slots[t] (slots NULL: at positions[t]).  heads may be 0 (rows of k and v alone, q_out NULL).  A request's tokens are consecutive rows with consecutive slots,
- * in one run per call.  A token at a record's first slot begins the record anew (slots behind the call's last are zero); else the record goes on from the slots
+ * in one run per call, in front of and behind which there may be rows without a slot, but none inside.  A token at a record's first slot begins the record anew (slots behind the call's last are zero); else the record goes on from the slots
  * before, whose codes are rounded again where its exponent grows.  Rows with a negative slot are not cached (their q is rotated all the same). */
 int pk_kv8_append(const void* qkv, int ld, const void* bias, const int* positions, const int* slots, const int* req, const int* page_off, const int* pages,
                   void* q_out, void* cache, long page_stride, int page_size, int heads, int kv_heads, int dim, int vdim, int dims, int interleaved,
@@ -753,7 +753,8 @@ typedef struct pk_kv8_options {
  * them, are separate; 16-byte aligned; any contents. */
 long pk_kv8_attention_workspace_bytes(int tokens, int heads, int kv_heads, int dim, int vdim, const pk_kv8_options* options, int f32);
 /* out[t,h] = sum_j w_j v_j, w = softmax over the visible slots j <= slots[t] of q[t,h] . k_j * scale (options applied; exp(sink[h]) added to the denominator when
- * sink != NULL).  A request's tokens are consecutive rows with ascending slots, in one run per call.  A row with a negative slot sees nothing: zeros. */
+ * sink != NULL).  A request's tokens are consecutive rows whose slots ascend by one at least, in one run per call; rows with a negative slot may lie anywhere, inside
+ * it too.  Such a row sees nothing: zeros. */
 int pk_kv8_attention(const void* q, const void* cache, const void* sink, const int* slots, const int* req, const int* page_off, const int* pages, void* out,
                      long page_stride, int page_size, int tokens, int heads, int kv_heads, int dim, int vdim, float scale, const pk_kv8_options* options,
                      void* workspace, long workspace_bytes, int f32, pk_stream st);

@@ -54,31 +54,48 @@ __device__ __forceinline__ Runs find_runs(uint32_t* starts, const AttnArgs& a) {
   __syncthreads();
   return Runs{starts, words, a.T};
 }
-// a run's largest and smallest slot, and where they are: slots ascend by one at least
+// a run's largest and smallest slot, where they are, and the rows without a slot between them: the others' slots ascend by one at least
 struct Ends {
-  int last, at_last, lowest, at_lowest;
+  int last, at_last, lowest, at_lowest, holes;
 };
 template <int WARPS>
-__device__ __forceinline__ Ends run_ends(int4* s_run, const AttnArgs& a, int t0, int t1) {
+struct RunRoom {
+  int4 ends[WARPS];
+  int valid[WARPS];
+};
+template <int WARPS>
+__device__ __forceinline__ Ends run_ends(RunRoom<WARPS>& room, const AttnArgs& a, int t0, int t1) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int last = -1, lowest = INT_MAX, at_last = -1, at_lowest = INT_MAX;
+  int last = -1, lowest = INT_MAX, at_last = -1, at_lowest = INT_MAX, valid = 0;
   for (int t = t0 + (int)threadIdx.x; t < t1; t += WARPS * 32) {
     const int p = a.slots[t];
+    valid += p >= 0;
     if (p >= 0 && p >= last) last = p, at_last = t;
     if (p >= 0 && p < lowest) lowest = p, at_lowest = t;
   }
-  const int wl = __reduce_max_sync(0xffffffffu, last), ws = __reduce_min_sync(0xffffffffu, lowest);
+  const int wl = __reduce_max_sync(0xffffffffu, last), ws = __reduce_min_sync(0xffffffffu, lowest), wv = __reduce_add_sync(0xffffffffu, valid);
   const int al = __reduce_max_sync(0xffffffffu, last == wl ? at_last : -1), as = __reduce_min_sync(0xffffffffu, lowest == ws ? at_lowest : INT_MAX);
   __syncthreads();  // (the words of a run before)
-  if (lane == 0) s_run[warp] = make_int4(wl, al, ws, as);
+  if (lane == 0) {
+    room.ends[warp] = make_int4(wl, al, ws, as);
+    room.valid[warp] = wv;
+  }
   __syncthreads();
-  const int4 x = s_run[lane % WARPS];
+  const int4 x = room.ends[lane % WARPS];
   Ends e;
   e.last = __reduce_max_sync(0xffffffffu, x.x);
   e.at_last = __reduce_max_sync(0xffffffffu, x.x == e.last ? x.y : -1);
   e.lowest = __reduce_min_sync(0xffffffffu, x.z);
   e.at_lowest = __reduce_min_sync(0xffffffffu, x.z == e.lowest ? x.w : INT_MAX);
+  e.holes = e.last < 0 ? 0 : e.at_last - e.at_lowest + 1 - (int)__reduce_add_sync(0xffffffffu, lane < WARPS ? room.valid[lane] : 0);
   return e;
+}
+// rows of a run that may see one of the keys key0 .. key1: from the first (before it the slots are below key0) to the second (from it on key1 is outside the window)
+struct Span {
+  int from, to;
+};
+__device__ __forceinline__ Span run_span(const Ends& e, int t0, int t1, int key0, int key1, int window) {
+  return Span{max(t0, e.at_last - (e.last - key0) - e.holes), window > 0 ? (int)min((long)t1, (long)e.at_lowest + e.holes + (key1 + (long)window - e.lowest)) : t1};
 }
 
 template <int D, int RECS>
@@ -88,7 +105,7 @@ __global__ void __launch_bounds__(kMassWarps * 32) kv8_mass_kernel(const bf16* _
   __shared__ __align__(8) float s_lse[2][kMassRows];  // log2; +inf: no such row
   __shared__ __align__(8) int s_p[2][kMassRows];
   __shared__ uint32_t ms_starts[kMassTokens / 32];
-  __shared__ int4 s_run[kMassWarps];
+  __shared__ RunRoom<kMassWarps> s_run;
   __shared__ int s_half[2][2];  // whether 32 rows see every key of the CTA
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gq = lane >> 2, tq = lane & 3, g = blockIdx.y, R = a.H / a.pool.G, V = a.pool.vdim;
   const int b0 = (blockIdx.x * kMassWarps + warp) * RECS;  // the warp's first record
@@ -102,7 +119,8 @@ __global__ void __launch_bounds__(kMassWarps * 32) kv8_mass_kernel(const bf16* _
     t1 = runs.after(t0);
     if (nth % (int)gridDim.z != (int)blockIdx.z) continue;
     const int req = a.req[t0];
-    const auto [last, at_last, lowest, at_lowest] = run_ends<kMassWarps>(s_run, a, t0, t1);
+    const Ends ends = run_ends<kMassWarps>(s_run, a, t0, t1);
+    const int last = ends.last, lowest = ends.lowest;
     if (key0 > last || (a.window > 0 && key1 <= lowest - a.window)) continue;  // (for all threads alike)
 
     // the warp's keys: a product's 16 tokens are a record's, its inner index the entries in order
@@ -144,8 +162,7 @@ __global__ void __launch_bounds__(kMassWarps * 32) kv8_mass_kernel(const bf16* _
       }
       cp_async_commit();
     };
-    // rows that see none of the CTA's keys: before token `from`, and from token `to` on where there is a window
-    const int from = max(t0, at_last - (last - key0)), to = a.window > 0 ? (int)min((long)t1, (long)at_lowest + (key1 + (long)a.window - lowest)) : t1;
+    const auto [from, to] = run_span(ends, t0, t1, key0, key1, a.window);
     const int tile0 = (int)((long)(from - t0) * R / kMassRows), tile1 = min(tiles, (int)(((long)(to - t0) * R + kMassRows - 1) / kMassRows));
     int s = 0;
     if (tile0 < tile1) load(tile0, 0);
@@ -246,7 +263,7 @@ __global__ void __launch_bounds__(kWideWarps * 32, 2) kv8_mass_wide_kernel(const
   __shared__ __align__(16) int s_p[4][kWideRows];
   __shared__ int s_all[4][kWideRows / 32];  // whether 32 rows see every key of the CTA
   __shared__ uint32_t ms_starts[kMassTokens / 32];
-  __shared__ int4 s_run[kWideWarps];
+  __shared__ RunRoom<kWideWarps> s_run;
   __shared__ uint64_t s_full[2], drained;
   __shared__ uint32_t tmem_slot;
   __shared__ int s_dead;
@@ -276,11 +293,11 @@ __global__ void __launch_bounds__(kWideWarps * 32, 2) kv8_mass_wide_kernel(const
     t1 = runs.after(t0);
     if (nth % (int)gridDim.z != (int)blockIdx.z) continue;
     const int req = a.req[t0];
-    const auto [last, at_last, lowest, at_lowest] = run_ends<kWideWarps>(s_run, a, t0, t1);
+    const Ends ends = run_ends<kWideWarps>(s_run, a, t0, t1);
+    const int last = ends.last, lowest = ends.lowest;
     if (key0 > last || (a.window > 0 && key1 <= lowest - a.window)) continue;  // (for all threads alike)
-    // rows that see none of the CTA's keys: before token `from`, and from token `to` on where there is a window
     const int rows = (t1 - t0) * R, tiles = (rows + kWideRows - 1) / kWideRows;
-    const int from = max(t0, at_last - (last - key0)), to = a.window > 0 ? (int)min((long)t1, (long)at_lowest + (key1 + (long)a.window - lowest)) : t1;
+    const auto [from, to] = run_span(ends, t0, t1, key0, key1, a.window);
     const int tile0 = (int)((long)(from - t0) * R / kWideRows), count = min(tiles, (int)(((long)(to - t0) * R + kWideRows - 1) / kWideRows)) - tile0;
     const bf16* q_run = q + ((size_t)t0 * a.H + g * R) * D;
     auto by_r = [&](int at) { return (int)((unsigned long long)(uint32_t)at * r_inv >> 32); };
@@ -455,7 +472,7 @@ constexpr int kPlainWarps = 8, kPlainRows = 4;
 template <typename E>
 __global__ void __launch_bounds__(kPlainWarps * 32) kv8_mass_plain_kernel(const E* __restrict__ q, AttnArgs a) {
   __shared__ uint32_t ms_starts[kMassTokens / 32];
-  __shared__ int4 s_run[kPlainWarps];
+  __shared__ RunRoom<kPlainWarps> s_run;
   __shared__ float s_sum[kPlainWarps][kBlock];
   pdl_wait();
   pdl_launch_dependents();
@@ -468,9 +485,10 @@ __global__ void __launch_bounds__(kPlainWarps * 32) kv8_mass_plain_kernel(const 
     t1 = runs.after(t0);
     if (nth % (int)gridDim.z != (int)blockIdx.z) continue;
     const int req = a.req[t0];
-    const auto [last, at_last, lowest, at_lowest] = run_ends<kPlainWarps>(s_run, a, t0, t1);
+    const Ends ends = run_ends<kPlainWarps>(s_run, a, t0, t1);
+    const int last = ends.last, lowest = ends.lowest;
     if (key0 > last || (a.window > 0 && key1 <= lowest - a.window)) continue;  // (for all threads alike)
-    const int from = max(t0, at_last - (last - key0)), to = a.window > 0 ? (int)min((long)t1, (long)at_lowest + (key1 + (long)a.window - lowest)) : t1;
+    const auto [from, to] = run_span(ends, t0, t1, key0, key1, a.window);
     const uint8_t* rec = a.pool.record(req, key0, g);
     const float ek = pow2(tail_ek(*reinterpret_cast<const uint32_t*>(rec + kBlock * (D + V))));
     const uint8_t* k = rec + (tok >> 3) * (8 * D) + part * chunks * 128 + (tok & 7) * 16;

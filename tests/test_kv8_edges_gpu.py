@@ -76,3 +76,33 @@ def test_groups_of_many_heads(lib, R):
     c = filled([41, 7, 300], 1, 32, 32, 16)
     check(lib, c, rows(3, R, 32, BF16), [40, 6, 299], [0, 1, 2], [41, 7, 300], 0.2)
     check(lib, c, rows(5, R, 32, BF16), [38, 39, 40, 6, 299], [0, 0, 0, 1, 2], [41, 7, 300], 0.2, sink=rows(1, R, 1, BF16).view(R), max_q=0)
+
+
+# ------------------------------------------------------------------ padding
+def holes(n, pattern):
+    """slots 0 .. n - 1 with rows of no slot in between: (valid, padding) by turns"""
+    out, s, i = [], 0, 0
+    while s < n:
+        a, b = pattern[i % len(pattern)]
+        out += list(range(s, min(n, s + a))) + [-1] * b
+        s, i = s + a, i + 1
+    return out
+
+
+@pytest.mark.parametrize("H,G,D,V,f32", [(8, 2, 64, 64, False), (4, 1, 128, 128, False), (8, 2, 96, 96, False), (6, 2, 32, 32, False), (6, 2, 192, 192, False), (4, 2, 64, 32, False),
+                                         (4, 2, 64, 64, True), (3, 1, 96, 160, True)])
+@pytest.mark.parametrize("pattern", [[(1, 1)], [(30, 100), (7, 1)], [(1, 300), (150, 2)]], ids=["each", "some", "many"])
+@pytest.mark.parametrize("window", [0, 40])
+def test_padding_inside_a_request(lib, H, G, D, V, f32, pattern, window):
+    """rows without a slot between the others: every key has the weights of all rows that see it"""
+    n = 200
+    slots = [-1, -1] + holes(n, pattern) + [-1]
+    T = len(slots)
+    c = filled([n, 17], G, D, V, 16)
+    check(lib, c, rows(T + 1, H, D, F32 if f32 else BF16), slots + [16], [0] * T + [1], [n, 17], D ** -0.5, window=window)
+
+
+@pytest.mark.parametrize("f32", [False, True])
+def test_padding_between_three_tokens(lib, f32):
+    c = filled([34], 2, 64, 64, 16)
+    check(lib, c, rows(3, 4, 64, F32 if f32 else BF16), [32, -1, 33], [0, 0, 0], [34], 0.125)
