@@ -10,13 +10,15 @@
 //     short one; a tile of up to 16 rows (WIDE) takes two.  K's and V's codes become f16 in registers (exactly; two codes an instruction), q becomes f16 with a power of
 //     two for each row that puts its largest entry at 2^14 .. 2^15 (bf16 entries down to 2^-21 of it stay exact), and P, which is held 2^15 times too large,
 //     keeps 11 bits down to 2^-29.  movmatrix turns P.  (The e4m3 form of mma.sync is two of these products and a conversion of both operands each time.)
-//   * Scores: the exponents of K and of the row's q multiply them.  P takes V's exponent e in as 2^(e - E), E the largest so far, so that records of different
-//     exponents add up.
+//   * Scores: the exponents of K and of the row's q multiply them.  P takes V's exponent e in as 2^(e - E), E the largest so far, which costs P up to kNear of its 29 bits of
+//     range while V's exponents lie no further apart; once they do, every row has its own E, m + E being its largest (score + e) so far: what a row does not see, or gives no
+//     weight, costs its other tokens no bits, however large its values.  (One way for all calls: 3 to 10 % slower, groups of 16 heads of 64 most, 37 -> 41 us.)
 // A group of more than 16 heads is several tiles, which read the records again (from L2).
 // B200: 32 requests of about 3350, 32 heads of 128 in 8 groups (229 MB): 45 us (5.1 TB/s), and 6 for the pieces; one request of 301: 7.5 and 5.4, latency; 48 requests in a
 // window of 1024, 64 heads of 64 in 8 groups, scores capped (50 MB): 25 us, of which 8 are start and end, the rest the instructions of a stage (its 4 KB are half as
 // many as at 128 entries, the maxima, sums and caps of its 32 tokens as many).
 #include <algorithm>
+#include <type_traits>
 
 #include "kv8_attention.cuh"
 #include "mma.cuh"
@@ -25,6 +27,8 @@ namespace pk {
 namespace kv8 {
 
 constexpr size_t kMostScores = (size_t)1 << 30;  // bytes that are kept for the weights' sums; with more the scores are computed again (kv8_mass.cu)
+constexpr float kNoneYet = -1000.f;  // E of a row that has seen nothing
+constexpr int kNear = 8;             // V's exponents within so much: one E for all rows
 constexpr int kFewTokens = 512;  // of a launch: their tiles are looked up in shared memory
 template <int D>
 constexpr int few_warps() { return D <= 128 ? 8 : 4; }
@@ -285,6 +289,11 @@ __global__ void __launch_bounds__(few_warps<D>() * 32, 1) kv8_few_kernel(const b
   const uint32_t v_at = (uint32_t)(kBlock * D + (mi & 1) * 128 + mr * 16);
   const int tok[2] = {token_of(0, gq), token_of(1, gq)};  // this thread's tokens of a record
   const float c = a.scale * kLog2e, cap2 = a.cap * kLog2e, cap_c = a.cap > 0.f ? 2.f * a.scale / a.cap * kLog2e : 0.f;
+  auto max_of_rows = [](float x) {  // over the lanes that have other tokens of the same rows
+    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+    return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+  };
 
   uint32_t parity = 0;
   int slot = 0;
@@ -352,13 +361,24 @@ __global__ void __launch_bounds__(few_warps<D>() * 32, 1) kv8_few_kernel(const b
       while (tile_rows < 16 && token(row0 + tile_rows) >= 0) tile_rows += R <= 16 ? R : 1;
       kept = f.scores + ((size_t)unit * f.t_all + f.t_first + t) * min(R, 16) * f.scores_ld;
     }
-    int E = kLowExp - 1, j0 = (s_b0[t] + cc.rec) * kBlock;
-    for (int i = 0; i < count; j0 += 2 * kBlock) {
-      const int take = min(2, count - i);
+    int done = 0, j0 = (s_b0[t] + cc.rec) * kBlock;
+    // l is held relative to 2^m, O to 2^(m + E), where E is one number for all rows first, and a row's own from the stage on whose V's exponents lie too far apart
+    int E = kLowExp - 1, e_low = INT_MAX;  // V's largest and smallest exponent so far
+    float E_row[2 * NT];
+    // A stage; false: its V's exponents lie too far from the others, nothing has happened
+    auto weigh = [&](auto each) {
+      constexpr bool EACH = decltype(each)::value;
+      const int take = min(2, count - done);
       if (alive) alive = mbar_wait_bounded(&s_full[warp][slot], parity, dead);
       __syncwarp();
       const uint8_t* stage = ring + slot * 2 * REC;
       const uint32_t at = smem_u32(stage), second = take == 2 ? REC : 0;  // (a missing second record: the first again, with P = 0)
+      const uint32_t tail_a = *reinterpret_cast<const uint32_t*>(stage + kBlock * 2 * D), tail_b = *reinterpret_cast<const uint32_t*>(stage + second + kBlock * 2 * D);
+      const int ea = tail_ev(tail_a), eb = tail_ev(tail_b), e_new = max(E, max(ea, eb));
+      if constexpr (!EACH) {
+        e_low = min(e_low, min(ea, eb));
+        if (e_new - e_low > kNear) return false;
+      }
       float s[2][NT][4] = {};
 #pragma unroll
       for (int kk = 0; kk < D / 32; ++kk) {
@@ -376,17 +396,14 @@ __global__ void __launch_bounds__(few_warps<D>() * 32, 1) kv8_few_kernel(const b
           }
         }
       }
-      const uint32_t tail_a = *reinterpret_cast<const uint32_t*>(stage + kBlock * 2 * D), tail_b = *reinterpret_cast<const uint32_t*>(stage + second + kBlock * 2 * D);
       const bool inside = j0 >= all_lo && j0 + 31 <= all_p && take == 2;
-      const int ea = tail_ev(tail_a), eb = tail_ev(tail_b), e_new = max(E, max(ea, eb));
-      const float fe = pow2(max(E - e_new, -126)), fka = pow2(tail_ek(tail_a)), fkb = pow2(tail_ek(tail_b));
-      E = e_new;
+      const float fe = EACH ? 1.f : pow2(max(E - e_new, -126)), fka = pow2(tail_ek(tail_a)), fkb = pow2(tail_ek(tail_b));
       float fo[2 * NT], ref[2 * NT];
       bool same = true;
 #pragma unroll
       for (int i2 = 0; i2 < 2 * NT; ++i2) {
         const int w = i2 >> 1, e = i2 & 1;
-        float mx = m[i2];
+        float most[2] = {-INFINITY, -INFINITY};
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           const float fk = (r ? fkb : fka) * row_c[i2];
@@ -399,19 +416,24 @@ __global__ void __launch_bounds__(few_warps<D>() * 32, 1) kv8_few_kernel(const b
               v = j >= lo[i2] && j <= p[i2] && r < take ? v : -INFINITY;
             }
             s[r][w][2 * y + e] = v;
-            mx = fmaxf(mx, v);
+            most[r] = fmaxf(most[r], v);
           }
         }
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+        const float mx = max_of_rows(fmaxf(m[i2], fmaxf(most[0], most[1])));
         ref[i2] = mx == -INFINITY ? 0.f : mx;
         const float fl = ex2(m[i2] - ref[i2]);
-        fo[i2] = fl * fe;
+        if constexpr (EACH) {
+          const float E_old = m[i2] == -INFINITY ? kNoneYet : E_row[i2] - (mx - m[i2]);
+          E_row[i2] = fmaxf(E_old, max_of_rows(fmaxf(most[0] - ref[i2] + (float)ea, most[1] - ref[i2] + (float)eb)));
+          fo[i2] = ex2(E_old - E_row[i2]);
+        } else {
+          fo[i2] = fl * fe;
+        }
         same = same && fo[i2] == 1.f;
         m[i2] = mx;
         l[i2] *= fl;
       }
+      if constexpr (!EACH) E = e_new;
       if constexpr (SCORES) {  // [slot][row of the tile]
 #pragma unroll
         for (int w = 0; w < NT; ++w)
@@ -441,16 +463,19 @@ __global__ void __launch_bounds__(few_warps<D>() * 32, 1) kv8_few_kernel(const b
       uint32_t pb[2][2 * NT];  // of a record: tokens 4 tq, 4 tq + 1 and 4 tq + 2, 4 tq + 3 of row gq
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        const float fv = pow2(max((r ? eb : ea) - E, -100) + kTopP);
+        const float fv = EACH ? 0.f : pow2(max((r ? eb : ea) - E, -100) + kTopP);
 #pragma unroll
         for (int w = 0; w < NT; ++w) {
           uint32_t y[2];
+          // (more than 2^85 only where the weights are nothing: a product with infinity would not be)
+          auto own = [&](int i2) { return ex2(fminf((float)(r ? eb : ea) - E_row[i2], 85.f) + (float)kTopP); };
+          const float f0 = EACH ? own(2 * w) : fv, f1 = EACH ? own(2 * w + 1) : fv;
 #pragma unroll
           for (int n = 0; n < 2; ++n) {
             const float p0 = ex2(s[r][w][2 * n] - ref[2 * w]), p1 = ex2(s[r][w][2 * n + 1] - ref[2 * w + 1]);
             l[2 * w] += p0;
             l[2 * w + 1] += p1;
-            y[n] = turned(pack_f16(p0 * fv, p1 * fv));
+            y[n] = turned(pack_f16(p0 * f0, p1 * f1));
           }
           pb[r][2 * w] = tq < 2 ? y[0] : y[1];
           pb[r][2 * w + 1] = tq < 2 ? y[1] : y[0];
@@ -469,7 +494,8 @@ __global__ void __launch_bounds__(few_warps<D>() * 32, 1) kv8_few_kernel(const b
           for (int w = 0; w < NT; ++w) mma_f16(o[d][w], a0, a1, a2, a3, pb[r][2 * w], pb[r][2 * w + 1]);
         }
       }
-      i += take;
+      done += take;
+      j0 += 2 * kBlock;
       __syncwarp();
       if (alive && p_take > 0) {  // this stage is free again
         ++issued;
@@ -484,9 +510,16 @@ __global__ void __launch_bounds__(few_warps<D>() * 32, 1) kv8_few_kernel(const b
         slot = 0;
         parity ^= 1u;
       }
+      return true;
+    };
+    bool near = true;
+    while (near && done < count) near = weigh(std::false_type{});
+    if (!near) {
+#pragma unroll
+      for (int i = 0; i < 2 * NT; ++i) E_row[i] = m[i] == -INFINITY ? kNoneYet : (float)E;
+      while (done < count) weigh(std::true_type{});
     }
     // ---- the piece's state: the accumulated values are turned back in shared memory, so that rows leave in 16-byte pieces
-    const float up = pow2(max(E, kLowExp) - kTopP);
     const bool whole = count == cc.n;
     const size_t part = (((size_t)who + (size_t)t * U + cc.u) * AB + mine) * (8 * NT);
 #pragma unroll
@@ -499,7 +532,7 @@ __global__ void __launch_bounds__(few_warps<D>() * 32, 1) kv8_few_kernel(const b
         sum += __shfl_xor_sync(0xffffffffu, sum, 8);
         sum += __shfl_xor_sync(0xffffffffu, sum, 16);
         const float top = sum != sum ? INFINITY : m[2 * w + e];  // a NaN among the scores: no other piece may hide it
-        float fac = up;
+        float fac = near ? pow2(max(E, kLowExp) - kTopP) : ex2(E_row[2 * w + e] - (float)kTopP);  // (of a row that saw nothing: 0)
         if (whole) {
           const RowEnd end = row_end(top, sum, sink ? bf2f(sink[h]) : 0.f, sink != nullptr);
           fac *= end.factor;

@@ -8,7 +8,8 @@
 //     end of the codes' range: a bf16 entry is exact down to 2^-17 of the row's largest.
 //   * O += P V in f16: the warps that rescale O turn a block's V into f16 (exactly) before, once for both tiles' 256 rows, which is an eighth of the instructions that
 //     P in two 8-bit parts takes (B200, prompt of 4096, 32 heads in 8 groups: 240 us so).
-//   * K's exponents multiply the scores 16 columns at a time, V's go into P's exponent: 2^(s - m + e - E + 7), E the largest so far; the denominator takes them out.
+//   * K's exponents multiply the scores 16 columns at a time, V's go into P's exponent: 2^(s - m + e - E + 7), m + E the row's largest s + e so far, so that what a row does not
+//     see, or gives no weight, costs its other tokens no bits, however large its values; the denominator takes them out.
 //   * Blocks of 64 keys with two S per tile: S of the block after next is issued behind P V of this one, so the softmax finds its scores waiting.  (Blocks of 128 with one S: a
 //     tile waited 1600 of 5200 clocks for it.)
 //   * m is a maximum of before that the row's own may have passed by up to 2^8: O, which stays in tensor memory, is rescaled only where one did by more.  P, held 2^7 times
@@ -33,6 +34,7 @@ constexpr int kPrCorr = 8, kPrMma = 12, kPrLoad = 14, kPrThreads = 16 * 32;
 constexpr int kPrRegsSoft = 192, kPrRegsCorr = 80, kPrRegsMma = 48;
 static_assert(256 * kPrRegsSoft + 128 * kPrRegsCorr + 128 * kPrRegsMma <= kPrThreads * (65536 / kPrThreads), "more registers than the block was launched with");
 constexpr int kPrTop = 7, kPrSlack = 8;  // exponents of P = 1 and of what a row's maximum may grow by before O is rescaled: 2^15 in f16
+constexpr float kPrNone = -1000.f;  // E of a row that has seen nothing
 constexpr uint32_t kRestA = 1u << 7;  // instruction descriptor: A is e5m2
 constexpr int kPrMaxSeg = 256;     // runs that a CTA's tokens can belong to
 
@@ -49,6 +51,9 @@ __device__ __forceinline__ float pr_ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// whole numbers of a few bits: as a float, and two to them (-126 .. 127), in the ordinary pipes
+__device__ __forceinline__ float small_float(int x) { return __int_as_float(0x4b400000 + x) - 12582912.f; }
+__device__ __forceinline__ float whole_pow2(float x) { return __int_as_float(__float_as_int(x + (12582912.f + 127.f)) << 23); }
 __device__ __forceinline__ void pr_fma2(float& x0, float& x1, float s, float c) {
   unsigned long long v, sv, cv;
   asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x0), "f"(x1));
@@ -547,8 +552,8 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* _
 
     const uint32_t t_tile = tmem_base + ((uint32_t)(q4 * 32) << 16) + (uint32_t)(i * 2 * kPrKeys);
     const float cap2 = a.cap * kLog2e, cap_c = a.cap > 0.f ? 2.f * a.scale / a.cap * kLog2e : 0.f;
-    float m = -INFINITY, l = 0.f;
-    int E = kLowExp - 1, mine = 0;
+    float m = -INFINITY, l = 0.f, E = kPrNone;  // l is held relative to 2^m, O to 2^(m + E); both are whole numbers, so that every rescaling is exact
+    int mine = 0;
     for (Step x = begin(); x.seg < segs; next(x)) {
       if (!needs(i, x.seg, x.j)) continue;
       const int sv = x.n % kPrStagesV;
@@ -560,15 +565,13 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* _
       tmem_ld32_nowait(t_s, v);
       tmem_ld32_nowait(t_s + 32, v + 32);
       mbar_wait_bounded(h_full + sv, (uint32_t)((x.n / kPrStagesV) & 1), dead, tries);
-      int ev[kPrRecords], e_new = E;
-      float fk[kPrRecords];
+      float ev[kPrRecords], fk[kPrRecords];
 #pragma unroll
       for (int b = 0; b < kPrRecords; ++b) {
         const uint32_t tail = Es[sv * kPrRecords + b];
-        ev[b] = tail_ev(tail);
+        ev[b] = small_float(tail_ev(tail));
         const float y = pow2(tail_ek(tail)) * row_c;
         fk[b] = y < 1e-37f ? 1e-37f : y;  // never zero: -inf times it stays -inf (and a NaN stays one)
-        e_new = max(e_new, ev[b]);
       }
       const int c0 = my_seg == x.seg ? max(lo - x.j * kPrKeys, 0) : kPrKeys, c1 = my_seg == x.seg ? min(p - x.j * kPrKeys, kPrKeys - 1) : -1;  // the columns that the row sees
       const bool masked = !__all_sync(0xffffffffu, c0 <= 0 && c1 >= kPrKeys - 1);
@@ -584,7 +587,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* _
         for (int k = 0; k < kPrKeys; ++k)
           if (k < c0 || k > c1) v[k] = 0xff800000u;
       }
-      float mx = m;
+      float mx = m, high = -INFINITY;  // largest score, and with V's exponent added
 #pragma unroll
       for (int b = 0; b < kPrRecords; ++b) {
         float y = fmaxf(__uint_as_float(v[b * 16]), __uint_as_float(v[b * 16 + 1])), z = fmaxf(__uint_as_float(v[b * 16 + 2]), __uint_as_float(v[b * 16 + 3]));
@@ -593,23 +596,27 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* _
           y = fmaxf(fmaxf(y, __uint_as_float(v[b * 16 + k])), __uint_as_float(v[b * 16 + k + 1]));
           z = fmaxf(fmaxf(z, __uint_as_float(v[b * 16 + k + 2])), __uint_as_float(v[b * 16 + k + 3]));
         }
-        mx = fmaxf(mx, fmaxf(y, z) * factor(b));
+        y = fmaxf(y, z) * factor(b);
+        mx = fmaxf(mx, y);
+        high = fmaxf(high, y + ev[b]);
       }
-      const float m_new = mx > m + (float)kPrSlack ? mx : m;  // (m = -inf: mx)
-      const float ref = m_new == -INFINITY ? 0.f : m_new, fl = pr_ex2(m - ref);
+      const float m_new = mx > m + (float)kPrSlack ? ceilf(mx) : m;  // (m = -inf: mx)
+      const float ref = m_new == -INFINITY ? 0.f : m_new, grown = m == -INFINITY ? 0.f : fminf(m_new - m, 2000.f);
+      high = fmaf(fabsf(ref), 1.2e-7f, high - ref);  // (and what its sum was rounded by, so that P stays in range)
+      const float E_old = E - grown, E_new = high > E_old + (float)kPrSlack ? ceilf(high) : E_old;
       // (a row that saw nothing so far has nothing in O; nothing is rescaled at the first block)
-      alpha_s[(i * 2 + (mine & 1)) * kPrRows + r] = (m == -INFINITY ? 1.f : fl) * pow2(max(E - e_new, -126));
+      alpha_s[(i * 2 + (mine & 1)) * kPrRows + r] = m == -INFINITY ? 1.f : whole_pow2(fmaxf(E_old - E_new, -126.f));
       __syncwarp();
       if (lane == 0) mbar_arrive(a_ready + i * 2 + (mine & 1));
       m = m_new;
-      E = e_new;
-      l *= fl;
+      E = E_new;
+      l *= whole_pow2(fmaxf(-grown, -126.f));
       // P of 16 columns -> eight columns
       uint32_t w[kPrKeys / 2];
 #pragma unroll
       for (int b = 0; b < kPrRecords; ++b) {
-        const int shift = max(ev[b] - E, -60) + kPrTop;
-        const float fb = factor(b), add = (float)shift - ref;
+        // (more than 2^110 only where the weights are nothing)
+        const float shift = fminf(fmaxf(ev[b] - E, -60.f), 110.f) + (float)kPrTop, fb = factor(b), add = shift - ref;
         float d0 = 0.f, d1 = 0.f;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
@@ -620,7 +627,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* _
           pr_add2(d0, d1, s0, s1);
           w[b * 8 + k] = pr_pack(s0, s1);
         }
-        l = fmaf(d0 + d1, pow2(-shift), l);
+        l = fmaf(d0 + d1, whole_pow2(-shift), l);
       }
       tmem_put32(t_s, w);
       tmem_put_wait();
@@ -630,7 +637,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* _
       ++mine;
     }
     const float top = l != l ? INFINITY : m;  // a NaN among the scores
-    const float up = pow2(max(E, kLowExp) - kPrTop);
+    const float up = whole_pow2(fmaxf(E, (float)(kLowExp - kPrSlack - 1)) - (float)kPrTop);
     if constexpr (CUT) {  // a share's state: kv8_merge_kernel
       end_s[i * kPrRows + r] = up;
       if (on) a.part_ml[((size_t)blockIdx.x * a.T + t0 + ti) * a.H + h] = make_float2(top, l);

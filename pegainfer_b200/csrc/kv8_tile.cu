@@ -5,7 +5,8 @@
 //   * mma.sync m16n8k16 in f16: codes widen exactly.  A row of q is scaled by a power of two that puts its largest entry at 2^14 .. 2^15; bf16 entries fit one f16 (down to
 //     2^-21 of the row's largest), fp32 ones go in as the nearest f16 and the rest (22 bits).  So do the weights P, held 2^15 times too large.
 //   * The inner indices of both products are permuted so that four consecutive codes are what a thread needs of K (entries) and of V (tokens).
-//   * K's exponents multiply the scores, V's go into P relative to E, the largest so far.
+//   * K's exponents multiply the scores, V's go into P relative to the row's largest (score + exponent) so far, m + X: what a row does not see, or gives no weight, costs its
+//     other tokens no bits, however large its values.  m and X are whole numbers, so that every rescaling is exact.
 // Bound by the products where rows are many: two of them for each fp32 one.
 #include <algorithm>
 
@@ -16,6 +17,7 @@ namespace pk {
 namespace kv8 {
 
 constexpr int kTileWarps = 4, kTileRows = kTileWarps * 16, kTileRecs = 4, kTileKeys = kTileRecs * kBlock;
+constexpr int kNone = -1000;  // X of a row that has seen nothing
 
 __device__ __forceinline__ void rest_f16(float lo, float hi, uint32_t near, uint32_t& rest) {
   const float2 n = __half22float2(*reinterpret_cast<const __half2*>(&near));
@@ -24,7 +26,7 @@ __device__ __forceinline__ void rest_f16(float lo, float hi, uint32_t near, uint
 
 // VM: the values' size at most
 template <typename E, int VM>
-__global__ void __launch_bounds__(kTileWarps * 32) kv8_tile_kernel(const E* __restrict__ q, const E* __restrict__ sink, E* __restrict__ out, AttnArgs a, int per, int slices) {
+__global__ void __launch_bounds__(kTileWarps * 32, VM > 128 ? 2 : VM > 64 || sizeof(E) == 4 ? 3 : 4) kv8_tile_kernel(const E* __restrict__ q, const E* __restrict__ sink, E* __restrict__ out, AttnArgs a, int per, int slices) {
   constexpr int PARTS = sizeof(E) == 4 ? 2 : 1;
   extern __shared__ __align__(16) uint8_t tl_sm[];
   __shared__ int s_slot[kTileRows], s_req[kTileRows];
@@ -142,7 +144,7 @@ __global__ void __launch_bounds__(kTileWarps * 32) kv8_tile_kernel(const E* __re
   const uint32_t k_at = (uint32_t)((mt >> 3) * (8 * D) + (mi >> 1) * 128 + (mt & 7) * 16), v_at = (uint32_t)(kBlock * D + (mi * 8 + mr) * 16);
   const uint32_t ring_at = smem_u32(ring);
   const uint32_t* q_row = reinterpret_cast<const uint32_t*>(qs + (warp * 16 + gq) * LD + 4 * tq);
-  int Ev = kLowExp - 1, s = 0;
+  int X[2] = {kNone, kNone}, s = 0;  // l is held relative to 2^m, O to 2^(m + X)
   if (now.from < n_tok && left > 0) load(now, 0);
   while (now.from < n_tok && left > 0) {
     Step after = now;
@@ -182,8 +184,8 @@ __global__ void __launch_bounds__(kTileWarps * 32) kv8_tile_kernel(const E* __re
       }
     }
     // scores: this thread's tokens of a record are 4 tq + 2 n + e, its rows gq and gq + 8
-    int ev[kTileRecs], E_new = Ev;
-    float mx[2] = {m[0], m[1]};
+    int ev[kTileRecs];
+    float mx[2] = {-INFINITY, -INFINITY}, high[2] = {-INFINITY, -INFINITY};  // largest score, and with V's exponent added
 #pragma unroll
     for (int r = 0; r < kTileRecs; ++r) {
       ev[r] = kLowExp;
@@ -191,10 +193,10 @@ __global__ void __launch_bounds__(kTileWarps * 32) kv8_tile_kernel(const E* __re
         const uint32_t tail = *reinterpret_cast<const uint32_t*>(ring + ((size_t)s * kTileRecs + r) * REC + kBlock * (D + V));
         const float fk = pow2(tail_ek(tail));
         ev[r] = tail_ev(tail);
-        E_new = max(E_new, ev[r]);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const float f = fk * row_c[i];
+          float most = -INFINITY;
           const bool in = mine[i] >= now.from && mine[i] < now.to;
 #pragma unroll
           for (int n = 0; n < 2; ++n)
@@ -203,8 +205,10 @@ __global__ void __launch_bounds__(kTileWarps * 32) kv8_tile_kernel(const E* __re
               const int j = now.j * kTileKeys + r * kBlock + 4 * tq + 2 * n + e;
               const float v = in && j >= lo[i] && j <= p[i] ? shaped(acc[r][n][2 * i + e] * f, c, a.cap) : -INFINITY;
               acc[r][n][2 * i + e] = v;
-              mx[i] = fmaxf(mx[i], v);
+              most = fmaxf(most, v);
             }
+          mx[i] = fmaxf(mx[i], most);
+          high[i] = fmaxf(high[i], most + (float)ev[r]);
         }
       }
     }
@@ -213,13 +217,17 @@ __global__ void __launch_bounds__(kTileWarps * 32) kv8_tile_kernel(const E* __re
     for (int i = 0; i < 2; ++i) {
       mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
       mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
-      ref[i] = mx[i] == -INFINITY ? 0.f : mx[i];
-      fo[i] = ex2(m[i] - ref[i]);
-      m[i] = mx[i];
-      l[i] *= fo[i];
-      fo[i] *= pow2(max(Ev - E_new, -126));
+      const float m_new = fmaxf(m[i], ceilf(mx[i]));
+      ref[i] = m_new == -INFINITY ? 0.f : m_new;
+      high[i] = fmaxf(high[i], __shfl_xor_sync(0xffffffffu, high[i], 1));
+      high[i] = fmaxf(high[i], __shfl_xor_sync(0xffffffffu, high[i], 2));
+      const float e = fmaf(fabsf(ref[i]), 1.2e-7f, high[i] - ref[i]);  // (and what its sum was rounded by, so that P stays in range)
+      const int grown = m[i] == -INFINITY ? 0 : (int)fminf(m_new - m[i], 2000.f), X_old = X[i] - grown;
+      X[i] = max(X_old, (int)ceilf(fminf(fmaxf(e, (float)kNone), 1000.f)));
+      fo[i] = pow2(max(X_old - X[i], -126));
+      l[i] *= pow2(max(-grown, -126));
+      m[i] = m_new;
     }
-    Ev = E_new;
     if (fo[0] != 1.f || fo[1] != 1.f) {
 #pragma unroll
       for (int i = 0; i < VM / 8; ++i) {
@@ -230,16 +238,18 @@ __global__ void __launch_bounds__(kTileWarps * 32) kv8_tile_kernel(const E* __re
 #pragma unroll
     for (int r = 0; r < kTileRecs; ++r) {
       if (r >= recs) break;
-      const float up = pow2(max(ev[r] - Ev, -110) + kTopP);
       uint32_t x[PARTS][4];
+      float up[2];  // (more than 2^100 only where the weights are nothing)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) up[i] = pow2(min(max(ev[r] - X[i], -110), 100) + kTopP);
 #pragma unroll
       for (int n = 0; n < 2; ++n)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const float w0 = ex2(acc[r][n][2 * i] - ref[i]), w1 = ex2(acc[r][n][2 * i + 1] - ref[i]);
           l[i] += w0 + w1;
-          x[0][2 * n + i] = pack_f16(w0 * up, w1 * up);
-          if (PARTS == 2) rest_f16(w0 * up, w1 * up, x[0][2 * n + i], x[PARTS - 1][2 * n + i]);
+          x[0][2 * n + i] = pack_f16(w0 * up[i], w1 * up[i]);
+          if (PARTS == 2) rest_f16(w0 * up[i], w1 * up[i], x[0][2 * n + i], x[PARTS - 1][2 * n + i]);
         }
 #pragma unroll
       for (int d = 0; d < VM / 32; ++d) {
@@ -262,9 +272,9 @@ __global__ void __launch_bounds__(kTileWarps * 32) kv8_tile_kernel(const E* __re
   asm volatile("cp.async.wait_all;" ::: "memory");
 
   // ---- results: rows gq and gq + 8, entries 8 i + 2 tq + e
-  const float unit = pow2(max(Ev, kLowExp) - kTopP);
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
+    const float unit = pow2(max(X[i], kLowExp) - kTopP);
     l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
     l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
     if (mine[i] < 0) continue;

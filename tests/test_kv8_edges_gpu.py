@@ -106,3 +106,101 @@ def test_padding_inside_a_request(lib, H, G, D, V, f32, pattern, window):
 def test_padding_between_three_tokens(lib, f32):
     c = filled([34], 2, 64, 64, 16)
     check(lib, c, rows(3, 4, 64, F32 if f32 else BF16), [32, -1, 33], [0, 0, 0], [34], 0.125)
+
+
+# ------------------------------------------------------------------ records of different sizes
+def sized(lens, G, D, V, factors, seed=0, page=16, push=0.0):
+    """factors: (request, first record, last record, factor of the values, push of the keys' first entry)"""
+    c = K.Cache(lens, G, D, V, page, seed=seed)
+    g = torch.Generator().manual_seed(seed + 1)
+    for r, n in enumerate(lens):
+        k, v = torch.randn(n, G, D, generator=g).to(BF16).double(), torch.randn(n, G, V, generator=g).to(BF16).double()
+        for q, a, b, f, x in factors:
+            if q == r:
+                v[a * 16:b * 16 + 16] *= f
+                k[a * 16:b * 16 + 16, :, 0] += x
+        K.fill(c, r, k, v)
+    c.data, c.page_off, c.pages = c.data.to(DEV), c.page_off.to(DEV), c.pages.to(DEV)
+    return c
+
+
+FORMS = [(8, 2, 64, 64, False), (16, 4, 128, 128, False), (3, 1, 96, 96, False), (6, 2, 32, 32, False), (4, 1, 192, 192, False), (4, 2, 64, 96, False), (8, 2, 64, 64, True), (3, 3, 128, 32, True)]
+
+
+@pytest.mark.parametrize("H,G,D,V,f32", FORMS)
+@pytest.mark.parametrize("big", [1e12, 1e-12, 1e30])
+@pytest.mark.parametrize("which", [0, 1])
+def test_large_values_of_another_request(lib, H, G, D, V, f32, big, which):
+    """rows of several requests in one tile, one of them with far larger values: the others are as if it were not there"""
+    lens = [70, 75, 71, 33]
+    c = sized(lens, G, D, V, [(which, 0, 4, big, 0.0)])
+    for steps in ((40, 45, 40, 3), (3, 5, 2, 1), (1, 1, 1, 1)):
+        slots = [n - s + i for n, s in zip(lens, steps) for i in range(s)]
+        req = [r for r, s in enumerate(steps) for _ in range(s)]
+        check(lib, c, rows(len(slots), H, D, F32 if f32 else BF16), slots, req, lens, D ** -0.5)
+
+
+@pytest.mark.parametrize("H,G,D,V,f32", FORMS)
+@pytest.mark.parametrize("big", [1e12, 1e30])
+def test_large_values_behind_the_query(lib, H, G, D, V, f32, big):
+    """tokens that come later in the same portion: rows before them do not know of them"""
+    lens = [200]
+    c = sized(lens, G, D, V, [(0, 3, 3, big, 0.0), (0, 9, 9, big ** 1.2, 0.0)])
+    check(lib, c, rows(200, H, D, F32 if f32 else BF16), list(range(200)), [0] * 200, lens, D ** -0.5)
+    for first, T in ((42, 12), (46, 4), (141, 6)):
+        check(lib, c, rows(T, H, D, F32 if f32 else BF16), list(range(first, first + T)), [0] * T, lens, D ** -0.5)
+
+
+@pytest.mark.parametrize("H,G,D,V,f32", FORMS)
+@pytest.mark.parametrize("big", [1e12, 1e30])
+def test_large_values_outside_the_window(lib, H, G, D, V, f32, big):
+    lens = [200]
+    c = sized(lens, G, D, V, [(0, 1, 1, big, 0.0), (0, 6, 6, big, 0.0)])
+    check(lib, c, rows(200, H, D, F32 if f32 else BF16), list(range(200)), [0] * 200, lens, D ** -0.5, window=20)
+    for first, T in ((42, 12), (49, 4), (128, 6), (131, 1)):
+        check(lib, c, rows(T, H, D, F32 if f32 else BF16), list(range(first, first + T)), [0] * T, lens, D ** -0.5, window=20)
+
+
+@pytest.mark.parametrize("H,G,D,V,f32", FORMS)
+@pytest.mark.parametrize("n,T", [(200, 200), (200, 12), (200, 1), (3000, 70), (3000, 1)])
+@pytest.mark.parametrize("where", ["first", "inside", "next"])
+def test_large_values_of_no_weight(lib, H, G, D, V, f32, n, T, where):
+    """keys that a row sees and gives next to no weight: 1e12 times e^-60"""
+    rec = {"first": 0, "inside": 5, "next": 8}[where]
+    c = sized([n], G, D, V, [(0, rec, rec, 1e12, -10.0)])
+    q = rows(T, H, D, F32 if f32 else BF16)
+    q[..., 0] = 6.0
+    check(lib, c, q, list(range(n - T, n)), [0] * T, [n], 1.0 if D == 32 else 0.9, mass=False)
+
+
+@pytest.mark.parametrize("H,G,D,V,f32", FORMS)
+@pytest.mark.parametrize("T", [1, 6, 150])
+def test_values_of_all_sizes(lib, H, G, D, V, f32, T):
+    """every record of a size of its own, growing, falling and by turns; several requests"""
+    lens = [190, 175, 160, 48]
+    f = [(0, b, b, 10.0 ** (b - 6), 0.0) for b in range(12)] + [(1, b, b, 10.0 ** (6 - b), 0.0) for b in range(11)] + [(2, b, b, 1e8 if b & 1 else 1e-8, 0.0) for b in range(10)]
+    f += [(3, 1, 1, 0.0, 0.0)]  # a record of zeros
+    c = sized(lens, G, D, V, f)
+    E = F32 if f32 else BF16
+    for window, sink in ((0, None), (37, rows(1, H, 1, E).view(H))):
+        each = [min(T, n) for n in lens]
+        slots = [n - s + i for n, s in zip(lens, each) for i in range(s)]
+        check(lib, c, rows(len(slots), H, D, E), slots, [r for r, s in enumerate(each) for _ in range(s)], lens, D ** -0.5, window=window, sink=sink)
+
+
+@pytest.mark.parametrize("H,G,D,V,f32", FORMS)
+def test_scores_that_rise_all_the_way(lib, H, G, D, V, f32):
+    """every block of keys is far above the one before: a reference of before is left behind again and again"""
+    n = 1500
+    c = K.Cache([n], G, D, V, 16)
+    g = torch.Generator().manual_seed(3)
+    k, v = torch.randn(n, G, D, generator=g).to(BF16).double(), torch.randn(n, G, V, generator=g).to(BF16).double()
+    k[..., 0] = (torch.arange(n) / 4.0).to(BF16).double()[:, None]
+    v[:16] *= 1e15
+    K.fill(c, 0, k, v)
+    c.data, c.page_off, c.pages = c.data.to(DEV), c.page_off.to(DEV), c.pages.to(DEV)
+    for T in (1, 10, 100):
+        q = rows(T, H, D, F32 if f32 else BF16)
+        for sign in (1.0, -1.0):
+            q[..., 0] = 3.0 * sign
+            check(lib, c, q, list(range(n - T, n)), [0] * T, [n], 0.25, mass=False)
