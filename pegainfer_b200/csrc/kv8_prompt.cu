@@ -532,8 +532,9 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* _
         for (int x = 0; x < 4; ++x) amax = fmaxf(amax, fmaxf(fabsf(bf16_lo(w[x])), fabsf(bf16_hi(w[x]))));
       }
       const int e = exponent_for(amax);
-      const float down = pow2(-e), qf = amax == INFINITY ? NAN : pow2(e);  // (an infinite entry: the row is NaN)
-      row_c = a.cap > 0.f ? qf : qf * a.scale * kLog2e;
+      // scale's sign goes into q: maxima are taken before the columns' factors, which have to be positive
+      const float down = a.scale < 0.f ? -pow2(-e) : pow2(-e), qf = amax == INFINITY ? NAN : pow2(e);  // (an infinite entry: the row is NaN)
+      row_c = a.cap > 0.f ? qf : qf * fabsf(a.scale) * kLog2e;
 #pragma unroll
       for (int c = 0; c < D / 16; ++c) {
         uint32_t hi[4], rest[4];
@@ -551,7 +552,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* _
     asm volatile("bar.sync 1, %0;" ::"n"(10 * 32) : "memory");
 
     const uint32_t t_tile = tmem_base + ((uint32_t)(q4 * 32) << 16) + (uint32_t)(i * 2 * kPrKeys);
-    const float cap2 = a.cap * kLog2e, cap_c = a.cap > 0.f ? 2.f * a.scale / a.cap * kLog2e : 0.f;
+    const float cap2 = a.cap * kLog2e, cap_c = a.cap > 0.f ? 2.f * fabsf(a.scale) / a.cap * kLog2e : 0.f;
     float m = -INFINITY, l = 0.f, E = kPrNone;  // l is held relative to 2^m, O to 2^(m + E); both are whole numbers, so that every rescaling is exact
     int mine = 0;
     for (Step x = begin(); x.seg < segs; next(x)) {

@@ -204,3 +204,13 @@ def test_scores_that_rise_all_the_way(lib, H, G, D, V, f32):
         for sign in (1.0, -1.0):
             q[..., 0] = 3.0 * sign
             check(lib, c, q, list(range(n - T, n)), [0] * T, [n], 0.25, mass=False)
+
+
+# ------------------------------------------------------------------ scales
+@pytest.mark.parametrize("H,G,D,V,f32", FORMS)
+@pytest.mark.parametrize("T", [1, 20, 150])
+@pytest.mark.parametrize("scale,softcap", [(-0.125, 0.0), (-0.2, 10.0), (0.0, 0.0), (0.0, 5.0)])
+def test_scales_of_any_sign(lib, H, G, D, V, f32, T, scale, softcap):
+    c = filled([160, 31], G, D, V, 16)
+    slots, req = list(range(160 - T, 160)) + [30], [0] * T + [1]
+    check(lib, c, rows(T + 1, H, D, F32 if f32 else BF16), slots, req, [160, 31], scale, softcap=softcap)
