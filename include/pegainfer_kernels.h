@@ -754,7 +754,7 @@ typedef struct pk_kv8_options {
 long pk_kv8_attention_workspace_bytes(int tokens, int heads, int kv_heads, int dim, int vdim, const pk_kv8_options* options, int f32);
 /* out[t,h] = sum_j w_j v_j, w = softmax over the visible slots j <= slots[t] of q[t,h] . k_j * scale (options applied; exp(sink[h]) added to the denominator when
  * sink != NULL).  A request's tokens are consecutive rows whose slots ascend by one at least, in one run per call; rows with a negative slot may lie anywhere, inside
- * it too.  Such a row sees nothing: zeros. */
+ * it too.  Such a row sees nothing: zeros.  A row of q with an entry that is not finite gives NaN in that head (with a soft cap too). */
 int pk_kv8_attention(const void* q, const void* cache, const void* sink, const int* slots, const int* req, const int* page_off, const int* pages, void* out,
                      long page_stride, int page_size, int tokens, int heads, int kv_heads, int dim, int vdim, float scale, const pk_kv8_options* options,
                      void* workspace, long workspace_bytes, int f32, pk_stream st);

@@ -25,9 +25,13 @@ __global__ void __launch_bounds__(kRowWarps * 32) kv8_row_kernel(const E* __rest
   pdl_launch_dependents();
   const int t = blockIdx.x, h = blockIdx.y, g = h / (a.H / a.pool.G), p = a.slots[t];
   const int lo = a.window > 0 ? max(0, p - a.window + 1) : 0;
-  const float c = a.scale * kLog2e;
-  for (int d = threadIdx.x; d < D; d += blockDim.x) sq[d] = to_f(q[((size_t)t * a.H + h) * D + d]);
-  __syncthreads();
+  bool odd = false;
+  for (int d = threadIdx.x; d < D; d += blockDim.x) {
+    const float v = to_f(q[((size_t)t * a.H + h) * D + d]);
+    odd |= (__float_as_uint(v) & 0x7f800000u) == 0x7f800000u;
+    sq[d] = v;
+  }
+  const float c = __syncthreads_or(odd) ? NAN : a.scale * kLog2e;  // (an entry that is not finite: the row is NaN, as in the other kernels)
   float m = -INFINITY, l = 0.f, acc[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) acc[i] = 0.f;

@@ -214,3 +214,17 @@ def test_scales_of_any_sign(lib, H, G, D, V, f32, T, scale, softcap):
     c = filled([160, 31], G, D, V, 16)
     slots, req = list(range(160 - T, 160)) + [30], [0] * T + [1]
     check(lib, c, rows(T + 1, H, D, F32 if f32 else BF16), slots, req, [160, 31], scale, softcap=softcap)
+
+
+# ------------------------------------------------------------------ queries that are not finite
+@pytest.mark.parametrize("H,G,D,V,f32", FORMS)
+@pytest.mark.parametrize("T", [1, 3, 150])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("softcap", [0.0, 20.0])
+def test_a_query_that_is_not_finite_whatever_the_cap(lib, H, G, D, V, f32, T, bad, softcap):
+    """its row is NaN in that head, in every kernel alike, and no other"""
+    n = 300
+    c = filled([n], G, D, V, 16)
+    q = rows(T, H, D, F32 if f32 else BF16)
+    q[T // 2, H - 1, D - 3] = bad
+    check(lib, c, q, list(range(n - T, n)), [0] * T, [n], D ** -0.5, softcap=softcap, mass=False, skip=[(T // 2, H - 1)])
