@@ -73,9 +73,10 @@ __global__ void __launch_bounds__(few_warps<D>() * 32, 1) kv8_few_kernel(const b
   const int R = a.H / a.pool.G, O = (R + 15) / 16, AB = f.abreast, U = f.U / AB, per = f.per;  // U: of the tiles that a warp sees
   volatile int* dead = &s_dead;
   if (tid == 0) s_dead = 0;
-  if (lane == 0)
+  if (lane == 0) {
     for (int s = 0; s < ST; ++s) mbar_init(&s_full[warp][s], 1);
-  if (tid == 0) mbar_fence_init();
+    mbar_fence_init();
+  }
   pdl_wait();
   pdl_launch_dependents();
 
