@@ -73,7 +73,7 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   return r;
 }
 // records of a warp's run (kv8_few.cu), an even number: `total` records over `warps` warps
-__host__ __device__ inline int few_run(int total, int warps) { return max(2, ((total + warps - 1) / warps + 1) / 2 * 2); }
+__host__ __device__ inline int few_run(long total, int warps) { return max(2, (int)(((total + warps - 1) / warps + 1) / 2 * 2)); }
 // kv8_few.cu: whether it takes a call, what it needs (bytes), the call itself (with the weights' sums)
 struct FewNeed {
   size_t o, ml, plan, scores;

@@ -165,7 +165,7 @@ __global__ void __launch_bounds__(few_warps<D>() * 32, 1) kv8_few_kernel(const b
     if (tid == 0) f.plan[2 * a.T + 1] = run;
   }
   const int who = (blockIdx.x * WARPS + warp) / AB, mine = warp % AB;
-  const int x0 = min(who * (long)run, (long)total), x1 = min(x0 + run, total);
+  const int x0 = (int)min(who * (long)run, (long)total), x1 = (int)min((long)x0 + run, (long)total);
 
   // ---- the run's records: stages of two, never of two tiles
   constexpr int TURN_LD = D + 4;
