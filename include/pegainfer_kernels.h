@@ -724,7 +724,7 @@ int pk_logistic_decay(float* z, const float* bias, float tau, int tokens, int ch
  *   record: K [2 groups of 8 slots][dim/16][8 slots][16 entries] | V [vdim][16 slots] | int8 exponent of K, int8 exponent of V, 14 zero bytes
  *   page:   [kv_heads][page_size/16] records, pk_kv8_page_bytes() bytes; page_stride (bytes, a multiple of 16) may be larger.  cache: 16-byte aligned.
  * The slot s of request r is in page pages[page_off[r] + s / page_size].  A slot is an index into the request's cache: the token's position, or less where
- * tokens were evicted.  page_size is a multiple of 16, dim and vdim multiples of 32 up to 256.  A token with an entry of k or v that is not finite makes the
+ * tokens were evicted.  page_size is a multiple of 16, dim and vdim multiples of 32 up to 256, heads and kv_heads up to 65535.  A token with an entry of k or v that is not finite makes the
  * rows that see it NaN (in the heads that read that kv head), and no others.  f32 selects the element type of activations, as above; the cache has one form.
  * -1: invalid argument.  Nothing is allocated, everything may be captured into a graph. */
 /* Bytes of a page; -1: sizes that the cache does not have */

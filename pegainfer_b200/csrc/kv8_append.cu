@@ -792,9 +792,9 @@ extern "C" long pk_kv8_page_bytes(int page_size, int kv_heads, int dim, int vdim
 extern "C" int pk_kv8_append(const void* qkv, int ld, const void* bias, const int* positions, const int* slots, const int* req, const int* page_off,
                              const int* pages, void* q_out, void* cache, long page_stride, int page_size, int heads, int kv_heads, int dim, int vdim,
                              int dims, int interleaved, const float* freq, float mag, int tokens, int f32, pk_stream st) {
-  if (!qkv || !positions || !req || !page_off || !pages || !cache || tokens <= 0 || heads < 0 || (heads > 0 && !q_out) || !kv8::sizes_ok(page_size, kv_heads, dim, vdim) ||
+  if (!qkv || !positions || !req || !page_off || !pages || !cache || tokens <= 0 || heads < 0 || heads > 65535 || kv_heads > 65535 || (heads > 0 && !q_out) || !kv8::sizes_ok(page_size, kv_heads, dim, vdim) ||
       !kv8::pool_ok(cache, page_stride, page_size, kv_heads, dim, vdim) || dims < 0 || dims > dim || (dims & 1) || (dims > 0 && !freq) ||
-      ld < heads * dim + kv_heads * (dim + vdim))
+      ld < (long)heads * dim + (long)kv_heads * (dim + vdim))
     return -1;
   const int es = f32 ? 4 : 2;
   const bool vec = ((reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(q_out)) & 15) == 0 && (long)ld * es % 16 == 0;
