@@ -762,7 +762,7 @@ int pk_kv8_attention(const void* q, const void* cache, const void* sink, const i
  * largest mass (equal: the lower slot; NaN least).  They move, in order, to the pages of new_pages / new_page_off (other pages of the same pool, room for
  * min(lens[r], budget) slots each), into records with exponents of their own; the old pages are left as they were.  kept [requests, kv_heads, budget]: the
  * old slot of each new one, -1 behind the last; new_mass [requests, kv_heads, new_mass_ld]: the masses of the kept, zero behind; new_lens[r]: slots kept.
- * new_lens, new_mass and new_pages are other arrays than the old ones.  keep_first + keep_recent <= budget; max_kv_len <= 2^30; mass_ld >= max_kv_len, new_mass_ld >= budget.  New tokens go on at slot new_lens[r] with their true positions. */
+ * new_lens, new_mass and new_pages are other arrays than the old ones.  keep_first + keep_recent <= budget; budget and max_kv_len <= 2^30; mass_ld >= max_kv_len, new_mass_ld >= budget.  New tokens go on at slot new_lens[r] with their true positions. */
 int pk_kv8_evict(void* cache, long page_stride, int page_size, const int* page_off, const int* pages, const int* lens, const float* mass, long mass_ld,
                  const int* new_page_off, const int* new_pages, int* new_lens, float* new_mass, long new_mass_ld, int* kept, int requests, int kv_heads,
                  int dim, int vdim, int budget, int keep_first, int keep_recent, int max_kv_len, pk_stream st);

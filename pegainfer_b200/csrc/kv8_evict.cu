@@ -325,7 +325,7 @@ extern "C" int pk_kv8_evict(void* cache, long page_stride, int page_size, const 
                             const int* new_page_off, const int* new_pages, int* new_lens, float* new_mass, long new_mass_ld, int* kept, int requests, int kv_heads,
                             int dim, int vdim, int budget, int keep_first, int keep_recent, int max_kv_len, pk_stream st) {
   if (!cache || !page_off || !pages || !lens || !mass || !new_page_off || !new_pages || !new_lens || !new_mass || !kept || requests <= 0 || requests > 65535 ||
-      budget <= 0 || keep_first < 0 || keep_recent < 0 || (long)keep_first + keep_recent > budget || max_kv_len <= 0 || max_kv_len > kv8::kMaxSlots || mass_ld < max_kv_len ||
+      budget <= 0 || budget > kv8::kMaxSlots || keep_first < 0 || keep_recent < 0 || (long)keep_first + keep_recent > budget || max_kv_len <= 0 || max_kv_len > kv8::kMaxSlots || mass_ld < max_kv_len ||
       new_mass_ld < budget || new_mass == mass || new_pages == pages || new_lens == lens || !kv8::sizes_ok(page_size, kv_heads, dim, vdim) || kv_heads > 65535 ||
       !kv8::pool_ok(cache, page_stride, page_size, kv_heads, dim, vdim))
     return -1;
