@@ -534,16 +534,11 @@ __global__ void __launch_bounds__(kPlainWarps * 32) kv8_mass_plain_kernel(const 
 }
 
 static int mass_mma(const bf16* q, const AttnArgs& a, int runs, cudaStream_t st) {
-  const long R = a.H / a.pool.G;
-  if (a.T * R * R < 1L << 32) {  // (rows are divided by R through a product)
-    if (a.pool.dim == 64) return launch_mass_wide<64>(q, a, runs, st);
-    if (a.pool.dim == 128) return launch_mass_wide<128>(q, a, runs, st);
-  }
   switch (a.pool.dim) {
     case 32: return launch_mass<32>(q, a, runs, st);
-    case 64: return launch_mass<64>(q, a, runs, st);
+    case 64: return launch_mass_wide<64>(q, a, runs, st);
     case 96: return launch_mass<96>(q, a, runs, st);
-    case 128: return launch_mass<128>(q, a, runs, st);
+    case 128: return launch_mass_wide<128>(q, a, runs, st);
     case 192: return launch_mass<192>(q, a, runs, st);
     default: return launch_mass<256>(q, a, runs, st);
   }
@@ -551,9 +546,12 @@ static int mass_mma(const bf16* q, const AttnArgs& a, int runs, cudaStream_t st)
 template <typename E>
 int mass_rows(const E* q, const AttnArgs& a, int max_q_len, cudaStream_t st) {
   const int T = a.T, D = a.pool.dim;
-  for (int t0 = 0; t0 < T; t0 += kMassTokens) {  // (a run that a launch's end cuts is added up in both)
+  // a launch's rows are counted in an int and divided by R through a product, which is exact below 2^32 / R rows
+  const long R = a.H / a.pool.G;
+  const int most = (int)std::min((long)kMassTokens, ((1L << 32) - 1) / (R * R));
+  for (int t0 = 0; t0 < T; t0 += most) {  // (a run that a launch's end cuts is added up in both)
     AttnArgs x = a;
-    x.T = std::min(kMassTokens, T - t0);
+    x.T = std::min(most, T - t0);
     x.slots += t0;
     x.req += t0;
     x.lse += (size_t)t0 * a.H;

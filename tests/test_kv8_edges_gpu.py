@@ -78,6 +78,13 @@ def test_groups_of_many_heads(lib, R):
     check(lib, c, rows(5, R, 32, BF16), [38, 39, 40, 6, 299], [0, 0, 0, 1, 2], [41, 7, 300], 0.2, sink=rows(1, R, 1, BF16).view(R), max_q=0)
 
 
+@pytest.mark.parametrize("D", [64, 96])
+def test_weights_of_more_rows_than_a_launch_counts(lib, D):
+    """255 tokens of 4096 heads are a launch's; the request lies on both sides"""
+    c = filled([300], 1, D, D, 16)
+    check(lib, c, rows(300, 4096, D, BF16, size=0.5), list(range(300)), [0] * 300, [300], 0.1)
+
+
 # ------------------------------------------------------------------ padding
 def holes(n, pattern):
     """slots 0 .. n - 1 with rows of no slot in between: (valid, padding) by turns"""
