@@ -115,6 +115,25 @@ def test_padding_between_three_tokens(lib, f32):
     check(lib, c, rows(3, 4, 64, F32 if f32 else BF16), [32, -1, 33], [0, 0, 0], [34], 0.125)
 
 
+@pytest.mark.parametrize("H,G,D,V,f32", [(8, 2, 64, 64, False), (4, 1, 128, 128, False), (8, 2, 96, 96, False), (4, 2, 64, 32, False), (4, 2, 64, 64, True), (3, 1, 96, 160, True)])
+@pytest.mark.parametrize("T", [4, 100])
+@pytest.mark.parametrize("softcap", [0.0, 15.0])
+def test_padding_of_any_contents(lib, H, G, D, V, f32, T, softcap):
+    """rows without a slot hold NaN and name requests that there are not: zeros, the sink's lse, no weight"""
+    E = F32 if f32 else BF16
+    c = filled([130, 60], G, D, V, 16)
+    slots = [-1] + list(range(130 - T, 130)) + [-1, 59, -1, -1]
+    req = [77] + [0] * T + [0, 1, 1, 99999]
+    q = rows(len(slots), H, D, E)
+    for t, s in enumerate(slots):
+        if s < 0:
+            q[t] = math.nan
+    sink = rows(1, H, 1, E).view(H)
+    out, lse = check(lib, c, q, slots, req, [130, 60], 0.2, sink=sink, softcap=softcap)
+    pad = torch.tensor([s < 0 for s in slots], device=DEV)
+    assert (out[pad] == 0).all() and torch.allclose(lse[pad], sink.float().expand(int(pad.sum()), H), atol=1e-6)
+
+
 # ------------------------------------------------------------------ records of different sizes
 def sized(lens, G, D, V, factors, seed=0, page=16, push=0.0):
     """factors: (request, first record, last record, factor of the values, push of the keys' first entry)"""
