@@ -18,11 +18,6 @@ namespace kv8 {
 
 constexpr int kMassWarps = 4, kMassRows = 64, kMassTokens = 65536;  // of a launch, at most
 
-__device__ __forceinline__ float ms_ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 // two codes -> two bf16
 __device__ __forceinline__ uint32_t bf16_of(uint32_t two) {
   const float2 v = values2(two);
@@ -201,10 +196,10 @@ __global__ void __launch_bounds__(kMassWarps * 32) kv8_mass_kernel(const bf16* _
               for (int y = 0; y < 2; ++y) {
                 float w;
                 if (a.cap > 0.f) {
-                  const float v = fmaf(-2.f * cap2, __fdividef(1.f, ms_ex2(at_most80(acc[x][r][2 * y + e] * fk[r] * cap_c)) + 1.f), cap2);
-                  w = ms_ex2(v - (e ? lse.y : lse.x));
+                  const float v = fmaf(-2.f * cap2, __fdividef(1.f, ex2(at_most80(acc[x][r][2 * y + e] * fk[r] * cap_c)) + 1.f), cap2);
+                  w = ex2(v - (e ? lse.y : lse.x));
                 } else {
-                  w = ms_ex2(fmaf(acc[x][r][2 * y + e], fk[r], e ? -lse.y : -lse.x));
+                  w = ex2(fmaf(acc[x][r][2 * y + e], fk[r], e ? -lse.y : -lse.x));
                 }
                 if (!whole) {
                   const int j = (b0 + r) * kBlock + 8 * y + gq, pe = e ? p.y : p.x;
@@ -243,8 +238,8 @@ __device__ __forceinline__ void add_weights(float& s0, float& s1, uint32_t x0, u
   asm("fma.rn.f32x2 %0, %0, %1, %2;" : "+l"(x) : "l"(y), "l"(z));
   float w0, w1;
   asm("mov.b64 {%0, %1}, %2;" : "=f"(w0), "=f"(w1) : "l"(x));
-  w0 = ms_ex2(w0);
-  w1 = ms_ex2(w1);
+  w0 = ex2(w0);
+  w1 = ex2(w1);
   asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(w0), "f"(w1));
   asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "f"(s0), "f"(s1));
   asm("add.rn.f32x2 %0, %0, %1;" : "+l"(y) : "l"(x));
@@ -380,7 +375,7 @@ __global__ void __launch_bounds__(kWideWarps * 32, 2) kv8_mass_wide_kernel(const
       if (a.cap > 0.f) {
 #pragma unroll
         for (int j = 0; j < 64; ++j)
-          v[j] = __float_as_uint(fmaf(-2.f * cap2, __fdividef(1.f, ms_ex2(at_most80(__uint_as_float(v[j]) * fk)) + 1.f), cap2));
+          v[j] = __float_as_uint(fmaf(-2.f * cap2, __fdividef(1.f, ex2(at_most80(__uint_as_float(v[j]) * fk)) + 1.f), cap2));
       }
       const float f = a.cap > 0.f ? 1.f : fk;
       if (whole) {
@@ -394,7 +389,7 @@ __global__ void __launch_bounds__(kWideWarps * 32, 2) kv8_mass_wide_kernel(const
 #pragma unroll
         for (int j = 0; j < 64; ++j) {
           const int p = s_p[s][col0 + j];
-          const float w = ms_ex2(fmaf(__uint_as_float(v[j]), f, s_neg[s][col0 + j]));
+          const float w = ex2(fmaf(__uint_as_float(v[j]), f, s_neg[s][col0 + j]));
           (j & 1 ? sum1 : sum0) += key <= p && (a.window <= 0 || key > p - a.window) ? w : 0.f;
         }
       }

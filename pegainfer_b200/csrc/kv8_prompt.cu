@@ -46,11 +46,6 @@ struct PromptArgs {
   unsigned int* err;
 };
 
-__device__ __forceinline__ float pr_ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 // whole numbers of a few bits: as a float, and two to them (-126 .. 127), in the ordinary pipes
 __device__ __forceinline__ float small_float(int x) { return __int_as_float(0x4b400000 + x) - 12582912.f; }
 __device__ __forceinline__ float whole_pow2(float x) { return __int_as_float(__float_as_int(x + (12582912.f + 127.f)) << 23); }
@@ -87,15 +82,6 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, ui
 __device__ __forceinline__ void pr_copy(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
 }
-__device__ __forceinline__ uint32_t pr_pack(float lo, float hi) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-// four codes -> two pairs of f16
-__device__ __forceinline__ void pr_widen(uint32_t four, uint32_t& lo, uint32_t& hi) {
-  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=&r"(lo), "=&r"(hi) : "r"(four));
-}
 // {a0, a1} += {x0, x1}
 __device__ __forceinline__ void pr_add2(float& a0, float& a1, float x0, float x1) {
   unsigned long long v, w;
@@ -106,7 +92,7 @@ __device__ __forceinline__ void pr_add2(float& a0, float& a1, float x0, float x1
 }
 // four bf16 times a power of two (448 at most) -> the nearest e4m3 and the rests as e5m2.  f16 holds them exactly but below 2^-14, and there to 2^-25.
 __device__ __forceinline__ void q_parts(uint32_t w0, uint32_t w1, float down, uint32_t& near, uint32_t& rest) {
-  const uint32_t h0 = pr_pack(bf16_lo(w0) * down, bf16_hi(w0) * down), h1 = pr_pack(bf16_lo(w1) * down, bf16_hi(w1) * down);
+  const uint32_t h0 = pack_f16(bf16_lo(w0) * down, bf16_hi(w0) * down), h1 = pack_f16(bf16_lo(w1) * down, bf16_hi(w1) * down);
   uint16_t c[2], d[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i)
@@ -418,10 +404,10 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* _
         const int b = u / D, d = u - b * D;
         const uint4 x = *reinterpret_cast<const uint4*>(from + u * 16);
         uint32_t h[8];
-        pr_widen(x.x, h[0], h[1]);
-        pr_widen(x.y, h[2], h[3]);
-        pr_widen(x.z, h[4], h[5]);
-        pr_widen(x.w, h[6], h[7]);
+        widen(x.x, h[0], h[1]);
+        widen(x.y, h[2], h[3]);
+        widen(x.z, h[4], h[5]);
+        widen(x.w, h[6], h[7]);
         *reinterpret_cast<uint4*>(to + (2 * b) * REC_K + d * 16) = make_uint4(h[0], h[1], h[2], h[3]);
         *reinterpret_cast<uint4*>(to + (2 * b + 1) * REC_K + d * 16) = make_uint4(h[4], h[5], h[6], h[7]);
       }
@@ -581,7 +567,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* _
       if (a.cap > 0.f) {  // (the columns' factors are in the scores then)
 #pragma unroll
         for (int k = 0; k < kPrKeys; ++k)
-          v[k] = __float_as_uint(fmaf(-2.f * cap2, __fdividef(1.f, pr_ex2(at_most80(__uint_as_float(v[k]) * fk[k / kBlock] * cap_c)) + 1.f), cap2));
+          v[k] = __float_as_uint(fmaf(-2.f * cap2, __fdividef(1.f, ex2(at_most80(__uint_as_float(v[k]) * fk[k / kBlock] * cap_c)) + 1.f), cap2));
       }
       if (masked) {
 #pragma unroll
@@ -623,10 +609,10 @@ __global__ void __launch_bounds__(kPrThreads, 1) kv8_prompt_kernel(const bf16* _
         for (int k = 0; k < 8; ++k) {
           float s0 = __uint_as_float(v[b * 16 + 2 * k]), s1 = __uint_as_float(v[b * 16 + 2 * k + 1]);
           pr_fma2(s0, s1, fb, add);
-          s0 = pr_ex2(s0);
-          s1 = pr_ex2(s1);
+          s0 = ex2(s0);
+          s1 = ex2(s1);
           pr_add2(d0, d1, s0, s1);
-          w[b * 8 + k] = pr_pack(s0, s1);
+          w[b * 8 + k] = pack_f16(s0, s1);
         }
         l = fmaf(d0 + d1, whole_pow2(-shift), l);
       }
