@@ -730,10 +730,11 @@ int pk_logistic_decay(float* z, const float* bias, float tau, int tokens, int ch
 /* Bytes of a page; -1: sizes that the cache does not have */
 long pk_kv8_page_bytes(int page_size, int kv_heads, int dim, int vdim);
 /* qkv [tokens, ld] = [q (heads*dim) | k (kv_heads*dim) | v (kv_heads*vdim)] (+ bias of the same layout, may be NULL): q and k rotate over their first `dims`
- * entries by positions[t] * freq[i] as in pk_gqa_rope_append (angles are reduced in 64 bits; those of bf16 q have sine and cosine to 2^-20); q goes to q_out [tokens, heads*dim], k and v into the cache at
- * slots[t] (slots NULL: at positions[t]).  heads may be 0 (rows of k and v alone, q_out NULL).  A request's tokens are consecutive rows with consecutive slots,
- * in one run per call, in front of and behind which there may be rows without a slot, but none inside.  A token at a record's first slot begins the record anew (slots behind the call's last are zero); else the record goes on from the slots
- * before, whose codes are rounded again where its exponent grows.  Rows with a negative slot are not cached (their q is rotated all the same). */
+ * entries by positions[t] * freq[i] as in pk_gqa_rope_append (angles are reduced in 64 bits; those of bf16 q have sine and cosine to 2^-20); q goes to q_out
+ * [tokens, heads*dim], k and v into the cache at slots[t] (slots NULL: at positions[t]).  heads may be 0 (rows of k and v alone, q_out NULL).  A request's tokens are consecutive rows with consecutive slots,
+ * in one run per call, in front of and behind which there may be rows without a slot, but none inside.  A token at a record's first slot begins the record anew (slots
+ * behind the call's last are zero); else the record goes on from the slots before, whose codes are rounded again where its exponent grows.  Rows with a negative slot are
+ * not cached (their q is rotated all the same).  q_out is another array than qkv.  The rotation is fp32, so a value next to the border of two codes may get either. */
 int pk_kv8_append(const void* qkv, int ld, const void* bias, const int* positions, const int* slots, const int* req, const int* page_off, const int* pages,
                   void* q_out, void* cache, long page_stride, int page_size, int heads, int kv_heads, int dim, int vdim, int dims, int interleaved,
                   const float* freq, float mag, int tokens, int f32, pk_stream st);
@@ -742,8 +743,9 @@ typedef struct pk_kv8_options {
   int window;      /* the query at slot p sees slots p - window + 1 .. p */
   float softcap;   /* scaled score <- softcap * tanh(score / softcap) */
   int max_kv_len;  /* no query's slot is max_kv_len or more; 2^30 at most */
-  int max_q_len;   /* no request has more tokens in the call (1: decoded tokens): a hint for the choice of a kernel; with 0 (unknown) calls of up to 512
-                      tokens are taken for decoded ones, larger ones for prompts */
+  int max_q_len;   /* no request has more tokens in the call (1: decoded tokens): a hint for the choice of a kernel, one for the whole call; with 0 (unknown) calls of
+                      up to 512 tokens are taken for decoded ones, larger ones for prompts.  Decoded tokens and portions of more than 32 tokens are faster in calls of
+                      their own: the kernels for portions read the context of every request for itself */
   long out_ld;     /* elements from one row of out to the next (0: heads * vdim) */
   float* lse;      /* [tokens, heads]: log(sum over the visible slots of exp(score), plus exp(sink)); -inf where there is neither */
   float* mass;     /* [requests, kv_heads, mass_ld]: mass[req[t]][g][j] += the weights of slot j in the rows of the call, over the heads of group g */
@@ -754,7 +756,9 @@ typedef struct pk_kv8_options {
 long pk_kv8_attention_workspace_bytes(int tokens, int heads, int kv_heads, int dim, int vdim, const pk_kv8_options* options, int f32);
 /* out[t,h] = sum_j w_j v_j, w = softmax over the visible slots j <= slots[t] of q[t,h] . k_j * scale (options applied; exp(sink[h]) added to the denominator when
  * sink != NULL).  A request's tokens are consecutive rows whose slots ascend by one at least, in one run per call; rows with a negative slot may lie anywhere, inside
- * it too.  Such a row sees nothing: zeros.  A row of q with an entry that is not finite gives NaN in that head (with a soft cap too). */
+ * it too.  Such a row sees nothing: zeros.  A row of q with an entry that is not finite gives NaN in that head (with a soft cap too).  out is another array than q.
+ * Sums, maxima and lse are fp32; into the products weights go with 11 bits (f32: 22), q with its 8 down to 2^-17 of the row's largest entry (f32: 22, or 24 with few
+ * rows).  With mass q should lie on a 16-byte boundary: elsewhere prompts' weights are summed without tensor cores. */
 int pk_kv8_attention(const void* q, const void* cache, const void* sink, const int* slots, const int* req, const int* page_off, const int* pages, void* out,
                      long page_stride, int page_size, int tokens, int heads, int kv_heads, int dim, int vdim, float scale, const pk_kv8_options* options,
                      void* workspace, long workspace_bytes, int f32, pk_stream st);
@@ -762,7 +766,8 @@ int pk_kv8_attention(const void* q, const void* cache, const void* sink, const i
  * largest mass (equal: the lower slot; NaN least).  They move, in order, to the pages of new_pages / new_page_off (other pages of the same pool, room for
  * min(lens[r], budget) slots each), into records with exponents of their own; the old pages are left as they were.  kept [requests, kv_heads, budget]: the
  * old slot of each new one, -1 behind the last; new_mass [requests, kv_heads, new_mass_ld]: the masses of the kept, zero behind; new_lens[r]: slots kept.
- * new_lens, new_mass and new_pages are other arrays than the old ones.  keep_first + keep_recent <= budget; budget and max_kv_len <= 2^30; mass_ld >= max_kv_len, new_mass_ld >= budget.  New tokens go on at slot new_lens[r] with their true positions. */
+ * new_lens, new_mass and new_pages are other arrays than the old ones.  keep_first + keep_recent <= budget; budget and max_kv_len <= 2^30; mass_ld >= max_kv_len,
+ * new_mass_ld >= budget.  New tokens go on at slot new_lens[r] with their true positions. */
 int pk_kv8_evict(void* cache, long page_stride, int page_size, const int* page_off, const int* pages, const int* lens, const float* mass, long mass_ld,
                  const int* new_page_off, const int* new_pages, int* new_lens, float* new_mass, long new_mass_ld, int* kept, int requests, int kv_heads,
                  int dim, int vdim, int budget, int keep_first, int keep_recent, int max_kv_len, pk_stream st);

@@ -8,7 +8,8 @@
 //   kv8_move_kernel   a warp to a new record.  Bound by the bytes it has to look at: a token's V lies in every 16-byte row of its record, so nearly the whole old cache is
 //                     read where a quarter of it is kept.  A source record's V is loaded once for all its kept tokens (rows of 16 tokens a lane), codes whose exponent
 //                     stays are moved as they are.
-// B200, 16 requests of 16384, 8 kv heads of 128 in both, to 4096: 24 us and 109 (142 together, 175 by histograms; of 32768 271 and 312); the sources' V rows and the kept K rows are 0.5 GB, 4.6 TB/s.
+// B200, 16 requests of 16384, 8 kv heads of 128 in both, to 4096: choice 24 us, move 109; the call 135, and 144 after other data went through L2, where histograms take 175 (of 32768
+// slots 273 and 312).  The sources' V rows and the kept K rows are 0.5 GB: 4.8 TB/s in the move.
 #include <algorithm>
 
 #include "kv8.cuh"

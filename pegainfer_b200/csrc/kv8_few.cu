@@ -26,7 +26,10 @@
 namespace pk {
 namespace kv8 {
 
-constexpr size_t kMostScores = (size_t)1 << 30;  // bytes that are kept for the weights' sums; with more the scores are computed again (kv8_mass.cu)
+// Bytes of scores that are kept for the weights' sums; with more they are computed again (kv8_mass.cu).  B200, 32 heads of 128 in 8 groups, us kept : again: decoded tokens of one
+// request behind 2000 17 : 23, behind 131072 81 : 463, of 16 behind 8190 78 : 445, of 64 247 : 1422 (64 MB); portions, whose keys several rows share, 4 of 16 tokens behind 4000
+// 105 : 87, one of 32 behind 16000 171 : 108.  So the limit is there for the workspace alone, which grows with max_kv_len.
+constexpr size_t kMostScores = (size_t)1 << 30;
 constexpr float kNoneYet = -1000.f;  // E of a row that has seen nothing
 constexpr int kNear = 8;             // V's exponents within so much: one E for all rows
 constexpr int kFewTokens = 512;  // of a launch: their tiles are looked up in shared memory
@@ -707,7 +710,7 @@ static int launch_few(const bf16* q, const bf16* sink, bf16* out, const FewArgs&
 // 32 54 : 52, 64 81 : 63, 256 234 : 89; 16 portions of 16 behind 2000 83 : 176, 8 of 32 83 : 95, 4 of 64 83 : 60; decoded tokens of 64 requests 69 : 2637 (there a tile's
 // tokens belong to 64 requests, one after the other).  So up to 32 tokens of a request come here; with no word about them calls of up to 512 tokens, where a wrong guess
 // costs a factor of 3 here and 40 there.  Against tiles (kv8_tile.cu), where the kernel for prompts does not take the heads' size: 64 behind 2000, 16 heads of 32 in 4
-// groups, 29 : 53, 16 of 256 in one 70 : 113, 32 of 192 in 8 82 : 102; 256 70 : 59, 135 : 129, 277 : 186; six prompts of 608 596 : 98, 2270 : 311, 2360 : 571.
+// groups, 29 : 53, 16 of 256 in one 70 : 113, 32 of 192 in 8 82 : 102; 256 73 : 65, 142 : 132, 286 : 198; six prompts of 608 618 : 104, 2347 : 324, 2461 : 596.
 bool few_takes(int T, int H, int G, int dim, int vdim, int max_kv_len, int max_q_len) {
   if (T > 65535 || dim != vdim || !(dim == 32 || dim == 64 || dim == 96 || dim == 128 || dim == 192 || dim == 256)) return false;
   if ((long)std::min(T, kFewTokens) * G * ((H / G + 15) / 16) * (max_kv_len / kBlock + 2) >= 1L << 31) return false;

@@ -5,7 +5,8 @@
 // through shared memory, as they are (mma.sync m16n8k16 in bf16, S^T = K q^T, fp32 sums).  A thread has the scores of two rows of four keys: the exponential and the sum
 // over rows need no exchange.  The grid's z axis takes the runs by turns.
 //
-// Dims 64 and 128 go through tcgen05 instead (kv8_mass_wide_kernel).  B200, two portions of 333 tokens behind 5003, 16 heads of 128 in 4 groups (54 Mi scores): 59 us, with
+// Dims 64 and 128 go through tcgen05 instead (kv8_mass_wide_kernel); rows of q off 16-byte boundaries, fp32 and other dims through plain sums (kv8_mass_plain_kernel: the call below
+// takes 1934 us instead of 141 with q on 2 bytes).  B200, two portions of 333 tokens behind 5003, 16 heads of 128 in 4 groups (54 Mi scores): 59 us, with
 // mma.sync 89.
 #include <algorithm>
 

@@ -14,8 +14,8 @@
 //     tile waited 1600 of 5200 clocks for it.)
 //   * m is a maximum of before that the row's own may have passed by up to 2^8: O, which stays in tensor memory, is rescaled only where one did by more.  P, held 2^7 times
 //     too large, stays within f16's range then, with 11 bits down to 2^-21 of the largest weight.
-// B200, prompt of 4096 tokens, 32 heads of 128 in 8 groups: 193 us, 0.71 PFLOP/s.  Bound by a softmax thread's latency: 1200 of 2500 clocks of a block of 64 keys are its
-// exponentials and P, 500 waits; a CTA's start takes 12000.  Tried and slower: operands in the 128-byte swizzle (206), a degree-4 polynomial for a quarter of the
+// B200, prompt of 4096 tokens, 32 heads of 128 in 8 groups: 193 us, 0.71 PFLOP/s.  Bound by a softmax thread's latency: 1200 of 2500 clocks of a block of 64 keys (1.35 us) are its
+// exponentials and P, 500 waits; a CTA takes 6.3 us to its first scores and 3.1 behind its last block.  Tried and slower: operands in the 128-byte swizzle (206), a degree-4 polynomial for a quarter of the
 // exponentials (210), blocks of 128 keys (231).
 // Warps: 0-3 softmax tile 0, a thread per row | 4-7 softmax tile 1 | 8-11 V, rescaling, results | 12, 13 MMA issuers | 14 copies | 15 nothing.  Of the block's registers a
 // softmax thread has 192, the others 80 and 48.
@@ -670,14 +670,15 @@ bool prompt_takes(int T, int H, int G, int dim, int vdim) {
   return dim == vdim && (dim == 64 || dim == 96 || dim == 128) && tokens > 0 && (T + tokens - 1) / tokens <= 65535;
 }
 // Shares of the keys where the tiles leave SMs idle: as many CTAs as SMs, and 16 blocks of keys to a share at least (of the longest context, which is all that is known).
-// A share's start and end take 6 us, a block 1.5; the merge 13 for 10656 rows.  (666 tokens of two portions behind 5003, 16 heads: 80 + 14 us in shares of 28 blocks, 248 whole.)
+// (666 tokens of two portions behind 5003, 16 heads: 79 us in shares of 29 blocks and 14 for the merge of 10656 rows, 248 whole.  A share takes 7 us to its first scores, 1.4 a block
+// and 6 to its end, 54 in all; the last of the 144 begin at 23 us, behind CTAs without a share, which hold an SM for 4 us each.)
 static int prompt_span(int H, int G, int max_kv_len, int window) { return window > 0 ? std::min(max_kv_len, window + 2 * (kPrRows / (H / G))) : max_kv_len; }
 static int prompt_pieces(int T, int H, int G, int max_kv_len, int window) {
   const int per = kPrRows / (H / G), ctas = (T + 2 * per - 1) / (2 * per) * G;
   return std::max(1, std::min(sm_count() / std::max(ctas, 1), prompt_span(H, G, max_kv_len, window) / (16 * kPrKeys)));
 }
 // Twice as many CTAs to a tile as one context makes shares: a tile whose tokens belong to two requests has two contexts to read, and its shares are as long as the others'
-// (their other CTAs leave at once).  (The same portions: 80 us, 104 with three CTAs to a
+// (their other CTAs leave early).  (The same portions: 80 us, 104 with three CTAs to a
 // tile.)  A tile's CTAs follow one another in the grid: those that leave make room for the next tile's (94 us with a tile's shares a grid of tiles apart).
 int prompt_shares(int T, int H, int G, int max_kv_len, int window) {
   const int pieces = prompt_pieces(T, H, G, max_kv_len, window);

@@ -320,8 +320,8 @@ int tile_attention(const E* q, const E* sink, E* out, const AttnArgs& a, int sha
 template int tile_attention<float>(const float*, const float*, float*, const AttnArgs&, int, cudaStream_t);
 template int tile_attention<bf16>(const bf16*, const bf16*, bf16*, const AttnArgs&, int, cudaStream_t);
 
-// Against the kernel with a CTA to a row (B200, us here : there).  fp32, 32 heads of 128 in 8 groups: portions behind 2000 of 16 tokens 98 : 75, 64 89 : 221, 256 157 : 758;
-// 16 portions behind 500 of 4 tokens 219 : 72, 8 123 : 121, 16 78 : 228; decoded tokens of 64 requests 805 : 79; a prompt of 1024 166 : 817.  fp32, 8 heads of 64 in 8
+// Against the kernel with a CTA to a row (B200, us here : there).  fp32, 32 heads of 128 in 8 groups: portions behind 2000 of 16 tokens 98 : 75, 64 91 : 229, 256 159 : 760;
+// 16 portions behind 500 of 4 tokens 217 : 73, 8 123 : 121, 16 80 : 229; decoded tokens of 64 requests 790 : 80; a prompt of 1024 168 : 821.  fp32, 8 heads of 64 in 8
 // groups (a tile has 64 tokens): 64 behind 2000 71 : 52, 256 73 : 154, 16 portions of 16 behind 500 170 : 55.  So it takes a thousand rows with few requests in a tile;
 // with no word about those, calls of more than 512 tokens.
 bool tile_takes(int T, int H, int G, int max_q_len) {
