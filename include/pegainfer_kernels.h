@@ -772,6 +772,32 @@ int pk_kv8_evict(void* cache, long page_stride, int page_size, const int* page_o
                  const int* new_page_off, const int* new_pages, int* new_lens, float* new_mass, long new_mass_ld, int* kept, int requests, int kv_heads,
                  int dim, int vdim, int budget, int keep_first, int keep_recent, int max_kv_len, pk_stream st);
 
+/* =============== linear layers of 8 bits: rows, weights, products ===============
+ * A value is an e4m3 code times its block's float scale.  Rows of activations: codes [tokens][ld] (bytes), a scale for 128 consecutive entries of a row, block by block at
+ * scales[b * ld_s + t].  Weights: codes [rows][ld], a scale for 128 rows x 128 entries at scales[(r / 128) * ceil(width / 128) + b].  The last blocks may be smaller.
+ * ld is a multiple of 16 and at least the width, codes lie on a 16-byte boundary; ld_s is a multiple of 4 and at least the number of tokens, a row's scales lie on a 16-byte boundary
+ * and have room for ld_s floats a block.  Bytes of a row behind its width and scales behind the last token are neither written nor used.
+ * Quantising: scale = max(largest magnitude of the block, 2^-100) / 448, code = the e4m3 number nearest to value / scale (ties to even; a value next to the border of two codes may get
+ * either).  A block with an entry that is not finite has the scale NaN and codes NaN.  All arithmetic is fp32; a value is rounded once, to its code.
+ * Nothing is allocated and there are no workspaces, so calls may run at the same time and be captured.  -1: invalid argument, -2: sizes outside the kernels' range. */
+/* x[t] += y[t] (y bf16, NULL: nothing is added and x not written; x bf16, rounded when stored, or float);  codes of x[t] / sqrt(mean(x[t]^2) + eps) * (offset + w), of the
+ * unrounded sum.  x, y [tokens, width], w [width] bf16, offset 0 or 1 as the weights are kept.  y is another array than x.  width up to 16384. */
+int pk_fp8_add_norm(const void* y, void* x, int x_f32, const void* w, float offset, void* codes, long ld, float* scales, long ld_s, int width, int tokens, float eps,
+                    pk_stream st);
+/* codes of the activated rows.  in bf16, rows of ld_in elements (0: as many as are read).  kind as for pk_act_ex: 0 silu(in[t][f]) * in[t][F + f], 1 relu(in[t][f])^2,
+ * 2 relu(in[t][f]) * in[t][F + f], 3 gelu_tanh(in[t][f]) * in[t][F + f];  4: in[t][f] as it is. */
+int pk_fp8_act(const void* in, long ld_in, int kind, void* codes, long ld, float* scales, long ld_s, int F, int tokens, pk_stream st);
+/* codes of weights w [rows, width], bf16 or float, rows of ld_w elements (0: width) */
+int pk_fp8_weights(const void* w, int w_f32, long ld_w, void* codes, long ld, float* scales, int rows, int width, pk_stream st);
+/* y[t][m] = sum over k of x[t][k] * w[m][k], M features, N tokens, y bf16 or float in rows of ld_y elements (0: M).  Scales may be any numbers (a checkpoint's own), but the product of a
+ * row's and a weight's has to be finite, and is as exact as a normal float where it is at least 2^-126.  A token's result does not depend on the other tokens' values. */
+int pk_fp8_gemm(const void* w, long ld_w, const float* w_scales, const void* x, long ld_x, const float* x_scales, long ld_xs, void* y, long ld_y, int y_f32, int M, int N, int K,
+                pk_stream st);
+/* codes of act(x w_gate^T) * (x w_up^T), F features: pk_fp8_gemm of both, pk_fp8_act and nothing rounded between.  act 0 SiLU, 1 ReLU, 2 GELU in its tanh form.  w_gate and w_up
+ * [F, K] have one ld_w; halves of one array are fine.  codes is another array than x. */
+int pk_fp8_gemm_gated(const void* w_gate, const float* gate_scales, const void* w_up, const float* up_scales, long ld_w, const void* x, long ld_x, const float* x_scales, long ld_xs,
+                      void* codes, long ld, float* scales, long ld_s, int F, int N, int K, int act, pk_stream st);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,133 @@
+// Linear layers in 8 bits: what their kernels share.
+//
+// A value is its e4m3 code times its block's scale.  Rows of activations have a scale for 128 consecutive entries, weights one for 128 rows x 128 entries:
+//   s = max(largest magnitude of the block, 2^-100) / 448,  code = the e4m3 number nearest to v / s (ties to even)
+// so a block's largest entry has the code 448 and an entry is off by at most 2^-4 of itself, or by 2^-10 s below 2^-6 s.  The floor of 2^-100 keeps 1 / s finite; a block of
+// zeros has codes of zero.  A block with an entry that is not finite has the scale NaN and codes NaN: the products that read it give NaN, and no others do.
+#pragma once
+
+#include "typed.cuh"
+
+namespace pk {
+namespace fp8 {
+
+constexpr int kBlock = 128;
+constexpr int kAct = 5;  // kinds of pk_fp8_act
+
+inline bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+__host__ __device__ inline int blocks_of(int n) { return (int)(((long)n + kBlock - 1) / kBlock); }
+// codes [rows][ld] and their scales as every entry point takes them
+inline bool codes_ok(const void* codes, long ld, int width) { return codes && al16(codes) && ld % 16 == 0 && ld >= width && ld < 1L << 39; }
+inline bool row_scales_ok(const float* scales, long ld_s, int tokens) { return scales && al16(scales) && ld_s % 4 == 0 && ld_s >= tokens; }
+
+__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }  // as bits: a maximum of those keeps infinities and NaN
+
+struct Scale {
+  float s, inv;  // NaN where the block has an entry that is not finite
+};
+__device__ __forceinline__ Scale scale_of(uint32_t amax) {
+  Scale r;
+  r.s = amax >= 0x7f800000u ? __uint_as_float(0x7fffffffu) : fmaxf(__uint_as_float(amax), 7.888609e-31f) / 448.f;
+  r.inv = 1.f / r.s;
+  return r;
+}
+// v / s to its nearest fp32 number: v * (1 / s) and a step of Newton's, whose remainder v - q s is exact.  Without it a quotient that lies just between two codes,
+// as bf16 entries have them often, went to either.
+__device__ __forceinline__ float quotient(float v, Scale k) {
+  const float q = v * k.inv;
+  return fmaf(fmaf(-q, k.s, v), k.inv, q);
+}
+__device__ __forceinline__ uint32_t codes2(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ uint32_t codes4(const float* v, Scale k) {
+  return codes2(quotient(v[0], k), quotient(v[1], k)) | codes2(quotient(v[2], k), quotient(v[3], k)) << 16;
+}
+// the largest of 16 lanes, which have a block together
+__device__ __forceinline__ uint32_t max16(uint32_t m) {
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+  return m;
+}
+__device__ __forceinline__ uint32_t max8(const float* v) {
+  uint32_t m = magnitude(v[0]);
+#pragma unroll
+  for (int e = 1; e < 8; ++e) m = max(m, magnitude(v[e]));
+  return m;
+}
+
+// 8 entries from p on, of which the first n exist (the others are zero); VEC: n is 0 or 8 and p on a 16-byte boundary
+template <bool VEC>
+__device__ __forceinline__ void load8(const bf16* p, int n, float* v) {
+  if constexpr (VEC) {
+    const uint4 a = n > 0 ? *reinterpret_cast<const uint4*>(p) : make_uint4(0, 0, 0, 0);
+    const uint32_t u[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      v[2 * e] = bf16_lo(u[e]);
+      v[2 * e + 1] = bf16_hi(u[e]);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = e < n ? bf2f(p[e]) : 0.f;
+  }
+}
+template <bool VEC>
+__device__ __forceinline__ void load8(const float* p, int n, float* v) {
+  if constexpr (VEC) {
+    const float4 none = make_float4(0.f, 0.f, 0.f, 0.f);
+    const float4 a = n > 0 ? reinterpret_cast<const float4*>(p)[0] : none, b = n > 0 ? reinterpret_cast<const float4*>(p)[1] : none;
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = e < n ? p[e] : 0.f;
+  }
+}
+template <bool VEC>
+__device__ __forceinline__ void store8(bf16* p, int n, const float* v) {
+  if constexpr (VEC) {
+    if (n > 0) *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < n) p[e] = f2bf(v[e]);
+  }
+}
+template <bool VEC>
+__device__ __forceinline__ void store8(float* p, int n, const float* v) {
+  if constexpr (VEC) {
+    if (n > 0) {
+      reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+      reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < n) p[e] = v[e];
+  }
+}
+// 8 codes of which the first n exist; p is on an 8-byte boundary
+__device__ __forceinline__ void store_codes8(uint8_t* p, int n, const float* v, Scale k) {
+  const uint32_t lo = codes4(v, k), hi = codes4(v + 4, k);
+  if (n >= 8) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(lo, hi);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < n) p[e] = (uint8_t)((e < 4 ? lo : hi) >> (8 * (e & 3)));
+  }
+}
+
+// act 0 SiLU, 1 ReLU, 2 GELU in its tanh form, of z; fp32, the exponential by the special-function unit (2^-22)
+template <int ACT>
+__device__ __forceinline__ float gate_act(float z) {
+  if constexpr (ACT == 1) return z < 0.f ? 0.f : z;  // (NaN stays)
+  if constexpr (ACT == 2) return __fdividef(z, 1.f + __expf(-1.5957691216057308f * (z + 0.044715f * z * z * z)));
+  return __fdividef(z, 1.f + __expf(-z));
+}
+
+}  // namespace fp8
+}  // namespace pk

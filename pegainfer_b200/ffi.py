@@ -216,6 +216,12 @@ RES32_SIGNATURES = {
     "pk_kv8_attention_workspace_bytes": (i64l, [i32] * 5 + [C.POINTER(Kv8Options), i32]),
     "pk_kv8_attention": (i32, [vp] * 8 + [i64l] + [i32] * 6 + [f32, C.POINTER(Kv8Options), vp, i64l, i32, vp]),
     "pk_kv8_evict": (i32, [vp, i64l, i32, vp, vp, vp, vp, i64l, vp, vp, vp, vp, i64l, vp] + [i32] * 8 + [vp]),
+    # linear layers of 8 bits
+    "pk_fp8_add_norm": (i32, [vp, vp, i32, vp, f32, vp, i64l, vp, i64l, i32, i32, f32, vp]),
+    "pk_fp8_act": (i32, [vp, i64l, i32, vp, i64l, vp, i64l, i32, i32, vp]),
+    "pk_fp8_weights": (i32, [vp, i32, i64l, vp, i64l, vp, i32, i32, vp]),
+    "pk_fp8_gemm": (i32, [vp, i64l, vp, vp, i64l, vp, i64l, vp, i64l] + [i32] * 4 + [vp]),
+    "pk_fp8_gemm_gated": (i32, [vp, vp, vp, vp, i64l, vp, i64l, vp, i64l, vp, i64l, vp, i64l] + [i32] * 4 + [vp]),
 }
 
 
