@@ -1,13 +1,13 @@
 // The product of 8-bit rows and weights for prompts, on CTA pairs (fp8_gemm.cuh): y = x w^T, and act(x w^T) * (x w2^T) quantised again.
 //
-// A pair (cluster of two, tcgen05 cta_group::2) has a tile of 256 tokens x BN features: A = X, 128 tokens to a CTA, B = W, half the features to a CTA.
-//   warp 0  TMA producer (both CTAs): 128 entries of K a stage, completing on the leader's barrier
-//   warp 1  MMA issuer (leader): four tcgen05.mma (M 256, N BN, K 32) a block of K into one of two partial sums in tensor memory
-//   warps 4-11  take a block's partial sum out of tensor memory while the next one is computed, multiply it by its scales and add it to the tile's sum, which they hold in registers
-//           (thread = token, BN / 2 features).  A thread's token has one scale a block, its features one: a multiplication for all, and half an instruction
-//           (fma.rn.f32x2) for an entry, 256 of the 512 clocks that the block's MMAs take.
-// Gated: B is 128 rows of w (leader) and the same 128 of w2 (peer), so a thread has 64 features of both; 128 features are a block of the result's scales, whose largest magnitude two threads
-// find together.
+// A pair (cluster of two, tcgen05 cta_group::2) has a tile of 256 tokens x 256 features: A = X, 128 tokens to a CTA, B = W, half the features to a CTA.
+//   warp 0     TMA producer (both CTAs): 128 entries of K a stage, completing on the leader's barrier
+//   warp 1     MMA issuer (leader): a block of K is two products (M 256, N 128: the tile's halves) of four tcgen05.mma each, into partial sums in tensor memory, two of each half
+//   warps 2, 3 the scales of even and odd blocks of K into shared memory, a token's times the weights'
+//   warps 4-19 (eight to a half) take a half's partial sum out of tensor memory while the others are computed and add it, times its scale, to the tile's sum, which they hold in registers
+//              (thread = token, 64 features): half an instruction an entry (fma.rn.f32x2)
+// Gated: B is 128 rows of w (leader) and the same 128 of w2 (peer); a half is 64 features of both, a thread has 32 features of both; 128 features are a block of the result's
+// scales, whose largest magnitude four threads find together.
 // Every barrier wait is bounded (mbar_wait_bounded, common.cuh).
 #include <cuda.h>
 
@@ -20,13 +20,35 @@ namespace fp8 {
 
 namespace {
 
-constexpr int kBM = 128;                     // tokens per CTA
-constexpr int kEpi = 8;                      // epilogue warps
-constexpr int kThreads = 128 + 32 * kEpi;     // warps 0 to 3: TMA, MMA, two without work (registers are given out by four warps)
-// registers of a thread: the 65536 of an SM by 384 threads, then by role
-constexpr int kRegsLaunch = 168, kRegsOther = 56, kRegsEpi = 224;
+constexpr int kBM = 128, kBN = 256, kHalf = kBN / 2;  // tokens per CTA; features of a tile, of its halves
+constexpr int kStages = 6;
+constexpr int kEpi = 16;                     // epilogue warps
+constexpr int kThreads = 128 + 32 * kEpi;
+constexpr int kABytes = kBM * kBK, kBBytes = kHalf * kBK, kStageBytes = kABytes + kBBytes;
+// registers of a thread: the 65536 of an SM by 640 threads, then by role
+constexpr int kRegsLaunch = 96, kRegsOther = 64, kRegsEpi = 104;
 static_assert(128 * kRegsOther + 32 * kEpi * kRegsEpi <= kThreads * kRegsLaunch, "what the block was launched with");
+constexpr int kAhead = 4;  // blocks of its own that a scales' warp fetches ahead
 
+struct Shared {  // behind the stages
+  uint64_t full[kStages];    // used in the leader
+  uint64_t empty[kStages];   // one per CTA (multicast commit)
+  uint64_t tfull[2][2];      // [buffer][half] one per CTA: the MMAs' commit, the scales
+  uint64_t tempty[2][2];     // used in the leader: an arrival per epilogue warp of the half, of both CTAs
+  uint64_t done;             // behind a run-out: the MMAs under way
+  uint32_t tmem;
+  int dead;
+  float scale[8][2][kBM];    // of eight blocks of K: of the first half and the second; gated: of w and w2
+  uint32_t largest[2][4][kBM];  // gated: magnitudes of two tiles' rows, by 32 features
+};
+constexpr size_t kSmem = 227 * 1024;  // all of it: nobody else is resident on an SM whose tensor memory this kernel has (fp8_gemm_few.cu)
+static_assert((size_t)kStages * kStageBytes + 1024 + sizeof(Shared) <= kSmem, "shared memory of a CTA");
+
+// An arrival without a release: what it reports are reads of tensor memory, complete and fenced (tcgen05.wait::ld, fence::before_thread_sync); no memory is handed over.  A release at the
+// cluster's scope waits for the thread's loads in flight as well, 1500 to 2000 clocks for each block of K.
+__device__ __forceinline__ void arrive_relaxed(uint32_t bar_cluster_addr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster_addr) : "memory");
+}
 __device__ __forceinline__ void umma_f8_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
@@ -56,33 +78,23 @@ __device__ __forceinline__ void store32(float* base, long ld, int tok, int N, in
 }
 
 template <int ACT>
-__device__ __forceinline__ void activate(uint64_t* acc, float* v) {  // acc: 32 pairs of the gate, 32 of the factor
+__device__ __forceinline__ void activate(const uint64_t* acc, float* v) {  // acc: 16 pairs of the gate, 16 of the factor
 #pragma unroll
-  for (int j = 0; j < 32; ++j) {
-    v[2 * j] = gate_act<ACT>(lo_of(acc[j])) * lo_of(acc[32 + j]);
-    v[2 * j + 1] = gate_act<ACT>(hi_of(acc[j])) * hi_of(acc[32 + j]);
+  for (int j = 0; j < 16; ++j) {
+    v[2 * j] = gate_act<ACT>(lo_of(acc[j])) * lo_of(acc[16 + j]);
+    v[2 * j + 1] = gate_act<ACT>(hi_of(acc[j])) * hi_of(acc[16 + j]);
   }
 }
 
 // GATED: O is the codes' type
-template <int BN, int STAGES, bool GATED, typename O>
+template <bool GATED, typename O>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_w2, const Product p) {
-  constexpr int HB = BN / 2;  // B rows staged per CTA; features of a thread
-  constexpr int A_BYTES = kBM * kBK, B_BYTES = HB * kBK, STAGE_BYTES = A_BYTES + B_BYTES;
-  constexpr int FEATURES = GATED ? HB : BN;  // of a tile
-  static_assert(!GATED || BN == 256, "128 features are a block of the result's scales");
+  constexpr int FEATURES = GATED ? kHalf : kBN;  // of a tile
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + (size_t)STAGES * STAGE_BYTES);  // used in the leader
-  uint64_t* empty = full + STAGES;   // one per CTA (multicast commit)
-  uint64_t* tfull = empty + STAGES;  // [2] one per CTA
-  uint64_t* tempty = tfull + 2;      // [2] used in the leader (an arrival per epilogue warp of both CTAs)
-  uint64_t* done = tempty + 2;       // behind a run-out: the MMAs under way
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
-  volatile int* dead = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  uint32_t* largest = tmem_slot + 2;  // [2][2][128] gated: magnitudes of two tiles' rows, by half
-  static_assert((2 * STAGES + 5) * 8 + 8 + 2048 <= 2304, "room behind the stages");
+  Shared& sh = *reinterpret_cast<Shared*>(smem + (size_t)kStages * kStageBytes);
+  volatile int* dead = &sh.dead;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
@@ -94,24 +106,24 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
   const int pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < STAGES; ++s) {
-      mbar_init(full + s, 1);
-      mbar_init(empty + s, 1);
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(sh.full + s, 1);
+      mbar_init(sh.empty + s, 1);
     }
-    for (int s = 0; s < 2; ++s) {
-      mbar_init(tfull + s, 1);
-      mbar_init(tempty + s, 2 * kEpi);
+    for (int s = 0; s < 4; ++s) {
+      mbar_init(&sh.tfull[0][0] + s, 2);
+      mbar_init(&sh.tempty[0][0] + s, kEpi);
     }
-    mbar_init(done, 1);
+    mbar_init(&sh.done, 1);
     *dead = 0;
     mbar_fence_init();
   }
-  if (warp == 1) g2_tmem_alloc(tmem_slot, 2 * BN);
+  if (warp == 1) g2_tmem_alloc(&sh.tmem, 2 * kBN);
   tc_fence_before();
   __syncthreads();
   cluster_barrier();  // both CTAs' barriers are initialised and both TMEM allocations are done
   tc_fence_after();
-  const uint32_t tmem_base = *tmem_slot;
+  const uint32_t tmem_base = sh.tmem;
   pdl_wait();
 
   if (warp < 4) {
@@ -127,16 +139,18 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
         for (long tile = pair; tile < num_tiles && go; tile += num_pairs) {
           const int mb = (int)(tile % m_tiles), nb = (int)(tile / m_tiles);
           const int tok0 = mb * 2 * kBM + (int)rank * kBM;
-          const int row0 = GATED ? nb * HB : nb * BN + (int)rank * HB;
+          // 64 rows of each half: a product's columns are the leader's 64 rows, then the peer's
+          const int row0 = GATED ? nb * kHalf : nb * kBN + (int)rank * 64, row1 = row0 + (GATED ? 64 : kHalf);
           for (int kb = 0; kb < kb_n; ++kb) {
-            go = mbar_wait_bounded(empty + s, ph, dead);
+            go = mbar_wait_bounded(sh.empty + s, ph, dead);
             if (!go) break;
-            const uint32_t fb = g2_map(smem_u32(full + s), 0);
-            if (leader) mbar_expect_tx(full + s, 2 * STAGE_BYTES);
-            uint8_t* st = smem + (size_t)s * STAGE_BYTES;
+            const uint32_t fb = g2_map(smem_u32(sh.full + s), 0);
+            if (leader) mbar_expect_tx(sh.full + s, 2 * kStageBytes);
+            uint8_t* st = smem + (size_t)s * kStageBytes;
             g2_tma_2d(st, &map_x, kb * kBK, tok0, fb);
-            g2_tma_2d(st + A_BYTES, mw, kb * kBK, row0, fb);
-            if (++s == STAGES) {
+            g2_tma_2d(st + kABytes, mw, kb * kBK, row0, fb);
+            g2_tma_2d(st + kABytes + kBBytes / 2, mw, kb * kBK, row1, fb);
+            if (++s == kStages) {
               s = 0;
               ph ^= 1u;
             }
@@ -146,23 +160,33 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
       }
     } else if (warp == 1) {
       if (leader && tc_elect_one()) {
-        constexpr uint32_t idesc = f8_idesc(2 * kBM, BN);
+        constexpr uint32_t idesc = f8_idesc(2 * kBM, kHalf);
         int s = 0, buf = 0;
         uint32_t ph = 0, tph = 1;
         bool go = true;
         for (long tile = pair; tile < num_tiles && go; tile += num_pairs) {
           for (int kb = 0; kb < kb_n; ++kb) {
-            go = mbar_wait_bounded(tempty + buf, tph, dead) && mbar_wait_bounded(full + s, ph, dead);
+            // three looks at once: a wait costs this thread 200 clocks where nothing is to be waited for, a block's MMAs take 512
+            const bool here = mbar_test_wait(sh.full + s, ph), free0 = mbar_test_wait(&sh.tempty[buf][0], tph), free1 = mbar_test_wait(&sh.tempty[buf][1], tph);
+            if (!here) go = mbar_wait_bounded(sh.full + s, ph, dead);
+            if (go && !free0) go = mbar_wait_bounded(&sh.tempty[buf][0], tph, dead);
             if (!go) break;
             tc_fence_after();
-            const uint32_t a_addr = smem_u32(smem + (size_t)s * STAGE_BYTES);
-            const uint64_t adesc = make_sw128_desc(a_addr), bdesc = make_sw128_desc(a_addr + A_BYTES);
-            const uint32_t d = tmem_base + (uint32_t)(buf * BN);
-  #pragma unroll
+            const uint32_t a_addr = smem_u32(smem + (size_t)s * kStageBytes);
+            const uint64_t adesc = make_sw128_desc(a_addr), bdesc = make_sw128_desc(a_addr + kABytes);
+            const uint32_t d = tmem_base + (uint32_t)(buf * kBN);
+#pragma unroll
             for (int k = 0; k < kBK / 32; ++k) umma_f8_pair(d, adesc + (uint64_t)(k * 2), bdesc + (uint64_t)(k * 2), idesc, k > 0 ? 1u : 0u);
-            g2_commit_both(empty + s);
-            g2_commit_both(tfull + buf);
-            if (++s == STAGES) {
+            g2_commit_both(&sh.tfull[buf][0]);
+            if (!free1) go = mbar_wait_bounded(&sh.tempty[buf][1], tph, dead);
+            if (!go) break;
+            tc_fence_after();
+#pragma unroll
+            for (int k = 0; k < kBK / 32; ++k)
+              umma_f8_pair(d + kHalf, adesc + (uint64_t)(k * 2), bdesc + (uint64_t)((kBBytes / 2 >> 4) + k * 2), idesc, k > 0 ? 1u : 0u);
+            g2_commit_both(&sh.tfull[buf][1]);
+            g2_commit_both(sh.empty + s);
+            if (++s == kStages) {
               s = 0;
               ph ^= 1u;
             }
@@ -173,78 +197,129 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
           }
         }
         if (!go) {
-          g2_commit_both(done);
-          mbar_drain(done, 0);
+          g2_commit_both(&sh.done);
+          mbar_drain(&sh.done, 0);
         }
+      }
+    } else {
+      // Blocks of K as they come, tile behind tile, every second one.  A lane has four tokens.  Slot it % 8 held block it - 8: whoever
+      // gave back the partial sums of block it - 4 had used it, and without those the MMAs of block it - 2, whose end is waited for here, did not begin.
+      const int mine = warp - 2;
+      float4 x_at[kAhead];
+      float a_at[kAhead], b_at[kAhead];
+      long f_tile = pair;
+      int f_kb = 0;
+      auto step = [&](long& tile, int& kb, int by) {
+        kb += by;
+        while (kb >= kb_n && tile < num_tiles) {
+          kb -= kb_n;
+          tile += num_pairs;
+        }
+      };
+      auto fetch = [&](int i) {  // (asm: where it stands)
+        x_at[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        a_at[i] = b_at[i] = 0.f;
+        if (f_tile < num_tiles) {
+          const int mb = (int)(f_tile % m_tiles), nb = (int)(f_tile / m_tiles);
+          const int tok = mb * 2 * kBM + (int)rank * kBM + lane * 4;
+          const int w0 = GATED ? nb : 2 * nb, w1 = GATED ? nb : (2 * nb + 1) * kBlock < M ? 2 * nb + 1 : 2 * nb;
+          if (tok < N)  // (rows of scales are whole fours)
+            asm volatile("ld.global.nc.v4.f32 {%0, %1, %2, %3}, [%4];"
+                         : "=f"(x_at[i].x), "=f"(x_at[i].y), "=f"(x_at[i].z), "=f"(x_at[i].w)
+                         : "l"(p.sx + (size_t)f_kb * p.ld_sx + tok));
+          asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(a_at[i]) : "l"(p.sw + (size_t)w0 * kb_n + f_kb));
+          asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(b_at[i]) : "l"((GATED ? p.sw2 : p.sw) + (size_t)w1 * kb_n + f_kb));
+        }
+        step(f_tile, f_kb, 2);
+      };
+      step(f_tile, f_kb, mine);
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) fetch(i);
+      long tile = pair;
+      int kb = 0;
+      step(tile, kb, mine);
+      uint32_t ph = 1;  // of tfull[mine]: before its first phase
+      for (int slot = mine; tile < num_tiles; slot = (slot + 2) & 7) {
+        const float4 x = x_at[0];
+        const float a = a_at[0], b = b_at[0];
+#pragma unroll
+        for (int i = 0; i + 1 < kAhead; ++i) {
+          x_at[i] = x_at[i + 1];
+          a_at[i] = a_at[i + 1];
+          b_at[i] = b_at[i + 1];
+        }
+        fetch(kAhead - 1);
+        mbar_wait_bounded(&sh.tfull[mine][0], ph, dead);
+        mbar_wait_bounded(&sh.tfull[mine][1], ph, dead);
+        reinterpret_cast<float4*>(sh.scale[slot][0])[lane] = make_float4(x.x * a, x.y * a, x.z * a, x.w * a);
+        reinterpret_cast<float4*>(sh.scale[slot][1])[lane] = make_float4(x.x * b, x.y * b, x.z * b, x.w * b);
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&sh.tfull[mine][0]);
+          mbar_arrive(&sh.tfull[mine][1]);
+        }
+        ph ^= 1u;
+        step(tile, kb, 2);
       }
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsEpi));
-    const int q = warp & 3, half = (warp - 4) >> 2, row = q * 32 + lane;
-    const uint32_t tempty_leader = g2_map(smem_u32(tempty), 0);
-    const uint32_t t_row = tmem_base + ((uint32_t)(q * 32) << 16);
-    int buf = 0, lt = 0;
+    const int q = warp & 3, part = (warp - 4) >> 2, half = part >> 1, sub = part & 1, row = q * 32 + lane;
+    const uint32_t tempty_leader = g2_map(smem_u32(&sh.tempty[0][half]), 0);
+    // the thread's two pieces of 32 columns; gated: 32 of the gate, then the same 32 of the factor
+    const uint32_t t_row = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(half * kHalf + sub * (GATED ? 32 : 64));
+    constexpr uint32_t kPiece = GATED ? 64 : 32;
+    int buf = 0, it = 0, lt = 0;
     uint32_t tph = 0;
+    bool ready = false;
     for (long tile = pair; tile < num_tiles; tile += num_pairs, ++lt) {
       const int mb = (int)(tile % m_tiles), nb = (int)(tile / m_tiles);
       const int tok = mb * 2 * kBM + (int)rank * kBM + row;
-      const int f0 = GATED ? nb * HB + half * (HB / 2) : nb * BN + half * HB;  // the thread's first feature
-      const float* sx = p.sx + (tok < N ? tok : 0);
-      const float* sw = p.sw + (size_t)(f0 < M ? f0 / kBlock : 0) * kb_n;
-      const float* sw2 = GATED ? p.sw2 + (size_t)(f0 < M ? f0 / kBlock : 0) * kb_n : nullptr;
-      uint64_t acc[HB / 2];
+      const int f0 = GATED ? nb * kHalf + half * 64 + sub * 32 : nb * kBN + half * kHalf + sub * 64;  // the thread's first feature
+      uint64_t acc[32];
 #pragma unroll
-      for (int j = 0; j < HB / 2; ++j) acc[j] = 0;
-      float x_next = __ldg(sx), w_next = __ldg(sw), w2_next = GATED ? __ldg(sw2) : 0.f;
+      for (int j = 0; j < 32; ++j) acc[j] = 0;
 #pragma unroll 1
-      for (int kb = 0; kb < kb_n; ++kb) {
-        const float s1 = x_next * w_next, s2 = GATED ? x_next * w2_next : s1;
-        if (kb + 1 < kb_n) {
-          x_next = __ldg(sx + (size_t)(kb + 1) * p.ld_sx);
-          w_next = __ldg(sw + kb + 1);
-          if (GATED) w2_next = __ldg(sw2 + kb + 1);
-        }
-        mbar_wait_bounded(tfull + buf, tph, dead);
+      for (int kb = 0; kb < kb_n; ++kb, ++it) {
+        if (!ready) mbar_wait_bounded(&sh.tfull[buf][half], tph, dead);
         tc_fence_after();
-        const uint32_t t0 = t_row + (uint32_t)(buf * BN);
-        // columns of the thread's piece c of 32; gated: 64 of the gate, then 64 of the factor
-        auto column = [&](int c) { return (uint32_t)(GATED ? (c < HB / 2 ? half * (HB / 2) + c : HB / 2 + half * (HB / 2) + c) : half * HB + c); };
-        uint32_t v[2][32];
-        tmem_ld32_nowait(t0 + column(0), v[0]);
+        const uint32_t t0 = t_row + (uint32_t)(buf * kBN);
+        uint32_t v[32];
+        tmem_ld32_nowait(t0, v);
+        const float s1 = sh.scale[it & 7][GATED ? 0 : half][row], s2 = GATED ? sh.scale[it & 7][1][row] : s1;
+        const uint64_t ss1 = pair_of(s1, s1), ss2 = pair_of(s2, s2);
+        tmem_wait32(v);
 #pragma unroll
-        for (int c = 0; c < HB; c += 32) {
-          uint32_t* now = v[(c / 32) & 1];
-          tmem_wait32(now);
-          if (c + 32 < HB) tmem_ld32_nowait(t0 + column(c + 32), v[(c / 32 + 1) & 1]);
-          const float s = GATED && c >= HB / 2 ? s2 : s1;
-          const uint64_t ss = pair_of(s, s);
-#pragma unroll
-          for (int j = 0; j < 16; ++j) fma2(acc[c / 2 + j], pair_of(now[2 * j], now[2 * j + 1]), ss);
-        }
+        for (int j = 0; j < 16; ++j) fma2(acc[j], pair_of(v[2 * j], v[2 * j + 1]), ss1);
+        tmem_ld32_nowait(t0 + kPiece, v);
+        const int next = buf ^ 1;
+        const uint32_t next_ph = buf ? tph ^ 1u : tph;
+        ready = mbar_test_wait(&sh.tfull[next][half], next_ph);  // (asked for early)
+        tmem_wait32(v);
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) g2_arrive_cluster(tempty_leader + (uint32_t)(buf * 8));
-        if (++buf == 2) {
-          buf = 0;
-          tph ^= 1u;
-        }
+        if (lane == 0) arrive_relaxed(tempty_leader + (uint32_t)(buf * 2 * sizeof(uint64_t)));
+#pragma unroll
+        for (int j = 0; j < 16; ++j) fma2(acc[16 + j], pair_of(v[2 * j], v[2 * j + 1]), ss2);
+        buf = next;
+        tph = next_ph;
       }
       if constexpr (GATED) {
-        float v[HB / 2];
+        float v[32];
         if (p.act == 0) activate<0>(acc, v);
         else if (p.act == 1) activate<1>(acc, v);
         else activate<2>(acc, v);
         uint32_t m = 0;
 #pragma unroll
-        for (int j = 0; j < HB / 2; ++j) m = max(m, magnitude(v[j]));
-        uint32_t* mine = largest + (lt & 1) * 256;  // (the other tile's are read until the barrier behind this one)
-        mine[half * 128 + row] = m;
+        for (int j = 0; j < 32; ++j) m = max(m, magnitude(v[j]));
+        uint32_t(*mine)[kBM] = sh.largest[lt & 1];  // (the other tile's are read until the barrier behind this one)
+        mine[part][row] = m;
         asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpi) : "memory");
-        const Scale k = scale_of(max(mine[row], mine[128 + row]));
+        const Scale k = scale_of(max(max(mine[0][row], mine[1][row]), max(mine[2][row], mine[3][row])));
         if (tok < N && f0 < M) {
           uint8_t* dst = p.codes + (size_t)tok * p.ld + f0;
 #pragma unroll
-          for (int c = 0; c < HB / 2; c += 16) {
+          for (int c = 0; c < 32; c += 16) {
             uint32_t u[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) u[j] = codes4(v + c + 4 * j, k);
@@ -256,13 +331,13 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
                 if (f0 + c + j < M) dst[c + j] = (uint8_t)(u[j / 4] >> (8 * (j & 3)));
             }
           }
-          if (half == 0) p.scales[(size_t)(f0 / kBlock) * p.ld_s + tok] = k.s;
+          if (part == 0) p.scales[(size_t)nb * p.ld_s + tok] = k.s;
         }
       } else {
         O* y = static_cast<O*>(p.y);
         const bool vec = (p.ld_y * (long)sizeof(O)) % 16 == 0 && (reinterpret_cast<uintptr_t>(y) & 15) == 0;
 #pragma unroll
-        for (int c = 0; c < HB; c += 32) {
+        for (int c = 0; c < 64; c += 32) {
           if (tok - lane >= N || f0 + c >= M) continue;  // (a warp at a time: the lanes store for one another)
           if (vec && f0 + c + 32 <= M) {
             store32(y + f0 + c, p.ld_y, tok, N, lane, acc + c / 2);
@@ -280,26 +355,23 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
   cluster_barrier();  // the peer's MMAs / loads may still target this CTA's shared memory and TMEM
   if (warp == 1) {
     tc_fence_after();
-    g2_tmem_dealloc(tmem_base, 2 * BN);
+    g2_tmem_dealloc(tmem_base, 2 * kBN);
   }
   if (threadIdx.x == 0) count_run_out(dead, p.err);
 }
 
-template <int BN, int STAGES, bool GATED, typename O>
+template <bool GATED, typename O>
 int launch_pair(const Product& p, cudaStream_t st) {
-  static_assert((size_t)STAGES * (kBM + BN / 2) * kBK + 1024 + 2304 <= 227 * 1024, "shared memory of a CTA");
-  constexpr size_t smem = 227 * 1024;  // all of it: nobody else is resident on an SM whose tensor memory this kernel has (fp8_gemm_few.cu)
-  auto kern = fp8_gemm_kernel<BN, STAGES, GATED, O>;
+  auto kern = fp8_gemm_kernel<GATED, O>;
   static std::atomic<uint64_t> set{0};
-  if (const cudaError_t e = allow_smem(set, (const void*)kern, smem); e != cudaSuccess) return (int)e;
+  if (const cudaError_t e = allow_smem(set, (const void*)kern, kSmem); e != cudaSuccess) return (int)e;
   CUtensorMap mx, mw, mw2;
-  if (!make_codes_map(&mx, p.x, p.N, p.K, p.ld_x, kBM) || !make_codes_map(&mw, p.w, p.M, p.K, p.ld_w, BN / 2) ||
-      !make_codes_map(&mw2, GATED ? p.w2 : p.w, p.M, p.K, p.ld_w, BN / 2))
+  if (!make_codes_map(&mx, p.x, p.N, p.K, p.ld_x, kBM) || !make_codes_map(&mw, p.w, p.M, p.K, p.ld_w, 64) || !make_codes_map(&mw2, GATED ? p.w2 : p.w, p.M, p.K, p.ld_w, 64))
     return (int)cudaErrorInvalidValue;
-  constexpr int features = GATED ? BN / 2 : BN;
+  constexpr int features = GATED ? kHalf : kBN;
   const long tiles = (long)((p.N + 2 * kBM - 1) / (2 * kBM)) * ((p.M + features - 1) / features);
   const int pairs = (int)std::min<long>(std::max(1, sm_count() / 2), tiles);
-  return (int)launch(kern, dim3(2 * pairs), dim3(kThreads), smem, st, true, mx, mw, mw2, p);
+  return (int)launch(kern, dim3(2 * pairs), dim3(kThreads), kSmem, st, true, mx, mw, mw2, p);
 }
 
 }  // namespace
@@ -333,7 +405,7 @@ extern "C" int pk_fp8_gemm(const void* w, long ld_w, const float* w_scales, cons
   p.kb = fp8::blocks_of(K);
   p.err = wait_err_word();
   if (fp8::few_takes(p, false)) return fp8::launch_few(p, false, y_f32, st);
-  return y_f32 ? fp8::launch_pair<256, 6, false, float>(p, st) : fp8::launch_pair<256, 6, false, bf16>(p, st);
+  return y_f32 ? fp8::launch_pair<false, float>(p, st) : fp8::launch_pair<false, bf16>(p, st);
 }
 
 extern "C" int pk_fp8_gemm_gated(const void* w_gate, const float* gate_scales, const void* w_up, const float* up_scales, long ld_w, const void* x, long ld_x,
@@ -363,5 +435,5 @@ extern "C" int pk_fp8_gemm_gated(const void* w_gate, const float* gate_scales, c
   p.act = act;
   p.err = wait_err_word();
   if (fp8::few_takes(p, true)) return fp8::launch_few(p, true, false, st);
-  return fp8::launch_pair<256, 6, true, uint8_t>(p, st);
+  return fp8::launch_pair<true, uint8_t>(p, st);
 }
