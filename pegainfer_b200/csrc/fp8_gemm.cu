@@ -26,9 +26,8 @@ constexpr int kEpi = 16;                     // epilogue warps
 constexpr int kThreads = 128 + 32 * kEpi;
 constexpr int kABytes = kBM * kBK, kBBytes = kHalf * kBK, kStageBytes = kABytes + kBBytes;
 // registers of a thread: the 65536 of an SM by 640 threads, then by role
-constexpr int kRegsLaunch = 96, kRegsOther = 64, kRegsEpi = 104;
+constexpr int kRegsLaunch = 96, kRegsOther = 32, kRegsEpi = 112;
 static_assert(128 * kRegsOther + 32 * kEpi * kRegsEpi <= kThreads * kRegsLaunch, "what the block was launched with");
-constexpr int kAhead = 4;  // blocks of its own that a scales' warp fetches ahead
 
 struct Shared {  // behind the stages
   uint64_t full[kStages];    // used in the leader
@@ -58,11 +57,39 @@ __device__ __forceinline__ void umma_f8_pair(uint32_t d_tmem, uint64_t adesc, ui
       : "memory");
 }
 
+// Shared memory by its 32-bit address: what a loop with 64 sums and 32 of what comes to them keeps beside those has to be little
+__device__ __forceinline__ bool test_wait_at(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ float ld_shared_at(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]),
+        "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// acc += v * s, behind the wait that it stands behind (volatile: nothing moves it in front of that)
+__device__ __forceinline__ void fma_at(float& acc, uint32_t v, float s) { asm volatile("fma.rn.f32 %0, %1, %2, %0;" : "+f"(acc) : "f"(__uint_as_float(v)), "f"(s)); }
+
 // 32 columns of a warp's 32 rows; the lanes store for one another, four lanes 64 bytes of a row at a time (a lane that stored its own row would touch a line per 16 bytes)
-__device__ __forceinline__ void store32(bf16* base, long ld, int tok, int N, int lane, const uint64_t* acc) {
+__device__ __forceinline__ void store32(bf16* base, long ld, int tok, int N, int lane, const float* acc) {
   uint32_t u[16];
 #pragma unroll
-  for (int j = 0; j < 16; ++j) u[j] = pack_bf16(lo_of(acc[j]), hi_of(acc[j]));
+  for (int j = 0; j < 16; ++j) u[j] = pack_bf16(acc[2 * j], acc[2 * j + 1]);
   transpose4(u, lane);
   const int tok4 = tok & ~3;
   bf16* dst = base + (size_t)tok4 * ld + (lane & 3) * 8;
@@ -70,27 +97,23 @@ __device__ __forceinline__ void store32(bf16* base, long ld, int tok, int N, int
   for (int j = 0; j < 4; ++j)
     if (tok4 + j < N) *reinterpret_cast<uint4*>(dst + (size_t)j * ld) = make_uint4(u[4 * j], u[4 * j + 1], u[4 * j + 2], u[4 * j + 3]);
 }
-__device__ __forceinline__ void store32(float* base, long ld, int tok, int N, int lane, const uint64_t* acc) {
+__device__ __forceinline__ void store32(float* base, long ld, int tok, int N, int lane, const float* acc) {
   if (tok >= N) return;
   float4* dst = reinterpret_cast<float4*>(base + (size_t)tok * ld);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) dst[j] = make_float4(lo_of(acc[2 * j]), hi_of(acc[2 * j]), lo_of(acc[2 * j + 1]), hi_of(acc[2 * j + 1]));
+  for (int j = 0; j < 8; ++j) dst[j] = make_float4(acc[4 * j], acc[4 * j + 1], acc[4 * j + 2], acc[4 * j + 3]);
 }
 
 template <int ACT>
-__device__ __forceinline__ void activate(const uint64_t* acc, float* v) {  // acc: 16 pairs of the gate, 16 of the factor
+__device__ __forceinline__ void activate(const float* acc, float* v) {  // acc: 32 of the gate, 32 of the factor
 #pragma unroll
-  for (int j = 0; j < 16; ++j) {
-    v[2 * j] = gate_act<ACT>(lo_of(acc[j])) * lo_of(acc[16 + j]);
-    v[2 * j + 1] = gate_act<ACT>(hi_of(acc[j])) * hi_of(acc[16 + j]);
-  }
+  for (int j = 0; j < 32; ++j) v[j] = gate_act<ACT>(acc[j]) * acc[32 + j];
 }
 
 // GATED: O is the codes' type
 template <bool GATED, typename O>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_w2, const Product p) {
-  constexpr int FEATURES = GATED ? kHalf : kBN;  // of a tile
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   Shared& sh = *reinterpret_cast<Shared*>(smem + (size_t)kStages * kStageBytes);
@@ -101,8 +124,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
   const bool leader = rank == 0;
   const int M = p.M, N = p.N, kb_n = p.kb;
   const int m_tiles = (N + 2 * kBM - 1) / (2 * kBM);
-  const int n_tiles = (M + FEATURES - 1) / FEATURES;
-  const long num_tiles = (long)m_tiles * n_tiles;
+  const int num_tiles = p.tiles;
   const int pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
 
   if (threadIdx.x == 0) {
@@ -136,8 +158,8 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
         int s = 0;
         uint32_t ph = 1;
         bool go = true;
-        for (long tile = pair; tile < num_tiles && go; tile += num_pairs) {
-          const int mb = (int)(tile % m_tiles), nb = (int)(tile / m_tiles);
+        for (int tile = pair; tile < num_tiles && go; tile += num_pairs) {
+          const int mb = tile % m_tiles, nb = tile / m_tiles;
           const int tok0 = mb * 2 * kBM + (int)rank * kBM;
           // 64 rows of each half: a product's columns are the leader's 64 rows, then the peer's
           const int row0 = GATED ? nb * kHalf : nb * kBN + (int)rank * 64, row1 = row0 + (GATED ? 64 : kHalf);
@@ -164,7 +186,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
         int s = 0, buf = 0;
         uint32_t ph = 0, tph = 1;
         bool go = true;
-        for (long tile = pair; tile < num_tiles && go; tile += num_pairs) {
+        for (int tile = pair; tile < num_tiles && go; tile += num_pairs) {
           for (int kb = 0; kb < kb_n; ++kb) {
             // three looks at once: a wait costs this thread 200 clocks where nothing is to be waited for, a block's MMAs take 512
             const bool here = mbar_test_wait(sh.full + s, ph), free0 = mbar_test_wait(&sh.tempty[buf][0], tph), free1 = mbar_test_wait(&sh.tempty[buf][1], tph);
@@ -202,53 +224,33 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
         }
       }
     } else {
-      // Blocks of K as they come, tile behind tile, every second one.  A lane has four tokens.  Slot it % 8 held block it - 8: whoever
-      // gave back the partial sums of block it - 4 had used it, and without those the MMAs of block it - 2, whose end is waited for here, did not begin.
+      // Blocks of K as they come, tile behind tile, every second one, fetched one ahead.  A lane has four tokens.  Slot it % 8 held block it - 8: whoever gave back the partial sums of
+      // block it - 4 had used it, and without those the MMAs of block it - 2, whose end is waited for here, did not begin.
       const int mine = warp - 2;
-      float4 x_at[kAhead];
-      float a_at[kAhead], b_at[kAhead];
-      long f_tile = pair;
-      int f_kb = 0;
-      auto step = [&](long& tile, int& kb, int by) {
-        kb += by;
-        while (kb >= kb_n && tile < num_tiles) {
+      int tile = pair, kb = mine;
+      auto settle = [&]() {
+        while (kb >= kb_n) {
           kb -= kb_n;
           tile += num_pairs;
         }
       };
-      auto fetch = [&](int i) {  // (asm: where it stands)
-        x_at[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-        a_at[i] = b_at[i] = 0.f;
-        if (f_tile < num_tiles) {
-          const int mb = (int)(f_tile % m_tiles), nb = (int)(f_tile / m_tiles);
-          const int tok = mb * 2 * kBM + (int)rank * kBM + lane * 4;
-          const int w0 = GATED ? nb : 2 * nb, w1 = GATED ? nb : (2 * nb + 1) * kBlock < M ? 2 * nb + 1 : 2 * nb;
-          if (tok < N)  // (rows of scales are whole fours)
-            asm volatile("ld.global.nc.v4.f32 {%0, %1, %2, %3}, [%4];"
-                         : "=f"(x_at[i].x), "=f"(x_at[i].y), "=f"(x_at[i].z), "=f"(x_at[i].w)
-                         : "l"(p.sx + (size_t)f_kb * p.ld_sx + tok));
-          asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(a_at[i]) : "l"(p.sw + (size_t)w0 * kb_n + f_kb));
-          asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(b_at[i]) : "l"((GATED ? p.sw2 : p.sw) + (size_t)w1 * kb_n + f_kb));
-        }
-        step(f_tile, f_kb, 2);
+      float4 x;
+      float a, b;
+      auto fetch = [&]() {  // (asm: where it stands)
+        x = make_float4(0.f, 0.f, 0.f, 0.f);
+        a = b = 0.f;
+        if (tile >= num_tiles) return;
+        const int nb = tile / m_tiles, tok = (tile - nb * m_tiles) * 2 * kBM + (int)rank * kBM + lane * 4;
+        const int w0 = GATED ? nb : 2 * nb, w1 = GATED ? nb : (2 * nb + 1) * kBlock < M ? 2 * nb + 1 : 2 * nb;
+        if (tok < N)  // (rows of scales are whole fours)
+          asm volatile("ld.global.nc.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "l"(p.sx + (size_t)kb * p.ld_sx + tok));
+        asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(a) : "l"(p.sw + (size_t)w0 * kb_n + kb));
+        asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(b) : "l"((GATED ? p.sw2 : p.sw) + (size_t)w1 * kb_n + kb));
       };
-      step(f_tile, f_kb, mine);
-#pragma unroll
-      for (int i = 0; i < kAhead; ++i) fetch(i);
-      long tile = pair;
-      int kb = 0;
-      step(tile, kb, mine);
+      settle();
+      fetch();
       uint32_t ph = 1;  // of tfull[mine]: before its first phase
       for (int slot = mine; tile < num_tiles; slot = (slot + 2) & 7) {
-        const float4 x = x_at[0];
-        const float a = a_at[0], b = b_at[0];
-#pragma unroll
-        for (int i = 0; i + 1 < kAhead; ++i) {
-          x_at[i] = x_at[i + 1];
-          a_at[i] = a_at[i + 1];
-          b_at[i] = b_at[i + 1];
-        }
-        fetch(kAhead - 1);
         mbar_wait_bounded(&sh.tfull[mine][0], ph, dead);
         mbar_wait_bounded(&sh.tfull[mine][1], ph, dead);
         reinterpret_cast<float4*>(sh.scale[slot][0])[lane] = make_float4(x.x * a, x.y * a, x.z * a, x.w * a);
@@ -259,51 +261,53 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
           mbar_arrive(&sh.tfull[mine][1]);
         }
         ph ^= 1u;
-        step(tile, kb, 2);
+        kb += 2;
+        settle();
+        fetch();
       }
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsEpi));
     const int q = warp & 3, part = (warp - 4) >> 2, half = part >> 1, sub = part & 1, row = q * 32 + lane;
-    const uint32_t tempty_leader = g2_map(smem_u32(&sh.tempty[0][half]), 0);
+    const uint32_t tempty = g2_map(smem_u32(&sh.tempty[0][half]), 0), tfull = smem_u32(&sh.tfull[0][half]);
+    const uint32_t scales = smem_u32(&sh.scale[0][GATED ? 0 : half][row]);
     // the thread's two pieces of 32 columns; gated: 32 of the gate, then the same 32 of the factor
     const uint32_t t_row = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(half * kHalf + sub * (GATED ? 32 : 64));
     constexpr uint32_t kPiece = GATED ? 64 : 32;
-    int buf = 0, it = 0, lt = 0;
-    uint32_t tph = 0;
+    uint32_t it = 0, lt = 0;  // blocks of K so far, tiles
     bool ready = false;
-    for (long tile = pair; tile < num_tiles; tile += num_pairs, ++lt) {
-      const int mb = (int)(tile % m_tiles), nb = (int)(tile / m_tiles);
+    for (int tile = pair; tile < num_tiles; tile += num_pairs, ++lt) {
+      float acc[64];
+#pragma unroll
+      for (int j = 0; j < 64; ++j) acc[j] = 0.f;
+#pragma unroll 1
+      for (int kb = kb_n; kb > 0; --kb) {
+        const uint32_t buf = it & 1;
+        if (!ready) mbar_wait_bounded(&sh.tfull[buf][half], (it >> 1) & 1, dead);
+        tc_fence_after();
+        const uint32_t t0 = t_row + buf * kBN;
+        uint32_t v[2][16];
+        tmem_ld16(t0, v[0]);
+        const float s1 = ld_shared_at(scales + (it & 7) * (uint32_t)sizeof(sh.scale[0])), s2 = GATED ? ld_shared_at(scales + (it & 7) * (uint32_t)sizeof(sh.scale[0]) + kBM * 4) : s1;
+        ++it;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          tmem_wait();
+          if (c < 3) {
+            tmem_ld16(t0 + (c + 1 < 2 ? 16 : kPiece + (c - 1) * 16), v[(c + 1) & 1]);
+          } else {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) arrive_relaxed(tempty + buf * (uint32_t)sizeof(sh.tempty[0]));
+          }
+          if (c == 2) ready = test_wait_at(tfull + (it & 1) * (uint32_t)sizeof(sh.tfull[0]), (it >> 1) & 1);  // (asked for early)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) fma_at(acc[16 * c + j], v[c & 1][j], c < 2 ? s1 : s2);
+        }
+      }
+      const int mb = tile % m_tiles, nb = tile / m_tiles;
       const int tok = mb * 2 * kBM + (int)rank * kBM + row;
       const int f0 = GATED ? nb * kHalf + half * 64 + sub * 32 : nb * kBN + half * kHalf + sub * 64;  // the thread's first feature
-      uint64_t acc[32];
-#pragma unroll
-      for (int j = 0; j < 32; ++j) acc[j] = 0;
-#pragma unroll 1
-      for (int kb = 0; kb < kb_n; ++kb, ++it) {
-        if (!ready) mbar_wait_bounded(&sh.tfull[buf][half], tph, dead);
-        tc_fence_after();
-        const uint32_t t0 = t_row + (uint32_t)(buf * kBN);
-        uint32_t v[32];
-        tmem_ld32_nowait(t0, v);
-        const float s1 = sh.scale[it & 7][GATED ? 0 : half][row], s2 = GATED ? sh.scale[it & 7][1][row] : s1;
-        const uint64_t ss1 = pair_of(s1, s1), ss2 = pair_of(s2, s2);
-        tmem_wait32(v);
-#pragma unroll
-        for (int j = 0; j < 16; ++j) fma2(acc[j], pair_of(v[2 * j], v[2 * j + 1]), ss1);
-        tmem_ld32_nowait(t0 + kPiece, v);
-        const int next = buf ^ 1;
-        const uint32_t next_ph = buf ? tph ^ 1u : tph;
-        ready = mbar_test_wait(&sh.tfull[next][half], next_ph);  // (asked for early)
-        tmem_wait32(v);
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) arrive_relaxed(tempty_leader + (uint32_t)(buf * 2 * sizeof(uint64_t)));
-#pragma unroll
-        for (int j = 0; j < 16; ++j) fma2(acc[16 + j], pair_of(v[2 * j], v[2 * j + 1]), ss2);
-        buf = next;
-        tph = next_ph;
-      }
       if constexpr (GATED) {
         float v[32];
         if (p.act == 0) activate<0>(acc, v);
@@ -340,11 +344,11 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
         for (int c = 0; c < 64; c += 32) {
           if (tok - lane >= N || f0 + c >= M) continue;  // (a warp at a time: the lanes store for one another)
           if (vec && f0 + c + 32 <= M) {
-            store32(y + f0 + c, p.ld_y, tok, N, lane, acc + c / 2);
+            store32(y + f0 + c, p.ld_y, tok, N, lane, acc + c);
           } else if (tok < N) {
 #pragma unroll
             for (int j = 0; j < 32; ++j)
-              if (f0 + c + j < M) y[(size_t)tok * p.ld_y + f0 + c + j] = from_f<O>(j & 1 ? hi_of(acc[c / 2 + j / 2]) : lo_of(acc[c / 2 + j / 2]));
+              if (f0 + c + j < M) y[(size_t)tok * p.ld_y + f0 + c + j] = from_f<O>(acc[c + j]);
           }
         }
       }
@@ -361,16 +365,19 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
 }
 
 template <bool GATED, typename O>
-int launch_pair(const Product& p, cudaStream_t st) {
+int launch_pair(const Product& product, cudaStream_t st) {
+  constexpr int features = GATED ? kHalf : kBN;
+  Product p = product;
+  const long tiles = (long)((p.N + 2 * kBM - 1) / (2 * kBM)) * ((p.M + features - 1) / features);
+  const int pairs = (int)std::min<long>(std::max(1, sm_count() / 2), tiles);
+  if (tiles > 0x7fffffffL - 4 * pairs) return -2;
+  p.tiles = (int)tiles;
   auto kern = fp8_gemm_kernel<GATED, O>;
   static std::atomic<uint64_t> set{0};
   if (const cudaError_t e = allow_smem(set, (const void*)kern, kSmem); e != cudaSuccess) return (int)e;
   CUtensorMap mx, mw, mw2;
   if (!make_codes_map(&mx, p.x, p.N, p.K, p.ld_x, kBM) || !make_codes_map(&mw, p.w, p.M, p.K, p.ld_w, 64) || !make_codes_map(&mw2, GATED ? p.w2 : p.w, p.M, p.K, p.ld_w, 64))
     return (int)cudaErrorInvalidValue;
-  constexpr int features = GATED ? kHalf : kBN;
-  const long tiles = (long)((p.N + 2 * kBM - 1) / (2 * kBM)) * ((p.M + features - 1) / features);
-  const int pairs = (int)std::min<long>(std::max(1, sm_count() / 2), tiles);
   return (int)launch(kern, dim3(2 * pairs), dim3(kThreads), kSmem, st, true, mx, mw, mw2, p);
 }
 

@@ -28,6 +28,7 @@ struct Product {
   float* scales;
   long ld, ld_s;
   int M, N, K, kb;          // features, tokens, reduction, its blocks
+  int tiles;                // fp8_gemm.cu: of 256 tokens
   int act;                  // gated: 0 SiLU, 1 ReLU, 2 GELU
   unsigned int* err;        // wait_err_word()
 };
