@@ -21,7 +21,8 @@ namespace fp8 {
 namespace {
 
 constexpr int kBM = 128, kBN = 256, kHalf = kBN / 2;  // tokens per CTA; features of a tile, of its halves
-constexpr int kStages = 6;
+constexpr int kStages = 4;
+constexpr int kPieceBytes = 32 * 128;  // of the output: 32 tokens x 128 bytes, an epilogue warp's at a time
 constexpr int kEpi = 16;                     // epilogue warps
 constexpr int kThreads = 128 + 32 * kEpi;
 constexpr int kABytes = kBM * kBK, kBBytes = kHalf * kBK, kStageBytes = kABytes + kBBytes;
@@ -31,9 +32,9 @@ static_assert(128 * kRegsOther + 32 * kEpi * kRegsEpi <= kThreads * kRegsLaunch,
 
 struct Shared {  // behind the stages
   uint64_t full[kStages];    // used in the leader
-  uint64_t empty[kStages];   // one per CTA (multicast commit)
-  uint64_t tfull[2][2];      // [buffer][half] one per CTA: the MMAs' commit, the scales
-  uint64_t tempty[2][2];     // used in the leader: an arrival per epilogue warp of the half, of both CTAs
+  uint64_t empty[kStages];   // one per CTA, by the scales' warps
+  uint64_t tfull[2];         // one per CTA: the MMAs' commit, the scales
+  uint64_t tempty[2];        // used in the leader: an arrival per epilogue warp of both CTAs
   uint64_t done;             // behind a run-out: the MMAs under way
   uint32_t tmem;
   int dead;
@@ -41,7 +42,7 @@ struct Shared {  // behind the stages
   uint32_t largest[2][4][kBM];  // gated: magnitudes of two tiles' rows, by 32 features
 };
 constexpr size_t kSmem = 227 * 1024;  // all of it: nobody else is resident on an SM whose tensor memory this kernel has (fp8_gemm_few.cu)
-static_assert((size_t)kStages * kStageBytes + 1024 + sizeof(Shared) <= kSmem, "shared memory of a CTA");
+static_assert((size_t)kStages * kStageBytes + kEpi * kPieceBytes + 1024 + sizeof(Shared) <= kSmem, "shared memory of a CTA");
 
 // An arrival without a release: what it reports are reads of tensor memory, complete and fenced (tcgen05.wait::ld, fence::before_thread_sync); no memory is handed over.  A release at the
 // cluster's scope waits for the thread's loads in flight as well, 1500 to 2000 clocks for each block of K.
@@ -74,34 +75,18 @@ __device__ __forceinline__ float ld_shared_at(uint32_t addr) {
   asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
   return v;
 }
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* v) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]),
-        "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
-      : "r"(taddr));
-}
-__device__ __forceinline__ void tmem_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-// acc += v * s, behind the wait that it stands behind (volatile: nothing moves it in front of that)
-__device__ __forceinline__ void fma_at(float& acc, uint32_t v, float s) { asm volatile("fma.rn.f32 %0, %1, %2, %0;" : "+f"(acc) : "f"(__uint_as_float(v)), "f"(s)); }
 
-// 32 columns of a warp's 32 rows; the lanes store for one another, four lanes 64 bytes of a row at a time (a lane that stored its own row would touch a line per 16 bytes)
-__device__ __forceinline__ void store32(bf16* base, long ld, int tok, int N, int lane, const float* acc) {
-  uint32_t u[16];
+// 128 bytes of a row (lane = row) into the warp's piece, laid out as a tensor map with 128-byte swizzle has it
+__device__ __forceinline__ void put_row(uint32_t piece, int lane, const uint32_t* u) {
 #pragma unroll
-  for (int j = 0; j < 16; ++j) u[j] = pack_bf16(acc[2 * j], acc[2 * j + 1]);
-  transpose4(u, lane);
-  const int tok4 = tok & ~3;
-  bf16* dst = base + (size_t)tok4 * ld + (lane & 3) * 8;
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-    if (tok4 + j < N) *reinterpret_cast<uint4*>(dst + (size_t)j * ld) = make_uint4(u[4 * j], u[4 * j + 1], u[4 * j + 2], u[4 * j + 3]);
+  for (int c = 0; c < 8; ++c)
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(piece + (uint32_t)(lane * 128 + ((c ^ (lane & 7)) << 4))), "r"(u[4 * c]), "r"(u[4 * c + 1]), "r"(u[4 * c + 2]),
+                 "r"(u[4 * c + 3])
+                 : "memory");
 }
-__device__ __forceinline__ void store32(float* base, long ld, int tok, int N, int lane, const float* acc) {
-  if (tok >= N) return;
-  float4* dst = reinterpret_cast<float4*>(base + (size_t)tok * ld);
-#pragma unroll
-  for (int j = 0; j < 8; ++j) dst[j] = make_float4(acc[4 * j], acc[4 * j + 1], acc[4 * j + 2], acc[4 * j + 3]);
+__device__ __forceinline__ void store_piece(const CUtensorMap* map, uint32_t piece, int c0, int c1) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(c0), "r"(c1), "r"(piece) : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
 
 template <int ACT>
@@ -113,10 +98,12 @@ __device__ __forceinline__ void activate(const float* acc, float* v) {  // acc: 
 // GATED: O is the codes' type
 template <bool GATED, typename O>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
-fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_w2, const Product p) {
+fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_w2,
+                const __grid_constant__ CUtensorMap map_y, const Product p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  Shared& sh = *reinterpret_cast<Shared*>(smem + (size_t)kStages * kStageBytes);
+  uint8_t* pieces = smem + (size_t)kStages * kStageBytes;
+  Shared& sh = *reinterpret_cast<Shared*>(pieces + kEpi * kPieceBytes);
   volatile int* dead = &sh.dead;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -132,9 +119,9 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
       mbar_init(sh.full + s, 1);
       mbar_init(sh.empty + s, 1);
     }
-    for (int s = 0; s < 4; ++s) {
-      mbar_init(&sh.tfull[0][0] + s, 2);
-      mbar_init(&sh.tempty[0][0] + s, kEpi);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(sh.tfull + s, 2);
+      mbar_init(sh.tempty + s, 2 * kEpi);
     }
     mbar_init(&sh.done, 1);
     *dead = 0;
@@ -161,8 +148,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
         for (int tile = pair; tile < num_tiles && go; tile += num_pairs) {
           const int mb = tile % m_tiles, nb = tile / m_tiles;
           const int tok0 = mb * 2 * kBM + (int)rank * kBM;
-          // 64 rows of each half: a product's columns are the leader's 64 rows, then the peer's
-          const int row0 = GATED ? nb * kHalf : nb * kBN + (int)rank * 64, row1 = row0 + (GATED ? 64 : kHalf);
+          const int row0 = GATED ? nb * kHalf : nb * kBN + (int)rank * kHalf;
           for (int kb = 0; kb < kb_n; ++kb) {
             go = mbar_wait_bounded(sh.empty + s, ph, dead);
             if (!go) break;
@@ -171,7 +157,6 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
             uint8_t* st = smem + (size_t)s * kStageBytes;
             g2_tma_2d(st, &map_x, kb * kBK, tok0, fb);
             g2_tma_2d(st + kABytes, mw, kb * kBK, row0, fb);
-            g2_tma_2d(st + kABytes + kBBytes / 2, mw, kb * kBK, row1, fb);
             if (++s == kStages) {
               s = 0;
               ph ^= 1u;
@@ -182,16 +167,16 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
       }
     } else if (warp == 1) {
       if (leader && tc_elect_one()) {
-        constexpr uint32_t idesc = f8_idesc(2 * kBM, kHalf);
+        constexpr uint32_t idesc = f8_idesc(2 * kBM, kBN);
         int s = 0, buf = 0;
         uint32_t ph = 0, tph = 1;
         bool go = true;
         for (int tile = pair; tile < num_tiles && go; tile += num_pairs) {
           for (int kb = 0; kb < kb_n; ++kb) {
-            // three looks at once: a wait costs this thread 200 clocks where nothing is to be waited for, a block's MMAs take 512
-            const bool here = mbar_test_wait(sh.full + s, ph), free0 = mbar_test_wait(&sh.tempty[buf][0], tph), free1 = mbar_test_wait(&sh.tempty[buf][1], tph);
+            // two looks at once: a wait costs this thread 200 clocks where nothing is to be waited for, a block's MMAs take 443
+            const bool here = mbar_test_wait(sh.full + s, ph), free = mbar_test_wait(sh.tempty + buf, tph);
             if (!here) go = mbar_wait_bounded(sh.full + s, ph, dead);
-            if (go && !free0) go = mbar_wait_bounded(&sh.tempty[buf][0], tph, dead);
+            if (go && !free) go = mbar_wait_bounded(sh.tempty + buf, tph, dead);
             if (!go) break;
             tc_fence_after();
             const uint32_t a_addr = smem_u32(smem + (size_t)s * kStageBytes);
@@ -199,15 +184,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
             const uint32_t d = tmem_base + (uint32_t)(buf * kBN);
 #pragma unroll
             for (int k = 0; k < kBK / 32; ++k) umma_f8_pair(d, adesc + (uint64_t)(k * 2), bdesc + (uint64_t)(k * 2), idesc, k > 0 ? 1u : 0u);
-            g2_commit_both(&sh.tfull[buf][0]);
-            if (!free1) go = mbar_wait_bounded(&sh.tempty[buf][1], tph, dead);
-            if (!go) break;
-            tc_fence_after();
-#pragma unroll
-            for (int k = 0; k < kBK / 32; ++k)
-              umma_f8_pair(d + kHalf, adesc + (uint64_t)(k * 2), bdesc + (uint64_t)((kBBytes / 2 >> 4) + k * 2), idesc, k > 0 ? 1u : 0u);
-            g2_commit_both(&sh.tfull[buf][1]);
-            g2_commit_both(sh.empty + s);
+            g2_commit_both(sh.tfull + buf);
             if (++s == kStages) {
               s = 0;
               ph ^= 1u;
@@ -250,16 +227,15 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
       settle();
       fetch();
       uint32_t ph = 1;  // of tfull[mine]: before its first phase
+      int stage = -1;   // of block it - 2
       for (int slot = mine; tile < num_tiles; slot = (slot + 2) & 7) {
-        mbar_wait_bounded(&sh.tfull[mine][0], ph, dead);
-        mbar_wait_bounded(&sh.tfull[mine][1], ph, dead);
+        mbar_wait_bounded(sh.tfull + mine, ph, dead);
+        if (lane == 0 && stage >= 0) mbar_arrive(sh.empty + stage);  // (the MMAs of block it - 2 have read it)
+        stage = stage < 0 ? mine : stage + 2 < kStages ? stage + 2 : stage + 2 - kStages;
         reinterpret_cast<float4*>(sh.scale[slot][0])[lane] = make_float4(x.x * a, x.y * a, x.z * a, x.w * a);
         reinterpret_cast<float4*>(sh.scale[slot][1])[lane] = make_float4(x.x * b, x.y * b, x.z * b, x.w * b);
         __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&sh.tfull[mine][0]);
-          mbar_arrive(&sh.tfull[mine][1]);
-        }
+        if (lane == 0) mbar_arrive(sh.tfull + mine);
         ph ^= 1u;
         kb += 2;
         settle();
@@ -268,12 +244,13 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsEpi));
-    const int q = warp & 3, part = (warp - 4) >> 2, half = part >> 1, sub = part & 1, row = q * 32 + lane;
-    const uint32_t tempty = g2_map(smem_u32(&sh.tempty[0][half]), 0), tfull = smem_u32(&sh.tfull[0][half]);
-    const uint32_t scales = smem_u32(&sh.scale[0][GATED ? 0 : half][row]);
+    const int q = warp & 3, part = (warp - 4) >> 2, row = q * 32 + lane;
+    const uint32_t tempty = g2_map(smem_u32(sh.tempty), 0), tfull = smem_u32(sh.tfull);
+    const uint32_t scales = smem_u32(&sh.scale[0][GATED ? 0 : part >> 1][row]);
     // the thread's two pieces of 32 columns; gated: 32 of the gate, then the same 32 of the factor
-    const uint32_t t_row = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(half * kHalf + sub * (GATED ? 32 : 64));
-    constexpr uint32_t kPiece = GATED ? 64 : 32;
+    const uint32_t t_row = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(part * (GATED ? 32 : 64));
+    constexpr uint32_t kPiece = GATED ? kHalf : 32;
+    const uint32_t piece = smem_u32(pieces) + (uint32_t)((warp - 4) * kPieceBytes);
     uint32_t it = 0, lt = 0;  // blocks of K so far, tiles
     bool ready = false;
     for (int tile = pair; tile < num_tiles; tile += num_pairs, ++lt) {
@@ -283,31 +260,28 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
 #pragma unroll 1
       for (int kb = kb_n; kb > 0; --kb) {
         const uint32_t buf = it & 1;
-        if (!ready) mbar_wait_bounded(&sh.tfull[buf][half], (it >> 1) & 1, dead);
+        if (!ready) mbar_wait_bounded(sh.tfull + buf, (it >> 1) & 1, dead);
         tc_fence_after();
         const uint32_t t0 = t_row + buf * kBN;
-        uint32_t v[2][16];
-        tmem_ld16(t0, v[0]);
+        uint32_t v[32];
+        tmem_ld32_nowait(t0, v);
         const float s1 = ld_shared_at(scales + (it & 7) * (uint32_t)sizeof(sh.scale[0])), s2 = GATED ? ld_shared_at(scales + (it & 7) * (uint32_t)sizeof(sh.scale[0]) + kBM * 4) : s1;
         ++it;
+        tmem_wait32(v);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          tmem_wait();
-          if (c < 3) {
-            tmem_ld16(t0 + (c + 1 < 2 ? 16 : kPiece + (c - 1) * 16), v[(c + 1) & 1]);
-          } else {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) arrive_relaxed(tempty + buf * (uint32_t)sizeof(sh.tempty[0]));
-          }
-          if (c == 2) ready = test_wait_at(tfull + (it & 1) * (uint32_t)sizeof(sh.tfull[0]), (it >> 1) & 1);  // (asked for early)
+        for (int j = 0; j < 32; ++j) acc[j] = fmaf(__uint_as_float(v[j]), s1, acc[j]);
+        tmem_ld32_nowait(t0 + kPiece, v);
+        ready = test_wait_at(tfull + (it & 1) * 8u, (it >> 1) & 1);  // (asked for early)
+        tmem_wait32(v);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) arrive_relaxed(tempty + buf * 8u);
 #pragma unroll
-          for (int j = 0; j < 16; ++j) fma_at(acc[16 * c + j], v[c & 1][j], c < 2 ? s1 : s2);
-        }
+        for (int j = 0; j < 32; ++j) acc[32 + j] = fmaf(__uint_as_float(v[j]), s2, acc[32 + j]);
       }
       const int mb = tile % m_tiles, nb = tile / m_tiles;
       const int tok = mb * 2 * kBM + (int)rank * kBM + row;
-      const int f0 = GATED ? nb * kHalf + half * 64 + sub * 32 : nb * kBN + half * kHalf + sub * 64;  // the thread's first feature
+      const int f0 = GATED ? nb * kHalf + part * 32 : nb * kBN + part * 64;  // the thread's first feature
       if constexpr (GATED) {
         float v[32];
         if (p.act == 0) activate<0>(acc, v);
@@ -339,20 +313,29 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
         }
       } else {
         O* y = static_cast<O*>(p.y);
-        const bool vec = (p.ld_y * (long)sizeof(O)) % 16 == 0 && (reinterpret_cast<uintptr_t>(y) & 15) == 0;
+        const int tok0 = tok - lane;
+        if (p.y_map) {
+          constexpr int kCols = 128 / (int)sizeof(O);
 #pragma unroll
-        for (int c = 0; c < 64; c += 32) {
-          if (tok - lane >= N || f0 + c >= M) continue;  // (a warp at a time: the lanes store for one another)
-          if (vec && f0 + c + 32 <= M) {
-            store32(y + f0 + c, p.ld_y, tok, N, lane, acc + c);
-          } else if (tok < N) {
+          for (int c = 0; c < 64; c += kCols) {
+            if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the piece before
+            __syncwarp();
+            uint32_t u[32];
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (f0 + c + j < M) y[(size_t)tok * p.ld_y + f0 + c + j] = from_f<O>(acc[c + j]);
+            for (int j = 0; j < 32; ++j) u[j] = sizeof(O) == 4 ? __float_as_uint(acc[c + j]) : pack_bf16(acc[2 * j], acc[2 * j + 1]);
+            put_row(piece, lane, u);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0 && tok0 < N && f0 + c < M) store_piece(&map_y, piece, f0 + c, tok0);
           }
+        } else if (tok < N) {
+#pragma unroll
+          for (int j = 0; j < 64; ++j)
+            if (f0 + j < M) y[(size_t)tok * p.ld_y + f0 + j] = from_f<O>(acc[j]);
         }
       }
     }
+    if (!GATED && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
   tc_fence_before();
   __syncthreads();
@@ -362,6 +345,19 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
     g2_tmem_dealloc(tmem_base, 2 * kBN);
   }
   if (threadIdx.x == 0) count_run_out(dead, p.err);
+}
+
+// rows x M of the output in pieces of 32 rows x 128 bytes; false: its rows do not start on 16-byte boundaries
+template <typename O>
+bool make_out_map(CUtensorMap* map, void* y, int rows, int M, long ld) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn || !al16(y) || ld * (long)sizeof(O) % 16 != 0 || ld * (long)sizeof(O) >= 1L << 40) return false;
+  cuuint64_t dims[2] = {(cuuint64_t)M, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)ld * sizeof(O)};
+  cuuint32_t box[2] = {128 / sizeof(O), 32};
+  cuuint32_t estr[2] = {1, 1};
+  return fn(map, sizeof(O) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, y, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <bool GATED, typename O>
@@ -375,10 +371,11 @@ int launch_pair(const Product& product, cudaStream_t st) {
   auto kern = fp8_gemm_kernel<GATED, O>;
   static std::atomic<uint64_t> set{0};
   if (const cudaError_t e = allow_smem(set, (const void*)kern, kSmem); e != cudaSuccess) return (int)e;
-  CUtensorMap mx, mw, mw2;
-  if (!make_codes_map(&mx, p.x, p.N, p.K, p.ld_x, kBM) || !make_codes_map(&mw, p.w, p.M, p.K, p.ld_w, 64) || !make_codes_map(&mw2, GATED ? p.w2 : p.w, p.M, p.K, p.ld_w, 64))
+  CUtensorMap mx, mw, mw2, my{};
+  if (!make_codes_map(&mx, p.x, p.N, p.K, p.ld_x, kBM) || !make_codes_map(&mw, p.w, p.M, p.K, p.ld_w, kHalf) || !make_codes_map(&mw2, GATED ? p.w2 : p.w, p.M, p.K, p.ld_w, kHalf))
     return (int)cudaErrorInvalidValue;
-  return (int)launch(kern, dim3(2 * pairs), dim3(kThreads), kSmem, st, true, mx, mw, mw2, p);
+  if constexpr (!GATED) p.y_map = make_out_map<O>(&my, p.y, p.N, p.M, p.ld_y);
+  return (int)launch(kern, dim3(2 * pairs), dim3(kThreads), kSmem, st, true, mx, mw, mw2, my, p);
 }
 
 }  // namespace

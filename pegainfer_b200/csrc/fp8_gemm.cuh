@@ -24,6 +24,7 @@ struct Product {
   long ld_w, ld_x, ld_sx;
   void* y;                  // [N][ld_y], bf16 or float
   long ld_y;
+  bool y_map;               // fp8_gemm.cu: the output goes by tensor map
   uint8_t* codes;           // gated: the activated rows [N][ld], their scales [blocks of M][ld_s]
   float* scales;
   long ld, ld_s;
