@@ -30,6 +30,8 @@ constexpr int kABytes = kBM * kBK, kBBytes = kHalf * kBK, kStageBytes = kABytes 
 constexpr int kRegsLaunch = 96, kRegsOther = 32, kRegsEpi = 112;
 static_assert(128 * kRegsOther + 32 * kEpi * kRegsEpi <= kThreads * kRegsLaunch, "what the block was launched with");
 
+constexpr int kLooks = 512;  // at a barrier before its wait proper, which wakes up 50 to 100 clocks later
+
 struct Shared {  // behind the stages
   uint64_t full[kStages];    // used in the leader
   uint64_t empty[kStages];   // one per CTA, by the scales' warps
@@ -174,14 +176,17 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
         for (int tile = pair; tile < num_tiles && go; tile += num_pairs) {
           for (int kb = 0; kb < kb_n; ++kb) {
             // two looks at once: a wait costs this thread 200 clocks where nothing is to be waited for, a block's MMAs take 443
-            const bool here = mbar_test_wait(sh.full + s, ph), free = mbar_test_wait(sh.tempty + buf, tph);
+            const bool here = mbar_test_wait(sh.full + s, ph);
+            bool free = mbar_test_wait(sh.tempty + buf, tph);
             if (!here) go = mbar_wait_bounded(sh.full + s, ph, dead);
-            if (go && !free) go = mbar_wait_bounded(sh.tempty + buf, tph, dead);
             if (!go) break;
-            tc_fence_after();
             const uint32_t a_addr = smem_u32(smem + (size_t)s * kStageBytes);
             const uint64_t adesc = make_sw128_desc(a_addr), bdesc = make_sw128_desc(a_addr + kABytes);
             const uint32_t d = tmem_base + (uint32_t)(buf * kBN);
+            for (int i = 0; !free && i < kLooks; ++i) free = mbar_test_wait(sh.tempty + buf, tph);
+            if (!free) go = mbar_wait_bounded(sh.tempty + buf, tph, dead);
+            if (!go) break;
+            tc_fence_after();
 #pragma unroll
             for (int k = 0; k < kBK / 32; ++k) umma_f8_pair(d, adesc + (uint64_t)(k * 2), bdesc + (uint64_t)(k * 2), idesc, k > 0 ? 1u : 0u);
             g2_commit_both(sh.tfull + buf);
@@ -260,6 +265,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
 #pragma unroll 1
       for (int kb = kb_n; kb > 0; --kb) {
         const uint32_t buf = it & 1;
+        for (int i = 0; !ready && i < kLooks; ++i) ready = test_wait_at(tfull + buf * 8u, (it >> 1) & 1);
         if (!ready) mbar_wait_bounded(sh.tfull + buf, (it >> 1) & 1, dead);
         tc_fence_after();
         const uint32_t t0 = t_row + buf * kBN;
