@@ -58,12 +58,13 @@ constexpr int tmem_columns(int na, int nt) { return 2 * na * nt <= 32 ? 32 : 2 *
 
 // NA tiles of A
 template <int NT, int NA, typename O>
-__global__ void __launch_bounds__(64 + 128 * NA)
+__global__ void __launch_bounds__(64 + 128 * NA, 2)
 fp8_gemm_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_w2, const Product p,
                     const FewPlan plan) {
   constexpr int THREADS = 64 + 128 * NA;
   constexpr uint32_t TMEM_COLS = tmem_columns(NA, NT);
   static_assert(2 * NA * NT <= 256, "two CTAs on an SM");
+  constexpr bool ROOM = NA * NT < 128;  // registers for 16 columns on their way beside those at work
   const int stages = plan.stages, rows = plan.rows;
   const uint32_t A_BYTES = rows * kBK, STAGE = NA * A_BYTES + NT * kBK;
   extern __shared__ uint8_t smem_raw[];
@@ -85,7 +86,7 @@ fp8_gemm_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
   if (threadIdx.x == 0) {
     for (int s = 0; s < stages; ++s) {
       mbar_init(full + s, 1);
-      mbar_init(empty + s, 1 + 4 * NA);  // the MMAs' commit, the warps that read the scales
+      mbar_init(empty + s, 4 * NA);  // the warps that read the scales, behind the MMAs' end
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(tfull + s, 1);
@@ -132,7 +133,11 @@ fp8_gemm_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       uint32_t ph = 0;
       for (; i < nk; ++i) {
         const int buf = i & 1;
-        if (!mbar_wait_bounded(tempty + buf, (uint32_t)(((i >> 1) & 1) ^ 1), dead) || !mbar_wait_bounded(full + s, ph, dead)) break;
+        const uint32_t tph = (uint32_t)(((i >> 1) & 1) ^ 1);
+        // two looks at once: a wait costs a thread 200 clocks where nothing is to be waited for
+        const bool here = mbar_test_wait(full + s, ph), free = mbar_test_wait(tempty + buf, tph);
+        if (!here && !mbar_wait_bounded(full + s, ph, dead)) break;
+        if (!free && !mbar_wait_bounded(tempty + buf, tph, dead)) break;
         tc_fence_after();
         const uint32_t a_addr = smem_u32(smem + (size_t)s * STAGE);
         const uint64_t bdesc = make_sw128_desc(a_addr + NA * A_BYTES);
@@ -143,7 +148,6 @@ fp8_gemm_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
           for (int k = 0; k < kBK / 32; ++k)
             umma_f8(tmem_base + (uint32_t)((buf * NA + h) * NT), adesc + (uint64_t)(k * 2), bdesc + (uint64_t)(k * 2), idesc, k > 0 ? 1u : 0u);
         }
-        umma_commit(empty + s);
         umma_commit(tfull + buf);
         if (++s == stages) {
           s = 0;
@@ -170,25 +174,50 @@ fp8_gemm_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       const int buf = i & 1;
       const uint64_t w = pair_of(w_next, w_next);
       if (i + 1 < nk) w_next = __ldg(sw + i + 1);
-      mbar_wait_bounded(full + s, ph, dead);  // (the scales)
-      mbar_wait_bounded(tfull + buf, (uint32_t)((i >> 1) & 1), dead);
+      const uint32_t tph = (uint32_t)((i >> 1) & 1);
+      const bool here = mbar_test_wait(full + s, ph), done = mbar_test_wait(tfull + buf, tph);
+      if (!here) mbar_wait_bounded(full + s, ph, dead);  // (the scales)
+      if (!done) mbar_wait_bounded(tfull + buf, tph, dead);
       tc_fence_after();
-#pragma unroll
-      for (int c = 0; c < NT; c += 16) {
-        uint32_t v[16];
-        tmem_ld16_wait(tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)((buf * NA + h) * NT + c), v);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float4 x = *reinterpret_cast<const float4*>(xs + s * NT + c + 4 * j);
-          fma2(acc[c / 2 + 2 * j], pair_of(v[4 * j], v[4 * j + 1]), mul2(w, pair_of(x.x, x.y)));
-          fma2(acc[c / 2 + 2 * j + 1], pair_of(v[4 * j + 2], v[4 * j + 3]), mul2(w, pair_of(x.z, x.w)));
+      const uint32_t t0 = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)((buf * NA + h) * NT);
+      auto release = [&]() {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(tempty + buf);
+          mbar_arrive(empty + s);
         }
-      }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(tempty + buf);
-        mbar_arrive(empty + s);
+      };
+      auto add4 = [&](int at, const uint32_t* u, float4 x) {
+        fma2(acc[at / 2], pair_of(u[0], u[1]), mul2(w, pair_of(x.x, x.y)));
+        fma2(acc[at / 2 + 1], pair_of(u[2], u[3]), mul2(w, pair_of(x.z, x.w)));
+      };
+      auto scale4 = [&](int at) { return *reinterpret_cast<const float4*>(xs + s * NT + at); };
+      if constexpr (ROOM) {
+        uint32_t v[2][16];
+        tmem_ld16(t0, v[0]);
+#pragma unroll
+        for (int c = 0; c < NT; c += 16) {
+          float4 x[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x[j] = scale4(c + 4 * j);
+          uint32_t* now = v[(c / 16) & 1];
+          tmem_wait16(now);
+          if (c + 16 < NT) tmem_ld16(t0 + (uint32_t)(c + 16), v[(c / 16 + 1) & 1]);
+          else release();
+#pragma unroll
+          for (int j = 0; j < 4; ++j) add4(c + 4 * j, now + 4 * j, x[j]);
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < NT; c += 16) {
+          uint32_t v[16];
+          tmem_ld16(t0 + (uint32_t)c, v);
+          tmem_wait16(v);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) add4(c + 4 * j, v + 4 * j, scale4(c + 4 * j));
+        }
+        release();
       }
       if (++s == stages) {
         s = 0;
