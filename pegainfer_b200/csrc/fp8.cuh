@@ -20,45 +20,74 @@ __host__ __device__ inline int blocks_of(int n) { return (int)(((long)n + kBlock
 inline bool codes_ok(const void* codes, long ld, int width) { return codes && al16(codes) && ld % 16 == 0 && ld >= width && ld < 1L << 39; }
 inline bool row_scales_ok(const float* scales, long ld_s, int tokens) { return scales && al16(scales) && ld_s % 4 == 0 && ld_s >= tokens; }
 
-__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }  // as bits: a maximum of those keeps infinities and NaN
+// two fp32 numbers to an instruction
+__device__ __forceinline__ uint64_t pair_of(uint32_t lo, uint32_t hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
+  return r;
+}
+__device__ __forceinline__ uint64_t pair_of(float lo, float hi) { return pair_of(__float_as_uint(lo), __float_as_uint(hi)); }
+__device__ __forceinline__ float lo_of(uint64_t v) { return __uint_as_float((uint32_t)v); }
+__device__ __forceinline__ float hi_of(uint64_t v) { return __uint_as_float((uint32_t)(v >> 32)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// the largest magnitude; infinities and NaN stay
+__device__ __forceinline__ float max_abs(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(fabsf(a)), "f"(fabsf(b)));
+  return r;
+}
+__device__ __forceinline__ float max_abs(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(fabsf(a)), "f"(fabsf(b)), "f"(fabsf(c)));
+  return r;
+}
+__device__ __forceinline__ float max8(const float* v) {
+  return max_abs(max_abs(v[0], v[1], v[2]), max_abs(v[3], v[4], v[5]), max_abs(v[6], v[7]));
+}
+// the largest of 16 lanes, which have a block together
+__device__ __forceinline__ float max16(float m) {
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) m = max_abs(m, __shfl_xor_sync(0xffffffffu, m, o));
+  return m;
+}
 
 struct Scale {
   float s, inv;  // NaN where the block has an entry that is not finite
 };
-__device__ __forceinline__ Scale scale_of(uint32_t amax) {
+// amax / 448 to its nearest fp32 number: a product and a step of Newton's, whose remainder is exact
+__device__ __forceinline__ Scale scale_of(float amax) {
+  constexpr float kTo = 1.f / 448.f;
+  const float a = amax < 7.888609e-31f ? 7.888609e-31f : amax - (amax - amax);  // (an infinity becomes NaN)
+  const float s = a * kTo;
   Scale r;
-  r.s = amax >= 0x7f800000u ? __uint_as_float(0x7fffffffu) : fmaxf(__uint_as_float(amax), 7.888609e-31f) / 448.f;
-  r.inv = 1.f / r.s;
+  r.s = fmaf(fmaf(-s, 448.f, a), kTo, s);
+  asm("rcp.approx.f32 %0, %1;" : "=f"(r.inv) : "f"(r.s));
   return r;
 }
-// v / s to its nearest fp32 number: v * (1 / s) and a step of Newton's, whose remainder v - q s is exact.  Without it a quotient that lies just between two codes,
+// codes of v / s, each quotient to its nearest fp32 number: v * (1 / s) and the same step, whose remainder v - q s is exact.  Without it a quotient that lies just between two codes,
 // as bf16 entries have them often, went to either.
-__device__ __forceinline__ float quotient(float v, Scale k) {
-  const float q = v * k.inv;
-  return fmaf(fmaf(-q, k.s, v), k.inv, q);
-}
-__device__ __forceinline__ uint32_t codes2(float lo, float hi) {
+__device__ __forceinline__ uint32_t codes2(float lo, float hi, Scale k) {
+  const uint64_t v = pair_of(lo, hi), inv = pair_of(k.inv, k.inv), s = pair_of(-k.s, -k.s);
+  uint64_t q = mul2(v, inv);
+  q = fma2(fma2(q, s, v), inv, q);
   uint16_t r;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi_of(q)), "f"(lo_of(q)));
   return r;
 }
-__device__ __forceinline__ uint32_t codes4(const float* v, Scale k) {
-  return codes2(quotient(v[0], k), quotient(v[1], k)) | codes2(quotient(v[2], k), quotient(v[3], k)) << 16;
-}
-// the largest of 16 lanes, which have a block together
-__device__ __forceinline__ uint32_t max16(uint32_t m) {
-#pragma unroll
-  for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-  return m;
-}
-__device__ __forceinline__ uint32_t max8(const float* v) {
-  uint32_t m = magnitude(v[0]);
-#pragma unroll
-  for (int e = 1; e < 8; ++e) m = max(m, magnitude(v[e]));
-  return m;
-}
+__device__ __forceinline__ uint32_t codes4(const float* v, Scale k) { return codes2(v[0], v[1], k) | codes2(v[2], v[3], k) << 16; }
 
-// 8 entries from p on, of which the first n exist (the others are zero); VEC: n is 0 or 8 and p on a 16-byte boundary
+// 8 entries from p on, of which the first n exist (the others are zero).  VEC: n is at most 0 or at least 8 and p on a 16-byte boundary (a choice between the two forms here, by n, would keep
+// the loads of a loop from being under way together)
 template <bool VEC>
 __device__ __forceinline__ void load8(const bf16* p, int n, float* v) {
   if constexpr (VEC) {

@@ -41,7 +41,7 @@ struct Shared {  // behind the stages
   uint32_t tmem;
   int dead;
   float scale[8][2][kBM];    // of eight blocks of K: of the first half and the second; gated: of w and w2
-  uint32_t largest[2][4][kBM];  // gated: magnitudes of two tiles' rows, by 32 features
+  float largest[2][4][kBM];  // gated: magnitudes of two tiles' rows, by 32 features
 };
 constexpr size_t kSmem = 227 * 1024;  // all of it: nobody else is resident on an SM whose tensor memory this kernel has (fp8_gemm_few.cu)
 static_assert((size_t)kStages * kStageBytes + kEpi * kPieceBytes + 1024 + sizeof(Shared) <= kSmem, "shared memory of a CTA");
@@ -293,13 +293,13 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
         if (p.act == 0) activate<0>(acc, v);
         else if (p.act == 1) activate<1>(acc, v);
         else activate<2>(acc, v);
-        uint32_t m = 0;
+        float m = max_abs(v[0], v[1]);
 #pragma unroll
-        for (int j = 0; j < 32; ++j) m = max(m, magnitude(v[j]));
-        uint32_t(*mine)[kBM] = sh.largest[lt & 1];  // (the other tile's are read until the barrier behind this one)
+        for (int j = 2; j < 32; j += 2) m = max_abs(m, v[j], v[j + 1]);
+        float(*mine)[kBM] = sh.largest[lt & 1];  // (the other tile's are read until the barrier behind this one)
         mine[part][row] = m;
         asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpi) : "memory");
-        const Scale k = scale_of(max(max(mine[0][row], mine[1][row]), max(mine[2][row], mine[3][row])));
+        const Scale k = scale_of(max_abs(max_abs(mine[0][row], mine[1][row], mine[2][row]), mine[3][row]));
         if (tok < N && f0 < M) {
           uint8_t* dst = p.codes + (size_t)tok * p.ld + f0;
 #pragma unroll

@@ -189,8 +189,8 @@ fp8_gemm_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
         }
       };
       auto add4 = [&](int at, const uint32_t* u, float4 x) {
-        fma2(acc[at / 2], pair_of(u[0], u[1]), mul2(w, pair_of(x.x, x.y)));
-        fma2(acc[at / 2 + 1], pair_of(u[2], u[3]), mul2(w, pair_of(x.z, x.w)));
+        acc[at / 2] = fma2(pair_of(u[0], u[1]), mul2(w, pair_of(x.x, x.y)), acc[at / 2]);
+        acc[at / 2 + 1] = fma2(pair_of(u[2], u[3]), mul2(w, pair_of(x.z, x.w)), acc[at / 2 + 1]);
       };
       auto scale4 = [&](int at) { return *reinterpret_cast<const float4*>(xs + s * NT + at); };
       if constexpr (ROOM) {
@@ -281,8 +281,8 @@ fp8_gemm_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       const float w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
       for (int j = 0; j < 4; ++j) v[j] = (p.act == 0 ? gate_act<0>(v[j]) : p.act == 1 ? gate_act<1>(v[j]) : gate_act<2>(v[j])) * w[j];
-      const uint32_t m = max(max(magnitude(v[0]), magnitude(v[1])), max(magnitude(v[2]), magnitude(v[3])));
-      const Scale k = scale_of(__reduce_max_sync(0xffffffffu, m));
+      const float m = max16(max_abs(max_abs(v[0], v[1], v[2]), v[3]));
+      const Scale k = scale_of(max_abs(m, __shfl_xor_sync(0xffffffffu, m, 16)));
       const uint32_t c = codes4(v, k);
       const int f = m0 + lane * 4;
       uint8_t* dst = p.codes + (size_t)(t0 + t) * p.ld + f;

@@ -5,33 +5,33 @@
 namespace pk {
 namespace fp8 {
 
-// x += y (rounded when stored), v = x * rsqrt(mean(x^2) + eps) * (offset + w) of the unrounded x, quantised.  A CTA has a row, in registers from its load to its codes.
-constexpr int kNormThreads = 256;
-constexpr int kNormWidest = kNormThreads * 8 * 8;
+// x += y (rounded when stored), v = x * rsqrt(mean(x^2) + eps) * (offset + w) of the unrounded x, quantised.  A CTA has a row, in registers from its load to its codes, NV pieces of 8
+// entries a thread and as many warps as that takes.
+constexpr int kNormWarps = 32, kNormWidest = kNormWarps * 256 * 2;
 
 template <typename E, int NV, bool VEC>
-__global__ void __launch_bounds__(kNormThreads) fp8_add_norm_kernel(const bf16* __restrict__ y, E* __restrict__ x, const bf16* __restrict__ w, float offset,
-                                                                    uint8_t* __restrict__ codes, long ld, float* __restrict__ scales, long ld_s, int width, float eps) {
-  __shared__ float red[kNormThreads / 32];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const size_t base = (size_t)blockIdx.x * width;
+__global__ void __launch_bounds__(32 * kNormWarps) fp8_add_norm_kernel(const bf16* __restrict__ y, E* __restrict__ x, const bf16* __restrict__ w, float offset,
+                                                                      uint8_t* __restrict__ codes, long ld, float* __restrict__ scales, long ld_s, int width, float eps) {
+  __shared__ float red[kNormWarps];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  const size_t t = blockIdx.x, base = t * width;
   pdl_wait();
   float v[NV][8];
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    const int at = (j * kNormThreads + threadIdx.x) * 8;
+    const int at = (j * blockDim.x + threadIdx.x) * 8;
     load8<VEC>(x + base + at, width - at, v[j]);
   }
   if (y) {
     float add[NV][8];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int at = (j * kNormThreads + threadIdx.x) * 8;
+      const int at = (j * blockDim.x + threadIdx.x) * 8;
       load8<VEC>(y + base + at, width - at, add[j]);
     }
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int at = (j * kNormThreads + threadIdx.x) * 8;
+      const int at = (j * blockDim.x + threadIdx.x) * 8;
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[j][e] += add[j][e];
       store8<VEC>(x + base + at, width - at, v[j]);
@@ -43,15 +43,15 @@ __global__ void __launch_bounds__(kNormThreads) fp8_add_norm_kernel(const bf16* 
 #pragma unroll
     for (int e = 0; e < 8; ++e) ss = fmaf(v[j][e], v[j][e], ss);
   ss = warp_sum(ss);
-  if (lane == 0) red[warp] = ss;
-  __syncthreads();
-  ss = 0.f;
-#pragma unroll
-  for (int i = 0; i < kNormThreads / 32; ++i) ss += red[i];
+  if (warps > 1) {
+    if (lane == 0) red[warp] = ss;
+    __syncthreads();
+    ss = warp_sum(lane < warps ? red[lane] : 0.f);
+  }
   const float r = 1.f / sqrtf(ss / (float)width + eps);
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    const int at = (j * kNormThreads + threadIdx.x) * 8;
+    const int at = (j * blockDim.x + threadIdx.x) * 8;
     if (at - (at & 255) >= width) break;  // (a warp at a time: its lanes find a maximum together)
     float g[8];
     load8<VEC>(w + at, width - at, g);
@@ -59,62 +59,70 @@ __global__ void __launch_bounds__(kNormThreads) fp8_add_norm_kernel(const bf16* 
     for (int e = 0; e < 8; ++e) v[j][e] = at + e < width ? v[j][e] * r * (offset + g[e]) : 0.f;  // (an r that is not finite stays inside the row)
     const Scale k = scale_of(max16(max8(v[j])));
     if (at < width) {
-      store_codes8(codes + (size_t)blockIdx.x * ld + at, width - at, v[j], k);
-      if ((lane & 15) == 0) scales[(size_t)(at / kBlock) * ld_s + blockIdx.x] = k.s;
+      store_codes8(codes + t * ld + at, width - at, v[j], k);
+      if ((lane & 15) == 0) scales[(size_t)(at / kBlock) * ld_s + t] = k.s;
     }
   }
 }
 
 // KIND 0: silu(a) * b, 1: relu(a)^2, 2: relu(a) * b, 3: gelu(a) * b, 4: a, with a = in[t][f], b = in[t][F + f].  16 lanes have a block of a token.
-constexpr int kActThreads = 256;
+constexpr int kActThreads = 128, kActRows = 2;
 
 template <int KIND, bool VEC>
 __global__ void __launch_bounds__(kActThreads) fp8_act_kernel(const bf16* __restrict__ in, long ld_in, uint8_t* __restrict__ codes, long ld, float* __restrict__ scales,
-                                                              long ld_s, int F, int nb, long items) {
+                                                              long ld_s, int F, int nb, long items, int tokens) {
   const long item = ((long)blockIdx.x * kActThreads + threadIdx.x) >> 4;
-  const long t = item / nb;
-  const int b = (int)(item - t * nb), at = b * kBlock + (threadIdx.x & 15) * 8;
+  const long group = item / nb;
+  const int b = (int)(item - group * nb), at = b * kBlock + (threadIdx.x & 15) * 8, t0 = (int)(group * kActRows);
   pdl_wait();
-  const int n = item < items ? F - at : 0;
-  float v[8];
-  const bf16* row = in + (size_t)(item < items ? t : 0) * ld_in + at;
-  load8<VEC>(row, n, v);
-  if constexpr (KIND == 1) {
+  float v[kActRows][8], u[kActRows][8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float u = v[e] < 0.f ? 0.f : v[e];
-      v[e] = u * u;
-    }
-  } else if constexpr (KIND != 4) {
-    float u[8];
-    load8<VEC>(row + F, n, u);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = gate_act<KIND == 0 ? 0 : KIND - 1>(v[e]) * u[e];
+  for (int r = 0; r < kActRows; ++r) {
+    const int n = item < items && t0 + r < tokens ? F - at : 0;
+    const bf16* row = in + (size_t)(n > 0 ? t0 + r : 0) * ld_in + at;
+    load8<VEC>(row, n, v[r]);
+    if constexpr (KIND != 1 && KIND != 4) load8<VEC>(row + F, n, u[r]);
   }
-  const Scale k = scale_of(max16(max8(v)));
-  if (n > 0) {
-    store_codes8(codes + (size_t)t * ld + at, n, v, k);
-    if ((threadIdx.x & 15) == 0) scales[(size_t)b * ld_s + t] = k.s;
+#pragma unroll
+  for (int r = 0; r < kActRows; ++r) {
+    const int n = item < items && t0 + r < tokens ? F - at : 0;
+    if constexpr (KIND == 1) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float z = v[r][e] < 0.f ? 0.f : v[r][e];
+        v[r][e] = z * z;
+      }
+    } else if constexpr (KIND != 4) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[r][e] = gate_act<KIND == 0 ? 0 : KIND - 1>(v[r][e]) * u[r][e];
+    }
+    const Scale k = scale_of(max16(max8(v[r])));
+    if (n > 0) {
+      store_codes8(codes + (size_t)(t0 + r) * ld + at, n, v[r], k);
+      if ((threadIdx.x & 15) == 0) scales[(size_t)b * ld_s + t0 + r] = k.s;
+    }
   }
 }
 
 template <typename E, bool VEC>
 cudaError_t add_norm(const bf16* y, E* x, const bf16* w, float offset, uint8_t* codes, long ld, float* scales, long ld_s, int width, int tokens, float eps, cudaStream_t st) {
-  auto go = [&](auto kern) { return launch(kern, dim3(tokens), dim3(kNormThreads), 0, st, true, y, x, w, offset, codes, ld, scales, ld_s, width, eps); };
-  const int nv = (width + kNormThreads * 8 - 1) / (kNormThreads * 8);
-  if (nv <= 1) return go(fp8_add_norm_kernel<E, 1, VEC>);
-  if (nv <= 2) return go(fp8_add_norm_kernel<E, 2, VEC>);
-  if (nv <= 4) return go(fp8_add_norm_kernel<E, 4, VEC>);
-  return go(fp8_add_norm_kernel<E, 8, VEC>);
+  auto go = [&](auto kern, int nv) {
+    const int warps = (width + 256 * nv - 1) / (256 * nv);
+    return launch(kern, dim3(tokens), dim3(32 * warps), 0, st, true, y, x, w, offset, codes, ld, scales, ld_s, width, eps);
+  };
+  // B200, us, one piece a thread : two, x bf16: 8 x 2560 2.3 : 2.8, 512 x 2560 4.0 : 4.3, 1024 x 2560 7.2 : 6.2, 3001 x 2560 14.6 : 13.5, 4096 x 4096 28.6 : 25.2;
+  // x float: 512 x 2560 5.1 : 5.9, 3001 x 2560 15.6 : 18.4, 4096 x 4096 30.8 : 34.7, 2048 x 8192 34.1 : 35.5
+  if (width <= kNormWarps * 256 && (sizeof(E) == 4 || tokens < 5 * sm_count())) return go(fp8_add_norm_kernel<E, 1, VEC>, 1);
+  return go(fp8_add_norm_kernel<E, 2, VEC>, 2);
 }
 
 template <int KIND>
 cudaError_t act(const bf16* in, long ld_in, uint8_t* codes, long ld, float* scales, long ld_s, int F, int tokens, bool vec, cudaStream_t st) {
   const int nb = blocks_of(F);
-  const long items = (long)tokens * nb;
+  const long items = ((long)tokens + kActRows - 1) / kActRows * nb;
   const dim3 grid((unsigned)((items + kActThreads / 16 - 1) / (kActThreads / 16)));
-  if (vec) return launch(fp8_act_kernel<KIND, true>, grid, dim3(kActThreads), 0, st, true, in, ld_in, codes, ld, scales, ld_s, F, nb, items);
-  return launch(fp8_act_kernel<KIND, false>, grid, dim3(kActThreads), 0, st, true, in, ld_in, codes, ld, scales, ld_s, F, nb, items);
+  if (vec) return launch(fp8_act_kernel<KIND, true>, grid, dim3(kActThreads), 0, st, true, in, ld_in, codes, ld, scales, ld_s, F, nb, items, tokens);
+  return launch(fp8_act_kernel<KIND, false>, grid, dim3(kActThreads), 0, st, true, in, ld_in, codes, ld, scales, ld_s, F, nb, items, tokens);
 }
 
 }  // namespace fp8
@@ -144,7 +152,7 @@ extern "C" int pk_fp8_act(const void* in, long ld_in, int kind, void* codes, lon
     return -1;
   const long from = ld_in ? ld_in : need;
   if (F > 1 << 30 || (long)tokens * fp8::blocks_of(F) > 1L << 34) return -2;  // (the grid's CTAs are counted in 31 bits)
-  const bool vec = F % 8 == 0 && from % 8 == 0 && fp8::al16(in);
+  const bool vec = (F % 8 == 0 || kind == 1 || kind == 4) && from % 8 == 0 && fp8::al16(in);
   auto go = [&](auto f) { return (int)f((const bf16*)in, from, (uint8_t*)codes, ld, scales, ld_s, F, tokens, vec, st); };
   switch (kind) {
     case 0: return go(fp8::act<0>);
