@@ -6,32 +6,6 @@ namespace fp8 {
 
 constexpr int kWThreads = 256, kWRows = kWThreads / 16, kWSteps = kBlock / kWRows;  // 16 lanes a row, 16 rows at a time
 
-// 8 entries as they were read (bf16: packed, so that a CTA's block is 32 registers a thread and not 64)
-template <typename E, bool VEC>
-struct Piece {
-  float v[8];
-  __device__ __forceinline__ void load(const E* p, int n) { load8<VEC>(p, n, v); }
-  __device__ __forceinline__ void get(float* to) const {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) to[e] = v[e];
-  }
-  __device__ __forceinline__ void keep() {}
-};
-template <>
-struct Piece<bf16, true> {
-  uint4 v;
-  __device__ __forceinline__ void load(const bf16* p, int n) { v = n > 0 ? *reinterpret_cast<const uint4*>(p) : make_uint4(0, 0, 0, 0); }
-  __device__ __forceinline__ void get(float* to) const {
-    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      to[2 * e] = bf16_lo(u[e]);
-      to[2 * e + 1] = bf16_hi(u[e]);
-    }
-  }
-  __device__ __forceinline__ void keep() { asm volatile("" : "+r"(v.x), "+r"(v.y), "+r"(v.z), "+r"(v.w)); }  // (what is got behind this is not kept from before it)
-};
-
 template <typename E, bool VEC>
 __global__ void __launch_bounds__(kWThreads) fp8_weights_kernel(const E* __restrict__ w, long ld_w, uint8_t* __restrict__ codes, long ld, float* __restrict__ scales, int rows,
                                                                 int width, int nb) {
@@ -39,19 +13,15 @@ __global__ void __launch_bounds__(kWThreads) fp8_weights_kernel(const E* __restr
   const int b = blockIdx.x % nb, at = b * kBlock + (threadIdx.x & 15) * 8;
   const long r0 = (long)(blockIdx.x / nb) * kBlock + (threadIdx.x >> 4);
   pdl_wait();
-  Piece<E, VEC> piece[kWSteps];
+  float v[kWSteps][8];
   float m = 0.f;
 #pragma unroll
   for (int j = 0; j < kWSteps; ++j) {
     const long r = r0 + j * kWRows;
-    piece[j].load(w + (size_t)(r < rows ? r : 0) * ld_w + at, r < rows ? width - at : 0);
+    load8<VEC>(w + (size_t)(r < rows ? r : 0) * ld_w + at, r < rows ? width - at : 0, v[j]);
   }
 #pragma unroll
-  for (int j = 0; j < kWSteps; ++j) {
-    float v[8];
-    piece[j].get(v);
-    m = max_abs(m, max8(v));
-  }
+  for (int j = 0; j < kWSteps; ++j) m = max_abs(m, max8(v[j]));
   m = max16(m);
   m = max_abs(m, __shfl_xor_sync(0xffffffffu, m, 16));
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
@@ -62,10 +32,7 @@ __global__ void __launch_bounds__(kWThreads) fp8_weights_kernel(const E* __restr
 #pragma unroll
   for (int j = 0; j < kWSteps; ++j) {
     const long r = r0 + j * kWRows;
-    float v[8];
-    piece[j].keep();
-    piece[j].get(v);
-    if (r < rows && at < width) store_codes8(codes + (size_t)r * ld + at, width - at, v, k);
+    if (r < rows && at < width) store_codes8(codes + (size_t)r * ld + at, width - at, v[j], k);
   }
   if (threadIdx.x == 0) scales[blockIdx.x] = k.s;
 }
