@@ -18,9 +18,11 @@ namespace fp8 {
 namespace {
 
 constexpr int kRows = 128, kMaxSplit = 8, kMaxStages = 12;  // 8: the portable cluster size
+// CTAs on an SM: one where a thread holds many columns' sums
+constexpr int per_sm(int na, int nt) { return na * nt >= 128 ? 1 : 2; }
+constexpr int smem_most(int na, int nt) { return per_sm(na, nt) == 2 ? 113 * 1024 : 227 * 1024; }
 // A CTA's share of an SM's shared memory (228 KB, of which it takes 1 KB more than it asks for) is at least its share of the tensor memory, and more than any kernel with all 512
 // columns leaves: whoever is resident has its columns at once.  (CTAs that wait for columns while the rest of their cluster waits for them could wait for one another.)
-constexpr int kSmemMax = 113 * 1024;  // two CTAs on an SM
 constexpr size_t smem_least(int columns) { return columns > 128 ? 113 * 1024 : 56 * 1024; }
 
 __device__ __forceinline__ float4 ld_dsmem(uint32_t addr, uint32_t rank) {
@@ -58,14 +60,13 @@ constexpr int tmem_columns(int na, int nt) { return 2 * na * nt <= 32 ? 32 : 2 *
 
 // NA tiles of A
 template <int NT, int NA, typename O>
-__global__ void __launch_bounds__(64 + 128 * NA, 2)
+__global__ void __launch_bounds__(64 + 128 * NA, per_sm(NA, NT))
 fp8_gemm_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_w2, const Product p,
                     const FewPlan plan) {
   constexpr int THREADS = 64 + 128 * NA;
   constexpr uint32_t TMEM_COLS = tmem_columns(NA, NT);
   static_assert(2 * NA * NT <= 256, "two CTAs on an SM");
-  constexpr bool ROOM = NA * NT < 128;  // registers for 16 columns on their way beside those at work
-  const int stages = plan.stages, rows = plan.rows;
+    const int stages = plan.stages, rows = plan.rows;
   const uint32_t A_BYTES = rows * kBK, STAGE = NA * A_BYTES + NT * kBK;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -83,7 +84,22 @@ fp8_gemm_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
   const int m0 = (blockIdx.y / plan.n_tiles) * rows, t0 = (blockIdx.y % plan.n_tiles) * NT;
   const int kb0 = (int)((long)sp * p.kb / S), nk = (int)((long)(sp + 1) * p.kb / S) - kb0;
 
-  if (threadIdx.x == 0) {
+  const uint32_t n_scales = (uint32_t)min(NT, (p.N - t0 + 3) & ~3);  // (rows of scales are whole fours)
+  auto copy = [&](int i, int s) {  // block i of this CTA's into stage s
+    mbar_expect_tx(full + s, STAGE + n_scales * 4u);
+    uint8_t* st = smem + (size_t)s * STAGE;
+    const int kb = kb0 + i;
+    tma_load_2d(st, &map_w, kb * kBK, m0, full + s);
+    if (NA == 2) tma_load_2d(st + A_BYTES, &map_w2, kb * kBK, m0, full + s);
+    tma_load_2d(st + NA * A_BYTES, &map_x, kb * kBK, t0, full + s);
+    bulk_copy(xs + s * NT, p.sx + (size_t)kb * p.ld_sx + t0, n_scales * 4u, full + s);
+  };
+  // the thread that starts the copies fills the ring before anybody waits for anybody
+  const bool copies = warp == 0 && tc_elect_one();
+  if (copies) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_w) : "memory");
+    if (NA == 2) asm volatile("prefetch.tensormap [%0];" ::"l"(&map_w2) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_x) : "memory");
     for (int s = 0; s < stages; ++s) {
       mbar_init(full + s, 1);
       mbar_init(empty + s, 4 * NA);  // the warps that read the scales, behind the MMAs' end
@@ -94,30 +110,25 @@ fp8_gemm_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     }
     *dead = 0;
     mbar_fence_init();
+    // no early trigger: gemv.cu streams its weights before it waits for its predecessor, and they may be this kernel's output
+    pdl_wait();
+    for (int i = 0; i < stages && i < nk; ++i) copy(i, i);
   }
   if (warp == 1) tmem_alloc(tmem_slot, TMEM_COLS);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  // no early trigger: gemv.cu streams its weights before it waits for its predecessor, and they may be this kernel's output
   pdl_wait();
 
   float* part = reinterpret_cast<float*>(smem);  // [NT tokens][NA * rows features], over the ring
   if (warp == 0) {
-    if (tc_elect_one()) {
-      const uint32_t n_scales = (uint32_t)min(NT, (p.N - t0 + 3) & ~3);  // (rows of scales are whole fours)
-      int s = 0, i = 0;
-      uint32_t ph = 1;
+    if (copies) {
+      int s = 0, i = stages;
+      uint32_t ph = 0;
       for (; i < nk; ++i) {
         if (!mbar_wait_bounded(empty + s, ph, dead)) break;
-        mbar_expect_tx(full + s, STAGE + n_scales * 4u);
-        uint8_t* st = smem + (size_t)s * STAGE;
-        const int kb = kb0 + i;
-        tma_load_2d(st, &map_w, kb * kBK, m0, full + s);
-        if (NA == 2) tma_load_2d(st + A_BYTES, &map_w2, kb * kBK, m0, full + s);
-        tma_load_2d(st + NA * A_BYTES, &map_x, kb * kBK, t0, full + s);
-        bulk_copy(xs + s * NT, p.sx + (size_t)kb * p.ld_sx + t0, n_scales * 4u, full + s);
+        copy(i, s);
         if (++s == stages) {
           s = 0;
           ph ^= 1u;
@@ -193,31 +204,19 @@ fp8_gemm_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
         acc[at / 2 + 1] = fma2(pair_of(u[2], u[3]), mul2(w, pair_of(x.z, x.w)), acc[at / 2 + 1]);
       };
       auto scale4 = [&](int at) { return *reinterpret_cast<const float4*>(xs + s * NT + at); };
-      if constexpr (ROOM) {
-        uint32_t v[2][16];
-        tmem_ld16(t0, v[0]);
+      uint32_t v[2][16];
+      tmem_ld16(t0, v[0]);
 #pragma unroll
-        for (int c = 0; c < NT; c += 16) {
-          float4 x[4];
+      for (int c = 0; c < NT; c += 16) {
+        float4 x[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) x[j] = scale4(c + 4 * j);
-          uint32_t* now = v[(c / 16) & 1];
-          tmem_wait16(now);
-          if (c + 16 < NT) tmem_ld16(t0 + (uint32_t)(c + 16), v[(c / 16 + 1) & 1]);
-          else release();
+        for (int j = 0; j < 4; ++j) x[j] = scale4(c + 4 * j);
+        uint32_t* now = v[(c / 16) & 1];
+        tmem_wait16(now);
+        if (c + 16 < NT) tmem_ld16(t0 + (uint32_t)(c + 16), v[(c / 16 + 1) & 1]);
+        else release();
 #pragma unroll
-          for (int j = 0; j < 4; ++j) add4(c + 4 * j, now + 4 * j, x[j]);
-        }
-      } else {
-#pragma unroll
-        for (int c = 0; c < NT; c += 16) {
-          uint32_t v[16];
-          tmem_ld16(t0 + (uint32_t)c, v);
-          tmem_wait16(v);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) add4(c + 4 * j, v + 4 * j, scale4(c + 4 * j));
-        }
-        release();
+        for (int j = 0; j < 4; ++j) add4(c + 4 * j, now + 4 * j, x[j]);
       }
       if (++s == stages) {
         s = 0;
@@ -275,23 +274,35 @@ fp8_gemm_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
   } else {
     // a warp has a token's 128 features, a block of the result's scales
     const int i0 = (int)((long)sp * tokens / S), i1 = (int)((long)(sp + 1) * tokens / S);
-    for (int t = i0 + warp; t < i1; t += THREADS / 32) {
-      const float4 g = sum4(t * 256 + lane * 4), u = sum4(t * 256 + 128 + lane * 4);
-      float v[4] = {g.x, g.y, g.z, g.w};
-      const float w[4] = {u.x, u.y, u.z, u.w};
+    constexpr int WARPS = THREADS / 32;
+    for (int t = i0 + warp; t < i1; t += 2 * WARPS) {  // two at once: the others' shared memory is 1 us away
+      float4 g[2], u[2];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = (p.act == 0 ? gate_act<0>(v[j]) : p.act == 1 ? gate_act<1>(v[j]) : gate_act<2>(v[j])) * w[j];
-      const float m = max16(max_abs(max_abs(v[0], v[1], v[2]), v[3]));
-      const Scale k = scale_of(max_abs(m, __shfl_xor_sync(0xffffffffu, m, 16)));
-      const uint32_t c = codes4(v, k);
-      const int f = m0 + lane * 4;
-      uint8_t* dst = p.codes + (size_t)(t0 + t) * p.ld + f;
-      if (f + 4 <= p.M) {
-        *reinterpret_cast<uint32_t*>(dst) = c;
-      } else {
-        for (int j = 0; j < 4 && f + j < p.M; ++j) dst[j] = (uint8_t)(c >> (8 * j));
+      for (int j = 0; j < 2; ++j)
+        if (t + j * WARPS < i1) {
+          g[j] = sum4((t + j * WARPS) * 256 + lane * 4);
+          u[j] = sum4((t + j * WARPS) * 256 + 128 + lane * 4);
+        }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int tok = t + j * WARPS;
+        if (tok >= i1) break;
+        float v[4] = {g[j].x, g[j].y, g[j].z, g[j].w};
+        const float w[4] = {u[j].x, u[j].y, u[j].z, u[j].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = (p.act == 0 ? gate_act<0>(v[e]) : p.act == 1 ? gate_act<1>(v[e]) : gate_act<2>(v[e])) * w[e];
+        const float m = max16(max_abs(max_abs(v[0], v[1], v[2]), v[3]));
+        const Scale k = scale_of(max_abs(m, __shfl_xor_sync(0xffffffffu, m, 16)));
+        const uint32_t c = codes4(v, k);
+        const int f = m0 + lane * 4;
+        uint8_t* dst = p.codes + (size_t)(t0 + tok) * p.ld + f;
+        if (f + 4 <= p.M) {
+          *reinterpret_cast<uint32_t*>(dst) = c;
+        } else {
+          for (int e = 0; e < 4 && f + e < p.M; ++e) dst[e] = (uint8_t)(c >> (8 * e));
+        }
+        if (lane == 0) p.scales[(size_t)(m0 / kBlock) * p.ld_s + t0 + tok] = k.s;
       }
-      if (lane == 0) p.scales[(size_t)(m0 / kBlock) * p.ld_s + t0 + t] = k.s;
     }
   }
   if (threadIdx.x == 0) count_run_out(dead, p.err);  // (every wait lies before the barrier above)
@@ -303,15 +314,15 @@ fp8_gemm_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
   }
 }
 
-// Clusters of `splits` CTAs that can be resident at once, two CTAs on an SM (a cluster lives inside one GPC: gemm_skinny.cu)
-int resident(int splits, int sms) { return splits == 8 ? sms * 32 / 148 : splits == 4 ? sms * 70 / 148 : 2 * sms / splits; }
+// Clusters of `splits` CTAs that can be resident at once (a cluster lives inside one GPC: gemm_skinny.cu)
+int resident(int splits, int sms, int per) { return (splits == 8 ? sms * 16 / 148 : splits == 4 ? sms * 35 / 148 : sms / splits) * per; }
 
 // The most parts of K for which all tiles run at once, and the lowest tiles for which they still do, so that every SM has the same share of the weights.
 FewPlan few_plan(int M, int N, int kb, int na, int nt, int sms) {
   FewPlan p{kRows, 1, 2, (N + nt - 1) / nt};
   for (int S = kMaxSplit; S >= 1; S /= 2) {
     if (S > 1 && S > kb / 2) continue;  // at least two blocks a part
-    const int fit = resident(S, sms) / p.n_tiles;  // tiles of features
+    const int fit = resident(S, sms, per_sm(na, nt)) / p.n_tiles;  // tiles of features
     if (S > 1 && (long)fit * kRows < M) continue;
     p.splits = S;
     if (na == 1 && fit > 0 && (long)fit * kRows >= M) p.rows = std::max(32, ((M + fit - 1) / fit + 7) / 8 * 8);
@@ -320,7 +331,7 @@ FewPlan few_plan(int M, int N, int kb, int na, int nt, int sms) {
   const int nk = (kb + p.splits - 1) / p.splits;
   const size_t part = (size_t)nt * na * p.rows * 4;
   p.stages = kMaxStages;
-  while (p.stages > 2 && few_smem(na, p.rows, nt, p.stages) > kSmemMax) --p.stages;
+  while (p.stages > 2 && few_smem(na, p.rows, nt, p.stages) > (size_t)smem_most(na, nt)) --p.stages;
   const int hold = (int)((part + stage_bytes(na, p.rows, nt) - 1) / stage_bytes(na, p.rows, nt));  // stages that the part covers
   if (p.stages > nk) p.stages = std::max(nk, hold);
   return p;
@@ -330,7 +341,7 @@ template <int NT, int NA, typename O>
 int run_few(const Product& p, cudaStream_t st) {
   auto kern = fp8_gemm_few_kernel<NT, NA, O>;
   static std::atomic<uint64_t> set{0};
-  if (const cudaError_t e = allow_smem(set, (const void*)kern, kSmemMax); e != cudaSuccess) return (int)e;
+  if (const cudaError_t e = allow_smem(set, (const void*)kern, smem_most(NA, NT)); e != cudaSuccess) return (int)e;
   const FewPlan plan = few_plan(p.M, p.N, p.kb, NA, NT, sm_count());
   CUtensorMap mx, mw, mw2;
   if (!make_codes_map(&mx, p.x, p.N, p.K, p.ld_x, NT) || !make_codes_map(&mw, p.w, p.M, p.K, p.ld_w, plan.rows) ||
