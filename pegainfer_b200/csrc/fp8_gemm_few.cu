@@ -1,11 +1,12 @@
 // The product of 8-bit rows and weights for few tokens (fp8_gemm.cuh): a pass over the weights, so what counts is that every SM streams the same share of them.
 //
-//   A = W: `rows` <= 128 features per tile (tensor-memory lane = feature), B = X: NT tokens (column = token).  Gated: two tiles of A, 128 rows of w and the same of w2.
-//   A tile's K is cut into parts, one CTA each, and those CTAs are a cluster: each leaves its fp32 part in its own shared memory ([token][feature], over the operand ring), and
-//   after a cluster barrier adds up its share of the tile in rank order over distributed shared memory, so a result does not depend on timing.
-//   warp 0 TMA producer | warp 1 MMA issuer | the others: a block's partial sum out of tensor memory, times its scales (a token's come with the stage, a feature's is the thread's own),
+//   A = W: NA tiles of `rows` <= 128 features (tensor-memory lane = feature), B = X: NT tokens (column = token).  Gated: 128 rows of w and the same of w2.
+//   A tile's K is cut into parts, one CTA each, and those CTAs are a cluster: each sends its fp32 part to the CTAs that own a share of the tile's results (features; gated: tokens, whose
+//   128 features are a block of the result's scales), and behind one cluster barrier they add them up in rank order, so a result does not depend on timing.
+//   warp 0 TMA producer | warps 1 and 2 MMA issuers of even and odd blocks (looks, four MMAs and a commit take a thread 650 clocks) | the others: a block's partial sum out of tensor memory, times its scales (a token's come with the stage, a feature's is the thread's own),
 //   onto the sum in registers; then the part.  All warps: sums -> output.
 // Any number of rows may make a tile: the MMAs read 128, and what lies behind the tile's own ends in lanes that nobody reads.
+// One CTA has an SM: a second one on it would start 1 us later, and a cluster of eight with two on an SM 2 us.
 #include <cuda.h>
 
 #include <algorithm>
@@ -18,19 +19,15 @@ namespace fp8 {
 namespace {
 
 constexpr int kRows = 128, kMaxSplit = 8, kMaxStages = 12;  // 8: the portable cluster size
-// CTAs on an SM: one where a thread holds many columns' sums
-constexpr int per_sm(int na, int nt) { return na * nt >= 128 ? 1 : 2; }
-constexpr int smem_most(int na, int nt) { return per_sm(na, nt) == 2 ? 113 * 1024 : 227 * 1024; }
-// A CTA's share of an SM's shared memory (228 KB, of which it takes 1 KB more than it asks for) is at least its share of the tensor memory, and more than any kernel with all 512
-// columns leaves: whoever is resident has its columns at once.  (CTAs that wait for columns while the rest of their cluster waits for them could wait for one another.)
-constexpr size_t smem_least(int columns) { return columns > 128 ? 113 * 1024 : 56 * 1024; }
+constexpr int kSmemMost = 227 * 1024;
+// A CTA asks for more than half of an SM's shared memory, so it is alone with its kind, and for more than any kernel with all 512 columns of tensor memory leaves: whoever is resident has
+// its columns at once.  (CTAs that wait for columns while the rest of their cluster waits for them could wait for one another.)
+constexpr size_t kSmemLeast = 116 * 1024;
 
-__device__ __forceinline__ float4 ld_dsmem(uint32_t addr, uint32_t rank) {
+__device__ __forceinline__ void st_cluster(uint32_t addr, uint32_t rank, float v) {
   uint32_t a;
-  float4 v;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
-  return v;
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(a), "f"(v) : "memory");
 }
 __device__ __forceinline__ void umma_f8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -48,31 +45,36 @@ __device__ __forceinline__ void bulk_copy(void* dst, const void* src, uint32_t b
 }
 
 struct FewPlan {
-  int rows, splits, stages;  // features of a tile, parts of K
+  int rows, splits, stages;  // features of a tile of A, parts of K
   int n_tiles;               // tiles of tokens
+  int own;                   // features (gated: tokens) of the tile that a CTA adds up
 };
 constexpr size_t stage_bytes(int na, int rows, int nt) { return (size_t)(na * rows + nt) * kBK; }
-constexpr size_t few_smem(int na, int rows, int nt, int stages) {
-  return stages * (stage_bytes(na, rows, nt) + nt * sizeof(float)) + (size_t)(kRows - rows) * kBK + 1024 + (2 * kMaxStages + 4) * 8 + 16;
+// parts that a CTA receives; a tile in one part lies over the ring
+size_t received_bytes(int na, const FewPlan& p, int nt, bool gated) { return p.splits == 1 ? 0 : (size_t)p.splits * p.own * (gated ? na * p.rows : nt) * sizeof(float); }
+size_t few_smem(int na, const FewPlan& p, int nt, bool gated) {
+  return p.stages * (stage_bytes(na, p.rows, nt) + nt * sizeof(float)) + (size_t)(kRows - p.rows) * kBK + received_bytes(na, p, nt, gated) + 1024 + (2 * kMaxStages + 4) * 8 + 16;
 }
+constexpr int tmem_columns(int na, int nt) { return 2 * na * nt <= 32 ? 32 : 2 * na * nt <= 64 ? 64 : 2 * na * nt <= 128 ? 128 : 2 * na * nt <= 256 ? 256 : 512; }
 
-constexpr int tmem_columns(int na, int nt) { return 2 * na * nt <= 32 ? 32 : 2 * na * nt <= 64 ? 64 : 2 * na * nt <= 128 ? 128 : 256; }
-
-// NA tiles of A
-template <int NT, int NA, typename O>
-__global__ void __launch_bounds__(64 + 128 * NA, per_sm(NA, NT))
+// GATED: NA = 2, O is the codes' type
+template <int NT, int NA, bool GATED, typename O>
+__global__ void __launch_bounds__(96 + 128 * NA, 1)
 fp8_gemm_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_w2, const Product p,
                     const FewPlan plan) {
-  constexpr int THREADS = 64 + 128 * NA;
+  constexpr int THREADS = 96 + 128 * NA;
   constexpr uint32_t TMEM_COLS = tmem_columns(NA, NT);
-  static_assert(2 * NA * NT <= 256, "two CTAs on an SM");
+  static_assert(2 * NA * NT <= 512 && (!GATED || NA == 2), "tensor memory");
     const int stages = plan.stages, rows = plan.rows;
   const uint32_t A_BYTES = rows * kBK, STAGE = NA * A_BYTES + NT * kBK;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   // (behind the last stage lies room for the rows of A that the MMAs read beyond the tile's own)
   float* xs = reinterpret_cast<float*>(smem + (size_t)stages * STAGE + (kRows - rows) * kBK);  // [stages][NT] scales of the tokens
-  uint64_t* full = reinterpret_cast<uint64_t*>(xs + stages * NT);
+  const int S = gridDim.x, sp = (int)cluster_ctarank();  // the cluster spans the whole x axis
+  const int features = NA * rows, own = plan.own;
+  float* received = S > 1 ? xs + stages * NT : reinterpret_cast<float*>(smem);  // [S][NT][own features]; gated [S][own tokens][256]
+  uint64_t* full = reinterpret_cast<uint64_t*>(xs + stages * NT + (S > 1 ? S * own * (GATED ? 256 : NT) : 0));
   uint64_t* empty = full + kMaxStages;
   uint64_t* tfull = empty + kMaxStages;  // [2]
   uint64_t* tempty = tfull + 2;          // [2]
@@ -80,8 +82,7 @@ fp8_gemm_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
   volatile int* dead = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int S = gridDim.x, sp = (int)cluster_ctarank();  // the cluster spans the whole x axis
-  const int m0 = (blockIdx.y / plan.n_tiles) * rows, t0 = (blockIdx.y % plan.n_tiles) * NT;
+  const int m0 = (blockIdx.y / plan.n_tiles) * (GATED ? rows : features), t0 = (blockIdx.y % plan.n_tiles) * NT;
   const int kb0 = (int)((long)sp * p.kb / S), nk = (int)((long)(sp + 1) * p.kb / S) - kb0;
 
   const uint32_t n_scales = (uint32_t)min(NT, (p.N - t0 + 3) & ~3);  // (rows of scales are whole fours)
@@ -90,7 +91,7 @@ fp8_gemm_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     uint8_t* st = smem + (size_t)s * STAGE;
     const int kb = kb0 + i;
     tma_load_2d(st, &map_w, kb * kBK, m0, full + s);
-    if (NA == 2) tma_load_2d(st + A_BYTES, &map_w2, kb * kBK, m0, full + s);
+    if (NA == 2) tma_load_2d(st + A_BYTES, GATED ? &map_w2 : &map_w, kb * kBK, GATED ? m0 : m0 + rows, full + s);
     tma_load_2d(st + NA * A_BYTES, &map_x, kb * kBK, t0, full + s);
     bulk_copy(xs + s * NT, p.sx + (size_t)kb * p.ld_sx + t0, n_scales * 4u, full + s);
   };
@@ -98,7 +99,7 @@ fp8_gemm_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
   const bool copies = warp == 0 && tc_elect_one();
   if (copies) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(&map_w) : "memory");
-    if (NA == 2) asm volatile("prefetch.tensormap [%0];" ::"l"(&map_w2) : "memory");
+    if (GATED) asm volatile("prefetch.tensormap [%0];" ::"l"(&map_w2) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&map_x) : "memory");
     for (int s = 0; s < stages; ++s) {
       mbar_init(full + s, 1);
@@ -119,9 +120,11 @@ fp8_gemm_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  if (S > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // (waited for in front of the first word for another CTA)
   pdl_wait();
 
-  float* part = reinterpret_cast<float*>(smem);  // [NT tokens][NA * rows features], over the ring
+  const int tokens = min(NT, p.N - t0);
+  uint64_t acc[NT / 2];
   if (warp == 0) {
     if (copies) {
       int s = 0, i = stages;
@@ -137,14 +140,13 @@ fp8_gemm_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       if (i < nk) ring_drain(full, stages, i);
     }
     __syncwarp();
-  } else if (warp == 1) {
+  } else if (warp < 3) {
     if (tc_elect_one()) {
       constexpr uint32_t idesc = f8_idesc(kRows, NT);
-      int s = 0, i = 0;
-      uint32_t ph = 0;
-      for (; i < nk; ++i) {
-        const int buf = i & 1;
-        const uint32_t tph = (uint32_t)(((i >> 1) & 1) ^ 1);
+      const int buf = warp - 1;
+      int s = buf, i = buf;
+      uint32_t ph = 0, tph = 1;
+      for (; i < nk; i += 2) {
         // two looks at once: a wait costs a thread 200 clocks where nothing is to be waited for
         const bool here = mbar_test_wait(full + s, ph), free = mbar_test_wait(tempty + buf, tph);
         if (!here && !mbar_wait_bounded(full + s, ph, dead)) break;
@@ -160,22 +162,23 @@ fp8_gemm_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
             umma_f8(tmem_base + (uint32_t)((buf * NA + h) * NT), adesc + (uint64_t)(k * 2), bdesc + (uint64_t)(k * 2), idesc, k > 0 ? 1u : 0u);
         }
         umma_commit(tfull + buf);
-        if (++s == stages) {
-          s = 0;
+        tph ^= 1u;
+        s += 2;
+        if (s >= stages) {
+          s -= stages;
           ph ^= 1u;
         }
       }
       if (i < nk) {  // MMAs under way end in a partial sum that nobody waits for any more
-        umma_commit(tfull + (i & 1));
-        mbar_drain(tfull + (i & 1), (uint32_t)((i >> 1) & 1));
+        umma_commit(tfull + buf);
+        mbar_drain(tfull + buf, tph ^ 1u);
       }
     }
     __syncwarp();
   } else {
-    const int q = warp & 3, h = (warp - 2) >> 2, f = q * 32 + lane;  // tensor-memory lanes that this warp may read; lane = feature
-    const int row = m0 + f < p.M ? m0 + f : p.M - 1;
-    const float* sw = (NA == 2 && h == 1 ? p.sw2 : p.sw) + (size_t)(row / kBlock) * p.kb + kb0;
-    uint64_t acc[NT / 2];
+    const int q = warp & 3, h = (warp - 3) >> 2, f = q * 32 + lane;  // tensor-memory lanes that this warp may read; lane = feature
+    const int at = m0 + (GATED ? f : h * rows + f), row = at < p.M ? at : p.M - 1;
+    const float* sw = (GATED && h == 1 ? p.sw2 : p.sw) + (size_t)(row / kBlock) * p.kb + kb0;
 #pragma unroll
     for (int j = 0; j < NT / 2; ++j) acc[j] = 0;
     float w_next = __ldg(sw);
@@ -223,12 +226,29 @@ fp8_gemm_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
         ph ^= 1u;
       }
     }
-    // every MMA has read its operands: the ring takes the part (but another warp may still read its last scales: those lie behind the ring)
+  }
+  // ---- the part to its owners: every MMA has read its operands (a tile in one part lies over the ring), and all CTAs of the cluster are there
+  __syncwarp();
+  if (S > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  if (warp >= 3) {
+    const int q = warp & 3, h = (warp - 3) >> 2, f = q * 32 + lane;
     if (f < rows) {
+      const int g = h * rows + f;
+      const uint32_t to = smem_u32(received);
+      if constexpr (GATED) {
+        const int shift = 31 - __clz(own);  // (a power of two)
 #pragma unroll
-      for (int c = 0; c < NT; c += 2) {
-        part[(size_t)c * (NA * rows) + h * rows + f] = lo_of(acc[c / 2]);
-        part[(size_t)(c + 1) * (NA * rows) + h * rows + f] = hi_of(acc[c / 2]);
+        for (int c = 0; c < NT; ++c) {
+          const int rank = c >> shift;
+          if (c < tokens) st_cluster(to + (uint32_t)(((sp * own + c - (rank << shift)) * 256 + g) * 4), (uint32_t)(S > 1 ? rank : 0), c & 1 ? hi_of(acc[c / 2]) : lo_of(acc[c / 2]));
+        }
+      } else {
+        const int rank = g / own;
+        const uint32_t mine = to + (uint32_t)((sp * NT * own + g - rank * own) * 4);
+#pragma unroll
+        for (int c = 0; c < NT; ++c) {
+          if (c < tokens) st_cluster(mine + (uint32_t)(c * own * 4), (uint32_t)rank, c & 1 ? hi_of(acc[c / 2]) : lo_of(acc[c / 2]));
+        }
       }
     }
   }
@@ -236,132 +256,155 @@ fp8_gemm_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
   __syncthreads();
   if (S > 1) cluster_barrier();
   // ---- this CTA's share of the tile, added up in rank order
-  const uint32_t part_addr = smem_u32(part);
-  const int tokens = min(NT, p.N - t0);
-  auto sum4 = [&](int at) {  // four features of a token
-    float4 v[kMaxSplit];
-#pragma unroll
-    for (int r = 0; r < kMaxSplit; ++r)
-      if (r < S) v[r] = S > 1 ? ld_dsmem(part_addr + (uint32_t)at * 4u, (uint32_t)r) : *reinterpret_cast<const float4*>(part + at);
-    float4 t = v[0];
+  auto sum4 = [&](int at, int stride) {  // four features of a token
+    float4 t = *reinterpret_cast<const float4*>(received + at);
 #pragma unroll
     for (int r = 1; r < kMaxSplit; ++r)
       if (r < S) {
-        t.x += v[r].x;
-        t.y += v[r].y;
-        t.z += v[r].z;
-        t.w += v[r].w;
+        const float4 v = *reinterpret_cast<const float4*>(received + r * stride + at);
+        t.x += v.x;
+        t.y += v.y;
+        t.z += v.z;
+        t.w += v.w;
       }
     return t;
   };
-  if constexpr (NA == 1) {
-    const int quads = rows / 4, items = tokens * quads;
-    const int i0 = (int)((long)sp * items / S), i1 = (int)((long)(sp + 1) * items / S);
+  if constexpr (!GATED) {
+    const int quads = (max(0, min(own, features - sp * own))) / 4, items = tokens * quads;
     O* y = static_cast<O*>(p.y);
-    for (int it = i0 + threadIdx.x; it < i1; it += THREADS) {
-      const int t = it / quads, f = m0 + (it - t * quads) * 4;
-      const float4 v = sum4(it * 4);
+    for (int it = threadIdx.x; it < items; it += THREADS) {
+      const int t = it / quads, j = (it - t * quads) * 4, f = m0 + sp * own + j;
       if (f >= p.M) continue;
+      const float4 v = sum4(t * own + j, NT * own);
       O* dst = y + (size_t)(t0 + t) * p.ld_y + f;
       if (f + 4 <= p.M && (reinterpret_cast<uintptr_t>(dst) & (4 * sizeof(O) - 1)) == 0) {
         if constexpr (sizeof(O) == 4) *reinterpret_cast<float4*>(dst) = v;
         else *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
       } else {
         const float o[4] = {v.x, v.y, v.z, v.w};
-        for (int j = 0; j < 4 && f + j < p.M; ++j) dst[j] = from_f<O>(o[j]);
+        for (int e = 0; e < 4 && f + e < p.M; ++e) dst[e] = from_f<O>(o[e]);
       }
     }
   } else {
     // a warp has a token's 128 features, a block of the result's scales
-    const int i0 = (int)((long)sp * tokens / S), i1 = (int)((long)(sp + 1) * tokens / S);
-    constexpr int WARPS = THREADS / 32;
-    for (int t = i0 + warp; t < i1; t += 2 * WARPS) {  // two at once: the others' shared memory is 1 us away
-      float4 g[2], u[2];
+    const int mine = min(own, tokens - sp * own);
+    for (int t = warp; t < mine; t += THREADS / 32) {
+      const float4 g = sum4(t * 256 + lane * 4, own * 256), u = sum4(t * 256 + 128 + lane * 4, own * 256);
+      float v[4] = {g.x, g.y, g.z, g.w};
+      const float w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
-        if (t + j * WARPS < i1) {
-          g[j] = sum4((t + j * WARPS) * 256 + lane * 4);
-          u[j] = sum4((t + j * WARPS) * 256 + 128 + lane * 4);
-        }
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int tok = t + j * WARPS;
-        if (tok >= i1) break;
-        float v[4] = {g[j].x, g[j].y, g[j].z, g[j].w};
-        const float w[4] = {u[j].x, u[j].y, u[j].z, u[j].w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = (p.act == 0 ? gate_act<0>(v[e]) : p.act == 1 ? gate_act<1>(v[e]) : gate_act<2>(v[e])) * w[e];
-        const float m = max16(max_abs(max_abs(v[0], v[1], v[2]), v[3]));
-        const Scale k = scale_of(max_abs(m, __shfl_xor_sync(0xffffffffu, m, 16)));
-        const uint32_t c = codes4(v, k);
-        const int f = m0 + lane * 4;
-        uint8_t* dst = p.codes + (size_t)(t0 + tok) * p.ld + f;
-        if (f + 4 <= p.M) {
-          *reinterpret_cast<uint32_t*>(dst) = c;
-        } else {
-          for (int e = 0; e < 4 && f + e < p.M; ++e) dst[e] = (uint8_t)(c >> (8 * e));
-        }
-        if (lane == 0) p.scales[(size_t)(m0 / kBlock) * p.ld_s + t0 + tok] = k.s;
+      for (int e = 0; e < 4; ++e) v[e] = (p.act == 0 ? gate_act<0>(v[e]) : p.act == 1 ? gate_act<1>(v[e]) : gate_act<2>(v[e])) * w[e];
+      const float m = max16(max_abs(max_abs(v[0], v[1], v[2]), v[3]));
+      const Scale k = scale_of(max_abs(m, __shfl_xor_sync(0xffffffffu, m, 16)));
+      const uint32_t c = codes4(v, k);
+      const int f = m0 + lane * 4, tok = t0 + sp * own + t;
+      uint8_t* dst = p.codes + (size_t)tok * p.ld + f;
+      if (f + 4 <= p.M) {
+        *reinterpret_cast<uint32_t*>(dst) = c;
+      } else {
+        for (int e = 0; e < 4 && f + e < p.M; ++e) dst[e] = (uint8_t)(c >> (8 * e));
       }
+      if (lane == 0) p.scales[(size_t)(m0 / kBlock) * p.ld_s + tok] = k.s;
     }
   }
   if (threadIdx.x == 0) count_run_out(dead, p.err);  // (every wait lies before the barrier above)
-  __syncwarp();
-  if (S > 1) cluster_barrier();  // the others may still read this CTA's part
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem_base, TMEM_COLS);
   }
 }
 
-// Clusters of `splits` CTAs that can be resident at once (a cluster lives inside one GPC: gemm_skinny.cu)
-int resident(int splits, int sms, int per) { return (splits == 8 ? sms * 16 / 148 : splits == 4 ? sms * 35 / 148 : sms / splits) * per; }
-
-// The most parts of K for which all tiles run at once, and the lowest tiles for which they still do, so that every SM has the same share of the weights.
-FewPlan few_plan(int M, int N, int kb, int na, int nt, int sms) {
-  FewPlan p{kRows, 1, 2, (N + nt - 1) / nt};
-  for (int S = kMaxSplit; S >= 1; S /= 2) {
-    if (S > 1 && S > kb / 2) continue;  // at least two blocks a part
-    const int fit = resident(S, sms, per_sm(na, nt)) / p.n_tiles;  // tiles of features
-    if (S > 1 && (long)fit * kRows < M) continue;
-    p.splits = S;
-    if (na == 1 && fit > 0 && (long)fit * kRows >= M) p.rows = std::max(32, ((M + fit - 1) / fit + 7) / 8 * 8);
-    break;
+// Clusters of 1, 2, 4 and 8 CTAs that the current device has at once, one CTA on an SM (a cluster lives inside one GPC, and GPCs differ): asked for once per device
+cudaError_t clusters_at_once(const void* kern, cudaLaunchConfig_t cfg, cudaLaunchAttribute& size, int* out) {
+  static std::atomic<uint64_t> known[64];  // by device: 16 bits each
+  int dev = 0;
+  if (const cudaError_t e = cudaGetDevice(&dev); e != cudaSuccess) return e;
+  uint64_t v = known[dev & 63].load(std::memory_order_acquire);
+  if (v == 0) {
+    cfg.dynamicSmemBytes = kSmemLeast;
+    cfg.numAttrs = 1;
+    for (int i = 0; i < 4; ++i) {
+      int n = 0;
+      size.val.clusterDim.x = 1 << i;
+      cfg.gridDim = dim3(1 << i);
+      if (const cudaError_t e = cudaOccupancyMaxActiveClusters(&n, kern, &cfg); e != cudaSuccess) return e;
+      v |= (uint64_t)std::min(n, 0xffff) << (16 * i);
+    }
+    known[dev & 63].store(v, std::memory_order_release);
   }
-  const int nk = (kb + p.splits - 1) / p.splits;
-  const size_t part = (size_t)nt * na * p.rows * 4;
-  p.stages = kMaxStages;
-  while (p.stages > 2 && few_smem(na, p.rows, nt, p.stages) > (size_t)smem_most(na, nt)) --p.stages;
-  const int hold = (int)((part + stage_bytes(na, p.rows, nt) - 1) / stage_bytes(na, p.rows, nt));  // stages that the part covers
-  if (p.stages > nk) p.stages = std::max(nk, hold);
-  return p;
+  for (int i = 0; i < 4; ++i) out[i] = (int)(v >> (16 * i) & 0xffff);
+  return cudaSuccess;
 }
 
-template <int NT, int NA, typename O>
+// Parts of K, features of a tile, stages.  A block of K takes a CTA as long as its bytes (55 of them a ns and SM where all SMs stream) or 0.3 us for its chain copy -> MMAs -> sum, a cluster's
+// joining 1 us; resident[i]: clusters of 2^i CTAs that the GPU has at once.  The lowest tiles for which the number of waves stays, so that every SM has the same share.
+FewPlan few_plan(int M, int N, int kb, int na, int nt, bool gated, const int* resident) {
+  const int per_tile = gated ? kRows : na * kRows, n_tiles = (N + nt - 1) / nt;
+  FewPlan best{};
+  double least = 0;
+  for (int i = 0; i < 4; ++i) {
+    const int S = 1 << i;
+    if (S > 1 && (S > kb / 2 || resident[i] < 1 || (!gated && na == 2))) continue;  // at least two blocks a part
+    const int at_once = std::max(1, resident[i]);
+    FewPlan p{kRows, S, 2, n_tiles, 0};
+    const long tiles = (long)((M + per_tile - 1) / per_tile) * n_tiles;
+    const long waves = (tiles + at_once - 1) / at_once;
+    if (!gated) {
+      const long m_tiles = std::max<long>(1, waves * at_once / n_tiles);  // that the waves have room for
+      p.rows = (int)std::min<long>(kRows, std::max<long>(32, ((M + m_tiles * na - 1) / (m_tiles * na) + 7) / 8 * 8));
+    }
+    p.own = gated ? std::max(1, nt / S) : ((na * p.rows / 4 + S - 1) / S) * 4;
+    const int nk = (kb + S - 1) / S;
+    const double block = std::max(300., (double)stage_bytes(na, p.rows, nt) / 55);
+    const double cost = (double)waves * (nk * block + 3000) + (S > 1 ? 1000 : 0);
+    while (p.stages < kMaxStages) {
+      ++p.stages;
+      if (few_smem(na, p, nt, gated) > (size_t)kSmemMost) {
+        --p.stages;
+        break;
+      }
+    }
+    if (few_smem(na, p, nt, gated) > (size_t)kSmemMost) continue;
+    const size_t part = S == 1 ? (size_t)p.own * (gated ? 256 : nt) * sizeof(float) : 0;  // over the ring
+    const int hold = (int)((part + stage_bytes(na, p.rows, nt) - 1) / stage_bytes(na, p.rows, nt));
+    if (hold > p.stages) continue;
+    if (p.stages > nk) p.stages = std::max({nk, hold, 1});
+    if (best.splits == 0 || cost < least) {
+      best = p;
+      least = cost;
+    }
+  }
+  return best;
+}
+
+template <int NT, int NA, bool GATED, typename O>
 int run_few(const Product& p, cudaStream_t st) {
-  auto kern = fp8_gemm_few_kernel<NT, NA, O>;
+  auto kern = fp8_gemm_few_kernel<NT, NA, GATED, O>;
   static std::atomic<uint64_t> set{0};
-  if (const cudaError_t e = allow_smem(set, (const void*)kern, smem_most(NA, NT)); e != cudaSuccess) return (int)e;
-  const FewPlan plan = few_plan(p.M, p.N, p.kb, NA, NT, sm_count());
-  CUtensorMap mx, mw, mw2;
-  if (!make_codes_map(&mx, p.x, p.N, p.K, p.ld_x, NT) || !make_codes_map(&mw, p.w, p.M, p.K, p.ld_w, plan.rows) ||
-      !make_codes_map(&mw2, NA == 2 ? p.w2 : p.w, p.M, p.K, p.ld_w, plan.rows))
-    return (int)cudaErrorInvalidValue;
-  ThreadState& ts = tls();
-  ts.launches++;
+  if (const cudaError_t e = allow_smem(set, (const void*)kern, kSmemMost); e != cudaSuccess) return (int)e;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(plan.splits, (p.M + plan.rows - 1) / plan.rows * plan.n_tiles);
-  cfg.blockDim = dim3(64 + 128 * NA);
-  cfg.dynamicSmemBytes = std::max(few_smem(NA, plan.rows, NT, plan.stages), smem_least(tmem_columns(NA, NT)));
-  cfg.stream = st;
+  cfg.blockDim = dim3(96 + 128 * NA);
   cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = ts.pdl ? 1 : 0;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = plan.splits;
-  attr[1].val.clusterDim.y = 1;
-  attr[1].val.clusterDim.z = 1;
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  ThreadState& ts = tls();
+  attr[1].val.programmaticStreamSerializationAllowed = ts.pdl ? 1 : 0;
   cfg.attrs = attr;
+  int resident[4];
+  if (const cudaError_t e = clusters_at_once((const void*)kern, cfg, attr[0], resident); e != cudaSuccess) return (int)e;
+  const FewPlan plan = few_plan(p.M, p.N, p.kb, NA, NT, GATED, resident);
+  CUtensorMap mx, mw, mw2;
+  if (plan.splits == 0 || !make_codes_map(&mx, p.x, p.N, p.K, p.ld_x, NT) || !make_codes_map(&mw, p.w, p.M, p.K, p.ld_w, plan.rows) ||
+      !make_codes_map(&mw2, GATED ? p.w2 : p.w, p.M, p.K, p.ld_w, plan.rows))
+    return (int)cudaErrorInvalidValue;
+  const int per_tile = GATED ? plan.rows : NA * plan.rows;
+  ts.launches++;
+  cfg.gridDim = dim3(plan.splits, (p.M + per_tile - 1) / per_tile * plan.n_tiles);
+  cfg.dynamicSmemBytes = std::max(few_smem(NA, plan, NT, GATED), kSmemLeast);
+  cfg.stream = st;
+  attr[0].val.clusterDim.x = plan.splits;
   cfg.numAttrs = 2;
   return (int)cudaLaunchKernelEx(&cfg, kern, mx, mw, mw2, p, plan);
 }
@@ -372,15 +415,21 @@ bool few_takes(const Product& p, bool gated) { return p.N <= (gated ? 64 : 128) 
 
 int launch_few(const Product& p, bool gated, bool y_f32, cudaStream_t st) {
   if (gated) {
-    if (p.N <= 16) return run_few<16, 2, uint8_t>(p, st);
-    if (p.N <= 32) return run_few<32, 2, uint8_t>(p, st);
-    return run_few<64, 2, uint8_t>(p, st);
+    if (p.N <= 16) return run_few<16, 2, true, uint8_t>(p, st);
+    if (p.N <= 32) return run_few<32, 2, true, uint8_t>(p, st);
+    return run_few<64, 2, true, uint8_t>(p, st);
   }
   auto go = [&](auto f, auto b) { return y_f32 ? f(p, st) : b(p, st); };
-  if (p.N <= 16) return go(run_few<16, 1, float>, run_few<16, 1, bf16>);
-  if (p.N <= 32) return go(run_few<32, 1, float>, run_few<32, 1, bf16>);
-  if (p.N <= 64) return go(run_few<64, 1, float>, run_few<64, 1, bf16>);
-  return go(run_few<128, 1, float>, run_few<128, 1, bf16>);
+  if (p.M > kRows * sm_count()) {  // two tiles of features a CTA: fewer CTAs that read all of X
+    if (p.N <= 16) return go(run_few<16, 2, false, float>, run_few<16, 2, false, bf16>);
+    if (p.N <= 32) return go(run_few<32, 2, false, float>, run_few<32, 2, false, bf16>);
+    if (p.N <= 64) return go(run_few<64, 2, false, float>, run_few<64, 2, false, bf16>);
+    return go(run_few<128, 2, false, float>, run_few<128, 2, false, bf16>);
+  }
+  if (p.N <= 16) return go(run_few<16, 1, false, float>, run_few<16, 1, false, bf16>);
+  if (p.N <= 32) return go(run_few<32, 1, false, float>, run_few<32, 1, false, bf16>);
+  if (p.N <= 64) return go(run_few<64, 1, false, float>, run_few<64, 1, false, bf16>);
+  return go(run_few<128, 1, false, float>, run_few<128, 1, false, bf16>);
 }
 
 }  // namespace fp8
