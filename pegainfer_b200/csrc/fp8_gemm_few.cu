@@ -1,8 +1,9 @@
 // The product of 8-bit rows and weights for few tokens (fp8_gemm.cuh): a pass over the weights, so what counts is that every SM streams the same share of them.
 //
 //   A = W: NA tiles of `rows` <= 128 features (tensor-memory lane = feature), B = X: NT tokens (column = token).  Gated: 128 rows of w and the same of w2.
-//   A tile's K is cut into parts, one CTA each, and those CTAs are a cluster: each sends its fp32 part to the CTAs that own a share of the tile's results (features; gated: tokens, whose
-//   128 features are a block of the result's scales), and behind one cluster barrier they add them up in rank order, so a result does not depend on timing.
+//   A tile's K is cut into parts, one CTA each, and those CTAs are a cluster: each leaves its fp32 part over its operand ring and sends it, 16 bytes a thread, to the CTAs that own a share of
+//   the tile's results (features; gated: tokens, whose 128 features are a block of the result's scales), which add them up in rank order, so a result does not depend on timing.
+//   B200, us a launch, 48 tokens of 4096 x 12288 in 4 parts: words sent by the threads that have them 16.7, bulk copies 18.1; one token of 2560 x 4096 6.8 and 7.7.
 //   warp 0 TMA producer | warps 1 and 2 MMA issuers of even and odd blocks (looks, four MMAs and a commit take a thread 650 clocks) | the others: a block's partial sum out of tensor memory, times its scales (a token's come with the stage, a feature's is the thread's own),
 //   onto the sum in registers; then the part.  All warps: sums -> output.
 // Any number of rows may make a tile: the MMAs read 128, and what lies behind the tile's own ends in lanes that nobody reads.
@@ -24,10 +25,13 @@ constexpr int kSmemMost = 227 * 1024;
 // its columns at once.  (CTAs that wait for columns while the rest of their cluster waits for them could wait for one another.)
 constexpr size_t kSmemLeast = 116 * 1024;
 
-__device__ __forceinline__ void st_cluster(uint32_t addr, uint32_t rank, float v) {
+__device__ __forceinline__ uint32_t map_to(uint32_t addr, uint32_t rank) {
   uint32_t a;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
-  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(a), "f"(v) : "memory");
+  return a;
+}
+__device__ __forceinline__ void st_cluster4(uint32_t dst_cluster, float4 v) {
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(dst_cluster), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
 }
 __device__ __forceinline__ void umma_f8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -50,7 +54,7 @@ struct FewPlan {
   int own;                   // features (gated: tokens) of the tile that a CTA adds up
 };
 constexpr size_t stage_bytes(int na, int rows, int nt) { return (size_t)(na * rows + nt) * kBK; }
-// parts that a CTA receives; a tile in one part lies over the ring
+// parts that a CTA receives
 size_t received_bytes(int na, const FewPlan& p, int nt, bool gated) { return p.splits == 1 ? 0 : (size_t)p.splits * p.own * (gated ? na * p.rows : nt) * sizeof(float); }
 size_t few_smem(int na, const FewPlan& p, int nt, bool gated) {
   return p.stages * (stage_bytes(na, p.rows, nt) + nt * sizeof(float)) + (size_t)(kRows - p.rows) * kBK + received_bytes(na, p, nt, gated) + 1024 + (2 * kMaxStages + 4) * 8 + 16;
@@ -73,7 +77,8 @@ fp8_gemm_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
   float* xs = reinterpret_cast<float*>(smem + (size_t)stages * STAGE + (kRows - rows) * kBK);  // [stages][NT] scales of the tokens
   const int S = gridDim.x, sp = (int)cluster_ctarank();  // the cluster spans the whole x axis
   const int features = NA * rows, own = plan.own;
-  float* received = S > 1 ? xs + stages * NT : reinterpret_cast<float*>(smem);  // [S][NT][own features]; gated [S][own tokens][256]
+  float* part = reinterpret_cast<float*>(smem);                // over the ring: [S owners][NT][own features]; gated [NT][256]
+  float* received = S > 1 ? xs + stages * NT : part;           // [S senders][NT][own features]; gated [S][own tokens][256]
   uint64_t* full = reinterpret_cast<uint64_t*>(xs + stages * NT + (S > 1 ? S * own * (GATED ? 256 : NT) : 0));
   uint64_t* empty = full + kMaxStages;
   uint64_t* tfull = empty + kMaxStages;  // [2]
@@ -85,6 +90,7 @@ fp8_gemm_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
   const int m0 = (blockIdx.y / plan.n_tiles) * (GATED ? rows : features), t0 = (blockIdx.y % plan.n_tiles) * NT;
   const int kb0 = (int)((long)sp * p.kb / S), nk = (int)((long)(sp + 1) * p.kb / S) - kb0;
 
+  const int tokens = min(NT, p.N - t0);
   const uint32_t n_scales = (uint32_t)min(NT, (p.N - t0 + 3) & ~3);  // (rows of scales are whole fours)
   auto copy = [&](int i, int s) {  // block i of this CTA's into stage s
     mbar_expect_tx(full + s, STAGE + n_scales * 4u);
@@ -123,7 +129,6 @@ fp8_gemm_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
   if (S > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // (waited for in front of the first word for another CTA)
   pdl_wait();
 
-  const int tokens = min(NT, p.N - t0);
   uint64_t acc[NT / 2];
   if (warp == 0) {
     if (copies) {
@@ -227,34 +232,36 @@ fp8_gemm_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       }
     }
   }
-  // ---- the part to its owners: every MMA has read its operands (a tile in one part lies over the ring), and all CTAs of the cluster are there
-  __syncwarp();
-  if (S > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  // ---- the part over the ring, whose operands every MMA has read, and to its owners
   if (warp >= 3) {
     const int q = warp & 3, h = (warp - 3) >> 2, f = q * 32 + lane;
     if (f < rows) {
-      const int g = h * rows + f;
-      const uint32_t to = smem_u32(received);
-      if constexpr (GATED) {
-        const int shift = 31 - __clz(own);  // (a power of two)
+      const int g = h * rows + f, rank = GATED ? 0 : g / own, step = GATED ? 256 : own;
+      float* to = part + (GATED ? g : rank * NT * own + g - rank * own);
 #pragma unroll
-        for (int c = 0; c < NT; ++c) {
-          const int rank = c >> shift;
-          if (c < tokens) st_cluster(to + (uint32_t)(((sp * own + c - (rank << shift)) * 256 + g) * 4), (uint32_t)(S > 1 ? rank : 0), c & 1 ? hi_of(acc[c / 2]) : lo_of(acc[c / 2]));
-        }
-      } else {
-        const int rank = g / own;
-        const uint32_t mine = to + (uint32_t)((sp * NT * own + g - rank * own) * 4);
-#pragma unroll
-        for (int c = 0; c < NT; ++c) {
-          if (c < tokens) st_cluster(mine + (uint32_t)(c * own * 4), (uint32_t)rank, c & 1 ? hi_of(acc[c / 2]) : lo_of(acc[c / 2]));
-        }
-      }
+      for (int c = 0; c < NT; ++c)
+        if (c < tokens) to[c * step] = c & 1 ? hi_of(acc[c / 2]) : lo_of(acc[c / 2]);
     }
   }
   tc_fence_before();
   __syncthreads();
-  if (S > 1) cluster_barrier();
+  if (S > 1) {
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // all CTAs of the cluster are there
+    const uint32_t to = smem_u32(received);
+    if constexpr (GATED) {
+      for (int i = threadIdx.x; i < tokens * 64; i += THREADS) {
+        const int t = i / 64, r = t / own;
+        st_cluster4(map_to(to + (uint32_t)(((sp * own + t - r * own) * 64 + i % 64) * 16), (uint32_t)r), reinterpret_cast<const float4*>(part)[i]);
+      }
+    } else {
+      const int quads = tokens * own / 4;  // to each
+      for (int r = 0; r < S; ++r)
+        for (int i = threadIdx.x; i < quads; i += THREADS)
+          st_cluster4(map_to(to + (uint32_t)((sp * NT * own + 4 * i) * 4), (uint32_t)r), *reinterpret_cast<const float4*>(part + r * NT * own + 4 * i));
+    }
+    __syncwarp();
+    cluster_barrier();
+  }
   // ---- this CTA's share of the tile, added up in rank order
   auto sum4 = [&](int at, int stride) {  // four features of a token
     float4 t = *reinterpret_cast<const float4*>(received + at);
@@ -365,7 +372,7 @@ FewPlan few_plan(int M, int N, int kb, int na, int nt, bool gated, const int* re
       }
     }
     if (few_smem(na, p, nt, gated) > (size_t)kSmemMost) continue;
-    const size_t part = S == 1 ? (size_t)p.own * (gated ? 256 : nt) * sizeof(float) : 0;  // over the ring
+    const size_t part = (size_t)(gated ? 256 : S * p.own) * nt * sizeof(float);  // over the ring
     const int hold = (int)((part + stage_bytes(na, p.rows, nt) - 1) / stage_bytes(na, p.rows, nt));
     if (hold > p.stages) continue;
     if (p.stages > nk) p.stages = std::max({nk, hold, 1});
