@@ -51,11 +51,13 @@ __device__ __forceinline__ void bulk_copy(void* dst, const void* src, uint32_t b
 struct FewPlan {
   int rows, splits, stages;  // features of a tile of A, parts of K
   int n_tiles;               // tiles of tokens
-  int own;                   // features (gated: tokens) of the tile that a CTA adds up
+  int own;                   // features (gated: tokens, a multiple of four) of the tile that a CTA adds up
 };
 constexpr size_t stage_bytes(int na, int rows, int nt) { return (size_t)(na * rows + nt) * kBK; }
+// floats from one feature of a part to the next: the lanes' 16-byte accesses at one token fall on different banks
+constexpr int part_ld(int nt) { return nt + 4; }
 // parts that a CTA receives
-size_t received_bytes(int na, const FewPlan& p, int nt, bool gated) { return p.splits == 1 ? 0 : (size_t)p.splits * p.own * (gated ? na * p.rows : nt) * sizeof(float); }
+size_t received_bytes(int na, const FewPlan& p, int nt, bool gated) { return p.splits == 1 ? 0 : (size_t)p.splits * p.own * (gated ? na * p.rows : part_ld(nt)) * sizeof(float); }
 size_t few_smem(int na, const FewPlan& p, int nt, bool gated) {
   return p.stages * (stage_bytes(na, p.rows, nt) + nt * sizeof(float)) + (size_t)(kRows - p.rows) * kBK + received_bytes(na, p, nt, gated) + 1024 + (2 * kMaxStages + 4) * 8 + 16;
 }
@@ -77,9 +79,10 @@ fp8_gemm_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
   float* xs = reinterpret_cast<float*>(smem + (size_t)stages * STAGE + (kRows - rows) * kBK);  // [stages][NT] scales of the tokens
   const int S = gridDim.x, sp = (int)cluster_ctarank();  // the cluster spans the whole x axis
   const int features = NA * rows, own = plan.own;
-  float* part = reinterpret_cast<float*>(smem);                // over the ring: [S owners][NT][own features]; gated [NT][256]
-  float* received = S > 1 ? xs + stages * NT : part;           // [S senders][NT][own features]; gated [S][own tokens][256]
-  uint64_t* full = reinterpret_cast<uint64_t*>(xs + stages * NT + (S > 1 ? S * own * (GATED ? 256 : NT) : 0));
+  constexpr int LD = part_ld(NT);
+  float* part = reinterpret_cast<float*>(smem);       // over the ring: [features][LD]
+  float* received = S > 1 ? xs + stages * NT : part;  // [S senders][own features][LD]; gated [S][256][own tokens]
+  uint64_t* full = reinterpret_cast<uint64_t*>(xs + stages * NT + (S > 1 ? S * own * (GATED ? 256 : LD) : 0));
   uint64_t* empty = full + kMaxStages;
   uint64_t* tfull = empty + kMaxStages;  // [2]
   uint64_t* tempty = tfull + 2;          // [2]
@@ -232,86 +235,85 @@ fp8_gemm_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       }
     }
   }
-  // ---- the part over the ring, whose operands every MMA has read, and to its owners
+  // ---- the part over the ring, whose operands every MMA has read, and to its owners.  (What runs once runs from cold instruction memory: few instructions, 16 bytes each.  One word each
+  // took 1.3 us for 64 tokens and 2.8 for 128.)
   if (warp >= 3) {
     const int q = warp & 3, h = (warp - 3) >> 2, f = q * 32 + lane;
     if (f < rows) {
-      const int g = h * rows + f, rank = GATED ? 0 : g / own, step = GATED ? 256 : own;
-      float* to = part + (GATED ? g : rank * NT * own + g - rank * own);
+      float4* to = reinterpret_cast<float4*>(part + (size_t)(h * rows + f) * LD);
 #pragma unroll
-      for (int c = 0; c < NT; ++c)
-        if (c < tokens) to[c * step] = c & 1 ? hi_of(acc[c / 2]) : lo_of(acc[c / 2]);
+      for (int c = 0; c < NT / 4; ++c) to[c] = make_float4(lo_of(acc[2 * c]), hi_of(acc[2 * c]), lo_of(acc[2 * c + 1]), hi_of(acc[2 * c + 1]));
     }
   }
   tc_fence_before();
   __syncthreads();
+  const int fours = (tokens + 3) / 4;  // tokens by fours
   if (S > 1) {
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // all CTAs of the cluster are there
     const uint32_t to = smem_u32(received);
-    if constexpr (GATED) {
-      for (int i = threadIdx.x; i < tokens * 64; i += THREADS) {
-        const int t = i / 64, r = t / own;
-        st_cluster4(map_to(to + (uint32_t)(((sp * own + t - r * own) * 64 + i % 64) * 16), (uint32_t)r), reinterpret_cast<const float4*>(part)[i]);
+    for (int i = threadIdx.x; i < features * fours; i += THREADS) {
+      const int g = i / fours, c = i - g * fours;
+      const float4 v = *reinterpret_cast<const float4*>(part + (size_t)g * LD + 4 * c);
+      if constexpr (GATED) {
+        const int r = 4 * c / own;
+        st_cluster4(map_to(to + (uint32_t)(((sp * 256 + g) * own + 4 * c - r * own) * 4), (uint32_t)r), v);
+      } else {
+        const int r = g / own;
+        st_cluster4(map_to(to + (uint32_t)(((sp * own + g - r * own) * LD + 4 * c) * 4), (uint32_t)r), v);
       }
-    } else {
-      const int quads = tokens * own / 4;  // to each
-      for (int r = 0; r < S; ++r)
-        for (int i = threadIdx.x; i < quads; i += THREADS)
-          st_cluster4(map_to(to + (uint32_t)((sp * NT * own + 4 * i) * 4), (uint32_t)r), *reinterpret_cast<const float4*>(part + r * NT * own + 4 * i));
     }
     __syncwarp();
     cluster_barrier();
   }
-  // ---- this CTA's share of the tile, added up in rank order
-  auto sum4 = [&](int at, int stride) {  // four features of a token
+  // ---- this CTA's share of the tile, added up in rank order: a feature of four tokens at a time
+  auto sum4 = [&](int at, int stride) {
     float4 t = *reinterpret_cast<const float4*>(received + at);
-#pragma unroll
-    for (int r = 1; r < kMaxSplit; ++r)
-      if (r < S) {
-        const float4 v = *reinterpret_cast<const float4*>(received + r * stride + at);
-        t.x += v.x;
-        t.y += v.y;
-        t.z += v.z;
-        t.w += v.w;
-      }
+    for (int r = 1; r < S; ++r) {
+      const float4 v = *reinterpret_cast<const float4*>(received + r * stride + at);
+      t.x += v.x;
+      t.y += v.y;
+      t.z += v.z;
+      t.w += v.w;
+    }
     return t;
   };
   if constexpr (!GATED) {
-    const int quads = (max(0, min(own, features - sp * own))) / 4, items = tokens * quads;
-    O* y = static_cast<O*>(p.y);
-    for (int it = threadIdx.x; it < items; it += THREADS) {
-      const int t = it / quads, j = (it - t * quads) * 4, f = m0 + sp * own + j;
-      if (f >= p.M) continue;
-      const float4 v = sum4(t * own + j, NT * own);
-      O* dst = y + (size_t)(t0 + t) * p.ld_y + f;
-      if (f + 4 <= p.M && (reinterpret_cast<uintptr_t>(dst) & (4 * sizeof(O) - 1)) == 0) {
-        if constexpr (sizeof(O) == 4) *reinterpret_cast<float4*>(dst) = v;
-        else *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
-      } else {
-        const float o[4] = {v.x, v.y, v.z, v.w};
-        for (int e = 0; e < 4 && f + e < p.M; ++e) dst[e] = from_f<O>(o[e]);
-      }
+    const int mine = max(0, min(own, min(features, p.M - m0) - sp * own));
+    O* y = static_cast<O*>(p.y) + (size_t)t0 * p.ld_y + m0 + sp * own;
+    for (int i = threadIdx.x; i < mine * fours; i += THREADS) {
+      const int c = i / mine, g = i - c * mine;
+      const float4 v = sum4(g * LD + 4 * c, own * LD);
+      O* dst = y + (size_t)(4 * c) * p.ld_y + g;
+      const float o[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (4 * c + e < tokens) dst[(size_t)e * p.ld_y] = from_f<O>(o[e]);
     }
   } else {
-    // a warp has a token's 128 features, a block of the result's scales
-    const int mine = min(own, tokens - sp * own);
-    for (int t = warp; t < mine; t += THREADS / 32) {
-      const float4 g = sum4(t * 256 + lane * 4, own * 256), u = sum4(t * 256 + 128 + lane * 4, own * 256);
-      float v[4] = {g.x, g.y, g.z, g.w};
-      const float w[4] = {u.x, u.y, u.z, u.w};
+    // a warp has four tokens' 128 features, a block of the result's scales each: a lane every 32nd feature
+    const int mine = max(0, min(own, tokens - sp * own)), ld = S > 1 ? own : LD;
+    for (int c = warp; 4 * c < mine; c += THREADS / 32) {
+      float v[4][4];  // [feature][token]
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = (p.act == 0 ? gate_act<0>(v[e]) : p.act == 1 ? gate_act<1>(v[e]) : gate_act<2>(v[e])) * w[e];
-      const float m = max16(max_abs(max_abs(v[0], v[1], v[2]), v[3]));
-      const Scale k = scale_of(max_abs(m, __shfl_xor_sync(0xffffffffu, m, 16)));
-      const uint32_t c = codes4(v, k);
-      const int f = m0 + lane * 4, tok = t0 + sp * own + t;
-      uint8_t* dst = p.codes + (size_t)tok * p.ld + f;
-      if (f + 4 <= p.M) {
-        *reinterpret_cast<uint32_t*>(dst) = c;
-      } else {
-        for (int e = 0; e < 4 && f + e < p.M; ++e) dst[e] = (uint8_t)(c >> (8 * e));
+      for (int j = 0; j < 4; ++j) {
+        const float4 g = sum4((lane + 32 * j) * ld + 4 * c, 256 * ld), u = sum4((128 + lane + 32 * j) * ld + 4 * c, 256 * ld);
+        const float a[4] = {g.x, g.y, g.z, g.w}, b[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[j][e] = (p.act == 0 ? gate_act<0>(a[e]) : p.act == 1 ? gate_act<1>(a[e]) : gate_act<2>(a[e])) * b[e];
       }
-      if (lane == 0) p.scales[(size_t)(m0 / kBlock) * p.ld_s + tok] = k.s;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int tok = t0 + sp * own + 4 * c + e;
+        const float m = max16(max_abs(max_abs(v[0][e], v[1][e], v[2][e]), v[3][e]));
+        const Scale k = scale_of(max_abs(m, __shfl_xor_sync(0xffffffffu, m, 16)));
+        if (4 * c + e >= mine) continue;
+        const uint32_t lo = codes2(v[0][e], v[1][e], k), hi = codes2(v[2][e], v[3][e], k);
+        uint8_t* dst = p.codes + (size_t)tok * p.ld + m0 + lane;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (m0 + lane + 32 * j < p.M) dst[32 * j] = (uint8_t)((j < 2 ? lo : hi) >> (8 * (j & 1)));
+        if (lane == 0) p.scales[(size_t)(m0 / kBlock) * p.ld_s + tok] = k.s;
+      }
     }
   }
   if (threadIdx.x == 0) count_run_out(dead, p.err);  // (every wait lies before the barrier above)
@@ -360,7 +362,7 @@ FewPlan few_plan(int M, int N, int kb, int na, int nt, bool gated, const int* re
       const long m_tiles = std::max<long>(1, waves * at_once / n_tiles);  // that the waves have room for
       p.rows = (int)std::min<long>(kRows, std::max<long>(32, ((M + m_tiles * na - 1) / (m_tiles * na) + 7) / 8 * 8));
     }
-    p.own = gated ? std::max(1, nt / S) : ((na * p.rows / 4 + S - 1) / S) * 4;
+    p.own = gated ? std::max(4, nt / S) : (na * p.rows + S - 1) / S;
     const int nk = (kb + S - 1) / S;
     const double block = std::max(300., (double)stage_bytes(na, p.rows, nt) / 55);
     const double cost = (double)waves * (nk * block + 3000) + (S > 1 ? 1000 : 0);
@@ -372,7 +374,7 @@ FewPlan few_plan(int M, int N, int kb, int na, int nt, bool gated, const int* re
       }
     }
     if (few_smem(na, p, nt, gated) > (size_t)kSmemMost) continue;
-    const size_t part = (size_t)(gated ? 256 : S * p.own) * nt * sizeof(float);  // over the ring
+    const size_t part = (size_t)na * p.rows * part_ld(nt) * sizeof(float);  // over the ring
     const int hold = (int)((part + stage_bytes(na, p.rows, nt) - 1) / stage_bytes(na, p.rows, nt));
     if (hold > p.stages) continue;
     if (p.stages > nk) p.stages = std::max({nk, hold, 1});
