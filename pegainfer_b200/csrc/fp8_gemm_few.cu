@@ -19,7 +19,7 @@ namespace fp8 {
 
 namespace {
 
-constexpr int kRows = 128, kMaxSplit = 8, kMaxStages = 12;  // 8: the portable cluster size
+constexpr int kRows = 128, kMaxStages = 12;
 constexpr int kSmemMost = 227 * 1024;
 // A CTA asks for more than half of an SM's shared memory, so it is alone with its kind, and for more than any kernel with all 512 columns of tensor memory leaves: whoever is resident has
 // its columns at once.  (CTAs that wait for columns while the rest of their cluster waits for them could wait for one another.)
@@ -63,12 +63,15 @@ size_t few_smem(int na, const FewPlan& p, int nt, bool gated) {
 }
 constexpr int tmem_columns(int na, int nt) { return 2 * na * nt <= 32 ? 32 : 2 * na * nt <= 64 ? 64 : 2 * na * nt <= 128 ? 128 : 2 * na * nt <= 256 ? 256 : 512; }
 
+// groups of four warps that take sums out of tensor memory: one to a tile of A, two where one tile has many columns (128 tokens: a block takes one group 530 ns)
+constexpr int groups(int na, int nt) { return na == 1 && nt >= 64 ? 2 : na; }
+
 // GATED: NA = 2, O is the codes' type
 template <int NT, int NA, bool GATED, typename O>
-__global__ void __launch_bounds__(96 + 128 * NA, 1)
+__global__ void __launch_bounds__(96 + 128 * groups(NA, NT), 1)
 fp8_gemm_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_w2, const Product p,
                     const FewPlan plan) {
-  constexpr int THREADS = 96 + 128 * NA;
+  constexpr int GROUPS = groups(NA, NT), COLS = NA == 2 ? NT : NT / GROUPS, THREADS = 96 + 128 * GROUPS;  // COLS: columns of a thread
   constexpr uint32_t TMEM_COLS = tmem_columns(NA, NT);
   static_assert(2 * NA * NT <= 512 && (!GATED || NA == 2), "tensor memory");
     const int stages = plan.stages, rows = plan.rows;
@@ -112,11 +115,11 @@ fp8_gemm_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     asm volatile("prefetch.tensormap [%0];" ::"l"(&map_x) : "memory");
     for (int s = 0; s < stages; ++s) {
       mbar_init(full + s, 1);
-      mbar_init(empty + s, 4 * NA);  // the warps that read the scales, behind the MMAs' end
+      mbar_init(empty + s, 4 * GROUPS);  // the warps that read the scales, behind the MMAs' end
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(tfull + s, 1);
-      mbar_init(tempty + s, 4 * NA);
+      mbar_init(tempty + s, 4 * GROUPS);
     }
     *dead = 0;
     mbar_fence_init();
@@ -132,7 +135,7 @@ fp8_gemm_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
   if (S > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // (waited for in front of the first word for another CTA)
   pdl_wait();
 
-  uint64_t acc[NT / 2];
+  uint64_t acc[COLS / 2];
   if (warp == 0) {
     if (copies) {
       int s = 0, i = stages;
@@ -184,11 +187,11 @@ fp8_gemm_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     }
     __syncwarp();
   } else {
-    const int q = warp & 3, h = (warp - 3) >> 2, f = q * 32 + lane;  // tensor-memory lanes that this warp may read; lane = feature
+    const int q = warp & 3, group = (warp - 3) >> 2, h = NA == 2 ? group : 0, c0 = NA == 2 ? 0 : group * COLS, f = q * 32 + lane;  // tensor-memory lanes that this warp may read; lane = feature
     const int at = m0 + (GATED ? f : h * rows + f), row = at < p.M ? at : p.M - 1;
     const float* sw = (GATED && h == 1 ? p.sw2 : p.sw) + (size_t)(row / kBlock) * p.kb + kb0;
 #pragma unroll
-    for (int j = 0; j < NT / 2; ++j) acc[j] = 0;
+    for (int j = 0; j < COLS / 2; ++j) acc[j] = 0;
     float w_next = __ldg(sw);
     int s = 0;
     uint32_t ph = 0;
@@ -201,7 +204,7 @@ fp8_gemm_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       if (!here) mbar_wait_bounded(full + s, ph, dead);  // (the scales)
       if (!done) mbar_wait_bounded(tfull + buf, tph, dead);
       tc_fence_after();
-      const uint32_t t0 = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)((buf * NA + h) * NT);
+      const uint32_t t0 = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)((buf * NA + h) * NT + c0);
       auto release = [&]() {
         tc_fence_before();
         __syncwarp();
@@ -214,17 +217,17 @@ fp8_gemm_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
         acc[at / 2] = fma2(pair_of(u[0], u[1]), mul2(w, pair_of(x.x, x.y)), acc[at / 2]);
         acc[at / 2 + 1] = fma2(pair_of(u[2], u[3]), mul2(w, pair_of(x.z, x.w)), acc[at / 2 + 1]);
       };
-      auto scale4 = [&](int at) { return *reinterpret_cast<const float4*>(xs + s * NT + at); };
+      auto scale4 = [&](int at) { return *reinterpret_cast<const float4*>(xs + s * NT + c0 + at); };
       uint32_t v[2][16];
       tmem_ld16(t0, v[0]);
 #pragma unroll
-      for (int c = 0; c < NT; c += 16) {
+      for (int c = 0; c < COLS; c += 16) {
         float4 x[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) x[j] = scale4(c + 4 * j);
         uint32_t* now = v[(c / 16) & 1];
         tmem_wait16(now);
-        if (c + 16 < NT) tmem_ld16(t0 + (uint32_t)(c + 16), v[(c / 16 + 1) & 1]);
+        if (c + 16 < COLS) tmem_ld16(t0 + (uint32_t)(c + 16), v[(c / 16 + 1) & 1]);
         else release();
 #pragma unroll
         for (int j = 0; j < 4; ++j) add4(c + 4 * j, now + 4 * j, x[j]);
@@ -238,11 +241,11 @@ fp8_gemm_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
   // ---- the part over the ring, whose operands every MMA has read, and to its owners.  (What runs once runs from cold instruction memory: few instructions, 16 bytes each.  One word each
   // took 1.3 us for 64 tokens and 2.8 for 128.)
   if (warp >= 3) {
-    const int q = warp & 3, h = (warp - 3) >> 2, f = q * 32 + lane;
+    const int q = warp & 3, group = (warp - 3) >> 2, h = NA == 2 ? group : 0, c0 = NA == 2 ? 0 : group * COLS, f = q * 32 + lane;
     if (f < rows) {
-      float4* to = reinterpret_cast<float4*>(part + (size_t)(h * rows + f) * LD);
+      float4* to = reinterpret_cast<float4*>(part + (size_t)(h * rows + f) * LD + c0);
 #pragma unroll
-      for (int c = 0; c < NT / 4; ++c) to[c] = make_float4(lo_of(acc[2 * c]), hi_of(acc[2 * c]), lo_of(acc[2 * c + 1]), hi_of(acc[2 * c + 1]));
+      for (int c = 0; c < COLS / 4; ++c) to[c] = make_float4(lo_of(acc[2 * c]), hi_of(acc[2 * c]), lo_of(acc[2 * c + 1]), hi_of(acc[2 * c + 1]));
     }
   }
   tc_fence_before();
@@ -392,7 +395,7 @@ int run_few(const Product& p, cudaStream_t st) {
   static std::atomic<uint64_t> set{0};
   if (const cudaError_t e = allow_smem(set, (const void*)kern, kSmemMost); e != cudaSuccess) return (int)e;
   cudaLaunchConfig_t cfg{};
-  cfg.blockDim = dim3(96 + 128 * NA);
+  cfg.blockDim = dim3(96 + 128 * groups(NA, NT));
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.y = 1;
