@@ -73,9 +73,8 @@ inline bool make_codes_map(CUtensorMap* map, const void* base, long rows, int K,
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// fp8_gemm_few.cu: whether it takes a call, and the call
-bool few_takes(const Product& p, bool gated);
-int launch_few(const Product& p, bool gated, bool y_f32, cudaStream_t st);
+// fp8_gemm_few.cu; -2: not one of its sizes, or it takes longer than within_ns
+int launch_few(const Product& p, bool gated, bool y_f32, double within_ns, cudaStream_t st);
 
 }  // namespace fp8
 }  // namespace pk

@@ -52,6 +52,7 @@ struct FewPlan {
   int rows, splits, stages;  // features of a tile of A, parts of K
   int n_tiles;               // tiles of tokens
   int own;                   // features (gated: tokens, a multiple of four) of the tile that a CTA adds up
+  double ns;                 // what a call takes, about
 };
 constexpr size_t stage_bytes(int na, int rows, int nt) { return (size_t)(na * rows + nt) * kBK; }
 // floats from one feature of a part to the next: the lanes' 16-byte accesses at one token fall on different banks
@@ -71,7 +72,7 @@ template <int NT, int NA, bool GATED, typename O>
 __global__ void __launch_bounds__(96 + 128 * groups(NA, NT), 1)
 fp8_gemm_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_w2, const Product p,
                     const FewPlan plan) {
-  constexpr int GROUPS = groups(NA, NT), COLS = NA == 2 ? NT : NT / GROUPS, THREADS = 96 + 128 * GROUPS;  // COLS: columns of a thread
+  constexpr int GROUPS = groups(NA, NT), COLS = NT * NA / GROUPS, THREADS = 96 + 128 * GROUPS;  // COLS: columns of a thread
   constexpr uint32_t TMEM_COLS = tmem_columns(NA, NT);
   static_assert(2 * NA * NT <= 512 && (!GATED || NA == 2), "tensor memory");
     const int stages = plan.stages, rows = plan.rows;
@@ -187,7 +188,7 @@ fp8_gemm_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     }
     __syncwarp();
   } else {
-    const int q = warp & 3, group = (warp - 3) >> 2, h = NA == 2 ? group : 0, c0 = NA == 2 ? 0 : group * COLS, f = q * 32 + lane;  // tensor-memory lanes that this warp may read; lane = feature
+    const int q = warp & 3, group = (warp - 3) >> 2, h = group % NA, c0 = group / NA * COLS, f = q * 32 + lane;  // tensor-memory lanes that this warp may read; lane = feature
     const int at = m0 + (GATED ? f : h * rows + f), row = at < p.M ? at : p.M - 1;
     const float* sw = (GATED && h == 1 ? p.sw2 : p.sw) + (size_t)(row / kBlock) * p.kb + kb0;
 #pragma unroll
@@ -241,7 +242,7 @@ fp8_gemm_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
   // ---- the part over the ring, whose operands every MMA has read, and to its owners.  (What runs once runs from cold instruction memory: few instructions, 16 bytes each.  One word each
   // took 1.3 us for 64 tokens and 2.8 for 128.)
   if (warp >= 3) {
-    const int q = warp & 3, group = (warp - 3) >> 2, h = NA == 2 ? group : 0, c0 = NA == 2 ? 0 : group * COLS, f = q * 32 + lane;
+    const int q = warp & 3, group = (warp - 3) >> 2, h = group % NA, c0 = group / NA * COLS, f = q * 32 + lane;
     if (f < rows) {
       float4* to = reinterpret_cast<float4*>(part + (size_t)(h * rows + f) * LD + c0);
 #pragma unroll
@@ -348,17 +349,17 @@ cudaError_t clusters_at_once(const void* kern, cudaLaunchConfig_t cfg, cudaLaunc
   return cudaSuccess;
 }
 
-// Parts of K, features of a tile, stages.  A block of K takes a CTA as long as its bytes (55 of them a ns and SM where all SMs stream) or 0.3 us for its chain copy -> MMAs -> sum, a cluster's
-// joining 1 us; resident[i]: clusters of 2^i CTAs that the GPU has at once.  The lowest tiles for which the number of waves stays, so that every SM has the same share.
+// Parts of K, features of a tile, stages, and about how many ns that takes: 4.5 us for the launch, the first copies and the end; a block of K as long as its bytes take (55 of them a ns and
+// SM where all SMs stream) or its chain copy -> MMAs -> sum; the joining of a cluster 0.8 us and 20 bytes of a part a ns.  resident[i]: clusters of 2^i CTAs that the GPU has at once.
+// The lowest tiles for which the number of waves stays, so that every SM has the same share.
 FewPlan few_plan(int M, int N, int kb, int na, int nt, bool gated, const int* resident) {
   const int per_tile = gated ? kRows : na * kRows, n_tiles = (N + nt - 1) / nt;
   FewPlan best{};
-  double least = 0;
   for (int i = 0; i < 4; ++i) {
     const int S = 1 << i;
     if (S > 1 && (S > kb / 2 || resident[i] < 1 || (!gated && na == 2))) continue;  // at least two blocks a part
     const int at_once = std::max(1, resident[i]);
-    FewPlan p{kRows, S, 2, n_tiles, 0};
+    FewPlan p{kRows, S, 2, n_tiles, 0, 0};
     const long tiles = (long)((M + per_tile - 1) / per_tile) * n_tiles;
     const long waves = (tiles + at_once - 1) / at_once;
     if (!gated) {
@@ -367,8 +368,6 @@ FewPlan few_plan(int M, int N, int kb, int na, int nt, bool gated, const int* re
     }
     p.own = gated ? std::max(4, nt / S) : (na * p.rows + S - 1) / S;
     const int nk = (kb + S - 1) / S;
-    const double block = std::max(300., (double)stage_bytes(na, p.rows, nt) / 55);
-    const double cost = (double)waves * (nk * block + 3000) + (S > 1 ? 1000 : 0);
     while (p.stages < kMaxStages) {
       ++p.stages;
       if (few_smem(na, p, nt, gated) > (size_t)kSmemMost) {
@@ -381,16 +380,16 @@ FewPlan few_plan(int M, int N, int kb, int na, int nt, bool gated, const int* re
     const int hold = (int)((part + stage_bytes(na, p.rows, nt) - 1) / stage_bytes(na, p.rows, nt));
     if (hold > p.stages) continue;
     if (p.stages > nk) p.stages = std::max({nk, hold, 1});
-    if (best.splits == 0 || cost < least) {
-      best = p;
-      least = cost;
-    }
+    const double block = std::max(nt > 64 ? 400. : 300., (double)stage_bytes(na, p.rows, nt) / 55);
+    p.ns = 4500 + (double)waves * (nk * block + (S > 1 ? 800 + (double)part / 20 : 0)) + (waves - 1) * 2500.;
+    if (best.splits == 0 || p.ns < best.ns) best = p;
   }
   return best;
 }
 
+// within_ns: what another kernel takes; -2: that is the faster one
 template <int NT, int NA, bool GATED, typename O>
-int run_few(const Product& p, cudaStream_t st) {
+int run_few(const Product& p, double within_ns, cudaStream_t st) {
   auto kern = fp8_gemm_few_kernel<NT, NA, GATED, O>;
   static std::atomic<uint64_t> set{0};
   if (const cudaError_t e = allow_smem(set, (const void*)kern, kSmemMost); e != cudaSuccess) return (int)e;
@@ -407,8 +406,9 @@ int run_few(const Product& p, cudaStream_t st) {
   int resident[4];
   if (const cudaError_t e = clusters_at_once((const void*)kern, cfg, attr[0], resident); e != cudaSuccess) return (int)e;
   const FewPlan plan = few_plan(p.M, p.N, p.kb, NA, NT, GATED, resident);
+  if (plan.splits == 0 || plan.ns > within_ns) return -2;
   CUtensorMap mx, mw, mw2;
-  if (plan.splits == 0 || !make_codes_map(&mx, p.x, p.N, p.K, p.ld_x, NT) || !make_codes_map(&mw, p.w, p.M, p.K, p.ld_w, plan.rows) ||
+  if (!make_codes_map(&mx, p.x, p.N, p.K, p.ld_x, NT) || !make_codes_map(&mw, p.w, p.M, p.K, p.ld_w, plan.rows) ||
       !make_codes_map(&mw2, GATED ? p.w2 : p.w, p.M, p.K, p.ld_w, plan.rows))
     return (int)cudaErrorInvalidValue;
   const int per_tile = GATED ? plan.rows : NA * plan.rows;
@@ -423,20 +423,18 @@ int run_few(const Product& p, cudaStream_t st) {
 
 }  // namespace
 
-bool few_takes(const Product& p, bool gated) { return p.N <= (gated ? 64 : 128) && (p.M + 31) / 32 <= 65535; }  // (tiles are counted on a grid's second axis)
-
-int launch_few(const Product& p, bool gated, bool y_f32, cudaStream_t st) {
+int launch_few(const Product& p, bool gated, bool y_f32, double within_ns, cudaStream_t st) {
+  if (p.N > 1024 || (p.M + 31) / 32 * ((p.N + 63) / 64) > 65535) return -2;  // (tiles are counted on a grid's second axis)
   if (gated) {
-    if (p.N <= 16) return run_few<16, 2, true, uint8_t>(p, st);
-    if (p.N <= 32) return run_few<32, 2, true, uint8_t>(p, st);
-    return run_few<64, 2, true, uint8_t>(p, st);
+    if (p.N <= 16) return run_few<16, 2, true, uint8_t>(p, within_ns, st);
+    if (p.N <= 32) return run_few<32, 2, true, uint8_t>(p, within_ns, st);
+    return run_few<64, 2, true, uint8_t>(p, within_ns, st);
   }
-  auto go = [&](auto f, auto b) { return y_f32 ? f(p, st) : b(p, st); };
+  auto go = [&](auto f, auto b) { return y_f32 ? f(p, within_ns, st) : b(p, within_ns, st); };
   if (p.M > kRows * sm_count()) {  // two tiles of features a CTA: fewer CTAs that read all of X
     if (p.N <= 16) return go(run_few<16, 2, false, float>, run_few<16, 2, false, bf16>);
     if (p.N <= 32) return go(run_few<32, 2, false, float>, run_few<32, 2, false, bf16>);
-    if (p.N <= 64) return go(run_few<64, 2, false, float>, run_few<64, 2, false, bf16>);
-    return go(run_few<128, 2, false, float>, run_few<128, 2, false, bf16>);
+    return go(run_few<64, 2, false, float>, run_few<64, 2, false, bf16>);
   }
   if (p.N <= 16) return go(run_few<16, 1, false, float>, run_few<16, 1, false, bf16>);
   if (p.N <= 32) return go(run_few<32, 1, false, float>, run_few<32, 1, false, bf16>);
