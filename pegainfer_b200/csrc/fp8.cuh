@@ -12,6 +12,7 @@ namespace pk {
 namespace fp8 {
 
 constexpr int kBlock = 128;
+constexpr float kLeast = 7.888609e-31f;  // 2^-100
 constexpr int kAct = 5;  // kinds of pk_fp8_act
 
 inline bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -67,7 +68,7 @@ struct Scale {
 // amax / 448 to its nearest fp32 number: a product and a step of Newton's, whose remainder is exact
 __device__ __forceinline__ Scale scale_of(float amax) {
   constexpr float kTo = 1.f / 448.f;
-  const float a = amax < 7.888609e-31f ? 7.888609e-31f : amax - (amax - amax);  // (an infinity becomes NaN)
+  const float a = amax < kLeast ? kLeast : amax - (amax - amax);  // (an infinity becomes NaN)
   const float s = a * kTo;
   Scale r;
   r.s = fmaf(fmaf(-s, 448.f, a), kTo, s);

@@ -7,6 +7,7 @@ namespace fp8 {
 
 // x += y (rounded when stored), v = x * rsqrt(mean(x^2) + eps) * (offset + w) of the unrounded x, quantised.  A CTA has a row, in registers from its load to its codes, NV pieces of 8
 // entries a thread and as many warps as that takes.
+// A code is v over its block's largest v, in which the root cancels: codes come from x * (offset + w), with two roundings less, and only the scales wait for the row's sum.
 constexpr int kNormWarps = 32, kNormWidest = kNormWarps * 256 * 2;
 
 template <typename E, int NV, bool VEC>
@@ -37,11 +38,19 @@ __global__ void __launch_bounds__(32 * kNormWarps) fp8_add_norm_kernel(const bf1
       store8<VEC>(x + base + at, width - at, v[j]);
     }
   }
-  float ss = 0.f;
+  float ss = 0.f, m[NV];
 #pragma unroll
-  for (int j = 0; j < NV; ++j)
+  for (int j = 0; j < NV; ++j) {
+    const int at = (j * blockDim.x + threadIdx.x) * 8;
+    float g[8];
+    load8<VEC>(w + at, width - at, g);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) ss = fmaf(v[j][e], v[j][e], ss);
+    for (int e = 0; e < 8; ++e) {
+      ss = fmaf(v[j][e], v[j][e], ss);
+      v[j][e] = at + e < width ? v[j][e] * (offset + g[e]) : 0.f;
+    }
+    m[j] = max16(max8(v[j]));
+  }
   ss = warp_sum(ss);
   if (warps > 1) {
     if (lane == 0) red[warp] = ss;
@@ -52,16 +61,16 @@ __global__ void __launch_bounds__(32 * kNormWarps) fp8_add_norm_kernel(const bf1
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     const int at = (j * blockDim.x + threadIdx.x) * 8;
-    if (at - (at & 255) >= width) break;  // (a warp at a time: its lanes find a maximum together)
-    float g[8];
-    load8<VEC>(w + at, width - at, g);
+    if (at >= width) break;
+    const Scale k = scale_of(m[j] * r);
+    if (m[j] * r > kLeast) {
+      store_codes8(codes + t * ld + at, width - at, v[j], scale_of(m[j]));
+    } else {  // the least scale, or none (NaN)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[j][e] = at + e < width ? v[j][e] * r * (offset + g[e]) : 0.f;  // (an r that is not finite stays inside the row)
-    const Scale k = scale_of(max16(max8(v[j])));
-    if (at < width) {
+      for (int e = 0; e < 8; ++e) v[j][e] *= r;
       store_codes8(codes + t * ld + at, width - at, v[j], k);
-      if ((lane & 15) == 0) scales[(size_t)(at / kBlock) * ld_s + t] = k.s;
     }
+    if ((lane & 15) == 0) scales[(size_t)(at / kBlock) * ld_s + t] = k.s;
   }
 }
 
