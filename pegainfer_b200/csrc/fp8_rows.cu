@@ -161,7 +161,7 @@ extern "C" int pk_fp8_act(const void* in, long ld_in, int kind, void* codes, lon
     return -1;
   const long from = ld_in ? ld_in : need;
   if (F > 1 << 30 || (long)tokens * fp8::blocks_of(F) > 1L << 34) return -2;  // (the grid's CTAs are counted in 31 bits)
-  const bool vec = (F % 8 == 0 || kind == 1 || kind == 4) && from % 8 == 0 && fp8::al16(in);
+  const bool vec = F % 8 == 0 && from % 8 == 0 && fp8::al16(in);
   auto go = [&](auto f) { return (int)f((const bf16*)in, from, (uint8_t*)codes, ld, scales, ld_s, F, tokens, vec, st); };
   switch (kind) {
     case 0: return go(fp8::act<0>);

@@ -113,6 +113,27 @@ def test_act(lib, kind, T, F, pad):
     untouched(codes, scales, T, F)
 
 
+@pytest.mark.parametrize("kind", range(5))
+def test_act_reads_nothing_behind_a_row(lib, kind):
+    """rows of an odd width whose strides are whole vectors: NaN wherever nothing may be read"""
+    T, F = 5, 125
+    n = F * (1 if kind in (1, 4) else 2)
+    x = torch.full((T, R.up(n, 8)), math.nan, device="cuda").to(BF16)
+    x[:, :n] = rn(gen(kind, 8), T, n).to(BF16)
+    codes, scales = out_rows(T, F)
+    assert lib.pk_fp8_act(x.data_ptr(), x.shape[1], kind, codes.data_ptr(), codes.shape[1], scales.data_ptr(), scales.shape[1], F, T, st()) == 0
+    R.hold_rows(codes, scales, R.act(kind, x[:, :F].double(), x[:, F:2 * F].double()), rel=2.0 ** -16)
+
+
+@pytest.mark.parametrize("f32", [False, True])
+def test_weights_read_nothing_behind_a_row(lib, f32):
+    w = torch.full((130, 136), math.nan, device="cuda").to(F32 if f32 else BF16)
+    w[:, :130] = rn(gen(f32, 9), 130, 130).to(w.dtype)
+    codes, scales = torch.zeros(130, 144, dtype=U8, device="cuda"), torch.empty(2, 2, device="cuda")
+    assert lib.pk_fp8_weights(w.data_ptr(), int(f32), 136, codes.data_ptr(), 144, scales.data_ptr(), 130, 130, st()) == 0
+    R.hold_weights(codes, scales, w[:, :130].double())
+
+
 def test_act_of_entries_that_are_not_finite(lib):
     F = 400
     x = rn(gen(3), 5, F).to(BF16)
@@ -210,6 +231,15 @@ def test_gemm(lib, T, M, K):
         near(gemm(lib, ops, T, M, K, f32), *R.product(*ops, T, M, K))
 
 
+@pytest.mark.parametrize("T,M,K", [(129, 300, 3333), (200, 513, 4096), (300, 500, 8000), (777, 130, 5000), (1000, 64, 2560), (1024, 100, 9000), (1025, 100, 9000), (513, 40, 128), (70, 19000, 200),
+                                   (64, 19000, 300), (33, 37889, 128), (16, 20001, 700)])
+def test_gemm_of_many_parts_and_tiles(lib, T, M, K):
+    """long reductions of few features are cut into parts however many tokens there are; many features go two tiles to a CTA, in waves"""
+    for f32 in (False, True):
+        ops = operands(T, M, K, gen(T, M, K))
+        near(gemm(lib, ops, T, M, K, f32, ld=M + 1), *(torch.nn.functional.pad(v, (0, 1), value=7.0 * i) for i, v in zip((1, 0), R.product(*ops, T, M, K))))
+
+
 @pytest.mark.parametrize("T", [1, 7, 40, 90, 300])
 @pytest.mark.parametrize("M,ld,off", [(256, 264, 0), (512, 515, 0), (300, 300, 1), (64, 0, 3), (640, 641, 2)])
 @pytest.mark.parametrize("f32", [False, True])
@@ -286,6 +316,16 @@ def test_gated(lib, T, M, K):
     act = (T + M) % 3
     codes, scales = gated(lib, ops, w2, T, M, K, act, more=T % 2)
     hold_gated(codes, scales, ops, w2, T, M, K, act)
+    untouched(codes, scales, T, M)
+
+
+@pytest.mark.parametrize("T,M,K", [(100, 640, 8192), (130, 128, 4000), (300, 257, 5000), (1000, 128, 3333), (64, 19000, 256)])
+def test_gated_of_many_parts_and_tiles(lib, T, M, K):
+    g = gen(T, M, K)
+    ops = operands(T, M, K, g)
+    w2 = operands(1, M, K, g)[2:]
+    codes, scales = gated(lib, ops, w2, T, M, K, T % 3, more=1)
+    hold_gated(codes, scales, ops, w2, T, M, K, T % 3)
     untouched(codes, scales, T, M)
 
 
@@ -423,3 +463,40 @@ def test_with_dependent_launches(lib):
             assert torch.equal(f.step(x.clone(), y, f.buffers(9)), want)
     finally:
         lib.pk_b200_set_pdl(0)
+
+
+FIRST = """
+import torch
+from pegainfer_b200 import ffi
+from tests import fp8_ref as R
+lib = ffi.lib()
+lib.cuda_set_device(0)
+lib.cublas_init()
+cases = []
+for T in (4, 500):
+    xc, xs = R.quant_rows(torch.randn(T, 700, device="cuda"))
+    wc, ws = R.quant_weights(torch.randn(900, 700, device="cuda"))
+    y = torch.zeros(T, 900, device="cuda")
+    cases.append((T, xc, xs, wc, ws, y))
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    s = torch.cuda.current_stream().cuda_stream
+    for T, xc, xs, wc, ws, y in cases:
+        assert lib.pk_fp8_gemm(wc.data_ptr(), wc.shape[1], ws.data_ptr(), xc.data_ptr(), xc.shape[1], xs.data_ptr(), xs.shape[1], y.data_ptr(), 0, 1, 900, T, 700, s) == 0
+graph.replay()
+torch.cuda.synchronize()
+for T, xc, xs, wc, ws, y in cases:
+    want, size = R.product(xc, xs, wc, ws, T, 900, 700)
+    assert ((y.double() - want).abs() <= size * R.SUM).all()
+print("captured first")
+"""
+
+
+def test_the_first_call_of_a_process_may_be_captured():
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    run = subprocess.run([sys.executable, "-c", FIRST], cwd=root, env=dict(os.environ, PYTHONPATH=root), capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and "captured first" in run.stdout, run.stdout[-2000:] + run.stderr[-4000:]
