@@ -41,6 +41,23 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
   return r;
 }
 
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// by the special-function unit (2^-22); results below 2^-126 are zero
+__device__ __forceinline__ float rcp_ftz(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float exp2_ftz(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+
 // the largest magnitude; infinities and NaN stay
 __device__ __forceinline__ float max_abs(float a, float b) {
   float r;
@@ -72,7 +89,7 @@ __device__ __forceinline__ Scale scale_of(float amax) {
   const float s = a * kTo;
   Scale r;
   r.s = fmaf(fmaf(-s, 448.f, a), kTo, s);
-  asm("rcp.approx.f32 %0, %1;" : "=f"(r.inv) : "f"(r.s));
+  r.inv = rcp_ftz(r.s);  // (2^-109 to 2^120)
   return r;
 }
 // codes of v / s, each quotient to its nearest fp32 number: v * (1 / s) and the same step, whose remainder v - q s is exact.  Without it a quotient that lies just between two codes,
@@ -151,12 +168,14 @@ __device__ __forceinline__ void store_codes8(uint8_t* p, int n, const float* v, 
   }
 }
 
-// act 0 SiLU, 1 ReLU, 2 GELU in its tanh form, of z; fp32, the exponential by the special-function unit (2^-22)
+// act 0 SiLU, 1 ReLU, 2 GELU in its tanh form, of z: z times the logistic function of z or of sqrt(8 / pi) (z + 0.044715 z^3).  The special-function unit's exponential and quotient
+// without their ways for subnormal numbers, which took half of the instructions; what they lose lies below the least scale's codes.
 template <int ACT>
 __device__ __forceinline__ float gate_act(float z) {
   if constexpr (ACT == 1) return z < 0.f ? 0.f : z;  // (NaN stays)
-  if constexpr (ACT == 2) return __fdividef(z, 1.f + __expf(-1.5957691216057308f * (z + 0.044715f * z * z * z)));
-  return __fdividef(z, 1.f + __expf(-z));
+  constexpr float kLog2e = 1.4426950408889634f, kGelu = -1.5957691216057308f * kLog2e;
+  const float x = ACT == 2 ? z * fmaf(z * z, 0.044715f * kGelu, kGelu) : z * -kLog2e;
+  return z * rcp_ftz(1.f + exp2_ftz(x));
 }
 
 }  // namespace fp8

@@ -2,12 +2,19 @@
 //
 // A pair (cluster of two, tcgen05 cta_group::2) has a tile of 256 tokens x 256 features: A = X, 128 tokens to a CTA, B = W, half the features to a CTA.
 //   warp 0     TMA producer (both CTAs): 128 entries of K a stage, completing on the leader's barrier
-//   warp 1     MMA issuer (leader): a block of K is two products (M 256, N 128: the tile's halves) of four tcgen05.mma each, into partial sums in tensor memory, two of each half
-//   warps 2, 3 the scales of even and odd blocks of K into shared memory, a token's times the weights'
-//   warps 4-19 (eight to a half) take a half's partial sum out of tensor memory while the others are computed and add it, times its scale, to the tile's sum, which they hold in registers
-//              (thread = token, 64 features): half an instruction an entry (fma.rn.f32x2)
-// Gated: B is 128 rows of w (leader) and the same 128 of w2 (peer); a half is 64 features of both, a thread has 32 features of both; 128 features are a block of the result's
-// scales, whose largest magnitude four threads find together.
+//   warp 1     MMA issuer (leader): a block of K is four tcgen05.mma (M 256, N 256, K 32) into one of two partial sums, all of tensor memory
+//   warps 2, 3 the scales of even and odd blocks of K into shared memory, a token's times the weights'; they see a block's MMAs end and give its stage back
+//   warps 4-19 take a partial sum out of tensor memory while the other is computed and add it, times its scale, to the tile's sum, which they hold in registers (thread = token, 64 features);
+//              a finished tile leaves through shared memory by TMA
+// Gated: B is 128 rows of w (leader) and the same 128 of w2 (peer), so a thread has 32 features of both; 128 features are a block of the result's scales, whose largest magnitude four threads
+// find together.
+//
+// What bounds it, B200, 4096 tokens of 24576 x 4096 (825 GFLOP), us: 380 alone (2.17 PFLOP/s; 443 at the clocks of seconds under the power limit).  A block of K takes a tile 950 clocks, its
+// MMAs 512.  Without the sums' work 312, with half of the operands' bytes 324, without both 244: a partial sum's way (MMAs, commit, 64 columns out and added by 16 warps, arrival in the other
+// CTA: 1800 clocks, two of them under way) and the 32 KB a CTA reads of L2 for it (34 bytes a clock and SM) bound it together.  What it took to come here: 770 with a release at the cluster's scope in
+// the arrivals, 479 with 8 warps that hold 128 columns, 399 with sums and addresses that did not fit registers, 380 with tiles that leave by TMA (3300 clocks a tile before).  Measured and not
+// kept: halves of 128 columns with barriers of their own (A is read twice: 401), 16 columns at a time (428), packed fp32 products (equal), other orders of the tiles (389 to 431), 3 stages (386), 6
+// (equal).
 // Every barrier wait is bounded (mbar_wait_bounded, common.cuh).
 #include <cuda.h>
 
@@ -21,10 +28,10 @@ namespace fp8 {
 
 namespace {
 
-constexpr int kBM = 128, kBN = 256, kHalf = kBN / 2;  // tokens per CTA; features of a tile, of its halves
+constexpr int kBM = 128, kBN = 256, kHalf = kBN / 2;  // tokens per CTA; features of a tile, of a CTA's half of B
 constexpr int kStages = 4;
+constexpr int kEpi = 16;               // epilogue warps
 constexpr int kPieceBytes = 32 * 128;  // of the output: 32 tokens x 128 bytes, an epilogue warp's at a time
-constexpr int kEpi = 16;                     // epilogue warps
 constexpr int kThreads = 128 + 32 * kEpi;
 constexpr int kABytes = kBM * kBK, kBBytes = kHalf * kBK, kStageBytes = kABytes + kBBytes;
 // registers of a thread: the 65536 of an SM by 640 threads, then by role
@@ -41,7 +48,7 @@ struct Shared {  // behind the stages
   uint64_t done;             // behind a run-out: the MMAs under way
   uint32_t tmem;
   int dead;
-  float scale[8][2][kBM];    // of eight blocks of K: of the first half and the second; gated: of w and w2
+  float scale[8][2][kBM];    // of eight blocks of K, by token: with the first 128 features and the second; gated: with w and w2
   float largest[2][4][kBM];  // gated: magnitudes of two tiles' rows, by 32 features
 };
 constexpr size_t kSmem = 227 * 1024;  // all of it: nobody else is resident on an SM whose tensor memory this kernel has (fp8_gemm_few.cu)
@@ -176,7 +183,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
         bool go = true;
         for (int tile = pair; tile < num_tiles && go; tile += num_pairs) {
           for (int kb = 0; kb < kb_n; ++kb) {
-            // two looks at once: a wait costs this thread 200 clocks where nothing is to be waited for, a block's MMAs take 443
+            // two looks at once: a wait costs this thread 200 clocks where nothing is to be waited for, a block's MMAs take 512
             const bool here = mbar_test_wait(sh.full + s, ph);
             bool free = mbar_test_wait(sh.tempty + buf, tph);
             if (!here) go = mbar_wait_bounded(sh.full + s, ph, dead);
@@ -384,8 +391,8 @@ int launch_pair(const Product& product, cudaStream_t st) {
   auto kern = fp8_gemm_kernel<GATED, O>;
   static std::atomic<uint64_t> set{0};
   if (const cudaError_t e = allow_smem(set, (const void*)kern, kSmem); e != cudaSuccess) return (int)e;
-  CUtensorMap mx, mw, mw2, my{};
-  if (!make_codes_map(&mx, p.x, p.N, p.K, p.ld_x, kBM) || !make_codes_map(&mw, p.w, p.M, p.K, p.ld_w, kHalf) || !make_codes_map(&mw2, GATED ? p.w2 : p.w, p.M, p.K, p.ld_w, kHalf))
+  CUtensorMap mx, mw, mw2{}, my{};
+  if (!make_codes_map(&mx, p.x, p.N, p.K, p.ld_x, kBM) || !make_codes_map(&mw, p.w, p.M, p.K, p.ld_w, kHalf) || (GATED && !make_codes_map(&mw2, p.w2, p.M, p.K, p.ld_w, kHalf)))
     return (int)cudaErrorInvalidValue;
   if constexpr (!GATED) p.y_map = make_out_map<O>(&my, p.y, p.N, p.M, p.ld_y);
   return (int)launch(kern, dim3(2 * pairs), dim3(kThreads), kSmem, st, true, mx, mw, mw2, my, p);

@@ -3,11 +3,15 @@
 //   A = W: NA tiles of `rows` <= 128 features (tensor-memory lane = feature), B = X: NT tokens (column = token).  Gated: 128 rows of w and the same of w2.
 //   A tile's K is cut into parts, one CTA each, and those CTAs are a cluster: each leaves its fp32 part over its operand ring and sends it, 16 bytes a thread, to the CTAs that own a share of
 //   the tile's results (features; gated: tokens, whose 128 features are a block of the result's scales), which add them up in rank order, so a result does not depend on timing.
-//   B200, us a launch, 48 tokens of 4096 x 12288 in 4 parts: words sent by the threads that have them 16.7, bulk copies 18.1; one token of 2560 x 4096 6.8 and 7.7.
-//   warp 0 TMA producer | warps 1 and 2 MMA issuers of even and odd blocks (looks, four MMAs and a commit take a thread 650 clocks) | the others: a block's partial sum out of tensor memory, times its scales (a token's come with the stage, a feature's is the thread's own),
-//   onto the sum in registers; then the part.  All warps: sums -> output.
+//   warp 0 TMA producer | warps 1 and 2 MMA issuers of even and odd blocks (one for all: 64 tokens of 24576 x 4096 27.6 us for 25.2) | the others: a block's partial sum out of tensor memory,
+//   times its scales (a token's come with the stage, a feature's is the thread's own), onto the sum in registers; then the part.  All warps: sums -> output.
 // Any number of rows may make a tile: the MMAs read 128, and what lies behind the tile's own ends in lanes that nobody reads.
 // One CTA has an SM: a second one on it would start 1 us later, and a cluster of eight with two on an SM 2 us.
+//
+// What bounds it, B200, 48 tokens of 4096 x 12288 (51 MB), us: 14.6, of them 2 between launches, 3 to the first block (1.2 from the launch to the first copy's start; all rings are asked for at
+// once, so the first stage comes behind parts of the others), 7.5 for the stream (6.7 TB/s), 2 for the joining.  One token of 2560 x 4096: 6.6, the same without the stream.
+// A cluster's joining, measured: words sent by the threads that have them 16.7, bulk copies from shared to shared memory 18.1, 16 bytes a thread of a part laid down feature by feature 15.8
+// (then two groups of warps for the sums: 15.0; parts fetched behind a barrier instead, with two CTAs an SM: 15.6).
 #include <cuda.h>
 
 #include <algorithm>
@@ -407,9 +411,9 @@ int run_few(const Product& p, double within_ns, cudaStream_t st) {
   if (const cudaError_t e = clusters_at_once((const void*)kern, cfg, attr[0], resident); e != cudaSuccess) return (int)e;
   const FewPlan plan = few_plan(p.M, p.N, p.kb, NA, NT, GATED, resident);
   if (plan.splits == 0 || plan.ns > within_ns) return -2;
-  CUtensorMap mx, mw, mw2;
+  CUtensorMap mx, mw, mw2{};
   if (!make_codes_map(&mx, p.x, p.N, p.K, p.ld_x, NT) || !make_codes_map(&mw, p.w, p.M, p.K, p.ld_w, plan.rows) ||
-      !make_codes_map(&mw2, GATED ? p.w2 : p.w, p.M, p.K, p.ld_w, plan.rows))
+      (GATED && !make_codes_map(&mw2, p.w2, p.M, p.K, p.ld_w, plan.rows)))
     return (int)cudaErrorInvalidValue;
   const int per_tile = GATED ? plan.rows : NA * plan.rows;
   ts.launches++;

@@ -34,24 +34,31 @@ __global__ void __launch_bounds__(32 * kNormWarps) fp8_add_norm_kernel(const bf1
     for (int j = 0; j < NV; ++j) {
       const int at = (j * blockDim.x + threadIdx.x) * 8;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[j][e] += add[j][e];
+      for (int e = 0; e < 8; e += 2) {
+        const uint64_t sum = add2(pair_of(v[j][e], v[j][e + 1]), pair_of(add[j][e], add[j][e + 1]));
+        v[j][e] = lo_of(sum);
+        v[j][e + 1] = hi_of(sum);
+      }
       store8<VEC>(x + base + at, width - at, v[j]);
     }
   }
-  float ss = 0.f, m[NV];
+  uint64_t squares = 0;
+  float m[NV];
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     const int at = (j * blockDim.x + threadIdx.x) * 8;
     float g[8];
     load8<VEC>(w + at, width - at, g);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      ss = fmaf(v[j][e], v[j][e], ss);
-      v[j][e] = at + e < width ? v[j][e] * (offset + g[e]) : 0.f;
+    for (int e = 0; e < 8; e += 2) {  // (behind the width both are zero)
+      const uint64_t u = pair_of(v[j][e], v[j][e + 1]), t = mul2(u, add2(pair_of(offset, offset), pair_of(g[e], g[e + 1])));
+      squares = fma2(u, u, squares);
+      v[j][e] = lo_of(t);
+      v[j][e + 1] = hi_of(t);
     }
     m[j] = max16(max8(v[j]));
   }
-  ss = warp_sum(ss);
+  float ss = warp_sum(lo_of(squares) + hi_of(squares));
   if (warps > 1) {
     if (lane == 0) red[warp] = ss;
     __syncthreads();
