@@ -256,41 +256,43 @@ fp8_gemm_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
   tc_fence_before();
   __syncthreads();
   const int fours = (tokens + 3) / 4;  // tokens by fours
+  constexpr int WARPS = THREADS / 32, LANES = NT / 4, ROWS = 32 / LANES;  // a warp has ROWS features of all tokens
   if (S > 1) {
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // all CTAs of the cluster are there
     const uint32_t to = smem_u32(received);
-    for (int i = threadIdx.x; i < features * fours; i += THREADS) {
-      const int g = i / fours, c = i - g * fours;
-      const float4 v = *reinterpret_cast<const float4*>(part + (size_t)g * LD + 4 * c);
-      if constexpr (GATED) {
-        const int r = 4 * c / own;
-        st_cluster4(map_to(to + (uint32_t)(((sp * 256 + g) * own + 4 * c - r * own) * 4), (uint32_t)r), v);
-      } else {
-        const int r = g / own;
-        st_cluster4(map_to(to + (uint32_t)(((sp * own + g - r * own) * LD + 4 * c) * 4), (uint32_t)r), v);
+    const int c = lane % LANES, first = warp * ROWS + lane / LANES;
+    if constexpr (GATED) {
+      const int r = 4 * c / own;
+      const uint32_t dst = map_to(to + (uint32_t)((sp * 256 * own + 4 * c - r * own) * 4), (uint32_t)min(r, S - 1));
+      if (c < fours)
+        for (int g = first; g < 256; g += WARPS * ROWS) st_cluster4(dst + (uint32_t)(g * own * 4), *reinterpret_cast<const float4*>(part + g * LD + 4 * c));
+    } else {
+      for (int r = 0; r < S; ++r) {
+        const uint32_t dst = map_to(to + (uint32_t)((sp * own * LD + 4 * c) * 4), (uint32_t)r);
+        const int n = min(own, features - r * own);
+        if (c < fours)
+          for (int g = first; g < n; g += WARPS * ROWS) st_cluster4(dst + (uint32_t)(g * LD * 4), *reinterpret_cast<const float4*>(part + (r * own + g) * LD + 4 * c));
       }
     }
     __syncwarp();
     cluster_barrier();
   }
-  // ---- this CTA's share of the tile, added up in rank order: a feature of four tokens at a time
-  auto sum4 = [&](int at, int stride) {
-    float4 t = *reinterpret_cast<const float4*>(received + at);
-    for (int r = 1; r < S; ++r) {
-      const float4 v = *reinterpret_cast<const float4*>(received + r * stride + at);
-      t.x += v.x;
-      t.y += v.y;
-      t.z += v.z;
-      t.w += v.w;
-    }
-    return t;
-  };
+  // ---- this CTA's share of the tile, added up in rank order
   if constexpr (!GATED) {
+    // a thread has a feature of four tokens at a time
     const int mine = max(0, min(own, min(features, p.M - m0) - sp * own));
     O* y = static_cast<O*>(p.y) + (size_t)t0 * p.ld_y + m0 + sp * own;
     for (int i = threadIdx.x; i < mine * fours; i += THREADS) {
       const int c = i / mine, g = i - c * mine;
-      const float4 v = sum4(g * LD + 4 * c, own * LD);
+      float4 v = *reinterpret_cast<const float4*>(received + g * LD + 4 * c);
+#pragma unroll 1
+      for (int r = 1; r < S; ++r) {
+        const float4 u = *reinterpret_cast<const float4*>(received + (r * own + g) * LD + 4 * c);
+        v.x += u.x;
+        v.y += u.y;
+        v.z += u.z;
+        v.w += u.w;
+      }
       O* dst = y + (size_t)(4 * c) * p.ld_y + g;
       const float o[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -298,30 +300,33 @@ fp8_gemm_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
         if (4 * c + e < tokens) dst[(size_t)e * p.ld_y] = from_f<O>(o[e]);
     }
   } else {
-    // a warp has four tokens' 128 features, a block of the result's scales each: a lane every 32nd feature
+    // a warp has a token's 128 features, a block of the result's scales: a lane every 32nd.  The exponent of pk_fp8_act's formulas as c1 z + c2 z^3 for both
     const int mine = max(0, min(own, tokens - sp * own)), ld = S > 1 ? own : LD;
-    for (int c = warp; 4 * c < mine; c += THREADS / 32) {
-      float v[4][4];  // [feature][token]
+    const float c1 = p.act == 2 ? -2.302208198f : -1.4426950408889634f, c2 = p.act == 2 ? -0.1029432396f : 0.f;
+#pragma unroll 1
+    for (int t = warp; t < mine; t += WARPS) {
+      float v[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float4 g = sum4((lane + 32 * j) * ld + 4 * c, 256 * ld), u = sum4((128 + lane + 32 * j) * ld + 4 * c, 256 * ld);
-        const float a[4] = {g.x, g.y, g.z, g.w}, b[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[j][e] = (p.act == 0 ? gate_act<0>(a[e]) : p.act == 1 ? gate_act<1>(a[e]) : gate_act<2>(a[e])) * b[e];
+        const float* from = received + (lane + 32 * j) * ld + t;
+        float z = from[0], u = from[128 * ld];
+#pragma unroll 1
+        for (int r = 1; r < S; ++r) {
+          z += from[r * 256 * ld];
+          u += from[(r * 256 + 128) * ld];
+        }
+        const float gate = z * rcp_ftz(1.f + exp2_ftz(z * fmaf(fminf(z * z, 1e30f), c2, c1)));
+        v[j] = (p.act == 1 ? (z < 0.f ? 0.f : z) : gate) * u;
       }
+      const float m = max16(max_abs(max_abs(v[0], v[1], v[2]), v[3]));
+      const Scale k = scale_of(max_abs(m, __shfl_xor_sync(0xffffffffu, m, 16)));
+      const uint32_t lo = codes2(v[0], v[1], k), hi = codes2(v[2], v[3], k);
+      const int tok = t0 + sp * own + t;
+      uint8_t* dst = p.codes + (size_t)tok * p.ld + m0 + lane;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int tok = t0 + sp * own + 4 * c + e;
-        const float m = max16(max_abs(max_abs(v[0][e], v[1][e], v[2][e]), v[3][e]));
-        const Scale k = scale_of(max_abs(m, __shfl_xor_sync(0xffffffffu, m, 16)));
-        if (4 * c + e >= mine) continue;
-        const uint32_t lo = codes2(v[0][e], v[1][e], k), hi = codes2(v[2][e], v[3][e], k);
-        uint8_t* dst = p.codes + (size_t)tok * p.ld + m0 + lane;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (m0 + lane + 32 * j < p.M) dst[32 * j] = (uint8_t)((j < 2 ? lo : hi) >> (8 * (j & 1)));
-        if (lane == 0) p.scales[(size_t)(m0 / kBlock) * p.ld_s + tok] = k.s;
-      }
+      for (int j = 0; j < 4; ++j)
+        if (m0 + lane + 32 * j < p.M) dst[32 * j] = (uint8_t)((j < 2 ? lo : hi) >> (8 * (j & 1)));
+      if (lane == 0) p.scales[(size_t)(m0 / kBlock) * p.ld_s + tok] = k.s;
     }
   }
   if (threadIdx.x == 0) count_run_out(dead, p.err);  // (every wait lies before the barrier above)
