@@ -328,24 +328,31 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
       } else {
         O* y = static_cast<O*>(p.y);
         const int tok0 = tok - lane;
-        if (p.y_map) {
-          constexpr int kCols = 128 / (int)sizeof(O);
+        constexpr int kCols = 128 / (int)sizeof(O);
 #pragma unroll
-          for (int c = 0; c < 64; c += kCols) {
-            if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the piece before
-            __syncwarp();
-            uint32_t u[32];
+        for (int c = 0; c < 64; c += kCols) {
+          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the piece before
+          __syncwarp();
+          uint32_t u[32];
 #pragma unroll
-            for (int j = 0; j < 32; ++j) u[j] = sizeof(O) == 4 ? __float_as_uint(acc[c + j]) : pack_bf16(acc[2 * j], acc[2 * j + 1]);
-            put_row(piece, lane, u);
+          for (int j = 0; j < 32; ++j) u[j] = sizeof(O) == 4 ? __float_as_uint(acc[c + j]) : pack_bf16(acc[2 * j], acc[2 * j + 1]);
+          put_row(piece, lane, u);
+          if (p.y_map) {
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0 && tok0 < N && f0 + c < M) store_piece(&map_y, piece, f0 + c, tok0);
-          }
-        } else if (tok < N) {
+          } else {  // rows that start anywhere: 32 entries of one at a time
+            __syncwarp();
+            const O* from = reinterpret_cast<const O*>(pieces + (warp - 4) * kPieceBytes);
+            for (int r = 0; r < 32 && tok0 + r < N; ++r)
 #pragma unroll
-          for (int j = 0; j < 64; ++j)
-            if (f0 + j < M) y[(size_t)tok * p.ld_y + f0 + j] = from_f<O>(acc[j]);
+              for (int j = lane; j < kCols; j += 32) {
+                const int byte = j * (int)sizeof(O);
+                if (f0 + c + j < M)
+                  y[(size_t)(tok0 + r) * p.ld_y + f0 + c + j] = from[(r * 128 + (((byte >> 4) ^ (r & 7)) << 4) + (byte & 15)) / (int)sizeof(O)];
+              }
+            __syncwarp();
+          }
         }
       }
     }
