@@ -779,6 +779,7 @@ int pk_kv8_evict(void* cache, long page_stride, int page_size, const int* page_o
  * and have room for ld_s floats a block.  Bytes of a row behind its width and scales behind the last token are neither written nor used.
  * Quantising: scale = max(largest magnitude of the block, 2^-100) / 448, code = the e4m3 number nearest to value / scale (ties to even; a value next to the border of two codes may get
  * either).  A block with an entry that is not finite has the scale NaN and codes NaN.  All arithmetic is fp32; a value is rounded once, to its code.
+ * What a call writes overlaps nothing that it reads (x of the norm, which it does both to, aside).
  * Nothing is allocated and there are no workspaces, so calls may run at the same time and be captured.  -1: invalid argument, -2: sizes outside the kernels' range. */
 /* x[t] += y[t] (y bf16, NULL: nothing is added and x not written; x bf16, rounded when stored, or float);  codes of x[t] / sqrt(mean(x[t]^2) + eps) * (offset + w), of the
  * unrounded sum.  x, y [tokens, width], w [width] bf16, offset 0 or 1 as the weights are kept.  y is another array than x.  width up to 16384. */
@@ -794,7 +795,7 @@ int pk_fp8_weights(const void* w, int w_f32, long ld_w, void* codes, long ld, fl
 int pk_fp8_gemm(const void* w, long ld_w, const float* w_scales, const void* x, long ld_x, const float* x_scales, long ld_xs, void* y, long ld_y, int y_f32, int M, int N, int K,
                 pk_stream st);
 /* codes of act(x w_gate^T) * (x w_up^T), F features: pk_fp8_gemm of both, pk_fp8_act and nothing rounded between.  act 0 SiLU, 1 ReLU, 2 GELU in its tanh form.  w_gate and w_up
- * [F, K] have one ld_w; halves of one array are fine.  codes is another array than x. */
+ * [F, K] have one ld_w and scales of their own; they may be halves of one array of 2 F rows, quantised as one where F is a multiple of 128, else each by itself. */
 int pk_fp8_gemm_gated(const void* w_gate, const float* gate_scales, const void* w_up, const float* up_scales, long ld_w, const void* x, long ld_x, const float* x_scales, long ld_xs,
                       void* codes, long ld, float* scales, long ld_s, int F, int N, int K, int act, pk_stream st);
 

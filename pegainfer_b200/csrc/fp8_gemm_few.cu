@@ -79,7 +79,7 @@ fp8_gemm_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
   constexpr int GROUPS = groups(NA, NT), COLS = NT * NA / GROUPS, THREADS = 96 + 128 * GROUPS;  // COLS: columns of a thread
   constexpr uint32_t TMEM_COLS = tmem_columns(NA, NT);
   static_assert(2 * NA * NT <= 512 && (!GATED || NA == 2), "tensor memory");
-    const int stages = plan.stages, rows = plan.rows;
+  const int stages = plan.stages, rows = plan.rows;
   const uint32_t A_BYTES = rows * kBK, STAGE = NA * A_BYTES + NT * kBK;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);

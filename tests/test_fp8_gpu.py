@@ -75,6 +75,20 @@ def test_norm(lib, T, W, x_f32, add):
     untouched(codes, scales, T, W)
 
 
+@pytest.mark.parametrize("T,W", [(800, 333), (1500, 2049), (2000, 128), (900, 520)])
+@pytest.mark.parametrize("x_f32", [False, True])
+def test_norm_of_many_rows(lib, T, W, x_f32):
+    g = gen(T, W, x_f32, 3)
+    x, y, w = (2 * rn(g, T, W)).to(F32 if x_f32 else BF16), rn(g, T, W).to(BF16), (1 + 0.3 * rn(g, W)).to(BF16)
+    codes, scales = out_rows(T, W, more=1)
+    want = x.double() + y.double()
+    stored = (x.float() + y.float()).to(x.dtype)
+    assert lib.pk_fp8_add_norm(y.data_ptr(), x.data_ptr(), int(x_f32), w.data_ptr(), 0.0, codes.data_ptr(), codes.shape[1], scales.data_ptr(), scales.shape[1], W, T, 1e-6, st()) == 0
+    assert torch.equal(x, stored)
+    R.hold_rows(codes, scales, want / torch.sqrt((want * want).mean(-1, keepdim=True) + 1e-6) * w.double(), rel=2.0 ** -17)  # as in test_norm
+    untouched(codes, scales, T, W)
+
+
 def norm_of(lib, x, w=None):
     T, W = x.shape
     w = torch.ones(W, device="cuda").to(BF16) if w is None else w
@@ -338,6 +352,22 @@ def test_gated_of_model_sizes(lib, T, M, K, act):
     hold_gated(*gated(lib, ops, w2, T, M, K, act), ops, w2, T, M, K, act)
 
 
+@pytest.mark.parametrize("T", [5, 90, 300])
+def test_gated_with_one_matrix_for_both(lib, T):
+    ops = operands(T, 200, 400, gen(T, 78))
+    hold_gated(*gated(lib, ops, ops[2:], T, 200, 400, 1), ops, ops[2:], T, 200, 400, 1)
+
+
+@pytest.mark.parametrize("T", [7, 300])
+def test_gated_halves_of_one_array(lib, T):
+    """gate and up quantised as one array of rows, where a half is whole blocks"""
+    M, K = 256, 500
+    g = gen(T, 79)
+    xc, xs, wc, ws = operands(T, 2 * M, K, g)
+    ops, w2 = (xc, xs, wc[:M], ws[:M // 128]), (wc[M:], ws[M // 128:])
+    hold_gated(*gated(lib, ops, w2, T, M, K, 2), ops, w2, T, M, K, 2)
+
+
 @pytest.mark.parametrize("T", [6, 100])
 def test_gated_keeps_what_is_not_finite_apart(lib, T):
     M, K = 300, 300
@@ -461,6 +491,20 @@ def test_with_dependent_launches(lib):
     try:
         for _ in range(20):
             assert torch.equal(f.step(x.clone(), y, f.buffers(9)), want)
+    finally:
+        lib.pk_b200_set_pdl(0)
+
+
+@pytest.mark.parametrize("fused", [True, False])
+def test_with_dependent_launches_of_a_prompt(lib, fused):
+    """the same through the kernels for many tokens, and for rows of odd widths"""
+    f = FeedForward(lib, 999, 1300, 9)
+    x, y = rn(gen(9, 1), 300, 999), rn(gen(9, 2), 300, 999).to(BF16)
+    want = f.step(x.clone(), y, f.buffers(300), fused).clone()
+    lib.pk_b200_set_pdl(1)
+    try:
+        for _ in range(20):
+            assert torch.equal(f.step(x.clone(), y, f.buffers(300), fused), want)
     finally:
         lib.pk_b200_set_pdl(0)
 
