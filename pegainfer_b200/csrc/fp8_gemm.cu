@@ -1,20 +1,21 @@
 // The product of 8-bit rows and weights for prompts, on CTA pairs (fp8_gemm.cuh): y = x w^T, and act(x w^T) * (x w2^T) quantised again.
 //
-// A pair (cluster of two, tcgen05 cta_group::2) has a tile of 256 tokens x 256 features: A = X, 128 tokens to a CTA, B = W, half the features to a CTA.
+// A pair (cluster of two, tcgen05 cta_group::2) has a tile of 256 tokens x 128, 192 or 256 features: A = X, 128 tokens to a CTA, B = W, half the features to a CTA.
 //   warp 0     TMA producer (both CTAs): 128 entries of K a stage, completing on the leader's barrier
-//   warp 1     MMA issuer (leader): a block of K is four tcgen05.mma (M 256, N 256, K 32) into one of two partial sums, all of tensor memory
+//   warp 1     MMA issuer (leader): a block of K is four tcgen05.mma (M 256, K 32) into one of two partial sums (128 features: of four), which have tensor memory
 //   warps 2, 3 the scales of even and odd blocks of K into shared memory, a token's times the weights'; they see a block's MMAs end and give its stage back
-//   warps 4-19 take a partial sum out of tensor memory while the other is computed and add it, times its scale, to the tile's sum, which they hold in registers (thread = token, 64 features);
-//              a finished tile leaves through shared memory by TMA
+//   the others (16, 12 or 8 warps) take a partial sum out of tensor memory while the next is computed and add it, times its scale, to the tile's sum, which they hold in registers
+//              (thread = token, 64 features); a finished tile leaves through shared memory by TMA
 // Gated: B is 128 rows of w (leader) and the same 128 of w2 (peer), so a thread has 32 features of both; 128 features are a block of the result's scales, whose largest magnitude four threads
 // find together.
 //
-// What bounds it, B200, 4096 tokens of 24576 x 4096 (825 GFLOP), us: 380 alone (2.17 PFLOP/s; 443 at the clocks of seconds under the power limit).  A block of K takes a tile 950 clocks, its
+// What bounds it, B200, 4096 tokens of 24576 x 4096 (825 GFLOP), us: 372 alone (2.22 PFLOP/s; 436 at the clocks of seconds under the power limit).  A block of K takes a tile 930 clocks, its
 // MMAs 512.  Without the sums' work 312, with half of the operands' bytes 324, without both 244: a partial sum's way (MMAs, commit, 64 columns out and added by 16 warps, arrival in the other
 // CTA: 1800 clocks, two of them under way) and the 32 KB a CTA reads of L2 for it (34 bytes a clock and SM) bound it together.  What it took to come here: 770 with a release at the cluster's scope in
 // the arrivals, 479 with 8 warps that hold 128 columns, 399 with sums and addresses that did not fit registers, 380 with tiles that leave by TMA (3300 clocks a tile before).  Measured and not
 // kept: halves of 128 columns with barriers of their own (A is read twice: 401), 16 columns at a time (428), packed fp32 products (equal), other orders of the tiles (389 to 431), 3 stages (386), 6
-// (equal).
+// (equal).  Tiles of 128, whose MMAs take 256 clocks a block, are at 460: 350 without the sums' work and with weights in L2; four partial sums carry them (with two 590), and so do 64 columns at once
+// by 8 warps (32 by 16: 590).  Weights asked into L2 eight to 32 blocks ahead: equal.
 // Every barrier wait is bounded (mbar_wait_bounded, common.cuh).
 #include <cuda.h>
 
@@ -28,23 +29,27 @@ namespace fp8 {
 
 namespace {
 
-constexpr int kBM = 128, kBN = 256, kHalf = kBN / 2;  // tokens per CTA; features of a tile, of a CTA's half of B
-constexpr int kStages = 4;
-constexpr int kEpi = 16;               // epilogue warps
+constexpr int kBM = 128;               // tokens per CTA
 constexpr int kPieceBytes = 32 * 128;  // of the output: 32 tokens x 128 bytes, an epilogue warp's at a time
-constexpr int kThreads = 128 + 32 * kEpi;
-constexpr int kABytes = kBM * kBK, kBBytes = kHalf * kBK, kStageBytes = kABytes + kBBytes;
-// registers of a thread: the 65536 of an SM by 640 threads, then by role
+constexpr int kABytes = kBM * kBK;
+
+constexpr int stages_of(int bn) { return bn == 256 ? 4 : bn == 192 ? 5 : 6; }
+constexpr int epi_of(int bn) { return bn / 16; }             // epilogue warps
+constexpr int sums_of(int bn) { return bn == 128 ? 4 : 2; }  // partial sums in tensor memory
+constexpr int threads_of(int bn) { return 128 + 32 * epi_of(bn); }
+// registers of a thread of a tile of 256: the 65536 of an SM by the threads, then by role (the others have enough for all, 128 and 168)
 constexpr int kRegsLaunch = 96, kRegsOther = 32, kRegsEpi = 112;
-static_assert(128 * kRegsOther + 32 * kEpi * kRegsEpi <= kThreads * kRegsLaunch, "what the block was launched with");
+static_assert(128 * kRegsOther + 32 * epi_of(256) * kRegsEpi <= threads_of(256) * kRegsLaunch, "what the block was launched with");
+constexpr int stage_bytes_of(int bn) { return kABytes + bn / 2 * kBK; }
 
 constexpr int kLooks = 512;  // at a barrier before its wait proper, which wakes up 50 to 100 clocks later
 
+template <int STAGES, int SUMS>
 struct Shared {  // behind the stages
-  uint64_t full[kStages];    // used in the leader
-  uint64_t empty[kStages];   // one per CTA, by the scales' warps
-  uint64_t tfull[2];         // one per CTA: the MMAs' commit, the scales
-  uint64_t tempty[2];        // used in the leader: an arrival per epilogue warp of both CTAs
+  uint64_t full[STAGES];     // used in the leader
+  uint64_t empty[STAGES];    // one per CTA, by the scales' warps
+  uint64_t tfull[SUMS];      // one per CTA: the MMAs' commit, the scales
+  uint64_t tempty[SUMS];     // used in the leader: an arrival per epilogue warp of both CTAs
   uint64_t done;             // behind a run-out: the MMAs under way
   uint32_t tmem;
   int dead;
@@ -52,7 +57,6 @@ struct Shared {  // behind the stages
   float largest[2][4][kBM];  // gated: magnitudes of two tiles' rows, by 32 features
 };
 constexpr size_t kSmem = 227 * 1024;  // all of it: nobody else is resident on an SM whose tensor memory this kernel has (fp8_gemm_few.cu)
-static_assert((size_t)kStages * kStageBytes + kEpi * kPieceBytes + 1024 + sizeof(Shared) <= kSmem, "shared memory of a CTA");
 
 // An arrival without a release: what it reports are reads of tensor memory, complete and fenced (tcgen05.wait::ld, fence::before_thread_sync); no memory is handed over.  A release at the
 // cluster's scope waits for the thread's loads in flight as well, 1500 to 2000 clocks for each block of K.
@@ -105,15 +109,20 @@ __device__ __forceinline__ void activate(const float* acc, float* v) {  // acc: 
   for (int j = 0; j < 32; ++j) v[j] = gate_act<ACT>(acc[j]) * acc[32 + j];
 }
 
-// GATED: O is the codes' type
-template <bool GATED, typename O>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+// BN: features of a tile; gated: 256, O is the codes' type
+template <int BN, bool GATED, typename O>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(BN), 1)
 fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_w2,
                 const __grid_constant__ CUtensorMap map_y, const Product p) {
+  constexpr int kHalf = BN / 2, kStages = stages_of(BN), kEpi = epi_of(BN), kSums = sums_of(BN), kStageBytes = stage_bytes_of(BN);
+  constexpr bool kSplit = BN == 256;              // registers by role
+  constexpr int kAtOnce = BN > 128 ? 32 : 64;    // columns of a partial sum that a thread has at once
+  static_assert(!GATED || BN == 256, "a block of the result's scales");
+  static_assert((size_t)kStages * kStageBytes + kEpi * kPieceBytes + 1024 + sizeof(Shared<kStages, kSums>) <= kSmem, "shared memory of a CTA");
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   uint8_t* pieces = smem + (size_t)kStages * kStageBytes;
-  Shared& sh = *reinterpret_cast<Shared*>(pieces + kEpi * kPieceBytes);
+  Shared<kStages, kSums>& sh = *reinterpret_cast<Shared<kStages, kSums>*>(pieces + kEpi * kPieceBytes);
   volatile int* dead = &sh.dead;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -129,7 +138,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
       mbar_init(sh.full + s, 1);
       mbar_init(sh.empty + s, 1);
     }
-    for (int s = 0; s < 2; ++s) {
+    for (int s = 0; s < kSums; ++s) {
       mbar_init(sh.tfull + s, 2);
       mbar_init(sh.tempty + s, 2 * kEpi);
     }
@@ -137,7 +146,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
     *dead = 0;
     mbar_fence_init();
   }
-  if (warp == 1) g2_tmem_alloc(&sh.tmem, 2 * kBN);
+  if (warp == 1) g2_tmem_alloc(&sh.tmem, 512);
   tc_fence_before();
   __syncthreads();
   cluster_barrier();  // both CTAs' barriers are initialised and both TMEM allocations are done
@@ -146,7 +155,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
   pdl_wait();
 
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
+    if constexpr (kSplit) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
     if (warp == 0) {
       if (tc_elect_one()) {
         const CUtensorMap* mw = GATED && rank == 1 ? &map_w2 : &map_w;
@@ -158,7 +167,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
         for (int tile = pair; tile < num_tiles && go; tile += num_pairs) {
           const int mb = tile % m_tiles, nb = tile / m_tiles;
           const int tok0 = mb * 2 * kBM + (int)rank * kBM;
-          const int row0 = GATED ? nb * kHalf : nb * kBN + (int)rank * kHalf;
+          const int row0 = GATED ? nb * kHalf : nb * BN + (int)rank * kHalf;
           for (int kb = 0; kb < kb_n; ++kb) {
             go = mbar_wait_bounded(sh.empty + s, ph, dead);
             if (!go) break;
@@ -177,7 +186,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
       }
     } else if (warp == 1) {
       if (leader && tc_elect_one()) {
-        constexpr uint32_t idesc = f8_idesc(2 * kBM, kBN);
+        constexpr uint32_t idesc = f8_idesc(2 * kBM, BN);
         int s = 0, buf = 0;
         uint32_t ph = 0, tph = 1;
         bool go = true;
@@ -190,7 +199,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
             if (!go) break;
             const uint32_t a_addr = smem_u32(smem + (size_t)s * kStageBytes);
             const uint64_t adesc = make_sw128_desc(a_addr), bdesc = make_sw128_desc(a_addr + kABytes);
-            const uint32_t d = tmem_base + (uint32_t)(buf * kBN);
+            const uint32_t d = tmem_base + (uint32_t)(buf * BN);
             for (int i = 0; !free && i < kLooks; ++i) free = mbar_test_wait(sh.tempty + buf, tph);
             if (!free) go = mbar_wait_bounded(sh.tempty + buf, tph, dead);
             if (!go) break;
@@ -202,7 +211,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
               s = 0;
               ph ^= 1u;
             }
-            if (++buf == 2) {
+            if (++buf == kSums) {
               buf = 0;
               tph ^= 1u;
             }
@@ -214,52 +223,65 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
         }
       }
     } else {
-      // Blocks of K as they come, tile behind tile, every second one, fetched one ahead.  A lane has four tokens.  Slot it % 8 held block it - 8: whoever gave back the partial sums of
-      // block it - 4 had used it, and without those the MMAs of block it - 2, whose end is waited for here, did not begin.
+      // Blocks of K as they come, tile behind tile, every second one, fetched kAhead of them ahead (512 tokens of 2560 x 9728 in tiles of 128: one 31.7 us, two 26.0, three 24.6, four
+      // 24.2).  A lane has four tokens.  Slot it % 8 held block it - 8: whoever gave back the partial sums of block it - 4 (it - 6 where there are four) had used it, and without those the
+      // MMAs of block it - 2, whose end is waited for here, did not begin.
+      constexpr int kAhead = BN == 256 ? 1 : BN == 192 ? 2 : 3;
       const int mine = warp - 2;
       int tile = pair, kb = mine;
-      auto settle = [&]() {
+      struct Next {
+        float4 x;
+        float a, b;
+        bool there;
+      } next[kAhead];
+      auto fetch = [&](Next& n) {  // (asm: where it stands)
         while (kb >= kb_n) {
           kb -= kb_n;
           tile += num_pairs;
         }
-      };
-      float4 x;
-      float a, b;
-      auto fetch = [&]() {  // (asm: where it stands)
-        x = make_float4(0.f, 0.f, 0.f, 0.f);
-        a = b = 0.f;
-        if (tile >= num_tiles) return;
+        n.x = make_float4(0.f, 0.f, 0.f, 0.f);
+        n.a = n.b = 0.f;
+        n.there = tile < num_tiles;
+        if (!n.there) return;
         const int nb = tile / m_tiles, tok = (tile - nb * m_tiles) * 2 * kBM + (int)rank * kBM + lane * 4;
-        const int w0 = GATED ? nb : 2 * nb, w1 = GATED ? nb : (2 * nb + 1) * kBlock < M ? 2 * nb + 1 : 2 * nb;
+        const int w0 = GATED ? nb : nb * BN / kBlock, w1 = GATED ? nb : (w0 + 1) * kBlock < M ? w0 + 1 : w0;
         if (tok < N)  // (rows of scales are whole fours)
-          asm volatile("ld.global.nc.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "l"(p.sx + (size_t)kb * p.ld_sx + tok));
-        asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(a) : "l"(p.sw + (size_t)w0 * kb_n + kb));
-        asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(b) : "l"((GATED ? p.sw2 : p.sw) + (size_t)w1 * kb_n + kb));
-      };
-      settle();
-      fetch();
-      uint32_t ph = 1;  // of tfull[mine]: before its first phase
-      int stage = -1;   // of block it - 2
-      for (int slot = mine; tile < num_tiles; slot = (slot + 2) & 7) {
-        mbar_wait_bounded(sh.tfull + mine, ph, dead);
-        if (lane == 0 && stage >= 0) mbar_arrive(sh.empty + stage);  // (the MMAs of block it - 2 have read it)
-        stage = stage < 0 ? mine : stage + 2 < kStages ? stage + 2 : stage + 2 - kStages;
-        reinterpret_cast<float4*>(sh.scale[slot][0])[lane] = make_float4(x.x * a, x.y * a, x.z * a, x.w * a);
-        reinterpret_cast<float4*>(sh.scale[slot][1])[lane] = make_float4(x.x * b, x.y * b, x.z * b, x.w * b);
-        __syncwarp();
-        if (lane == 0) mbar_arrive(sh.tfull + mine);
-        ph ^= 1u;
+          asm volatile("ld.global.nc.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(n.x.x), "=f"(n.x.y), "=f"(n.x.z), "=f"(n.x.w) : "l"(p.sx + (size_t)kb * p.ld_sx + tok));
+        asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(n.a) : "l"(p.sw + (size_t)w0 * kb_n + kb));
+        if (BN > kBlock) asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(n.b) : "l"((GATED ? p.sw2 : p.sw) + (size_t)w1 * kb_n + kb));
         kb += 2;
-        settle();
-        fetch();
+      };
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) fetch(next[u]);
+      uint32_t slot = mine, buf = mine, ph = 1;  // of this block; the phase of block it - 2's partial sum
+      int stage = -1;                            // of block it - 2
+      for (bool go = true; go;) {
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+          Next& n = next[u];
+          go = go && n.there;
+          if (!go) break;
+          mbar_wait_bounded(sh.tfull + (kSums == 2 ? buf : buf ^ 2), ph, dead);
+          if (kSums == 2 || buf < 2) ph ^= 1u;
+          if (lane == 0 && stage >= 0) mbar_arrive(sh.empty + stage);  // (the MMAs of block it - 2 have read it)
+          stage = stage < 0 ? mine : stage + 2 < kStages ? stage + 2 : stage + 2 - kStages;
+          reinterpret_cast<float4*>(sh.scale[slot][0])[lane] = make_float4(n.x.x * n.a, n.x.y * n.a, n.x.z * n.a, n.x.w * n.a);
+          if (BN > kBlock) reinterpret_cast<float4*>(sh.scale[slot][1])[lane] = make_float4(n.x.x * n.b, n.x.y * n.b, n.x.z * n.b, n.x.w * n.b);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(sh.tfull + buf);
+          slot = (slot + 2) & 7;
+          if (kSums == 4) buf ^= 2;
+          fetch(n);
+        }
       }
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsEpi));
+    if constexpr (kSplit) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsEpi));
     const int q = warp & 3, part = (warp - 4) >> 2, row = q * 32 + lane;
     const uint32_t tempty = g2_map(smem_u32(sh.tempty), 0), tfull = smem_u32(sh.tfull);
-    const uint32_t scales = smem_u32(&sh.scale[0][GATED ? 0 : part >> 1][row]);
+    // its scales: its features are in the tile's first or second block of weights
+    auto scales_of = [&](int half) { return smem_u32(&sh.scale[0][GATED ? 0 : (part + half) >> 1][row]); };
+    uint32_t scales = scales_of(0);
     // the thread's two pieces of 32 columns; gated: 32 of the gate, then the same 32 of the factor
     const uint32_t t_row = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(part * (GATED ? 32 : 64));
     constexpr uint32_t kPiece = GATED ? kHalf : 32;
@@ -267,35 +289,44 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
     uint32_t it = 0, lt = 0;  // blocks of K so far, tiles
     bool ready = false;
     for (int tile = pair; tile < num_tiles; tile += num_pairs, ++lt) {
+      if (BN % kBlock) scales = scales_of(tile / m_tiles & 1);  // (a tile of 192 begins at a block or in the middle of one)
       float acc[64];
 #pragma unroll
       for (int j = 0; j < 64; ++j) acc[j] = 0.f;
 #pragma unroll 1
       for (int kb = kb_n; kb > 0; --kb) {
-        const uint32_t buf = it & 1;
-        for (int i = 0; !ready && i < kLooks; ++i) ready = test_wait_at(tfull + buf * 8u, (it >> 1) & 1);
-        if (!ready) mbar_wait_bounded(sh.tfull + buf, (it >> 1) & 1, dead);
+        const uint32_t buf = it % kSums;
+        for (int i = 0; !ready && i < kLooks; ++i) ready = test_wait_at(tfull + buf * 8u, it / kSums & 1);
+        if (!ready) mbar_wait_bounded(sh.tfull + buf, it / kSums & 1, dead);
         tc_fence_after();
-        const uint32_t t0 = t_row + buf * kBN;
-        uint32_t v[32];
+        const uint32_t t0 = t_row + buf * BN;
+        uint32_t v[kAtOnce];
         tmem_ld32_nowait(t0, v);
+        if constexpr (kAtOnce == 64) tmem_ld32_nowait(t0 + kPiece, v + 32);
         const float s1 = ld_shared_at(scales + (it & 7) * (uint32_t)sizeof(sh.scale[0])), s2 = GATED ? ld_shared_at(scales + (it & 7) * (uint32_t)sizeof(sh.scale[0]) + kBM * 4) : s1;
         ++it;
-        tmem_wait32(v);
+        if constexpr (kAtOnce == 32) {
+          tmem_wait32(v);
 #pragma unroll
-        for (int j = 0; j < 32; ++j) acc[j] = fmaf(__uint_as_float(v[j]), s1, acc[j]);
-        tmem_ld32_nowait(t0 + kPiece, v);
-        ready = test_wait_at(tfull + (it & 1) * 8u, (it >> 1) & 1);  // (asked for early)
+          for (int j = 0; j < 32; ++j) acc[j] = fmaf(__uint_as_float(v[j]), s1, acc[j]);
+          tmem_ld32_nowait(t0 + kPiece, v);
+        }
+        ready = test_wait_at(tfull + it % kSums * 8u, it / kSums & 1);  // (asked for early)
         tmem_wait32(v);
+        if constexpr (kAtOnce == 64) tmem_wait32(v + 32);
         tc_fence_before();
         __syncwarp();
         if (lane == 0) arrive_relaxed(tempty + buf * 8u);
+        if constexpr (kAtOnce == 64) {
 #pragma unroll
-        for (int j = 0; j < 32; ++j) acc[32 + j] = fmaf(__uint_as_float(v[j]), s2, acc[32 + j]);
+          for (int j = 0; j < 32; ++j) acc[j] = fmaf(__uint_as_float(v[j]), s1, acc[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < 32; ++j) acc[32 + j] = fmaf(__uint_as_float(v[kAtOnce - 32 + j]), s2, acc[32 + j]);
       }
       const int mb = tile % m_tiles, nb = tile / m_tiles;
       const int tok = mb * 2 * kBM + (int)rank * kBM + row;
-      const int f0 = GATED ? nb * kHalf + part * 32 : nb * kBN + part * 64;  // the thread's first feature
+      const int f0 = GATED ? nb * kHalf + part * 32 : nb * BN + part * 64;  // the thread's first feature
       if constexpr (GATED) {
         float v[32];
         if (p.act == 0) activate<0>(acc, v);
@@ -304,10 +335,10 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
         float m = max_abs(v[0], v[1]);
 #pragma unroll
         for (int j = 2; j < 32; j += 2) m = max_abs(m, v[j], v[j + 1]);
-        float(*mine)[kBM] = sh.largest[lt & 1];  // (the other tile's are read until the barrier behind this one)
-        mine[part][row] = m;
+        float(*largest)[kBM] = sh.largest[lt & 1];  // (the other tile's are read until the barrier behind this one)
+        largest[part][row] = m;
         asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpi) : "memory");
-        const Scale k = scale_of(max_abs(max_abs(mine[0][row], mine[1][row], mine[2][row]), mine[3][row]));
+        const Scale k = scale_of(max_abs(max_abs(largest[0][row], largest[1][row], largest[2][row]), largest[3][row]));
         if (tok < N && f0 < M) {
           uint8_t* dst = p.codes + (size_t)tok * p.ld + f0;
 #pragma unroll
@@ -341,7 +372,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0 && tok0 < N && f0 + c < M) store_piece(&map_y, piece, f0 + c, tok0);
-          } else {  // rows that start anywhere: 32 entries of one at a time
+          } else {  // rows that start or end anywhere: 32 entries of one at a time
             __syncwarp();
             const O* from = reinterpret_cast<const O*>(pieces + (warp - 4) * kPieceBytes);
             for (int r = 0; r < 32 && tok0 + r < N; ++r)
@@ -363,16 +394,17 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
   cluster_barrier();  // the peer's MMAs / loads may still target this CTA's shared memory and TMEM
   if (warp == 1) {
     tc_fence_after();
-    g2_tmem_dealloc(tmem_base, 2 * kBN);
+    g2_tmem_dealloc(tmem_base, 512);
   }
   if (threadIdx.x == 0) count_run_out(dead, p.err);
 }
 
-// rows x M of the output in pieces of 32 rows x 128 bytes; false: its rows do not start on 16-byte boundaries
+// rows x M of the output in pieces of 32 rows x 128 bytes; false: its rows do not start or end on 16-byte boundaries (a
+// store that is clipped at the map's end writes whole 16 bytes)
 template <typename O>
 bool make_out_map(CUtensorMap* map, void* y, int rows, int M, long ld) {
   EncodeTiledFn fn = encode_fn();
-  if (!fn || !al16(y) || ld * (long)sizeof(O) % 16 != 0 || ld * (long)sizeof(O) >= 1L << 40) return false;
+  if (!fn || !al16(y) || ld * (long)sizeof(O) % 16 != 0 || M * (long)sizeof(O) % 16 != 0 || ld * (long)sizeof(O) >= 1L << 40) return false;
   cuuint64_t dims[2] = {(cuuint64_t)M, (cuuint64_t)rows};
   cuuint64_t strides[1] = {(cuuint64_t)ld * sizeof(O)};
   cuuint32_t box[2] = {128 / sizeof(O), 32};
@@ -381,28 +413,32 @@ bool make_out_map(CUtensorMap* map, void* y, int rows, int M, long ld) {
             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// about what a call takes here, in ns: 5.5 us for the launch and the first copies, 0.455 us a block of K, the end of a tile
-double pair_ns(const Product& p, bool gated) {
-  const double tiles = (double)((p.N + 2 * kBM - 1) / (2 * kBM)) * ((p.M + (gated ? kHalf : kBN) - 1) / (gated ? kHalf : kBN));
-  return 5500 + std::ceil(tiles / std::max(1, sm_count() / 2)) * (p.kb * 455. + (gated ? 1500 : 700));
+// About what a call takes in tiles of bn features, in ns: 5.5 us for the launch and the first copies, a block of K of every tile, the end of a tile.  Narrow tiles have shorter blocks, wide ones
+// less traffic for as much work, so the widths differ in how well their tiles fill the SMs.  B200, 256 : 192 : 128, us: 512 tokens of 2560 x 9728 38.9 : 31.5 : 24.6, 168 of 8192 x 4096 20.9 :
+// 17.4 : 14.3, 333 of 6144 x 2560 15.1 : 13.0 : 15.4, 256 of 24576 x 4096 40.0 : 32.9 : 33.2, 1024 of 4096 x 4096 21.4 : 29.6 : 22.3, 426 of 16384 x 9728 82.3 : 90.2 : 91.0, 4096 of 24576 x 4096
+// 372 : 393 : 405.  Of 50 drawn shapes the choice among these and the kernel for few tokens was within 3 % of the best at 42, 17 % behind at the worst (848 of 512 x 2560, 9.1 us).
+double pair_ns(const Product& p, bool gated, int bn) {
+  const int features = gated ? kBlock : bn;
+  const double tiles = (double)((p.N + 2 * kBM - 1) / (2 * kBM)) * ((p.M + features - 1) / features);
+  return 5500 + std::ceil(tiles / std::max(1, sm_count() / 2)) * (p.kb * (bn == 256 ? 455. : bn == 192 ? 345. : 250.) + (gated ? 1500 : 700));
 }
 
-template <bool GATED, typename O>
+template <int BN, bool GATED, typename O>
 int launch_pair(const Product& product, cudaStream_t st) {
-  constexpr int features = GATED ? kHalf : kBN;
+  constexpr int features = GATED ? kBlock : BN;
   Product p = product;
   const long tiles = (long)((p.N + 2 * kBM - 1) / (2 * kBM)) * ((p.M + features - 1) / features);
   const int pairs = (int)std::min<long>(std::max(1, sm_count() / 2), tiles);
   if (tiles > 0x7fffffffL - 4 * pairs) return -2;
   p.tiles = (int)tiles;
-  auto kern = fp8_gemm_kernel<GATED, O>;
+  auto kern = fp8_gemm_kernel<BN, GATED, O>;
   static std::atomic<uint64_t> set{0};
   if (const cudaError_t e = allow_smem(set, (const void*)kern, kSmem); e != cudaSuccess) return (int)e;
   CUtensorMap mx, mw, mw2{}, my{};
-  if (!make_codes_map(&mx, p.x, p.N, p.K, p.ld_x, kBM) || !make_codes_map(&mw, p.w, p.M, p.K, p.ld_w, kHalf) || (GATED && !make_codes_map(&mw2, p.w2, p.M, p.K, p.ld_w, kHalf)))
+  if (!make_codes_map(&mx, p.x, p.N, p.K, p.ld_x, kBM) || !make_codes_map(&mw, p.w, p.M, p.K, p.ld_w, BN / 2) || (GATED && !make_codes_map(&mw2, p.w2, p.M, p.K, p.ld_w, BN / 2)))
     return (int)cudaErrorInvalidValue;
   if constexpr (!GATED) p.y_map = make_out_map<O>(&my, p.y, p.N, p.M, p.ld_y);
-  return (int)launch(kern, dim3(2 * pairs), dim3(kThreads), kSmem, st, true, mx, mw, mw2, my, p);
+  return (int)launch(kern, dim3(2 * pairs), dim3(threads_of(BN)), kSmem, st, true, mx, mw, mw2, my, p);
 }
 
 }  // namespace
@@ -435,8 +471,11 @@ extern "C" int pk_fp8_gemm(const void* w, long ld_w, const float* w_scales, cons
   p.K = K;
   p.kb = fp8::blocks_of(K);
   p.err = wait_err_word();
-  if (const int rc = fp8::launch_few(p, false, y_f32, fp8::pair_ns(p, false), st); rc != -2) return rc;
-  return y_f32 ? fp8::launch_pair<false, float>(p, st) : fp8::launch_pair<false, bf16>(p, st);
+  const double ns256 = fp8::pair_ns(p, false, 256), ns192 = fp8::pair_ns(p, false, 192), ns128 = fp8::pair_ns(p, false, 128), least = std::min({ns256, ns192, ns128});
+  if (const int rc = fp8::launch_few(p, false, y_f32, least, st); rc != -2) return rc;
+  if (ns128 == least) return y_f32 ? fp8::launch_pair<128, false, float>(p, st) : fp8::launch_pair<128, false, bf16>(p, st);
+  if (ns192 == least) return y_f32 ? fp8::launch_pair<192, false, float>(p, st) : fp8::launch_pair<192, false, bf16>(p, st);
+  return y_f32 ? fp8::launch_pair<256, false, float>(p, st) : fp8::launch_pair<256, false, bf16>(p, st);
 }
 
 extern "C" int pk_fp8_gemm_gated(const void* w_gate, const float* gate_scales, const void* w_up, const float* up_scales, long ld_w, const void* x, long ld_x,
@@ -465,6 +504,6 @@ extern "C" int pk_fp8_gemm_gated(const void* w_gate, const float* gate_scales, c
   p.kb = fp8::blocks_of(K);
   p.act = act;
   p.err = wait_err_word();
-  if (const int rc = fp8::launch_few(p, true, false, fp8::pair_ns(p, true), st); rc != -2) return rc;
-  return fp8::launch_pair<true, uint8_t>(p, st);
+  if (const int rc = fp8::launch_few(p, true, false, fp8::pair_ns(p, true, 256), st); rc != -2) return rc;
+  return fp8::launch_pair<256, true, uint8_t>(p, st);
 }

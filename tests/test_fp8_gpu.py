@@ -265,6 +265,33 @@ def test_gemm_rows_of_any_stride(lib, T, M, ld, off, f32):
     assert (y[:, M:] == 7).all()
 
 
+@pytest.mark.parametrize("T,M,K,ld,off", [(257, 4100, 4000, 4104, 0), (300, 4095, 3900, 0, 0), (200, 8100, 1000, 8101, 1),  # as few waves of narrow tiles as of wide ones,
+                                          (300, 9610, 300, 9616, 0), (333, 6145, 2560, 0, 1), (520, 9611, 400, 9700, 0), (150, 24500, 130, 0, 0),  # fewer than of the narrowest,
+                                          (2100, 24500, 300, 24504, 0), (430, 16383, 520, 0, 0)])  # fewer of the widest than of any
+@pytest.mark.parametrize("f32", [False, True])
+def test_gemm_of_tiles_of_any_width(lib, T, M, K, ld, off, f32):
+    ops = operands(T, M, K, gen(T, M, K), wild=T % 2 == 1)
+    y = gemm(lib, ops, T, M, K, f32, ld=ld, off=off)
+    near(y[:, :M], *R.product(*ops, T, M, K))
+    assert (y[:, M:] == 7).all()
+
+
+def with_nan_behind(codes, K):
+    codes = codes.clone()
+    codes[:, K:] = 0x7f
+    return codes
+
+
+@pytest.mark.parametrize("T", [3, 50, 120, 300])
+@pytest.mark.parametrize("K", [1, 5, 127, 129, 515])
+def test_products_use_nothing_behind_the_width(lib, T, K):
+    M = 200
+    xc, xs, wc, ws = operands(T, M, K, gen(T, K, 6), pad=1)
+    ops = with_nan_behind(xc, K), xs, with_nan_behind(wc, K), ws
+    near(gemm(lib, ops, T, M, K), *R.product(*ops, T, M, K))
+    hold_gated(*gated(lib, ops, ops[2:], T, M, K, 1), ops, ops[2:], T, M, K, 1)
+
+
 @pytest.mark.parametrize("T", [3, 50, 120, 400])
 def test_gemm_with_scales_of_any_size_and_sign(lib, T):
     M, K = 1200, 1100
