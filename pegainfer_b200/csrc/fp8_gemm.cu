@@ -13,7 +13,7 @@
 // MMAs 512.  Without the sums' work 312, with half of the operands' bytes 324, without both 244: a partial sum's way (MMAs, commit, 64 columns out and added by 16 warps, arrival in the other
 // CTA: 1800 clocks, two of them under way) and the 32 KB a CTA reads of L2 for it (34 bytes a clock and SM) bound it together.  What it took to come here: 770 with a release at the cluster's scope in
 // the arrivals, 479 with 8 warps that hold 128 columns, 399 with sums and addresses that did not fit registers, 380 with tiles that leave by TMA (3300 clocks a tile before).  Measured and not
-// kept: halves of 128 columns with barriers of their own (A is read twice: 401), 16 columns at a time (428), packed fp32 products (equal), other orders of the tiles (389 to 431), 3 stages (386), 6
+// kept: halves of 128 columns with barriers of their own (A is read twice: 401), 16 columns at a time (428), other orders of the tiles (389 to 431), 3 stages (386), 6
 // (equal).  Tiles of 128, whose MMAs take 256 clocks a block, are at 460: 350 without the sums' work and with weights in L2; four partial sums carry them (with two 590), and so do 64 columns at once
 // by 8 warps (32 by 16: 590).  Weights asked into L2 eight to 32 blocks ahead: equal.
 // Every barrier wait is bounded (mbar_wait_bounded, common.cuh).
@@ -102,6 +102,36 @@ __device__ __forceinline__ void store_piece(const CUtensorMap* map, uint32_t pie
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(c0), "r"(c1), "r"(piece) : "memory");
   asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
+
+// A thread's 64 sums, two to an instruction or one.  B200, us, one : two: 512 tokens of 2560 x 9728 (tiles of 128) 24.5 : 23.3, gated 200 of 9728 x 2560 28.9 : 28.5; but in tiles of 192 and 256,
+// whose registers are short for pairs side by side, 333 of 6144 x 2560 13.1 : 13.7, 4096 of 4096 x 4096 70.2 : 74.7
+template <bool TWO>
+struct Sums {
+  float v[64];
+  __device__ __forceinline__ Sums() {
+#pragma unroll
+    for (int j = 0; j < 64; ++j) v[j] = 0.f;
+  }
+  __device__ __forceinline__ void add(int at, const uint32_t* u, float scale) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[at + j] = fmaf(__uint_as_float(u[j]), scale, v[at + j]);
+  }
+  __device__ __forceinline__ float operator[](int j) const { return v[j]; }
+};
+template <>
+struct Sums<true> {
+  uint64_t v[32];
+  __device__ __forceinline__ Sums() {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = 0;
+  }
+  __device__ __forceinline__ void add(int at, const uint32_t* u, float scale) {
+    const uint64_t s = pair_of(scale, scale);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[at / 2 + j] = fma2(pair_of(u[2 * j], u[2 * j + 1]), s, v[at / 2 + j]);
+  }
+  __device__ __forceinline__ float operator[](int j) const { return j & 1 ? hi_of(v[j / 2]) : lo_of(v[j / 2]); }
+};
 
 template <int ACT>
 __device__ __forceinline__ void activate(const float* acc, float* v) {  // acc: 32 of the gate, 32 of the factor
@@ -290,9 +320,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
     bool ready = false;
     for (int tile = pair; tile < num_tiles; tile += num_pairs, ++lt) {
       if (BN % kBlock) scales = scales_of(tile / m_tiles & 1);  // (a tile of 192 begins at a block or in the middle of one)
-      float acc[64];
-#pragma unroll
-      for (int j = 0; j < 64; ++j) acc[j] = 0.f;
+      Sums<GATED || BN == 128> sums;
 #pragma unroll 1
       for (int kb = kb_n; kb > 0; --kb) {
         const uint32_t buf = it % kSums;
@@ -307,8 +335,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
         ++it;
         if constexpr (kAtOnce == 32) {
           tmem_wait32(v);
-#pragma unroll
-          for (int j = 0; j < 32; ++j) acc[j] = fmaf(__uint_as_float(v[j]), s1, acc[j]);
+          sums.add(0, v, s1);
           tmem_ld32_nowait(t0 + kPiece, v);
         }
         ready = test_wait_at(tfull + it % kSums * 8u, it / kSums & 1);  // (asked for early)
@@ -317,13 +344,12 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
         tc_fence_before();
         __syncwarp();
         if (lane == 0) arrive_relaxed(tempty + buf * 8u);
-        if constexpr (kAtOnce == 64) {
-#pragma unroll
-          for (int j = 0; j < 32; ++j) acc[j] = fmaf(__uint_as_float(v[j]), s1, acc[j]);
-        }
-#pragma unroll
-        for (int j = 0; j < 32; ++j) acc[32 + j] = fmaf(__uint_as_float(v[kAtOnce - 32 + j]), s2, acc[32 + j]);
+        if constexpr (kAtOnce == 64) sums.add(0, v, s1);
+        sums.add(32, v + kAtOnce - 32, s2);
       }
+      float acc[64];
+#pragma unroll
+      for (int j = 0; j < 64; ++j) acc[j] = sums[j];
       const int mb = tile % m_tiles, nb = tile / m_tiles;
       const int tok = mb * 2 * kBM + (int)rank * kBM + row;
       const int f0 = GATED ? nb * kHalf + part * 32 : nb * BN + part * 64;  // the thread's first feature
