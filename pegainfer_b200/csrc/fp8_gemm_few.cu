@@ -8,7 +8,7 @@
 // Any number of rows may make a tile: the MMAs read 128, and what lies behind the tile's own ends in lanes that nobody reads.
 // One CTA has an SM: a second one on it would start 1 us later, and a cluster of eight with two on an SM 2 us.
 //
-// What bounds it, B200, 48 tokens of 4096 x 12288 (51 MB), us: 14.6, of them 2 between launches, 3 to the first block (1.2 from the launch to the first copy's start; all rings are asked for at
+// What bounds it, B200, 48 tokens of 4096 x 12288 (51 MB), us: 14.8, of them 2 between launches, 3 to the first block (1.2 from the launch to the first copy's start; all rings are asked for at
 // once, so the first stage comes behind parts of the others), 7.5 for the stream (6.7 TB/s), 2 for the joining.  One token of 2560 x 4096: 6.6, the same without the stream.
 // A cluster's joining, measured: words sent by the threads that have them 16.7, bulk copies from shared to shared memory 18.1, 16 bytes a thread of a part laid down feature by feature 15.8
 // (then two groups of warps for the sums: 15.0; parts fetched behind a barrier instead, with two CTAs an SM: 15.6).
@@ -57,6 +57,7 @@ struct FewPlan {
   int n_tiles;               // tiles of tokens
   int own;                   // features (gated: tokens, a multiple of four) of the tile that a CTA adds up
   double ns;                 // what a call takes, about
+  uint32_t zero;             // 0, which the compiler does not know
 };
 constexpr size_t stage_bytes(int na, int rows, int nt) { return (size_t)(na * rows + nt) * kBK; }
 // floats from one feature of a part to the next: the lanes' 16-byte accesses at one token fall on different banks
@@ -210,12 +211,17 @@ fp8_gemm_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       if (!done) mbar_wait_bounded(tfull + buf, tph, dead);
       tc_fence_after();
       const uint32_t t0 = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)((buf * NA + h) * NT + c0);
-      auto release = [&]() {
+      // The stage goes back when its scales are in registers.  An arrival does not wait for loads on their way: with nothing more the copy of the stage's next block overtook the last of them
+      // once in some 1e8 blocks.  So its address takes a word of each of the last loads (a warp's loads of shared memory return in order): 1 to 2 % of a call, a proxy fence 3 to 5 %, words of
+      // all loads up to 20 %.
+      auto release = [&](uint32_t read) {
         tc_fence_before();
+        uint32_t bar = smem_u32(empty + s);
+        asm volatile("{\n.reg .b32 t;\nand.b32 t, %1, %2;\nadd.u32 %0, %0, t;\n}" : "+r"(bar) : "r"(read), "r"(plan.zero));
         __syncwarp();
         if (lane == 0) {
           mbar_arrive(tempty + buf);
-          mbar_arrive(empty + s);
+          asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
         }
       };
       auto add4 = [&](int at, const uint32_t* u, float4 x) {
@@ -233,7 +239,7 @@ fp8_gemm_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
         uint32_t* now = v[(c / 16) & 1];
         tmem_wait16(now);
         if (c + 16 < COLS) tmem_ld16(t0 + (uint32_t)(c + 16), v[(c / 16 + 1) & 1]);
-        else release();
+        else release(__float_as_uint(x[0].x) | __float_as_uint(x[1].x) | __float_as_uint(x[2].x) | __float_as_uint(x[3].x));
 #pragma unroll
         for (int j = 0; j < 4; ++j) add4(c + 4 * j, now + 4 * j, x[j]);
       }
@@ -368,7 +374,7 @@ FewPlan few_plan(int M, int N, int kb, int na, int nt, bool gated, const int* re
     const int S = 1 << i;
     if (S > 1 && (S > kb / 2 || resident[i] < 1 || (!gated && na == 2))) continue;  // at least two blocks a part
     const int at_once = std::max(1, resident[i]);
-    FewPlan p{kRows, S, 2, n_tiles, 0, 0};
+    FewPlan p{kRows, S, 2, n_tiles, 0, 0, 0};
     const long tiles = (long)((M + per_tile - 1) / per_tile) * n_tiles;
     const long waves = (tiles + at_once - 1) / at_once;
     if (!gated) {

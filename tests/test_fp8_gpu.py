@@ -319,6 +319,20 @@ def test_gemm_keeps_what_is_not_finite_apart(lib, T):
     assert torch.equal(torch.isnan(y), bad) and torch.equal(y[~bad], before[~bad])
 
 
+@pytest.mark.parametrize("T,M,K", [(28, 19000, 3000), (40, 9728, 2500), (100, 2560, 2900), (300, 19000, 2800)])
+def test_gemm_takes_every_block_with_its_own_scale(lib, T, M, K):
+    """a power of two for a block, so that the sum tells which were taken: exact, every time of many"""
+    kb = R.blocks(K)
+    xc, wc = torch.full((T, R.up(K, 16)), 0x38, dtype=U8, device="cuda"), torch.zeros(M, R.up(K, 16), dtype=U8, device="cuda")
+    wc[:, 0:K:128] = 0x38  # one product of 1 a block
+    xs, ws = (2.0 ** torch.arange(kb, device="cuda").float())[:, None].repeat(1, R.up(T, 4)).contiguous(), torch.ones(R.blocks(M), kb, device="cuda")
+    y, wrong = torch.zeros(T, M, device="cuda"), torch.zeros((), device="cuda", dtype=torch.int64)
+    for _ in range(1500):
+        gemm(lib, (xc, xs, wc, ws), T, M, K, True, y=y)
+        wrong += (y != 2.0 ** kb - 1).sum()
+    assert wrong.item() == 0
+
+
 @pytest.mark.parametrize("T", [5, 64, 130])
 def test_gemm_gives_a_token_its_bits_whatever_the_others_hold(lib, T):
     M, K = 513, 1300
