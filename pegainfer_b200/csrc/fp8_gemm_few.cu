@@ -67,7 +67,7 @@ size_t received_bytes(int na, const FewPlan& p, int nt, bool gated) { return p.s
 size_t few_smem(int na, const FewPlan& p, int nt, bool gated) {
   return p.stages * (stage_bytes(na, p.rows, nt) + nt * sizeof(float)) + (size_t)(kRows - p.rows) * kBK + received_bytes(na, p, nt, gated) + 1024 + (2 * kMaxStages + 4) * 8 + 16;
 }
-constexpr int tmem_columns(int na, int nt) { return 2 * na * nt <= 32 ? 32 : 2 * na * nt <= 64 ? 64 : 2 * na * nt <= 128 ? 128 : 2 * na * nt <= 256 ? 256 : 512; }
+constexpr int tmem_columns(int na, int nt) { return 2 * na * nt <= 32 ? 32 : 2 * na * nt <= 64 ? 64 : 2 * na * nt <= 128 ? 128 : 256; }
 
 // groups of four warps that take sums out of tensor memory: one to a tile of A, two where one tile has many columns (128 tokens: a block takes one group 530 ns)
 constexpr int groups(int na, int nt) { return na == 1 && nt >= 64 ? 2 : na; }
@@ -79,7 +79,7 @@ fp8_gemm_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
                     const FewPlan plan) {
   constexpr int GROUPS = groups(NA, NT), COLS = NT * NA / GROUPS, THREADS = 96 + 128 * GROUPS;  // COLS: columns of a thread
   constexpr uint32_t TMEM_COLS = tmem_columns(NA, NT);
-  static_assert(2 * NA * NT <= 512 && (!GATED || NA == 2), "tensor memory");
+  static_assert(2 * NA * NT <= 256 && (!GATED || NA == 2), "tensor memory");
   const int stages = plan.stages, rows = plan.rows;
   const uint32_t A_BYTES = rows * kBK, STAGE = NA * A_BYTES + NT * kBK;
   extern __shared__ uint8_t smem_raw[];
