@@ -782,7 +782,8 @@ int pk_kv8_evict(void* cache, long page_stride, int page_size, const int* page_o
  * What a call writes overlaps nothing that it reads (x of the norm, which it does both to, aside).
  * Nothing is allocated and there are no workspaces, so calls may run at the same time and be captured.  -1: invalid argument, -2: sizes outside the kernels' range. */
 /* x[t] += y[t] (y bf16, NULL: nothing is added and x not written; x bf16, rounded when stored, or float);  codes of x[t] / sqrt(mean(x[t]^2) + eps) * (offset + w), of the
- * unrounded sum.  x, y [tokens, width], w [width] bf16, offset 0 or 1 as the weights are kept.  y is another array than x.  width up to 16384. */
+ * unrounded sum.  x, y [tokens, width], w [width] bf16, offset 0 or 1 as the weights are kept.  y is another array than x.  width up to 16384.  The sum of a row's squares is an fp32
+ * number: it holds entries of up to 2^56 at any width; a row whose sum passes it has codes of zero. */
 int pk_fp8_add_norm(const void* y, void* x, int x_f32, const void* w, float offset, void* codes, long ld, float* scales, long ld_s, int width, int tokens, float eps,
                     pk_stream st);
 /* codes of the activated rows.  in bf16, rows of ld_in elements (0: as many as are read).  kind as for pk_act_ex: 0 silu(in[t][f]) * in[t][F + f], 1 relu(in[t][f])^2,

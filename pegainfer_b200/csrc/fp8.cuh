@@ -72,12 +72,14 @@ __device__ __forceinline__ float max_abs(float a, float b, float c) {
 __device__ __forceinline__ float max8(const float* v) {
   return max_abs(max_abs(v[0], v[1], v[2]), max_abs(v[3], v[4], v[5]), max_abs(v[6], v[7]));
 }
-// the largest of 16 lanes, which have a block together
-__device__ __forceinline__ float max16(float m) {
+// the largest of 16 lanes, which have a block together; lanes: those that are here
+__device__ __forceinline__ float max16(float m, uint32_t lanes = 0xffffffffu) {
 #pragma unroll
-  for (int o = 8; o > 0; o >>= 1) m = max_abs(m, __shfl_xor_sync(0xffffffffu, m, o));
+  for (int o = 8; o > 0; o >>= 1) m = max_abs(m, __shfl_xor_sync(lanes, m, o));
   return m;
 }
+// a block's largest magnitude that gives a scale without the floor
+__device__ __forceinline__ bool in_range(float amax) { return amax >= kLeast && amax < INFINITY; }
 
 struct Scale {
   float s, inv;  // NaN where the block has an entry that is not finite

@@ -1,6 +1,6 @@
 // Rows of activations quantised to 8 bits where they are made (fp8.cuh): RMS norm with the residual's addition, gated activations, and rows as they are.
 // All of them are one pass over memory: 16 lanes have a block of 128 entries, 8 each, and find its scale by four exchanges.
-// B200, GPU time of one call in a row of them: norm of 4096 x 4096 with float x 30.6 us (185 MB, 6.04 TB/s), with bf16 x 23.4 (5.0 TB/s), of one token 2.0; silu product of 4096 x 12288 42.5
+// B200, GPU time of one call in a row of them: norm of 4096 x 4096 with float x 30.6 us (185 MB, 6.04 TB/s), with bf16 x 23.9 (4.9 TB/s), of one token 2.1; silu product of 4096 x 12288 42.5
 // (253 MB, 5.95 TB/s), of 32 x 12288 2.0.  Memory bounds the large ones (a copy reaches 6.54 TB/s), the launch the small ones.
 #include "fp8.cuh"
 
@@ -9,11 +9,13 @@ namespace fp8 {
 
 // x += y (rounded when stored), v = x * rsqrt(mean(x^2) + eps) * (offset + w) of the unrounded x, quantised.  A CTA has a row, in registers from its load to its codes, NV pieces of 8
 // entries a thread and as many warps as that takes.
-// A code is v over its block's largest v, in which the root cancels: codes come from x * (offset + w), with two roundings less, and only the scales wait for the row's sum.
+// A code is v over its block's largest v, in which the root cancels: codes come from x * (offset + w), with two roundings less, and only the scales wait for the row's sum.  A block whose
+// largest such product has no scale of its own (below 2^-100, the root may bring it above; or past fp32, the root may bring it back) keeps x instead, and its codes wait for the root.
 constexpr int kNormWarps = 32, kNormWidest = kNormWarps * 256 * 2;
 
+// Registers: with 40 two pieces have six CTAs of eight warps on an SM (4096 x 4096 bf16 23.9 us; with the 52 that the compiler takes by itself 27.8).
 template <typename E, int NV, bool VEC>
-__global__ void __launch_bounds__(32 * kNormWarps) fp8_add_norm_kernel(const bf16* __restrict__ y, E* __restrict__ x, const bf16* __restrict__ w, float offset,
+__global__ void __maxnreg__(NV == 2 ? (VEC ? 40 : 56) : 32) fp8_add_norm_kernel(const bf16* __restrict__ y, E* __restrict__ x, const bf16* __restrict__ w, float offset,
                                                                       uint8_t* __restrict__ codes, long ld, float* __restrict__ scales, long ld_s, int width, float eps) {
   __shared__ float red[kNormWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
@@ -49,16 +51,20 @@ __global__ void __launch_bounds__(32 * kNormWarps) fp8_add_norm_kernel(const bf1
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     const int at = first_of<VEC>(j * blockDim.x + threadIdx.x);
-    float g[8];
+    float g[8], times[8];
     load8<VEC>(w + at, width - at, g);
 #pragma unroll
     for (int e = 0; e < 8; e += 2) {  // (behind the width both are zero)
-      const uint64_t u = pair_of(v[j][e], v[j][e + 1]), t = mul2(u, add2(pair_of(offset, offset), pair_of(g[e], g[e + 1])));
+      const uint64_t u = pair_of(v[j][e], v[j][e + 1]), p = mul2(u, add2(pair_of(offset, offset), pair_of(g[e], g[e + 1])));
       squares = fma2(u, u, squares);
-      v[j][e] = lo_of(t);
-      v[j][e + 1] = hi_of(t);
+      times[e] = lo_of(p);
+      times[e + 1] = hi_of(p);
     }
-    m[j] = max16(max8(v[j]));
+    m[j] = max16(max8(times));
+    if (in_range(m[j])) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[j][e] = times[e];
+    }
   }
   float ss = warp_sum(lo_of(squares) + hi_of(squares));
   if (warps > 1) {
@@ -70,16 +76,24 @@ __global__ void __launch_bounds__(32 * kNormWarps) fp8_add_norm_kernel(const bf1
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     const int at = first_of<VEC>(j * blockDim.x + threadIdx.x);
-    if (at >= width) break;
-    const Scale k = scale_of(m[j] * r);
-    if (m[j] * r > kLeast) {
-      store_codes8<VEC>(codes + t * ld + at, width - at, v[j], scale_of(m[j]));
-    } else {  // the least scale, or none (NaN)
+    Scale k = scale_of(m[j] * r), from = scale_of(m[j]);
+    if (const bool kept = !in_range(m[j]); kept || !(m[j] * r > kLeast)) {  // (the block's 16 lanes are of one mind)
+      if (kept) {
+        float g[8];
+        load8<VEC>(w + at, width - at, g);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[j][e] *= r;
-      store_codes8<VEC>(codes + t * ld + at, width - at, v[j], k);
+        for (int e = 0; e < 8; ++e) v[j][e] = v[j][e] * r * (offset + g[e]);
+        k = scale_of(max16(max8(v[j]), 0xffffu << (lane & 16)));
+      } else {  // the least scale
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[j][e] *= r;
+      }
+      from = k;
     }
-    if ((lane & 15) == 0) scales[(size_t)(at / kBlock) * ld_s + t] = k.s;
+    if (at < width) {
+      store_codes8<VEC>(codes + t * ld + at, width - at, v[j], from);
+      if ((lane & 15) == 0) scales[(size_t)(at / kBlock) * ld_s + t] = k.s;
+    }
   }
 }
 
