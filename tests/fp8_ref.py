@@ -109,6 +109,12 @@ def product(xc, xs, wc, ws, T, M, K):
     return x @ w.T, x.abs() @ w.abs().T
 
 
+def hold_product(y, want, size):
+    """y within one rounding of the result and the sum's bound (`size`: of its products' magnitudes); NaN is within nothing"""
+    ok = (y.double() - want).abs() <= want.abs() * (torch.finfo(y.dtype).eps / 2) + size * SUM
+    assert ok.all(), ((~ok).sum().item(), (~ok).nonzero()[:4].tolist(), y[~ok][:4].tolist(), want[~ok][:4].tolist())
+
+
 def act(kind, a, b=None):
     """pk_fp8_act's kinds (GELU by the logistic function: 1 + tanh of a large negative number loses its bits in 64 of them too)"""
     f = torch.nn.functional
