@@ -57,6 +57,11 @@ __device__ __forceinline__ float exp2_ftz(float v) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
   return r;
 }
+__device__ __forceinline__ float exp2_any(float v) {  // (those below 2^-126 too)
+  float r;
+  asm("ex2.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
 
 // the largest magnitude; infinities and NaN stay
 __device__ __forceinline__ float max_abs(float a, float b) {
@@ -187,14 +192,39 @@ __device__ __forceinline__ void store_codes8(uint8_t* p, int n, const float* v, 
   }
 }
 
-// act 0 SiLU, 1 ReLU, 2 GELU in its tanh form, of z: z times the logistic function of z or of sqrt(8 / pi) (z + 0.044715 z^3).  The special-function unit's exponential and quotient
-// without their ways for subnormal numbers, which took half of the instructions; what they lose lies below the least scale's codes.
+// act 0 SiLU, 1 ReLU, 2 GELU in its tanh form, of z, times u.  SiLU and GELU: z times the logistic function of z or of sqrt(8 / pi) (z + 0.044715 z^3), as z / (1 + 2^x) by the
+// special-function unit's exponential and quotient without their ways for subnormal numbers, which took half of the instructions.  That loses gates whose 1 + 2^x has no normal reciprocal
+// (x from 126 on), and times a large factor they count: they are (z 2^(-x/2)) (2^(-x/2) u).
 template <int ACT>
-__device__ __forceinline__ float gate_act(float z) {
-  if constexpr (ACT == 1) return z < 0.f ? 0.f : z;  // (NaN stays)
+__device__ __forceinline__ float gate_exponent(float z) {
   constexpr float kLog2e = 1.4426950408889634f, kGelu = -1.5957691216057308f * kLog2e;
-  const float x = ACT == 2 ? z * fmaf(z * z, 0.044715f * kGelu, kGelu) : z * -kLog2e;
-  return z * rcp_ftz(1.f + exp2_ftz(x));
+  return ACT == 2 ? z * fmaf(z * z, 0.044715f * kGelu, kGelu) : z * -kLog2e;
+}
+__host__ __device__ constexpr float far_below(int act) { return act == 2 ? -9.9f : -84.f; }  // (x = 122.7, 121.2)
+__device__ __forceinline__ float far_gated(float z, float x, float u) {
+  const float h = exp2_any(-0.5f * x);
+  return (z * h) * (h * u);
+}
+template <int ACT>
+__device__ __forceinline__ float near_gated(float z, float u) {
+  if constexpr (ACT == 1) return (z < 0.f ? 0.f : z) * u;  // (NaN stays)
+  return z * rcp_ftz(1.f + exp2_ftz(gate_exponent<ACT>(z))) * u;
+}
+// eight gates z with their factors u, to v (which may be z); true: some are far, and their results not in v yet
+template <int ACT>
+__device__ __forceinline__ bool gated8(const float* z, const float* u, float* v) {
+  float least = z[0];
+#pragma unroll
+  for (int j = 1; j < 8; ++j) least = fminf(least, z[j]);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = near_gated<ACT>(z[j], u[j]);
+  return ACT != 1 && least < far_below(ACT);
+}
+template <int ACT>
+__device__ __forceinline__ void far_gated8(const float* z, const float* u, float* v) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (z[j] < far_below(ACT)) v[j] = far_gated(z[j], gate_exponent<ACT>(z[j]), u[j]);
 }
 
 }  // namespace fp8

@@ -136,7 +136,8 @@ struct Sums<true> {
 template <int ACT>
 __device__ __forceinline__ void activate(const float* acc, float* v) {  // acc: 32 of the gate, 32 of the factor
 #pragma unroll
-  for (int j = 0; j < 32; ++j) v[j] = gate_act<ACT>(acc[j]) * acc[32 + j];
+  for (int j = 0; j < 32; j += 8)
+    if (__builtin_expect(gated8<ACT>(acc + j, acc + 32 + j, v + j), 0)) far_gated8<ACT>(acc + j, acc + 32 + j, v + j);
 }
 
 // BN: features of a tile; gated: 256, O is the codes' type

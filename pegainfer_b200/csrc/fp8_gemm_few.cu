@@ -306,7 +306,7 @@ fp8_gemm_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
         if (4 * c + e < tokens) dst[(size_t)e * p.ld_y] = from_f<O>(o[e]);
     }
   } else {
-    // a warp has a token's 128 features, a block of the result's scales: a lane every 32nd.  The exponent of pk_fp8_act's formulas as c1 z + c2 z^3 for both
+    // a warp has a token's 128 features, a block of the result's scales: a lane every 32nd.  The exponent as c1 z + c2 z^3 for both (fp8.cuh has the formulas)
     const int mine = max(0, min(own, tokens - sp * own)), ld = S > 1 ? own : LD;
     const float c1 = p.act == 2 ? -2.302208198f : -1.4426950408889634f, c2 = p.act == 2 ? -0.1029432396f : 0.f;
 #pragma unroll 1
@@ -321,8 +321,9 @@ fp8_gemm_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
           z += from[r * 256 * ld];
           u += from[(r * 256 + 128) * ld];
         }
-        const float gate = z * rcp_ftz(1.f + exp2_ftz(z * fmaf(fminf(z * z, 1e30f), c2, c1)));
-        v[j] = (p.act == 1 ? (z < 0.f ? 0.f : z) : gate) * u;
+        const float x = z * fmaf(fminf(z * z, 1e30f), c2, c1);
+        v[j] = (p.act == 1 ? (z < 0.f ? 0.f : z) : z * rcp_ftz(1.f + exp2_ftz(x))) * u;
+        if (p.act != 1 && z < far_below(p.act)) v[j] = far_gated(z, x, u);
       }
       const float m = max16(max_abs(max_abs(v[0], v[1], v[2]), v[3]));
       const Scale k = scale_of(max_abs(m, __shfl_xor_sync(0xffffffffu, m, 16)));

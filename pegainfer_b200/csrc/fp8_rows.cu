@@ -1,7 +1,7 @@
 // Rows of activations quantised to 8 bits where they are made (fp8.cuh): RMS norm with the residual's addition, gated activations, and rows as they are.
 // All of them are one pass over memory: 16 lanes have a block of 128 entries, 8 each, and find its scale by four exchanges.
-// B200, GPU time of one call in a row of them: norm of 4096 x 4096 with float x 30.6 us (185 MB, 6.04 TB/s), with bf16 x 23.9 (4.9 TB/s), of one token 2.1; silu product of 4096 x 12288 42.5
-// (253 MB, 5.95 TB/s), of 32 x 12288 2.0.  Memory bounds the large ones (a copy reaches 6.54 TB/s), the launch the small ones.
+// B200, GPU time of one call in a row of them: norm of 4096 x 4096 with float x 30.6 us (185 MB, 6.04 TB/s), with bf16 x 23.9 (4.9 TB/s), of one token 2.1; silu product of 4096 x 12288 42.3
+// (253 MB, 6.0 TB/s), gelu 45, relu 38.7, relu2 29.6 and plain rows 26.5 (153 MB, 5.75 TB/s), silu of 32 x 9728 2.2.  Memory bounds the large ones (a copy reaches 6.54 TB/s), the launch the small ones.
 #include "fp8.cuh"
 
 namespace pk {
@@ -126,8 +126,16 @@ __global__ void __launch_bounds__(kActThreads) fp8_act_kernel(const bf16* __rest
         v[r][e] = z * z;
       }
     } else if constexpr (KIND != 4) {
+      constexpr int ACT = KIND == 0 ? 0 : KIND - 1;
+      if (__builtin_expect(gated8<ACT>(v[r], u[r], v[r]), 0)) {  // (read again, one by one: gates and factors kept until here took twice the registers, 46.4 us for 41.7)
+        const bf16* row = in + (size_t)(n > 0 ? t0 + r : 0) * ld_in + at;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[r][e] = gate_act<KIND == 0 ? 0 : KIND - 1>(v[r][e]) * u[r][e];
+        for (int e = 0; e < 8; ++e) {
+          const int i = VEC ? e : 16 * e;
+          const float z = load_if(row + i, i < n);
+          if (z < far_below(ACT)) v[r][e] = far_gated(z, gate_exponent<ACT>(z), load_if(row + F + i, i < n));
+        }
+      }
     }
     const Scale k = scale_of(max16(max8(v[r])));
     if (n > 0) {
