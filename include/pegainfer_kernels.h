@@ -787,7 +787,8 @@ int pk_kv8_evict(void* cache, long page_stride, int page_size, const int* page_o
 int pk_fp8_add_norm(const void* y, void* x, int x_f32, const void* w, float offset, void* codes, long ld, float* scales, long ld_s, int width, int tokens, float eps,
                     pk_stream st);
 /* codes of the activated rows.  in bf16, rows of ld_in elements (0: as many as are read).  kind as for pk_act_ex: 0 silu(in[t][f]) * in[t][F + f], 1 relu(in[t][f])^2,
- * 2 relu(in[t][f]) * in[t][F + f], 3 gelu_tanh(in[t][f]) * in[t][F + f];  4: in[t][f] as it is. */
+ * 2 relu(in[t][f]) * in[t][F + f], 3 gelu_tanh(in[t][f]) * in[t][F + f];  4: in[t][f] as it is.  Before its code SiLU is within (1.25 |z| + 16) 2^-24 of itself, GELU's tanh form within
+ * (7 |z + 0.045 z^3| + 16) 2^-24, z its argument; so they are in pk_fp8_gemm_gated. */
 int pk_fp8_act(const void* in, long ld_in, int kind, void* codes, long ld, float* scales, long ld_s, int F, int tokens, pk_stream st);
 /* codes of weights w [rows, width], bf16 or float, rows of ld_w elements (0: width) */
 int pk_fp8_weights(const void* w, int w_f32, long ld_w, void* codes, long ld, float* scales, int rows, int width, pk_stream st);

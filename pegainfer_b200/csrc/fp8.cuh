@@ -195,6 +195,8 @@ __device__ __forceinline__ void store_codes8(uint8_t* p, int n, const float* v, 
 // act 0 SiLU, 1 ReLU, 2 GELU in its tanh form, of z, times u.  SiLU and GELU: z times the logistic function of z or of sqrt(8 / pi) (z + 0.044715 z^3), as z / (1 + 2^x) by the
 // special-function unit's exponential and quotient without their ways for subnormal numbers, which took half of the instructions.  That loses gates whose 1 + 2^x has no normal reciprocal
 // (x from 126 on), and times a large factor they count: they are (z 2^(-x/2)) (2^(-x/2) u).
+// What is less exact than fp32's exp and division: the unit's results have 2^-22, and the rounding of x grows with it.  SiLU is within (1.25 |z| + 16) 2^-24 of itself (3e-6 at z = -30, a code's
+// own rounding is 6e-2), GELU within (4 |x| ln 2 + 16) 2^-24; x as a sum of two numbers takes more instructions, in a kernel whose issue slots are 0.8 busy.
 template <int ACT>
 __device__ __forceinline__ float gate_exponent(float z) {
   constexpr float kLog2e = 1.4426950408889634f, kGelu = -1.5957691216057308f * kLog2e;

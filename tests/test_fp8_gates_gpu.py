@@ -61,6 +61,23 @@ def test_act_of_far_gates_and_large_factors(lib, kind, lo, hi, power):
     R.hold_rows(codes, scales, R.act(kind, x[:, :1].double(), x[:, 1:].double()), rel=REL)
 
 
+@pytest.mark.parametrize("kind", [0, 3])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_act_is_as_exact_as_the_header_says(lib, kind, sign):
+    """SiLU: x is z times a constant, each within 2^-24 and 2^-26 of itself, so 2^x is off by 1.25 |z| 2^-24 of itself at most.  GELU: a square, two constants, a fused sum and a product make x,
+    each within 2^-24 at most and on one side of zero: 4 |x| ln(2) 2^-24 <= 4 * 1.5958 |z + 0.044715 z^3| 2^-24.  Then the exponential and the quotient by the special-function unit
+    (4 + 2), a sum, two products and the scale's product and rounding (1 + 2 + 3), in 2^-24."""
+    z = -sign * every_bf16(2.0 ** -7, 80.0 if kind == 0 else 9.5)
+    z = z[(z > 0) | (R.act(kind, z.double(), torch.ones_like(z).double()).abs() > 2.0 ** -99)]
+    x = torch.stack([z, torch.ones_like(z)], 1).contiguous()
+    codes, scales = activate(lib, x, 1, kind)
+    want = R.act(kind, z.double(), torch.ones_like(z).double())
+    got = R.values(codes[:, 0]) * scales[0, :len(z)].double()
+    a = z.double().abs()
+    size = 1.25 * a if kind == 0 else 4 * 1.5958 * (a + 0.044715 * a ** 3)
+    assert ((got - want).abs() <= want.abs() * (size + 12) * 2.0 ** -24).all()
+
+
 @pytest.mark.parametrize("kind,far", [(0, 90.0), (3, 10.5)])
 @pytest.mark.parametrize("F", [128, 256, 1000, 333])
 def test_act_of_far_gates_beside_others(lib, kind, far, F):
