@@ -212,7 +212,7 @@ fp8_gemm_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       tc_fence_after();
       const uint32_t t0 = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)((buf * NA + h) * NT + c0);
       // The stage goes back when its scales are in registers.  An arrival does not wait for loads on their way: with nothing more the copy of the stage's next block overtook the last of them
-      // once in some 1e8 blocks.  So its address takes a word of each of the last loads (a warp's loads of shared memory return in order): 1 to 2 % of a call, a proxy fence 3 to 5 %, words of
+      // in 8 of 60000 calls.  So its address takes a word of each of the last loads (a warp's loads of shared memory return in order): 1 to 2 % of a call, a proxy fence 3 to 5 %, words of
       // all loads up to 20 %.
       auto release = [&](uint32_t read) {
         tc_fence_before();
