@@ -66,3 +66,20 @@ def test_weights_that_take_an_entry_past_fp32_before_the_root(lib, W, x_f32):
     w[128:256] *= 2.0 ** -110
     w[256:384] *= 2.0 ** -128  # most of them bf16 numbers below 2^-126
     hold(lib, x, w.to(BF16), 1e-6)
+
+
+@pytest.mark.parametrize("W", [300, 2560, 9000])
+@pytest.mark.parametrize("x_f32", [False, True])
+def test_rows_whose_squares_pass_fp32(lib, W, x_f32):
+    """as the header has it: entries of 2^56 are held, a row whose sum of squares is no fp32 number has codes of zero, and its neighbours their own"""
+    x = rn(7, 4, W).sign()
+    x *= torch.tensor([1.0, 2.0 ** 56, 2.0 ** 66, 2.0 ** -20], device="cuda")[:, None]
+    x = x.to(F32 if x_f32 else BF16)
+    w = (1 + 0.3 * rn(8, W)).to(BF16)
+    codes, scales = torch.zeros(4, R.up(W, 16), dtype=torch.uint8, device="cuda"), torch.zeros(R.blocks(W), 4, device="cuda")
+    assert lib.pk_fp8_add_norm(None, x.data_ptr(), int(x_f32), w.data_ptr(), 0.0, codes.data_ptr(), codes.shape[1], scales.data_ptr(), 4, W, 4, 1e-6,
+                               torch.cuda.current_stream().cuda_stream) == 0
+    assert (codes[2, :W] & 127 == 0).all() and (scales[:, 2] * 448 == R.LEAST).all()
+    held = [0, 1, 3]
+    v = x[held].double()
+    R.hold_rows(codes[held], scales[:, held], v / torch.sqrt((v * v).mean(-1, keepdim=True) + 1e-6) * w.double(), rel=2.0 ** -17)
