@@ -112,7 +112,7 @@ __device__ __forceinline__ uint32_t codes2(float lo, float hi, Scale k) {
 __device__ __forceinline__ uint32_t codes4(const float* v, Scale k) { return codes2(v[0], v[1], k) | codes2(v[2], v[3], k) << 16; }
 
 // A thread has 8 entries of a block, 16 threads a block.  VEC: 8 in a row, read at once, for rows on 16-byte boundaries whose widths are multiples of 8.  Else every 16th, read one by one, so
-// that the threads' single entries lie side by side (B200, norm of 1328 x 2958, us, 8 in a row : every 16th: float 18.9 : 11.2, bf16 18.9 : 10.7; read at once, 1328 x 2960: float 9.3).
+// that the threads' single entries lie side by side (B200, norm of 1328 x 2958, us, 8 in a row : every 16th: float 18.9 : 11.8, bf16 18.9 : 11.3; read at once, 1328 x 2960: float 10.1).
 // of the q-th thread of a row: its first entry
 template <bool VEC>
 __device__ __forceinline__ int first_of(int q) { return VEC ? q * 8 : (q >> 4) * kBlock + (q & 15); }
@@ -196,7 +196,7 @@ __device__ __forceinline__ void store_codes8(uint8_t* p, int n, const float* v, 
 // special-function unit's exponential and quotient without their ways for subnormal numbers, which took half of the instructions.  That loses gates whose 1 + 2^x has no normal reciprocal
 // (x from 126 on), and times a large factor they count: they are (z 2^(-x/2)) (2^(-x/2) u).
 // What is less exact than fp32's exp and division: the unit's results have 2^-22, and the rounding of x grows with it.  SiLU is within (1.25 |z| + 16) 2^-24 of itself (3e-6 at z = -30, a code's
-// own rounding is 6e-2), GELU within (4 |x| ln 2 + 16) 2^-24; x as a sum of two numbers takes more instructions, in a kernel whose issue slots are 0.8 busy.
+// own rounding is 6e-2), GELU within (4 |x| ln 2 + 16) 2^-24; x as a sum of two numbers takes more instructions, in a kernel whose issue slots are 0.7 busy.
 template <int ACT>
 __device__ __forceinline__ float gate_exponent(float z) {
   constexpr float kLog2e = 1.4426950408889634f, kGelu = -1.5957691216057308f * kLog2e;

@@ -1,7 +1,8 @@
 // Rows of activations quantised to 8 bits where they are made (fp8.cuh): RMS norm with the residual's addition, gated activations, and rows as they are.
 // All of them are one pass over memory: 16 lanes have a block of 128 entries, 8 each, and find its scale by four exchanges.
-// B200, GPU time of one call in a row of them: norm of 4096 x 4096 with float x 30.6 us (185 MB, 6.04 TB/s), with bf16 x 23.9 (4.9 TB/s), of one token 2.1; silu product of 4096 x 12288 42.3
-// (253 MB, 6.0 TB/s), gelu 45, relu 38.7, relu2 29.6 and plain rows 26.5 (153 MB, 5.75 TB/s), silu of 32 x 9728 2.2.  Memory bounds the large ones (a copy reaches 6.54 TB/s), the launch the small ones.
+// B200, GPU time of one call in a row of them, us: norm of 4096 x 4096 with float x 30.2 (185 MB, 6.1 TB/s), with bf16 x 23.7 (5.0 TB/s), of 8 x 2560 2.3; of 4096 x 12288 silu product 42.7
+// (253 MB, 5.9 TB/s), gelu 44.8, relu product 39.4, relu^2 30.9 (153 MB, 4.9 TB/s), plain rows 26.9; silu product of 32 x 9728 2.1.  Memory bounds the large ones (a copy reaches 6.54 TB/s),
+// the launch the small ones.
 #include "fp8.cuh"
 
 namespace pk {
@@ -13,7 +14,7 @@ namespace fp8 {
 // largest such product has no scale of its own (below 2^-100, the root may bring it above; or past fp32, the root may bring it back) keeps x instead, and its codes wait for the root.
 constexpr int kNormWarps = 32, kNormWidest = kNormWarps * 256 * 2;
 
-// Registers: with 40 two pieces have six CTAs of eight warps on an SM (4096 x 4096 bf16 23.9 us; with the 52 that the compiler takes by itself 27.8).
+// Registers: with 40 two pieces have six CTAs of eight warps on an SM (4096 x 4096 bf16 23.7 us; with the 52 that the compiler takes by itself 27.8).
 template <typename E, int NV, bool VEC>
 __global__ void __maxnreg__(NV == 2 ? (VEC ? 40 : 56) : 32) fp8_add_norm_kernel(const bf16* __restrict__ y, E* __restrict__ x, const bf16* __restrict__ w, float offset,
                                                                       uint8_t* __restrict__ codes, long ld, float* __restrict__ scales, long ld_s, int width, float eps) {
@@ -97,7 +98,7 @@ __global__ void __maxnreg__(NV == 2 ? (VEC ? 40 : 56) : 32) fp8_add_norm_kernel(
   }
 }
 
-// Two tokens a group of lanes: their loads are under way together, which carries this kernel (silu product of 4096 x 12288, one token : two: 59 : 44.8 us).
+// Two tokens a group of lanes: their loads are under way together, which carries this kernel (silu product of 4096 x 12288, one token : two, when this was tried: 59 : 44.8 us).
 // KIND 0: silu(a) * b, 1: relu(a)^2, 2: relu(a) * b, 3: gelu(a) * b, 4: a, with a = in[t][f], b = in[t][F + f].  16 lanes have a block of a token.
 constexpr int kActThreads = 128, kActRows = 2;
 
@@ -127,7 +128,7 @@ __global__ void __launch_bounds__(kActThreads) fp8_act_kernel(const bf16* __rest
       }
     } else if constexpr (KIND != 4) {
       constexpr int ACT = KIND == 0 ? 0 : KIND - 1;
-      if (__builtin_expect(gated8<ACT>(v[r], u[r], v[r]), 0)) {  // (read again, one by one: gates and factors kept until here took twice the registers, 46.4 us for 41.7)
+      if (__builtin_expect(gated8<ACT>(v[r], u[r], v[r]), 0)) {  // (read again, one by one: kept until here, gates and factors took twice the registers: 46.4 us for 42.3)
         const bf16* row = in + (size_t)(n > 0 ? t0 + r : 0) * ld_in + at;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -151,8 +152,8 @@ cudaError_t add_norm(const bf16* y, E* x, const bf16* w, float offset, uint8_t* 
     const int warps = (width + 256 * nv - 1) / (256 * nv);
     return launch(kern, dim3(tokens), dim3(32 * warps), 0, st, true, y, x, w, offset, codes, ld, scales, ld_s, width, eps);
   };
-  // B200, us, one piece a thread : two, x bf16: 8 x 2560 2.3 : 2.8, 512 x 2560 4.0 : 4.3, 1024 x 2560 7.2 : 6.2, 3001 x 2560 14.6 : 13.5, 4096 x 4096 28.6 : 25.2;
-  // x float: 512 x 2560 5.1 : 5.9, 3001 x 2560 15.6 : 18.4, 4096 x 4096 30.8 : 34.7, 2048 x 8192 34.1 : 35.5
+  // B200, us, one piece a thread : two, x bf16: 8 x 2560 2.3 : 2.7, 512 x 2560 3.7 : 3.9, 800 x 2560 5.0 : 5.2, 1024 x 2560 7.1 : 6.2, 3001 x 2560 14.0 : 13.2,
+  // 4096 x 4096 26.5 : 24.1; x float: 512 x 2560 4.8 : 5.2, 3001 x 2560 15.6 : 16.8, 4096 x 4096 30.6 : 31.6, 2048 x 8192 32.6 : 32.2
   if (width <= kNormWarps * 256 && (sizeof(E) == 4 || tokens < 5 * sm_count())) return go(fp8_add_norm_kernel<E, 1, VEC>, 1);
   return go(fp8_add_norm_kernel<E, 2, VEC>, 2);
 }
